@@ -198,6 +198,129 @@ int lc_attention_decode_maxlen(lc_context* ctx, const float* q, const float* k, 
  * the maximum (ties -> lowest index; 0 when values[0] is NaN). */
 int lc_argmax(lc_context* ctx, const float* values, int n, int32_t* out_index);
 
+/* ------------------------------------------------ paged 8-bit KV cache ---- *
+ * One serving step over a cache of pages: rotary positions, page bookkeeping,
+ * quantised append, attention.  No counterpart in the reference, whose cache
+ * is one contiguous fp32 array per sequence (H/LlamaInference.java:79-89).
+ * Row buffers ("rows") are F32 or F16 (dtype 0 or 1, as
+ * lc_model_upload_tensor), row i at i * stride elements; int32 arrays and rows
+ * may be host or device memory, the cache itself is device memory.  With
+ * device memory throughout, the calls only enqueue on the context's stream,
+ * allocate nothing and can be captured in a CUDA graph. */
+
+enum { LC_ROPE_INTERLEAVED = 0, /* pairs (2j, 2j + 1), as lc_rope */
+       LC_ROPE_HALF = 1 };      /* pairs (j, j + rot_dim / 2) */
+enum { LC_ROPE_SCALE_NONE = 0, LC_ROPE_SCALE_LINEAR = 1, LC_ROPE_SCALE_LLAMA3 = 2, LC_ROPE_SCALE_YARN = 3 };
+
+/* Pair j turns by pos * f_j, f_j = theta^(-2j / rot_dim), scaled to g_j:
+ *   LINEAR  g = f / factor
+ *   LLAMA3  with t = original_max_pos * f / (2 pi) turns in the trained length
+ *           and k = clamp((t - low_freq_factor) / (high - low), 0, 1):
+ *           g = k f + (1 - k) f / factor
+ *   YARN    r = clamp((j - a) / (b - a), 0, 1) between the pairs that make
+ *           beta_fast and beta_slow turns in the trained length (a rounded
+ *           down, b up): g = r f / factor + (1 - r) f; cos and sin times
+ *           attn_factor (0: 0.1 ln(factor) + 1). */
+typedef struct lc_rope_config {
+    int32_t head_dim;  /* <= 512 */
+    int32_t rot_dim;   /* rotated elements at the head's start, even; the rest is copied */
+    int32_t layout;
+    int32_t scaling;
+    float theta;
+    float factor;
+    float low_freq_factor, high_freq_factor;
+    float beta_fast, beta_slow, attn_factor;
+    int32_t original_max_pos;
+    int32_t reserved[4];
+} lc_rope_config;
+
+/* What Llama 3.2 uses for 128 Ki positions: theta 500000, LLAMA3 scaling 32
+ * (1, 4, 8192), head_dim 64, interleaved pairs. */
+void lc_rope_config_llama32(lc_rope_config* out);
+
+/* y[i] = rotation of x[i] (num_heads heads of head_dim) at pos[i]; in place
+ * when y == x (equal strides), otherwise the buffers must not overlap.
+ * transpose != 0: the transposed map, the gradient of x from that of y.  Rows
+ * with pos < 0 are left as they are.  Angles are reduced in fp64, so far
+ * positions keep fp32 accuracy. */
+int lc_rope_apply(lc_context* ctx, const lc_rope_config* cfg, const void* x, void* y, const int32_t* pos, int32_t rows,
+                  int32_t num_heads, int64_t x_stride, int64_t y_stride, int32_t dtype, int32_t transpose);
+
+/* Page bookkeeping of one step for n_seqs (<= 4096) sequences.  Token t of
+ * sequence s lies in page table[s * table_stride + t / page_size] at
+ * t % page_size; its slot is page * page_size + t % page_size.
+ *   lens[s]   tokens held; n_new[s] >= 0 tokens to add, < 0: the sequence ends
+ *   free_list [n_pages] stack of free pages, *free_count entries
+ * First every ended sequence pushes its pages (sequence order, table order);
+ * then every growing one pops the pages it lacks from the top.  Written:
+ *   table     the new pages' entries       lens_out   lens + n_new; 0: ended
+ *   q_start   [n_seqs + 1] first new token of each sequence
+ *   slots, positions, seq_ids  [capacity] of every new token in sequence
+ *             order; -1 behind the last
+ *   free_list, free_count_out  the stack after the step
+ *   status    {code, detail}: 0 done; 1 pages short by detail; 2 sequence
+ *             detail does not fit its table row; 3 detail tokens exceed
+ *             capacity; 4 lens[detail] < 0; 5 the free stack does not fit
+ *             n_pages.  Unless 0 nothing changes: lens_out = lens, q_start 0,
+ *             slots, positions and seq_ids -1, free_count_out = free_count.
+ * lens_out may be lens and free_count_out may be free_count; no other buffers
+ * may overlap. */
+int lc_pages_step(lc_context* ctx, const int32_t* lens, const int32_t* n_new, int32_t n_seqs, int32_t page_size,
+                  int32_t* table, int32_t table_stride, int32_t* free_list, const int32_t* free_count, int32_t n_pages,
+                  int32_t capacity, int32_t* lens_out, int32_t* q_start, int32_t* slots, int32_t* positions,
+                  int32_t* seq_ids, int32_t* free_count_out, int32_t* status);
+
+enum { LC_KV8_I8 = 0,    /* signed bytes, -127..127 */
+       LC_KV8_E4M3 = 1 };/* e4m3 values up to 448 */
+
+/* A cache of pages in 8 bits, in device memory that the caller owns: codes
+ * [n_pages][n_kv_heads][page_size][head_dim] (16-byte aligned) and fp32 scales
+ * [n_pages][n_kv_heads]; a value is code * scale. */
+typedef struct lc_kv8 {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t n_pages;
+    int32_t page_size;  /* 16, 32, 64 or 128 tokens */
+    int32_t n_kv_heads;
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t format;     /* LC_KV8_* */
+    int32_t reserved[3];
+} lc_kv8;
+
+/* Writes row i of k and v ([rows][n_kv_heads * head_dim]) at slots[i]; rows
+ * whose slot is negative or behind the last page are skipped.  A run of
+ * neighbouring rows with consecutive slots of one page is one write: the
+ * page's scale becomes max(scale, largest finite |x| of the run / limit)
+ * (limit 127 or 448; the old scale counts as 0 when the run starts the page),
+ * the codes before the run are rounded anew when the scale grows, the tokens
+ * behind the run count as gone.  Each code is the one nearest to the exact
+ * quotient, ties to even; NaN is stored as 0, infinities at the limit.
+ * Runs of one page that only skipped rows separate are written in row order;
+ * rows of one page must not have rows of another page between them: the
+ * first page's contents would be unspecified. */
+int lc_kv8_append(lc_context* ctx, const lc_kv8* kv, const void* k, const void* v, int64_t row_stride, int32_t dtype,
+                  const int32_t* slots, int32_t rows);
+
+/* Rows of k and v = the values at slots[i]; rows whose slot is negative or
+ * behind the last page are left as they are. */
+int lc_kv8_read(lc_context* ctx, const lc_kv8* kv, void* k, void* v, int64_t row_stride, int32_t dtype,
+                const int32_t* slots, int32_t rows);
+
+/* Causal attention of n_heads query heads (n_heads / n_kv_heads share a kv
+ * head) over the pages.  Rows q_start[s]..q_start[s + 1] - 1 of q and out
+ * ([rows][n_heads * head_dim]) are the queries of sequence s, whose cache holds
+ * kv_lens[s] positions, theirs included: query j of n stands at position
+ * kv_lens[s] - n + j and sees the positions up to it.  q_start NULL: row s is
+ * the one query of sequence s (rows == n_seqs).  out = softmax(scale q.k) v; a
+ * query that sees nothing gives zeros; rows behind q_start[n_seqs] are left as
+ * they are; pages outside the cache are not seen.  max_q: the largest
+ * number of queries of a sequence, which chooses the kernel (results hold for
+ * any value).  n_seqs <= 4096.  lens, tables and q_start are read on the
+ * device. */
+int lc_kv8_attention(lc_context* ctx, const lc_kv8* kv, const void* q, void* out, int64_t q_stride, int64_t out_stride,
+                     int32_t dtype, int32_t rows, const int32_t* q_start, const int32_t* kv_lens, const int32_t* table,
+                     int32_t table_stride, int32_t n_seqs, int32_t max_q, int32_t n_heads, float scale);
+
 /* ------------------------------------------------------------- model ---- */
 typedef struct lc_config {
     int32_t dim;        /* HIDDEN_SIZE 2048          (H/LlamaModel.java:30) */

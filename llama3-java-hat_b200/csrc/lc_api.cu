@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -21,6 +22,7 @@
 #include "../../include/llamacuda.h"
 #include "lc_attention.cuh"
 #include "lc_internal.h"
+#include "lc_paged.h"
 
 using namespace lc;
 
@@ -602,6 +604,314 @@ extern "C" int lc_argmax(lc_context* c, const float* values, int n, int32_t* out
     if (s.status != LC_OK) return s.status;
     launch_argmax(dv, n, di, c->stream);
     return s.finish(cudaGetLastError());
+}
+
+// ------------------------------------------------ paged 8-bit KV cache ----
+
+namespace {
+
+// The calling thread's device is the context's for the scope of a call.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t status;
+    explicit DeviceScope(int device) {
+        status = cudaGetDevice(&before);
+        if (status == cudaSuccess && before != device) status = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// Bytes of `rows` rows of `width` elements, `stride` elements apart.
+size_t rows_bytes(int rows, int64_t stride, int64_t width, int elem) {
+    return (size_t)((int64_t)(rows - 1) * stride + width) * elem;
+}
+
+int row_elem(int dtype) { return dtype == kRowF32 ? 4 : dtype == kRowF16 ? 2 : 0; }
+
+// Runs the body of an entry point on the context's device; no C++ exception
+// leaves it.
+template <typename F>
+int on_device(lc_context* c, F&& body) {
+    if (!c) return fail(LC_ERR_INVALID_ARG, "context is NULL");
+    DeviceScope scope(c->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return fail(LC_ERR_OUT_OF_MEMORY, "host memory");
+    } catch (...) {
+        return fail(LC_ERR_STATE, "unexpected exception");
+    }
+}
+
+int log2_exact(int v) {
+    int k = 0;
+    while ((1 << k) < v) ++k;
+    return k;
+}
+
+// Checks a cache descriptor and fills the kernels' view of it.
+int kv8_view(lc_context* c, const lc_kv8* kv, Kv8* out) {
+    if (!kv) return fail(LC_ERR_INVALID_ARG, "cache is NULL");
+    if (kv->n_pages <= 0 || kv->n_kv_heads <= 0)
+        return fail(LC_ERR_INVALID_ARG, "n_pages=%d n_kv_heads=%d", kv->n_pages, kv->n_kv_heads);
+    if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 && kv->page_size != 128)
+        return fail(LC_ERR_UNSUPPORTED, "page_size %d (16, 32, 64 or 128)", kv->page_size);
+    if (kv->head_dim != 64 && kv->head_dim != 128)
+        return fail(LC_ERR_UNSUPPORTED, "head_dim %d (64 or 128)", kv->head_dim);
+    if (kv->format != LC_KV8_I8 && kv->format != LC_KV8_E4M3)
+        return fail(LC_ERR_INVALID_ARG, "format %d (LC_KV8_I8 = 0, LC_KV8_E4M3 = 1)", kv->format);
+    if ((int64_t)kv->n_pages * kv->page_size > INT32_MAX)
+        return fail(LC_ERR_UNSUPPORTED, "%d pages of %d tokens: slots are 32-bit", kv->n_pages, kv->page_size);
+    Stager s(c);
+    const void* p[4] = {kv->k, kv->v, kv->k_scale, kv->v_scale};
+    for (const void* q : p) {
+        int rc = LC_OK;
+        if (!q || !s.is_device(q, &rc)) return fail(LC_ERR_INVALID_ARG, "cache pages and scales must be device memory");
+        if (rc != LC_OK) return rc;
+    }
+    if (((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) return fail(LC_ERR_INVALID_ARG, "cache pages must be 16-byte aligned");
+    *out = Kv8{(uint8_t*)kv->k, (uint8_t*)kv->v, kv->k_scale, kv->v_scale,
+               kv->n_pages,     log2_exact(kv->page_size), kv->n_kv_heads, kv->head_dim, kv->format};
+    return LC_OK;
+}
+
+}  // namespace
+
+extern "C" void lc_rope_config_llama32(lc_rope_config* o) {
+    if (!o) return;
+    memset(o, 0, sizeof(*o));
+    o->head_dim = o->rot_dim = 64;
+    o->layout = LC_ROPE_INTERLEAVED;
+    o->scaling = LC_ROPE_SCALE_LLAMA3;
+    o->theta = 500000.0f;
+    o->factor = 32.0f;
+    o->low_freq_factor = 1.0f;
+    o->high_freq_factor = 4.0f;
+    o->original_max_pos = 8192;
+}
+
+// Turns per position of every rotated pair in fp64, and the factor on cos and sin.
+static int rope_turns(const lc_rope_config* g, RopeTurns* out, float* mult) {
+    if (!g) return fail(LC_ERR_INVALID_ARG, "config is NULL");
+    if (g->head_dim <= 0 || g->head_dim > 2 * kRopeMaxPairs || g->rot_dim < 0 || g->rot_dim > g->head_dim ||
+        (g->rot_dim & 1))
+        return fail(LC_ERR_INVALID_ARG, "head_dim=%d rot_dim=%d (rot_dim even, 0..head_dim <= %d)", g->head_dim,
+                    g->rot_dim, 2 * kRopeMaxPairs);
+    if (g->layout != LC_ROPE_INTERLEAVED && g->layout != LC_ROPE_HALF)
+        return fail(LC_ERR_INVALID_ARG, "layout %d", g->layout);
+    if (!(g->theta > 1.0f) || isinf(g->theta)) return fail(LC_ERR_INVALID_ARG, "theta=%g (> 1)", g->theta);
+    const bool scaled = g->scaling != LC_ROPE_SCALE_NONE;
+    if (scaled && (!(g->factor >= 1.0f) || isinf(g->factor))) return fail(LC_ERR_INVALID_ARG, "factor=%g (>= 1)", g->factor);
+    if ((g->scaling == LC_ROPE_SCALE_LLAMA3 || g->scaling == LC_ROPE_SCALE_YARN) && g->original_max_pos <= 0)
+        return fail(LC_ERR_INVALID_ARG, "original_max_pos=%d", g->original_max_pos);
+    const double pi2 = 6.283185307179586476925286766559, rot = g->rot_dim, theta = g->theta, factor = g->factor;
+    double low = 0, high = 0;
+    *mult = 1.0f;
+    switch (g->scaling) {
+        case LC_ROPE_SCALE_NONE:
+        case LC_ROPE_SCALE_LINEAR:
+            break;
+        case LC_ROPE_SCALE_LLAMA3:
+            if (!(g->high_freq_factor > g->low_freq_factor) || !(g->low_freq_factor > 0.0f) || isinf(g->high_freq_factor))
+                return fail(LC_ERR_INVALID_ARG, "low_freq_factor=%g high_freq_factor=%g (0 < low < high)",
+                            g->low_freq_factor, g->high_freq_factor);
+            break;
+        case LC_ROPE_SCALE_YARN: {
+            if (!(g->beta_fast > g->beta_slow) || !(g->beta_slow > 0.0f) || isinf(g->beta_fast) || !(g->attn_factor >= 0.0f) ||
+                isinf(g->attn_factor))
+                return fail(LC_ERR_INVALID_ARG, "beta_fast=%g beta_slow=%g attn_factor=%g (0 < slow < fast, factor >= 0)",
+                            g->beta_fast, g->beta_slow, g->attn_factor);
+            auto dim_of = [&](double turns) {  // the pair that makes `turns` turns within the trained length
+                return rot * log(g->original_max_pos / (turns * pi2)) / (2.0 * log(theta));
+            };
+            low = fmax(floor(dim_of(g->beta_fast)), 0.0);
+            high = fmin(ceil(dim_of(g->beta_slow)), rot - 1.0);
+            *mult = (float)(g->attn_factor > 0.0f ? g->attn_factor : 0.1 * log(factor) + 1.0);
+            break;
+        }
+        default:
+            return fail(LC_ERR_INVALID_ARG, "scaling %d", g->scaling);
+    }
+    for (int j = 0; j < g->rot_dim / 2; ++j) {
+        double f = pow(theta, -2.0 * j / rot);
+        if (g->scaling == LC_ROPE_SCALE_LINEAR) {
+            f /= factor;
+        } else if (g->scaling == LC_ROPE_SCALE_LLAMA3) {
+            const double turns = g->original_max_pos * f / pi2;
+            double keep = (turns - g->low_freq_factor) / ((double)g->high_freq_factor - g->low_freq_factor);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f = keep * f + (1.0 - keep) * f / factor;
+        } else if (g->scaling == LC_ROPE_SCALE_YARN) {
+            double ramp = (j - low) / fmax(high - low, 0.001);
+            ramp = ramp < 0.0 ? 0.0 : ramp > 1.0 ? 1.0 : ramp;
+            f = ramp * f / factor + (1.0 - ramp) * f;
+        }
+        out->t[j] = f / pi2;
+    }
+    return LC_OK;
+}
+
+extern "C" int lc_rope_apply(lc_context* c, const lc_rope_config* cfg, const void* x, void* y, const int32_t* pos,
+                             int32_t rows, int32_t num_heads, int64_t x_stride, int64_t y_stride, int32_t dtype,
+                             int32_t transpose) {
+    return on_device(c, [&]() -> int {
+        RopeTurns turns;
+        RopeApply a;
+        memset(&a, 0, sizeof(a));
+        if (int rc = rope_turns(cfg, &turns, &a.mult)) return rc;
+        const int elem = row_elem(dtype);
+        if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
+        const int64_t width = (int64_t)num_heads * cfg->head_dim;
+        if (rows < 0 || num_heads <= 0 || x_stride < 0 || (y_stride < width && rows > 1))
+            return fail(LC_ERR_INVALID_ARG, "rows=%d num_heads=%d x_stride=%lld y_stride=%lld", rows, num_heads,
+                        (long long)x_stride, (long long)y_stride);
+        if (x == y && x_stride != y_stride) return fail(LC_ERR_INVALID_ARG, "in place, the strides must be equal");
+        if (rows == 0) return LC_OK;
+        Stager s(c);
+        const bool in_place = x == y;
+        a.y = s.arg(y, rows_bytes(rows, y_stride, width, elem), kInOut);
+        a.x = in_place ? a.y : s.arg(x, rows_bytes(rows, x_stride, width, elem), kIn);
+        a.pos = (const int32_t*)s.arg(pos, (size_t)rows * 4, kIn);
+        if (s.status != LC_OK) return s.status;
+        a.rows = rows;
+        a.heads = num_heads;
+        a.head_dim = cfg->head_dim;
+        a.rot_dim = cfg->rot_dim;
+        a.x_stride = x_stride;
+        a.y_stride = y_stride;
+        a.sign = transpose ? -1.0f : 1.0f;
+        a.half = cfg->layout == LC_ROPE_HALF;
+        a.dtype = dtype;
+        return s.finish(launch_rope_apply(a, turns, c->sms, c->stream));
+    });
+}
+
+extern "C" int lc_pages_step(lc_context* c, const int32_t* lens, const int32_t* n_new, int32_t n_seqs,
+                             int32_t page_size, int32_t* table, int32_t table_stride, int32_t* free_list,
+                             const int32_t* free_count, int32_t n_pages, int32_t capacity, int32_t* lens_out,
+                             int32_t* q_start, int32_t* slots, int32_t* positions, int32_t* seq_ids,
+                             int32_t* free_count_out, int32_t* status) {
+    return on_device(c, [&]() -> int {
+        if (n_seqs <= 0 || n_seqs > kPagesMaxSeqs) return fail(LC_ERR_INVALID_ARG, "n_seqs=%d (1..%d)", n_seqs, kPagesMaxSeqs);
+        if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+            return fail(LC_ERR_UNSUPPORTED, "page_size %d (16, 32, 64 or 128)", page_size);
+        if (table_stride <= 0 || n_pages <= 0 || capacity < 0)
+            return fail(LC_ERR_INVALID_ARG, "table_stride=%d n_pages=%d capacity=%d", table_stride, n_pages, capacity);
+        if ((int64_t)n_pages * page_size > INT32_MAX || (int64_t)table_stride * page_size > INT32_MAX)
+            return fail(LC_ERR_UNSUPPORTED, "slots and positions are 32-bit");
+        Stager s(c);
+        PagesStep p;
+        memset(&p, 0, sizeof(p));
+        const size_t n4 = (size_t)n_seqs * 4, cap4 = (size_t)capacity * 4;
+        const bool same_lens = lens == lens_out, same_count = free_count == free_count_out;
+        p.lens_out = (int32_t*)s.arg(lens_out, n4, same_lens ? kInOut : kOut);
+        p.lens = same_lens ? p.lens_out : (const int32_t*)s.arg(lens, n4, kIn);
+        p.n_new = (const int32_t*)s.arg(n_new, n4, kIn);
+        p.table = (int32_t*)s.arg(table, (size_t)n_seqs * table_stride * 4, kInOut);
+        p.free_list = (int32_t*)s.arg(free_list, (size_t)n_pages * 4, kInOut);
+        p.free_count_out = (int32_t*)s.arg(free_count_out, 4, same_count ? kInOut : kOut);
+        p.free_count = same_count ? p.free_count_out : (const int32_t*)s.arg(free_count, 4, kIn);
+        p.q_start = (int32_t*)s.arg(q_start, n4 + 4, kOut);
+        p.status = (int32_t*)s.arg(status, 8, kOut);
+        if (capacity) {
+            p.slots = (int32_t*)s.arg(slots, cap4, kOut);
+            p.positions = (int32_t*)s.arg(positions, cap4, kOut);
+            p.seq_ids = (int32_t*)s.arg(seq_ids, cap4, kOut);
+        }
+        if (s.status != LC_OK) return s.status;
+        p.n_seqs = n_seqs;
+        p.page_shift = log2_exact(page_size);
+        p.table_stride = table_stride;
+        p.n_pages = n_pages;
+        p.capacity = capacity;
+        return s.finish(launch_pages_step(p, c->stream));
+    });
+}
+
+static int kv8_rows(lc_context* c, const lc_kv8* kv, void* k, void* v, int64_t row_stride, int32_t dtype,
+                    const int32_t* slots, int32_t rows, bool append) {
+    return on_device(c, [&]() -> int {
+        Kv8 view;
+        if (int rc = kv8_view(c, kv, &view)) return rc;
+        const int elem = row_elem(dtype);
+        if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
+        const int64_t width = (int64_t)kv->n_kv_heads * kv->head_dim;
+        if (rows < 0 || row_stride < 0 || (!append && rows > 1 && row_stride < width))
+            return fail(LC_ERR_INVALID_ARG, "rows=%d row_stride=%lld", rows, (long long)row_stride);
+        if (rows == 0) return LC_OK;
+        Stager s(c);
+        Kv8Rows r;
+        const size_t bytes = rows_bytes(rows, row_stride, width, elem);
+        // Rows without a slot are left as they are: host rows that are read into travel both ways.
+        r.k = s.arg(k, bytes, append ? kIn : kInOut);
+        r.v = s.arg(v, bytes, append ? kIn : kInOut);
+        r.slots = (const int32_t*)s.arg(slots, (size_t)rows * 4, kIn);
+        if (s.status != LC_OK) return s.status;
+        r.row_stride = row_stride;
+        r.rows = rows;
+        r.dtype = dtype;
+        return s.finish(append ? launch_kv8_append(view, r, c->sms, c->stream) : launch_kv8_read(view, r, c->sms, c->stream));
+    });
+}
+
+extern "C" int lc_kv8_append(lc_context* c, const lc_kv8* kv, const void* k, const void* v, int64_t row_stride,
+                             int32_t dtype, const int32_t* slots, int32_t rows) {
+    return kv8_rows(c, kv, const_cast<void*>(k), const_cast<void*>(v), row_stride, dtype, slots, rows, true);
+}
+
+extern "C" int lc_kv8_read(lc_context* c, const lc_kv8* kv, void* k, void* v, int64_t row_stride, int32_t dtype,
+                           const int32_t* slots, int32_t rows) {
+    return kv8_rows(c, kv, k, v, row_stride, dtype, slots, rows, false);
+}
+
+extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, void* out, int64_t q_stride,
+                                int64_t out_stride, int32_t dtype, int32_t rows, const int32_t* q_start,
+                                const int32_t* kv_lens, const int32_t* table, int32_t table_stride, int32_t n_seqs,
+                                int32_t max_q, int32_t n_heads, float scale) {
+    return on_device(c, [&]() -> int {
+        Kv8 view;
+        if (int rc = kv8_view(c, kv, &view)) return rc;
+        const int elem = row_elem(dtype);
+        if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
+        if (n_heads <= 0 || n_heads % kv->n_kv_heads)
+            return fail(LC_ERR_INVALID_ARG, "n_heads=%d n_kv_heads=%d", n_heads, kv->n_kv_heads);
+        const int64_t width = (int64_t)n_heads * kv->head_dim;
+        if (rows < 0 || n_seqs < 0 || n_seqs > kPagesMaxSeqs || table_stride <= 0 || max_q < 1 || q_stride < 0 ||
+            (rows > 1 && out_stride < width))
+            return fail(LC_ERR_INVALID_ARG, "rows=%d n_seqs=%d (0..%d) table_stride=%d max_q=%d q_stride=%lld out_stride=%lld",
+                        rows, n_seqs, kPagesMaxSeqs, table_stride, max_q, (long long)q_stride, (long long)out_stride);
+        if ((int64_t)table_stride * kv->page_size > INT32_MAX)
+            return fail(LC_ERR_UNSUPPORTED, "positions are 32-bit");
+        if (!q_start && (max_q != 1 || rows != n_seqs))
+            return fail(LC_ERR_INVALID_ARG, "without q_start every sequence has one query: rows=%d n_seqs=%d max_q=%d", rows,
+                        n_seqs, max_q);
+        if (!(scale > 0.0f) || isinf(scale)) return fail(LC_ERR_INVALID_ARG, "scale=%g", scale);
+        if (rows == 0 || n_seqs == 0) return LC_OK;
+        if ((int64_t)rows * n_heads > INT32_MAX) return fail(LC_ERR_UNSUPPORTED, "rows * n_heads exceeds 2^31 - 1");
+        Stager s(c);
+        Kv8Attention a;
+        memset(&a, 0, sizeof(a));
+        a.q = s.arg(q, rows_bytes(rows, q_stride, width, elem), kIn);
+        a.out = s.arg(out, rows_bytes(rows, out_stride, width, elem), kInOut);
+        if (q_start) a.q_start = (const int32_t*)s.arg(q_start, (size_t)(n_seqs + 1) * 4, kIn);
+        a.kv_lens = (const int32_t*)s.arg(kv_lens, (size_t)n_seqs * 4, kIn);
+        a.table = (const int32_t*)s.arg(table, (size_t)n_seqs * table_stride * 4, kIn);
+        if (s.status != LC_OK) return s.status;
+        a.q_stride = q_stride;
+        a.out_stride = out_stride;
+        a.table_stride = table_stride;
+        a.n_seqs = n_seqs;
+        a.rows = rows;
+        a.max_q = max_q;
+        a.n_heads = n_heads;
+        a.dtype = dtype;
+        a.scale = scale;
+        return s.finish(launch_kv8_attention(view, a, c->sms, c->stream));
+    });
 }
 
 // -------------------------------------------------------------- model ----

@@ -66,6 +66,23 @@ class LcConfig(ctypes.Structure):
     ]
 
 
+class LcRopeConfig(ctypes.Structure):
+    _fields_ = [
+        ("head_dim", c_int32), ("rot_dim", c_int32), ("layout", c_int32), ("scaling", c_int32),
+        ("theta", c_float), ("factor", c_float), ("low_freq_factor", c_float), ("high_freq_factor", c_float),
+        ("beta_fast", c_float), ("beta_slow", c_float), ("attn_factor", c_float), ("original_max_pos", c_int32),
+        ("reserved", c_int32 * 4),
+    ]
+
+
+class LcKv8(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("n_pages", c_int32), ("page_size", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32),
+        ("format", c_int32), ("reserved", c_int32 * 3),
+    ]
+
+
 # lc_token_callback: void (*)(int32_t token, int32_t index, void* user)
 TOKEN_CALLBACK = ctypes.CFUNCTYPE(None, c_int32, c_int32, c_void_p)
 
@@ -109,6 +126,15 @@ SIGNATURES = {
     "lc_attention_decode_static": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                            c_int, c_int, c_int, c_int64, c_int64, c_int64]),
     "lc_argmax": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
+    "lc_rope_config_llama32": (None, [POINTER(LcRopeConfig)]),
+    "lc_rope_apply": (c_int, [c_void_p, POINTER(LcRopeConfig), c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int64,
+                              c_int64, c_int32, c_int32]),
+    "lc_pages_step": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+                              c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "lc_kv8_append": (c_int, [c_void_p, POINTER(LcKv8), c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32]),
+    "lc_kv8_read": (c_int, [c_void_p, POINTER(LcKv8), c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32]),
+    "lc_kv8_attention": (c_int, [c_void_p, POINTER(LcKv8), c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
+                                 c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float]),
     "lc_config_llama32_1b": (None, [POINTER(LcConfig)]),
     "lc_model_create": (c_int, [c_void_p, POINTER(LcConfig), POINTER(c_void_p)]),
     "lc_model_upload_tensor": (c_int, [c_void_p, c_char_p, c_void_p, c_int64, c_int32]),

@@ -7,9 +7,11 @@ rope theta TransformerBlock.java:136, eps kernels/RMSNorm.java:22).
 from __future__ import annotations
 
 import enum
+import functools
 from dataclasses import dataclass, replace
+from typing import ClassVar
 
-from ._lib import LcConfig
+from ._lib import LcConfig, LcRopeConfig
 
 
 @dataclass(frozen=True)
@@ -52,6 +54,47 @@ class LlamaConfig:
         """F16 projection + embedding bytes streamed by one batch-1 decode step."""
         per_layer = 2 * (self.dim * (self.q_dim + 2 * self.kv_dim) + self.dim * self.q_dim + 3 * self.dim * self.hidden)
         return self.n_layers * per_layer + 2 * self.vocab * self.dim
+
+
+@dataclass(frozen=True)
+class RopeConfig:
+    """Rotary positions of `CudaRoPE.apply_scaled` (lc_rope_config): layout
+    "interleaved" or "half"; scaling "none", "linear", "llama3" or "yarn";
+    rot_dim None rotates the whole head."""
+    head_dim: int = 64
+    rot_dim: int | None = None
+    layout: str = "interleaved"
+    scaling: str = "none"
+    theta: float = 500000.0
+    factor: float = 1.0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attn_factor: float = 0.0
+    original_max_pos: int = 8192
+
+    LAYOUTS: ClassVar = ("interleaved", "half")
+    SCALINGS: ClassVar = ("none", "linear", "llama3", "yarn")
+
+    def __post_init__(self):
+        if self.layout not in self.LAYOUTS or self.scaling not in self.SCALINGS:
+            raise ValueError(f"layout {self.layout!r} (of {self.LAYOUTS}), scaling {self.scaling!r} (of {self.SCALINGS})")
+
+    @staticmethod
+    def llama32() -> "RopeConfig":
+        """lc_rope_config_llama32: what Llama 3.2 uses for 128 Ki positions."""
+        return RopeConfig(scaling="llama3", factor=32.0)
+
+    @functools.cached_property
+    def lc(self) -> LcRopeConfig:
+        c = LcRopeConfig()
+        for name in ("head_dim", "theta", "factor", "low_freq_factor", "high_freq_factor", "beta_fast", "beta_slow",
+                     "attn_factor", "original_max_pos"):
+            setattr(c, name, getattr(self, name))
+        c.rot_dim = self.head_dim if self.rot_dim is None else self.rot_dim
+        c.layout, c.scaling = self.LAYOUTS.index(self.layout), self.SCALINGS.index(self.scaling)
+        return c
 
 
 LLAMA_3_2_1B = LlamaConfig()

@@ -20,6 +20,7 @@ from abc import ABC, abstractmethod
 import numpy as np
 
 from . import _lib
+from .config import RopeConfig
 
 
 def _addr(buf, kind: str, min_len: int, writable: bool = False) -> int:
@@ -52,6 +53,35 @@ def _addr(buf, kind: str, min_len: int, writable: bool = False) -> int:
             raise ValueError(f"tensor holds {buf.numel()} elements, need {min_len}")
         return buf.data_ptr()
     raise TypeError(f"unsupported buffer type {type(buf)!r}")
+
+
+_ROW_TYPES = {"float32": 0, "float16": 1, "torch.float32": 0, "torch.float16": 1}
+
+
+def _rows(buf, writable: bool = False):
+    """(address, rows, width, row stride in elements, dtype id) of a buffer of
+    F32 or F16 rows: [rows, ...] with contiguous rows, any row stride."""
+    dt = _ROW_TYPES.get(str(buf.dtype))
+    if dt is None:
+        raise TypeError(f"expected float32 or float16 rows, got {buf.dtype}")
+    shape = buf.shape
+    if len(shape) < 2:
+        raise ValueError(f"expected [rows, ...], got shape {tuple(shape)}")
+    if isinstance(buf, np.ndarray):
+        if writable and not buf.flags.writeable:
+            raise ValueError("buffer is read-only")
+        strides, addr = [s // buf.itemsize for s in buf.strides], buf.ctypes.data
+    else:
+        strides, addr = buf.stride(), buf.data_ptr()
+    width = 1
+    for n, st in zip(reversed(shape[1:]), reversed(strides[1:])):
+        if st != width and n > 1:
+            raise ValueError("rows must be contiguous")
+        width *= n
+    stride = strides[0] if shape[0] > 1 else width
+    if stride < 0 or (writable and stride < width):
+        raise ValueError(f"row stride {stride} of rows of {width}")
+    return addr, shape[0], width, stride, dt
 
 
 class Accelerator:
@@ -251,6 +281,104 @@ class CudaRoPE(_CudaKernel, IRoPE):
                                          _addr(positions, "i32", rows), rows, numHeads, headDim, theta))
 
 
+    def apply_scaled(self, x, out, positions, config: RopeConfig, transpose: bool = False) -> None:
+        """Rows [rows, heads, head_dim] (F32 or F16) at their positions under a
+        RopeConfig (see lc_rope_apply); out may be x.  transpose: the gradient
+        of x from that of out.  Rows at negative positions are left as they are."""
+        xa, rows, width, xs, dt = _rows(x)
+        if out is x:
+            ya, ys = xa, xs
+        else:
+            ya, orows, owidth, ys, odt = _rows(out, True)
+            if (orows, owidth, odt) != (rows, width, dt):
+                raise ValueError("x and out differ in shape or type")
+        if width == 0 or width % config.head_dim:
+            raise ValueError(f"rows of {width} elements, head_dim {config.head_dim}")
+        _lib.check(self.lib.lc_rope_apply(self.ctx, config.lc, xa, ya, _addr(positions, "i32", rows), rows,
+                                          width // config.head_dim, xs, ys, dt, int(transpose)))
+
+
+class CudaPages(_CudaKernel):
+    """Page bookkeeping of one serving step (see lc_pages_step)."""
+
+    def step(self, lens, n_new, table, free_list, free_count, page_size: int, lens_out, q_start, slots, positions,
+             seq_ids, free_count_out, status) -> None:
+        """lens, n_new [n]; table [n, stride]; free_list [n_pages]; slots,
+        positions, seq_ids [capacity]; q_start [n + 1]; free_count(_out) [1];
+        status [2] = (code, detail), code 0 when the step was done."""
+        n, stride = table.shape
+        cap = slots.shape[0]
+        _lib.check(self.lib.lc_pages_step(
+            self.ctx, _addr(lens, "i32", n), _addr(n_new, "i32", n), n, page_size, _addr(table, "i32", n * stride, True),
+            stride, _addr(free_list, "i32", 1, True), _addr(free_count, "i32", 1), free_list.shape[0], cap,
+            _addr(lens_out, "i32", n, True), _addr(q_start, "i32", n + 1, True), _addr(slots, "i32", cap, True),
+            _addr(positions, "i32", cap, True), _addr(seq_ids, "i32", cap, True),
+            _addr(free_count_out, "i32", 1, True), _addr(status, "i32", 2, True)))
+
+
+class PagedKV8(_CudaKernel):
+    """A paged KV cache in 8 bits (see lc_kv8): codes k, v [n_pages, n_kv_heads,
+    page_size, head_dim] (uint8, int8 or float8_e4m3fn) and scales k_scale,
+    v_scale [n_pages, n_kv_heads] (float32), CUDA tensors that this object keeps
+    alive and the caller owns."""
+
+    FORMATS = {"i8": 0, "e4m3": 1}
+
+    def __init__(self, k, v, k_scale, v_scale, format: str = "i8", acc: Accelerator | None = None):
+        super().__init__(acc)
+        if format not in self.FORMATS:
+            raise ValueError(f"format {format!r} (of {tuple(self.FORMATS)})")
+        n_pages, n_kv, page, d = k.shape
+        for codes, scale in ((k, k_scale), (v, v_scale)):
+            if tuple(codes.shape) != (n_pages, n_kv, page, d) or tuple(scale.shape) != (n_pages, n_kv):
+                raise ValueError("codes are [n_pages, n_kv_heads, page_size, head_dim], scales [n_pages, n_kv_heads]")
+            if str(codes.dtype) not in ("torch.uint8", "torch.int8", "torch.float8_e4m3fn"):
+                raise TypeError(f"expected 8-bit codes, got {codes.dtype}")
+            if str(scale.dtype) != "torch.float32":
+                raise TypeError(f"expected float32 scales, got {scale.dtype}")
+            if not codes.is_contiguous() or not scale.is_contiguous():
+                raise ValueError("codes and scales must be contiguous")
+        self.tensors = (k, v, k_scale, v_scale)
+        self.n_kv_heads, self.page_size, self.head_dim = n_kv, page, d
+        c = _lib.LcKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page, n_kv, d,
+                       self.FORMATS[format])
+        self._kv = c
+
+    def _two(self, k, v, slots, writable: bool):
+        ka, rows, width, stride, dt = _rows(k, writable)
+        va, *rest = _rows(v, writable)
+        if rest != [rows, width, stride, dt]:
+            raise ValueError("k and v rows differ in shape, stride or type")
+        if width != self.n_kv_heads * self.head_dim:
+            raise ValueError(f"rows of {width} elements, the cache holds {self.n_kv_heads} x {self.head_dim}")
+        return ka, va, stride, dt, _addr(slots, "i32", rows), rows
+
+    def append(self, k, v, slots) -> None:
+        """Rows [rows, n_kv_heads, head_dim] (F32 or F16) into their slots (see lc_kv8_append)."""
+        _lib.check(self.lib.lc_kv8_append(self.ctx, self._kv, *self._two(k, v, slots, False)))
+
+    def read(self, k, v, slots) -> None:
+        """Rows [rows, n_kv_heads, head_dim] (F32 or F16) = the values at their slots (see lc_kv8_read)."""
+        _lib.check(self.lib.lc_kv8_read(self.ctx, self._kv, *self._two(k, v, slots, True)))
+
+    def attention(self, q, out, q_start, kv_lens, table, max_q: int = 1, scale: float | None = None) -> None:
+        """Causal attention of rows q [rows, n_heads, head_dim] (see
+        lc_kv8_attention); table [n_seqs, stride]; q_start [n_seqs + 1], or None
+        when every sequence has one query; scale None: 1 / sqrt(head_dim)."""
+        qa, rows, width, qs, dt = _rows(q)
+        oa, orows, owidth, os_, odt = _rows(out, True)
+        if (orows, owidth, odt) != (rows, width, dt):
+            raise ValueError("q and out differ in shape or type")
+        d = self.head_dim
+        if width == 0 or width % d:
+            raise ValueError(f"rows of {width} elements, head_dim {d}")
+        n, stride = table.shape
+        _lib.check(self.lib.lc_kv8_attention(
+            self.ctx, self._kv, qa, oa, qs, os_, dt, rows, None if q_start is None else _addr(q_start, "i32", n + 1),
+            _addr(kv_lens, "i32", n), _addr(table, "i32", n * stride), stride, n, max_q, width // d,
+            d ** -0.5 if scale is None else scale))
+
+
 class CudaSiLU(_CudaKernel, ISiLU):
     """SiLU.java:32-40 on the GPU."""
 
@@ -316,6 +444,9 @@ class CudaKernelFactory(IKernelFactory):
 
     def createRoPE(self, acc=None) -> CudaRoPE:
         return CudaRoPE(acc)
+
+    def createPages(self, acc=None) -> CudaPages:
+        return CudaPages(acc)
 
     def createSiLU(self, acc=None) -> CudaSiLU:
         return CudaSiLU(acc)
