@@ -205,8 +205,11 @@ int lc_argmax(lc_context* ctx, const float* values, int n, int32_t* out_index);
  * Row buffers ("rows") are F32 or F16 (dtype 0 or 1, as
  * lc_model_upload_tensor), row i at i * stride elements; int32 arrays and rows
  * may be host or device memory, the cache itself is device memory.  With
- * device memory throughout, the calls only enqueue on the context's stream,
- * allocate nothing and can be captured in a CUDA graph. */
+ * device memory throughout, the calls only enqueue on the context's stream
+ * and can be captured in a CUDA graph; the first lc_kv8_attention of a
+ * context allocates its workspace (make it before a capture), whose size is
+ * the same for all calls.  Graphs captured from one context share it:
+ * replay them one after the other. */
 
 enum { LC_ROPE_INTERLEAVED = 0, /* pairs (2j, 2j + 1), as lc_rope */
        LC_ROPE_HALF = 1 };      /* pairs (j, j + rot_dim / 2) */

@@ -84,6 +84,7 @@ struct lc_context {
     void* gemm_scratch = nullptr;   // row scales, pre-split activations, partial sums
     size_t gemm_scratch_bytes = 0;
     bool gemm_ready = false;        // shared-memory attribute of the GEMM kernel set
+    void* kv8_ws = nullptr;         // workspace of lc_kv8_attention, one size for all calls
 };
 
 extern "C" int lc_device_count(int* count) {
@@ -122,6 +123,7 @@ extern "C" int lc_context_destroy(lc_context* c) {
     for (void* p : c->pool) cudaFree(p);
     if (c->attn_scratch) cudaFree(c->attn_scratch);
     if (c->gemm_scratch) cudaFree(c->gemm_scratch);
+    if (c->kv8_ws) cudaFree(c->kv8_ws);
     if (c->d_err) cudaFree(c->d_err);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
@@ -910,7 +912,21 @@ extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, 
         a.n_heads = n_heads;
         a.dtype = dtype;
         a.scale = scale;
-        return s.finish(launch_kv8_attention(view, a, c->sms, c->stream));
+        if (!c->kv8_ws) {
+            cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+            CK(cudaStreamIsCapturing(c->stream, &capture), "cudaStreamIsCapturing");
+            if (capture != cudaStreamCaptureStatusNone)
+                return fail(LC_ERR_STATE, "the first lc_kv8_attention of a context allocates its workspace: make it before the capture");
+            void* ws = nullptr;
+            CK(cudaMalloc(&ws, kv8_attention_ws_bytes(c->sms)), "attention workspace");
+            const cudaError_t e = kv8_attention_prepare(ws, c->sms, c->stream);
+            if (e != cudaSuccess) {
+                cudaFree(ws);
+                return cuda_fail(e, "attention workspace");
+            }
+            c->kv8_ws = ws;
+        }
+        return s.finish(launch_kv8_attention(view, a, c->sms, c->kv8_ws, c->stream));
     });
 }
 

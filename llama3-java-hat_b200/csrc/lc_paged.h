@@ -68,6 +68,10 @@ struct Kv8Attention {
     int table_stride, n_seqs, rows, max_q, n_heads, dtype;
     float scale;
 };
-cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, cudaStream_t st);
+// Workspace of one call at a time: its size depends on the device alone.
+// prepare clears its counters and sets the kernels' attributes, once.
+size_t kv8_attention_ws_bytes(int num_sms);
+cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st);
+cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, cudaStream_t st);
 
 }  // namespace lc
