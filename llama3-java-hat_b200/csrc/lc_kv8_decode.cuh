@@ -47,12 +47,12 @@ struct DecShape {
     static constexpr int kPartFloats = kDecRows * (D + 2);  // O[8][D], m[8], l[8]
 };
 
-// Workspace: a counter per CTA (zero between calls), then per warp two pieces
-// and per CTA two joined pieces.
+// Workspace: a counter per CTA (zero between calls), then per warp a piece and
+// per CTA two joined pieces.
 inline size_t kv8_counter_bytes(int num_sms) { return ((size_t)num_sms * 2 * sizeof(int) + 255) / 256 * 256; }
 inline size_t kv8_decode_ws_bytes(int num_sms) {
     const size_t a = DecShape<64>::kCtasPerSm * DecShape<64>::kPartFloats, b = DecShape<128>::kCtasPerSm * DecShape<128>::kPartFloats;
-    return kv8_counter_bytes(num_sms) + (size_t)num_sms * (kDecWarps + 1) * 2 * (a > b ? a : b) * sizeof(float);
+    return kv8_counter_bytes(num_sms) + (size_t)num_sms * (kDecWarps + 2) * (a > b ? a : b) * sizeof(float);
 }
 
 LC_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -146,25 +146,22 @@ LC_DEV SeqInfo kv8_seq(const Kv8Attention& a, int page_shift, int s) {
     return q;
 }
 
-// A place on the line of steps.
+// A unit of the line of steps: rows [8 chunk, 8 chunk + 8) of the (query, head)
+// pairs of one sequence and kv head, and a step within it.
 struct DecCursor {
-    int s, head, chunk;  // unit
-    int step, steps;     // within the unit
     SeqInfo q;
-    int chunks;          // of the sequence
+    int s, head, chunk, chunks;
+    int seen;         // positions that its last row sees
+    int step, steps;  // steps up to there; at least one, which then sees nothing and writes zeros
 };
 
-// Steps of rows [8 chunk, 8 chunk + 8) of a sequence: up to the last query's
-// last position, at least one (which then sees nothing and writes zeros).
+// Positions that row `row` (query row / group) of a sequence sees.
 LC_DEV int dec_seen(const SeqInfo& q, int group, int room, int row) {
     const int j = row / group;
     const int seen = q.len - q.nq + (j < q.nq ? j : q.nq - 1) + 1;
     return seen < 0 ? 0 : seen > room ? room : seen;
 }
-LC_DEV int dec_steps(const SeqInfo& q, int group, int room, int chunk) {
-    const int seen = dec_seen(q, group, room, chunk * kDecRows + kDecRows - 1);
-    return seen <= 0 ? 1 : (seen + kDecStep - 1) / kDecStep;
-}
+LC_DEV int dec_steps(int seen) { return seen <= kDecStep ? 1 : (seen + kDecStep - 1) / kDecStep; }
 
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(kDecWarps * 32, DecShape<D>::kCtasPerSm)
@@ -189,7 +186,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         if (s < a.n_seqs) {
             const SeqInfo q = kv8_seq(a, sh, s);
             const int chunks = (q.nq * group + kDecRows - 1) / kDecRows;
-            for (int k = 0; k < chunks; ++k) cost += dec_steps(q, group, room, k);
+            for (int k = 0; k < chunks; ++k) cost += dec_steps(dec_seen(q, group, room, k * kDecRows + kDecRows - 1));
             cost *= c.n_kv;
         }
         unsigned v = cost;
@@ -211,57 +208,72 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     }
     if (tid == 0) prefix[a.n_seqs] = carry;
     __syncthreads();
-    const long long total = carry;
+    // Worker w has steps [begin_of(w), begin_of(w + 1)): equal shares, the first
+    // `extra` workers one step more.
+    const unsigned total = carry;
     if (total == 0) return;
-    const long long workers = min((long long)gridDim.x * kDecWarps, total);
-    auto begin_of = [&](long long w) { return w * total / workers; };
-    auto worker_of = [&](long long x) { return ((x + 1) * workers - 1) / total; };  // the worker of step x
-    const long long w0 = (long long)blockIdx.x * kDecWarps;  // this CTA's first worker
+    const unsigned workers = min(gridDim.x * kDecWarps, total);
+    const unsigned share = total / workers, extra = total - share * workers;
+    auto begin_of = [&](unsigned w) { return w * share + min(w, extra); };
+    auto worker_of = [&](unsigned x) {
+        const unsigned big = extra * (share + 1);
+        return x < big ? x / (share + 1) : extra + (x - big) / share;
+    };
+    const unsigned w0 = blockIdx.x * kDecWarps;  // this CTA's first worker
     if (w0 >= workers) return;
-    const int my_warps = (int)min((long long)kDecWarps, workers - w0);
-    const long long cta_lo = begin_of(w0), cta_hi = begin_of(w0 + my_warps);
-    const long long lo = warp < my_warps ? begin_of(w0 + warp) : cta_hi;
-    const long long hi = warp < my_warps ? begin_of(w0 + warp + 1) : cta_hi;
+    const unsigned my_warps = min((unsigned)kDecWarps, workers - w0);
+    const unsigned cta_lo = begin_of(w0), cta_hi = begin_of(w0 + my_warps);
+    const unsigned lo = warp < my_warps ? begin_of(w0 + warp) : cta_hi;
+    const unsigned hi = warp < my_warps ? begin_of(w0 + warp + 1) : cta_hi;
 
-    auto locate = [&](DecCursor& cur, long long x) {  // the unit and step at place x
+    auto set_chunk = [&](DecCursor& cur, int chunk) {
+        cur.chunk = chunk;
+        cur.seen = dec_seen(cur.q, group, room, chunk * kDecRows + kDecRows - 1);
+        cur.steps = dec_steps(cur.seen);
+    };
+    auto set_seq = [&](DecCursor& cur, int s) {
+        cur.s = s;
+        cur.q = kv8_seq(a, sh, s);
+        cur.chunks = (cur.q.nq * group + kDecRows - 1) / kDecRows;
+    };
+    auto locate = [&](DecCursor& cur, unsigned x) {  // the unit and step at place x
         int a0 = 0, a1 = a.n_seqs;
         while (a1 - a0 > 1) {
             const int mid = (a0 + a1) >> 1;
             if (prefix[mid] <= x) a0 = mid;
             else a1 = mid;
         }
-        cur.s = a0;
-        cur.q = kv8_seq(a, sh, a0);
-        cur.chunks = (cur.q.nq * group + kDecRows - 1) / kDecRows;
-        unsigned rem = (unsigned)(x - prefix[a0]);
+        set_seq(cur, a0);
+        unsigned rem = x - prefix[a0];
         const unsigned per = (prefix[a0 + 1] - prefix[a0]) / c.n_kv;
         cur.head = rem / per;
         rem -= cur.head * per;
-        cur.chunk = 0;
-        cur.steps = dec_steps(cur.q, group, room, 0);
+        set_chunk(cur, 0);
         while (rem >= (unsigned)cur.steps) {
             rem -= cur.steps;
-            cur.steps = dec_steps(cur.q, group, room, ++cur.chunk);
+            set_chunk(cur, cur.chunk + 1);
         }
         cur.step = rem;
     };
     auto next_unit = [&](DecCursor& cur) {
         cur.step = 0;
-        if (++cur.chunk == cur.chunks) {
-            cur.chunk = 0;
-            if (++cur.head == c.n_kv) {
-                cur.head = 0;
-                do ++cur.s;
-                while (cur.s < a.n_seqs - 1 && prefix[cur.s + 1] == prefix[cur.s]);
-                cur.q = kv8_seq(a, sh, cur.s);
-                cur.chunks = (cur.q.nq * group + kDecRows - 1) / kDecRows;
-            }
+        if (cur.chunk + 1 < cur.chunks) {
+            set_chunk(cur, cur.chunk + 1);
+            return;
         }
-        cur.steps = dec_steps(cur.q, group, room, cur.chunk);
+        if (++cur.head == c.n_kv) {
+            cur.head = 0;
+            int s = cur.s;
+            do ++s;
+            while (s < a.n_seqs - 1 && prefix[s + 1] == prefix[s]);
+            set_seq(cur, s);
+        }
+        if (cur.chunk != 0 || cur.head == 0) set_chunk(cur, 0);
     };
 
-    float* const warp_parts = ws;                                                            // [workers][2]
-    float* const cta_parts = ws + (size_t)gridDim.x * kDecWarps * 2 * S::kPartFloats;       // [CTAs][2]
+    float* const warp_parts = ws;                                                   // [workers]
+    float* const cta_parts = ws + (size_t)gridDim.x * kDecWarps * S::kPartFloats;  // [CTAs][2]
+    auto ring_part = [&](int w) { return reinterpret_cast<float*>(smem + w * kDecStages * S::kStageBytes); };
     const uint32_t ring = smem_u32(smem) + warp * kDecStages * S::kStageBytes;
     const int row_sel = sh == 4 ? 1 : 0;  // pages of 16 tokens: a step's second half is another page
 
@@ -272,18 +284,18 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         return (T*)a.out + (int64_t)(cur.q.row0 + j) * a.out_stride + (cur.head * group + row - j * group) * D;
     };
 
+    DecCursor cur;  // in the end: the unit of step hi - 1, cur.step behind that step
     if (lo < hi) {
         // ---- issue side ----
         DecCursor ic;  // the next step to ask for
         locate(ic, lo);
-        long long ahead = lo;
+        unsigned ahead = lo;
         int id0 = 0, id1 = 0;  // its pages
         auto ids = [&]() {
-            const int seen = dec_seen(ic.q, group, room, ic.chunk * kDecRows + kDecRows - 1);
             const int32_t* row = a.table + (int64_t)ic.s * a.table_stride;
             const int t0 = ic.step * kDecStep;
-            id0 = t0 < seen ? row[t0 >> sh] : -1;
-            id1 = !row_sel ? id0 : t0 + 16 < seen ? row[(t0 + 16) >> sh] : -1;
+            id0 = t0 < ic.seen ? row[t0 >> sh] : -1;
+            id1 = !row_sel ? id0 : t0 + 16 < ic.seen ? row[(t0 + 16) >> sh] : -1;
         };
         ids();
         const int off0 = lane * 16;  // this lane's first chunk of a half
@@ -321,21 +333,21 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             }
             cp_async_commit();
         };
+        const DecCursor ic0 = ic;
         for (int k = 0; k < kDecStages - 1; ++k) issue(k);
 
         // ---- compute side ----
-        DecCursor cur;
-        locate(cur, lo);
+        cur = ic0;
         int stage = 0;
-        for (long long x = lo; x < hi;) {
+        for (unsigned x = lo; x < hi;) {
             // One segment: steps [cur.step, last) of the unit.
             const int first_step = cur.step;
-            const int last = (int)min((long long)cur.steps, cur.step + (hi - x));
+            const int last = min(cur.steps, cur.step + (int)(hi - x));
             const int row = cur.chunk * kDecRows + g, j = row / group;
             const bool live = j < cur.q.nq;
             const int seen = live ? dec_seen(cur.q, group, room, row) : 0;
             const int seen_min = dec_seen(cur.q, group, room, cur.chunk * kDecRows);
-            const int seen_max = dec_seen(cur.q, group, room, cur.chunk * kDecRows + kDecRows - 1);
+            const int seen_max = cur.seen;
             const bool all_live = (cur.chunk + 1) * kDecRows <= cur.q.nq * group;
             // Query fragments: k-step ks of thread t covers 4 neighbouring elements.
             uint32_t qa[KS][4];
@@ -496,7 +508,14 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                         for (int i = 0; i < NV; ++i) dst[(2 * t + b) * NV + i] = (T)(l == 0.0f ? 0.0f : (o[i][b] + o[i][2 + b]) * f);
                 }
             } else {
-                float* part = warp_parts + ((size_t)(w0 + warp) * 2 + (first_step == 0 ? 1 : 0)) * S::kPartFloats;
+                // The warp's last segment: its ring is read out and takes the piece.
+                // An earlier one (the end of a unit begun before): global memory.
+                float* part = warp_parts + (size_t)(w0 + warp) * S::kPartFloats;
+                if (x == hi) {
+                    cp_async_wait<0>();
+                    __syncwarp();
+                    part = ring_part(warp);
+                }
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -508,82 +527,133 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             }
             if (cur.step == cur.steps && x < hi) next_unit(cur);
         }
-        cp_async_wait<0>();
     }
+    __shared__ int done_unit[2];  // cross-CTA units whose last piece this CTA brought
+    if (tid < 2) done_unit[tid] = 0;
     __syncthreads();
 
     // ---- joining pieces ----
-    // Sum of n pieces (piece(i) gives the i-th) by one warp: lane's four
-    // neighbouring elements of rows (lane * 4 + 128 k) / D.
+    // Adds n pieces (piece(i) is the i-th) by one warp, two at a time so that
+    // their loads are under way together: lane's four neighbouring elements of
+    // rows (lane * 4 + 128 k) / D.
     constexpr int KM = kDecRows * D / 128;
-    auto join = [&](int n, auto piece, float* to, const DecCursor& cur, bool finish) {
-        float mx[KM], sum[KM];
-        float4 acc[KM];
+    struct Sum {
+        float m[KM], l[KM];
+        float4 o[KM];
+    };
+    auto clear = [&](Sum& z) {
 #pragma unroll
-        for (int k = 0; k < KM; ++k) mx[k] = -INFINITY, sum[k] = 0.0f, acc[k] = make_float4(0, 0, 0, 0);
-        for (int i = 0; i < n; ++i)
+        for (int k = 0; k < KM; ++k) z.m[k] = -INFINITY, z.l[k] = 0.0f, z.o[k] = make_float4(0, 0, 0, 0);
+    };
+    auto add = [&](Sum& z, int n, auto piece) {
+        for (int i0 = 0; i0 < n; i0 += 2) {
+            float pm[2][KM], pl[2][KM];
+            float4 po[2][KM];
 #pragma unroll
-            for (int k = 0; k < KM; ++k) mx[k] = fmaxf(mx[k], __ldcg(piece(i) + kDecRows * D + (lane * 4 + 128 * k) / D));
-        for (int i = 0; i < n; ++i) {
-            const float* p = piece(i);
+            for (int i = 0; i < 2; ++i) {
+                if (i0 + i >= n) continue;
+                const float* p = piece(i0 + i);
 #pragma unroll
-            for (int k = 0; k < KM; ++k) {
-                const int e = lane * 4 + 128 * k, r = e / D;
-                const float pm = __ldcg(p + kDecRows * D + r);
-                const float f = pm == -INFINITY ? 0.0f : ex2(pm - mx[k]);
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(p + e));
-                sum[k] += f * __ldcg(p + kDecRows * D + kDecRows + r);
-                acc[k].x += f * v.x, acc[k].y += f * v.y, acc[k].z += f * v.z, acc[k].w += f * v.w;
+                for (int k = 0; k < KM; ++k) {
+                    const int e = lane * 4 + 128 * k, r = e / D;
+                    pm[i][k] = p[kDecRows * D + r];
+                    pl[i][k] = p[kDecRows * D + kDecRows + r];
+                    po[i][k] = *reinterpret_cast<const float4*>(p + e);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i0 + i >= n) continue;
+#pragma unroll
+                for (int k = 0; k < KM; ++k) {
+                    const float m = fmaxf(z.m[k], pm[i][k]);
+                    const float f = z.m[k] == -INFINITY ? 0.0f : ex2(z.m[k] - m), h = pm[i][k] == -INFINITY ? 0.0f : ex2(pm[i][k] - m);
+                    z.m[k] = m;
+                    z.l[k] = z.l[k] * f + pl[i][k] * h;
+                    z.o[k].x = z.o[k].x * f + po[i][k].x * h, z.o[k].y = z.o[k].y * f + po[i][k].y * h;
+                    z.o[k].z = z.o[k].z * f + po[i][k].z * h, z.o[k].w = z.o[k].w * f + po[i][k].w * h;
+                }
             }
         }
+    };
+    auto store = [&](const Sum& z, float* to) {
 #pragma unroll
         for (int k = 0; k < KM; ++k) {
             const int e = lane * 4 + 128 * k, r = e / D;
-            if (finish) {
-                T* dst = out_row(cur, r);
-                if (!dst) continue;
-                dst += e % D;
-                const float inv = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
-                dst[0] = (T)(acc[k].x * inv), dst[1] = (T)(acc[k].y * inv);
-                dst[2] = (T)(acc[k].z * inv), dst[3] = (T)(acc[k].w * inv);
-            } else {
-                *reinterpret_cast<float4*>(to + e) = acc[k];
-                if (e % D == 0) to[kDecRows * D + r] = mx[k], to[kDecRows * D + kDecRows + r] = sum[k];
-            }
+            *reinterpret_cast<float4*>(to + e) = z.o[k];
+            if (e % D == 0) to[kDecRows * D + r] = z.m[k], to[kDecRows * D + kDecRows + r] = z.l[k];
+        }
+    };
+    auto finish = [&](const Sum& z, const DecCursor& u) {
+#pragma unroll
+        for (int k = 0; k < KM; ++k) {
+            const int e = lane * 4 + 128 * k;
+            T* dst = out_row(u, e / D);
+            if (!dst) continue;
+            dst += e % D;
+            const float inv = z.l[k] == 0.0f ? 0.0f : 1.0f / z.l[k];
+            dst[0] = (T)(z.o[k].x * inv), dst[1] = (T)(z.o[k].y * inv);
+            dst[2] = (T)(z.o[k].z * inv), dst[3] = (T)(z.o[k].w * inv);
         }
     };
     // A warp joins the pieces of the unit that begins in it and goes on, and
     // warp 0 those of the unit that was under way at the CTA's start.
-    if (lo >= hi) return;
-    for (int side = warp == 0 ? 0 : 1; side < 2; ++side) {
-        DecCursor cur;
-        const long long at = side == 0 ? lo : hi - 1;
-        locate(cur, at);
-        const long long u0 = at - cur.step, u1 = u0 + cur.steps;  // the unit's place on the line
+    for (int side = warp == 0 ? 0 : 1; side < 2 && lo < hi; ++side) {
+        DecCursor u = cur;
+        unsigned u0 = hi - u.step;  // the unit's place on the line
+        if (side == 0) {
+            locate(u, lo);
+            u0 = lo - u.step;
+        }
+        const unsigned u1 = u0 + u.steps;
         if (side == 0 ? u0 >= lo : !(u0 >= lo && u1 > hi)) continue;
-        const long long end = min(u1, cta_hi);
-        const int wn = (int)(worker_of(end - 1) - (w0 + warp)) + 1;  // warps with a piece, from this one
-        auto mine = [&](int i) -> const float* {
-            return warp_parts + ((size_t)(w0 + warp + i) * 2 + (i == 0 ? side : 0)) * S::kPartFloats;
-        };
+        const int wn = (int)(worker_of(min(u1, cta_hi) - 1) - (w0 + warp)) + 1;  // warps with a piece, from this one
+        Sum z;
+        clear(z);
+        // All but the last lie in the ring; so does the last unless that warp went on to another unit.
+        const bool tail_out = begin_of(w0 + warp + wn) > u1;
+        add(z, wn, [&](int i) -> const float* {
+            return i == wn - 1 && tail_out ? warp_parts + (size_t)(w0 + warp + i) * S::kPartFloats : ring_part(warp + i);
+        });
         if (u0 >= cta_lo && u1 <= cta_hi) {
-            join(wn, mine, nullptr, cur, true);
+            finish(z, u);
             continue;
         }
-        join(wn, mine, cta_parts + ((size_t)blockIdx.x * 2 + side) * S::kPartFloats, cur, false);
+        store(z, cta_parts + ((size_t)blockIdx.x * 2 + side) * S::kPartFloats);
         const int first = (int)(worker_of(u0) / kDecWarps), final = (int)(worker_of(u1 - 1) / kDecWarps);
         __threadfence();
         __syncwarp();
-        int old = 0;
-        if (lane == 0) old = atomicAdd(counters + first, 1);
-        old = __shfl_sync(0xffffffffu, old, 0);
-        if (old != final - first) continue;
-        if (lane == 0) counters[first] = 0;
-        __threadfence();
-        auto all = [&](int i) -> const float* {
-            return cta_parts + ((size_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * S::kPartFloats;
-        };
-        join(final - first + 1, all, nullptr, cur, true);
+        if (lane == 0 && atomicAdd(counters + first, 1) == final - first) {
+            counters[first] = 0;
+            __threadfence();
+            done_unit[side] = 1 + warp;
+        }
+    }
+    __syncthreads();
+    // The pieces of a unit that spans CTAs, by all warps of the last CTA to
+    // finish: each a range of them, then one adds the warps' sums in order.
+    for (int side = 0; side < 2; ++side) {
+        if (!done_unit[side]) continue;  // uniform over the CTA
+        DecCursor u;
+        const unsigned at = side == 0 ? cta_lo : begin_of(w0 + done_unit[side]) - 1;
+        locate(u, at);
+        const unsigned u0 = at - u.step, u1 = u0 + u.steps;
+        const int first = (int)(worker_of(u0) / kDecWarps), n = (int)(worker_of(u1 - 1) / kDecWarps) - first + 1;
+        const int i0 = n * warp / kDecWarps, i1 = n * (warp + 1) / kDecWarps;
+        Sum z;
+        clear(z);
+        add(z, i1 - i0, [&](int i) -> const float* {
+            return cta_parts + ((size_t)(first + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0)) * S::kPartFloats;
+        });
+        __syncthreads();  // the ring's pieces are read
+        store(z, ring_part(warp));
+        __syncthreads();
+        if (warp == 0) {
+            clear(z);
+            add(z, kDecWarps, [&](int i) -> const float* { return ring_part(i); });
+            finish(z, u);
+        }
+        __syncthreads();
     }
 }
 
