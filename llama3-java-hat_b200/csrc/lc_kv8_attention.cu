@@ -28,7 +28,8 @@ size_t kv8_attention_ws_bytes(int num_sms) { return kv8_decode_ws_bytes(num_sms)
 cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st) {
     for (int i = 0; i < 8; ++i) {
         const cudaError_t e = by_shape(i & 1, (i >> 1) & 1, i & 4 ? 128 : 64, [](auto row, auto fmt, auto d) {
-            return kv8_decode_prepare<decltype(row), fmt.value, d.value>();
+            const cudaError_t e = kv8_decode_prepare<decltype(row), fmt.value, d.value, 1>();
+            return e != cudaSuccess ? e : kv8_decode_prepare<decltype(row), fmt.value, d.value, 2>();
         });
         if (e != cudaSuccess) return e;
     }
@@ -37,7 +38,11 @@ cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st) {
 
 cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, cudaStream_t st) {
     return by_shape(a.dtype, c.format, c.head_dim, [&](auto row, auto fmt, auto d) {
-        return launch_kv8_decode<decltype(row), fmt.value, d.value>(c, a, num_sms, ws, st);
+        // Units of 4 rows where a sequence has no more, of 8 where it has:
+        // more rows share one reading of the codes.
+        return a.n_heads / c.n_kv * a.max_q <= 4
+                   ? launch_kv8_decode<decltype(row), fmt.value, d.value, 1>(c, a, num_sms, ws, st)
+                   : launch_kv8_decode<decltype(row), fmt.value, d.value, 2>(c, a, num_sms, ws, st);
     });
 }
 

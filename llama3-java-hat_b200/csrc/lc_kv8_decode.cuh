@@ -5,11 +5,15 @@
 // 8 rows, a row being one (query, head) pair that shares the kv head.
 //
 // Products.  mma.m16n8k16 on f16: codes are exact in f16 (signed bytes and
-// e4m3 both), a query row is split into f16 hi + lo under a power-of-two row
-// scale (22 bits), hi in MMA row g and lo in row g + 8, so both halves of the
-// sum sit in one thread and the split costs no instruction beyond the 8 rows
-// that GQA leaves unused anyway.  The weights p are split the same way.
-// tcgen05 has no use for 8 rows of 128.
+// e4m3 both).  Keys and values are the 16-row operand (tokens, or elements of
+// the head), the rows of the unit the 8-column one: row h is split into f16
+// hi + lo under a power-of-two row scale (22 bits), columns 2h and 2h + 1 of a
+// tile, so both halves of a sum meet in one thread and four rows, a common
+// group, fill a tile.  The weights p are split the same way and change from
+// the score's layout (tokens over lanes) to the operand's (tokens along k)
+// through 512 bytes of shared memory.  With the rows as the 16-row operand
+// instead half the products and half the exponentials were spent on empty
+// rows.  tcgen05 has no use for 8 rows of 128.
 //
 // Softmax.  In powers of two, with a running maximum that is only moved when
 // a score passes it by more than 1; p is held as 2^(x - m + 12), times the
@@ -17,9 +21,9 @@
 // below 2^15 and leaves 37 bits between the largest weight and the smallest
 // step of the lo half.
 //
-// Work.  A step is 32 tokens of one (sequence, kv head, 8 rows); all steps of
+// Work.  A step is 32 tokens of one (sequence, kv head, 4 or 8 rows); all steps of
 // the call form one line, cut into equal pieces, one per warp, so ragged
-// lengths leave no warp idle.  A unit (all steps of 8 rows) that one warp
+// lengths leave no warp idle.  A unit (all steps of those rows) that one warp
 // covers is written at once; pieces of a unit are joined first within the
 // CTA, then by the last CTA to finish, always in the order of the line, so
 // the result does not depend on timing.
@@ -34,24 +38,28 @@
 
 namespace lc {
 
-constexpr int kDecWarps = 8;    // per CTA
-constexpr int kDecStages = 3;   // ring stages per warp
-constexpr int kDecStep = 32;    // tokens of a step
-constexpr int kDecRows = 8;     // (query, head) rows of a unit
+constexpr int kDecWarps = 8;  // per CTA
+constexpr int kDecStep = 32;  // tokens of a step
 
-template <int D>
+// D: head size; NR: tiles of 4 rows of a unit, 1 or 2.
+template <int D, int NR>
 struct DecShape {
+    static constexpr int kRows = 4 * NR;
     static constexpr int kCtasPerSm = D == 64 ? 2 : 1;
-    static constexpr int kStageBytes = 2 * kDecStep * D + 32;  // K, V, four scales and the page flags
-    static constexpr int kRingBytes = kDecWarps * kDecStages * kStageBytes;
-    static constexpr int kPartFloats = kDecRows * (D + 2);  // O[8][D], m[8], l[8]
+    static constexpr int kStages = 3;
+    static constexpr int kStageBytes = 2 * kDecStep * D + 32;           // K, V, four scales and the page flags
+    static constexpr int kWarpBytes = kStages * kStageBytes + 512 * NR;  // and the weights
+    static constexpr int kRingBytes = kDecWarps * kWarpBytes;
+    static constexpr int kPartFloats = kRows * (D + 2);  // O[rows][D], m[rows], l[rows]
+    static_assert(kPartFloats * 4 <= kStages * kStageBytes, "a piece fits the warp's ring");
 };
 
 // Workspace: a counter per CTA (zero between calls), then per warp a piece and
 // per CTA two joined pieces.
 inline size_t kv8_counter_bytes(int num_sms) { return ((size_t)num_sms * 2 * sizeof(int) + 255) / 256 * 256; }
 inline size_t kv8_decode_ws_bytes(int num_sms) {
-    const size_t a = DecShape<64>::kCtasPerSm * DecShape<64>::kPartFloats, b = DecShape<128>::kCtasPerSm * DecShape<128>::kPartFloats;
+    const size_t a = DecShape<64, 2>::kCtasPerSm * DecShape<64, 2>::kPartFloats;
+    const size_t b = DecShape<128, 2>::kCtasPerSm * DecShape<128, 2>::kPartFloats;
     return kv8_counter_bytes(num_sms) + (size_t)num_sms * (kDecWarps + 2) * (a > b ? a : b) * sizeof(float);
 }
 
@@ -115,6 +123,9 @@ LC_DEV uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
 }
+LC_DEV void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 LC_DEV uint2 lds64(uint32_t a) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
@@ -146,7 +157,7 @@ LC_DEV SeqInfo kv8_seq(const Kv8Attention& a, int page_shift, int s) {
     return q;
 }
 
-// A unit of the line of steps: rows [8 chunk, 8 chunk + 8) of the (query, head)
+// A unit of the line of steps: rows [R chunk, R chunk + R) of the (query, head)
 // pairs of one sequence and kv head, and a step within it.
 struct DecCursor {
     SeqInfo q;
@@ -163,12 +174,13 @@ LC_DEV int dec_seen(const SeqInfo& q, int group, int room, int row) {
 }
 LC_DEV int dec_steps(int seen) { return seen <= kDecStep ? 1 : (seen + kDecStep - 1) / kDecStep; }
 
-template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kDecWarps * 32, DecShape<D>::kCtasPerSm)
+template <typename T, int FMT, int D, int NR>
+__global__ void __launch_bounds__(kDecWarps * 32, DecShape<D, NR>::kCtasPerSm)
 kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict__ counters) {
-    using S = DecShape<D>;
-    constexpr int KS = D / 16;   // k-steps of a score
-    constexpr int NV = D / 8;    // n-tiles of the output
+    using S = DecShape<D, NR>;
+    constexpr int R = S::kRows;
+    constexpr int KS = D / 16;  // k-steps of a score, and tiles of 16 elements of the output
+    constexpr int E = D / 8;    // elements of a row that a thread holds
     extern __shared__ __align__(128) uint8_t smem[];
     unsigned* prefix = reinterpret_cast<unsigned*>(smem + S::kRingBytes);  // [n_seqs + 1] steps before sequence s
     __shared__ unsigned scan[kDecWarps];
@@ -185,8 +197,8 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         unsigned cost = 0;
         if (s < a.n_seqs) {
             const SeqInfo q = kv8_seq(a, sh, s);
-            const int chunks = (q.nq * group + kDecRows - 1) / kDecRows;
-            for (int k = 0; k < chunks; ++k) cost += dec_steps(dec_seen(q, group, room, k * kDecRows + kDecRows - 1));
+            const int chunks = (q.nq * group + R - 1) / R;
+            for (int k = 0; k < chunks; ++k) cost += dec_steps(dec_seen(q, group, room, k * R + R - 1));
             cost *= c.n_kv;
         }
         unsigned v = cost;
@@ -228,13 +240,13 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
 
     auto set_chunk = [&](DecCursor& cur, int chunk) {
         cur.chunk = chunk;
-        cur.seen = dec_seen(cur.q, group, room, chunk * kDecRows + kDecRows - 1);
+        cur.seen = dec_seen(cur.q, group, room, chunk * R + R - 1);
         cur.steps = dec_steps(cur.seen);
     };
     auto set_seq = [&](DecCursor& cur, int s) {
         cur.s = s;
         cur.q = kv8_seq(a, sh, s);
-        cur.chunks = (cur.q.nq * group + kDecRows - 1) / kDecRows;
+        cur.chunks = (cur.q.nq * group + R - 1) / R;
     };
     auto locate = [&](DecCursor& cur, unsigned x) {  // the unit and step at place x
         int a0 = 0, a1 = a.n_seqs;
@@ -273,13 +285,14 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
 
     float* const warp_parts = ws;                                                   // [workers]
     float* const cta_parts = ws + (size_t)gridDim.x * kDecWarps * S::kPartFloats;  // [CTAs][2]
-    auto ring_part = [&](int w) { return reinterpret_cast<float*>(smem + w * kDecStages * S::kStageBytes); };
-    const uint32_t ring = smem_u32(smem) + warp * kDecStages * S::kStageBytes;
+    auto ring_part = [&](int w) { return reinterpret_cast<float*>(smem + w * S::kWarpBytes); };
+    const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
+    const uint32_t weights = ring + S::kStages * S::kStageBytes;
     const int row_sel = sh == 4 ? 1 : 0;  // pages of 16 tokens: a step's second half is another page
 
-    // Writes row r (0..7 of the unit at `cur`) of the result.
+    // Row r of the unit at `cur` in the result.
     auto out_row = [&](const DecCursor& cur, int r) -> T* {
-        const int row = cur.chunk * kDecRows + r, j = row / group;
+        const int row = cur.chunk * R + r, j = row / group;
         if (j >= cur.q.nq) return nullptr;
         return (T*)a.out + (int64_t)(cur.q.row0 + j) * a.out_stride + (cur.head * group + row - j * group) * D;
     };
@@ -334,7 +347,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             cp_async_commit();
         };
         const DecCursor ic0 = ic;
-        for (int k = 0; k < kDecStages - 1; ++k) issue(k);
+        for (int k = 0; k < S::kStages - 1; ++k) issue(k);
 
         // ---- compute side ----
         cur = ic0;
@@ -343,16 +356,24 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             // One segment: steps [cur.step, last) of the unit.
             const int first_step = cur.step;
             const int last = min(cur.steps, cur.step + (int)(hi - x));
-            const int row = cur.chunk * kDecRows + g, j = row / group;
-            const bool live = j < cur.q.nq;
-            const int seen = live ? dec_seen(cur.q, group, room, row) : 0;
-            const int seen_min = dec_seen(cur.q, group, room, cur.chunk * kDecRows);
+            const int seen_min = dec_seen(cur.q, group, room, cur.chunk * R);
             const int seen_max = cur.seen;
-            const bool all_live = (cur.chunk + 1) * kDecRows <= cur.q.nq * group;
-            // Query fragments: k-step ks of thread t covers 4 neighbouring elements.
-            uint32_t qa[KS][4];
-            float qf;
-            {
+            const bool all_live = (cur.chunk + 1) * R <= cur.q.nq * group;
+            // Rows 4 r + t are this thread's in scores and output.
+            int seen[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int row = cur.chunk * R + 4 * r + t;
+                seen[r] = row < cur.q.nq * group ? dec_seen(cur.q, group, room, row) : 0;
+            }
+            // Query columns: this thread holds column g of tile r, the hi (g even)
+            // or lo part of row 4 r + g / 2; k-step ks covers 4 neighbouring elements.
+            uint32_t qb[NR][KS][2];
+            float qf[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int row = cur.chunk * R + 4 * r + (g >> 1), j = row / group;
+                const bool live = j < cur.q.nq;
                 float v[KS * 4];
                 const T* q = (const T*)a.q + (int64_t)(cur.q.row0 + (live ? j : 0)) * a.q_stride +
                              (cur.head * group + (live ? row - j * group : 0)) * D;
@@ -368,22 +389,30 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                 int e = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
                 e = max(-126, min(126, e));
                 const float up = __int_as_float((127 + e) << 23);
-                qf = a.scale * 1.4426950408889634f * __int_as_float((127 - e) << 23);
+                const float down = a.scale * 1.4426950408889634f * __int_as_float((127 - e) << 23);
+                qf[r] = __shfl_sync(0xffffffffu, down, 8 * t);  // of row 4 r + t: column 2 t
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    split_f16(v[4 * ks] * up, v[4 * ks + 1] * up, qa[ks][0], qa[ks][1]);
-                    split_f16(v[4 * ks + 2] * up, v[4 * ks + 3] * up, qa[ks][2], qa[ks][3]);
+                    uint32_t h0, l0, h1, l1;
+                    split_f16(v[4 * ks] * up, v[4 * ks + 1] * up, h0, l0);
+                    split_f16(v[4 * ks + 2] * up, v[4 * ks + 3] * up, h1, l1);
+                    qb[r][ks][0] = (g & 1) ? l0 : h0;
+                    qb[r][ks][1] = (g & 1) ? l1 : h1;
                 }
             }
-            float o[NV][4];
+            float o[NR][KS][4];
+            float m[NR], l[NR], vref = 0.0f, vinv = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-            float m = -INFINITY, l = 0.0f, vref = 0.0f, vinv = 0.0f;
+            for (int r = 0; r < NR; ++r) {
+                m[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.0f;
+            }
 
             for (; cur.step < last; ++cur.step, ++x) {
-                cp_async_wait<kDecStages - 2>();
+                cp_async_wait<S::kStages - 2>();
                 __syncwarp();  // the stage's copies of all lanes are there, and the previous stage is read
-                issue(stage == 0 ? kDecStages - 1 : stage - 1);
+                issue(stage == 0 ? S::kStages - 1 : stage - 1);
                 const uint32_t kb = ring + stage * S::kStageBytes, vb = kb + kDecStep * D, sb = vb + kDecStep * D;
                 const uint4 sc = lds128(sb);
                 uint32_t flags;
@@ -392,79 +421,107 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                 const float vs0 = (flags & 1) ? __uint_as_float(sc.z) : 0.0f, vs1 = (flags & 2) ? __uint_as_float(sc.w) : 0.0f;
                 const int t0 = cur.step * kDecStep;
 
-                float s[4][4];
+                // Scores: 16 tokens (rows g, g + 8) by 4 rows' hi and lo columns.
+                float s[2][NR][4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+                for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) s[mt][r][0] = s[mt][r][1] = s[mt][r][2] = s[mt][r][3] = 0.0f;
 #pragma unroll
                     for (int hf = 0; hf < D / 64; ++hf) {
-                        const uint4 w = lds128(kb + n * 8 * D + ring_offset<D>(g, hf * 4 + t));
-                        const uint32_t wk[4] = {w.x, w.y, w.z, w.w};
+                        const uint4 wa = lds128(kb + mt * 16 * D + ring_offset<D>(g, hf * 4 + t));
+                        const uint4 wb = lds128(kb + (mt * 16 + 8) * D + ring_offset<D>(g, hf * 4 + t));
+                        const uint32_t ka[4] = {wa.x, wa.y, wa.z, wa.w}, kc[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            uint32_t b0, b1;
-                            codes_f16<FMT>(wk[k], b0, b1);
-                            mma_f16(s[n], qa[hf * 4 + k], b0, b1);
+                            uint32_t f[4];
+                            codes_f16<FMT>(ka[k], f[0], f[2]);
+                            codes_f16<FMT>(kc[k], f[1], f[3]);
+#pragma unroll
+                            for (int r = 0; r < NR; ++r) mma_f16(s[mt][r], f, qb[r][hf * 4 + k][0], qb[r][hf * 4 + k][1]);
                         }
                     }
                 }
-                // Scores in powers of two; hi and lo halves meet here.
-                float p[8];
-                const float c0 = qf * ks0, c1 = qf * ks1;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    p[2 * n] = (s[n][0] + s[n][2]) * (n < 2 ? c0 : c1);
-                    p[2 * n + 1] = (s[n][1] + s[n][3]) * (n < 2 ? c0 : c1);
-                }
+                // In powers of two; hi and lo meet here.  Token of p[r][i]: 8 i + g.
+                float p[NR][4];
                 const bool whole = t0 + kDecStep <= seen_min && flags == 3 && all_live;
-                if (!whole) {
+                bool move = false;
+                float top[NR];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int tok = t0 + (i >> 1) * 8 + 2 * t + (i & 1);
-                        if (tok >= seen || !(flags & (i < 4 ? 1 : 2))) p[i] = -INFINITY;
+                for (int r = 0; r < NR; ++r) {
+                    const float c0 = qf[r] * ks0, c1 = qf[r] * ks1;
+                    p[r][0] = (s[0][r][0] + s[0][r][1]) * c0;
+                    p[r][1] = (s[0][r][2] + s[0][r][3]) * c0;
+                    p[r][2] = (s[1][r][0] + s[1][r][1]) * c1;
+                    p[r][3] = (s[1][r][2] + s[1][r][3]) * c1;
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (t0 + 8 * i + g >= seen[r] || !(flags & (i < 2 ? 1 : 2))) p[r][i] = -INFINITY;
                     }
+                    top[r] = fmaxf(fmaxf(p[r][0], p[r][1]), fmaxf(p[r][2], p[r][3]));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 4));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 8));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 16));
+                    move |= top[r] > m[r] + 1.0f;
                 }
-                float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const bool move = top > m + 1.0f;
                 const float vmax = fmaxf(vs0, vs1);
                 if (__any_sync(0xffffffffu, move) || vmax > 4.0f * vref) {
-                    float f = 1.0f;
-                    if (move) {
-                        f = ex2(m - top);
-                        l *= f;
-                        m = top;
-                    }
+                    float fv = 1.0f;
                     if (vmax > 4.0f * vref) {
                         const float next = fmaxf(vmax, 1e-30f);
                         vinv = 1.0f / next;
-                        f *= vref * vinv;
+                        fv = vref * vinv;
                         vref = next;
                     }
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) o[i][0] *= f, o[i][1] *= f, o[i][2] *= f, o[i][3] *= f;
+                    for (int r = 0; r < NR; ++r) {
+                        float f = fv;
+                        if (top[r] > m[r] + 1.0f) {
+                            const float fm = ex2(m[r] - top[r]);
+                            l[r] *= fm;
+                            f *= fm;
+                            m[r] = top[r];
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) o[r][i][0] *= f, o[r][i][1] *= f, o[r][i][2] *= f, o[r][i][3] *= f;
+                    }
                 }
-                const float bias = m == -INFINITY ? 0.0f : 12.0f - m;
                 const float v0 = vs0 * vinv, v1 = vs1 * vinv;
-                uint32_t pa[2][4];
+                // Weights: from (token 8 i + g, row t) to columns of the operand.  A lane's
+                // 16 bytes {hi of tokens g, g + 8; hi of g + 16, g + 24; lo of both} lie at
+                // place t ^ (g / 2) of line g.
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] = ex2(p[i] + bias);
-                    l += p[i];
-                    p[i] *= i < 4 ? v0 : v1;
+                for (int r = 0; r < NR; ++r) {
+                    const float bias = m[r] == -INFINITY ? 0.0f : 12.0f - m[r];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[r][i] = ex2(p[r][i] + bias);
+                        l[r] += p[r][i];
+                        p[r][i] *= i < 2 ? v0 : v1;
+                    }
+                    uint4 w;
+                    split_f16(p[r][0], p[r][1], w.x, w.z);
+                    split_f16(p[r][2], p[r][3], w.y, w.w);
+                    sts128(weights + r * 512 + (g * 4 + (t ^ (g >> 1))) * 16, w);
                 }
+                __syncwarp();
+                uint2 pb[NR][2];  // k 2t, 2t + 1: tokens 2t, 2t + 8; k 2t + 8, 2t + 9: tokens 2t + 1, 2t + 9
 #pragma unroll
-                for (int n = 0; n < 4; ++n) split_f16(p[2 * n], p[2 * n + 1], pa[n >> 1][(n & 1) * 2], pa[n >> 1][(n & 1) * 2 + 1]);
-                // Values: thread t's tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each 16, elements g D / 8 ...
+                for (int r = 0; r < NR; ++r) {
+                    const uint32_t at = weights + r * 512 + t * 128 + ((g >> 1) ^ t) * 16 + (g & 1) * 8;
+                    pb[r][0] = lds64(at);
+                    pb[r][1] = lds64(at + 64);
+                }
+                // Values: elements g E .. g E + E - 1 of tokens 2t, 2t + 8, 2t + 1, 2t + 9 of each 16.
                 const bool clean = FMT == kKv8I8 || (t0 + kDecStep <= seen_max && flags == 3);
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
+                for (int mt = 0; mt < 2; ++mt) {
                     uint32_t w[4][D / 32];  // token, word
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
-                        const int r = 2 * t + (b & 1);
-                        const uint32_t at = vb + (kk * 16 + (b >> 1) * 8) * D;
+                        const int r = 2 * t + (b >> 1), r8 = (b & 1) * 8;
+                        const uint32_t at = vb + (mt * 16 + r8) * D;
                         if (D == 64) {
                             const uint2 u = lds64(at + ring_offset<D>(r, g >> 1) + (g & 1) * 8);
                             w[b][0] = u.x, w[b][1] = u.y;
@@ -473,56 +530,60 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                             w[b][0] = u.x, w[b][1] = u.y, w[b][D / 32 - 2] = u.z, w[b][D / 32 - 1] = u.w;
                         }
                         if (!clean) {  // what lies behind the end may be NaN
-                            const int tok = t0 + kk * 16 + (b >> 1) * 8 + r;
-                            if (tok >= seen_max || !(flags & (kk ? 2 : 1)))
+                            const int tok = t0 + mt * 16 + r8 + r;
+                            if (tok >= seen_max || !(flags & (mt ? 2 : 1)))
 #pragma unroll
                                 for (int e = 0; e < D / 32; ++e) w[b][e] = 0;
                         }
                     }
 #pragma unroll
                     for (int e = 0; e < D / 32; ++e) {
-                        // bytes of two tokens side by side: (token 2t, token 2t + 1) of an element
-                        uint32_t b0[4], b1[4];
-                        codes_f16<FMT>(__byte_perm(w[0][e], w[1][e], 0x5140), b0[0], b0[1]);
-                        codes_f16<FMT>(__byte_perm(w[0][e], w[1][e], 0x7362), b0[2], b0[3]);
-                        codes_f16<FMT>(__byte_perm(w[2][e], w[3][e], 0x5140), b1[0], b1[1]);
-                        codes_f16<FMT>(__byte_perm(w[2][e], w[3][e], 0x7362), b1[2], b1[3]);
+                        // bytes of two tokens side by side; tile 2 e + i: elements 4 e + 2 i and + 1
+                        uint32_t f[2][4];
+                        codes_f16<FMT>(__byte_perm(w[0][e], w[1][e], 0x5140), f[0][0], f[0][1]);
+                        codes_f16<FMT>(__byte_perm(w[0][e], w[1][e], 0x7362), f[1][0], f[1][1]);
+                        codes_f16<FMT>(__byte_perm(w[2][e], w[3][e], 0x5140), f[0][2], f[0][3]);
+                        codes_f16<FMT>(__byte_perm(w[2][e], w[3][e], 0x7362), f[1][2], f[1][3]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma_f16(o[e * 4 + i], pa[kk], b0[i], b1[i]);
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < NR; ++r)
+                                mma_f16(o[r][2 * e + i], f[i], mt ? pb[r][0].y : pb[r][0].x, mt ? pb[r][1].y : pb[r][1].x);
                     }
                 }
-                stage = stage == kDecStages - 1 ? 0 : stage + 1;
+                stage = stage == S::kStages - 1 ? 0 : stage + 1;
             }
             // ---- the segment's end ----
-            l += __shfl_xor_sync(0xffffffffu, l, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            // Thread t holds elements [2t D/8, (2t + 2) D/8) of row g.
             const bool whole_unit = first_step == 0 && last == cur.steps;
-            const float f = whole_unit ? (l > 0.0f ? vref / l : (l == 0.0f ? 0.0f : l)) : vref;
-            if (whole_unit) {
-                T* dst = out_row(cur, g);
-                if (dst) {
+            // The warp's last segment: its ring is read out and takes the piece.
+            // An earlier one (the end of a unit begun before): global memory.
+            float* part = warp_parts + (size_t)(w0 + warp) * S::kPartFloats;
+            if (!whole_unit && x == hi) {
+                cp_async_wait<0>();
+                __syncwarp();
+                part = ring_part(warp);
+            }
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+            for (int r = 0; r < NR; ++r) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 4);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 8);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
+                if (whole_unit) {
+                    T* dst = out_row(cur, 4 * r + t);
+                    if (!dst) continue;
+                    dst += g * E;
+                    const float f = l[r] == 0.0f ? 0.0f : vref / l[r];
 #pragma unroll
-                        for (int i = 0; i < NV; ++i) dst[(2 * t + b) * NV + i] = (T)(l == 0.0f ? 0.0f : (o[i][b] + o[i][2 + b]) * f);
-                }
-            } else {
-                // The warp's last segment: its ring is read out and takes the piece.
-                // An earlier one (the end of a unit begun before): global memory.
-                float* part = warp_parts + (size_t)(w0 + warp) * S::kPartFloats;
-                if (x == hi) {
-                    cp_async_wait<0>();
-                    __syncwarp();
-                    part = ring_part(warp);
-                }
+                    for (int i = 0; i < E; ++i)
+                        dst[i] = (T)(l[r] == 0.0f ? 0.0f : (o[r][i >> 1][(i & 1) * 2] + o[r][i >> 1][(i & 1) * 2 + 1]) * f);
+                } else {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < NV; ++i) part[g * D + (2 * t + b) * NV + i] = (o[i][b] + o[i][2 + b]) * f;
-                if (t == 0) {
-                    part[kDecRows * D + g] = m;
-                    part[kDecRows * D + kDecRows + g] = l;
+                    for (int i = 0; i < E; ++i)
+                        part[(4 * r + t) * D + g * E + i] = (o[r][i >> 1][(i & 1) * 2] + o[r][i >> 1][(i & 1) * 2 + 1]) * vref;
+                    if (g == 0) {
+                        part[R * D + 4 * r + t] = m[r];
+                        part[R * D + R + 4 * r + t] = l[r];
+                    }
                 }
             }
             if (cur.step == cur.steps && x < hi) next_unit(cur);
@@ -536,7 +597,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     // Adds n pieces (piece(i) is the i-th) by one warp, two at a time so that
     // their loads are under way together: lane's four neighbouring elements of
     // rows (lane * 4 + 128 k) / D.
-    constexpr int KM = kDecRows * D / 128;
+    constexpr int KM = R * D / 128;
     struct Sum {
         float m[KM], l[KM];
         float4 o[KM];
@@ -556,8 +617,8 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
 #pragma unroll
                 for (int k = 0; k < KM; ++k) {
                     const int e = lane * 4 + 128 * k, r = e / D;
-                    pm[i][k] = p[kDecRows * D + r];
-                    pl[i][k] = p[kDecRows * D + kDecRows + r];
+                    pm[i][k] = p[R * D + r];
+                    pl[i][k] = p[R * D + R + r];
                     po[i][k] = *reinterpret_cast<const float4*>(p + e);
                 }
             }
@@ -581,7 +642,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         for (int k = 0; k < KM; ++k) {
             const int e = lane * 4 + 128 * k, r = e / D;
             *reinterpret_cast<float4*>(to + e) = z.o[k];
-            if (e % D == 0) to[kDecRows * D + r] = z.m[k], to[kDecRows * D + kDecRows + r] = z.l[k];
+            if (e % D == 0) to[R * D + r] = z.m[k], to[R * D + R + r] = z.l[k];
         }
     };
     auto finish = [&](const Sum& z, const DecCursor& u) {
@@ -657,19 +718,20 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     }
 }
 
-template <typename T, int FMT, int D>
+template <typename T, int FMT, int D, int NR>
 cudaError_t kv8_decode_prepare() {
-    return cudaFuncSetAttribute(kv8_decode_kernel<T, FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                DecShape<D>::kRingBytes + (kPagesMaxSeqs + 1) * (int)sizeof(unsigned));
+    return cudaFuncSetAttribute(kv8_decode_kernel<T, FMT, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                DecShape<D, NR>::kRingBytes + (kPagesMaxSeqs + 1) * (int)sizeof(unsigned));
 }
 
-template <typename T, int FMT, int D>
+template <typename T, int FMT, int D, int NR>
 cudaError_t launch_kv8_decode(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, cudaStream_t st) {
-    const int smem = DecShape<D>::kRingBytes + (a.n_seqs + 1) * (int)sizeof(unsigned);
+    using S = DecShape<D, NR>;
+    const int smem = S::kRingBytes + (a.n_seqs + 1) * (int)sizeof(unsigned);
     int* counters = (int*)ws;
     float* parts = (float*)((uint8_t*)ws + kv8_counter_bytes(num_sms));
-    return launch_ex(kv8_decode_kernel<T, FMT, D>, dim3(num_sms * DecShape<D>::kCtasPerSm), dim3(kDecWarps * 32), smem, st,
-                     true, c, a, parts, counters);
+    return launch_ex(kv8_decode_kernel<T, FMT, D, NR>, dim3(num_sms * S::kCtasPerSm), dim3(kDecWarps * 32), smem, st, true,
+                     c, a, parts, counters);
 }
 
 }  // namespace lc
