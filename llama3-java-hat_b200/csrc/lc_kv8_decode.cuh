@@ -39,15 +39,17 @@
 namespace lc {
 
 constexpr int kDecWarps = 8;  // per CTA
-constexpr int kDecStep = 32;  // tokens of a step
+constexpr int kDecUnitCost = 1;     // a unit's beginning and end, in steps
+constexpr int kDecSeqsShared = 512;  // up to here the sequences' places are kept in shared memory
 
 // D: head size; NR: tiles of 4 rows of a unit, 1 or 2.
 template <int D, int NR>
 struct DecShape {
     static constexpr int kRows = 4 * NR;
-    static constexpr int kCtasPerSm = D == 64 ? 2 : 1;
+    static constexpr int kStep = 2048 / D;  // tokens of a step: 4 KB of codes
+    static constexpr int kCtasPerSm = D == 128 && NR == 2 ? 1 : 2;  // 128 registers would spill there
     static constexpr int kStages = 3;
-    static constexpr int kStageBytes = 2 * kDecStep * D + 32;           // K, V, four scales and the page flags
+    static constexpr int kStageBytes = 2 * kStep * D + 32;              // K, V, four scales and the page flags
     static constexpr int kWarpBytes = kStages * kStageBytes + 512 * NR;  // and the weights
     static constexpr int kRingBytes = kDecWarps * kWarpBytes;
     static constexpr int kPartFloats = kRows * (D + 2);  // O[rows][D], m[rows], l[rows]
@@ -58,9 +60,7 @@ struct DecShape {
 // per CTA two joined pieces.
 inline size_t kv8_counter_bytes(int num_sms) { return ((size_t)num_sms * 2 * sizeof(int) + 255) / 256 * 256; }
 inline size_t kv8_decode_ws_bytes(int num_sms) {
-    const size_t a = DecShape<64, 2>::kCtasPerSm * DecShape<64, 2>::kPartFloats;
-    const size_t b = DecShape<128, 2>::kCtasPerSm * DecShape<128, 2>::kPartFloats;
-    return kv8_counter_bytes(num_sms) + (size_t)num_sms * (kDecWarps + 2) * (a > b ? a : b) * sizeof(float);
+    return kv8_counter_bytes(num_sms) + (size_t)num_sms * 2 * (kDecWarps + 2) * DecShape<128, 2>::kPartFloats * sizeof(float);
 }
 
 LC_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -172,7 +172,10 @@ LC_DEV int dec_seen(const SeqInfo& q, int group, int room, int row) {
     const int seen = q.len - q.nq + (j < q.nq ? j : q.nq - 1) + 1;
     return seen < 0 ? 0 : seen > room ? room : seen;
 }
-LC_DEV int dec_steps(int seen) { return seen <= kDecStep ? 1 : (seen + kDecStep - 1) / kDecStep; }
+template <int STEP>
+LC_DEV int dec_steps(int seen) {
+    return seen <= STEP ? 1 : (seen + STEP - 1) / STEP;
+}
 
 template <typename T, int FMT, int D, int NR>
 __global__ void __launch_bounds__(kDecWarps * 32, DecShape<D, NR>::kCtasPerSm)
@@ -181,24 +184,41 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     constexpr int R = S::kRows;
     constexpr int KS = D / 16;  // k-steps of a score, and tiles of 16 elements of the output
     constexpr int E = D / 8;    // elements of a row that a thread holds
+    constexpr int STEP = S::kStep, MT = STEP / 16;
     extern __shared__ __align__(128) uint8_t smem[];
-    unsigned* prefix = reinterpret_cast<unsigned*>(smem + S::kRingBytes);  // [n_seqs + 1] steps before sequence s
+    unsigned* prefix = reinterpret_cast<unsigned*>(smem + S::kRingBytes);  // [n_seqs + 1] the line before sequence s
     __shared__ unsigned scan[kDecWarps];
+    __shared__ SeqInfo infos[kDecSeqsShared];
+    __shared__ DecCursor first_unit;  // warp 0's first unit, for the joining
+    __shared__ DecCursor done_cursor[2];
+    __shared__ int done_pieces[2];
+    __shared__ int done_unit[2];  // cross-CTA units whose last piece this CTA brought
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.n_heads / c.n_kv, sh = c.page_shift;
     const int room = (int)min((long long)a.table_stride << sh, 0x7fffffffll);
     griddep_launch();
     griddep_wait();
 
+    // The queries come to L2 while the line is laid out.
+    if (a.q_stride >= 0) {
+        const int64_t bytes = (int64_t)a.n_heads * D * sizeof(T);  // of a row, 128 at a time
+        const int per = (int)((bytes + 127) / 128);
+        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + tid; i < (int64_t)a.rows * per; i += (int64_t)gridDim.x * blockDim.x)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"((const uint8_t*)a.q + (i / per) * a.q_stride * (int)sizeof(T) + min((i % per) * 128, bytes - 1)));
+    }
+    if (tid < 2) done_unit[tid] = 0;
+
     // ---- the line of steps ----
+    // A unit takes its steps and kDecUnitCost empty places behind them.
     unsigned carry = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += kDecWarps * 32) {
         const int s = s0 + tid;
         unsigned cost = 0;
         if (s < a.n_seqs) {
             const SeqInfo q = kv8_seq(a, sh, s);
+            if (s < kDecSeqsShared) infos[s] = q;
             const int chunks = (q.nq * group + R - 1) / R;
-            for (int k = 0; k < chunks; ++k) cost += dec_steps(dec_seen(q, group, room, k * R + R - 1));
+            for (int k = 0; k < chunks; ++k) cost += kDecUnitCost + dec_steps<STEP>(dec_seen(q, group, room, k * R + R - 1));
             cost *= c.n_kv;
         }
         unsigned v = cost;
@@ -235,17 +255,17 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     if (w0 >= workers) return;
     const unsigned my_warps = min((unsigned)kDecWarps, workers - w0);
     const unsigned cta_lo = begin_of(w0), cta_hi = begin_of(w0 + my_warps);
-    const unsigned lo = warp < my_warps ? begin_of(w0 + warp) : cta_hi;
+    unsigned lo = warp < my_warps ? begin_of(w0 + warp) : cta_hi;
     const unsigned hi = warp < my_warps ? begin_of(w0 + warp + 1) : cta_hi;
 
     auto set_chunk = [&](DecCursor& cur, int chunk) {
         cur.chunk = chunk;
         cur.seen = dec_seen(cur.q, group, room, chunk * R + R - 1);
-        cur.steps = dec_steps(cur.seen);
+        cur.steps = dec_steps<STEP>(cur.seen);
     };
     auto set_seq = [&](DecCursor& cur, int s) {
         cur.s = s;
-        cur.q = kv8_seq(a, sh, s);
+        cur.q = s < kDecSeqsShared ? infos[s] : kv8_seq(a, sh, s);
         cur.chunks = (cur.q.nq * group + R - 1) / R;
     };
     auto locate = [&](DecCursor& cur, unsigned x) {  // the unit and step at place x
@@ -261,8 +281,8 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         cur.head = rem / per;
         rem -= cur.head * per;
         set_chunk(cur, 0);
-        while (rem >= (unsigned)cur.steps) {
-            rem -= cur.steps;
+        while (rem >= (unsigned)(cur.steps + kDecUnitCost)) {
+            rem -= cur.steps + kDecUnitCost;
             set_chunk(cur, cur.chunk + 1);
         }
         cur.step = rem;
@@ -297,51 +317,60 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         return (T*)a.out + (int64_t)(cur.q.row0 + j) * a.out_stride + (cur.head * group + row - j * group) * D;
     };
 
-    DecCursor cur;  // in the end: the unit of step hi - 1, cur.step behind that step
+    DecCursor cur;       // in the end: the unit of the warp's last step, cur.step behind it
+    unsigned x_end = 0;  // the place behind the warp's last step
     if (lo < hi) {
         // ---- issue side ----
         DecCursor ic;  // the next step to ask for
         locate(ic, lo);
+        if (ic.step >= ic.steps) {  // the empty places behind a unit
+            lo = min(hi, lo + ic.steps + kDecUnitCost - ic.step);
+            if (lo < hi) next_unit(ic);
+        }
+        if (warp == 0 && lane == 0) first_unit = ic;
         unsigned ahead = lo;
         int id0 = 0, id1 = 0;  // its pages
         auto ids = [&]() {
             const int32_t* row = a.table + (int64_t)ic.s * a.table_stride;
-            const int t0 = ic.step * kDecStep;
+            const int t0 = ic.step * STEP;
             id0 = t0 < ic.seen ? row[t0 >> sh] : -1;
-            id1 = !row_sel ? id0 : t0 + 16 < ic.seen ? row[(t0 + 16) >> sh] : -1;
+            id1 = MT == 1 || !row_sel ? id0 : t0 + 16 < ic.seen ? row[(t0 + 16) >> sh] : -1;
         };
-        ids();
+        if (lo < hi) ids();
         const int off0 = lane * 16;  // this lane's first chunk of a half
         const int r0 = off0 / D, ch0 = (off0 % D) / 16;
         const int dst0 = ring_offset<D>(r0, ch0);
-        constexpr int kCopies = kDecStep * D / 512;  // 16-byte copies per lane for K, and for V
+        constexpr int kCopies = STEP * D / 512;  // 16-byte copies per lane for K, and for V
         auto issue = [&](int stage) {
             if (ahead < hi) {
                 const uint32_t st = ring + stage * S::kStageBytes;
                 const bool ok0 = (unsigned)id0 < (unsigned)c.n_pages, ok1 = (unsigned)id1 < (unsigned)c.n_pages;
-                const int in_page = (ic.step * kDecStep) & ((1 << sh) - 1);
+                const int in_page = (ic.step * STEP) & ((1 << sh) - 1);
                 const int64_t b0 = ((((int64_t)id0 * c.n_kv + ic.head) << sh) + in_page) * D;
                 const int64_t b1 = row_sel ? (((int64_t)id1 * c.n_kv + ic.head) << sh) * D : b0 + 16 * D;
 #pragma unroll
                 for (int k = 0; k < kCopies; ++k) {
-                    const bool second = k >= kCopies / 2;
+                    const bool second = MT == 2 && k >= kCopies / 2;
                     if (second ? ok1 : ok0) {
                         const int64_t at = (second ? b1 + (k - kCopies / 2) * 512 : b0 + k * 512) + off0;
                         // rows of copy k are 512 / D further: a multiple of the swizzle's period only for D = 64
                         const uint32_t d = D == 64 ? dst0 + k * 512 : ring_offset<D>(r0 + k * (512 / D), ch0);
                         cp_async16(st + d, c.k + at);
-                        cp_async16(st + kDecStep * D + d, c.v + at);
+                        cp_async16(st + STEP * D + d, c.v + at);
                     }
                 }
                 if (lane < 4) {
                     const bool ok = (lane & 1) ? ok1 : ok0;
                     const int64_t at = (int64_t)((lane & 1) ? id1 : id0) * c.n_kv + ic.head;
-                    if (ok) cp_async4(st + 2 * kDecStep * D + lane * 4, (lane & 2 ? c.v_scale : c.k_scale) + at);
+                    if (ok) cp_async4(st + 2 * STEP * D + lane * 4, (lane & 2 ? c.v_scale : c.k_scale) + at);
                 }
                 if (lane == 0)
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(st + 2 * kDecStep * D + 16), "r"((ok0 ? 1 : 0) | (ok1 ? 2 : 0)) : "memory");
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(st + 2 * STEP * D + 16), "r"((ok0 ? 1 : 0) | (MT == 2 && ok1 ? 2 : 0)) : "memory");
                 ++ahead;
-                if (++ic.step == ic.steps && ahead < hi) next_unit(ic);
+                if (++ic.step == ic.steps) {
+                    ahead += kDecUnitCost;
+                    if (ahead < hi) next_unit(ic);
+                }
                 if (ahead < hi) ids();
             }
             cp_async_commit();
@@ -413,18 +442,18 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                 cp_async_wait<S::kStages - 2>();
                 __syncwarp();  // the stage's copies of all lanes are there, and the previous stage is read
                 issue(stage == 0 ? S::kStages - 1 : stage - 1);
-                const uint32_t kb = ring + stage * S::kStageBytes, vb = kb + kDecStep * D, sb = vb + kDecStep * D;
+                const uint32_t kb = ring + stage * S::kStageBytes, vb = kb + STEP * D, sb = vb + STEP * D;
                 const uint4 sc = lds128(sb);
                 uint32_t flags;
                 asm volatile("ld.shared.u32 %0, [%1];" : "=r"(flags) : "r"(sb + 16));
                 const float ks0 = (flags & 1) ? __uint_as_float(sc.x) : 0.0f, ks1 = (flags & 2) ? __uint_as_float(sc.y) : 0.0f;
                 const float vs0 = (flags & 1) ? __uint_as_float(sc.z) : 0.0f, vs1 = (flags & 2) ? __uint_as_float(sc.w) : 0.0f;
-                const int t0 = cur.step * kDecStep;
+                const int t0 = cur.step * STEP;
 
                 // Scores: 16 tokens (rows g, g + 8) by 4 rows' hi and lo columns.
-                float s[2][NR][4];
+                float s[MT][NR][4];
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
+                for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                     for (int r = 0; r < NR; ++r) s[mt][r][0] = s[mt][r][1] = s[mt][r][2] = s[mt][r][3] = 0.0f;
 #pragma unroll
@@ -443,29 +472,31 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                     }
                 }
                 // In powers of two; hi and lo meet here.  Token of p[r][i]: 8 i + g.
-                float p[NR][4];
-                const bool whole = t0 + kDecStep <= seen_min && flags == 3 && all_live;
+                float p[NR][2 * MT];
+                const bool whole = t0 + STEP <= seen_min && flags == (MT == 2 ? 3 : 1) && all_live;
                 bool move = false;
                 float top[NR];
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    const float c0 = qf[r] * ks0, c1 = qf[r] * ks1;
-                    p[r][0] = (s[0][r][0] + s[0][r][1]) * c0;
-                    p[r][1] = (s[0][r][2] + s[0][r][3]) * c0;
-                    p[r][2] = (s[1][r][0] + s[1][r][1]) * c1;
-                    p[r][3] = (s[1][r][2] + s[1][r][3]) * c1;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const float f = qf[r] * (mt ? ks1 : ks0);
+                        p[r][2 * mt] = (s[mt][r][0] + s[mt][r][1]) * f;
+                        p[r][2 * mt + 1] = (s[mt][r][2] + s[mt][r][3]) * f;
+                    }
                     if (!whole) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 2 * MT; ++i)
                             if (t0 + 8 * i + g >= seen[r] || !(flags & (i < 2 ? 1 : 2))) p[r][i] = -INFINITY;
                     }
-                    top[r] = fmaxf(fmaxf(p[r][0], p[r][1]), fmaxf(p[r][2], p[r][3]));
+                    top[r] = fmaxf(p[r][0], p[r][1]);
+                    if (MT == 2) top[r] = fmaxf(top[r], fmaxf(p[r][2 * MT - 2], p[r][2 * MT - 1]));
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 4));
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 8));
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 16));
                     move |= top[r] > m[r] + 1.0f;
                 }
-                const float vmax = fmaxf(vs0, vs1);
+                const float vmax = MT == 2 ? fmaxf(vs0, vs1) : vs0;
                 if (__any_sync(0xffffffffu, move) || vmax > 4.0f * vref) {
                     float fv = 1.0f;
                     if (vmax > 4.0f * vref) {
@@ -495,14 +526,14 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                 for (int r = 0; r < NR; ++r) {
                     const float bias = m[r] == -INFINITY ? 0.0f : 12.0f - m[r];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 2 * MT; ++i) {
                         p[r][i] = ex2(p[r][i] + bias);
                         l[r] += p[r][i];
                         p[r][i] *= i < 2 ? v0 : v1;
                     }
-                    uint4 w;
+                    uint4 w = make_uint4(0, 0, 0, 0);
                     split_f16(p[r][0], p[r][1], w.x, w.z);
-                    split_f16(p[r][2], p[r][3], w.y, w.w);
+                    if (MT == 2) split_f16(p[r][2 * MT - 2], p[r][2 * MT - 1], w.y, w.w);
                     sts128(weights + r * 512 + (g * 4 + (t ^ (g >> 1))) * 16, w);
                 }
                 __syncwarp();
@@ -514,9 +545,9 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                     pb[r][1] = lds64(at + 64);
                 }
                 // Values: elements g E .. g E + E - 1 of tokens 2t, 2t + 8, 2t + 1, 2t + 9 of each 16.
-                const bool clean = FMT == kKv8I8 || (t0 + kDecStep <= seen_max && flags == 3);
+                const bool clean = FMT == kKv8I8 || (t0 + STEP <= seen_max && flags == (MT == 2 ? 3 : 1));
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
+                for (int mt = 0; mt < MT; ++mt) {
                     uint32_t w[4][D / 32];  // token, word
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
@@ -555,10 +586,12 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             }
             // ---- the segment's end ----
             const bool whole_unit = first_step == 0 && last == cur.steps;
+            x_end = x;
+            if (cur.step == cur.steps) x += kDecUnitCost;
             // The warp's last segment: its ring is read out and takes the piece.
             // An earlier one (the end of a unit begun before): global memory.
             float* part = warp_parts + (size_t)(w0 + warp) * S::kPartFloats;
-            if (!whole_unit && x == hi) {
+            if (!whole_unit && x >= hi) {
                 cp_async_wait<0>();
                 __syncwarp();
                 part = ring_part(warp);
@@ -589,8 +622,6 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             if (cur.step == cur.steps && x < hi) next_unit(cur);
         }
     }
-    __shared__ int done_unit[2];  // cross-CTA units whose last piece this CTA brought
-    if (tid < 2) done_unit[tid] = 0;
     __syncthreads();
 
     // ---- joining pieces ----
@@ -660,19 +691,15 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     // A warp joins the pieces of the unit that begins in it and goes on, and
     // warp 0 those of the unit that was under way at the CTA's start.
     for (int side = warp == 0 ? 0 : 1; side < 2 && lo < hi; ++side) {
-        DecCursor u = cur;
-        unsigned u0 = hi - u.step;  // the unit's place on the line
-        if (side == 0) {
-            locate(u, lo);
-            u0 = lo - u.step;
-        }
-        const unsigned u1 = u0 + u.steps;
+        const DecCursor u = side == 0 ? first_unit : cur;
+        // The unit's place on the line: `cur` stands behind the warp's last step.
+        const unsigned u0 = side == 0 ? lo - u.step : x_end - u.step, u1 = u0 + u.steps;
         if (side == 0 ? u0 >= lo : !(u0 >= lo && u1 > hi)) continue;
         const int wn = (int)(worker_of(min(u1, cta_hi) - 1) - (w0 + warp)) + 1;  // warps with a piece, from this one
         Sum z;
         clear(z);
         // All but the last lie in the ring; so does the last unless that warp went on to another unit.
-        const bool tail_out = begin_of(w0 + warp + wn) > u1;
+        const bool tail_out = begin_of(w0 + warp + wn) > u1 + kDecUnitCost;
         add(z, wn, [&](int i) -> const float* {
             return i == wn - 1 && tail_out ? warp_parts + (size_t)(w0 + warp + i) * S::kPartFloats : ring_part(warp + i);
         });
@@ -687,7 +714,9 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
         if (lane == 0 && atomicAdd(counters + first, 1) == final - first) {
             counters[first] = 0;
             __threadfence();
-            done_unit[side] = 1 + warp;
+            done_unit[side] = 1 + first;
+            done_cursor[side] = u;
+            done_pieces[side] = final - first + 1;
         }
     }
     __syncthreads();
@@ -695,11 +724,8 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     // finish: each a range of them, then one adds the warps' sums in order.
     for (int side = 0; side < 2; ++side) {
         if (!done_unit[side]) continue;  // uniform over the CTA
-        DecCursor u;
-        const unsigned at = side == 0 ? cta_lo : begin_of(w0 + done_unit[side]) - 1;
-        locate(u, at);
-        const unsigned u0 = at - u.step, u1 = u0 + u.steps;
-        const int first = (int)(worker_of(u0) / kDecWarps), n = (int)(worker_of(u1 - 1) / kDecWarps) - first + 1;
+        const DecCursor u = done_cursor[side];
+        const int first = done_unit[side] - 1, n = done_pieces[side];
         const int i0 = n * warp / kDecWarps, i1 = n * (warp + 1) / kDecWarps;
         Sum z;
         clear(z);
