@@ -926,7 +926,7 @@ extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, 
             }
             c->kv8_ws = ws;
         }
-        return s.finish(launch_kv8_attention(view, a, c->sms, c->kv8_ws, c->stream));
+        return s.finish(launch_kv8_attention(view, a, c->sms, c->kv8_ws, c->d_err, c->stream));
     });
 }
 

@@ -5,6 +5,7 @@
 // with k_t, v_t = code * scale of the page and head.  A query that sees
 // nothing gives zeros; rows behind the last sequence are left as they were.
 #include "lc_kv8_decode.cuh"
+#include "lc_kv8_prefill.cuh"
 
 namespace lc {
 namespace {
@@ -23,26 +24,36 @@ cudaError_t by_shape(int dtype, int format, int head_dim, F&& f) {
 
 }  // namespace
 
-size_t kv8_attention_ws_bytes(int num_sms) { return kv8_decode_ws_bytes(num_sms); }
+// The two kernels' workspaces, one behind the other.
+static size_t decode_ws(int num_sms) { return (kv8_decode_ws_bytes(num_sms) + 255) / 256 * 256; }
+
+size_t kv8_attention_ws_bytes(int num_sms) { return decode_ws(num_sms) + kv8_prefill_ws_bytes(num_sms); }
 
 cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st) {
     for (int i = 0; i < 8; ++i) {
         const cudaError_t e = by_shape(i & 1, (i >> 1) & 1, i & 4 ? 128 : 64, [](auto row, auto fmt, auto d) {
-            const cudaError_t e = kv8_decode_prepare<decltype(row), fmt.value, d.value, 1>();
-            return e != cudaSuccess ? e : kv8_decode_prepare<decltype(row), fmt.value, d.value, 2>();
+            using T = decltype(row);
+            cudaError_t e = kv8_decode_prepare<T, fmt.value, d.value, 1>();
+            if (e == cudaSuccess) e = kv8_decode_prepare<T, fmt.value, d.value, 2>();
+            return e != cudaSuccess ? e : kv8_prefill_prepare<T, fmt.value, d.value>();
         });
         if (e != cudaSuccess) return e;
     }
-    return cudaMemsetAsync(ws, 0, kv8_counter_bytes(num_sms), st);
+    const cudaError_t e = cudaMemsetAsync(ws, 0, kv8_counter_bytes(num_sms), st);
+    if (e != cudaSuccess) return e;
+    return cudaMemsetAsync((uint8_t*)ws + decode_ws(num_sms), 0, kv8_prefill_counter_bytes(num_sms), st);
 }
 
-cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, cudaStream_t st) {
+cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, int* err, cudaStream_t st) {
+    const int rows = a.n_heads / c.n_kv * a.max_q;  // that share a kv head's codes, at most
     return by_shape(a.dtype, c.format, c.head_dim, [&](auto row, auto fmt, auto d) {
-        // Units of 4 rows where a sequence has no more, of 8 where it has:
-        // more rows share one reading of the codes.
-        return a.n_heads / c.n_kv * a.max_q <= 4
-                   ? launch_kv8_decode<decltype(row), fmt.value, d.value, 1>(c, a, num_sms, ws, st)
-                   : launch_kv8_decode<decltype(row), fmt.value, d.value, 2>(c, a, num_sms, ws, st);
+        using T = decltype(row);
+        // Units of 4 rows where a sequence has no more, of 8 where it has (more
+        // rows share one reading of the codes), and the tensor-core tiles of
+        // 128 beyond.
+        if (rows <= 4) return launch_kv8_decode<T, fmt.value, d.value, 1>(c, a, num_sms, ws, st);
+        if (rows <= 8) return launch_kv8_decode<T, fmt.value, d.value, 2>(c, a, num_sms, ws, st);
+        return launch_kv8_prefill<T, fmt.value, d.value>(c, a, num_sms, (uint8_t*)ws + decode_ws(num_sms), err, st);
     });
 }
 

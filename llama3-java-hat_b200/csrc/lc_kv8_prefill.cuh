@@ -1,0 +1,746 @@
+// lc_kv8_prefill.cuh -- attention over the 8-bit pages for many queries per
+// sequence (prompt chunks), on the tcgen05 tensor cores.
+//
+// A unit is 256 (query, head) rows that share a kv head, as two tiles of 128
+// MMA rows; a step is one tile of NT tokens.  Per step and row tile
+//   S = Q K^T   M 128, N NT, K head size: Q and K codes f16 in shared memory
+//   p = 2^(S c + b), running maximum and sum, one thread per row
+//   O += P V    M 128, N head size, K NT: P in tensor memory over S's columns
+// The codes are exact in f16, so scales enter only where scores leave tensor
+// memory: the key scale of a 16-token group in c, the value scale (over a
+// running reference, as its logarithm) in b; the sum takes it out again.
+// fp32 rows are split into f16 hi + lo under a power-of-two row scale, and P
+// likewise, at the price of twice the products; f16 rows take one pass and
+// round P to f16 (2^-12 of each weight), as the result is.
+//
+// What bounds it: for head size 64 one exponential costs as much as the 128
+// products of its score, so the special-function unit and the issue slots
+// around it, not the tensor cores, set the pace; hence two row tiles, whose
+// softmax warpgroups take turns with the tensor cores, and one dequantised
+// tile for both.
+//
+// Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: codes to f16.
+// Warp 12: issues the MMAs.  All steps of the call form one line that is cut
+// into equal pieces, one per CTA; pieces of a unit are joined, warp by warp,
+// by the last CTA to finish, in the order of the line.
+#pragma once
+
+#include "lc_internal.h"
+#include "lc_kv8_decode.cuh"
+#include "lc_tcgen05.cuh"
+
+namespace lc {
+
+constexpr int kPreRows = 256;      // rows of a unit
+constexpr int kPreThreads = 13 * 32;
+constexpr int kPreUnitCost = 1;    // a unit's beginning and end, in steps
+constexpr int kPreScaleRing = 4;
+
+template <typename T, int D>
+struct PreShape {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kTok = 8192 / D;                 // NT: 128 or 64 tokens
+    static constexpr int kGroups = kTok / 16;
+    static constexpr int kQPart = 128 * D * 2;            // bytes of one part (hi or lo) of one row tile
+    static constexpr int kQBytes = 2 * (kSplit ? 2 : 1) * kQPart;
+    static constexpr int kTileBytes = kTok * D * 2;       // 16 KB
+    static constexpr int kScaleBytes = kPreScaleRing * (kGroups * 8 + 8);
+    static constexpr int kSmem = kQBytes + 4 * kTileBytes + kScaleBytes;
+    static constexpr int kPieceFloats = kPreRows * (D + 2);
+    static constexpr uint32_t kOCol = 2 * kTok;           // tensor memory: S of both tiles, then O of both
+};
+
+inline size_t kv8_prefill_counter_bytes(int num_sms) { return ((size_t)num_sms * 8 * sizeof(int) + 255) / 256 * 256; }
+inline size_t kv8_prefill_ws_bytes(int num_sms) {
+    return kv8_prefill_counter_bytes(num_sms) + (size_t)num_sms * 2 * PreShape<float, 128>::kPieceFloats * sizeof(float);
+}
+
+LC_DEV void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+LC_DEV void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+// The loads before it are done; the values pass through, so that no use moves up.
+LC_DEV void tmem_wait_ld32(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                   "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                   "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+LC_DEV void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+LC_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+LC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A unit of the line and the step within it.
+struct PreCursor {
+    SeqInfo q;
+    int s, head, chunk, chunks;
+    int seen;         // positions that its last row sees
+    int step, steps;
+};
+
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(kPreThreads, 1)
+kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __restrict__ counters, int* err, uint64_t timeout_ns) {
+    using S = PreShape<T, D>;
+    constexpr int NT = S::kTok, G = S::kGroups;
+    constexpr bool SPLIT = S::kSplit;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* const sq = smem;                                   // [tile][part]
+    uint8_t* const sk = sq + S::kQBytes;                        // [2 stages]
+    uint8_t* const sv = sk + 2 * S::kTileBytes;                 // [2 stages]
+    float2* const scales = reinterpret_cast<float2*>(sv + 2 * S::kTileBytes);  // [ring][group]: key scale, log2 of the value scale
+    unsigned* const valid = reinterpret_cast<unsigned*>(scales + kPreScaleRing * G);  // [ring][2]
+    unsigned* const prefix = valid + kPreScaleRing * 2;                                // [n_seqs + 1]
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], pv_done[2], q_full[2],
+        sc_full[kPreScaleRing], drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
+    __shared__ unsigned scan[13];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = a.n_heads / c.n_kv, sh = c.page_shift;
+    const int room = (int)min((long long)a.table_stride << sh, 0x7fffffffll);
+
+    if (tid == 0) {
+        unset = 0;
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4), mbar_init(&v_full[i], 4);
+            mbar_init(&k_empty[i], 1), mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4), mbar_init(&pv_done[i], 1);
+            mbar_init(&q_full[i], 4);
+        }
+        for (int i = 0; i < kPreScaleRing; ++i) mbar_init(&sc_full[i], 1);
+        mbar_init(&drained, 1);
+        fence_mbar_init();
+    }
+    griddep_launch();
+    griddep_wait();
+
+    auto seen_of = [&](const SeqInfo& q, int row) { return dec_seen(q, group, room, row); };
+    auto steps_of = [&](const SeqInfo& q, int chunk) { return dec_steps<NT>(seen_of(q, chunk * kPreRows + kPreRows - 1)); };
+    auto chunks_of = [&](const SeqInfo& q) { return (int)(((int64_t)q.nq * group + kPreRows - 1) / kPreRows); };
+
+    // ---- the line of steps: a warp per sequence, lanes over its chunks ----
+    for (int s = warp; s < a.n_seqs; s += 13) {
+        const SeqInfo q = kv8_seq(a, sh, s);
+        const int chunks = chunks_of(q);
+        unsigned cost = 0;
+        for (int k = lane; k < chunks; k += 32) cost += steps_of(q, k) + kPreUnitCost;
+        cost = __reduce_add_sync(0xffffffffu, cost);
+        if (lane == 0) prefix[s] = cost * c.n_kv;
+    }
+    __syncthreads();
+    unsigned carry = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += kPreThreads) {
+        const int s = s0 + tid;
+        const unsigned cost = s < a.n_seqs ? prefix[s] : 0;
+        unsigned v = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) scan[warp] = v;
+        __syncthreads();
+        unsigned before = carry, all = carry;
+        for (int w = 0; w < 13; ++w) {
+            if (w < warp) before += scan[w];
+            all += scan[w];
+        }
+        if (s < a.n_seqs) prefix[s] = before + v - cost;
+        carry = all;
+        __syncthreads();
+    }
+    if (tid == 0) prefix[a.n_seqs] = carry;
+    // CTA b has steps [begin_of(b), begin_of(b + 1)).
+    const unsigned total = carry;
+    const unsigned workers = min(gridDim.x, total);
+    if (blockIdx.x >= workers) return;  // also where there is nothing at all
+    if (warp == 12) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const uint64_t deadline = globaltimer_ns() + timeout_ns;
+    const unsigned share = total / workers, extra = total - share * workers;
+    auto begin_of = [&](unsigned w) { return w * share + min(w, extra); };
+    auto worker_of = [&](unsigned x) {
+        const unsigned big = extra * (share + 1);
+        return x < big ? x / (share + 1) : extra + (x - big) / share;
+    };
+    const unsigned hi = begin_of(blockIdx.x + 1);
+    unsigned lo = begin_of(blockIdx.x);
+
+    auto set_chunk = [&](PreCursor& cur, int chunk) {
+        cur.chunk = chunk;
+        cur.seen = seen_of(cur.q, chunk * kPreRows + kPreRows - 1);
+        cur.steps = dec_steps<NT>(cur.seen);
+    };
+    auto set_seq = [&](PreCursor& cur, int s) {
+        cur.s = s;
+        cur.q = kv8_seq(a, sh, s);
+        cur.chunks = chunks_of(cur.q);
+    };
+    auto next_unit = [&](PreCursor& cur) {
+        cur.step = 0;
+        if (cur.chunk + 1 < cur.chunks) {
+            set_chunk(cur, cur.chunk + 1);
+            return;
+        }
+        if (++cur.head == c.n_kv) {
+            cur.head = 0;
+            int s = cur.s;
+            do ++s;
+            while (s < a.n_seqs - 1 && prefix[s + 1] == prefix[s]);
+            set_seq(cur, s);
+        }
+        set_chunk(cur, 0);
+    };
+    // The unit and step at place x; by whole warps.
+    PreCursor cur;
+    {
+        int a0 = 0, a1 = a.n_seqs;
+        while (a1 - a0 > 1) {
+            const int mid = (a0 + a1) >> 1;
+            if (prefix[mid] <= lo) a0 = mid;
+            else a1 = mid;
+        }
+        set_seq(cur, a0);
+        unsigned rem = lo - prefix[a0];
+        const unsigned per = (prefix[a0 + 1] - prefix[a0]) / c.n_kv;
+        cur.head = rem / per;
+        rem -= cur.head * per;
+        for (int k0 = 0;; k0 += 32) {
+            const unsigned cost = k0 + lane < cur.chunks ? steps_of(cur.q, k0 + lane) + kPreUnitCost : 0;
+            unsigned v = cost;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            const unsigned over = __ballot_sync(0xffffffffu, v > rem);
+            if (over || k0 + 32 >= cur.chunks) {
+                const int l = over ? __ffs(over) - 1 : 31;
+                rem -= __shfl_sync(0xffffffffu, v - cost, l);
+                set_chunk(cur, k0 + l);
+                break;
+            }
+            rem -= __shfl_sync(0xffffffffu, v, 31);
+        }
+        cur.step = rem;
+        if (cur.step >= cur.steps) {  // the empty places behind a unit
+            lo = min(hi, lo + cur.steps + kPreUnitCost - cur.step);
+            if (lo < hi) next_unit(cur);
+        }
+    }
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_wait_bounded(bar, parity, err, deadline, kDevTimeoutGrid);
+    };
+    auto tiles_of = [&](const PreCursor& u) { return (int64_t)u.q.nq * group - (int64_t)u.chunk * kPreRows > 128 ? 2 : 1; };
+    bool ok = true;
+
+    if (warp >= 8 && warp < 12) {
+        // ---- codes to f16 ----
+        const int cw = warp - 8;
+        uint4 kc[4], vc[4];
+        int id[4];
+        auto token_of = [&](int k) {  // of this thread's k-th 16 codes
+            const int i = k * 4 + cw;
+            return (D == 64 ? i : i >> 1) * 8 + (lane & 7);
+        };
+        auto chunk_of = [&](int k) { return (D == 64 ? 0 : ((k * 4 + cw) & 1) * 4) + (lane >> 3); };
+        auto load_ids = [&](const PreCursor& u) {
+            const int32_t* row = a.table + (int64_t)u.s * a.table_stride;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = u.step * NT + token_of(k);
+                id[k] = t < u.seen ? row[t >> sh] : -1;
+            }
+        };
+        float my_ks = 0.0f, my_lv = -120.0f;
+        bool my_ok = false;
+        auto load_codes = [&](const PreCursor& u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = u.step * NT + token_of(k);
+                kc[k] = vc[k] = make_uint4(0, 0, 0, 0);
+                if ((unsigned)id[k] < (unsigned)c.n_pages) {
+                    const int64_t at = ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16;
+                    kc[k] = __ldg(reinterpret_cast<const uint4*>(c.k + at));
+                    vc[k] = __ldg(reinterpret_cast<const uint4*>(c.v + at));
+                }
+            }
+            if (cw == 0 && lane < G) {  // scales of 16-token group `lane`
+                const int t = u.step * NT + lane * 16;
+                const int page = t < u.seen ? a.table[(int64_t)u.s * a.table_stride + (t >> sh)] : -1;
+                my_ok = (unsigned)page < (unsigned)c.n_pages;
+                my_ks = 0.0f, my_lv = -120.0f;
+                if (my_ok) {
+                    my_ks = c.k_scale[(int64_t)page * c.n_kv + u.head];
+                    const float v = c.v_scale[(int64_t)page * c.n_kv + u.head];
+                    my_lv = v < 1e-36f ? -120.0f : log2f(v);  // NaN stays
+                }
+            }
+        };
+        auto put = [&](uint8_t* tile, const uint4 (&w)[4]) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t f[8];
+                codes_f16<FMT>(w[k].x, f[0], f[1]);
+                codes_f16<FMT>(w[k].y, f[2], f[3]);
+                codes_f16<FMT>(w[k].z, f[4], f[5]);
+                codes_f16<FMT>(w[k].w, f[6], f[7]);
+                const uint32_t at = smem_u32(tile) + (token_of(k) >> 3) * (D * 16) + chunk_of(k) * 256 + (lane & 7) * 16;
+                sts128(at, make_uint4(f[0], f[1], f[2], f[3]));
+                sts128(at + 128, make_uint4(f[4], f[5], f[6], f[7]));
+            }
+        };
+        PreCursor nx = cur;
+        unsigned ahead = lo;
+        auto advance = [&]() {
+            ++ahead;
+            if (++nx.step == nx.steps) {
+                ahead += kPreUnitCost;
+                if (ahead < hi) next_unit(nx);
+            }
+        };
+        if (ahead < hi) load_ids(nx), load_codes(nx);
+        for (int i = 0; ahead < hi && ok; ++i) {
+            uint4 k0[4], v0[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) k0[k] = kc[k], v0[k] = vc[k];
+            const float ks = my_ks, lv = my_lv;
+            const bool group_ok = my_ok;
+            // Words whose token nobody sees stay zero: a tile's last tokens may be NaN codes.
+            advance();
+            if (ahead < hi) load_ids(nx), load_codes(nx);
+            const int st = i & 1, use = i >> 1;
+            if (use > 0) ok = wait(&k_empty[st], (use - 1) & 1);
+            if (!ok) break;
+            put(sk + st * S::kTileBytes, k0);
+            if (cw == 0) {
+                const int ring = i % kPreScaleRing;
+                if (lane < G) scales[ring * G + lane] = make_float2(ks, lv);
+                const unsigned m = __ballot_sync(0xffffffffu, lane < G && group_ok);
+                if (lane == 0) valid[ring * 2] = m;
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&k_full[st]);
+                if (cw == 0) mbar_arrive(&sc_full[i % kPreScaleRing]);
+            }
+            if (use > 0) ok = wait(&v_empty[st], (use - 1) & 1);
+            if (!ok) break;
+            put(sv + st * S::kTileBytes, v0);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[st]);
+        }
+    } else if (warp == 12) {
+        // ---- MMAs: one thread ----
+        if (lane == 0) {
+            constexpr uint32_t id_qk = tc_idesc_f16_f32(128, NT);
+            constexpr uint32_t id_pv = tc_idesc_f16_f32(128, D) | (1u << 16);  // B (values) with the head's elements contiguous
+            auto qk = [&](int tile, int st) {
+                const uint32_t d = tmem + tile * NT;
+                const uint64_t kd = tc_desc_kmajor(smem_u32(sk + st * S::kTileBytes), 128, D * 16);
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
+                    const uint64_t qd = tc_desc_kmajor(smem_u32(sq + (tile * (SPLIT ? 2 : 1) + part) * S::kQPart), 128, D * 16);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) tc_mma_f16(d, qd + k * 16, kd + k * 16, id_qk, part + k > 0);
+                }
+                tc_commit(&s_full[tile]);
+            };
+            auto pv = [&](int tile, int st, bool first) {
+                const uint32_t d = tmem + S::kOCol + tile * D, p = tmem + tile * NT;
+                // 8-token groups D * 16 bytes apart, 8-element groups 128 bytes
+                const uint64_t vd = tc_desc_kmajor(smem_u32(sv + st * S::kTileBytes), D * 16, 128);
+#pragma unroll
+                for (int k = 0; k < NT / 16; ++k) {
+                    const uint32_t ac = p + (k >> 1) * 32 + (k & 1) * 8;
+                    tc_mma_f16_ta(d, ac, vd + k * (2 * D), id_pv, !first || k > 0);
+                    if (SPLIT) tc_mma_f16_ta(d, ac + 16, vd + k * (2 * D), id_pv, 1);
+                }
+                tc_commit(&pv_done[tile]);
+            };
+            int i = 0;                  // steps, over all units
+            int np[2] = {0, 0};         // weights taken from each tile, over all units
+            int nq[2] = {0, 0};         // queries taken by each tile
+            for (unsigned x = lo; x < hi && ok;) {
+                const int n = min(cur.steps - cur.step, (int)(hi - x));
+                const int tiles = tiles_of(cur);
+                ok = wait(&k_full[i & 1], (i >> 1) & 1);
+                for (int tl = 0; tl < tiles && ok; ++tl) {
+                    ok = wait(&q_full[tl], nq[tl]++ & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    qk(tl, i & 1);
+                }
+                if (!ok) break;
+                tc_commit(&k_empty[i & 1]);
+                for (int k = 0; k < n && ok; ++k, ++i) {
+                    const bool more = k + 1 < n;
+                    ok = wait(&v_full[i & 1], (i >> 1) & 1);
+                    for (int tl = 0; tl < tiles && ok; ++tl) {
+                        ok = wait(&p_ready[tl], np[tl] & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        pv(tl, i & 1, k == 0);
+                        if (tl == tiles - 1) tc_commit(&v_empty[i & 1]);
+                        if (more) {
+                            // The next scores overwrite the weights that these products read.
+                            ok = wait(&pv_done[tl], np[tl] & 1) && wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            qk(tl, (i + 1) & 1);
+                            if (tl == tiles - 1) tc_commit(&k_empty[(i + 1) & 1]);
+                        }
+                        ++np[tl];
+                    }
+                }
+                x += n;
+                cur.step += n;
+                if (cur.step == cur.steps) {
+                    x += kPreUnitCost;
+                    if (x < hi) next_unit(cur);
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: one thread per row ----
+        const int tile = warp >> 2, r = tid & 127;  // row of the tile, its TMEM lane
+        const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4)
+        const uint32_t ts = tmem + lane_base + tile * NT, to = tmem + lane_base + S::kOCol + tile * D;
+        int i = 0, np = 0;
+        const bool q16 = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+        const bool o16 = ((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) % 16 == 0;
+        for (unsigned x = lo; x < hi && ok;) {
+            const int n = min(cur.steps - cur.step, (int)(hi - x));
+            const int tiles = tiles_of(cur);
+            const int row = cur.chunk * kPreRows + tile * 128 + r, j = row / group;
+            const bool live = j < cur.q.nq;
+            const int seen = live ? seen_of(cur.q, row) : 0;
+            const int64_t col = (int64_t)(cur.head * group + (live ? row - j * group : 0)) * D;
+            // The tile's first row sees least: below that nothing is masked.
+            const int seen_min = cur.chunk * kPreRows + tile * 128 + 127 < cur.q.nq * group
+                                     ? seen_of(cur.q, cur.chunk * kPreRows + tile * 128) : 0;
+            float qf = 0.0f;
+            if (tile < tiles) {
+                // The row, scaled so that its largest element lies in [2^9, 2^10), as f16 hi (and lo).
+                const T* q = (const T*)a.q + (int64_t)(cur.q.row0 + (live ? j : 0)) * a.q_stride + col;
+                float top = 0.0f;
+                constexpr int V = 16 / sizeof(T);
+                auto load = [&](int o, float (&v)[8]) {  // elements 8 o ..
+                    if (!live) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                    } else if (q16) {
+#pragma unroll
+                        for (int b = 0; b < 8 / V; ++b) {
+                            const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + o * 8 + b * V));
+                            const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                            for (int u = 0; u < V; ++u) v[b * V + u] = (float)e[u];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = (float)q[o * 8 + e];
+                    }
+                };
+#pragma unroll 4
+                for (int o = 0; o < D / 8; ++o) {
+                    float v[8];
+                    load(o, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+                }
+                int e = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
+                e = max(-126, min(126, e));
+                const float up = pow2f(e);
+                qf = a.scale * 1.4426950408889634f * pow2f(-e);
+                uint8_t* base = sq + tile * (SPLIT ? 2 : 1) * S::kQPart + (r >> 3) * (D * 16) + (r & 7) * 16;
+#pragma unroll 4
+                for (int o = 0; o < D / 8; ++o) {
+                    float v[8];
+                    load(o, v);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) v[u] *= up;
+                    uint4 h, l;
+                    split_octet(v, h, l);
+                    sts128(smem_u32(base + o * 128), h);
+                    if (SPLIT) sts128(smem_u32(base + S::kQPart + o * 128), l);
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[tile]);
+            }
+            const bool part_of_it = tile < tiles;
+            float m = -INFINITY, l = 0.0f, vl = -120.0f;  // vl: log2 of the reference value scale
+            for (int k = 0; k < n && ok && part_of_it; ++k, ++np) {
+                const int ring = (i + k) % kPreScaleRing;
+                ok = wait(&sc_full[ring], ((i + k) / kPreScaleRing) & 1) && wait(&s_full[tile], np & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const int t0 = (cur.step + k) * NT;
+                const unsigned groups = valid[ring * 2];
+                const bool whole = t0 + NT <= seen_min && groups == (1u << G) - 1u;
+                const float2* sc = scales + ring * G;
+                // Largest score, group by group: the scale is applied to a group's maximum.
+                float top = -INFINITY, lvmax = -120.0f;
+                uint32_t w[2][32];
+                tmem_ld32(ts, w[0]);
+#pragma unroll
+                for (int ch = 0; ch < NT / 32; ++ch) {
+                    tmem_wait_ld32(w[ch & 1]);
+                    if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 g2 = sc[ch * 2 + h];
+                        float mx = -INFINITY;
+                        if (whole) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(w[ch & 1][h * 16 + e]));
+                        } else if (groups >> (ch * 2 + h) & 1) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (t0 + ch * 32 + h * 16 + e < seen) mx = fmaxf(mx, __uint_as_float(w[ch & 1][h * 16 + e]));
+                        }
+                        if (mx > -INFINITY) top = fmaxf(top, mx * (g2.x * qf));
+                        lvmax = fmaxf(lvmax, g2.y);
+                    }
+                }
+                // p <= 2^6 * 2^6 * 2^3 < 65504
+                const bool move = top > m + 6.0f, vmove = lvmax > vl + 3.0f;
+                if (__any_sync(0xffffffffu, move) || vmove) {
+                    float f = 1.0f;
+                    if (move) {
+                        f = ex2(m - top);
+                        l *= f;
+                        m = top;
+                    }
+                    if (vmove) {
+                        f *= ex2(vl - lvmax);
+                        vl = lvmax;
+                    }
+                    if (k > 0) {
+#pragma unroll 1
+                        for (int ch = 0; ch < D / 32; ++ch) {
+                            tmem_ld32(to + ch * 32, w[0]);
+                            tmem_wait_ld32(w[0]);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) w[0][e] = __float_as_uint(__uint_as_float(w[0][e]) * f);
+                            tmem_st32(to + ch * 32, w[0]);
+                        }
+                    }
+                }
+                const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
+                tmem_ld32(ts, w[0]);
+#pragma unroll
+                for (int ch = 0; ch < NT / 32; ++ch) {
+                    tmem_wait_ld32(w[ch & 1]);
+                    if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
+                    uint32_t ph[16], pl[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 g2 = sc[ch * 2 + h];
+                        const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
+                        const float cf = g2.x * qf, b = bias + lr, out = ex2(-lr);
+                        const bool there = whole || (groups >> (ch * 2 + h) & 1);
+                        float p[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float xx = __fmaf_rn(__uint_as_float(w[ch & 1][h * 16 + e]), cf, b);
+                            if (!whole && (!there || t0 + ch * 32 + h * 16 + e >= seen)) xx = -INFINITY;
+                            p[e] = ex2(xx);
+                            if (!whole && !there) continue;
+                            l = __fmaf_rn(p[e], out, l);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (SPLIT) split_f16(p[2 * e], p[2 * e + 1], ph[h * 8 + e], pl[h * 8 + e]);
+                            else ph[h * 8 + e] = pack_f16(p[2 * e], p[2 * e + 1]);
+                        }
+                    }
+                    // Over the 32 columns just read: hi of 32 tokens, then lo.
+                    tmem_st16(ts + ch * 32, ph);
+                    if (SPLIT) tmem_st16(ts + ch * 32 + 16, pl);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[tile]);
+            }
+            i += n;
+            if (ok && part_of_it) {
+                // ---- the segment's end ----
+                ok = wait(&pv_done[tile], (np - 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const bool whole_unit = cur.step == 0 && n == cur.steps;
+                const float vref = ex2(vl);
+                T* dst = (T*)a.out + (int64_t)(cur.q.row0 + (live ? j : 0)) * a.out_stride + col;
+                auto write = [&](int e0, const float (&v)[8]) {
+                    if (!live) return;
+                    if (o16) {
+                        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+                        for (int b = 0; b < 8 / V; ++b) {
+                            uint4 u;
+                            T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+                            for (int q = 0; q < V; ++q) t[q] = (T)v[b * V + q];
+                            *reinterpret_cast<uint4*>(dst + e0 + b * V) = u;
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) dst[e0 + q] = (T)v[q];
+                    }
+                };
+                const int unit_row = tile * 128 + r;
+                const int side = cur.step == 0 ? 1 : 0;  // the piece begins its unit, or goes on with it
+                float* piece = pieces + ((size_t)blockIdx.x * 2 + side) * S::kPieceFloats;
+                const float f = whole_unit ? (l == 0.0f ? 0.0f : vref / l) : vref;
+#pragma unroll 1
+                for (int ch = 0; ch < D / 32; ++ch) {
+                    uint32_t w[32];
+                    tmem_ld32(to + ch * 32, w);
+                    tmem_wait_ld32(w);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = whole_unit && l == 0.0f ? 0.0f : __uint_as_float(w[b * 8 + e]) * f;
+                        if (whole_unit) {
+                            write(ch * 32 + b * 8, v);
+                        } else {  // [element / 4][row][4]
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+                                *reinterpret_cast<float4*>(piece + ((ch * 8 + b * 2 + q) * kPreRows + unit_row) * 4) =
+                                    make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                if (!whole_unit) {
+                    piece[kPreRows * D + unit_row] = m;
+                    piece[kPreRows * D + kPreRows + unit_row] = l;
+                    const unsigned u0 = x - cur.step, u1 = u0 + cur.steps;
+                    const int first = (int)worker_of(u0), last = (int)worker_of(u1 - 1);
+                    __threadfence();
+                    __syncwarp();
+                    int old = 0;
+                    if (lane == 0) old = atomicAdd(counters + first * 8 + warp, 1);
+                    old = __shfl_sync(0xffffffffu, old, 0);
+                    if (old == last - first) {  // every piece of these 32 rows is there
+                        if (lane == 0) counters[first * 8 + warp] = 0;
+                        __threadfence();
+                        auto at = [&](int b) { return pieces + ((size_t)b * 2 + (b == first ? 1 : 0)) * S::kPieceFloats; };
+                        float mx = -INFINITY, sum = 0.0f;
+                        for (int b = first; b <= last; ++b) mx = fmaxf(mx, __ldcg(at(b) + kPreRows * D + unit_row));
+                        for (int b = first; b <= last; ++b) {
+                            const float pm = __ldcg(at(b) + kPreRows * D + unit_row);
+                            sum += __ldcg(at(b) + kPreRows * D + kPreRows + unit_row) * (pm == -INFINITY ? 0.0f : ex2(pm - mx));
+                        }
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+                        for (int e0 = 0; e0 < D; e0 += 32) {
+                            float v[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+                            for (int b = first; b <= last; ++b) {
+                                const float* pc = at(b);
+                                const float pm = __ldcg(pc + kPreRows * D + unit_row);
+                                const float h = pm == -INFINITY ? 0.0f : ex2(pm - mx);
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) {
+                                    const float4 u = __ldcg(reinterpret_cast<const float4*>(pc + ((e0 / 4 + q) * kPreRows + unit_row) * 4));
+                                    v[4 * q] += u.x * h, v[4 * q + 1] += u.y * h, v[4 * q + 2] += u.z * h, v[4 * q + 3] += u.w * h;
+                                }
+                            }
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                float y[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) y[e] = sum == 0.0f ? 0.0f : v[b * 8 + e] * inv;
+                                write(e0 + b * 8, y);
+                            }
+                        }
+                    }
+                }
+            }
+            x += n;
+            cur.step += n;
+            if (cur.step == cur.steps) {
+                x += kPreUnitCost;
+                if (x < hi) next_unit(cur);
+            }
+        }
+    }
+    // Everyone meets when all products and their arrivals are done, also where
+    // a wait has given up.
+    if (warp == 12 && lane == 0) {
+        tc_commit(&drained);
+        mbar_wait_bounded(&drained, 0, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
+        if (unset) atomicCAS(err, 0, kDevTimeoutDrain);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int FMT, int D>
+cudaError_t kv8_prefill_prepare() {
+    return cudaFuncSetAttribute(kv8_prefill_kernel<T, FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                PreShape<T, D>::kSmem + (kPagesMaxSeqs + 1) * (int)sizeof(unsigned));
+}
+
+template <typename T, int FMT, int D>
+cudaError_t launch_kv8_prefill(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, int* err, cudaStream_t st) {
+    const int smem = PreShape<T, D>::kSmem + (a.n_seqs + 1) * (int)sizeof(unsigned);
+    int* counters = (int*)ws;
+    float* pieces = (float*)((uint8_t*)ws + kv8_prefill_counter_bytes(num_sms));
+    return launch_ex(kv8_prefill_kernel<T, FMT, D>, dim3(num_sms), dim3(kPreThreads), smem, st, true, c, a, pieces, counters,
+                     err, (uint64_t)2000000000ull);
+}
+
+}  // namespace lc

@@ -72,6 +72,6 @@ struct Kv8Attention {
 // prepare clears its counters and sets the kernels' attributes, once.
 size_t kv8_attention_ws_bytes(int num_sms);
 cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st);
-cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, cudaStream_t st);
+cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, int* err, cudaStream_t st);
 
 }  // namespace lc
