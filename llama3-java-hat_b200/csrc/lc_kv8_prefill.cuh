@@ -527,27 +527,28 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 // Largest score, group by group: the scale is applied to a group's maximum.
                 float top = -INFINITY, lvmax = -120.0f;
                 uint32_t w[2][32];
-                tmem_ld32(ts, w[0]);
+                auto largest = [&](auto masked) {
+                    tmem_ld32(ts, w[0]);
 #pragma unroll
-                for (int ch = 0; ch < NT / 32; ++ch) {
-                    tmem_wait_ld32(w[ch & 1]);
-                    if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
+                    for (int ch = 0; ch < NT / 32; ++ch) {
+                        tmem_wait_ld32(w[ch & 1]);
+                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float2 g2 = sc[ch * 2 + h];
-                        float mx = -INFINITY;
-                        if (whole) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(w[ch & 1][h * 16 + e]));
-                        } else if (groups >> (ch * 2 + h) & 1) {
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 g2 = sc[ch * 2 + h];
+                            const int left = masked ? (groups >> (ch * 2 + h) & 1 ? seen - t0 - ch * 32 - h * 16 : 0) : 16;
+                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
-                                if (t0 + ch * 32 + h * 16 + e < seen) mx = fmaxf(mx, __uint_as_float(w[ch & 1][h * 16 + e]));
+                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[ch & 1][h * 16 + e]) : -INFINITY);
+                            const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                            top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
+                            lvmax = fmaxf(lvmax, g2.y);
                         }
-                        if (mx > -INFINITY) top = fmaxf(top, mx * (g2.x * qf));
-                        lvmax = fmaxf(lvmax, g2.y);
                     }
-                }
+                };
+                if (whole) largest(std::false_type());
+                else largest(std::true_type());
                 // p <= 2^6 * 2^6 * 2^3 < 65504
                 const bool move = top > m + 6.0f, vmove = lvmax > vl + 3.0f;
                 if (__any_sync(0xffffffffu, move) || vmove) {
@@ -573,37 +574,41 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     }
                 }
                 const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
-                tmem_ld32(ts, w[0]);
+                auto weigh = [&](auto masked) {
+                    tmem_ld32(ts, w[0]);
 #pragma unroll
-                for (int ch = 0; ch < NT / 32; ++ch) {
-                    tmem_wait_ld32(w[ch & 1]);
-                    if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
-                    uint32_t ph[16], pl[16];
+                    for (int ch = 0; ch < NT / 32; ++ch) {
+                        tmem_wait_ld32(w[ch & 1]);
+                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
+                        uint32_t ph[16], pl[16];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float2 g2 = sc[ch * 2 + h];
-                        const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
-                        const float cf = g2.x * qf, b = bias + lr, out = ex2(-lr);
-                        const bool there = whole || (groups >> (ch * 2 + h) & 1);
-                        float p[16];
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 g2 = sc[ch * 2 + h];
+                            const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
+                            const float cf = g2.x * qf, b = bias + lr, out = ex2(-lr);
+                            const int left = masked ? (groups >> (ch * 2 + h) & 1 ? seen - t0 - ch * 32 - h * 16 : 0) : 16;
+                            float part[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float xx = __fmaf_rn(__uint_as_float(w[ch & 1][h * 16 + e]), cf, b);
-                            if (!whole && (!there || t0 + ch * 32 + h * 16 + e >= seen)) xx = -INFINITY;
-                            p[e] = ex2(xx);
-                            if (!whole && !there) continue;
-                            l = __fmaf_rn(p[e], out, l);
+                            for (int e = 0; e < 8; ++e) {
+                                float p[2];
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) {
+                                    const float xx = __fmaf_rn(__uint_as_float(w[ch & 1][h * 16 + 2 * e + u]), cf, b);
+                                    p[u] = ex2(!masked || 2 * e + u < left ? xx : -INFINITY);
+                                    part[u] += p[u];
+                                }
+                                if (SPLIT) split_f16(p[0], p[1], ph[h * 8 + e], pl[h * 8 + e]);
+                                else ph[h * 8 + e] = pack_f16(p[0], p[1]);
+                            }
+                            l = __fmaf_rn(part[0] + part[1], out, l);
                         }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (SPLIT) split_f16(p[2 * e], p[2 * e + 1], ph[h * 8 + e], pl[h * 8 + e]);
-                            else ph[h * 8 + e] = pack_f16(p[2 * e], p[2 * e + 1]);
-                        }
+                        // Over the 32 columns just read: hi of 32 tokens, then lo.
+                        tmem_st16(ts + ch * 32, ph);
+                        if (SPLIT) tmem_st16(ts + ch * 32 + 16, pl);
                     }
-                    // Over the 32 columns just read: hi of 32 tokens, then lo.
-                    tmem_st16(ts + ch * 32, ph);
-                    if (SPLIT) tmem_st16(ts + ch * 32 + 16, pl);
-                }
+                };
+                if (whole) weigh(std::false_type());
+                else weigh(std::true_type());
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
