@@ -13,14 +13,23 @@
 // likewise, at the price of twice the products; f16 rows take one pass and
 // round P to f16 (2^-12 of each weight), as the result is.
 //
+// The tensor cores' fp32 sums lose up to one unit of the last place, always
+// toward zero, at every product that is added; over thousands of tokens that
+// drifts (4.8e-6 of the result at 4096 tokens, against 1e-6 of fp32 sums), so
+// after kFlush steps O is added to a second accumulator in round-to-nearest
+// and begun anew: in tensor memory where there is room (head size 64), in the
+// CTA's piece in L2 otherwise.
+//
 // What bounds it: for head size 64 one exponential costs as much as the 128
 // products of its score, so the special-function unit and the issue slots
 // around it, not the tensor cores, set the pace; hence two row tiles, whose
 // softmax warpgroups take turns with the tensor cores, and one dequantised
 // tile for both.
 //
-// Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: codes to f16.
-// Warp 12: issues the MMAs.  All steps of the call form one line that is cut
+// Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: queries and
+// codes to f16 operands, a unit's queries while its predecessor's last step is
+// weighed.  Warp 12: issues the MMAs.  Registers move from the last two
+// warpgroups to the softmax.  All steps of the call form one line that is cut
 // into equal pieces, one per CTA; pieces of a unit are joined, warp by warp,
 // by the last CTA to finish, in the order of the line.
 #pragma once
@@ -32,8 +41,12 @@
 namespace lc {
 
 constexpr int kPreRows = 256;      // rows of a unit
-constexpr int kPreThreads = 13 * 32;
-constexpr int kPreUnitCost = 1;    // a unit's beginning and end, in steps
+constexpr int kPreThreads = 16 * 32;
+// Registers of the softmax, operand and MMA warpgroups after the split; their sum
+// over 128 threads each must not pass the launch's (checked on the host).
+constexpr int kPreRegsSoftmax = 168, kPreRegsOperand = 88, kPreRegsMma = 88;
+constexpr int kPreRegsLaunch = (2 * kPreRegsSoftmax + kPreRegsOperand + kPreRegsMma + 3) / 4;
+constexpr int kPreUnitCost = 2;    // a unit's beginning and end, in steps
 constexpr int kPreScaleRing = 4;
 
 template <typename T, int D>
@@ -45,9 +58,13 @@ struct PreShape {
     static constexpr int kQBytes = 2 * (kSplit ? 2 : 1) * kQPart;
     static constexpr int kTileBytes = kTok * D * 2;       // 16 KB
     static constexpr int kScaleBytes = kPreScaleRing * (kGroups * 8 + 8);
-    static constexpr int kSmem = kQBytes + 4 * kTileBytes + kScaleBytes;
+    static constexpr int kSmem = kQBytes + 4 * kTileBytes + kScaleBytes + kPreRows * 4;
     static constexpr int kPieceFloats = kPreRows * (D + 2);
-    static constexpr uint32_t kOCol = 2 * kTok;           // tensor memory: S of both tiles, then O of both
+    static constexpr uint32_t kOCol = 2 * kTok;           // tensor memory: S of both tiles, O of both,
+    static constexpr uint32_t kSumCol = kOCol + 2 * D;     // and for head size 64 the second accumulators
+    static constexpr bool kSumInTmem = D == 64;
+    // Steps between additions to it: 256 tokens (D 64) or 512 in fp32, 8192 in f16.
+    static constexpr int kFlush = kSplit ? (D == 64 ? 2 : 8) : 8192 / kTok;
 };
 
 inline size_t kv8_prefill_counter_bytes(int num_sms) { return ((size_t)num_sms * 8 * sizeof(int) + 255) / 256 * 256; }
@@ -134,12 +151,13 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     uint8_t* const sv = sk + 2 * S::kTileBytes;                 // [2 stages]
     float2* const scales = reinterpret_cast<float2*>(sv + 2 * S::kTileBytes);  // [ring][group]: key scale, log2 of the value scale
     unsigned* const valid = reinterpret_cast<unsigned*>(scales + kPreScaleRing * G);  // [ring][2]
-    unsigned* const prefix = valid + kPreScaleRing * 2;                                // [n_seqs + 1]
-    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], pv_done[2], q_full[2],
+    float* const qscale = reinterpret_cast<float*>(valid + kPreScaleRing * 2);         // [rows] score factor of each row
+    unsigned* const prefix = reinterpret_cast<unsigned*>(qscale + kPreRows);           // [n_seqs + 1]
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], pv_done[2], q_full, q_seen,
         sc_full[kPreScaleRing], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
-    __shared__ unsigned scan[13];
+    __shared__ unsigned scan[kPreThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = a.n_heads / c.n_kv, sh = c.page_shift;
     const int room = (int)min((long long)a.table_stride << sh, 0x7fffffffll);
@@ -150,10 +168,9 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             mbar_init(&k_full[i], 4), mbar_init(&v_full[i], 4);
             mbar_init(&k_empty[i], 1), mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4), mbar_init(&pv_done[i], 1);
-            mbar_init(&q_full[i], 4);
         }
         for (int i = 0; i < kPreScaleRing; ++i) mbar_init(&sc_full[i], 1);
-        mbar_init(&drained, 1);
+        mbar_init(&q_full, 4), mbar_init(&q_seen, 8), mbar_init(&drained, 1);
         fence_mbar_init();
     }
     griddep_launch();
@@ -164,7 +181,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     auto chunks_of = [&](const SeqInfo& q) { return (int)(((int64_t)q.nq * group + kPreRows - 1) / kPreRows); };
 
     // ---- the line of steps: a warp per sequence, lanes over its chunks ----
-    for (int s = warp; s < a.n_seqs; s += 13) {
+    for (int s = warp; s < a.n_seqs; s += kPreThreads / 32) {
         const SeqInfo q = kv8_seq(a, sh, s);
         const int chunks = chunks_of(q);
         unsigned cost = 0;
@@ -186,7 +203,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         if (lane == 31) scan[warp] = v;
         __syncthreads();
         unsigned before = carry, all = carry;
-        for (int w = 0; w < 13; ++w) {
+        for (int w = 0; w < kPreThreads / 32; ++w) {
             if (w < warp) before += scan[w];
             all += scan[w];
         }
@@ -286,7 +303,8 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     bool ok = true;
 
     if (warp >= 8 && warp < 12) {
-        // ---- codes to f16 ----
+        // ---- operands to f16 ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsOperand));
         const int cw = warp - 8;
         uint4 kc[4], vc[4];
         int id[4];
@@ -303,29 +321,28 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 id[k] = t < u.seen ? row[t >> sh] : -1;
             }
         };
-        float my_ks = 0.0f, my_lv = -120.0f;
+        float my_ks = 0.0f, my_lv = -120.0f;  // scales of 16-token group `lane`, by the first warp
         bool my_ok = false;
-        auto load_codes = [&](const PreCursor& u) {
+        auto load_codes = [&](const PreCursor& u, const uint8_t* codes, uint4 (&w)[4]) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int t = u.step * NT + token_of(k);
-                kc[k] = vc[k] = make_uint4(0, 0, 0, 0);
-                if ((unsigned)id[k] < (unsigned)c.n_pages) {
-                    const int64_t at = ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16;
-                    kc[k] = __ldg(reinterpret_cast<const uint4*>(c.k + at));
-                    vc[k] = __ldg(reinterpret_cast<const uint4*>(c.v + at));
-                }
+                w[k] = make_uint4(0, 0, 0, 0);  // tokens that nobody sees stay zero: there may be NaN codes
+                if ((unsigned)id[k] < (unsigned)c.n_pages)
+                    w[k] = __ldg(reinterpret_cast<const uint4*>(
+                        codes + ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16));
             }
-            if (cw == 0 && lane < G) {  // scales of 16-token group `lane`
-                const int t = u.step * NT + lane * 16;
-                const int page = t < u.seen ? a.table[(int64_t)u.s * a.table_stride + (t >> sh)] : -1;
-                my_ok = (unsigned)page < (unsigned)c.n_pages;
-                my_ks = 0.0f, my_lv = -120.0f;
-                if (my_ok) {
-                    my_ks = c.k_scale[(int64_t)page * c.n_kv + u.head];
-                    const float v = c.v_scale[(int64_t)page * c.n_kv + u.head];
-                    my_lv = v < 1e-36f ? -120.0f : log2f(v);  // NaN stays
-                }
+        };
+        auto load_scales = [&](const PreCursor& u) {
+            if (cw != 0 || lane >= G) return;
+            const int t = u.step * NT + lane * 16;
+            const int page = t < u.seen ? a.table[(int64_t)u.s * a.table_stride + (t >> sh)] : -1;
+            my_ok = (unsigned)page < (unsigned)c.n_pages;
+            my_ks = 0.0f, my_lv = -120.0f;
+            if (my_ok) {
+                my_ks = c.k_scale[(int64_t)page * c.n_kv + u.head];
+                const float v = c.v_scale[(int64_t)page * c.n_kv + u.head];
+                my_lv = v < 1e-36f ? -120.0f : log2f(v);  // NaN stays
             }
         };
         auto put = [&](uint8_t* tile, const uint4 (&w)[4]) {
@@ -341,6 +358,75 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 sts128(at + 128, make_uint4(f[4], f[5], f[6], f[7]));
             }
         };
+        // The unit's rows, each scaled so that its largest element lies in
+        // [2^9, 2^10), as f16 hi (and lo).
+        const bool q16 = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+        auto query = [&](const PreCursor& u, int r) -> const T* {  // row r of the unit; null behind its last
+            const int row = u.chunk * kPreRows + r, j = row / group;
+            if (j >= u.q.nq) return nullptr;
+            return (const T*)a.q + (int64_t)(u.q.row0 + j) * a.q_stride + (int64_t)(u.head * group + row - j * group) * D;
+        };
+        auto prefetch_queries = [&](PreCursor u) {  // of the next unit, to L2
+            next_unit(u);
+            const int rows = tiles_of(u) * 128;
+            for (int r = cw * 32 + lane; r < rows; r += 128) {
+                const T* q = query(u, r);
+                if (!q) break;
+#pragma unroll
+                for (int o = 0; o < D * (int)sizeof(T); o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"((const uint8_t*)q + o));
+            }
+        };
+        auto put_queries = [&](const PreCursor& u) {
+            const int rows = tiles_of(u) * 128;
+#pragma unroll 1
+            for (int r = cw * 32 + lane; r < rows; r += 128) {  // a thread per row
+                const T* q = query(u, r);
+                auto load = [&](int o, float (&v)[8]) {  // elements 8 o ..
+                    constexpr int V = 16 / sizeof(T);
+                    if (!q) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                    } else if (q16) {
+#pragma unroll
+                        for (int b = 0; b < 8 / V; ++b) {
+                            const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + o * 8 + b * V));
+                            const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                            for (int i = 0; i < V; ++i) v[b * V + i] = (float)e[i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = (float)q[o * 8 + e];
+                    }
+                };
+                float top = 0.0f;
+#pragma unroll 4
+                for (int o = 0; o < D / 8; ++o) {
+                    float v[8];
+                    load(o, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+                }
+                int ex = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
+                ex = max(-126, min(126, ex));
+                const float up = pow2f(ex);
+                qscale[r] = a.scale * 1.4426950408889634f * pow2f(-ex);
+                const uint32_t at = smem_u32(sq) + (r >> 7) * (SPLIT ? 2 : 1) * S::kQPart + ((r & 127) >> 3) * (D * 16) + (r & 7) * 16;
+#pragma unroll 4
+                for (int o = 0; o < D / 8; ++o) {  // the second reading comes from L1
+                    float v[8];
+                    load(o, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= up;
+                    uint4 h, l;
+                    split_octet(v, h, l);
+                    sts128(at + o * 128, h);
+                    if (SPLIT) sts128(at + S::kQPart + o * 128, l);
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+        };
         PreCursor nx = cur;
         unsigned ahead = lo;
         auto advance = [&]() {
@@ -350,24 +436,35 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 if (ahead < hi) next_unit(nx);
             }
         };
-        if (ahead < hi) load_ids(nx), load_codes(nx);
+        if (ahead < hi) {
+            load_ids(nx);
+            load_scales(nx);
+            load_codes(nx, c.k, kc);
+            load_codes(nx, c.v, vc);
+        }
+        int units = 0;
+        // The next step's loads are under way while this one's tiles are written.
         for (int i = 0; ahead < hi && ok; ++i) {
-            uint4 k0[4], v0[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) k0[k] = kc[k], v0[k] = vc[k];
-            const float ks = my_ks, lv = my_lv;
-            const bool group_ok = my_ok;
-            // Words whose token nobody sees stay zero: a tile's last tokens may be NaN codes.
+            if (i == 0 || nx.step == 0) {
+                // The previous unit's scores are all computed, its score factors read.
+                if (i > 0) ok = wait(&k_empty[(i - 1) & 1], ((i - 1) >> 1) & 1) && wait(&q_seen, (units - 1) & 1);
+                if (!ok) break;
+                put_queries(nx);
+                if (lane == 0) mbar_arrive(&q_full);
+                ++units;
+                if (ahead + (nx.steps - nx.step) + kPreUnitCost < hi) prefetch_queries(nx);
+            }
             advance();
-            if (ahead < hi) load_ids(nx), load_codes(nx);
+            const bool more = ahead < hi;
+            if (more) load_ids(nx);
             const int st = i & 1, use = i >> 1;
             if (use > 0) ok = wait(&k_empty[st], (use - 1) & 1);
             if (!ok) break;
-            put(sk + st * S::kTileBytes, k0);
+            put(sk + st * S::kTileBytes, kc);
             if (cw == 0) {
                 const int ring = i % kPreScaleRing;
-                if (lane < G) scales[ring * G + lane] = make_float2(ks, lv);
-                const unsigned m = __ballot_sync(0xffffffffu, lane < G && group_ok);
+                if (lane < G) scales[ring * G + lane] = make_float2(my_ks, my_lv);
+                const unsigned m = __ballot_sync(0xffffffffu, lane < G && my_ok);
                 if (lane == 0) valid[ring * 2] = m;
             }
             fence_async_shared();
@@ -376,16 +473,22 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 mbar_arrive(&k_full[st]);
                 if (cw == 0) mbar_arrive(&sc_full[i % kPreScaleRing]);
             }
+            if (more) {
+                load_codes(nx, c.k, kc);
+                load_scales(nx);
+            }
             if (use > 0) ok = wait(&v_empty[st], (use - 1) & 1);
             if (!ok) break;
-            put(sv + st * S::kTileBytes, v0);
+            put(sv + st * S::kTileBytes, vc);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[st]);
+            if (more) load_codes(nx, c.v, vc);
         }
-    } else if (warp == 12) {
+    } else if (warp >= 12) {
         // ---- MMAs: one thread of a warp that stays together ----
-        {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsMma));
+        if (warp == 12) {
             constexpr uint32_t id_qk = tc_idesc_f16_f32(128, NT);
             constexpr uint32_t id_pv = tc_idesc_f16_f32(128, D) | (1u << 16);  // B (values) with the head's elements contiguous
             auto qk = [&](int tile, int st) {
@@ -424,13 +527,13 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             };
             int i = 0;                  // steps, over all units
             int np[2] = {0, 0};         // weights taken from each tile, over all units
-            int nq[2] = {0, 0};         // queries taken by each tile
+            int units = 0;
             for (unsigned x = lo; x < hi && ok;) {
                 const int n = min(cur.steps - cur.step, (int)(hi - x));
                 const int tiles = tiles_of(cur);
-                ok = wait(&k_full[i & 1], (i >> 1) & 1);
+                ok = wait(&q_full, units++ & 1) && wait(&k_full[i & 1], (i >> 1) & 1);
                 for (int tl = 0; tl < tiles && ok; ++tl) {
-                    ok = wait(&q_full[tl], nq[tl]++ & 1);
+                    if (np[tl] > 0) ok = wait(&pv_done[tl], (np[tl] - 1) & 1);  // the weights of the unit before are read
                     if (!ok) break;
                     tc_fence_after();
                     qk(tl, i & 1);
@@ -444,7 +547,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                         ok = wait(&p_ready[tl], np[tl] & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        pv(tl, i & 1, k == 0);
+                        pv(tl, i & 1, k % S::kFlush == 0);
                         if (tl == tiles - 1) release(&v_empty[i & 1]);
                         if (more) {
                             // The next scores overwrite the weights that these products read.
@@ -468,11 +571,12 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         __syncwarp();
     } else {
         // ---- softmax: one thread per row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsSoftmax));
         const int tile = warp >> 2, r = tid & 127;  // row of the tile, its TMEM lane
         const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4)
         const uint32_t ts = tmem + lane_base + tile * NT, to = tmem + lane_base + S::kOCol + tile * D;
-        int i = 0, np = 0;
-        const bool q16 = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+        const uint32_t tsum = tmem + lane_base + S::kSumCol + tile * D;
+        int i = 0, np = 0, units = 0;
         const bool o16 = ((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) % 16 == 0;
         for (unsigned x = lo; x < hi && ok;) {
             const int n = min(cur.steps - cur.step, (int)(hi - x));
@@ -484,56 +588,51 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             // The tile's first row sees least: below that nothing is masked.
             const int seen_min = cur.chunk * kPreRows + tile * 128 + 127 < cur.q.nq * group
                                      ? seen_of(cur.q, cur.chunk * kPreRows + tile * 128) : 0;
-            float qf = 0.0f;
-            if (tile < tiles) {
-                // The row, scaled so that its largest element lies in [2^9, 2^10), as f16 hi (and lo).
-                const T* q = (const T*)a.q + (int64_t)(cur.q.row0 + (live ? j : 0)) * a.q_stride + col;
-                float top = 0.0f;
-                constexpr int V = 16 / sizeof(T);
-                auto load = [&](int o, float (&v)[8]) {  // elements 8 o ..
-                    if (!live) {
+            ok = wait(&q_full, units++ & 1);
+            if (!ok) break;
+            const float qf = qscale[tile * 128 + r];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_seen);
+            const int unit_row = tile * 128 + r;
+            const int side = cur.step == 0 ? 1 : 0;  // the piece begins its unit, or goes on with it
+            float* piece = pieces + ((size_t)blockIdx.x * 2 + side) * S::kPieceFloats;
+            // Adds O to the second accumulator, which carries the factor `since` behind its last addition.
+            bool flushed = false;
+            float since = 1.0f;
+            auto sum_at = [&](int e4) { return reinterpret_cast<float4*>(piece + ((size_t)e4 * kPreRows + unit_row) * 4); };
+            auto flush = [&]() {
+#pragma unroll 1
+                for (int ch = 0; ch < D / 32; ++ch) {
+                    uint32_t w[32];
+                    tmem_ld32(to + ch * 32, w);
+                    if constexpr (S::kSumInTmem) {
+                        uint32_t z[32];
+                        if (flushed) tmem_ld32(tsum + ch * 32, z);
+                        tmem_wait_ld32(w);
+                        if (flushed) {
+                            tmem_wait_ld32(z);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-                    } else if (q16) {
-#pragma unroll
-                        for (int b = 0; b < 8 / V; ++b) {
-                            const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + o * 8 + b * V));
-                            const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-                            for (int u = 0; u < V; ++u) v[b * V + u] = (float)e[u];
+                            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), since, __uint_as_float(w[e])));
                         }
+                        tmem_st32(tsum + ch * 32, w);
                     } else {
+                        float4 z[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = (float)q[o * 8 + e];
+                        for (int q = 0; q < 8; ++q) z[q] = flushed ? __ldcg(sum_at(ch * 8 + q)) : make_float4(0, 0, 0, 0);
+                        tmem_wait_ld32(w);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            z[q].x = __fmaf_rn(z[q].x, since, __uint_as_float(w[4 * q]));
+                            z[q].y = __fmaf_rn(z[q].y, since, __uint_as_float(w[4 * q + 1]));
+                            z[q].z = __fmaf_rn(z[q].z, since, __uint_as_float(w[4 * q + 2]));
+                            z[q].w = __fmaf_rn(z[q].w, since, __uint_as_float(w[4 * q + 3]));
+                            __stcg(sum_at(ch * 8 + q), z[q]);
+                        }
                     }
-                };
-#pragma unroll 4
-                for (int o = 0; o < D / 8; ++o) {
-                    float v[8];
-                    load(o, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
                 }
-                int e = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
-                e = max(-126, min(126, e));
-                const float up = pow2f(e);
-                qf = a.scale * 1.4426950408889634f * pow2f(-e);
-                uint8_t* base = sq + tile * (SPLIT ? 2 : 1) * S::kQPart + (r >> 3) * (D * 16) + (r & 7) * 16;
-#pragma unroll 4
-                for (int o = 0; o < D / 8; ++o) {
-                    float v[8];
-                    load(o, v);
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) v[u] *= up;
-                    uint4 h, l;
-                    split_octet(v, h, l);
-                    sts128(smem_u32(base + o * 128), h);
-                    if (SPLIT) sts128(smem_u32(base + S::kQPart + o * 128), l);
-                }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[tile]);
-            }
+                flushed = true;
+                since = 1.0f;
+            };
             const bool part_of_it = tile < tiles;
             float m = -INFINITY, l = 0.0f, vl = -120.0f;  // vl: log2 of the reference value scale
             for (int k = 0; k < n && ok && part_of_it; ++k, ++np) {
@@ -545,15 +644,20 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const unsigned groups = valid[ring * 2];
                 const bool whole = t0 + NT <= seen_min && groups == (1u << G) - 1u;
                 const float2* sc = scales + ring * G;
+                const bool anew = k % S::kFlush == 0;  // these products begin O anew
+                if (anew && k > 0) flush();
                 // Largest score, group by group: the scale is applied to a group's maximum.
                 float top = -INFINITY, lvmax = -120.0f;
                 uint32_t w[2][32];
                 auto largest = [&](auto masked) {
                     tmem_ld32(ts, w[0]);
+#pragma unroll 1
+                    for (int c2 = 0; c2 < NT / 32; c2 += 2)
 #pragma unroll
-                    for (int ch = 0; ch < NT / 32; ++ch) {
-                        tmem_wait_ld32(w[ch & 1]);
-                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
+                    for (int c1 = 0; c1 < 2; ++c1) {
+                        const int ch = c2 + c1;
+                        tmem_wait_ld32(w[c1]);
+                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[c1 ^ 1]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float2 g2 = sc[ch * 2 + h];
@@ -561,7 +665,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
-                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[ch & 1][h * 16 + e]) : -INFINITY);
+                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[c1][h * 16 + e]) : -INFINITY);
                             const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                             top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
                             lvmax = fmaxf(lvmax, g2.y);
@@ -583,7 +687,8 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                         f *= ex2(vl - lvmax);
                         vl = lvmax;
                     }
-                    if (k > 0) {
+                    since *= f;
+                    if (!anew) {
 #pragma unroll 1
                         for (int ch = 0; ch < D / 32; ++ch) {
                             tmem_ld32(to + ch * 32, w[0]);
@@ -597,10 +702,13 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
                 auto weigh = [&](auto masked) {
                     tmem_ld32(ts, w[0]);
+#pragma unroll 1
+                    for (int c2 = 0; c2 < NT / 32; c2 += 2)
 #pragma unroll
-                    for (int ch = 0; ch < NT / 32; ++ch) {
-                        tmem_wait_ld32(w[ch & 1]);
-                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[(ch + 1) & 1]);
+                    for (int c1 = 0; c1 < 2; ++c1) {
+                        const int ch = c2 + c1;
+                        tmem_wait_ld32(w[c1]);
+                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[c1 ^ 1]);
                         uint32_t ph[16], pl[16];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -614,7 +722,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                                 float p[2];
 #pragma unroll
                                 for (int u = 0; u < 2; ++u) {
-                                    const float xx = __fmaf_rn(__uint_as_float(w[ch & 1][h * 16 + 2 * e + u]), cf, b);
+                                    const float xx = __fmaf_rn(__uint_as_float(w[c1][h * 16 + 2 * e + u]), cf, b);
                                     p[u] = ex2(!masked || 2 * e + u < left ? xx : -INFINITY);
                                     part[u] += p[u];
                                 }
@@ -661,15 +769,33 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                         for (int q = 0; q < 8; ++q) dst[e0 + q] = (T)v[q];
                     }
                 };
-                const int unit_row = tile * 128 + r;
-                const int side = cur.step == 0 ? 1 : 0;  // the piece begins its unit, or goes on with it
-                float* piece = pieces + ((size_t)blockIdx.x * 2 + side) * S::kPieceFloats;
                 const float f = whole_unit ? (l == 0.0f ? 0.0f : vref / l) : vref;
 #pragma unroll 1
                 for (int ch = 0; ch < D / 32; ++ch) {
                     uint32_t w[32];
                     tmem_ld32(to + ch * 32, w);
-                    tmem_wait_ld32(w);
+                    if constexpr (S::kSumInTmem) {
+                        uint32_t z[32];
+                        if (flushed) tmem_ld32(tsum + ch * 32, z);
+                        tmem_wait_ld32(w);
+                        if (flushed) {
+                            tmem_wait_ld32(z);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), since, __uint_as_float(w[e])));
+                        }
+                    } else {
+                        tmem_wait_ld32(w);
+                        if (flushed) {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                const float4 z = __ldcg(sum_at(ch * 8 + q));
+                                w[4 * q] = __float_as_uint(__fmaf_rn(z.x, since, __uint_as_float(w[4 * q])));
+                                w[4 * q + 1] = __float_as_uint(__fmaf_rn(z.y, since, __uint_as_float(w[4 * q + 1])));
+                                w[4 * q + 2] = __float_as_uint(__fmaf_rn(z.z, since, __uint_as_float(w[4 * q + 2])));
+                                w[4 * q + 3] = __float_as_uint(__fmaf_rn(z.w, since, __uint_as_float(w[4 * q + 3])));
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         float v[8];
@@ -756,6 +882,11 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
 
 template <typename T, int FMT, int D>
 cudaError_t kv8_prefill_prepare() {
+    // The register split draws on what the launch has: more than that would wait forever.
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, kv8_prefill_kernel<T, FMT, D>);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs < kPreRegsLaunch) return cudaErrorInvalidKernelImage;
     return cudaFuncSetAttribute(kv8_prefill_kernel<T, FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 PreShape<T, D>::kSmem + (kPagesMaxSeqs + 1) * (int)sizeof(unsigned));
 }
