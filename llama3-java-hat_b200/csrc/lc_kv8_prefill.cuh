@@ -2,7 +2,7 @@
 // sequence (prompt chunks), on the tcgen05 tensor cores.
 //
 // A unit is 256 (query, head) rows that share a kv head, as two tiles of 128
-// MMA rows; a step is one tile of NT tokens.  Per step and row tile
+// MMA rows; a step is NT = 64 tokens.  Per step and row tile
 //   S = Q K^T   M 128, N NT, K head size: Q and K codes f16 in shared memory
 //   p = 2^(S c + b), running maximum and sum, one thread per row
 //   O += P V    M 128, N head size, K NT: P in tensor memory over S's columns
@@ -28,7 +28,7 @@
 //
 // Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: queries and
 // codes to f16 operands, a unit's queries while its predecessor's last step is
-// weighed.  Warp 12: issues the MMAs.  Registers move from the last two
+// weighed.  Warps 12 and 13: issue the MMAs of a row tile each.  Registers move from the last two
 // warpgroups to the softmax.  All steps of the call form one line that is cut
 // into equal pieces, one per CTA; pieces of a unit are joined, warp by warp,
 // by the last CTA to finish, in the order of the line.
@@ -44,27 +44,31 @@ constexpr int kPreRows = 256;      // rows of a unit
 constexpr int kPreThreads = 16 * 32;
 // Registers of the softmax, operand and MMA warpgroups after the split; their sum
 // over 128 threads each must not pass the launch's (checked on the host).
-constexpr int kPreRegsSoftmax = 168, kPreRegsOperand = 88, kPreRegsMma = 88;
+constexpr int kPreRegsSoftmax = 168, kPreRegsOperand = 120, kPreRegsMma = 56;
 constexpr int kPreRegsLaunch = (2 * kPreRegsSoftmax + kPreRegsOperand + kPreRegsMma + 3) / 4;
-constexpr int kPreUnitCost = 2;    // a unit's beginning and end, in steps
-constexpr int kPreScaleRing = 4;
+constexpr int kPreTok = 64;        // tokens of a step
+constexpr int kPreUnitCost = 3;    // a unit's beginning and end, in steps
+constexpr int kPreScaleRing = 8;   // more steps than the operand warps can be ahead of the softmax
 
 template <typename T, int D>
 struct PreShape {
     static constexpr bool kSplit = sizeof(T) == 4;
-    static constexpr int kTok = 8192 / D;                 // NT: 128 or 64 tokens
-    static constexpr int kGroups = kTok / 16;
+    static constexpr int kGroups = kPreTok / 16;
+    static constexpr int kStages = D == 64 ? 4 : 2;        // operand tiles of K, and of V
+    static constexpr int kQBufs = kSplit && D == 128 ? 1 : 2;  // units whose queries are held
     static constexpr int kQPart = 128 * D * 2;            // bytes of one part (hi or lo) of one row tile
     static constexpr int kQBytes = 2 * (kSplit ? 2 : 1) * kQPart;
-    static constexpr int kTileBytes = kTok * D * 2;       // 16 KB
+    static constexpr int kTileBytes = kPreTok * D * 2;
     static constexpr int kScaleBytes = kPreScaleRing * (kGroups * 8 + 8);
-    static constexpr int kSmem = kQBytes + 4 * kTileBytes + kScaleBytes + kPreRows * 4;
+    static constexpr int kSmem = kQBufs * (kQBytes + kPreRows * 4) + 2 * kStages * kTileBytes + kScaleBytes;
     static constexpr int kPieceFloats = kPreRows * (D + 2);
-    static constexpr uint32_t kOCol = 2 * kTok;           // tensor memory: S of both tiles, O of both,
-    static constexpr uint32_t kSumCol = kOCol + 2 * D;     // and for head size 64 the second accumulators
+    // Tensor memory: two buffers of S for each tile, so that the next step's
+    // scores are there when a step's weights are done; O of both tiles;
+    // and for head size 64 the second accumulators.
+    static constexpr uint32_t kOCol = 4 * kPreTok, kSumCol = kOCol + 2 * D;
     static constexpr bool kSumInTmem = D == 64;
     // Steps between additions to it: 256 tokens (D 64) or 512 in fp32, 8192 in f16.
-    static constexpr int kFlush = kSplit ? (D == 64 ? 2 : 8) : 8192 / kTok;
+    static constexpr int kFlush = kSplit ? (D == 64 ? 4 : 8) : 128;
 };
 
 inline size_t kv8_prefill_counter_bytes(int num_sms) { return ((size_t)num_sms * 8 * sizeof(int) + 255) / 256 * 256; }
@@ -143,17 +147,18 @@ template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(kPreThreads, 1)
 kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __restrict__ counters, int* err, uint64_t timeout_ns) {
     using S = PreShape<T, D>;
-    constexpr int NT = S::kTok, G = S::kGroups;
+    constexpr int NT = kPreTok, G = S::kGroups, NS = S::kStages;
     constexpr bool SPLIT = S::kSplit;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t* const sq = smem;                                   // [tile][part]
-    uint8_t* const sk = sq + S::kQBytes;                        // [2 stages]
-    uint8_t* const sv = sk + 2 * S::kTileBytes;                 // [2 stages]
-    float2* const scales = reinterpret_cast<float2*>(sv + 2 * S::kTileBytes);  // [ring][group]: key scale, log2 of the value scale
+    constexpr int NQ = S::kQBufs;
+    uint8_t* const sq = smem;                                   // [buffers][tile][part]
+    uint8_t* const sk = sq + NQ * S::kQBytes;                   // [stages]
+    uint8_t* const sv = sk + NS * S::kTileBytes;                // [stages]
+    float2* const scales = reinterpret_cast<float2*>(sv + NS * S::kTileBytes);  // [ring][group]: key scale, log2 of the value scale
     unsigned* const valid = reinterpret_cast<unsigned*>(scales + kPreScaleRing * G);  // [ring][2]
-    float* const qscale = reinterpret_cast<float*>(valid + kPreScaleRing * 2);         // [rows] score factor of each row
-    unsigned* const prefix = reinterpret_cast<unsigned*>(qscale + kPreRows);           // [n_seqs + 1]
-    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], pv_done[2], q_full, q_seen,
+    float* const qscale = reinterpret_cast<float*>(valid + kPreScaleRing * 2);         // [buffers][rows] score factor of each row
+    unsigned* const prefix = reinterpret_cast<unsigned*>(qscale + NQ * kPreRows);      // [n_seqs + 1]
+    __shared__ __align__(8) uint64_t k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full[4], p_ready[4], pv_done[2], q_full[NQ], q_seen[NQ],
         sc_full[kPreScaleRing], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
@@ -164,13 +169,15 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
 
     if (tid == 0) {
         unset = 0;
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 4), mbar_init(&v_full[i], 4);
-            mbar_init(&k_empty[i], 1), mbar_init(&v_empty[i], 1);
-            mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4), mbar_init(&pv_done[i], 1);
+            mbar_init(&k_empty[i], 2), mbar_init(&v_empty[i], 2);  // both MMA warps
         }
+        for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4);  // [tile][buffer]
+        mbar_init(&pv_done[0], 1), mbar_init(&pv_done[1], 1);
         for (int i = 0; i < kPreScaleRing; ++i) mbar_init(&sc_full[i], 1);
-        mbar_init(&q_full, 4), mbar_init(&q_seen, 8), mbar_init(&drained, 1);
+        for (int i = 0; i < NQ; ++i) mbar_init(&q_full[i], 4), mbar_init(&q_seen[i], 10);  // the softmax and MMA warps
+        mbar_init(&drained, 2);
         fence_mbar_init();
     }
     griddep_launch();
@@ -306,9 +313,16 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         // ---- operands to f16 ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsOperand));
         const int cw = warp - 8;
-        uint4 kc[4], vc[4];
-        int id[4];
-        auto token_of = [&](int k) {  // of this thread's k-th 16 codes
+        constexpr int CH = NT * D / 16 / 128;  // 16-code chunks per thread, for K and for V
+        // What a step needs from memory; two of them, so that a step's loads have
+        // two steps' time.
+        struct Codes {
+            uint4 k[CH], v[CH];
+            float ks, vs;  // scales of 16-token group `lane`, in the first warp
+            bool there;
+        };
+        int id[CH], group_id = -1;
+        auto token_of = [&](int k) {  // of this thread's k-th chunk
             const int i = k * 4 + cw;
             return (D == 64 ? i : i >> 1) * 8 + (lane & 7);
         };
@@ -316,38 +330,35 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         auto load_ids = [&](const PreCursor& u) {
             const int32_t* row = a.table + (int64_t)u.s * a.table_stride;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < CH; ++k) {
                 const int t = u.step * NT + token_of(k);
                 id[k] = t < u.seen ? row[t >> sh] : -1;
             }
+            if (cw == 0 && lane < G) {
+                const int t = u.step * NT + lane * 16;
+                group_id = t < u.seen ? row[t >> sh] : -1;
+            }
         };
-        float my_ks = 0.0f, my_lv = -120.0f;  // scales of 16-token group `lane`, by the first warp
-        bool my_ok = false;
-        auto load_codes = [&](const PreCursor& u, const uint8_t* codes, uint4 (&w)[4]) {
+        auto load_codes = [&](const PreCursor& u, Codes& w) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < CH; ++k) {
                 const int t = u.step * NT + token_of(k);
-                w[k] = make_uint4(0, 0, 0, 0);  // tokens that nobody sees stay zero: there may be NaN codes
-                if ((unsigned)id[k] < (unsigned)c.n_pages)
-                    w[k] = __ldg(reinterpret_cast<const uint4*>(
-                        codes + ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16));
+                w.k[k] = w.v[k] = make_uint4(0, 0, 0, 0);  // tokens that nobody sees stay zero: there may be NaN codes
+                if ((unsigned)id[k] < (unsigned)c.n_pages) {
+                    const int64_t at = ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16;
+                    w.k[k] = __ldg(reinterpret_cast<const uint4*>(c.k + at));
+                    w.v[k] = __ldg(reinterpret_cast<const uint4*>(c.v + at));
+                }
+            }
+            if (cw == 0 && lane < G) {
+                w.there = (unsigned)group_id < (unsigned)c.n_pages;
+                w.ks = w.there ? c.k_scale[(int64_t)group_id * c.n_kv + u.head] : 0.0f;
+                w.vs = w.there ? c.v_scale[(int64_t)group_id * c.n_kv + u.head] : 0.0f;
             }
         };
-        auto load_scales = [&](const PreCursor& u) {
-            if (cw != 0 || lane >= G) return;
-            const int t = u.step * NT + lane * 16;
-            const int page = t < u.seen ? a.table[(int64_t)u.s * a.table_stride + (t >> sh)] : -1;
-            my_ok = (unsigned)page < (unsigned)c.n_pages;
-            my_ks = 0.0f, my_lv = -120.0f;
-            if (my_ok) {
-                my_ks = c.k_scale[(int64_t)page * c.n_kv + u.head];
-                const float v = c.v_scale[(int64_t)page * c.n_kv + u.head];
-                my_lv = v < 1e-36f ? -120.0f : log2f(v);  // NaN stays
-            }
-        };
-        auto put = [&](uint8_t* tile, const uint4 (&w)[4]) {
+        auto put = [&](uint8_t* tile, const uint4 (&w)[CH]) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < CH; ++k) {
                 uint32_t f[8];
                 codes_f16<FMT>(w[k].x, f[0], f[1]);
                 codes_f16<FMT>(w[k].y, f[2], f[3]);
@@ -376,48 +387,41 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 for (int o = 0; o < D * (int)sizeof(T); o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"((const uint8_t*)q + o));
             }
         };
-        auto put_queries = [&](const PreCursor& u) {
+        auto put_queries = [&](const PreCursor& u, int buf) {
             const int rows = tiles_of(u) * 128;
+            constexpr int V = 16 / sizeof(T), N = D / 2 / V;  // elements of 16 bytes, loads of half a row
 #pragma unroll 1
-            for (int r = cw * 32 + lane; r < rows; r += 128) {  // a thread per row
+            for (int r = cw * 16 + (lane >> 1); r < rows; r += 64) {  // two neighbouring threads per row
+                const int e0 = (lane & 1) * (D / 2);
                 const T* q = query(u, r);
-                auto load = [&](int o, float (&v)[8]) {  // elements 8 o ..
-                    constexpr int V = 16 / sizeof(T);
-                    if (!q) {
+                uint4 w[N];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-                    } else if (q16) {
+                for (int b = 0; b < N; ++b) {
+                    w[b] = make_uint4(0, 0, 0, 0);
+                    if (q && q16) {
+                        w[b] = __ldg(reinterpret_cast<const uint4*>(q + e0 + b * V));
+                    } else if (q) {
+                        T* e = reinterpret_cast<T*>(&w[b]);
 #pragma unroll
-                        for (int b = 0; b < 8 / V; ++b) {
-                            const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + o * 8 + b * V));
-                            const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-                            for (int i = 0; i < V; ++i) v[b * V + i] = (float)e[i];
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = (float)q[o * 8 + e];
+                        for (int i = 0; i < V; ++i) e[i] = q[e0 + b * V + i];
                     }
-                };
-                float top = 0.0f;
-#pragma unroll 4
-                for (int o = 0; o < D / 8; ++o) {
-                    float v[8];
-                    load(o, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
                 }
+                const T* e = reinterpret_cast<const T*>(w);
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 2; ++i) top = fmaxf(top, fabsf((float)e[i]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 int ex = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
                 ex = max(-126, min(126, ex));
                 const float up = pow2f(ex);
-                qscale[r] = a.scale * 1.4426950408889634f * pow2f(-ex);
-                const uint32_t at = smem_u32(sq) + (r >> 7) * (SPLIT ? 2 : 1) * S::kQPart + ((r & 127) >> 3) * (D * 16) + (r & 7) * 16;
-#pragma unroll 4
-                for (int o = 0; o < D / 8; ++o) {  // the second reading comes from L1
-                    float v[8];
-                    load(o, v);
+                if (e0 == 0) qscale[buf * kPreRows + r] = a.scale * 1.4426950408889634f * pow2f(-ex);
+                const uint32_t at = smem_u32(sq) + buf * S::kQBytes + (r >> 7) * (SPLIT ? 2 : 1) * S::kQPart +
+                                    ((r & 127) >> 3) * (D * 16) + (r & 7) * 16 + (e0 >> 3) * 128;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= up;
+                for (int o = 0; o < D / 16; ++o) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = (float)e[o * 8 + i] * up;
                     uint4 h, l;
                     split_octet(v, h, l);
                     sts128(at + o * 128, h);
@@ -427,44 +431,51 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             fence_async_shared();
             __syncwarp();
         };
+        // `nx` is the next step to load, its pages' numbers under way; `cur` the
+        // one whose tiles are written.
         PreCursor nx = cur;
-        unsigned ahead = lo;
-        auto advance = [&]() {
+        unsigned ahead = lo, x = lo;
+        auto load_next = [&](Codes& w) {
+            if (ahead >= hi) return;
+            load_codes(nx, w);
             ++ahead;
             if (++nx.step == nx.steps) {
                 ahead += kPreUnitCost;
                 if (ahead < hi) next_unit(nx);
             }
+            if (ahead < hi) load_ids(nx);
         };
-        if (ahead < hi) {
-            load_ids(nx);
-            load_scales(nx);
-            load_codes(nx, c.k, kc);
-            load_codes(nx, c.v, vc);
-        }
-        int units = 0;
-        // The next step's loads are under way while this one's tiles are written.
-        for (int i = 0; ahead < hi && ok; ++i) {
-            if (i == 0 || nx.step == 0) {
-                // The previous unit's scores are all computed, its score factors read.
-                if (i > 0) ok = wait(&k_empty[(i - 1) & 1], ((i - 1) >> 1) & 1) && wait(&q_seen, (units - 1) & 1);
-                if (!ok) break;
-                put_queries(nx);
-                if (lane == 0) mbar_arrive(&q_full);
+        Codes even, odd;
+        even.ks = even.vs = odd.ks = odd.vs = 0.0f;
+        even.there = odd.there = false;
+        if (x < hi) load_ids(nx);
+        load_next(even);
+        load_next(odd);
+        int i = 0, units = 0, last_step[2] = {0, 0};
+        auto step = [&](Codes& w) {
+            if (i == 0 || cur.step == 0) {
+                // The buffer's last unit: its scores are all computed (where a later
+                // tile has not waited for that already), its factors read.
+                const int buf = units % NQ, l = buf ? last_step[1] : last_step[0];
+                if (units >= NQ) {
+                    if (l >= i - NS) ok = wait(&k_empty[l % NS], (l / NS) & 1);
+                    ok = ok && wait(&q_seen[buf], (units / NQ - 1) & 1);
+                }
+                if (!ok) return;
+                put_queries(cur, buf);
+                if (lane == 0) mbar_arrive(&q_full[buf]);
+                (buf ? last_step[1] : last_step[0]) = i + min(cur.steps - cur.step, (int)(hi - x)) - 1;
                 ++units;
-                if (ahead + (nx.steps - nx.step) + kPreUnitCost < hi) prefetch_queries(nx);
+                if (x + (cur.steps - cur.step) + kPreUnitCost < hi) prefetch_queries(cur);
             }
-            advance();
-            const bool more = ahead < hi;
-            if (more) load_ids(nx);
-            const int st = i & 1, use = i >> 1;
+            const int st = i % NS, use = i / NS;
             if (use > 0) ok = wait(&k_empty[st], (use - 1) & 1);
-            if (!ok) break;
-            put(sk + st * S::kTileBytes, kc);
+            if (!ok) return;
+            put(sk + st * S::kTileBytes, w.k);
             if (cw == 0) {
                 const int ring = i % kPreScaleRing;
-                if (lane < G) scales[ring * G + lane] = make_float2(my_ks, my_lv);
-                const unsigned m = __ballot_sync(0xffffffffu, lane < G && my_ok);
+                if (lane < G) scales[ring * G + lane] = make_float2(w.ks, w.vs < 1e-36f ? -120.0f : log2f(w.vs));  // NaN stays
+                const unsigned m = __ballot_sync(0xffffffffu, lane < G && w.there);
                 if (lane == 0) valid[ring * 2] = m;
             }
             fence_async_shared();
@@ -473,93 +484,100 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 mbar_arrive(&k_full[st]);
                 if (cw == 0) mbar_arrive(&sc_full[i % kPreScaleRing]);
             }
-            if (more) {
-                load_codes(nx, c.k, kc);
-                load_scales(nx);
-            }
             if (use > 0) ok = wait(&v_empty[st], (use - 1) & 1);
-            if (!ok) break;
-            put(sv + st * S::kTileBytes, vc);
+            if (!ok) return;
+            put(sv + st * S::kTileBytes, w.v);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[st]);
-            if (more) load_codes(nx, c.v, vc);
+            load_next(w);
+            ++i;
+            ++x;
+            if (++cur.step == cur.steps) {
+                x += kPreUnitCost;
+                if (x < hi) next_unit(cur);
+            }
+        };
+        while (x < hi && ok) {
+            step(even);
+            if (x < hi && ok) step(odd);
         }
     } else if (warp >= 12) {
-        // ---- MMAs: one thread of a warp that stays together ----
+        // ---- MMAs: a warp per row tile, one thread of it issues ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsMma));
-        if (warp == 12) {
+        if (warp < 14) {
+            const int tile = warp - 12;
             constexpr uint32_t id_qk = tc_idesc_f16_f32(128, NT);
             constexpr uint32_t id_pv = tc_idesc_f16_f32(128, D) | (1u << 16);  // B (values) with the head's elements contiguous
-            auto qk = [&](int tile, int st) {
-                const uint32_t d = tmem + tile * NT;
-                const uint64_t kd = tc_desc_kmajor(smem_u32(sk + st * S::kTileBytes), 128, D * 16);
-                if (elect_one()) {
-#pragma unroll
-                for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
-                    const uint64_t qd = tc_desc_kmajor(smem_u32(sq + (tile * (SPLIT ? 2 : 1) + part) * S::kQPart), 128, D * 16);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) tc_mma_f16(d, qd + k * 16, kd + k * 16, id_qk, part + k > 0);
-                }
-                tc_commit(&s_full[tile]);
-                }
-                __syncwarp();
-            };
-            auto pv = [&](int tile, int st, bool first) {
-                const uint32_t d = tmem + S::kOCol + tile * D, p = tmem + tile * NT;
-                // 8-token groups D * 16 bytes apart, 8-element groups 128 bytes
-                const uint64_t vd = tc_desc_kmajor(smem_u32(sv + st * S::kTileBytes), D * 16, 128);
-                if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < NT / 16; ++k) {
-                    const uint32_t ac = p + (k >> 1) * 32 + (k & 1) * 8;
-                    tc_mma_f16_ta(d, ac, vd + k * (2 * D), id_pv, !first || k > 0);
-                    if (SPLIT) tc_mma_f16_ta(d, ac + 16, vd + k * (2 * D), id_pv, 1);
-                }
-                tc_commit(&pv_done[tile]);
-                }
-                __syncwarp();
-            };
-            // One commit after the products of both tiles.
-            auto release = [&](uint64_t* bar) {
-                if (elect_one()) tc_commit(bar);
-                __syncwarp();
-            };
-            int i = 0;                  // steps, over all units
-            int np[2] = {0, 0};         // weights taken from each tile, over all units
-            int units = 0;
+            constexpr int PARTS = SPLIT ? 2 : 1;
+            const uint64_t qd0 = tc_desc_kmajor(smem_u32(sq + tile * PARTS * S::kQPart), 128, D * 16);
+            uint64_t qd = qd0;
+            const uint64_t kd0 = tc_desc_kmajor(smem_u32(sk), 128, D * 16);
+            // Values: 8-token groups D * 16 bytes apart, 8-element groups 128 bytes.
+            const uint64_t vd0 = tc_desc_kmajor(smem_u32(sv), D * 16, 128);
+            const uint32_t sbuf = tmem + tile * 2 * NT, obuf = tmem + S::kOCol + tile * D;
+            int i0 = 0, np = 0, units = 0;  // steps before this unit, those of this tile, units
             for (unsigned x = lo; x < hi && ok;) {
                 const int n = min(cur.steps - cur.step, (int)(hi - x));
-                const int tiles = tiles_of(cur);
-                ok = wait(&q_full, units++ & 1) && wait(&k_full[i & 1], (i >> 1) & 1);
-                for (int tl = 0; tl < tiles && ok; ++tl) {
-                    if (np[tl] > 0) ok = wait(&pv_done[tl], (np[tl] - 1) & 1);  // the weights of the unit before are read
+                const bool live = tile < tiles_of(cur);
+                // Scores of step k: its buffer's weights, two steps back, have been read.
+                auto scores = [&](int k) {
+                    const int st = (i0 + k) % NS;
+                    ok = wait(&k_full[st], ((i0 + k) / NS) & 1);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t d = sbuf + ((np + k) & 1) * NT;
+                    const uint64_t kd = kd0 + st * (S::kTileBytes / 16);
+                    if (elect_one()) {
+                        if (live) {
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                                for (int e = 0; e < D / 16; ++e)
+                                    tc_mma_f16(d, qd + part * (S::kQPart / 16) + e * 16, kd + e * 16, id_qk, part + e > 0);
+                            tc_commit(&s_full[tile * 2 + ((np + k) & 1)]);
+                            tc_commit(&k_empty[st]);
+                        } else {
+                            mbar_arrive(&k_empty[st]);
+                        }
+                    }
+                    __syncwarp();
+                };
+                const int buf = units % NQ;
+                ok = wait(&q_full[buf], (units++ / NQ) & 1);
+                if (ok && lane == 0) mbar_arrive(&q_seen[buf]);
+                __syncwarp();
+                qd = qd0 + buf * (S::kQBytes / 16);
+                for (int k = 0; k < 2 && k < n && ok; ++k) scores(k);
+                for (int k = 0; k < n && ok; ++k) {
+                    const int st = (i0 + k) % NS, b = np + k;
+                    ok = wait(&v_full[st], ((i0 + k) / NS) & 1);
+                    if (ok && live) ok = wait(&p_ready[tile * 2 + (b & 1)], (b >> 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    qk(tl, i & 1);
-                }
-                if (!ok) break;
-                release(&k_empty[i & 1]);
-                for (int k = 0; k < n && ok; ++k, ++i) {
-                    const bool more = k + 1 < n;
-                    ok = wait(&v_full[i & 1], (i >> 1) & 1);
-                    for (int tl = 0; tl < tiles && ok; ++tl) {
-                        ok = wait(&p_ready[tl], np[tl] & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        pv(tl, i & 1, k % S::kFlush == 0);
-                        if (tl == tiles - 1) release(&v_empty[i & 1]);
-                        if (more) {
-                            // The next scores overwrite the weights that these products read.
-                            ok = wait(&pv_done[tl], np[tl] & 1) && wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            qk(tl, (i + 1) & 1);
-                            if (tl == tiles - 1) release(&k_empty[(i + 1) & 1]);
+                    const uint32_t p = sbuf + (b & 1) * NT;
+                    const uint64_t vd = vd0 + st * (S::kTileBytes / 16);
+                    const uint32_t more = k % S::kFlush != 0;
+                    if (elect_one()) {
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < NT / 16; ++e) {
+                                const uint32_t ac = p + (e >> 1) * 32 + (e & 1) * 8;
+                                tc_mma_f16_ta(obuf, ac, vd + e * (2 * D), id_pv, e > 0 ? 1 : more);
+                                if (SPLIT) tc_mma_f16_ta(obuf, ac + 16, vd + e * (2 * D), id_pv, 1);
+                            }
+                            tc_commit(&pv_done[tile]);
+                            tc_commit(&v_empty[st]);
+                        } else {
+                            mbar_arrive(&v_empty[st]);
                         }
-                        ++np[tl];
                     }
+                    __syncwarp();
+                    if (live) ok = wait(&pv_done[tile], b & 1);
+                    if (ok && k + 2 < n) scores(k + 2);
                 }
+                if (live) np += n;
+                i0 += n;
                 x += n;
                 cur.step += n;
                 if (cur.step == cur.steps) {
@@ -574,7 +592,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsSoftmax));
         const int tile = warp >> 2, r = tid & 127;  // row of the tile, its TMEM lane
         const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4)
-        const uint32_t ts = tmem + lane_base + tile * NT, to = tmem + lane_base + S::kOCol + tile * D;
+        const uint32_t to = tmem + lane_base + S::kOCol + tile * D;
         const uint32_t tsum = tmem + lane_base + S::kSumCol + tile * D;
         int i = 0, np = 0, units = 0;
         const bool o16 = ((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) % 16 == 0;
@@ -588,11 +606,12 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             // The tile's first row sees least: below that nothing is masked.
             const int seen_min = cur.chunk * kPreRows + tile * 128 + 127 < cur.q.nq * group
                                      ? seen_of(cur.q, cur.chunk * kPreRows + tile * 128) : 0;
-            ok = wait(&q_full, units++ & 1);
+            const int buf = units % NQ;
+            ok = wait(&q_full[buf], (units++ / NQ) & 1);
             if (!ok) break;
-            const float qf = qscale[tile * 128 + r];
+            const float qf = qscale[buf * kPreRows + tile * 128 + r];
             __syncwarp();
-            if (lane == 0) mbar_arrive(&q_seen);
+            if (lane == 0) mbar_arrive(&q_seen[buf]);
             const int unit_row = tile * 128 + r;
             const int side = cur.step == 0 ? 1 : 0;  // the piece begins its unit, or goes on with it
             float* piece = pieces + ((size_t)blockIdx.x * 2 + side) * S::kPieceFloats;
@@ -637,7 +656,8 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             float m = -INFINITY, l = 0.0f, vl = -120.0f;  // vl: log2 of the reference value scale
             for (int k = 0; k < n && ok && part_of_it; ++k, ++np) {
                 const int ring = (i + k) % kPreScaleRing;
-                ok = wait(&sc_full[ring], ((i + k) / kPreScaleRing) & 1) && wait(&s_full[tile], np & 1);
+                const uint32_t ts = tmem + lane_base + tile * 2 * NT + (np & 1) * NT;
+                ok = wait(&sc_full[ring], ((i + k) / kPreScaleRing) & 1) && wait(&s_full[tile * 2 + (np & 1)], (np >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const int t0 = (cur.step + k) * NT;
@@ -645,19 +665,25 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const bool whole = t0 + NT <= seen_min && groups == (1u << G) - 1u;
                 const float2* sc = scales + ring * G;
                 const bool anew = k % S::kFlush == 0;  // these products begin O anew
-                if (anew && k > 0) flush();
+                // O is touched when the products before have been added to it.
+                auto settled = [&]() {
+                    ok = wait(&pv_done[tile], (np - 1) & 1);
+                    tc_fence_after();
+                    return ok;
+                };
+                if (anew && k > 0) {
+                    if (!settled()) break;
+                    flush();
+                }
                 // Largest score, group by group: the scale is applied to a group's maximum.
                 float top = -INFINITY, lvmax = -120.0f;
                 uint32_t w[2][32];
                 auto largest = [&](auto masked) {
                     tmem_ld32(ts, w[0]);
-#pragma unroll 1
-                    for (int c2 = 0; c2 < NT / 32; c2 += 2)
 #pragma unroll
-                    for (int c1 = 0; c1 < 2; ++c1) {
-                        const int ch = c2 + c1;
-                        tmem_wait_ld32(w[c1]);
-                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[c1 ^ 1]);
+                    for (int ch = 0; ch < NT / 32; ++ch) {
+                        tmem_wait_ld32(w[ch]);
+                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[ch + 1]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float2 g2 = sc[ch * 2 + h];
@@ -665,7 +691,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
-                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[c1][h * 16 + e]) : -INFINITY);
+                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[ch][h * 16 + e]) : -INFINITY);
                             const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                             top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
                             lvmax = fmaxf(lvmax, g2.y);
@@ -689,6 +715,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     }
                     since *= f;
                     if (!anew) {
+                        if (!settled()) break;
 #pragma unroll 1
                         for (int ch = 0; ch < D / 32; ++ch) {
                             tmem_ld32(to + ch * 32, w[0]);
@@ -702,13 +729,10 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
                 auto weigh = [&](auto masked) {
                     tmem_ld32(ts, w[0]);
-#pragma unroll 1
-                    for (int c2 = 0; c2 < NT / 32; c2 += 2)
 #pragma unroll
-                    for (int c1 = 0; c1 < 2; ++c1) {
-                        const int ch = c2 + c1;
-                        tmem_wait_ld32(w[c1]);
-                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[c1 ^ 1]);
+                    for (int ch = 0; ch < NT / 32; ++ch) {
+                        tmem_wait_ld32(w[ch]);
+                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[ch + 1]);
                         uint32_t ph[16], pl[16];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -722,7 +746,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                                 float p[2];
 #pragma unroll
                                 for (int u = 0; u < 2; ++u) {
-                                    const float xx = __fmaf_rn(__uint_as_float(w[c1][h * 16 + 2 * e + u]), cf, b);
+                                    const float xx = __fmaf_rn(__uint_as_float(w[ch][h * 16 + 2 * e + u]), cf, b);
                                     p[u] = ex2(!masked || 2 * e + u < left ? xx : -INFINITY);
                                     part[u] += p[u];
                                 }
@@ -741,7 +765,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_ready[tile]);
+                if (lane == 0) mbar_arrive(&p_ready[tile * 2 + (np & 1)]);
             }
             i += n;
             if (ok && part_of_it) {
@@ -869,7 +893,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     }
     // Everyone meets when all products and their arrivals are done, also where
     // a wait has given up.
-    if (warp == 12) {
+    if (warp == 12 || warp == 13) {
         if (elect_one()) tc_commit(&drained);
         mbar_wait_bounded(&drained, 0, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
         if (unset) atomicCAS(err, 0, kDevTimeoutDrain);
