@@ -85,6 +85,9 @@ struct lc_context {
     size_t gemm_scratch_bytes = 0;
     bool gemm_ready = false;        // shared-memory attribute of the GEMM kernel set
     void* kv8_ws = nullptr;         // workspace of lc_kv8_attention, one size for all calls
+    lc_rope_config rope_cfg;        // the last lc_rope_apply's configuration and its frequencies
+    RopeTurns rope_turns;
+    float rope_mult = 0.0f;         // 0: none yet
 };
 
 extern "C" int lc_device_count(int* count) {
@@ -698,7 +701,6 @@ extern "C" void lc_rope_config_llama32(lc_rope_config* o) {
 
 // Turns per position of every rotated pair in fp64, and the factor on cos and sin.
 static int rope_turns(const lc_rope_config* g, RopeTurns* out, float* mult) {
-    if (!g) return fail(LC_ERR_INVALID_ARG, "config is NULL");
     if (g->head_dim <= 0 || g->head_dim > 2 * kRopeMaxPairs || g->rot_dim < 0 || g->rot_dim > g->head_dim ||
         (g->rot_dim & 1))
         return fail(LC_ERR_INVALID_ARG, "head_dim=%d rot_dim=%d (rot_dim even, 0..head_dim <= %d)", g->head_dim,
@@ -761,10 +763,17 @@ extern "C" int lc_rope_apply(lc_context* c, const lc_rope_config* cfg, const voi
                              int32_t rows, int32_t num_heads, int64_t x_stride, int64_t y_stride, int32_t dtype,
                              int32_t transpose) {
     return on_device(c, [&]() -> int {
-        RopeTurns turns;
         RopeApply a;
         memset(&a, 0, sizeof(a));
-        if (int rc = rope_turns(cfg, &turns, &a.mult)) return rc;
+        if (!cfg) return fail(LC_ERR_INVALID_ARG, "config is NULL");
+        if (c->rope_mult == 0.0f || memcmp(&c->rope_cfg, cfg, sizeof(*cfg)) != 0) {
+            c->rope_mult = 0.0f;
+            float mult = 0.0f;
+            if (int rc = rope_turns(cfg, &c->rope_turns, &mult)) return rc;
+            c->rope_cfg = *cfg;
+            c->rope_mult = mult;
+        }
+        a.mult = c->rope_mult;
         const int elem = row_elem(dtype);
         if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
         const int64_t width = (int64_t)num_heads * cfg->head_dim;
@@ -788,7 +797,7 @@ extern "C" int lc_rope_apply(lc_context* c, const lc_rope_config* cfg, const voi
         a.sign = transpose ? -1.0f : 1.0f;
         a.half = cfg->layout == LC_ROPE_HALF;
         a.dtype = dtype;
-        return s.finish(launch_rope_apply(a, turns, c->sms, c->stream));
+        return s.finish(launch_rope_apply(a, c->rope_turns, c->sms, c->stream));
     });
 }
 

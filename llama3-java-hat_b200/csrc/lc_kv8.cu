@@ -15,21 +15,115 @@ namespace lc {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendWindow = 32;  // rows whose slots one CTA looks at
+constexpr int kAppendWindow = 32;  // rows whose slots one CTA looks at, at most
+constexpr int kAppendHold = 16;    // groups of four that a lane keeps
+
+// Four elements as they lie in memory.
+template <typename T>
+struct Raw;
+template <>
+struct Raw<float> {
+    float4 w;
+    LC_DEV void load(const float* p, bool aligned) { w = aligned ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(p[0], p[1], p[2], p[3]); }
+    LC_DEV float4 get() const { return w; }
+    LC_DEV void zero() { w = make_float4(0, 0, 0, 0); }
+};
+template <>
+struct Raw<__half> {
+    uint2 w;
+    LC_DEV void load(const __half* p, bool aligned) {
+        if (aligned) {
+            w = __ldg(reinterpret_cast<const uint2*>(p));
+        } else {
+            const __half2 a = __halves2half2(p[0], p[1]), b = __halves2half2(p[2], p[3]);
+            w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        }
+    }
+    LC_DEV float4 get() const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    LC_DEV void zero() { w = make_uint2(0, 0); }
+};
+template <typename T>
+LC_DEV float4 load4(const T* p, bool aligned) {
+    Raw<T> r;
+    r.load(p, aligned);
+    return r.get();
+}
 
 template <typename T>
-LC_DEV float row_value(const T* p) { return (float)*p; }
+LC_DEV void store4(T* p, float4 v, bool aligned);
 template <>
-LC_DEV float row_value<__half>(const __half* p) { return __half2float(*p); }
+LC_DEV void store4<float>(float* p, float4 v, bool aligned) {
+    if (aligned) *reinterpret_cast<float4*>(p) = v;
+    else p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
+}
+template <>
+LC_DEV void store4<__half>(__half* p, float4 v, bool aligned) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    if (aligned) *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    else p[0] = __low2half(a), p[1] = __high2half(a), p[2] = __low2half(b), p[3] = __high2half(b);
+}
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Rows r) {
+// Largest finite size of four values, over `top`: NaN and infinities do not set the scale.
+LC_DEV float top4(float4 v, float top) {
+    const float f[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (f[i] < INFINITY) top = fmaxf(top, f[i]);
+    return top;
+}
+
+// Four codes under scale s, inv = 1 / s rounded; byte i is value i.
+template <int FMT>
+LC_DEV uint32_t encode4(float4 v, float s, float inv) {
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    uint32_t w = 0;
+    bool sure = true;
+    if (FMT == kKv8I8) {
+        // y + 1.5 * 2^23 rounds y to a whole number, which stands in the sum's low
+        // bits.  |y| <= 127 is off by 2^-16 at most; within 2^-14 of a tie, or not
+        // finite, it is not sure.
+        uint32_t t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y = x[i] * inv, m = y + 12582912.0f;
+            t[i] = __float_as_uint(m);
+            sure = sure && fabsf(y - (m - 12582912.0f)) < 0.5f - 0x1p-14f;
+        }
+        w = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+    } else {
+        // A tie of a normal e4m3 value is 0x80000 in the low 20 bits of y; within
+        // four units of that, below the normal range, or not finite, it is not sure.
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = x[i] * inv;
+            const uint32_t b = __float_as_uint(y[i]);
+            sure = sure && ((b - (0x80000u - 4u)) & 0xfffffu) > 8u && ((b & 0x7fffffffu) >= 0x3c800000u || x[i] == 0.0f) &&
+                   (b & 0x7f800000u) != 0x7f800000u;
+        }
+        w = e4m3x2(y[0], y[1]) | (e4m3x2(y[2], y[3]) << 16);
+    }
+    if (!sure || !(inv < INFINITY) || !(s > 0.0f)) {
+        w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= kv8_encode<FMT>(x[i], s) << (8 * i);
+    }
+    return w;
+}
+
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Rows r, int window) {
+    constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows at a time
     griddep_launch();
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sh = c.page_shift, page = 1 << sh, d = c.head_dim;
+    const int sh = c.page_shift, page = 1 << sh;
     const int64_t n_slots = (int64_t)c.n_pages << sh;
-    const int row0 = blockIdx.x * kAppendWindow;
+    const int row0 = blockIdx.x * window;
+    const bool aligned = (((uintptr_t)r.k | (uintptr_t)r.v | (uintptr_t)(r.row_stride * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
     // Lane i: is row row0 + i the first of its page's rows?  Rows without a
     // slot are passed over.
     const int my = row0 + lane;
@@ -39,7 +133,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
     };
     int slot = -1;
     bool starts = false;
-    if (my < r.rows) {
+    if (lane < window && my < r.rows) {
         slot = slot_of(my);
         if (slot >= 0) {
             int i = my - 1, prev = -1;
@@ -48,16 +142,17 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
         }
     }
     unsigned starters = __ballot_sync(0xffffffffu, starts);
-    int n = 0;  // unit number within the CTA
+    const int sub = lane / LPR, e0 = (lane % LPR) * 4;  // this lane's row of those at a time, and its elements
+    int n = 0;                                          // unit number within the CTA
     while (starters) {
         const int l = __ffs(starters) - 1;
         starters &= starters - 1;
         const int pg = __shfl_sync(0xffffffffu, slot, l) >> sh;
-        for (int u = 0; u < 2 * c.n_kv; ++u, ++n) {
+        for (int u = blockIdx.y; u < 2 * c.n_kv; u += gridDim.y, ++n) {
             if (n % (kAppendThreads / 32) != warp) continue;
             const int head = u >> 1;
-            const T* rows = (const T*)((u & 1) ? r.v : r.k) + head * d;
-            uint8_t* codes = ((u & 1) ? c.v : c.k) + ((((int64_t)pg * c.n_kv + head) << sh) * d);
+            const T* rows = (const T*)((u & 1) ? r.v : r.k) + head * D + e0;
+            uint8_t* codes = ((u & 1) ? c.v : c.k) + ((((int64_t)pg * c.n_kv + head) << sh) * D) + e0;
             float* scale = ((u & 1) ? c.v_scale : c.k_scale) + (int64_t)pg * c.n_kv + head;
             float held = *scale;
             // The page's runs, one after the other: usually there is one.
@@ -80,18 +175,47 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
                     }
                 }
                 const T* x = rows + (int64_t)row * r.row_stride;
+                const bool keep = len <= kAppendHold * RPI;
+                Raw<T> v[kAppendHold];
                 float top = 0.0f;
-                for (int i = lane; i < len * d; i += 32) {
-                    const float v = fabsf(row_value(x + (int64_t)(i / d) * r.row_stride + i % d));
-                    if (v < INFINITY) top = fmaxf(top, v);  // NaN and infinities do not set the scale
+                if (keep) {
+#pragma unroll
+                    for (int i = 0; i < kAppendHold; ++i) {
+                        const int k = i * RPI + sub;
+                        if (k < len) v[i].load(x + (int64_t)k * r.row_stride, aligned);
+                        else v[i].zero();
+                    }
+#pragma unroll
+                    for (int i = 0; i < kAppendHold; ++i) top = top4(v[i].get(), top);
+                } else {
+#pragma unroll 8
+                    for (int k = sub; k < len; k += RPI) top = top4(load4(x + (int64_t)k * r.row_stride, aligned), top);
                 }
                 top = warp_max(top);
                 const float old = off ? held : 0.0f;
                 const float now = fmaxf(old, __fdiv_rn(top, kv8_limit(FMT)));
+                const float inv = __fdiv_rn(1.0f, now);
                 if (now > old)
-                    for (int i = lane; i < off * d; i += 32) codes[i] = (uint8_t)kv8_requant<FMT>(codes[i], old, now);
-                for (int i = lane; i < len * d; i += 32)
-                    codes[off * d + i] = (uint8_t)kv8_encode<FMT>(row_value(x + (int64_t)(i / d) * r.row_stride + i % d), now);
+                    for (int k = sub; k < off; k += RPI) {
+                        uint32_t* at = reinterpret_cast<uint32_t*>(codes + k * D);
+                        const uint32_t w = *at;
+                        uint32_t z = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) z |= kv8_requant<FMT>((w >> (8 * b)) & 0xffu, old, now) << (8 * b);
+                        *at = z;
+                    }
+                if (keep) {
+#pragma unroll
+                    for (int i = 0; i < kAppendHold; ++i) {
+                        const int k = i * RPI + sub;
+                        if (k < len) *reinterpret_cast<uint32_t*>(codes + (off + k) * D) = encode4<FMT>(v[i].get(), now, inv);
+                    }
+                } else {
+#pragma unroll 4
+                    for (int k = sub; k < len; k += RPI)
+                        *reinterpret_cast<uint32_t*>(codes + (off + k) * D) =
+                            encode4<FMT>(load4(x + (int64_t)k * r.row_stride, aligned), now, inv);
+                }
                 held = now;
                 row += len;
                 __syncwarp();  // the next run rounds these codes anew
@@ -101,39 +225,75 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
     }
 }
 
+// Four codes -> values.
+template <int FMT>
+LC_DEV float4 decode4(uint32_t w, float s) {
+    if (FMT == kKv8I8) {
+        w ^= 0x80808080u;  // 0x4b000000 | u is 2^23 + u, u = code + 128
+        const float m = 8388736.0f;
+        return make_float4((__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - m) * s,
+                           (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - m) * s,
+                           (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - m) * s,
+                           (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - m) * s);
+    }
+    uint32_t a, b;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    return make_float4(x.x * s, x.y * s, y.x * s, y.y * s);
+}
+
+// A thread per four elements of a row, of keys and of values; bound by the
+// rows written.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, Kv8Rows r) {
     griddep_launch();
     griddep_wait();
-    const int d = c.head_dim, width = c.n_kv * d, sh = c.page_shift;
+    const int d = c.head_dim, sh = c.page_shift, quads = c.n_kv * d / 4;
     const int64_t n_slots = (int64_t)c.n_pages << sh;
-    for (int row = blockIdx.x; row < r.rows; row += gridDim.x) {
+    const bool aligned = (((uintptr_t)r.k | (uintptr_t)r.v | (uintptr_t)(r.row_stride * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
+    const int per = quads < 256 ? 256 / quads : 1;  // rows of the CTA at a time
+    const int sub = threadIdx.x / quads, q0 = per > 1 ? threadIdx.x - sub * quads : threadIdx.x;
+    if (per > 1 && sub >= per) return;
+    const int lane_rows = per > 1 ? sub : 0;
+    for (int row = blockIdx.x * per + lane_rows; row < r.rows; row += gridDim.x * per) {
         const int slot = r.slots[row];
         if (slot < 0 || slot >= n_slots) continue;
         const int64_t pg = slot >> sh;
         const int off = slot & ((1 << sh) - 1);
-        for (int i = threadIdx.x; i < width; i += blockDim.x) {
-            const int head = i / d, e = i - head * d;
-            const int64_t at = (((pg * c.n_kv + head) << sh) + off) * d + e, st = pg * c.n_kv + head;
-            ((T*)r.k)[(int64_t)row * r.row_stride + i] = (T)(kv8_decode<FMT>(c.k[at]) * c.k_scale[st]);
-            ((T*)r.v)[(int64_t)row * r.row_stride + i] = (T)(kv8_decode<FMT>(c.v[at]) * c.v_scale[st]);
+        for (int q = q0; q < quads; q += 256) {
+            const int head = q * 4 / d, e = q * 4 - head * d;
+            const int64_t st = pg * c.n_kv + head, at = ((st << sh) + off) * d + e;
+            const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(c.k + at)), vw = __ldg(reinterpret_cast<const uint32_t*>(c.v + at));
+            const float ks = __ldg(c.k_scale + st), vs = __ldg(c.v_scale + st);
+            store4((T*)r.k + (int64_t)row * r.row_stride + q * 4, decode4<FMT>(kw, ks), aligned);
+            store4((T*)r.v + (int64_t)row * r.row_stride + q * 4, decode4<FMT>(vw, vs), aligned);
         }
     }
 }
 
 }  // namespace
 
+template <typename T, int FMT>
+static cudaError_t append(const Kv8& c, const Kv8Rows& r, int num_sms, cudaStream_t st) {
+    // A CTA looks at as many rows as leave every SM four CTAs: with 64 rows of
+    // 64 sequences and 32 rows a CTA, two CTAs took 119 us.
+    int window = r.rows / (num_sms * 4);
+    window = window < 1 ? 1 : window > kAppendWindow ? kAppendWindow : window;
+    // With many rows a window holds a page or two, 2 n_kv units each: a warp of
+    // two CTAs then has one of them.
+    const dim3 grid((r.rows + window - 1) / window, window >= 8 && c.n_kv >= 8 ? 2 : 1), block(kAppendThreads);
+    return c.head_dim == 64 ? launch_ex(kv8_append_kernel<T, FMT, 64>, grid, block, 0, st, true, c, r, window)
+                            : launch_ex(kv8_append_kernel<T, FMT, 128>, grid, block, 0, st, true, c, r, window);
+}
+
 cudaError_t launch_kv8_append(const Kv8& c, const Kv8Rows& r, int num_sms, cudaStream_t st) {
-    const dim3 grid((r.rows + kAppendWindow - 1) / kAppendWindow), block(kAppendThreads);
-    if (r.dtype == kRowF32)
-        return c.format == kKv8I8 ? launch_ex(kv8_append_kernel<float, kKv8I8>, grid, block, 0, st, true, c, r)
-                                  : launch_ex(kv8_append_kernel<float, kKv8E4M3>, grid, block, 0, st, true, c, r);
-    return c.format == kKv8I8 ? launch_ex(kv8_append_kernel<__half, kKv8I8>, grid, block, 0, st, true, c, r)
-                              : launch_ex(kv8_append_kernel<__half, kKv8E4M3>, grid, block, 0, st, true, c, r);
+    if (r.dtype == kRowF32) return c.format == kKv8I8 ? append<float, kKv8I8>(c, r, num_sms, st) : append<float, kKv8E4M3>(c, r, num_sms, st);
+    return c.format == kKv8I8 ? append<__half, kKv8I8>(c, r, num_sms, st) : append<__half, kKv8E4M3>(c, r, num_sms, st);
 }
 
 cudaError_t launch_kv8_read(const Kv8& c, const Kv8Rows& r, int num_sms, cudaStream_t st) {
-    const dim3 grid(r.rows < num_sms * 8 ? r.rows : num_sms * 8), block(256);
+    const int quads = c.n_kv * c.head_dim / 4, per = quads < 256 ? 256 / quads : 1, ctas = (r.rows + per - 1) / per;
+    const dim3 grid(ctas < num_sms * 8 ? ctas : num_sms * 8), block(256);
     if (r.dtype == kRowF32)
         return c.format == kKv8I8 ? launch_ex(kv8_read_kernel<float, kKv8I8>, grid, block, 0, st, true, c, r)
                                   : launch_ex(kv8_read_kernel<float, kKv8E4M3>, grid, block, 0, st, true, c, r);

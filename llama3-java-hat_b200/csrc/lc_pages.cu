@@ -39,6 +39,25 @@ LC_DEV int find_owner(const int* prefix, int lo, int hi, int i) {
     return lo;
 }
 
+// The owners of 32 neighbouring places i0 + lane: the first by a search of the
+// whole warp (32 probes a round), the others from the few borders behind it.
+LC_DEV int find_owners(const int* prefix, int n, int i0, int lane, int last) {
+    int lo = 0, hi = n;  // the owner of i0 is in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && prefix[at] <= i0);
+        const int k = 31 - __clz(below);  // lane 0 holds: prefix[lo] <= i0
+        hi = min(hi, lo + (k + 1) * step);
+        lo += k * step;
+    }
+    const int border = lo + 1 + lane <= n ? prefix[lo + 1 + lane] : 0x7fffffff;
+    const unsigned inside = __ballot_sync(0xffffffffu, border <= last);
+    if (inside == 0xffffffffu) return find_owner(prefix, lo, n, min(i0 + lane, last));
+    int s = lo;
+    for (int e = 0; e < __popc(inside); ++e) s += __shfl_sync(0xffffffffu, border, e) <= i0 + lane;
+    return s;
+}
+
 __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) {
     extern __shared__ int sm[];
     int* tok = sm;                       // [n + 1] tokens before sequence s
@@ -153,15 +172,16 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
         const int s = find_owner(give, 0, n, i);
         return p.table[(long long)s * p.table_stride + (i - give[s])];
     };
-    // Tokens.  A table read is a trip to L2 or HBM behind a search in shared
-    // memory, so four tokens of a thread are under way together.
-    for (int i0 = gtid; i0 < tokens; i0 += 4 * gthreads) {
+    // Tokens, 32 neighbours to a warp.  A table read is a trip to L2 or HBM
+    // behind the search in shared memory, so four rounds are under way together.
+    for (int b0 = gtid - lane; b0 < tokens; b0 += 4 * gthreads) {
         int seq[4], pos[4], id[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int i = i0 + k * gthreads;
-            if (i >= tokens) continue;
-            const int s = seq[k] = find_owner(tok, 0, n, i);
+            const int i0 = b0 + k * gthreads;
+            if (i0 >= tokens) continue;  // uniform over the warp
+            const int i = min(i0 + lane, tokens - 1);
+            const int s = seq[k] = find_owners(tok, n, i0, lane, min(i0 + 31, tokens - 1));
             pos[k] = base[s] + i - tok[s];
             const int pg = pos[k] >> sh, first_new = (int)(((long long)base[s] + (1 << sh) - 1) >> sh);
             id[k] = pg < first_new ? p.table[(long long)s * p.table_stride + pg]
@@ -169,7 +189,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int i = i0 + k * gthreads;
+            const int i = b0 + k * gthreads + lane;
             if (i >= tokens) continue;
             p.slots[i] = (id[k] << sh) + (pos[k] & ((1 << sh) - 1));
             p.positions[i] = pos[k];

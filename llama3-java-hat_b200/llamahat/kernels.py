@@ -55,33 +55,66 @@ def _addr(buf, kind: str, min_len: int, writable: bool = False) -> int:
     raise TypeError(f"unsupported buffer type {type(buf)!r}")
 
 
-_ROW_TYPES = {"float32": 0, "float16": 1, "torch.float32": 0, "torch.float16": 1}
+_NP_ROWS = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
+_TORCH_ROWS: dict = {}  # torch dtypes of rows, and of int32 arrays, filled at the first tensor
+_TORCH_I32 = None
+
+
+def _torch_types() -> None:
+    global _TORCH_I32
+    import torch
+    _TORCH_ROWS.update({torch.float32: 0, torch.float16: 1})
+    _TORCH_I32 = torch.int32
+
+
+def _i32(buf, min_len: int, writable: bool = False) -> int:
+    """_addr(buf, "i32", ...) with few steps for a tensor: these calls are short."""
+    if isinstance(buf, np.ndarray):
+        return _addr(buf, "i32", min_len, writable)
+    if _TORCH_I32 is None:
+        _torch_types()
+    if buf.dtype is not _TORCH_I32:
+        raise TypeError(f"expected i32 tensor, got {buf.dtype}")
+    if not buf.is_contiguous():
+        raise ValueError("tensor must be contiguous")
+    if buf.numel() < min_len:
+        raise ValueError(f"tensor holds {buf.numel()} elements, need {min_len}")
+    return buf.data_ptr()
 
 
 def _rows(buf, writable: bool = False):
     """(address, rows, width, row stride in elements, dtype id) of a buffer of
     F32 or F16 rows: [rows, ...] with contiguous rows, any row stride."""
-    dt = _ROW_TYPES.get(str(buf.dtype))
-    if dt is None:
-        raise TypeError(f"expected float32 or float16 rows, got {buf.dtype}")
     shape = buf.shape
     if len(shape) < 2:
         raise ValueError(f"expected [rows, ...], got shape {tuple(shape)}")
     if isinstance(buf, np.ndarray):
+        dt = _NP_ROWS.get(buf.dtype)
         if writable and not buf.flags.writeable:
             raise ValueError("buffer is read-only")
-        strides, addr = [s // buf.itemsize for s in buf.strides], buf.ctypes.data
+        whole, addr = buf.flags.c_contiguous, buf.ctypes.data
     else:
-        strides, addr = buf.stride(), buf.data_ptr()
-    width = 1
-    for n, st in zip(reversed(shape[1:]), reversed(strides[1:])):
-        if st != width and n > 1:
-            raise ValueError("rows must be contiguous")
+        if _TORCH_I32 is None:
+            _torch_types()
+        dt = _TORCH_ROWS.get(buf.dtype)
+        whole, addr = buf.is_contiguous(), buf.data_ptr()
+    if dt is None:
+        raise TypeError(f"expected float32 or float16 rows, got {buf.dtype}")
+    rows, width = shape[0], 1
+    for n in shape[1:]:
         width *= n
-    stride = strides[0] if shape[0] > 1 else width
+    if whole:
+        return addr, rows, width, width, dt
+    strides = [s // buf.itemsize for s in buf.strides] if isinstance(buf, np.ndarray) else buf.stride()
+    inner = 1
+    for n, st in zip(reversed(shape[1:]), reversed(strides[1:])):
+        if st != inner and n > 1:
+            raise ValueError("rows must be contiguous")
+        inner *= n
+    stride = strides[0] if rows > 1 else width
     if stride < 0 or (writable and stride < width):
         raise ValueError(f"row stride {stride} of rows of {width}")
-    return addr, shape[0], width, stride, dt
+    return addr, rows, width, stride, dt
 
 
 class Accelerator:
@@ -294,7 +327,7 @@ class CudaRoPE(_CudaKernel, IRoPE):
                 raise ValueError("x and out differ in shape or type")
         if width == 0 or width % config.head_dim:
             raise ValueError(f"rows of {width} elements, head_dim {config.head_dim}")
-        _lib.check(self.lib.lc_rope_apply(self.ctx, config.lc, xa, ya, _addr(positions, "i32", rows), rows,
+        _lib.check(self.lib.lc_rope_apply(self.ctx, config.lc, xa, ya, _i32(positions, rows), rows,
                                           width // config.head_dim, xs, ys, dt, int(transpose)))
 
 
@@ -309,11 +342,11 @@ class CudaPages(_CudaKernel):
         n, stride = table.shape
         cap = slots.shape[0]
         _lib.check(self.lib.lc_pages_step(
-            self.ctx, _addr(lens, "i32", n), _addr(n_new, "i32", n), n, page_size, _addr(table, "i32", n * stride, True),
-            stride, _addr(free_list, "i32", 1, True), _addr(free_count, "i32", 1), free_list.shape[0], cap,
-            _addr(lens_out, "i32", n, True), _addr(q_start, "i32", n + 1, True), _addr(slots, "i32", cap, True),
-            _addr(positions, "i32", cap, True), _addr(seq_ids, "i32", cap, True),
-            _addr(free_count_out, "i32", 1, True), _addr(status, "i32", 2, True)))
+            self.ctx, _i32(lens, n), _i32(n_new, n), n, page_size, _i32(table, n * stride, True),
+            stride, _i32(free_list, 1, True), _i32(free_count, 1), free_list.shape[0], cap,
+            _i32(lens_out, n, True), _i32(q_start, n + 1, True), _i32(slots, cap, True),
+            _i32(positions, cap, True), _i32(seq_ids, cap, True),
+            _i32(free_count_out, 1, True), _i32(status, 2, True)))
 
 
 class PagedKV8(_CudaKernel):
@@ -351,7 +384,7 @@ class PagedKV8(_CudaKernel):
             raise ValueError("k and v rows differ in shape, stride or type")
         if width != self.n_kv_heads * self.head_dim:
             raise ValueError(f"rows of {width} elements, the cache holds {self.n_kv_heads} x {self.head_dim}")
-        return ka, va, stride, dt, _addr(slots, "i32", rows), rows
+        return ka, va, stride, dt, _i32(slots, rows), rows
 
     def append(self, k, v, slots) -> None:
         """Rows [rows, n_kv_heads, head_dim] (F32 or F16) into their slots (see lc_kv8_append)."""
@@ -374,8 +407,8 @@ class PagedKV8(_CudaKernel):
             raise ValueError(f"rows of {width} elements, head_dim {d}")
         n, stride = table.shape
         _lib.check(self.lib.lc_kv8_attention(
-            self.ctx, self._kv, qa, oa, qs, os_, dt, rows, None if q_start is None else _addr(q_start, "i32", n + 1),
-            _addr(kv_lens, "i32", n), _addr(table, "i32", n * stride), stride, n, max_q, width // d,
+            self.ctx, self._kv, qa, oa, qs, os_, dt, rows, None if q_start is None else _i32(q_start, n + 1),
+            _i32(kv_lens, n), _i32(table, n * stride), stride, n, max_q, width // d,
             d ** -0.5 if scale is None else scale))
 
 
