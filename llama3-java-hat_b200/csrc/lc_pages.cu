@@ -39,17 +39,9 @@ LC_DEV int find_owner(const int* prefix, int lo, int hi, int i) {
     return lo;
 }
 
-// The owners of 32 neighbouring places i0 + lane: the first by a search of the
-// whole warp (32 probes a round), the others from the few borders behind it.
-LC_DEV int find_owners(const int* prefix, int n, int i0, int lane, int last) {
-    int lo = 0, hi = n;  // the owner of i0 is in [lo, hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
-        const unsigned below = __ballot_sync(0xffffffffu, at < hi && prefix[at] <= i0);
-        const int k = 31 - __clz(below);  // lane 0 holds: prefix[lo] <= i0
-        hi = min(hi, lo + (k + 1) * step);
-        lo += k * step;
-    }
+// The owners of 32 neighbouring places i0 + lane (up to `last`), given that
+// `lo` owns i0 or a place before it: by counting the few borders in between.
+LC_DEV int find_owners(const int* prefix, int lo, int n, int i0, int lane, int last) {
     const int border = lo + 1 + lane <= n ? prefix[lo + 1 + lane] : 0x7fffffff;
     const unsigned inside = __ballot_sync(0xffffffffu, border <= last);
     if (inside == 0xffffffffu) return find_owner(prefix, lo, n, min(i0 + lane, last));
@@ -166,31 +158,41 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
     if (code != kPagesOk) return;
 
     const int held = count + (int)total[2], left = held - (int)total[1];
-    auto stack = [&](int i) {  // entry i of the free stack after the pushes
-        if (i < count) return p.free_list[i];
+    auto stack = [&](int i) -> const int32_t* {  // where entry i of the free stack after the pushes lies
+        if (i < count) return p.free_list + i;
         i -= count;
         const int s = find_owner(give, 0, n, i);
-        return p.table[(long long)s * p.table_stride + (i - give[s])];
+        return p.table + (long long)s * p.table_stride + (i - give[s]);
     };
-    // Tokens, 32 neighbours to a warp.  A table read is a trip to L2 or HBM
-    // behind the search in shared memory, so four rounds are under way together.
-    for (int b0 = gtid - lane; b0 < tokens; b0 += 4 * gthreads) {
+    // Tokens: a range of neighbours per warp, 32 at a time, so that an owner is
+    // searched once and followed from there (searched for every token, the
+    // instructions of that took 30 us of 42 at 177,000 tokens).  Table reads
+    // are trips to L2 or HBM: four rounds are under way together.
+    const int warps = gthreads >> 5, span = ((tokens + warps - 1) / warps + 31) & ~31;
+    const int begin = (gtid >> 5) * span, end = min(tokens, begin + span);
+    int owner = begin < end ? find_owner(tok, 0, n, begin) : 0;
+    for (int b0 = begin; b0 < end; b0 += 128) {
         int seq[4], pos[4], id[4];
+        const int32_t* at[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int i0 = b0 + k * gthreads;
-            if (i0 >= tokens) continue;  // uniform over the warp
-            const int i = min(i0 + lane, tokens - 1);
-            const int s = seq[k] = find_owners(tok, n, i0, lane, min(i0 + 31, tokens - 1));
+            const int i0 = b0 + k * 32;
+            at[k] = p.status;  // any place to read, where there is no token
+            if (i0 >= end) continue;  // uniform over the warp
+            const int i = min(i0 + lane, end - 1);
+            const int s = seq[k] = find_owners(tok, owner, n, i0, lane, min(i0 + 31, end - 1));
+            owner = __shfl_sync(0xffffffffu, s, 31);
             pos[k] = base[s] + i - tok[s];
             const int pg = pos[k] >> sh, first_new = (int)(((long long)base[s] + (1 << sh) - 1) >> sh);
-            id[k] = pg < first_new ? p.table[(long long)s * p.table_stride + pg]
+            at[k] = pg < first_new ? p.table + (long long)s * p.table_stride + pg
                                    : stack(held - 1 - (take[s] + pg - first_new));
         }
 #pragma unroll
+        for (int k = 0; k < 4; ++k) id[k] = *at[k];
+#pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int i = b0 + k * gthreads + lane;
-            if (i >= tokens) continue;
+            const int i = b0 + k * 32 + lane;
+            if (i >= end) continue;
             p.slots[i] = (id[k] << sh) + (pos[k] & ((1 << sh) - 1));
             p.positions[i] = pos[k];
             p.seq_ids[i] = seq[k];
@@ -200,9 +202,9 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
     for (int a = gtid; a < (int)total[1]; a += gthreads) {
         const int s = find_owner(take, 0, n, a);
         const int first_new = (int)(((long long)base[s] + (1 << sh) - 1) >> sh);
-        p.table[(long long)s * p.table_stride + first_new + a - take[s]] = stack(held - 1 - a);
+        p.table[(long long)s * p.table_stride + first_new + a - take[s]] = *stack(held - 1 - a);
     }
-    for (int i = count + gtid; i < left; i += gthreads) p.free_list[i] = stack(i);
+    for (int i = count + gtid; i < left; i += gthreads) p.free_list[i] = *stack(i);
 }
 
 }  // namespace
