@@ -13,7 +13,7 @@
 // The work is a few dependent reads; latency bounds it.  One cluster (not
 // more, so that a cluster barrier can separate all reads of lens and
 // free_count from the writes of lens_out and free_count_out, which may be the
-// same buffers) of 1 to 8 CTAs.
+// same buffers) of 1 to 16 CTAs.
 #include "lc_internal.h"
 #include "lc_paged.h"
 
@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
     int* take = tok + p.n_seqs + 1;      // [n + 1] pages taken before s
     int* give = take + p.n_seqs + 1;     // [n + 1] pages returned before s
     int* base = give + p.n_seqs + 1;     // [n] lens
+    int* top = base + p.n_seqs;          // [n] stack entry of page 0, had it been taken: page pg lies at top - pg
     __shared__ long long warp_sum3[3][32];
     __shared__ unsigned long long bad;
     griddep_launch();
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
             if (s >= n) continue;
             base[s] = len[k];
             const int before = (int)(((long long)len[k] + (1 << sh) - 1) >> sh);
+            top[s] = (int)(count + total[2]) - 1 - ((int)sum[1] - before);
             if (add[k] < 0) sum[2] += before;
             else sum[0] += add[k], sum[1] += (int)(((long long)len[k] + add[k] + (1 << sh) - 1) >> sh) - before;
         }
@@ -183,9 +185,9 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
             const int s = seq[k] = find_owners(tok, owner, n, i0, lane, min(i0 + 31, end - 1));
             owner = __shfl_sync(0xffffffffu, s, 31);
             pos[k] = base[s] + i - tok[s];
-            const int pg = pos[k] >> sh, first_new = (int)(((long long)base[s] + (1 << sh) - 1) >> sh);
+            const int pg = pos[k] >> sh, first_new = (int)(((unsigned)base[s] + (1u << sh) - 1) >> sh);
             at[k] = pg < first_new ? p.table + (long long)s * p.table_stride + pg
-                                   : stack(held - 1 - (take[s] + pg - first_new));
+                                   : stack(top[s] - pg);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) id[k] = *at[k];
@@ -210,16 +212,21 @@ __global__ void __launch_bounds__(kPagesThreads) pages_step_kernel(PagesStep p) 
 }  // namespace
 
 cudaError_t launch_pages_step(const PagesStep& p, cudaStream_t st) {
-    const int smem = (4 * p.n_seqs + 3) * (int)sizeof(int);
+    const int smem = (5 * p.n_seqs + 3) * (int)sizeof(int);
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(pages_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (4 * kPagesMaxSeqs + 3) * (int)sizeof(int));
+                                                   (5 * kPagesMaxSeqs + 3) * (int)sizeof(int));
         if (e != cudaSuccess) return e;
     }
     // One CTA handles 1024 tokens at a time; more CTAs only where there is a
-    // second round of them.
+    // second round of them.  A cluster of 16 is not portable to every device,
+    // but to the one this library is built for.
     int ctas = 1;
-    while (ctas < 8 && ctas * 2 * kPagesThreads <= p.capacity) ctas *= 2;
+    while (ctas < 16 && ctas * 2 * kPagesThreads <= p.capacity) ctas *= 2;
+    if (ctas > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(pages_step_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kPagesThreads);
