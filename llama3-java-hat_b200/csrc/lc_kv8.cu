@@ -27,6 +27,11 @@ struct Raw<float> {
     LC_DEV void load(const float* p, bool aligned) { w = aligned ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(p[0], p[1], p[2], p[3]); }
     LC_DEV float4 get() const { return w; }
     LC_DEV void zero() { w = make_float4(0, 0, 0, 0); }
+    // Running largest size; a NaN never is.
+    typedef float Top;
+    static LC_DEV Top none() { return 0.0f; }
+    LC_DEV Top top(Top t) const { return fmaxf(fmaxf(fmaxf(t, fabsf(w.x)), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))); }
+    static LC_DEV float value(Top t) { return t; }
 };
 template <>
 struct Raw<__half> {
@@ -44,6 +49,12 @@ struct Raw<__half> {
         return make_float4(a.x, a.y, b.x, b.y);
     }
     LC_DEV void zero() { w = make_uint2(0, 0); }
+    typedef __half2 Top;
+    static LC_DEV Top none() { return __half2half2(__ushort_as_half(0)); }
+    LC_DEV Top top(Top t) const {
+        return __hmax2(t, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&w.x)), __habs2(*reinterpret_cast<const __half2*>(&w.y))));
+    }
+    static LC_DEV float value(Top t) { return fmaxf(__low2float(t), __high2float(t)); }
 };
 template <typename T>
 LC_DEV float4 load4(const T* p, bool aligned) {
@@ -66,7 +77,7 @@ LC_DEV void store4<__half>(__half* p, float4 v, bool aligned) {
     else p[0] = __low2half(a), p[1] = __high2half(a), p[2] = __low2half(b), p[3] = __high2half(b);
 }
 
-// Largest finite size of four values, over `top`: NaN and infinities do not set the scale.
+// Largest finite size of four values, over `top`.
 LC_DEV float top4(float4 v, float top) {
     const float f[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
 #pragma unroll
@@ -82,15 +93,15 @@ LC_DEV uint32_t encode4(float4 v, float s, float inv) {
     uint32_t w = 0;
     bool sure = true;
     if (FMT == kKv8I8) {
-        // y + 1.5 * 2^23 rounds y to a whole number, which stands in the sum's low
-        // bits.  |y| <= 127 is off by 2^-16 at most; within 2^-14 of a tie, or not
-        // finite, it is not sure.
+        // x inv + 1.5 * 2^23 rounds to a whole number, which stands in the sum's low
+        // bits.  A quotient of at most 127 is off by 2^-16 at most; what is left
+        // within 2^-14 of a half, or not finite, is not sure.
         uint32_t t[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float y = x[i] * inv, m = y + 12582912.0f;
+            const float m = __fmaf_rn(x[i], inv, 12582912.0f);
             t[i] = __float_as_uint(m);
-            sure = sure && fabsf(y - (m - 12582912.0f)) < 0.5f - 0x1p-14f;
+            sure = sure && fabsf(__fmaf_rn(x[i], inv, 12582912.0f - m)) < 0.5f - 0x1p-14f;
         }
         w = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
     } else {
@@ -100,10 +111,11 @@ LC_DEV uint32_t encode4(float4 v, float s, float inv) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             y[i] = x[i] * inv;
-            const uint32_t b = __float_as_uint(y[i]);
-            sure = sure && ((b - (0x80000u - 4u)) & 0xfffffu) > 8u && ((b & 0x7fffffffu) >= 0x3c800000u || x[i] == 0.0f) &&
-                   (b & 0x7f800000u) != 0x7f800000u;
+            sure = sure && ((__float_as_uint(y[i]) - (0x80000u - 4u)) & 0xfffffu) > 8u;
         }
+        const float low = fminf(fminf(fabsf(y[0]), fabsf(y[1])), fminf(fabsf(y[2]), fabsf(y[3])));
+        const float sum = fabsf(y[0]) + fabsf(y[1]) + fabsf(y[2]) + fabsf(y[3]);  // carries a NaN or an infinity
+        sure = sure && low >= 0x1p-6f && sum < 2048.0f;
         w = e4m3x2(y[0], y[1]) | (e4m3x2(y[2], y[3]) << 16);
     }
     if (!sure || !(inv < INFINITY) || !(s > 0.0f)) {
@@ -115,7 +127,7 @@ LC_DEV uint32_t encode4(float4 v, float s, float inv) {
 }
 
 template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Rows r, int window) {
+__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_append_kernel(Kv8 c, Kv8Rows r, int window) {
     constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows at a time
     griddep_launch();
     griddep_wait();
@@ -164,8 +176,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
                 }
                 if ((first >> sh) != pg) break;
                 const int off = first & (page - 1);
-                int len = 1;  // rows row .. row + len - 1, at most to the page's end
-                for (;; len += 32) {
+                // Rows row .. row + len - 1, at most to the page's end; those of this
+                // window are in the lanes' `slot`.
+                int len = 1;
+                if (row < row0 + window) {
+                    const int k = my - row;
+                    const unsigned m = __ballot_sync(0xffffffffu, k < 0 || (lane < window && off + k < page && slot == first + k));
+                    len = (m == 0xffffffffu ? 32 : __ffs(~m) - 1) - (row - row0);
+                }
+                for (; row + len >= row0 + window && off + len < page; len += 32) {
                     const int k = len + lane;
                     const bool ok = off + k < page && row + k < r.rows && r.slots[row + k] == first + k;
                     const unsigned m = __ballot_sync(0xffffffffu, ok);
@@ -177,7 +196,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
                 const T* x = rows + (int64_t)row * r.row_stride;
                 const bool keep = len <= kAppendHold * RPI;
                 Raw<T> v[kAppendHold];
-                float top = 0.0f;
+                typename Raw<T>::Top most = Raw<T>::none();
                 if (keep) {
 #pragma unroll
                     for (int i = 0; i < kAppendHold; ++i) {
@@ -186,12 +205,21 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, Kv8Ro
                         else v[i].zero();
                     }
 #pragma unroll
-                    for (int i = 0; i < kAppendHold; ++i) top = top4(v[i].get(), top);
+                    for (int i = 0; i < kAppendHold; ++i) most = v[i].top(most);
                 } else {
 #pragma unroll 8
-                    for (int k = sub; k < len; k += RPI) top = top4(load4(x + (int64_t)k * r.row_stride, aligned), top);
+                    for (int k = sub; k < len; k += RPI) {
+                        Raw<T> w;
+                        w.load(x + (int64_t)k * r.row_stride, aligned);
+                        most = w.top(most);
+                    }
                 }
-                top = warp_max(top);
+                float top = warp_max(Raw<T>::value(most));
+                if (top == INFINITY) {  // infinities do not set the scale
+                    top = 0.0f;
+                    for (int k = sub; k < len; k += RPI) top = top4(load4(x + (int64_t)k * r.row_stride, aligned), top);
+                    top = warp_max(top);
+                }
                 const float old = off ? held : 0.0f;
                 const float now = fmaxf(old, __fdiv_rn(top, kv8_limit(FMT)));
                 const float inv = __fdiv_rn(1.0f, now);
@@ -242,31 +270,48 @@ LC_DEV float4 decode4(uint32_t w, float s) {
     return make_float4(x.x * s, x.y * s, y.x * s, y.y * s);
 }
 
-// A thread per four elements of a row, of keys and of values; bound by the
-// rows written.
+// A thread per eight elements of a row, of keys and of values, two rows under
+// way together; bound by the rows written.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, Kv8Rows r) {
     griddep_launch();
     griddep_wait();
-    const int d = c.head_dim, sh = c.page_shift, quads = c.n_kv * d / 4;
+    const int d = c.head_dim, sh = c.page_shift, octs = c.n_kv * d / 8;
     const int64_t n_slots = (int64_t)c.n_pages << sh;
     const bool aligned = (((uintptr_t)r.k | (uintptr_t)r.v | (uintptr_t)(r.row_stride * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
-    const int per = quads < 256 ? 256 / quads : 1;  // rows of the CTA at a time
-    const int sub = threadIdx.x / quads, q0 = per > 1 ? threadIdx.x - sub * quads : threadIdx.x;
+    const int per = octs < 256 ? 256 / octs : 1;  // rows of the CTA at a time
+    const int sub = threadIdx.x / octs, q0 = per > 1 ? threadIdx.x - sub * octs : threadIdx.x;
     if (per > 1 && sub >= per) return;
-    const int lane_rows = per > 1 ? sub : 0;
-    for (int row = blockIdx.x * per + lane_rows; row < r.rows; row += gridDim.x * per) {
-        const int slot = r.slots[row];
-        if (slot < 0 || slot >= n_slots) continue;
-        const int64_t pg = slot >> sh;
-        const int off = slot & ((1 << sh) - 1);
-        for (int q = q0; q < quads; q += 256) {
-            const int head = q * 4 / d, e = q * 4 - head * d;
-            const int64_t st = pg * c.n_kv + head, at = ((st << sh) + off) * d + e;
-            const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(c.k + at)), vw = __ldg(reinterpret_cast<const uint32_t*>(c.v + at));
-            const float ks = __ldg(c.k_scale + st), vs = __ldg(c.v_scale + st);
-            store4((T*)r.k + (int64_t)row * r.row_stride + q * 4, decode4<FMT>(kw, ks), aligned);
-            store4((T*)r.v + (int64_t)row * r.row_stride + q * 4, decode4<FMT>(vw, vs), aligned);
+    const int64_t step = (int64_t)gridDim.x * per;
+    for (int64_t row = blockIdx.x * per + (per > 1 ? sub : 0); row < r.rows; row += 2 * step) {
+        int slot[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            slot[b] = row + b * step < r.rows ? r.slots[row + b * step] : -1;
+            if (slot[b] >= n_slots) slot[b] = -1;
+        }
+        for (int q = q0; q < octs; q += 256) {
+            const int head = q * 8 / d, e = q * 8 - head * d;
+            uint2 kw[2], vw[2];
+            float ks[2], vs[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (slot[b] < 0) continue;
+                const int64_t st = (int64_t)(slot[b] >> sh) * c.n_kv + head;
+                const int64_t at = ((st << sh) + (slot[b] & ((1 << sh) - 1))) * d + e;
+                kw[b] = __ldg(reinterpret_cast<const uint2*>(c.k + at)), vw[b] = __ldg(reinterpret_cast<const uint2*>(c.v + at));
+                ks[b] = __ldg(c.k_scale + st), vs[b] = __ldg(c.v_scale + st);
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (slot[b] < 0) continue;  // rows without a slot are left as they are
+                T* k = (T*)r.k + (row + b * step) * r.row_stride + q * 8;
+                T* v = (T*)r.v + (row + b * step) * r.row_stride + q * 8;
+                store4(k, decode4<FMT>(kw[b].x, ks[b]), aligned);
+                store4(k + 4, decode4<FMT>(kw[b].y, ks[b]), aligned);
+                store4(v, decode4<FMT>(vw[b].x, vs[b]), aligned);
+                store4(v + 4, decode4<FMT>(vw[b].y, vs[b]), aligned);
+            }
         }
     }
 }
@@ -292,7 +337,7 @@ cudaError_t launch_kv8_append(const Kv8& c, const Kv8Rows& r, int num_sms, cudaS
 }
 
 cudaError_t launch_kv8_read(const Kv8& c, const Kv8Rows& r, int num_sms, cudaStream_t st) {
-    const int quads = c.n_kv * c.head_dim / 4, per = quads < 256 ? 256 / quads : 1, ctas = (r.rows + per - 1) / per;
+    const int octs = c.n_kv * c.head_dim / 8, per = octs < 256 ? 256 / octs : 1, ctas = (r.rows + per - 1) / per;
     const dim3 grid(ctas < num_sms * 8 ? ctas : num_sms * 8), block(256);
     if (r.dtype == kRowF32)
         return c.format == kKv8I8 ? launch_ex(kv8_read_kernel<float, kKv8I8>, grid, block, 0, st, true, c, r)
