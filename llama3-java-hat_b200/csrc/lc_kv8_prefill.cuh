@@ -116,6 +116,11 @@ LC_DEV void tmem_wait_ld32(uint32_t (&v)[32]) {
                  :
                  : "memory");
 }
+LC_DEV void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 LC_DEV void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -133,6 +138,28 @@ LC_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+// Two fp32 values in one register pair, and the instructions that take them.
+LC_DEV uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+LC_DEV float2 unpair(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+LC_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+LC_DEV uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+
 LC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A unit of the line and the step within it.
@@ -562,9 +589,9 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                         if (live) {
 #pragma unroll
                             for (int e = 0; e < NT / 16; ++e) {
-                                const uint32_t ac = p + (e >> 1) * 32 + (e & 1) * 8;
+                                const uint32_t ac = p + e * 16;
                                 tc_mma_f16_ta(obuf, ac, vd + e * (2 * D), id_pv, e > 0 ? 1 : more);
-                                if (SPLIT) tc_mma_f16_ta(obuf, ac + 16, vd + e * (2 * D), id_pv, 1);
+                                if (SPLIT) tc_mma_f16_ta(obuf, ac + 8, vd + e * (2 * D), id_pv, 1);
                             }
                             tc_commit(&pv_done[tile]);
                             tc_commit(&v_empty[st]);
@@ -675,27 +702,29 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     if (!settled()) break;
                     flush();
                 }
-                // Largest score, group by group: the scale is applied to a group's maximum.
+                // Largest score, group by group: the scale is applied to a group's
+                // maximum.  The loops over groups stay loops: unrolled, their code is
+                // larger than the schedulers' instruction caches.
                 float top = -INFINITY, lvmax = -120.0f;
-                uint32_t w[2][32];
                 auto largest = [&](auto masked) {
-                    tmem_ld32(ts, w[0]);
+                    uint32_t w[16];
+                    tmem_ld16(ts, w);
+#pragma unroll 1
+                    for (int gr = 0; gr < G; ++gr) {
+                        uint32_t z[16];
+                        const float2 g2 = sc[gr];
+                        tmem_wait_ld(w);
 #pragma unroll
-                    for (int ch = 0; ch < NT / 32; ++ch) {
-                        tmem_wait_ld32(w[ch]);
-                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[ch + 1]);
+                        for (int e = 0; e < 16; ++e) z[e] = w[e];
+                        if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w);
+                        const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float2 g2 = sc[ch * 2 + h];
-                            const int left = masked ? (groups >> (ch * 2 + h) & 1 ? seen - t0 - ch * 32 - h * 16 : 0) : 16;
-                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[ch][h * 16 + e]) : -INFINITY);
-                            const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                            top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
-                            lvmax = fmaxf(lvmax, g2.y);
-                        }
+                        for (int e = 0; e < 16; ++e)
+                            mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(z[e]) : -INFINITY);
+                        const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
+                        lvmax = fmaxf(lvmax, g2.y);
                     }
                 };
                 if (whole) largest(std::false_type());
@@ -717,47 +746,52 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     if (!anew) {
                         if (!settled()) break;
 #pragma unroll 1
-                        for (int ch = 0; ch < D / 32; ++ch) {
-                            tmem_ld32(to + ch * 32, w[0]);
-                            tmem_wait_ld32(w[0]);
+                        for (int ch = 0; ch < D / 16; ++ch) {
+                            uint32_t z[16];
+                            tmem_ld16(to + ch * 16, z);
+                            tmem_wait_ld(z);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) w[0][e] = __float_as_uint(__uint_as_float(w[0][e]) * f);
-                            tmem_st32(to + ch * 32, w[0]);
+                            for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * f);
+                            tmem_st16(to + ch * 16, z);
                         }
                     }
                 }
                 const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
                 auto weigh = [&](auto masked) {
-                    tmem_ld32(ts, w[0]);
+                    uint32_t w[16];
+                    tmem_ld16(ts, w);
+#pragma unroll 1
+                    for (int gr = 0; gr < G; ++gr) {
+                        uint32_t z[16], ph[8], pl[8];
+                        const float2 g2 = sc[gr];
+                        tmem_wait_ld(w);
 #pragma unroll
-                    for (int ch = 0; ch < NT / 32; ++ch) {
-                        tmem_wait_ld32(w[ch]);
-                        if (ch + 1 < NT / 32) tmem_ld32(ts + (ch + 1) * 32, w[ch + 1]);
-                        uint32_t ph[16], pl[16];
+                        for (int e = 0; e < 16; ++e) z[e] = w[e];
+                        if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w);
+                        const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
+                        const float cf = g2.x * qf, b = bias + lr, out = ex2(-lr);
+                        const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
+                        const uint64_t cf2 = pair(cf, cf), b2 = pair(b, b);
+                        uint64_t part = 0;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float2 g2 = sc[ch * 2 + h];
-                            const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
-                            const float cf = g2.x * qf, b = bias + lr, out = ex2(-lr);
-                            const int left = masked ? (groups >> (ch * 2 + h) & 1 ? seen - t0 - ch * 32 - h * 16 : 0) : 16;
-                            float part[2] = {0.0f, 0.0f};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                float p[2];
-#pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                    const float xx = __fmaf_rn(__uint_as_float(w[ch][h * 16 + 2 * e + u]), cf, b);
-                                    p[u] = ex2(!masked || 2 * e + u < left ? xx : -INFINITY);
-                                    part[u] += p[u];
-                                }
-                                if (SPLIT) split_f16(p[0], p[1], ph[h * 8 + e], pl[h * 8 + e]);
-                                else ph[h * 8 + e] = pack_f16(p[0], p[1]);
+                        for (int e = 0; e < 8; ++e) {
+                            const float2 xx = unpair(fma2(pair(__uint_as_float(z[2 * e]), __uint_as_float(z[2 * e + 1])), cf2, b2));
+                            const float p0 = ex2(!masked || 2 * e < left ? xx.x : -INFINITY);
+                            const float p1 = ex2(!masked || 2 * e + 1 < left ? xx.y : -INFINITY);
+                            const uint64_t p = pair(p0, p1);
+                            part = add2(part, p);
+                            const __half2 hh = __floats2half2_rn(p0, p1);
+                            ph[e] = *reinterpret_cast<const uint32_t*>(&hh);
+                            if (SPLIT) {
+                                const float2 f = __half22float2(hh), r = unpair(add2(p, pair(-f.x, -f.y)));
+                                pl[e] = pack_f16(r.x, r.y);
                             }
-                            l = __fmaf_rn(part[0] + part[1], out, l);
                         }
-                        // Over the 32 columns just read: hi of 32 tokens, then lo.
-                        tmem_st16(ts + ch * 32, ph);
-                        if (SPLIT) tmem_st16(ts + ch * 32 + 16, pl);
+                        const float2 s2 = unpair(part);
+                        l = __fmaf_rn(s2.x + s2.y, out, l);
+                        // Over the 16 columns of these tokens: hi, then lo.
+                        tmem_st8(ts + gr * 16, ph);
+                        if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
                     }
                 };
                 if (whole) weigh(std::false_type());
