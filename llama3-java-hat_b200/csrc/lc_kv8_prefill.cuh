@@ -472,14 +472,15 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             }
             if (ahead < hi) load_ids(nx);
         };
-        Codes even, odd;
-        even.ks = even.vs = odd.ks = odd.vs = 0.0f;
-        even.there = odd.there = false;
+        Codes w, behind;
+        w.ks = w.vs = behind.ks = behind.vs = 0.0f;
+        w.there = behind.there = false;
         if (x < hi) load_ids(nx);
-        load_next(even);
-        load_next(odd);
+        load_next(w);
+        load_next(behind);
         int i = 0, units = 0, last_step[2] = {0, 0};
-        auto step = [&](Codes& w) {
+#pragma unroll 1
+        while (x < hi && ok) {
             if (i == 0 || cur.step == 0) {
                 // The buffer's last unit: its scores are all computed (where a later
                 // tile has not waited for that already), its factors read.
@@ -488,7 +489,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     if (l >= i - NS) ok = wait(&k_empty[l % NS], (l / NS) & 1);
                     ok = ok && wait(&q_seen[buf], (units / NQ - 1) & 1);
                 }
-                if (!ok) return;
+                if (!ok) break;
                 put_queries(cur, buf);
                 if (lane == 0) mbar_arrive(&q_full[buf]);
                 (buf ? last_step[1] : last_step[0]) = i + min(cur.steps - cur.step, (int)(hi - x)) - 1;
@@ -497,7 +498,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             }
             const int st = i % NS, use = i / NS;
             if (use > 0) ok = wait(&k_empty[st], (use - 1) & 1);
-            if (!ok) return;
+            if (!ok) break;
             put(sk + st * S::kTileBytes, w.k);
             if (cw == 0) {
                 const int ring = i % kPreScaleRing;
@@ -512,22 +513,19 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 if (cw == 0) mbar_arrive(&sc_full[i % kPreScaleRing]);
             }
             if (use > 0) ok = wait(&v_empty[st], (use - 1) & 1);
-            if (!ok) return;
+            if (!ok) break;
             put(sv + st * S::kTileBytes, w.v);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[st]);
-            load_next(w);
+            w = behind;
+            load_next(behind);
             ++i;
             ++x;
             if (++cur.step == cur.steps) {
                 x += kPreUnitCost;
                 if (x < hi) next_unit(cur);
             }
-        };
-        while (x < hi && ok) {
-            step(even);
-            if (x < hi && ok) step(odd);
         }
     } else if (warp >= 12) {
         // ---- MMAs: a warp per row tile, one thread of it issues ----
