@@ -705,25 +705,25 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 // larger than the schedulers' instruction caches.
                 float top = -INFINITY, lvmax = -120.0f;
                 auto largest = [&](auto masked) {
-                    uint32_t w[16];
-                    tmem_ld16(ts, w);
+                    uint32_t w[2][16];
+                    tmem_ld16(ts, w[0]);
 #pragma unroll 1
-                    for (int gr = 0; gr < G; ++gr) {
-                        uint32_t z[16];
-                        const float2 g2 = sc[gr];
-                        tmem_wait_ld(w);
+                    for (int g0 = 0; g0 < G; g0 += 2)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) z[e] = w[e];
-                        if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w);
-                        const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
-                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int b = 0; b < 2; ++b) {
+                            const int gr = g0 + b;
+                            const float2 g2 = sc[gr];
+                            tmem_wait_ld(w[b]);
+                            if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w[b ^ 1]);
+                            const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
+                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(z[e]) : -INFINITY);
-                        const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                        top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
-                        lvmax = fmaxf(lvmax, g2.y);
-                    }
+                            for (int e = 0; e < 16; ++e)
+                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[b][e]) : -INFINITY);
+                            const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                            top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
+                            lvmax = fmaxf(lvmax, g2.y);
+                        }
                 };
                 if (whole) largest(std::false_type());
                 else largest(std::true_type());
@@ -756,41 +756,42 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 }
                 const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
                 auto weigh = [&](auto masked) {
-                    uint32_t w[16];
-                    tmem_ld16(ts, w);
+                    uint32_t w[2][16];
+                    tmem_ld16(ts, w[0]);
 #pragma unroll 1
-                    for (int gr = 0; gr < G; ++gr) {
-                        uint32_t z[16], ph[8], pl[8];
-                        const float2 g2 = sc[gr];
-                        tmem_wait_ld(w);
+                    for (int g0 = 0; g0 < G; g0 += 2)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) z[e] = w[e];
-                        if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w);
-                        const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
-                        const float cf = g2.x * qf, b = bias + lr, out = ex2(-lr);
-                        const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
-                        const uint64_t cf2 = pair(cf, cf), b2 = pair(b, b);
-                        uint64_t part = 0;
+                        for (int b = 0; b < 2; ++b) {
+                            const int gr = g0 + b;
+                            uint32_t ph[8], pl[8];
+                            const float2 g2 = sc[gr];
+                            tmem_wait_ld(w[b]);
+                            if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w[b ^ 1]);
+                            const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
+                            const float cf = g2.x * qf, bb = bias + lr, out = ex2(-lr);
+                            const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
+                            const uint64_t cf2 = pair(cf, cf), b2 = pair(bb, bb);
+                            uint64_t part = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float2 xx = unpair(fma2(pair(__uint_as_float(z[2 * e]), __uint_as_float(z[2 * e + 1])), cf2, b2));
-                            const float p0 = ex2(!masked || 2 * e < left ? xx.x : -INFINITY);
-                            const float p1 = ex2(!masked || 2 * e + 1 < left ? xx.y : -INFINITY);
-                            const uint64_t p = pair(p0, p1);
-                            part = add2(part, p);
-                            const __half2 hh = __floats2half2_rn(p0, p1);
-                            ph[e] = *reinterpret_cast<const uint32_t*>(&hh);
-                            if (SPLIT) {
-                                const float2 f = __half22float2(hh), r = unpair(add2(p, pair(-f.x, -f.y)));
-                                pl[e] = pack_f16(r.x, r.y);
+                            for (int e = 0; e < 8; ++e) {
+                                const float2 xx = unpair(fma2(pair(__uint_as_float(w[b][2 * e]), __uint_as_float(w[b][2 * e + 1])), cf2, b2));
+                                const float p0 = ex2(!masked || 2 * e < left ? xx.x : -INFINITY);
+                                const float p1 = ex2(!masked || 2 * e + 1 < left ? xx.y : -INFINITY);
+                                const uint64_t p = pair(p0, p1);
+                                part = add2(part, p);
+                                const __half2 hh = __floats2half2_rn(p0, p1);
+                                ph[e] = *reinterpret_cast<const uint32_t*>(&hh);
+                                if (SPLIT) {
+                                    const float2 f = __half22float2(hh);
+                                    pl[e] = pack_f16(p0 - f.x, p1 - f.y);
+                                }
                             }
+                            const float2 s2 = unpair(part);
+                            l = __fmaf_rn(s2.x + s2.y, out, l);
+                            // Over the 16 columns of these tokens: hi, then lo.
+                            tmem_st8(ts + gr * 16, ph);
+                            if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
                         }
-                        const float2 s2 = unpair(part);
-                        l = __fmaf_rn(s2.x + s2.y, out, l);
-                        // Over the 16 columns of these tokens: hi, then lo.
-                        tmem_st8(ts + gr * 16, ph);
-                        if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
-                    }
                 };
                 if (whole) weigh(std::false_type());
                 else weigh(std::true_type());
