@@ -331,7 +331,8 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         }
     }
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait_bounded(bar, parity, err, deadline, kDevTimeoutGrid);
+        // Whole warps wait; they go on together, as the tensor-memory instructions ask.
+        return (bool)__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err, deadline, kDevTimeoutGrid));
     };
     auto tiles_of = [&](const PreCursor& u) { return (int64_t)u.q.nq * group - (int64_t)u.chunk * kPreRows > 128 ? 2 : 1; };
     bool ok = true;
@@ -690,7 +691,9 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const bool whole = t0 + NT <= seen_min && groups == (1u << G) - 1u;
                 const float2* sc = scales + ring * G;
                 const bool anew = k % S::kFlush == 0;  // these products begin O anew
-                // O is touched when the products before have been added to it.
+                // The products of the step before are in O.  Waited for in every step,
+                // before its own weights are handed over: a wait knows only the
+                // parity of a phase, so none may be passed over.
                 auto settled = [&]() {
                     ok = wait(&pv_done[tile], (np - 1) & 1);
                     tc_fence_after();
@@ -705,25 +708,25 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 // larger than the schedulers' instruction caches.
                 float top = -INFINITY, lvmax = -120.0f;
                 auto largest = [&](auto masked) {
-                    uint32_t w[2][16];
-                    tmem_ld16(ts, w[0]);
 #pragma unroll 1
-                    for (int g0 = 0; g0 < G; g0 += 2)
+                    for (int g0 = 0; g0 < G; g0 += 2) {
+                        uint32_t w[32];
+                        tmem_ld32(ts + g0 * 16, w);
+                        tmem_wait_ld32(w);
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
                             const int gr = g0 + b;
                             const float2 g2 = sc[gr];
-                            tmem_wait_ld(w[b]);
-                            if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w[b ^ 1]);
                             const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
-                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[b][e]) : -INFINITY);
+                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[b * 16 + e]) : -INFINITY);
                             const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                             top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
                             lvmax = fmaxf(lvmax, g2.y);
                         }
+                    }
                 };
                 if (whole) largest(std::false_type());
                 else largest(std::true_type());
@@ -756,17 +759,16 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 }
                 const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
                 auto weigh = [&](auto masked) {
-                    uint32_t w[2][16];
-                    tmem_ld16(ts, w[0]);
 #pragma unroll 1
-                    for (int g0 = 0; g0 < G; g0 += 2)
+                    for (int g0 = 0; g0 < G; g0 += 2) {
+                        uint32_t w[32];
+                        tmem_ld32(ts + g0 * 16, w);
+                        tmem_wait_ld32(w);
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
                             const int gr = g0 + b;
                             uint32_t ph[8], pl[8];
                             const float2 g2 = sc[gr];
-                            tmem_wait_ld(w[b]);
-                            if (gr + 1 < G) tmem_ld16(ts + (gr + 1) * 16, w[b ^ 1]);
                             const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
                             const float cf = g2.x * qf, bb = bias + lr, out = ex2(-lr);
                             const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
@@ -774,7 +776,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                             uint64_t part = 0;
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
-                                const float2 xx = unpair(fma2(pair(__uint_as_float(w[b][2 * e]), __uint_as_float(w[b][2 * e + 1])), cf2, b2));
+                                const float2 xx = unpair(fma2(pair(__uint_as_float(w[b * 16 + 2 * e]), __uint_as_float(w[b * 16 + 2 * e + 1])), cf2, b2));
                                 const float p0 = ex2(!masked || 2 * e < left ? xx.x : -INFINITY);
                                 const float p1 = ex2(!masked || 2 * e + 1 < left ? xx.y : -INFINITY);
                                 const uint64_t p = pair(p0, p1);
@@ -792,10 +794,12 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                             tmem_st8(ts + gr * 16, ph);
                             if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
                         }
+                    }
                 };
                 if (whole) weigh(std::false_type());
                 else weigh(std::true_type());
                 tmem_wait_st();
+                if (k > 0 && !settled()) break;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[tile * 2 + (np & 1)]);

@@ -465,6 +465,59 @@ def test_attention_chunks(lib, kind, fmt, heads, kv, page, d, lens, counts):
     check_attention(lib, *case, lens, fmt, kind, max(counts))
 
 
+def exact_on_gpu(pool, table, q_start, lens, q, fmt, scale):
+    """Attention in 64 bits with torch, a sequence and kv head at a time; and
+    per row what an error bound needs: max_t sum |q k| scale and sum p |v|."""
+    t = {k: dev(v) for k, v in pool.items()}
+    page, group = pool["k"].shape[2], q.shape[1] // pool["k"].shape[1]
+    values = torch.from_numpy(ref.decode(np.arange(256, dtype=np.uint8), fmt)).cuda()
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    size, weight = (torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda") for _ in range(2))
+    x = dev(q).double()
+    for s, length in enumerate(lens):
+        b, e = int(q_start[s]), int(q_start[s + 1])
+        ids = dev(table[s, : -(-length // page)].astype(np.int64))
+        for h in range(pool["k"].shape[1]):
+            k, v = ((values[t[n][ids, h].long()] * t[n + "_scale"][ids, h].double()[:, None, None]).reshape(-1, q.shape[2])[:length]
+                    for n in "kv")
+            hidden = torch.arange(length, device="cuda")[None] > torch.arange(length - (e - b), length, device="cuda")[:, None]
+            for a in range(h * group, (h + 1) * group):
+                w = torch.softmax((x[b:e, a] @ k.T * scale).masked_fill(hidden, -torch.inf), -1)
+                out[b:e, a] = w @ v
+                size[b:e, a] = (x[b:e, a].abs() @ k.abs().T * scale).masked_fill(hidden, 0).amax(-1)
+                weight[b:e, a] = (w @ v.abs()).amax(-1)
+    return out, size, weight
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("heads,kv,page,d,lens,counts", [
+    (32, 8, 32, 64, [937, 3022, 3377, 3170, 2659], [253, 278, 262, 75, 461]),
+    (8, 2, 64, 128, [1500, 700], [1400, 333]),
+    (24, 8, 16, 64, [2100], [1000]),
+    (8, 8, 128, 64, [5000, 300, 64], [20, 300, 64]),
+])
+def test_attention_prompts_at_length(lib, kind, fmt, heads, kv, page, d, lens, counts):
+    """Many units, each over several CTAs: every row, every time, within its bound."""
+    rng = np.random.default_rng(heads + page)
+    pool, table, q_start, q = attention_case(lib, rng, lens, counts, heads, kv, page, d, fmt, kind, extra_rows=0)
+    want, size, weight = exact_on_gpu(pool, table, q_start, lens, q, fmt, d ** -0.5)
+    # attention_tolerance with the row's own terms; tokens of a row: at most max(lens)
+    rel = 2 * (d + 16) * 2.0 ** -23 * size + (16 + 2 * max(lens)) * 2.0 ** -23 + (2 * HALF["f16"] if kind == "f16" else 0.0)
+    bound = weight * rel + HALF[kind] * weight + TINY[kind]
+    cache, _ = cache_of(lib, pool, fmt)
+    args = dev(q_start), dev(np.array(lens, np.int32)), dev(table)
+    first = None
+    for _ in range(4):
+        out = torch.full(q.shape, 7.0, dtype=dev(q).dtype, device="cuda")
+        cache.attention(dev(q), out, *args, max_q=max(counts))
+        sync()
+        off = (out.double() - want).abs().amax(-1)
+        assert bool((off <= bound).all()), (off / bound).max()
+        first = out if first is None else first
+        assert torch.equal(first, out)
+
+
 @pytest.mark.parametrize("max_q", [1, 2, 9, 1000])
 def test_attention_holds_for_any_max_q(lib, max_q):
     rng = np.random.default_rng(4)
