@@ -891,7 +891,7 @@ extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, 
         if (n_heads <= 0 || n_heads % kv->n_kv_heads)
             return fail(LC_ERR_INVALID_ARG, "n_heads=%d n_kv_heads=%d", n_heads, kv->n_kv_heads);
         const int64_t width = (int64_t)n_heads * kv->head_dim;
-        if (rows < 0 || n_seqs < 0 || n_seqs > kPagesMaxSeqs || table_stride <= 0 || max_q < 1 || q_stride < 0 ||
+        if (rows < 0 || n_seqs < 0 || n_seqs > kPagesMaxSeqs || table_stride <= 0 || max_q < 1 || max_q > (1 << 24) || n_heads > (1 << 16) || q_stride < 0 ||
             (rows > 1 && out_stride < width))
             return fail(LC_ERR_INVALID_ARG, "rows=%d n_seqs=%d (0..%d) table_stride=%d max_q=%d q_stride=%lld out_stride=%lld",
                         rows, n_seqs, kPagesMaxSeqs, table_stride, max_q, (long long)q_stride, (long long)out_stride);
@@ -921,6 +921,9 @@ extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, 
         a.n_heads = n_heads;
         a.dtype = dtype;
         a.scale = scale;
+        if (!kv8_attention_fits(view, a))
+            return fail(LC_ERR_UNSUPPORTED, "rows=%d heads=%d max_q=%d table_stride=%d: more than 2^32 steps of work in one call",
+                        rows, n_heads, max_q, table_stride);
         if (!c->kv8_ws) {
             cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
             CK(cudaStreamIsCapturing(c->stream, &capture), "cudaStreamIsCapturing");

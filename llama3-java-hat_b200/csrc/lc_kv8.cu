@@ -148,8 +148,15 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_ap
     if (lane < window && my < r.rows) {
         slot = slot_of(my);
         if (slot >= 0) {
-            int i = my - 1, prev = -1;
-            while (i >= 0 && (prev = slot_of(i)) < 0) --i;
+            int prev = my > 0 ? slot_of(my - 1) : -1;
+            for (int i = my - 2; prev < 0 && i >= 0; i -= 8) {  // behind skipped rows, eight at a time
+                int v[8];
+#pragma unroll
+                for (int b = 0; b < 8; ++b) v[b] = i - b >= 0 ? slot_of(i - b) : -1;
+#pragma unroll
+                for (int b = 7; b >= 0; --b)
+                    if (v[b] >= 0) prev = v[b];
+            }
             starts = prev < 0 || (prev >> sh) != (slot >> sh);
         }
     }
@@ -170,8 +177,17 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_ap
             // The page's runs, one after the other: usually there is one.
             for (int row = row0 + l; row < r.rows;) {
                 const int first = slot_of(row);
-                if (first < 0) {
-                    ++row;
+                if (first < 0) {  // skipped rows, 128 at a time: a padded batch ends in many
+                    int v[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) v[b] = row + b * 32 + lane < r.rows ? slot_of(row + b * 32 + lane) : -1;
+                    int skip = 128;
+#pragma unroll
+                    for (int b = 3; b >= 0; --b) {
+                        const unsigned m = __ballot_sync(0xffffffffu, v[b] >= 0);
+                        if (m) skip = b * 32 + __ffs(m) - 1;
+                    }
+                    row += skip;
                     continue;
                 }
                 if ((first >> sh) != pg) break;

@@ -44,15 +44,24 @@ cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st) {
     return cudaMemsetAsync((uint8_t*)ws + decode_ws(num_sms), 0, kv8_prefill_counter_bytes(num_sms), st);
 }
 
+static int unit_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : kPreRows; }
+
+bool kv8_attention_fits(const Kv8& c, const Kv8Attention& a) {
+    const int group = a.n_heads / c.n_kv, unit = unit_rows((int64_t)group * a.max_q);
+    const int64_t step = unit == kPreRows ? kPreTok : 2048 / c.head_dim, room = (int64_t)a.table_stride << c.page_shift;
+    const double units = (double)c.n_kv * ((double)a.rows * group / unit + a.n_seqs);
+    return units * (double)(room / step + 1 + kPreUnitCost) < 4294967296.0;
+}
+
 cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, int* err, cudaStream_t st) {
-    const int rows = a.n_heads / c.n_kv * a.max_q;  // that share a kv head's codes, at most
+    const int unit = unit_rows((int64_t)(a.n_heads / c.n_kv) * a.max_q);  // of the rows that share a kv head's codes, at most
     return by_shape(a.dtype, c.format, c.head_dim, [&](auto row, auto fmt, auto d) {
         using T = decltype(row);
         // Units of 4 rows where a sequence has no more, of 8 where it has (more
         // rows share one reading of the codes), and the tensor-core tiles of
         // 128 beyond.
-        if (rows <= 4) return launch_kv8_decode<T, fmt.value, d.value, 1>(c, a, num_sms, ws, st);
-        if (rows <= 8) return launch_kv8_decode<T, fmt.value, d.value, 2>(c, a, num_sms, ws, st);
+        if (unit == 4) return launch_kv8_decode<T, fmt.value, d.value, 1>(c, a, num_sms, ws, st);
+        if (unit == 8) return launch_kv8_decode<T, fmt.value, d.value, 2>(c, a, num_sms, ws, st);
         return launch_kv8_prefill<T, fmt.value, d.value>(c, a, num_sms, (uint8_t*)ws + decode_ws(num_sms), err, st);
     });
 }

@@ -153,7 +153,7 @@ LC_DEV SeqInfo kv8_seq(const Kv8Attention& a, int page_shift, int s) {
         q.row0 = s;
         q.nq = 1;
     }
-    q.len = a.kv_lens[s];
+    q.len = max(0, a.kv_lens[s]);
     return q;
 }
 
@@ -187,7 +187,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     constexpr int STEP = S::kStep, MT = STEP / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     unsigned* prefix = reinterpret_cast<unsigned*>(smem + S::kRingBytes);  // [n_seqs + 1] the line before sequence s
-    __shared__ unsigned scan[kDecWarps];
+    __shared__ unsigned long long scan[kDecWarps];
     __shared__ SeqInfo infos[kDecSeqsShared];
     __shared__ DecCursor first_unit;  // warp 0's first unit, for the joining
     __shared__ DecCursor done_cursor[2];
@@ -210,10 +210,10 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
 
     // ---- the line of steps ----
     // A unit takes its steps and kDecUnitCost empty places behind them.
-    unsigned carry = 0;
+    unsigned long long carry = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += kDecWarps * 32) {
         const int s = s0 + tid;
-        unsigned cost = 0;
+        unsigned long long cost = 0;
         if (s < a.n_seqs) {
             const SeqInfo q = kv8_seq(a, sh, s);
             if (s < kDecSeqsShared) infos[s] = q;
@@ -221,28 +221,29 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
             for (int k = 0; k < chunks; ++k) cost += kDecUnitCost + dec_steps<STEP>(dec_seen(q, group, room, k * R + R - 1));
             cost *= c.n_kv;
         }
-        unsigned v = cost;
+        unsigned long long v = cost;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
+            const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
         if (lane == 31) scan[warp] = v;
         __syncthreads();
-        unsigned before = carry, all = carry;
+        unsigned long long before = carry, all = carry;
         for (int w = 0; w < kDecWarps; ++w) {
             if (w < warp) before += scan[w];
             all += scan[w];
         }
-        if (s < a.n_seqs) prefix[s] = before + v - cost;
+        if (s < a.n_seqs) prefix[s] = (unsigned)(before + v - cost);
         carry = all;
         __syncthreads();
     }
-    if (tid == 0) prefix[a.n_seqs] = carry;
+    if (carry > 0xffffffffull) return;  // the host has checked it for ascending q_start
+    if (tid == 0) prefix[a.n_seqs] = (unsigned)carry;
     __syncthreads();
     // Worker w has steps [begin_of(w), begin_of(w + 1)): equal shares, the first
     // `extra` workers one step more.
-    const unsigned total = carry;
+    const unsigned total = (unsigned)carry;
     if (total == 0) return;
     const unsigned workers = min(gridDim.x * kDecWarps, total);
     const unsigned share = total / workers, extra = total - share * workers;

@@ -189,7 +189,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         sc_full[kPreScaleRing], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
-    __shared__ unsigned scan[kPreThreads / 32];
+    __shared__ unsigned long long scan[kPreThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = a.n_heads / c.n_kv, sh = c.page_shift;
     const int room = (int)min((long long)a.table_stride << sh, 0x7fffffffll);
@@ -218,36 +218,39 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     for (int s = warp; s < a.n_seqs; s += kPreThreads / 32) {
         const SeqInfo q = kv8_seq(a, sh, s);
         const int chunks = chunks_of(q);
-        unsigned cost = 0;
+        unsigned long long cost = 0;
         for (int k = lane; k < chunks; k += 32) cost += steps_of(q, k) + kPreUnitCost;
-        cost = __reduce_add_sync(0xffffffffu, cost);
-        if (lane == 0) prefix[s] = cost * c.n_kv;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+        cost *= c.n_kv;
+        if (lane == 0) prefix[s] = cost > 0xffffffffull ? 0xffffffffu : (unsigned)cost;
     }
     __syncthreads();
-    unsigned carry = 0;
+    unsigned long long carry = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += kPreThreads) {
         const int s = s0 + tid;
         const unsigned cost = s < a.n_seqs ? prefix[s] : 0;
-        unsigned v = cost;
+        unsigned long long v = cost;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
+            const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
         if (lane == 31) scan[warp] = v;
         __syncthreads();
-        unsigned before = carry, all = carry;
+        unsigned long long before = carry, all = carry;
         for (int w = 0; w < kPreThreads / 32; ++w) {
             if (w < warp) before += scan[w];
             all += scan[w];
         }
-        if (s < a.n_seqs) prefix[s] = before + v - cost;
+        if (s < a.n_seqs) prefix[s] = (unsigned)(before + v - cost);
         carry = all;
         __syncthreads();
     }
-    if (tid == 0) prefix[a.n_seqs] = carry;
+    if (carry > 0xffffffffull) return;  // the host has checked it for ascending q_start
+    if (tid == 0) prefix[a.n_seqs] = (unsigned)carry;
     // CTA b has steps [begin_of(b), begin_of(b + 1)).
-    const unsigned total = carry;
+    const unsigned total = (unsigned)carry;
     const unsigned workers = min(gridDim.x, total);
     if (blockIdx.x >= workers) return;  // also where there is nothing at all
     if (warp == 12) {

@@ -518,6 +518,54 @@ def test_attention_prompts_at_length(lib, kind, fmt, heads, kv, page, d, lens, c
         assert torch.equal(first, out)
 
 
+@pytest.mark.parametrize("per", [1, 5])
+def test_attention_of_4096_sequences(lib, per):
+    """The largest number of sequences: no longer than a page or two each, some empty."""
+    rng = np.random.default_rng(per)
+    lens = rng.integers(0, 40, 4096)
+    counts = np.full(4096, per)
+    pool, table, q_start, q = attention_case(lib, rng, lens, counts, 4, 1, 16, 64, "i8", "f32", extra_rows=3)
+    cache, _ = cache_of(lib, pool, "i8")
+    out = torch.full(q.shape, 7.0, device="cuda")
+    cache.attention(dev(q), out, dev(q_start), dev(lens.astype(np.int32)), dev(table), max_q=per)
+    sync()
+    got = out.cpu().numpy()
+    assert (got[-3:] == 7).all()
+    some = list(range(0, 4096, 64)) + [4095]
+    for s in some:
+        rows = slice(q_start[s], q_start[s + 1])
+        terms = {}
+        want = ref.attention(q[rows], np.array([0, per]), [int(lens[s])], table[s:s + 1], pool["k"], pool["v"],
+                             pool["k_scale"], pool["v_scale"], "i8", 0.125, np.zeros((per, 4, 64)), terms)
+        for key in np.ndindex(per, 4):
+            off = np.abs(got[rows][key] - want[key]).max()
+            assert off <= (attention_tolerance(terms[key], "f32", 64) if key in terms else 0.0), (s, key)
+
+
+def test_append_of_a_padded_batch(lib):
+    """Rows without a slot before, between and behind: what is written is what the rows alone give."""
+    rng = np.random.default_rng(3)
+    pool = make_pool(rng, 9, 2, 32, 64, "i8")
+    slots = runs(rng, [(0, 3), (31, 2), (5, 1), (64, 40)], 32, 9)
+    rows = rng.standard_normal((len(slots), 2, 64)).astype(np.float32)
+    at = np.sort(rng.choice(np.arange(700, 2900), len(slots), replace=False))
+    at[1:3] = at[0] + 1 + np.arange(2)  # neighbours too
+    at = np.unique(at)
+    n = len(at)
+    padded = np.full(20000, -1, np.int32)
+    padded[at] = slots[:n]
+    wide = np.zeros((20000, 2, 64), np.float32)
+    wide[at] = rows[:n]
+    a, ta = cache_of(lib, pool, "i8")
+    want = {k: v.copy() for k, v in pool.items()}
+    a.append(dev(wide), dev(wide), dev(padded))
+    sync()
+    for name in "kv":
+        ref.append(want[name], want[name + "_scale"], wide, padded, "i8")
+    for name in want:
+        assert np.array_equal(ta[name].cpu().numpy(), want[name]), name
+
+
 @pytest.mark.parametrize("max_q", [1, 2, 9, 1000])
 def test_attention_holds_for_any_max_q(lib, max_q):
     rng = np.random.default_rng(4)
@@ -769,6 +817,9 @@ def test_refusals_of_the_library(lib):
         cache.attention(torch.zeros(1, 3, 64, device="cuda"), torch.zeros(1, 3, 64, device="cuda"), None, lens, table)
     with pytest.raises(L.IllegalArgumentError):  # without q_start, a row for every sequence
         cache.attention(torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda"), None, lens, table)
+    with pytest.raises(L.LlamaCudaError, match="2\\^32 steps"):  # 4096 rows one by one over 2^26 positions
+        cache.attention(torch.zeros(4096, 2, 64, device="cuda"), torch.zeros(4096, 2, 64, device="cuda"), i32(2), lens,
+                        torch.zeros(1, 1 << 21, dtype=torch.int32, device="cuda"), max_q=1)
     host = L.PagedKV8(torch.zeros(4, 2, 32, 64, dtype=torch.uint8), torch.zeros(4, 2, 32, 64, dtype=torch.uint8),
                       torch.zeros(4, 2), torch.zeros(4, 2), acc=acc)
     with pytest.raises(L.IllegalArgumentError, match="device memory"):
