@@ -68,23 +68,24 @@ def _torch_types() -> None:
 
 
 def _i32(buf, min_len: int, writable: bool = False) -> int:
-    """_addr(buf, "i32", ...) with few steps for a tensor: these calls are short."""
-    if isinstance(buf, np.ndarray):
-        return _addr(buf, "i32", min_len, writable)
-    if _TORCH_I32 is None:
+    """_addr(buf, "i32", ...); what a tensor in order needs comes first, for
+    these calls are short."""
+    if buf.dtype is _TORCH_I32 and buf.numel() >= min_len and buf.is_contiguous():
+        return buf.data_ptr()
+    if _TORCH_I32 is None and not isinstance(buf, np.ndarray):
         _torch_types()
-    if buf.dtype is not _TORCH_I32:
-        raise TypeError(f"expected i32 tensor, got {buf.dtype}")
-    if not buf.is_contiguous():
-        raise ValueError("tensor must be contiguous")
-    if buf.numel() < min_len:
-        raise ValueError(f"tensor holds {buf.numel()} elements, need {min_len}")
-    return buf.data_ptr()
+    return _addr(buf, "i32", min_len, writable)
 
 
 def _rows(buf, writable: bool = False):
     """(address, rows, width, row stride in elements, dtype id) of a buffer of
     F32 or F16 rows: [rows, ...] with contiguous rows, any row stride."""
+    dt = _TORCH_ROWS.get(buf.dtype)
+    if dt is not None and buf.is_contiguous() and buf.dim() >= 2:
+        rows = buf.size(0)
+        if rows:
+            width = buf.numel() // rows
+            return buf.data_ptr(), rows, width, width, dt
     shape = buf.shape
     if len(shape) < 2:
         raise ValueError(f"expected [rows, ...], got shape {tuple(shape)}")
@@ -325,10 +326,13 @@ class CudaRoPE(_CudaKernel, IRoPE):
             ya, orows, owidth, ys, odt = _rows(out, True)
             if (orows, owidth, odt) != (rows, width, dt):
                 raise ValueError("x and out differ in shape or type")
-        if width == 0 or width % config.head_dim:
-            raise ValueError(f"rows of {width} elements, head_dim {config.head_dim}")
-        _lib.check(self.lib.lc_rope_apply(self.ctx, config.lc, xa, ya, _i32(positions, rows), rows,
-                                          width // config.head_dim, xs, ys, dt, int(transpose)))
+        d = config.head_dim
+        if width == 0 or width % d:
+            raise ValueError(f"rows of {width} elements, head_dim {d}")
+        rc = self.lib.lc_rope_apply(self.acc.handle, config.lc, xa, ya, _i32(positions, rows), rows, width // d, xs, ys,
+                                    dt, transpose)
+        if rc:
+            _lib.check(rc)
 
 
 class CudaPages(_CudaKernel):
@@ -340,13 +344,15 @@ class CudaPages(_CudaKernel):
         positions, seq_ids [capacity]; q_start [n + 1]; free_count(_out) [1];
         status [2] = (code, detail), code 0 when the step was done."""
         n, stride = table.shape
-        cap = slots.shape[0]
-        _lib.check(self.lib.lc_pages_step(
-            self.ctx, _i32(lens, n), _i32(n_new, n), n, page_size, _i32(table, n * stride, True),
-            stride, _i32(free_list, 1, True), _i32(free_count, 1), free_list.shape[0], cap,
+        cap = len(slots)
+        rc = self.lib.lc_pages_step(
+            self.acc.handle, _i32(lens, n), _i32(n_new, n), n, page_size, _i32(table, n * stride, True),
+            stride, _i32(free_list, 1, True), _i32(free_count, 1), len(free_list), cap,
             _i32(lens_out, n, True), _i32(q_start, n + 1, True), _i32(slots, cap, True),
             _i32(positions, cap, True), _i32(seq_ids, cap, True),
-            _i32(free_count_out, 1, True), _i32(status, 2, True)))
+            _i32(free_count_out, 1, True), _i32(status, 2, True))
+        if rc:
+            _lib.check(rc)
 
 
 class PagedKV8(_CudaKernel):
@@ -373,26 +379,31 @@ class PagedKV8(_CudaKernel):
                 raise ValueError("codes and scales must be contiguous")
         self.tensors = (k, v, k_scale, v_scale)
         self.n_kv_heads, self.page_size, self.head_dim = n_kv, page, d
+        self._width, self._scale = n_kv * d, d ** -0.5
         c = _lib.LcKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page, n_kv, d,
                        self.FORMATS[format])
         self._kv = c
 
     def _two(self, k, v, slots, writable: bool):
         ka, rows, width, stride, dt = _rows(k, writable)
-        va, *rest = _rows(v, writable)
-        if rest != [rows, width, stride, dt]:
+        va, vrows, vwidth, vstride, vdt = _rows(v, writable)
+        if vrows != rows or vwidth != width or vstride != stride or vdt != dt:
             raise ValueError("k and v rows differ in shape, stride or type")
-        if width != self.n_kv_heads * self.head_dim:
+        if width != self._width:
             raise ValueError(f"rows of {width} elements, the cache holds {self.n_kv_heads} x {self.head_dim}")
         return ka, va, stride, dt, _i32(slots, rows), rows
 
     def append(self, k, v, slots) -> None:
         """Rows [rows, n_kv_heads, head_dim] (F32 or F16) into their slots (see lc_kv8_append)."""
-        _lib.check(self.lib.lc_kv8_append(self.ctx, self._kv, *self._two(k, v, slots, False)))
+        rc = self.lib.lc_kv8_append(self.acc.handle, self._kv, *self._two(k, v, slots, False))
+        if rc:
+            _lib.check(rc)
 
     def read(self, k, v, slots) -> None:
         """Rows [rows, n_kv_heads, head_dim] (F32 or F16) = the values at their slots (see lc_kv8_read)."""
-        _lib.check(self.lib.lc_kv8_read(self.ctx, self._kv, *self._two(k, v, slots, True)))
+        rc = self.lib.lc_kv8_read(self.acc.handle, self._kv, *self._two(k, v, slots, True))
+        if rc:
+            _lib.check(rc)
 
     def attention(self, q, out, q_start, kv_lens, table, max_q: int = 1, scale: float | None = None) -> None:
         """Causal attention of rows q [rows, n_heads, head_dim] (see
@@ -400,16 +411,18 @@ class PagedKV8(_CudaKernel):
         when every sequence has one query; scale None: 1 / sqrt(head_dim)."""
         qa, rows, width, qs, dt = _rows(q)
         oa, orows, owidth, os_, odt = _rows(out, True)
-        if (orows, owidth, odt) != (rows, width, dt):
+        if orows != rows or owidth != width or odt != dt:
             raise ValueError("q and out differ in shape or type")
         d = self.head_dim
         if width == 0 or width % d:
             raise ValueError(f"rows of {width} elements, head_dim {d}")
         n, stride = table.shape
-        _lib.check(self.lib.lc_kv8_attention(
-            self.ctx, self._kv, qa, oa, qs, os_, dt, rows, None if q_start is None else _i32(q_start, n + 1),
+        rc = self.lib.lc_kv8_attention(
+            self.acc.handle, self._kv, qa, oa, qs, os_, dt, rows, None if q_start is None else _i32(q_start, n + 1),
             _i32(kv_lens, n), _i32(table, n * stride), stride, n, max_q, width // d,
-            d ** -0.5 if scale is None else scale))
+            self._scale if scale is None else scale)
+        if rc:
+            _lib.check(rc)
 
 
 class CudaSiLU(_CudaKernel, ISiLU):
