@@ -21,17 +21,19 @@
 // CTA's piece in L2 otherwise.
 //
 // What bounds it: for head size 64 one exponential costs as much as the 128
-// products of its score, so the special-function unit and the issue slots
-// around it, not the tensor cores, set the pace; hence two row tiles, whose
-// softmax warpgroups take turns with the tensor cores, and one dequantised
-// tile for both.
+// products of its score, so the softmax, not the tensor cores, sets the pace
+// (4096 fp32 queries, 32 heads: 276 us, of which the products need 81; the
+// special-function unit is busy 28 % of the time, the issue slots 44 %).
+// Hence two row tiles per CTA, one dequantised tile for both, and loops over
+// 32 columns that are kept loops: unrolled over the step, their code no longer
+// fits the schedulers' instruction caches (297 against 263 us).
 //
 // Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: queries and
-// codes to f16 operands, a unit's queries while its predecessor's last step is
-// weighed.  Warps 12 and 13: issue the MMAs of a row tile each.  Registers move from the last two
-// warpgroups to the softmax.  All steps of the call form one line that is cut
-// into equal pieces, one per CTA; pieces of a unit are joined, warp by warp,
-// by the last CTA to finish, in the order of the line.
+// codes to f16 operands, a unit's queries while the unit before is under way.
+// Warps 12 and 13: issue the MMAs of a row tile each.  Registers move from the
+// last two warpgroups to the softmax.  All steps of the call form one line that
+// is cut into equal pieces, one per CTA; pieces of a unit are joined, warp by
+// warp, by the last CTA to finish, in the order of the line.
 #pragma once
 
 #include "lc_internal.h"
