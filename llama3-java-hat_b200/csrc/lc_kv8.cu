@@ -6,8 +6,16 @@
 // that the page holds below the run become round(c s / s') when s' > s, and the
 // run's are round(x / s').  Each rounding is to the nearest code of the exact
 // quotient, so a value is within half a code step of what was stored before,
-// whatever order the tokens came in.  One warp per unit: no sums, and no
-// order in which anything is added.
+// whatever order the tokens came in.  No sums, and no order in which anything is
+// added.
+//
+// Bound by memory: rows in once, codes out once.  A lane holds four neighbouring
+// elements, a warp 2048 of a unit, in registers between the search for the
+// maximum and the rounding; units of larger pages have 2, 4 or 8 warps, which meet
+// over the maximum (8000 rows of 8 heads x 128, f32: 30 us in pages of 16 or 32, 58
+// in pages of 128, where few units are left to go round; 71 with one warp a unit).
+// The quotient is x * (1 / s), two units of the last place off at most; only where
+// that could change the code (next to a tie) is it divided out.
 #include "lc_internal.h"
 #include "lc_kv8.cuh"
 
@@ -15,7 +23,8 @@ namespace lc {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendWindow = 32;  // rows whose slots one CTA looks at, at most
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kAppendWindow = 32;  // rows whose slots one CTA looks at together, at most
 constexpr int kAppendHold = 16;    // groups of four that a lane keeps
 
 // Four elements as they lie in memory.
@@ -126,145 +135,151 @@ LC_DEV uint32_t encode4(float4 v, float s, float inv) {
     return w;
 }
 
-template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_append_kernel(Kv8 c, Kv8Rows r, int window) {
+template <typename T, int FMT, int D, bool TEAMS>
+__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_append_kernel(Kv8 c, Kv8Rows r, int window, int windows, int team_size) {
     constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows at a time
     griddep_launch();
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sh = c.page_shift, page = 1 << sh;
     const int64_t n_slots = (int64_t)c.n_pages << sh;
-    const int row0 = blockIdx.x * window;
     const bool aligned = (((uintptr_t)r.k | (uintptr_t)r.v | (uintptr_t)(r.row_stride * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
-    // Lane i: is row row0 + i the first of its page's rows?  Rows without a
-    // slot are passed over.
-    const int my = row0 + lane;
-    auto slot_of = [&](int i) {
+    auto slot_of = [&](int64_t i) {
         const int v = r.slots[i];
         return v >= 0 && v < n_slots ? v : -1;
     };
-    int slot = -1;
-    bool starts = false;
-    if (lane < window && my < r.rows) {
-        slot = slot_of(my);
-        if (slot >= 0) {
-            int prev = my > 0 ? slot_of(my - 1) : -1;
-            for (int i = my - 2; prev < 0 && i >= 0; i -= 8) {  // behind skipped rows, eight at a time
-                int v[8];
-#pragma unroll
-                for (int b = 0; b < 8; ++b) v[b] = i - b >= 0 ? slot_of(i - b) : -1;
-#pragma unroll
-                for (int b = 7; b >= 0; --b)
-                    if (v[b] >= 0) prev = v[b];
-            }
-            starts = prev < 0 || (prev >> sh) != (slot >> sh);
-        }
-    }
-    unsigned starters = __ballot_sync(0xffffffffu, starts);
+    // `team` warps have a unit together, in TEAMS one at least two.
+    const int team = TEAMS ? team_size : 1;
+    const int part = warp % team, teams = kAppendWarps / team, mine = warp / team;
+    __shared__ float tops[2][kAppendWarps];
+    int flip = 0;
+    auto meet = [&]() {
+        if (TEAMS) named_bar_sync(1 + mine, team * 32);
+        else __syncwarp();
+    };
+    auto team_max = [&](float v) {  // of all lanes of the team
+        v = warp_max(v);
+        if (!TEAMS) return v;
+        if (lane == 0) tops[flip][warp] = v;
+        meet();
+        for (int k = 0; k < team; ++k) v = fmaxf(v, tops[flip][mine * team + k]);
+        flip ^= 1;  // the next one does not touch what others may still read
+        return v;
+    };
     const int sub = lane / LPR, e0 = (lane % LPR) * 4;  // this lane's row of those at a time, and its elements
-    int n = 0;                                          // unit number within the CTA
-    while (starters) {
-        const int l = __ffs(starters) - 1;
-        starters &= starters - 1;
-        const int pg = __shfl_sync(0xffffffffu, slot, l) >> sh;
-        for (int u = blockIdx.y; u < 2 * c.n_kv; u += gridDim.y, ++n) {
-            if (n % (kAppendThreads / 32) != warp) continue;
-            const int head = u >> 1;
-            const T* rows = (const T*)((u & 1) ? r.v : r.k) + head * D + e0;
-            uint8_t* codes = ((u & 1) ? c.v : c.k) + ((((int64_t)pg * c.n_kv + head) << sh) * D) + e0;
-            float* scale = ((u & 1) ? c.v_scale : c.k_scale) + (int64_t)pg * c.n_kv + head;
-            float held = *scale;
-            // The page's runs, one after the other: usually there is one.
-            for (int row = row0 + l; row < r.rows;) {
-                const int first = slot_of(row);
-                if (first < 0) {  // skipped rows, 128 at a time: a padded batch ends in many
-                    int v[4];
+    const int at0 = part * RPI + sub, step = team * RPI;  // this lane's first row of a unit, and the distance to the next
+    int n = 0;                                            // unit number within the CTA
+    for (int win = 0; win < (TEAMS ? windows : 1); ++win) {
+        const int64_t row0 = ((int64_t)blockIdx.x * windows + win) * window;
+        if (row0 >= r.rows) break;
+        // Lane i: is row row0 + i the first of its page's rows?  Rows without a
+        // slot are passed over.
+        const int64_t my = row0 + lane;
+        int slot = -1;
+        bool starts = false;
+        if (lane < window && my < r.rows) {
+            slot = slot_of(my);
+            if (slot >= 0) {
+                int prev = my > 0 ? slot_of(my - 1) : -1;
+                for (int64_t i = my - 2; prev < 0 && i >= 0; i -= 8) {  // behind skipped rows, eight at a time
+                    int v[8];
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) v[b] = row + b * 32 + lane < r.rows ? slot_of(row + b * 32 + lane) : -1;
-                    int skip = 128;
+                    for (int b = 0; b < 8; ++b) v[b] = i - b >= 0 ? slot_of(i - b) : -1;
 #pragma unroll
-                    for (int b = 3; b >= 0; --b) {
-                        const unsigned m = __ballot_sync(0xffffffffu, v[b] >= 0);
-                        if (m) skip = b * 32 + __ffs(m) - 1;
+                    for (int b = 7; b >= 0; --b)
+                        if (v[b] >= 0) prev = v[b];
+                }
+                starts = prev < 0 || (prev >> sh) != (slot >> sh);
+            }
+        }
+        unsigned starters = __ballot_sync(0xffffffffu, starts);
+        while (starters) {
+            const int l = __ffs(starters) - 1;
+            starters &= starters - 1;
+            const int pg = __shfl_sync(0xffffffffu, slot, l) >> sh;
+            for (int u = blockIdx.y; u < 2 * c.n_kv; u += gridDim.y, ++n) {
+                if (n % teams != mine) continue;
+                const int head = u >> 1;
+                const T* rows = (const T*)((u & 1) ? r.v : r.k) + head * D + e0;
+                uint8_t* codes = ((u & 1) ? c.v : c.k) + ((((int64_t)pg * c.n_kv + head) << sh) * D) + e0;
+                float* scale = ((u & 1) ? c.v_scale : c.k_scale) + (int64_t)pg * c.n_kv + head;
+                float held = *scale;
+                // The page's runs, one after the other: usually there is one.
+                for (int64_t row = row0 + l; row < r.rows;) {
+                    const int first = slot_of(row);
+                    if (first < 0) {  // skipped rows, 128 at a time: a padded batch ends in many
+                        int v[4];
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) v[b] = row + b * 32 + lane < r.rows ? slot_of(row + b * 32 + lane) : -1;
+                        int skip = 128;
+#pragma unroll
+                        for (int b = 3; b >= 0; --b) {
+                            const unsigned m = __ballot_sync(0xffffffffu, v[b] >= 0);
+                            if (m) skip = b * 32 + __ffs(m) - 1;
+                        }
+                        row += skip;
+                        continue;
                     }
-                    row += skip;
-                    continue;
-                }
-                if ((first >> sh) != pg) break;
-                const int off = first & (page - 1);
-                // Rows row .. row + len - 1, at most to the page's end; those of this
-                // window are in the lanes' `slot`.
-                int len = 1;
-                if (row < row0 + window) {
-                    const int k = my - row;
-                    const unsigned m = __ballot_sync(0xffffffffu, k < 0 || (lane < window && off + k < page && slot == first + k));
-                    len = (m == 0xffffffffu ? 32 : __ffs(~m) - 1) - (row - row0);
-                }
-                for (; row + len >= row0 + window && off + len < page; len += 32) {
-                    const int k = len + lane;
-                    const bool ok = off + k < page && row + k < r.rows && r.slots[row + k] == first + k;
-                    const unsigned m = __ballot_sync(0xffffffffu, ok);
-                    if (m != 0xffffffffu) {
-                        len += __ffs(~m) - 1;
-                        break;
+                    if ((first >> sh) != pg) break;
+                    const int off = first & (page - 1);
+                    // Rows row .. row + len - 1, at most to the page's end; those of this
+                    // window are in the lanes' `slot`.
+                    int len = 1;
+                    if (row < row0 + window) {
+                        const int k = (int)(my - row);
+                        const unsigned m = __ballot_sync(0xffffffffu, k < 0 || (lane < window && off + k < page && slot == first + k));
+                        len = (m == 0xffffffffu ? 32 : __ffs(~m) - 1) - (int)(row - row0);
                     }
-                }
-                const T* x = rows + (int64_t)row * r.row_stride;
-                const bool keep = len <= kAppendHold * RPI;
-                Raw<T> v[kAppendHold];
-                typename Raw<T>::Top most = Raw<T>::none();
-                if (keep) {
+                    for (; row + len >= row0 + window && off + len < page; len += 32) {
+                        const int k = len + lane;
+                        const bool ok = off + k < page && row + k < r.rows && r.slots[row + k] == first + k;
+                        const unsigned m = __ballot_sync(0xffffffffu, ok);
+                        if (m != 0xffffffffu) {
+                            len += __ffs(~m) - 1;
+                            break;
+                        }
+                    }
+                    const T* x = rows + row * r.row_stride;
+                    Raw<T> v[kAppendHold];
+                    typename Raw<T>::Top most = Raw<T>::none();
 #pragma unroll
                     for (int i = 0; i < kAppendHold; ++i) {
-                        const int k = i * RPI + sub;
+                        const int k = at0 + i * step;
                         if (k < len) v[i].load(x + (int64_t)k * r.row_stride, aligned);
                         else v[i].zero();
                     }
 #pragma unroll
                     for (int i = 0; i < kAppendHold; ++i) most = v[i].top(most);
-                } else {
-#pragma unroll 8
-                    for (int k = sub; k < len; k += RPI) {
-                        Raw<T> w;
-                        w.load(x + (int64_t)k * r.row_stride, aligned);
-                        most = w.top(most);
-                    }
-                }
-                float top = warp_max(Raw<T>::value(most));
-                if (top == INFINITY) {  // infinities do not set the scale
-                    top = 0.0f;
-                    for (int k = sub; k < len; k += RPI) top = top4(load4(x + (int64_t)k * r.row_stride, aligned), top);
-                    top = warp_max(top);
-                }
-                const float old = off ? held : 0.0f;
-                const float now = fmaxf(old, __fdiv_rn(top, kv8_limit(FMT)));
-                const float inv = __fdiv_rn(1.0f, now);
-                if (now > old)
-                    for (int k = sub; k < off; k += RPI) {
-                        uint32_t* at = reinterpret_cast<uint32_t*>(codes + k * D);
-                        const uint32_t w = *at;
-                        uint32_t z = 0;
+                    float top = team_max(Raw<T>::value(most));
+                    if (top == INFINITY) {  // infinities do not set the scale
+                        top = 0.0f;
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) z |= kv8_requant<FMT>((w >> (8 * b)) & 0xffu, old, now) << (8 * b);
-                        *at = z;
+                        for (int i = 0; i < kAppendHold; ++i) top = top4(v[i].get(), top);
+                        top = team_max(top);
                     }
-                if (keep) {
+                    const float old = off ? held : 0.0f;
+                    const float now = fmaxf(old, __fdiv_rn(top, kv8_limit(FMT)));
+                    const float inv = __fdiv_rn(1.0f, now);
+                    if (now > old)
+                        for (int k = at0; k < off; k += step) {
+                            uint32_t* at = reinterpret_cast<uint32_t*>(codes + k * D);
+                            const uint32_t w = *at;
+                            uint32_t z = 0;
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) z |= kv8_requant<FMT>((w >> (8 * b)) & 0xffu, old, now) << (8 * b);
+                            *at = z;
+                        }
 #pragma unroll
                     for (int i = 0; i < kAppendHold; ++i) {
-                        const int k = i * RPI + sub;
+                        const int k = at0 + i * step;
                         if (k < len) *reinterpret_cast<uint32_t*>(codes + (off + k) * D) = encode4<FMT>(v[i].get(), now, inv);
                     }
-                } else {
-#pragma unroll 4
-                    for (int k = sub; k < len; k += RPI)
-                        *reinterpret_cast<uint32_t*>(codes + (off + k) * D) =
-                            encode4<FMT>(load4(x + (int64_t)k * r.row_stride, aligned), now, inv);
+                    held = now;
+                    row += len;
+                    meet();  // the next run rounds these codes anew
                 }
-                held = now;
-                row += len;
-                __syncwarp();  // the next run rounds these codes anew
+                if (part == 0 && lane == 0) *scale = held;
             }
-            if (lane == 0) *scale = held;
         }
     }
 }
@@ -336,15 +351,21 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, Kv8Rows r) {
 
 template <typename T, int FMT>
 static cudaError_t append(const Kv8& c, const Kv8Rows& r, int num_sms, cudaStream_t st) {
-    // A CTA looks at as many rows as leave every SM four CTAs: with 64 rows of
-    // 64 sequences and 32 rows a CTA, two CTAs took 119 us.
+    // A CTA looks at as many rows as leave every SM four CTAs (with 64 rows of
+    // 64 sequences and 32 rows a CTA, two CTAs took 119 us), at most at a page
+    // or 32; a team of warps holds a page of one head, and the units of a page
+    // are shared out so that every team has one.
     int window = r.rows / (num_sms * 4);
     window = window < 1 ? 1 : window > kAppendWindow ? kAppendWindow : window;
-    // With many rows a window holds a page or two, 2 n_kv units each: a warp of
-    // two CTAs then has one of them.
-    const dim3 grid((r.rows + window - 1) / window, window >= 8 && c.n_kv >= 8 ? 2 : 1), block(kAppendThreads);
-    return c.head_dim == 64 ? launch_ex(kv8_append_kernel<T, FMT, 64>, grid, block, 0, st, true, c, r, window)
-                            : launch_ex(kv8_append_kernel<T, FMT, 128>, grid, block, 0, st, true, c, r, window);
+    const int page = 1 << c.page_shift, windows = window == kAppendWindow && page > window ? page / window : 1;
+    const int unit = page * c.head_dim, team = unit <= 2048 ? 1 : unit / 2048;
+    const int64_t span = (int64_t)window * windows;
+    int shares = 2 * c.n_kv * team / kAppendWarps;
+    shares = shares < 1 ? 1 : shares > 2 * c.n_kv ? 2 * c.n_kv : shares;
+    const dim3 grid((unsigned)((r.rows + span - 1) / span), shares), block(kAppendThreads);
+    auto go = [&](auto kernel) { return launch_ex(kernel, grid, block, 0, st, true, c, r, window, windows, team); };
+    if (c.head_dim == 64) return team > 1 ? go(kv8_append_kernel<T, FMT, 64, true>) : go(kv8_append_kernel<T, FMT, 64, false>);
+    return team > 1 ? go(kv8_append_kernel<T, FMT, 128, true>) : go(kv8_append_kernel<T, FMT, 128, false>);
 }
 
 cudaError_t launch_kv8_append(const Kv8& c, const Kv8Rows& r, int num_sms, cudaStream_t st) {

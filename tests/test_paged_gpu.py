@@ -566,6 +566,33 @@ def test_append_of_a_padded_batch(lib):
         assert np.array_equal(ta[name].cpu().numpy(), want[name]), name
 
 
+@pytest.mark.parametrize("fmt,kind,page,d", [("i8", "f32", 64, 64), ("e4m3", "f16", 128, 64), ("i8", "f16", 64, 128),
+                                             ("e4m3", "f32", 128, 128), ("i8", "f32", 32, 128)])
+def test_append_of_long_prompts_in_large_pages(lib, fmt, kind, page, d):
+    """More rows than there is room for side by side: pages longer than the rows
+    that are looked at together, begun in their middle, cut by skipped rows,
+    with infinities, and codes below that are rounded anew."""
+    rng = np.random.default_rng(page + d)
+    spans = [(0, 9000), (37, 5000), (1, 1), (page - 1, 2), (page // 2 + 3, 4000), (0, page), (90, 1400)]
+    n_pages = sum(-(-(a + b) // page) for a, b in spans) + 1
+    pool = make_pool(rng, n_pages, 1, page, d, fmt)
+    slots = runs(rng, spans, page, n_pages)
+    slots = np.insert(slots, [5, 6000, 6001, 9003, len(slots)], -1)
+    n = len(slots)
+    assert n >= 19000
+    rows = {k: (rng.standard_normal((n, 1, d)) * np.exp(rng.standard_normal((n, 1, 1)))).astype(NP[kind]) for k in "kv"}
+    rows["k"][[3, 8000, 14010], 0, 1:3] = [np.inf, -np.inf]
+    rows["v"][4:300] = 0.0
+    cache, t = cache_of(lib, pool, fmt)
+    want = {k: v.copy() for k, v in pool.items()}
+    for name in "kv":
+        ref.append(want[name], want[name + "_scale"], rows[name], slots, fmt)
+    cache.append(dev(rows["k"]), dev(rows["v"]), dev(slots))
+    sync()
+    for name in want:
+        assert_same_codes(t[name].cpu().numpy(), want[name], fmt, name)
+
+
 @pytest.mark.parametrize("max_q", [1, 2, 9, 1000])
 def test_attention_holds_for_any_max_q(lib, max_q):
     rng = np.random.default_rng(4)
