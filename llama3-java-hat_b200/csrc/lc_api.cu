@@ -138,6 +138,7 @@ static int check_device_error(lc_context* c) {
     CK(cudaMemcpy(&h, c->d_err, sizeof(int), cudaMemcpyDeviceToHost), "read device error word");
     if (h != 0) {
         cudaMemset(c->d_err, 0, sizeof(int));
+        if (c->kv8_ws) CK(kv8_attention_clear(c->kv8_ws, c->sms, c->stream), "clear the attention workspace");
         return fail(LC_ERR_TIMEOUT, "device-side wait gave up (code %d)", h);
     }
     return LC_OK;
@@ -891,18 +892,19 @@ extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, 
         if (n_heads <= 0 || n_heads % kv->n_kv_heads)
             return fail(LC_ERR_INVALID_ARG, "n_heads=%d n_kv_heads=%d", n_heads, kv->n_kv_heads);
         const int64_t width = (int64_t)n_heads * kv->head_dim;
+        constexpr int kSpare = 1023;  // the kernels round rows and positions up to whole units and steps
         if (rows < 0 || n_seqs < 0 || n_seqs > kPagesMaxSeqs || table_stride <= 0 || max_q < 1 || max_q > (1 << 24) || n_heads > (1 << 16) || q_stride < 0 ||
             (rows > 1 && out_stride < width))
             return fail(LC_ERR_INVALID_ARG, "rows=%d n_seqs=%d (0..%d) table_stride=%d max_q=%d q_stride=%lld out_stride=%lld",
                         rows, n_seqs, kPagesMaxSeqs, table_stride, max_q, (long long)q_stride, (long long)out_stride);
-        if ((int64_t)table_stride * kv->page_size > INT32_MAX)
+        if ((int64_t)table_stride * kv->page_size > INT32_MAX - kSpare)
             return fail(LC_ERR_UNSUPPORTED, "positions are 32-bit");
         if (!q_start && (max_q != 1 || rows != n_seqs))
             return fail(LC_ERR_INVALID_ARG, "without q_start every sequence has one query: rows=%d n_seqs=%d max_q=%d", rows,
                         n_seqs, max_q);
         if (!(scale > 0.0f) || isinf(scale)) return fail(LC_ERR_INVALID_ARG, "scale=%g", scale);
         if (rows == 0 || n_seqs == 0) return LC_OK;
-        if ((int64_t)rows * n_heads > INT32_MAX) return fail(LC_ERR_UNSUPPORTED, "rows * n_heads exceeds 2^31 - 1");
+        if ((int64_t)rows * n_heads > INT32_MAX - kSpare) return fail(LC_ERR_UNSUPPORTED, "rows * n_heads exceeds 2^31 - 1024");
         Stager s(c);
         Kv8Attention a;
         memset(&a, 0, sizeof(a));

@@ -39,6 +39,10 @@ cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st) {
         });
         if (e != cudaSuccess) return e;
     }
+    return kv8_attention_clear(ws, num_sms, st);
+}
+
+cudaError_t kv8_attention_clear(void* ws, int num_sms, cudaStream_t st) {
     const cudaError_t e = cudaMemsetAsync(ws, 0, kv8_counter_bytes(num_sms), st);
     if (e != cudaSuccess) return e;
     return cudaMemsetAsync((uint8_t*)ws + decode_ws(num_sms), 0, kv8_prefill_counter_bytes(num_sms), st);

@@ -209,7 +209,6 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         mbar_init(&drained, 2);
         fence_mbar_init();
     }
-    griddep_launch();
     griddep_wait();
 
     auto seen_of = [&](const SeqInfo& q, int row) { return dec_seen(q, group, room, row); };
@@ -262,8 +261,8 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    griddep_launch();  // here: the next kernel may ask for tensor memory before it waits for this one
     const uint32_t tmem = tmem_slot;
-    const uint64_t deadline = globaltimer_ns() + timeout_ns;
     const unsigned share = total / workers, extra = total - share * workers;
     auto begin_of = [&](unsigned w) { return w * share + min(w, extra); };
     auto worker_of = [&](unsigned x) {
@@ -337,7 +336,9 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
     }
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         // Whole warps wait; they go on together, as the tensor-memory instructions ask.
-        return (bool)__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err, deadline, kDevTimeoutGrid));
+        // The limit is each wait's own: a call of long prompts may take seconds.
+        return (bool)__all_sync(0xffffffffu, mbar_try_wait(bar, parity) ||
+                                                 mbar_wait_bounded(bar, parity, err, globaltimer_ns() + timeout_ns, kDevTimeoutGrid));
     };
     auto tiles_of = [&](const PreCursor& u) { return (int64_t)u.q.nq * group - (int64_t)u.chunk * kPreRows > 128 ? 2 : 1; };
     bool ok = true;

@@ -74,6 +74,8 @@ size_t kv8_attention_ws_bytes(int num_sms);
 // Whether the call's line of work can be counted in 32 bits.
 bool kv8_attention_fits(const Kv8& c, const Kv8Attention& a);
 cudaError_t kv8_attention_prepare(void* ws, int num_sms, cudaStream_t st);
+// Its counters to zero again, behind a call that gave up.
+cudaError_t kv8_attention_clear(void* ws, int num_sms, cudaStream_t st);
 cudaError_t launch_kv8_attention(const Kv8& c, const Kv8Attention& a, int num_sms, void* ws, int* err, cudaStream_t st);
 
 }  // namespace lc

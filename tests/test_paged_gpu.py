@@ -518,6 +518,28 @@ def test_attention_prompts_at_length(lib, kind, fmt, heads, kv, page, d, lens, c
         assert torch.equal(first, out)
 
 
+def test_attention_of_a_call_of_seconds(lib):
+    """A prompt of 420,000 positions, every query the same (row stride 0): its
+    waits have limits of seconds, the call as a whole has none."""
+    rng = np.random.default_rng(12)
+    n, heads, page, d = 420_000, 32, 128, 64
+    pool, table, _, _ = attention_case(lib, rng, [n], [1], 1, 1, page, d, "i8", "f32")
+    q = rng.standard_normal((heads, d)).astype(np.float32)
+    cache, _ = cache_of(lib, pool, "i8")
+    out = torch.full((n, heads, d), 7.0, device="cuda")
+    args = dev(np.array([0, n], np.int32)), dev(np.array([n], np.int32)), dev(table)
+    cache.attention(dev(q)[None].expand(n, heads, d), out, *args, max_q=n)
+    sync()
+    assert bool(torch.isfinite(out).all())
+    for j in (0, 63, 64, 4095, 211_111, n - 1):
+        terms = {}
+        want = ref.attention(q[None], np.array([0, 1]), [j + 1], table, pool["k"], pool["v"], pool["k_scale"],
+                             pool["v_scale"], "i8", d ** -0.5, np.zeros((1, heads, d)), terms)
+        got = out[j].cpu().numpy()
+        for h in range(0, heads, 5):
+            assert np.abs(got[h] - want[0, h]).max() <= attention_tolerance(terms[0, h], "f32", d), (j, h)
+
+
 @pytest.mark.parametrize("per", [1, 5])
 def test_attention_of_4096_sequences(lib, per):
     """The largest number of sequences: no longer than a page or two each, some empty."""
