@@ -44,10 +44,6 @@ namespace lc {
 
 constexpr int kPreRows = 256;      // rows of a unit
 constexpr int kPreThreads = 16 * 32;
-// Registers of the softmax, operand and MMA warpgroups after the split; their sum
-// over 128 threads each must not pass the launch's (checked on the host).
-constexpr int kPreRegsSoftmax = 168, kPreRegsOperand = 120, kPreRegsMma = 56;
-constexpr int kPreRegsLaunch = (2 * kPreRegsSoftmax + kPreRegsOperand + kPreRegsMma + 3) / 4;
 constexpr int kPreTok = 64;        // tokens of a step
 constexpr int kPreUnitCost = 3;    // a unit's beginning and end, in steps
 constexpr int kPreScaleRing = 8;   // more steps than the operand warps can be ahead of the softmax
@@ -64,6 +60,12 @@ struct PreShape {
     static constexpr int kScaleBytes = kPreScaleRing * (kGroups * 8 + 8);
     static constexpr int kSmem = kQBufs * (kQBytes + kPreRows * 4) + 2 * kStages * kTileBytes + kScaleBytes;
     static constexpr int kPieceFloats = kPreRows * (D + 2);
+    // Registers of the softmax, operand and MMA warpgroups after the split; their
+    // sum over 128 threads each must not pass the launch's (checked on the host).
+    // Head size 128 holds twice the codes: with 120 registers the operand warps
+    // spill (4096 f16 queries, 32 heads: 310 against 280 us).
+    static constexpr int kRegsSoftmax = D == 64 ? 168 : 160, kRegsOperand = D == 64 ? 120 : 128, kRegsMma = D == 64 ? 56 : 64;
+    static constexpr int kRegsLaunch = (2 * kRegsSoftmax + kRegsOperand + kRegsMma + 3) / 4;
     // Tensor memory: two buffers of S for each tile, so that the next step's
     // scores are there when a step's weights are done; O of both tiles;
     // and for head size 64 the second accumulators.
@@ -345,16 +347,14 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
 
     if (warp >= 8 && warp < 12) {
         // ---- operands to f16 ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsOperand));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegsOperand));
         const int cw = warp - 8;
         constexpr int CH = NT * D / 16 / 128;  // 16-code chunks per thread, for K and for V
-        // What a step needs from memory; two of them, so that a step's loads have
-        // two steps' time.
-        struct Codes {
-            uint4 k[CH], v[CH];
-            float ks, vs;  // scales of 16-token group `lane`, in the first warp
-            bool there;
-        };
+        // What a step needs from memory.  The next step's keys are asked for as soon as
+        // this one's are written as operands, then its values: each has a step's time.
+        uint4 wk[CH], wv[CH];
+        float ks = 0.0f, vs = 0.0f;  // scales of 16-token group `lane`, in the first warp
+        bool there = false;
         int id[CH], group_id = -1;
         auto token_of = [&](int k) {  // of this thread's k-th chunk
             const int i = k * 4 + cw;
@@ -373,21 +373,21 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 group_id = t < u.seen ? row[t >> sh] : -1;
             }
         };
-        auto load_codes = [&](const PreCursor& u, Codes& w) {
+        auto load_codes = [&](const PreCursor& u, const uint8_t* from, uint4 (&w)[CH]) {
 #pragma unroll
             for (int k = 0; k < CH; ++k) {
                 const int t = u.step * NT + token_of(k);
-                w.k[k] = w.v[k] = make_uint4(0, 0, 0, 0);  // tokens that nobody sees stay zero: there may be NaN codes
-                if ((unsigned)id[k] < (unsigned)c.n_pages) {
-                    const int64_t at = ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16;
-                    w.k[k] = __ldg(reinterpret_cast<const uint4*>(c.k + at));
-                    w.v[k] = __ldg(reinterpret_cast<const uint4*>(c.v + at));
-                }
+                w[k] = make_uint4(0, 0, 0, 0);  // tokens that nobody sees stay zero: there may be NaN codes
+                if ((unsigned)id[k] < (unsigned)c.n_pages)
+                    w[k] = __ldg(reinterpret_cast<const uint4*>(
+                        from + ((((int64_t)id[k] * c.n_kv + u.head) << sh) + (t & ((1 << sh) - 1))) * D + chunk_of(k) * 16));
             }
+        };
+        auto load_scales = [&](const PreCursor& u) {
             if (cw == 0 && lane < G) {
-                w.there = (unsigned)group_id < (unsigned)c.n_pages;
-                w.ks = w.there ? c.k_scale[(int64_t)group_id * c.n_kv + u.head] : 0.0f;
-                w.vs = w.there ? c.v_scale[(int64_t)group_id * c.n_kv + u.head] : 0.0f;
+                there = (unsigned)group_id < (unsigned)c.n_pages;
+                ks = there ? c.k_scale[(int64_t)group_id * c.n_kv + u.head] : 0.0f;
+                vs = there ? c.v_scale[(int64_t)group_id * c.n_kv + u.head] : 0.0f;
             }
         };
         auto put = [&](uint8_t* tile, const uint4 (&w)[CH]) {
@@ -423,10 +423,11 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         };
         auto put_queries = [&](const PreCursor& u, int buf) {
             const int rows = tiles_of(u) * 128;
-            constexpr int V = 16 / sizeof(T), N = D / 2 / V;  // elements of 16 bytes, loads of half a row
+            constexpr int TPR = D / 32;                // threads of a row, 32 elements each
+            constexpr int V = 16 / sizeof(T), N = 32 / V;  // elements of 16 bytes, loads of a thread
 #pragma unroll 1
-            for (int r = cw * 16 + (lane >> 1); r < rows; r += 64) {  // two neighbouring threads per row
-                const int e0 = (lane & 1) * (D / 2);
+            for (int r = cw * (32 / TPR) + lane / TPR; r < rows; r += 128 / TPR) {
+                const int e0 = (lane % TPR) * 32;
                 const T* q = query(u, r);
                 uint4 w[N];
 #pragma unroll
@@ -443,8 +444,9 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const T* e = reinterpret_cast<const T*>(w);
                 float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < D / 2; ++i) top = fmaxf(top, fabsf((float)e[i]));
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf((float)e[i]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                if (TPR == 4) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 int ex = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
                 ex = max(-126, min(126, ex));
                 const float up = pow2f(ex);
@@ -452,7 +454,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 const uint32_t at = smem_u32(sq) + buf * S::kQBytes + (r >> 7) * (SPLIT ? 2 : 1) * S::kQPart +
                                     ((r & 127) >> 3) * (D * 16) + (r & 7) * 16 + (e0 >> 3) * 128;
 #pragma unroll
-                for (int o = 0; o < D / 16; ++o) {
+                for (int o = 0; o < 4; ++o) {
                     float v[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = (float)e[o * 8 + i] * up;
@@ -469,9 +471,14 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         // one whose tiles are written.
         PreCursor nx = cur;
         unsigned ahead = lo, x = lo;
-        auto load_next = [&](Codes& w) {
+        auto load_keys = [&]() {
             if (ahead >= hi) return;
-            load_codes(nx, w);
+            load_codes(nx, c.k, wk);
+            load_scales(nx);
+        };
+        auto load_values = [&]() {
+            if (ahead >= hi) return;
+            load_codes(nx, c.v, wv);
             ++ahead;
             if (++nx.step == nx.steps) {
                 ahead += kPreUnitCost;
@@ -479,12 +486,9 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             }
             if (ahead < hi) load_ids(nx);
         };
-        Codes w, behind;
-        w.ks = w.vs = behind.ks = behind.vs = 0.0f;
-        w.there = behind.there = false;
         if (x < hi) load_ids(nx);
-        load_next(w);
-        load_next(behind);
+        load_keys();
+        load_values();
         int i = 0, units = 0, last_step[2] = {0, 0};
 #pragma unroll 1
         while (x < hi && ok) {
@@ -506,11 +510,11 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             const int st = i % NS, use = i / NS;
             if (use > 0) ok = wait(&k_empty[st], (use - 1) & 1);
             if (!ok) break;
-            put(sk + st * S::kTileBytes, w.k);
+            put(sk + st * S::kTileBytes, wk);
             if (cw == 0) {
                 const int ring = i % kPreScaleRing;
-                if (lane < G) scales[ring * G + lane] = make_float2(w.ks, w.vs < 1e-36f ? -120.0f : log2f(w.vs));  // NaN stays
-                const unsigned m = __ballot_sync(0xffffffffu, lane < G && w.there);
+                if (lane < G) scales[ring * G + lane] = make_float2(ks, vs < 1e-36f ? -120.0f : log2f(vs));  // NaN stays
+                const unsigned m = __ballot_sync(0xffffffffu, lane < G && there);
                 if (lane == 0) valid[ring * 2] = m;
             }
             fence_async_shared();
@@ -519,14 +523,14 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 mbar_arrive(&k_full[st]);
                 if (cw == 0) mbar_arrive(&sc_full[i % kPreScaleRing]);
             }
+            load_keys();
             if (use > 0) ok = wait(&v_empty[st], (use - 1) & 1);
             if (!ok) break;
-            put(sv + st * S::kTileBytes, w.v);
+            put(sv + st * S::kTileBytes, wv);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[st]);
-            w = behind;
-            load_next(behind);
+            load_values();
             ++i;
             ++x;
             if (++cur.step == cur.steps) {
@@ -536,7 +540,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         }
     } else if (warp >= 12) {
         // ---- MMAs: a warp per row tile, one thread of it issues ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsMma));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegsMma));
         if (warp < 14) {
             const int tile = warp - 12;
             constexpr uint32_t id_qk = tc_idesc_f16_f32(128, NT);
@@ -621,7 +625,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         __syncwarp();
     } else {
         // ---- softmax: one thread per row ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsSoftmax));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kRegsSoftmax));
         const int tile = warp >> 2, r = tid & 127;  // row of the tile, its TMEM lane
         const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp % 4)
         const uint32_t to = tmem + lane_base + S::kOCol + tile * D;
@@ -953,7 +957,7 @@ cudaError_t kv8_prefill_prepare() {
     cudaFuncAttributes attr;
     const cudaError_t e = cudaFuncGetAttributes(&attr, kv8_prefill_kernel<T, FMT, D>);
     if (e != cudaSuccess) return e;
-    if (attr.numRegs < kPreRegsLaunch) return cudaErrorInvalidKernelImage;
+    if (attr.numRegs < PreShape<T, D>::kRegsLaunch) return cudaErrorInvalidKernelImage;
     return cudaFuncSetAttribute(kv8_prefill_kernel<T, FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 PreShape<T, D>::kSmem + (kPagesMaxSeqs + 1) * (int)sizeof(unsigned));
 }
