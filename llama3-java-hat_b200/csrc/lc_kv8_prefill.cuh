@@ -657,31 +657,31 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             auto sum_at = [&](int e4) { return reinterpret_cast<float4*>(piece + ((size_t)e4 * kPreRows + unit_row) * 4); };
             auto flush = [&]() {
 #pragma unroll 1
-                for (int ch = 0; ch < D / 32; ++ch) {
-                    uint32_t w[32];
-                    tmem_ld32(to + ch * 32, w);
+                for (int ch = 0; ch < D / 16; ++ch) {
+                    uint32_t w[16];
+                    tmem_ld16(to + ch * 16, w);
                     if constexpr (S::kSumInTmem) {
-                        uint32_t z[32];
-                        if (flushed) tmem_ld32(tsum + ch * 32, z);
-                        tmem_wait_ld32(w);
+                        uint32_t z[16];
+                        if (flushed) tmem_ld16(tsum + ch * 16, z);
+                        tmem_wait_ld(w);
                         if (flushed) {
-                            tmem_wait_ld32(z);
+                            tmem_wait_ld(z);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), since, __uint_as_float(w[e])));
+                            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__fmaf_rn(__uint_as_float(z[e]), since, __uint_as_float(w[e])));
                         }
-                        tmem_st32(tsum + ch * 32, w);
+                        tmem_st16(tsum + ch * 16, w);
                     } else {
-                        float4 z[8];
+                        float4 z[4];
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) z[q] = flushed ? __ldcg(sum_at(ch * 8 + q)) : make_float4(0, 0, 0, 0);
-                        tmem_wait_ld32(w);
+                        for (int q = 0; q < 4; ++q) z[q] = flushed ? __ldcg(sum_at(ch * 4 + q)) : make_float4(0, 0, 0, 0);
+                        tmem_wait_ld(w);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
+                        for (int q = 0; q < 4; ++q) {
                             z[q].x = __fmaf_rn(z[q].x, since, __uint_as_float(w[4 * q]));
                             z[q].y = __fmaf_rn(z[q].y, since, __uint_as_float(w[4 * q + 1]));
                             z[q].z = __fmaf_rn(z[q].z, since, __uint_as_float(w[4 * q + 2]));
                             z[q].w = __fmaf_rn(z[q].w, since, __uint_as_float(w[4 * q + 3]));
-                            __stcg(sum_at(ch * 8 + q), z[q]);
+                            __stcg(sum_at(ch * 4 + q), z[q]);
                         }
                     }
                 }
