@@ -64,7 +64,7 @@ struct PreShape {
     // sum over 128 threads each must not pass the launch's (checked on the host).
     // Head size 128 holds twice the codes: with 120 registers the operand warps
     // spill (4096 f16 queries, 32 heads: 310 against 280 us).
-    static constexpr int kRegsSoftmax = D == 64 ? 168 : 160, kRegsOperand = D == 64 ? 120 : 128, kRegsMma = D == 64 ? 56 : 64;
+    static constexpr int kRegsSoftmax = D == 64 ? 144 : 160, kRegsOperand = 128, kRegsMma = D == 64 ? 96 : 64;
     static constexpr int kRegsLaunch = (2 * kRegsSoftmax + kRegsOperand + kRegsMma + 3) / 4;
     // Tensor memory: two buffers of S for each tile, so that the next step's
     // scores are there when a step's weights are done; O of both tiles;
@@ -690,129 +690,131 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             };
             const bool part_of_it = tile < tiles;
             float m = -INFINITY, l = 0.0f, vl = -120.0f;  // vl: log2 of the reference value scale
-            for (int k = 0; k < n && ok && part_of_it; ++k, ++np) {
-                const int ring = (i + k) % kPreScaleRing;
-                const uint32_t ts = tmem + lane_base + tile * 2 * NT + (np & 1) * NT;
-                ok = wait(&sc_full[ring], ((i + k) / kPreScaleRing) & 1) && wait(&s_full[tile * 2 + (np & 1)], (np >> 1) & 1);
-                if (!ok) break;
+            // The products of the step before are in O.  Waited for in every step,
+            // before its own weights are handed over: a wait knows only the
+            // parity of a phase, so none may be passed over.
+            auto settled = [&]() {
+                ok = wait(&pv_done[tile], (np - 1) & 1);
                 tc_fence_after();
-                const int t0 = (cur.step + k) * NT;
-                const unsigned groups = valid[ring * 2];
-                const bool whole = t0 + NT <= seen_min && groups == (1u << G) - 1u;
-                const float2* sc = scales + ring * G;
-                const bool anew = k % S::kFlush == 0;  // these products begin O anew
-                // The products of the step before are in O.  Waited for in every step,
-                // before its own weights are handed over: a wait knows only the
-                // parity of a phase, so none may be passed over.
-                auto settled = [&]() {
-                    ok = wait(&pv_done[tile], (np - 1) & 1);
-                    tc_fence_after();
-                    return ok;
-                };
-                if (anew && k > 0) {
+                return ok;
+            };
+            for (int k0 = 0; k0 < n && ok && part_of_it; k0 += S::kFlush) {
+                if (k0 > 0) {
                     if (!settled()) break;
                     flush();
                 }
-                // Largest score, group by group: the scale is applied to a group's
-                // maximum.  The loops over groups stay loops: unrolled, their code is
-                // larger than the schedulers' instruction caches.
-                float top = -INFINITY, lvmax = -120.0f;
-                auto largest = [&](auto masked) {
+                const int k1 = min(n, k0 + S::kFlush);
+                for (int k = k0; k < k1 && ok; ++k, ++np) {
+                    const int ring = (i + k) % kPreScaleRing;
+                    const uint32_t ts = tmem + lane_base + tile * 2 * NT + (np & 1) * NT;
+                    ok = wait(&sc_full[ring], ((i + k) / kPreScaleRing) & 1) && wait(&s_full[tile * 2 + (np & 1)], (np >> 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int t0 = (cur.step + k) * NT;
+                    const unsigned groups = valid[ring * 2];
+                    const bool whole = t0 + NT <= seen_min && groups == (1u << G) - 1u;
+                    const float2* sc = scales + ring * G;
+                    // Largest score, group by group: the scale is applied to a group's
+                    // maximum.  The loops over groups stay loops: unrolled, their code is
+                    // larger than the schedulers' instruction caches.
+                    float top = -INFINITY, lvmax = -120.0f;
+                    auto largest = [&](auto masked) {
 #pragma unroll 1
-                    for (int g0 = 0; g0 < G; g0 += 2) {
-                        uint32_t w[32];
-                        tmem_ld32(ts + g0 * 16, w);
-                        tmem_wait_ld32(w);
+                        for (int g0 = 0; g0 < G; g0 += 2) {
+                            uint32_t w[32];
+                            tmem_ld32(ts + g0 * 16, w);
+                            tmem_wait_ld32(w);
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const int gr = g0 + b;
-                            const float2 g2 = sc[gr];
-                            const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
-                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                            for (int b = 0; b < 2; ++b) {
+                                const int gr = g0 + b;
+                                const float2 g2 = sc[gr];
+                                const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
+                                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[b * 16 + e]) : -INFINITY);
-                            const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                            top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
-                            lvmax = fmaxf(lvmax, g2.y);
-                        }
-                    }
-                };
-                if (whole) largest(std::false_type());
-                else largest(std::true_type());
-                // p <= 2^6 * 2^6 * 2^3 < 65504
-                const bool move = top > m + 6.0f, vmove = lvmax > vl + 3.0f;
-                if (__any_sync(0xffffffffu, move) || vmove) {
-                    float f = 1.0f;
-                    if (move) {
-                        f = ex2(m - top);
-                        l *= f;
-                        m = top;
-                    }
-                    if (vmove) {
-                        f *= ex2(vl - lvmax);
-                        vl = lvmax;
-                    }
-                    since *= f;
-                    if (!anew) {
-                        if (!settled()) break;
-#pragma unroll 1
-                        for (int ch = 0; ch < D / 16; ++ch) {
-                            uint32_t z[16];
-                            tmem_ld16(to + ch * 16, z);
-                            tmem_wait_ld(z);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * f);
-                            tmem_st16(to + ch * 16, z);
-                        }
-                    }
-                }
-                const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
-                auto weigh = [&](auto masked) {
-#pragma unroll 1
-                    for (int g0 = 0; g0 < G; g0 += 2) {
-                        uint32_t w[32];
-                        tmem_ld32(ts + g0 * 16, w);
-                        tmem_wait_ld32(w);
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const int gr = g0 + b;
-                            uint32_t ph[8], pl[8];
-                            const float2 g2 = sc[gr];
-                            const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
-                            const float cf = g2.x * qf, bb = bias + lr, out = ex2(-lr);
-                            const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
-                            const uint64_t cf2 = pair(cf, cf), b2 = pair(bb, bb);
-                            uint64_t part = 0;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float2 xx = unpair(fma2(pair(__uint_as_float(w[b * 16 + 2 * e]), __uint_as_float(w[b * 16 + 2 * e + 1])), cf2, b2));
-                                const float p0 = ex2(!masked || 2 * e < left ? xx.x : -INFINITY);
-                                const float p1 = ex2(!masked || 2 * e + 1 < left ? xx.y : -INFINITY);
-                                const uint64_t p = pair(p0, p1);
-                                part = add2(part, p);
-                                const __half2 hh = __floats2half2_rn(p0, p1);
-                                ph[e] = *reinterpret_cast<const uint32_t*>(&hh);
-                                if (SPLIT) {
-                                    const float2 f = __half22float2(hh);
-                                    pl[e] = pack_f16(p0 - f.x, p1 - f.y);
-                                }
+                                for (int e = 0; e < 16; ++e)
+                                    mx[e & 3] = fmaxf(mx[e & 3], !masked || e < left ? __uint_as_float(w[b * 16 + e]) : -INFINITY);
+                                const float m4 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                                top = fmaxf(top, masked && left <= 0 ? -INFINITY : m4 * (g2.x * qf));
+                                lvmax = fmaxf(lvmax, g2.y);
                             }
-                            const float2 s2 = unpair(part);
-                            l = __fmaf_rn(s2.x + s2.y, out, l);
-                            // Over the 16 columns of these tokens: hi, then lo.
-                            tmem_st8(ts + gr * 16, ph);
-                            if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
+                        }
+                    };
+                    if (whole) largest(std::false_type());
+                    else largest(std::true_type());
+                    // p <= 2^6 * 2^6 * 2^3 < 65504
+                    const bool move = top > m + 6.0f, vmove = lvmax > vl + 3.0f;
+                    if (__any_sync(0xffffffffu, move) || vmove) {
+                        float f = 1.0f;
+                        if (move) {
+                            f = ex2(m - top);
+                            l *= f;
+                            m = top;
+                        }
+                        if (vmove) {
+                            f *= ex2(vl - lvmax);
+                            vl = lvmax;
+                        }
+                        since *= f;
+                        if (k > k0) {  // step k0 begins O anew
+                            if (!settled()) break;
+#pragma unroll 1
+                            for (int ch = 0; ch < D / 16; ++ch) {
+                                uint32_t z[16];
+                                tmem_ld16(to + ch * 16, z);
+                                tmem_wait_ld(z);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * f);
+                                tmem_st16(to + ch * 16, z);
+                            }
                         }
                     }
-                };
-                if (whole) weigh(std::false_type());
-                else weigh(std::true_type());
-                tmem_wait_st();
-                if (k > 0 && !settled()) break;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_ready[tile * 2 + (np & 1)]);
+                    const float bias = m == -INFINITY ? 0.0f : 6.0f - m;
+                    auto weigh = [&](auto masked) {
+#pragma unroll 1
+                        for (int g0 = 0; g0 < G; g0 += 2) {
+                            uint32_t w[32];
+                            tmem_ld32(ts + g0 * 16, w);
+                            tmem_wait_ld32(w);
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                const int gr = g0 + b;
+                                uint32_t ph[8], pl[8];
+                                const float2 g2 = sc[gr];
+                                const float lr0 = g2.y - vl, lr = lr0 < -40.0f ? -40.0f : lr0;  // a NaN stays
+                                const float cf = g2.x * qf, bb = bias + lr, out = ex2(-lr);
+                                const int left = masked ? (groups >> gr & 1 ? seen - t0 - gr * 16 : 0) : 16;
+                                const uint64_t cf2 = pair(cf, cf), b2 = pair(bb, bb);
+                                uint64_t part = 0;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float2 xx = unpair(fma2(pair(__uint_as_float(w[b * 16 + 2 * e]), __uint_as_float(w[b * 16 + 2 * e + 1])), cf2, b2));
+                                    const float p0 = ex2(!masked || 2 * e < left ? xx.x : -INFINITY);
+                                    const float p1 = ex2(!masked || 2 * e + 1 < left ? xx.y : -INFINITY);
+                                    const uint64_t p = pair(p0, p1);
+                                    part = add2(part, p);
+                                    const __half2 hh = __floats2half2_rn(p0, p1);
+                                    ph[e] = *reinterpret_cast<const uint32_t*>(&hh);
+                                    if (SPLIT) {
+                                        const float2 f = __half22float2(hh);
+                                        pl[e] = pack_f16(p0 - f.x, p1 - f.y);
+                                    }
+                                }
+                                const float2 s2 = unpair(part);
+                                l = __fmaf_rn(s2.x + s2.y, out, l);
+                                // Over the 16 columns of these tokens: hi, then lo.
+                                tmem_st8(ts + gr * 16, ph);
+                                if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
+                            }
+                        }
+                    };
+                    if (whole) weigh(std::false_type());
+                    else weigh(std::true_type());
+                    tmem_wait_st();
+                    if (k > 0 && !settled()) break;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_ready[tile * 2 + (np & 1)]);
+                }
             }
             i += n;
             if (ok && part_of_it) {
