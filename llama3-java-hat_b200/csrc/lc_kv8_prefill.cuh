@@ -22,16 +22,18 @@
 //
 // What bounds it: for head size 64 one exponential costs as much as the 128
 // products of its score, so the softmax, not the tensor cores, sets the pace
-// (4096 fp32 queries, 32 heads: 276 us, of which the products need 81; the
-// special-function unit is busy 28 % of the time, the issue slots 44 %).
+// (4096 fp32 queries, 32 heads: 249 us, of which the products need 81; with the
+// softmax's arithmetic left out it is 207: the rest is the steps' chain of
+// barriers and loads).
 // Hence two row tiles per CTA, one dequantised tile for both, and loops over
 // 32 columns that are kept loops: unrolled over the step, their code no longer
 // fits the schedulers' instruction caches (297 against 263 us).
 //
-// Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: queries and
-// codes to f16 operands, a unit's queries while the unit before is under way.
-// Warps 12 and 13: issue the MMAs of a row tile each.  Registers move from the
-// last two warpgroups to the softmax.  All steps of the call form one line that
+// Warps 0-3 and 4-7: softmax of row tiles 0 and 1.  Warps 8-11: codes to f16
+// operands.  Warps 12 and 13: issue the MMAs of a row tile each.  Warps 14 and 15:
+// queries to f16 operands, while the unit before is under way (as a part of the
+// operand warps' work: head size 128 420 against 397 us, head size 64 the same).
+// Registers move from the MMA warps' group to the softmax.  All steps of the call form one line that
 // is cut into equal pieces, one per CTA; pieces of a unit are joined, warp by
 // warp, by the last CTA to finish, in the order of the line.
 #pragma once
@@ -62,9 +64,9 @@ struct PreShape {
     static constexpr int kPieceFloats = kPreRows * (D + 2);
     // Registers of the softmax, operand and MMA warpgroups after the split; their
     // sum over 128 threads each must not pass the launch's (checked on the host).
-    // Head size 128 holds twice the codes: with 120 registers the operand warps
-    // spill (4096 f16 queries, 32 heads: 310 against 280 us).
-    static constexpr int kRegsSoftmax = D == 64 ? 144 : 160, kRegsOperand = 128, kRegsMma = D == 64 ? 96 : 64;
+    // With 168, 120 and 56 the compiler spills (4096 fp32 queries, 32 heads: 269
+    // against 255 us; f16 of head size 128, twice the codes: 310 against 280).
+    static constexpr int kRegsSoftmax = 144, kRegsOperand = 128, kRegsMma = 96;
     static constexpr int kRegsLaunch = (2 * kRegsSoftmax + kRegsOperand + kRegsMma + 3) / 4;
     // Tensor memory: two buffers of S for each tile, so that the next step's
     // scores are there when a step's weights are done; O of both tiles;
@@ -207,7 +209,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4);  // [tile][buffer]
         mbar_init(&pv_done[0], 1), mbar_init(&pv_done[1], 1);
         for (int i = 0; i < kPreScaleRing; ++i) mbar_init(&sc_full[i], 1);
-        for (int i = 0; i < NQ; ++i) mbar_init(&q_full[i], 4), mbar_init(&q_seen[i], 10);  // the softmax and MMA warps
+        for (int i = 0; i < NQ; ++i) mbar_init(&q_full[i], 6), mbar_init(&q_seen[i], 10);  // the softmax and MMA warps
         mbar_init(&drained, 2);
         fence_mbar_init();
     }
@@ -343,6 +345,70 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                                                  mbar_wait_bounded(bar, parity, err, globaltimer_ns() + timeout_ns, kDevTimeoutGrid));
     };
     auto tiles_of = [&](const PreCursor& u) { return (int64_t)u.q.nq * group - (int64_t)u.chunk * kPreRows > 128 ? 2 : 1; };
+    // The unit's rows, each scaled so that its largest element lies in
+    // [2^9, 2^10), as f16 hi (and lo).
+    const bool q16 = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+    auto query = [&](const PreCursor& u, int r) -> const T* {  // row r of the unit; null behind its last
+        const int row = u.chunk * kPreRows + r, j = row / group;
+        if (j >= u.q.nq) return nullptr;
+        return (const T*)a.q + (int64_t)(u.q.row0 + j) * a.q_stride + (int64_t)(u.head * group + row - j * group) * D;
+    };
+    auto prefetch_queries = [&](PreCursor u, int part, int parts) {  // of the next unit, to L2
+        next_unit(u);
+        const int rows = tiles_of(u) * 128;
+        for (int r = part * 32 + lane; r < rows; r += parts * 32) {
+            const T* q = query(u, r);
+            if (!q) break;
+#pragma unroll
+            for (int o = 0; o < D * (int)sizeof(T); o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"((const uint8_t*)q + o));
+        }
+    };
+    auto put_queries = [&](const PreCursor& u, int buf, int part, int parts) {  // by warp `part` of `parts`
+        const int rows = tiles_of(u) * 128;
+        constexpr int TPR = D / 32;                // threads of a row, 32 elements each
+        constexpr int V = 16 / sizeof(T), N = 32 / V;  // elements of 16 bytes, loads of a thread
+#pragma unroll 1
+        for (int r = part * (32 / TPR) + lane / TPR; r < rows; r += parts * (32 / TPR)) {
+            const int e0 = (lane % TPR) * 32;
+            const T* q = query(u, r);
+            uint4 w[N];
+#pragma unroll
+            for (int b = 0; b < N; ++b) {
+                w[b] = make_uint4(0, 0, 0, 0);
+                if (q && q16) {
+                    w[b] = __ldg(reinterpret_cast<const uint4*>(q + e0 + b * V));
+                } else if (q) {
+                    T* e = reinterpret_cast<T*>(&w[b]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) e[i] = q[e0 + b * V + i];
+                }
+            }
+            const T* e = reinterpret_cast<const T*>(w);
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf((float)e[i]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            if (TPR == 4) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int ex = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
+            ex = max(-126, min(126, ex));
+            const float up = pow2f(ex);
+            if (e0 == 0) qscale[buf * kPreRows + r] = a.scale * 1.4426950408889634f * pow2f(-ex);
+            const uint32_t at = smem_u32(sq) + buf * S::kQBytes + (r >> 7) * (SPLIT ? 2 : 1) * S::kQPart +
+                                ((r & 127) >> 3) * (D * 16) + (r & 7) * 16 + (e0 >> 3) * 128;
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = (float)e[o * 8 + i] * up;
+                uint4 h, l;
+                split_octet(v, h, l);
+                sts128(at + o * 128, h);
+                if (SPLIT) sts128(at + S::kQPart + o * 128, l);
+            }
+        }
+        fence_async_shared();
+        __syncwarp();
+    };
     bool ok = true;
 
     if (warp >= 8 && warp < 12) {
@@ -403,70 +469,6 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 sts128(at + 128, make_uint4(f[4], f[5], f[6], f[7]));
             }
         };
-        // The unit's rows, each scaled so that its largest element lies in
-        // [2^9, 2^10), as f16 hi (and lo).
-        const bool q16 = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
-        auto query = [&](const PreCursor& u, int r) -> const T* {  // row r of the unit; null behind its last
-            const int row = u.chunk * kPreRows + r, j = row / group;
-            if (j >= u.q.nq) return nullptr;
-            return (const T*)a.q + (int64_t)(u.q.row0 + j) * a.q_stride + (int64_t)(u.head * group + row - j * group) * D;
-        };
-        auto prefetch_queries = [&](PreCursor u) {  // of the next unit, to L2
-            next_unit(u);
-            const int rows = tiles_of(u) * 128;
-            for (int r = cw * 32 + lane; r < rows; r += 128) {
-                const T* q = query(u, r);
-                if (!q) break;
-#pragma unroll
-                for (int o = 0; o < D * (int)sizeof(T); o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"((const uint8_t*)q + o));
-            }
-        };
-        auto put_queries = [&](const PreCursor& u, int buf) {
-            const int rows = tiles_of(u) * 128;
-            constexpr int TPR = D / 32;                // threads of a row, 32 elements each
-            constexpr int V = 16 / sizeof(T), N = 32 / V;  // elements of 16 bytes, loads of a thread
-#pragma unroll 1
-            for (int r = cw * (32 / TPR) + lane / TPR; r < rows; r += 128 / TPR) {
-                const int e0 = (lane % TPR) * 32;
-                const T* q = query(u, r);
-                uint4 w[N];
-#pragma unroll
-                for (int b = 0; b < N; ++b) {
-                    w[b] = make_uint4(0, 0, 0, 0);
-                    if (q && q16) {
-                        w[b] = __ldg(reinterpret_cast<const uint4*>(q + e0 + b * V));
-                    } else if (q) {
-                        T* e = reinterpret_cast<T*>(&w[b]);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) e[i] = q[e0 + b * V + i];
-                    }
-                }
-                const T* e = reinterpret_cast<const T*>(w);
-                float top = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf((float)e[i]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                if (TPR == 4) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                int ex = top > 0.0f ? 9 - (((__float_as_int(top) >> 23) & 0xff) - 127) : 0;
-                ex = max(-126, min(126, ex));
-                const float up = pow2f(ex);
-                if (e0 == 0) qscale[buf * kPreRows + r] = a.scale * 1.4426950408889634f * pow2f(-ex);
-                const uint32_t at = smem_u32(sq) + buf * S::kQBytes + (r >> 7) * (SPLIT ? 2 : 1) * S::kQPart +
-                                    ((r & 127) >> 3) * (D * 16) + (r & 7) * 16 + (e0 >> 3) * 128;
-#pragma unroll
-                for (int o = 0; o < 4; ++o) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = (float)e[o * 8 + i] * up;
-                    uint4 h, l;
-                    split_octet(v, h, l);
-                    sts128(at + o * 128, h);
-                    if (SPLIT) sts128(at + S::kQPart + o * 128, l);
-                }
-            }
-            fence_async_shared();
-            __syncwarp();
-        };
         // `nx` is the next step to load, its pages' numbers under way; `cur` the
         // one whose tiles are written.
         PreCursor nx = cur;
@@ -489,23 +491,15 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         if (x < hi) load_ids(nx);
         load_keys();
         load_values();
-        int i = 0, units = 0, last_step[2] = {0, 0};
+        int i = 0, units = 0;
 #pragma unroll 1
         while (x < hi && ok) {
-            if (i == 0 || cur.step == 0) {
-                // The buffer's last unit: its scores are all computed (where a later
-                // tile has not waited for that already), its factors read.
-                const int buf = units % NQ, l = buf ? last_step[1] : last_step[0];
-                if (units >= NQ) {
-                    if (l >= i - NS) ok = wait(&k_empty[l % NS], (l / NS) & 1);
-                    ok = ok && wait(&q_seen[buf], (units / NQ - 1) & 1);
-                }
+            if ((i == 0 || cur.step == 0) && (NQ == 1 || units == 0)) {
+                if (units > 0) ok = wait(q_seen, (units - 1) & 1);
                 if (!ok) break;
-                put_queries(cur, buf);
-                if (lane == 0) mbar_arrive(&q_full[buf]);
-                (buf ? last_step[1] : last_step[0]) = i + min(cur.steps - cur.step, (int)(hi - x)) - 1;
+                put_queries(cur, 0, cw, 6);
+                if (lane == 0) mbar_arrive(q_full);
                 ++units;
-                if (x + (cur.steps - cur.step) + kPreUnitCost < hi) prefetch_queries(cur);
             }
             const int st = i % NS, use = i / NS;
             if (use > 0) ok = wait(&k_empty[st], (use - 1) & 1);
@@ -556,6 +550,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             for (unsigned x = lo; x < hi && ok;) {
                 const int n = min(cur.steps - cur.step, (int)(hi - x));
                 const bool live = tile < tiles_of(cur);
+                const int buf = units % NQ;
                 // Scores of step k: its buffer's weights, two steps back, have been read.
                 auto scores = [&](int k) {
                     const int st = (i0 + k) % NS;
@@ -573,16 +568,15 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                                     tc_mma_f16(d, qd + part * (S::kQPart / 16) + e * 16, kd + e * 16, id_qk, part + e > 0);
                             tc_commit(&s_full[tile * 2 + ((np + k) & 1)]);
                             tc_commit(&k_empty[st]);
+                            if (k == n - 1) tc_commit(&q_seen[buf]);
                         } else {
                             mbar_arrive(&k_empty[st]);
+                            if (k == n - 1) mbar_arrive(&q_seen[buf]);
                         }
                     }
                     __syncwarp();
                 };
-                const int buf = units % NQ;
                 ok = wait(&q_full[buf], (units++ / NQ) & 1);
-                if (ok && lane == 0) mbar_arrive(&q_seen[buf]);
-                __syncwarp();
                 qd = qd0 + buf * (S::kQBytes / 16);
                 for (int k = 0; k < 2 && k < n && ok; ++k) scores(k);
                 for (int k = 0; k < n && ok; ++k) {
@@ -619,6 +613,28 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 if (cur.step == cur.steps) {
                     x += kPreUnitCost;
                     if (x < hi) next_unit(cur);
+                }
+            }
+        } else {
+            // ---- queries to f16 operands, a unit's while the unit before is under way ----
+            int units = 0;
+            for (unsigned x = lo; x < hi && ok; ++units) {
+                const int n = min(cur.steps - cur.step, (int)(hi - x)), buf = units % NQ;
+                // The buffer's last unit: its scores are computed, its factors read.
+                if (units >= NQ) ok = wait(&q_seen[buf], (units / NQ - 1) & 1);
+                if (!ok) break;
+                // The first unit's, and all where there is one buffer, with the operand warps.
+                const bool alone = NQ == 2 && units > 0;
+                put_queries(cur, buf, alone ? warp - 14 : warp - 10, alone ? 2 : 6);
+                if (lane < (alone ? 3 : 1)) mbar_arrive(&q_full[buf]);
+                x += n;
+                cur.step += n;
+                if (cur.step == cur.steps) {
+                    x += kPreUnitCost;
+                    if (x < hi) {
+                        prefetch_queries(cur, warp - 14, 2);
+                        next_unit(cur);
+                    }
                 }
             }
         }
