@@ -33,9 +33,9 @@
 // operands.  Warps 12 and 13: issue the MMAs of a row tile each.  Warps 14 and 15:
 // queries to f16 operands, while the unit before is under way (as a part of the
 // operand warps' work: head size 128 420 against 397 us, head size 64 the same).
-// Registers move from the MMA warps' group to the softmax.  All steps of the call form one line that
-// is cut into equal pieces, one per CTA; pieces of a unit are joined, warp by
-// warp, by the last CTA to finish, in the order of the line.
+// Registers move from the MMA warps' group to the softmax.  All steps of the call
+// form one line that is cut into equal pieces, one per CTA; pieces of a unit are
+// joined, warp by warp, by the last CTA to finish, in the order of the line.
 #pragma once
 
 #include "lc_internal.h"
@@ -209,7 +209,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], 4);  // [tile][buffer]
         mbar_init(&pv_done[0], 1), mbar_init(&pv_done[1], 1);
         for (int i = 0; i < kPreScaleRing; ++i) mbar_init(&sc_full[i], 1);
-        for (int i = 0; i < NQ; ++i) mbar_init(&q_full[i], 6), mbar_init(&q_seen[i], 10);  // the softmax and MMA warps
+        for (int i = 0; i < NQ; ++i) mbar_init(&q_full[i], 6), mbar_init(&q_seen[i], 10);  // by operand and query warps; softmax and MMA warps
         mbar_init(&drained, 2);
         fence_mbar_init();
     }
@@ -494,11 +494,14 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
         int i = 0, units = 0;
 #pragma unroll 1
         while (x < hi && ok) {
-            if ((i == 0 || cur.step == 0) && (NQ == 1 || units == 0)) {
-                if (units > 0) ok = wait(q_seen, (units - 1) & 1);
+            if (i == 0 || cur.step == 0) {
+                // A unit is also announced here, behind all steps before it: a softmax
+                // group that had no rows in the unit before has not followed them.
+                const int buf = units % NQ;
+                if (units >= NQ) ok = wait(&q_seen[buf], (units / NQ - 1) & 1);
                 if (!ok) break;
-                put_queries(cur, 0, cw, 6);
-                if (lane == 0) mbar_arrive(q_full);
+                if (NQ == 1 || units == 0) put_queries(cur, buf, cw, 6);
+                if (lane == 0) mbar_arrive(&q_full[buf]);
                 ++units;
             }
             const int st = i % NS, use = i / NS;
@@ -626,7 +629,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 // The first unit's, and all where there is one buffer, with the operand warps.
                 const bool alone = NQ == 2 && units > 0;
                 put_queries(cur, buf, alone ? warp - 14 : warp - 10, alone ? 2 : 6);
-                if (lane < (alone ? 3 : 1)) mbar_arrive(&q_full[buf]);
+                if (lane == 0) mbar_arrive(&q_full[buf]);
                 x += n;
                 cur.step += n;
                 if (cur.step == cur.steps) {

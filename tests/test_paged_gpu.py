@@ -476,6 +476,8 @@ def exact_on_gpu(pool, table, q_start, lens, q, fmt, scale):
     x = dev(q).double()
     for s, length in enumerate(lens):
         b, e = int(q_start[s]), int(q_start[s + 1])
+        if b == e or length == 0:
+            continue
         ids = dev(table[s, : -(-length // page)].astype(np.int64))
         for h in range(pool["k"].shape[1]):
             k, v = ((values[t[n][ids, h].long()] * t[n + "_scale"][ids, h].double()[:, None, None]).reshape(-1, q.shape[2])[:length]
@@ -538,6 +540,31 @@ def test_attention_of_a_call_of_seconds(lib):
         got = out[j].cpu().numpy()
         for h in range(0, heads, 5):
             assert np.abs(got[h] - want[0, h]).max() <= attention_tolerance(terms[0, h], "f32", d), (j, h)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kv,page,d", [(16, 4, 16, 64), (8, 2, 64, 128)])
+def test_attention_of_units_of_one_tile_and_two(lib, kind, heads, kv, page, d):
+    """Prompts whose last rows fill one tile, two, or a corner of one, long ones
+    among many that end within a step."""
+    rng = np.random.default_rng(d)
+    counts = np.tile([3, 70, 40, 1, 64, 0, 33, 32, 129, 5], 9)
+    lens = counts + np.tile([0, 5, 1200, 0, 0, 700, 61, 0, 30], 10)
+    pool, table, q_start, q = attention_case(lib, rng, lens.tolist(), counts.tolist(), heads, kv, page, d, "e4m3", kind, extra_rows=0)
+    want, size, weight = exact_on_gpu(pool, table, q_start, lens.tolist(), q, "e4m3", d ** -0.5)
+    rel = 2 * (d + 16) * 2.0 ** -23 * size + (16 + 2 * lens.max()) * 2.0 ** -23 + (2 * HALF["f16"] if kind == "f16" else 0.0)
+    bound = weight * rel + HALF[kind] * weight + TINY[kind]
+    cache, _ = cache_of(lib, pool, "e4m3")
+    args = dev(q_start), dev(lens.astype(np.int32)), dev(table)
+    first = None
+    for _ in range(6):
+        out = torch.full(q.shape, 7.0, dtype=dev(q).dtype, device="cuda")
+        cache.attention(dev(q), out, *args, max_q=int(counts.max()))
+        sync()
+        off = (out.double() - want).abs().amax(-1)
+        assert bool((off <= bound).all()), (off / bound).max()
+        first = out if first is None else first
+        assert torch.equal(first, out)
 
 
 @pytest.mark.parametrize("per", [1, 5])
