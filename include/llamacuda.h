@@ -284,7 +284,7 @@ typedef struct lc_kv8 {
     float *k_scale, *v_scale;
     int32_t n_pages;
     int32_t page_size;  /* 16, 32, 64 or 128 tokens */
-    int32_t n_kv_heads;
+    int32_t n_kv_heads; /* up to 32767 */
     int32_t head_dim;   /* 64 or 128 */
     int32_t format;     /* LC_KV8_* */
     int32_t reserved[3];

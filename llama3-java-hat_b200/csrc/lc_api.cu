@@ -653,6 +653,9 @@ int on_device(lc_context* c, F&& body) {
     }
 }
 
+// Kernels step over rows, and over the elements of a row, in 32 bits.
+constexpr int32_t kMaxCount = INT32_MAX - (1 << 20);
+
 int log2_exact(int v) {
     int k = 0;
     while ((1 << k) < v) ++k;
@@ -668,6 +671,7 @@ int kv8_view(lc_context* c, const lc_kv8* kv, Kv8* out) {
         return fail(LC_ERR_UNSUPPORTED, "page_size %d (16, 32, 64 or 128)", kv->page_size);
     if (kv->head_dim != 64 && kv->head_dim != 128)
         return fail(LC_ERR_UNSUPPORTED, "head_dim %d (64 or 128)", kv->head_dim);
+    if (kv->n_kv_heads > 32767) return fail(LC_ERR_UNSUPPORTED, "n_kv_heads %d (up to 32767)", kv->n_kv_heads);
     if (kv->format != LC_KV8_I8 && kv->format != LC_KV8_E4M3)
         return fail(LC_ERR_INVALID_ARG, "format %d (LC_KV8_I8 = 0, LC_KV8_E4M3 = 1)", kv->format);
     if ((int64_t)kv->n_pages * kv->page_size > INT32_MAX)
@@ -782,6 +786,8 @@ extern "C" int lc_rope_apply(lc_context* c, const lc_rope_config* cfg, const voi
             return fail(LC_ERR_INVALID_ARG, "rows=%d num_heads=%d x_stride=%lld y_stride=%lld", rows, num_heads,
                         (long long)x_stride, (long long)y_stride);
         if (x == y && x_stride != y_stride) return fail(LC_ERR_INVALID_ARG, "in place, the strides must be equal");
+        if (rows > kMaxCount || width > kMaxCount)
+            return fail(LC_ERR_UNSUPPORTED, "rows=%d num_heads=%d: up to %d rows and elements of a row", rows, num_heads, kMaxCount);
         if (rows == 0) return LC_OK;
         Stager s(c);
         const bool in_place = x == y;
@@ -815,6 +821,7 @@ extern "C" int lc_pages_step(lc_context* c, const int32_t* lens, const int32_t* 
             return fail(LC_ERR_INVALID_ARG, "table_stride=%d n_pages=%d capacity=%d", table_stride, n_pages, capacity);
         if ((int64_t)n_pages * page_size > INT32_MAX || (int64_t)table_stride * page_size > INT32_MAX)
             return fail(LC_ERR_UNSUPPORTED, "slots and positions are 32-bit");
+        if (capacity > kMaxCount) return fail(LC_ERR_UNSUPPORTED, "capacity=%d (up to %d)", capacity, kMaxCount);
         Stager s(c);
         PagesStep p;
         memset(&p, 0, sizeof(p));
@@ -854,6 +861,7 @@ static int kv8_rows(lc_context* c, const lc_kv8* kv, void* k, void* v, int64_t r
         const int64_t width = (int64_t)kv->n_kv_heads * kv->head_dim;
         if (rows < 0 || row_stride < 0 || (!append && rows > 1 && row_stride < width))
             return fail(LC_ERR_INVALID_ARG, "rows=%d row_stride=%lld", rows, (long long)row_stride);
+        if (rows > kMaxCount) return fail(LC_ERR_UNSUPPORTED, "rows=%d (up to %d)", rows, kMaxCount);
         if (rows == 0) return LC_OK;
         Stager s(c);
         Kv8Rows r;

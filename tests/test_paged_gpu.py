@@ -1,6 +1,8 @@
 """Paged 8-bit cache operators against plain 64-bit references: rotary
 positions, page bookkeeping, quantised append and read, attention over the
 pages, and a serving loop of all of them."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -896,6 +898,18 @@ def test_refusals_of_the_library(lib):
     with pytest.raises(L.LlamaCudaError, match="2\\^32 steps"):  # 4096 rows one by one over 2^26 positions
         cache.attention(torch.zeros(4096, 2, 64, device="cuda"), torch.zeros(4096, 2, 64, device="cuda"), i32(2), lens,
                         torch.zeros(1, 1 << 21, dtype=torch.int32, device="cuda"), max_q=1)
+    # counts that 32-bit steps would pass: no buffer is looked at
+    many, raw, ctx, config = 2 ** 31 - 16, _lib.load(), acc.handle, _lib.LcRopeConfig()
+    raw.lc_rope_config_llama32(ctypes.byref(config))
+    at = x.data_ptr()
+    assert raw.lc_rope_apply(ctx, ctypes.byref(config), at, at, at, many, 1, 64, 64, 0, 0) == _lib.LC_ERR_UNSUPPORTED
+    assert raw.lc_rope_apply(ctx, ctypes.byref(config), at, at, at, 1, 2 ** 26, 64, 64, 0, 0) == _lib.LC_ERR_UNSUPPORTED
+    assert raw.lc_pages_step(ctx, at, at, 1, 16, at, 1, at, at, 1, many, *[at] * 7) == _lib.LC_ERR_UNSUPPORTED
+    kv = _lib.LcKv8(k=at, v=at, k_scale=at, v_scale=at, n_pages=1, page_size=16, n_kv_heads=1, head_dim=64, format=0)
+    assert raw.lc_kv8_append(ctx, ctypes.byref(kv), at, at, 64, 0, at, many) == _lib.LC_ERR_UNSUPPORTED
+    assert raw.lc_kv8_read(ctx, ctypes.byref(kv), at, at, 64, 0, at, many) == _lib.LC_ERR_UNSUPPORTED
+    kv.n_kv_heads = 32768
+    assert raw.lc_kv8_read(ctx, ctypes.byref(kv), at, at, 64, 0, at, 1) == _lib.LC_ERR_UNSUPPORTED
     host = L.PagedKV8(torch.zeros(4, 2, 32, 64, dtype=torch.uint8), torch.zeros(4, 2, 32, 64, dtype=torch.uint8),
                       torch.zeros(4, 2), torch.zeros(4, 2), acc=acc)
     with pytest.raises(L.IllegalArgumentError, match="device memory"):
