@@ -9,9 +9,11 @@
 // The codes are exact in f16, so scales enter only where scores leave tensor
 // memory: the key scale of a 16-token group in c, the value scale (over a
 // running reference, as its logarithm) in b; the sum takes it out again.
-// fp32 rows are split into f16 hi + lo under a power-of-two row scale, and P
-// likewise, at the price of twice the products; f16 rows take one pass and
-// round P to f16 (2^-12 of each weight), as the result is.
+// fp32 rows are split into f16 hi + lo under a power-of-two row scale, at the
+// price of twice the products; f16 rows are exact.  P is split the same way for
+// both: rounded to one f16 it is off by 2^-12 of each weight, which adds as much
+// error as the rounding of an f16 result itself (1.4 times its norm in all; six
+// chunks of f16 rows over 500 to 4000 positions 133 against 145 us with the split).
 //
 // The tensor cores' fp32 sums lose up to one unit of the last place, always
 // toward zero, at every product that is added; over thousands of tokens that
@@ -73,8 +75,10 @@ struct PreShape {
     // and for head size 64 the second accumulators.
     static constexpr uint32_t kOCol = 4 * kPreTok, kSumCol = kOCol + 2 * D;
     static constexpr bool kSumInTmem = D == 64;
-    // Steps between additions to it: 256 tokens (D 64) or 512 in fp32, 8192 in f16.
-    static constexpr int kFlush = kSplit ? (D == 64 ? 4 : 8) : 128;
+    // Steps between additions to it: 256 tokens (D 64) or 512 in fp32; 2048 in f16,
+    // whose 256 products lose 1e-5, a fortieth of the result's own rounding (after
+    // 1024 tokens 146.6 us instead of 145.5 for the chunks above, after 8192 145.0).
+    static constexpr int kFlush = kSplit ? (D == 64 ? 4 : 8) : 32;
 };
 
 inline size_t kv8_prefill_counter_bytes(int num_sms) { return ((size_t)num_sms * 8 * sizeof(int) + 255) / 256 * 256; }
@@ -597,7 +601,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                             for (int e = 0; e < NT / 16; ++e) {
                                 const uint32_t ac = p + e * 16;
                                 tc_mma_f16_ta(obuf, ac, vd + e * (2 * D), id_pv, e > 0 ? 1 : more);
-                                if (SPLIT) tc_mma_f16_ta(obuf, ac + 8, vd + e * (2 * D), id_pv, 1);
+                                tc_mma_f16_ta(obuf, ac + 8, vd + e * (2 * D), id_pv, 1);
                             }
                             tc_commit(&pv_done[tile]);
                             tc_commit(&v_empty[st]);
@@ -813,16 +817,14 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                                     part = add2(part, p);
                                     const __half2 hh = __floats2half2_rn(p0, p1);
                                     ph[e] = *reinterpret_cast<const uint32_t*>(&hh);
-                                    if (SPLIT) {
-                                        const float2 f = __half22float2(hh);
-                                        pl[e] = pack_f16(p0 - f.x, p1 - f.y);
-                                    }
+                                    const float2 f = __half22float2(hh);
+                                    pl[e] = pack_f16(p0 - f.x, p1 - f.y);
                                 }
                                 const float2 s2 = unpair(part);
                                 l = __fmaf_rn(s2.x + s2.y, out, l);
                                 // Over the 16 columns of these tokens: hi, then lo.
                                 tmem_st8(ts + gr * 16, ph);
-                                if (SPLIT) tmem_st8(ts + gr * 16 + 8, pl);
+                                tmem_st8(ts + gr * 16 + 8, pl);
                             }
                         }
                     };
