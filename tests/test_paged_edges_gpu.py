@@ -46,3 +46,34 @@ def test_attention_of_half_rows_is_off_by_the_rounding_of_the_result(lib, heads,
     sync()
     rounding = torch.linalg.vector_norm(want.half().double() - want)
     assert float(torch.linalg.vector_norm(out.double() - want) / rounding) <= 1.02
+
+
+# ------------------------------------------------------------ launch limits
+
+PAGES_OF_N = """
+import sys
+import numpy as np, torch
+import llamahat
+pages = llamahat.CudaKernelFactory().createPages(llamahat.Accelerator(0))
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+n = int(sys.argv[1])
+z = lambda k: torch.full((k,), -9, dtype=torch.int32, device="cuda")
+lens_out, start, slots, pos, ids, count, status = z(n), z(n + 1), z(n), z(n), z(n), z(1), z(2)
+table, free = torch.full((n, 1), -1, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+pages.step(i32([0] * n), i32([1] * n), table, free, i32([n]), 16, lens_out, start, slots, pos, ids, count, status)
+torch.cuda.synchronize()
+assert status.tolist() == [0, 0] and count.tolist() == [0]
+assert lens_out.tolist() == [1] * n and start.tolist() == list(range(n + 1)) and ids.tolist() == list(range(n))
+assert table[:, 0].tolist() == list(range(n - 1, -1, -1)) and slots.tolist() == [16 * p for p in range(n - 1, -1, -1)]
+"""
+
+
+@pytest.mark.parametrize("n", [2417, 2418, 2440, 2457, 2458])
+def test_pages_step_of_batches_whose_sums_need_48_kb(lib, n):
+    """In a process of its own: a larger batch before it would have raised the
+    kernel's shared-memory limit for good."""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(p for p in sys.path if p))
+    r = subprocess.run([sys.executable, "-c", PAGES_OF_N, str(n)],
+                       env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-800:]
