@@ -15,6 +15,14 @@
 // instead half the products and half the exponentials were spent on empty
 // rows.  tcgen05 has no use for 8 rows of 128.
 //
+// Sums.  The tensor cores' own fp32 sums lose up to one unit of the last place,
+// always toward zero, at every product that is added: over a unit of 65536
+// positions 5.5e-4 of the result where all values have one sign.  So a product of
+// weights and values begins at zero, its hi and lo sums meet, and are added to
+// the unit's in round-to-nearest.  That also halves the accumulators' registers
+// (decode of 64 sequences of 1 to 8191 positions, d 64 and fp32, 60.3 against
+// 60.7 us; d 128 112.5 against 106.8).
+//
 // Softmax.  In powers of two, with a running maximum that is only moved when
 // a score passes it by more than 1; p is held as 2^(x - m + 12), times the
 // page's value scale over a running reference scale (at most 4), which stays
@@ -68,6 +76,14 @@ LC_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The product alone.
+LC_DEV void mma_f16_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 LC_DEV float ex2(float x) {
@@ -430,13 +446,13 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                     qb[r][ks][1] = (g & 1) ? l1 : h1;
                 }
             }
-            float o[NR][KS][4];
+            float o[NR][KS][2];
             float m[NR], l[NR], vref = 0.0f, vinv = 0.0f;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 m[r] = -INFINITY, l[r] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < KS; ++i) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.0f;
+                for (int i = 0; i < KS; ++i) o[r][i][0] = o[r][i][1] = 0.0f;
             }
 
             for (; cur.step < last; ++cur.step, ++x) {
@@ -516,7 +532,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                             m[r] = top[r];
                         }
 #pragma unroll
-                        for (int i = 0; i < KS; ++i) o[r][i][0] *= f, o[r][i][1] *= f, o[r][i][2] *= f, o[r][i][3] *= f;
+                        for (int i = 0; i < KS; ++i) o[r][i][0] *= f, o[r][i][1] *= f;
                     }
                 }
                 const float v0 = vs0 * vinv, v1 = vs1 * vinv;
@@ -579,8 +595,12 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
-                            for (int r = 0; r < NR; ++r)
-                                mma_f16(o[r][2 * e + i], f[i], mt ? pb[r][0].y : pb[r][0].x, mt ? pb[r][1].y : pb[r][1].x);
+                            for (int r = 0; r < NR; ++r) {
+                                float z[4];
+                                mma_f16_zero(z, f[i], mt ? pb[r][0].y : pb[r][0].x, mt ? pb[r][1].y : pb[r][1].x);
+                                o[r][2 * e + i][0] += z[0] + z[1];  // hi and lo meet here
+                                o[r][2 * e + i][1] += z[2] + z[3];
+                            }
                     }
                 }
                 stage = stage == S::kStages - 1 ? 0 : stage + 1;
@@ -609,11 +629,11 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                     const float f = l[r] == 0.0f ? 0.0f : vref / l[r];
 #pragma unroll
                     for (int i = 0; i < E; ++i)
-                        dst[i] = (T)(l[r] == 0.0f ? 0.0f : (o[r][i >> 1][(i & 1) * 2] + o[r][i >> 1][(i & 1) * 2 + 1]) * f);
+                        dst[i] = (T)(l[r] == 0.0f ? 0.0f : o[r][i >> 1][i & 1] * f);
                 } else {
 #pragma unroll
                     for (int i = 0; i < E; ++i)
-                        part[(4 * r + t) * D + g * E + i] = (o[r][i >> 1][(i & 1) * 2] + o[r][i >> 1][(i & 1) * 2 + 1]) * vref;
+                        part[(4 * r + t) * D + g * E + i] = o[r][i >> 1][i & 1] * vref;
                     if (g == 0) {
                         part[R * D + 4 * r + t] = m[r];
                         part[R * D + R + 4 * r + t] = l[r];

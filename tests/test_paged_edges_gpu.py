@@ -77,3 +77,68 @@ def test_pages_step_of_batches_whose_sums_need_48_kb(lib, n):
     r = subprocess.run([sys.executable, "-c", PAGES_OF_N, str(n)],
                        env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-800:]
+
+
+# ---------------------------------------------------------------- long sums
+
+def sums_bound(size, weight, n, d, chain):
+    """Error of fp32 rows that does not grow with n as a chain of truncated sums
+    would.  Scores: each of the d products is off by 2^-22 of itself (rows in
+    two f16), the d / 8 sums of tensor-core products by a unit 2^-23 each, the
+    scales by 4 more: ds = (d / 8 + 6) 2^-23 max_t sum |q k| scale, a weight by
+    a factor exp(+-2 ds).  16 units for the exponential, the weight's two f16
+    and a step's own products; `chain` units where that many products are added
+    on the tensor cores before a sum in round-to-nearest.  The sums themselves:
+    the N additions of round-to-nearest are off by at most half a unit of the
+    result each, in either direction; by Hoeffding their sum passes
+    4 sqrt(N) halves once in 1500 times if each were off by all of it, and
+    they are off by a third of that (a running sum is smaller than the result,
+    a rounding smaller than half a unit).  N: n / 8 for the normaliser, n / 16
+    for the weighted values."""
+    ds = (d / 8 + 6) * 2.0 ** -23 * size
+    return weight * (2 * ds + (16 + chain) * 2.0 ** -23 + 4 * 2.0 ** -24 * (math.sqrt(n / 8) + math.sqrt(n / 16)))
+
+
+def one_sign(lib, rng, lens, counts, heads, kv, page, d, fmt):
+    """Values of one sign and small scores: what every sum loses, it loses in one direction."""
+    pool, table, q_start, q = attention_case(lib, rng, lens, counts, heads, kv, page, d, fmt, "f32", extra_rows=0)
+    pool["v"] = np.maximum(pool["v"] & 0x7F, 1) if fmt == "i8" else np.where(pool["v"] & 0x7F == 0x7F, pool["v"], pool["v"] & 0x7F)
+    return pool, table, q_start, q * np.float32(0.1)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("heads,d", [(4, 64), (8, 64), (4, 128), (8, 128)])
+@pytest.mark.parametrize("length,copies", [(65536, 800), (200, 1), (5000, 1)])
+def test_attention_of_long_decodes_does_not_drift(lib, fmt, heads, d, length, copies):
+    """2400 sequences over the same pages (three queries, 800 times each) leave
+    every warp whole units: 65,536 positions in one running sum."""
+    rng = np.random.default_rng(heads + d)
+    pool, table, _, q3 = one_sign(lib, rng, [length], [1], heads, 1, 128, d, fmt)
+    q3 = np.concatenate([q3, -q3, q3[:, ::-1]])
+    want, size, weight = exact_on_gpu(pool, np.repeat(table, 3, 0), [0, 1, 2, 3], [length] * 3, q3, fmt, d ** -0.5)
+    n = 3 * copies
+    cache, _ = cache_of(lib, pool, fmt)
+    q = dev(q3).repeat(copies, 1, 1)
+    out = torch.full_like(q, 7.0)
+    cache.attention(q, out, None, torch.full((n,), length, dtype=torch.int32, device="cuda"), dev(np.repeat(table, n, 0)))
+    sync()
+    off = (out.double().view(copies, 3, heads, d) - want).abs().amax((0, 3))
+    assert bool((off <= sums_bound(size, weight, length, d, 0)).all()), (off / sums_bound(size, weight, length, d, 0)).max()
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("heads,kv,page,d", [(8, 2, 64, 64), (8, 2, 128, 128)])
+@pytest.mark.parametrize("length", [200, 4096, 16384])
+def test_attention_of_long_prompts_does_not_drift(lib, fmt, heads, kv, page, d, length):
+    """At most 32 products of head size 64, 64 of head size 128, are added on the
+    tensor cores before a sum in round-to-nearest."""
+    rng = np.random.default_rng(length + d)
+    pool, table, q_start, q = one_sign(lib, rng, [length], [64], heads, kv, page, d, fmt)
+    want, size, weight = exact_on_gpu(pool, table, q_start, [length], q, fmt, d ** -0.5)
+    cache, _ = cache_of(lib, pool, fmt)
+    out = torch.full(q.shape, 7.0, device="cuda")
+    cache.attention(dev(q), out, dev(q_start), dev(np.array([length], np.int32)), dev(table), max_q=64)
+    sync()
+    bound = sums_bound(size, weight, length, d, 32 if d == 64 else 64)
+    off = (out.double() - want).abs().amax(-1)
+    assert bool((off <= bound).all()), (off / bound).max()
