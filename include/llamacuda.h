@@ -208,8 +208,10 @@ int lc_argmax(lc_context* ctx, const float* values, int n, int32_t* out_index);
  * device memory throughout, the calls only enqueue on the context's stream
  * and can be captured in a CUDA graph; the first lc_kv8_attention of a
  * context allocates its workspace (make it before a capture), whose size is
- * the same for all calls.  Graphs captured from one context share it:
- * replay them one after the other. */
+ * the same for all calls.  Graphs captured from one context share it, with
+ * each other and with the calls themselves: replay them one after the other,
+ * on the context's stream or ordered against it.  Threads may share a context:
+ * these calls (not those of other sections) take turns. */
 
 enum { LC_ROPE_INTERLEAVED = 0, /* pairs (2j, 2j + 1), as lc_rope */
        LC_ROPE_HALF = 1 };      /* pairs (j, j + rot_dim / 2) */

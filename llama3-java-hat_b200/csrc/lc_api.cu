@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <mutex>
 #include <new>
 #include <string>
 #include <thread>
@@ -84,7 +85,8 @@ struct lc_context {
     void* gemm_scratch = nullptr;   // row scales, pre-split activations, partial sums
     size_t gemm_scratch_bytes = 0;
     bool gemm_ready = false;        // shared-memory attribute of the GEMM kernel set
-    void* kv8_ws = nullptr;         // workspace of lc_kv8_attention, one size for all calls
+    std::mutex paged;               // held by a call of the paged operators: threads take turns
+    std::atomic<void*> kv8_ws{nullptr};  // workspace of lc_kv8_attention, one size for all calls
     lc_rope_config rope_cfg;        // the last lc_rope_apply's configuration and its frequencies
     RopeTurns rope_turns;
     float rope_mult = 0.0f;         // 0: none yet
@@ -126,7 +128,7 @@ extern "C" int lc_context_destroy(lc_context* c) {
     for (void* p : c->pool) cudaFree(p);
     if (c->attn_scratch) cudaFree(c->attn_scratch);
     if (c->gemm_scratch) cudaFree(c->gemm_scratch);
-    if (c->kv8_ws) cudaFree(c->kv8_ws);
+    if (void* ws = c->kv8_ws) cudaFree(ws);
     if (c->d_err) cudaFree(c->d_err);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
@@ -138,7 +140,7 @@ static int check_device_error(lc_context* c) {
     CK(cudaMemcpy(&h, c->d_err, sizeof(int), cudaMemcpyDeviceToHost), "read device error word");
     if (h != 0) {
         cudaMemset(c->d_err, 0, sizeof(int));
-        if (c->kv8_ws) CK(kv8_attention_clear(c->kv8_ws, c->sms, c->stream), "clear the attention workspace");
+        if (void* ws = c->kv8_ws) CK(kv8_attention_clear(ws, c->sms, c->stream), "clear the attention workspace");
         return fail(LC_ERR_TIMEOUT, "device-side wait gave up (code %d)", h);
     }
     return LC_OK;
@@ -637,14 +639,16 @@ size_t rows_bytes(int rows, int64_t stride, int64_t width, int elem) {
 
 int row_elem(int dtype) { return dtype == kRowF32 ? 4 : dtype == kRowF16 ? 2 : 0; }
 
-// Runs the body of an entry point on the context's device; no C++ exception
-// leaves it.
+// Runs the body of an entry point on the context's device, one call of a
+// context at a time: the frequencies of lc_rope_apply, the workspace's first
+// use and the staging buffers are the context's.  No C++ exception leaves it.
 template <typename F>
 int on_device(lc_context* c, F&& body) {
     if (!c) return fail(LC_ERR_INVALID_ARG, "context is NULL");
     DeviceScope scope(c->device);
     if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
     try {
+        std::lock_guard<std::mutex> turn(c->paged);
         return body();
     } catch (const std::bad_alloc&) {
         return fail(LC_ERR_OUT_OF_MEMORY, "host memory");

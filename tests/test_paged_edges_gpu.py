@@ -142,3 +142,91 @@ def test_attention_of_long_prompts_does_not_drift(lib, fmt, heads, kv, page, d, 
     bound = sums_bound(size, weight, length, d, 32 if d == 64 else 64)
     off = (out.double() - want).abs().amax(-1)
     assert bool((off <= bound).all()), (off / bound).max()
+
+
+# ------------------------------------------------------------------ threads
+
+def together(*bodies):
+    """Runs the bodies at once, each in a thread of its own."""
+    errors, gate = [], threading.Barrier(len(bodies))
+
+    def run(body):
+        try:
+            gate.wait()
+            body()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(b,)) for b in bodies]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+
+
+def test_rope_of_threads_with_configurations_of_their_own(lib):
+    """Threads of one context, each with its own configuration: none turns its
+    rows with another's frequencies."""
+    L, acc = lib[:2]
+    rope = L.CudaKernelFactory().createRoPE(acc)
+    configs = [L.RopeConfig(head_dim=512, scaling="yarn", factor=4.0, theta=10000.0 * (k + 1)) for k in range(4)]
+    rng = np.random.default_rng(1)
+    x = dev(rng.standard_normal((2, 1, 512)).astype(np.float32))
+    pos = dev(rng.integers(1000, 100000, 2).astype(np.int32))
+    want, outs = [], []
+    for c in configs:
+        y = torch.zeros_like(x)
+        sync()
+        rope.apply_scaled(x, y, pos, c)
+        sync()
+        want.append(y)
+        outs.append(list(torch.zeros(2000, *x.shape, device="cuda")))
+    sync()
+
+    def body(k):
+        for y in outs[k]:
+            rope.apply_scaled(x, y, pos, configs[k])
+
+    together(*[lambda k=k: body(k) for k in range(4)])
+    sync()
+    wrong = [sum(not torch.equal(y, w) for y in o) for w, o in zip(want, outs)]
+    assert wrong == [0, 0, 0, 0]
+
+
+def test_paged_calls_of_threads_that_share_a_context(lib):
+    """The first attention calls of a context from two threads (one workspace),
+    and host rows of two threads (one set of staging buffers)."""
+    L = lib[0]
+    rng = np.random.default_rng(2)
+    lens, counts = [300, 90], [40, 90]
+    pool, table, q_start, q = attention_case(lib, rng, lens, counts, 8, 2, 32, 64, "i8", "f32", extra_rows=0)
+    t = {k: dev(v) for k, v in pool.items()}
+    lens = np.array(lens, np.int32)
+    results = []
+    for _ in range(3):
+        acc = L.Accelerator(0)
+        caches = [L.PagedKV8(t["k"], t["v"], t["k_scale"], t["v_scale"], acc=acc) for _ in range(2)]
+        outs = [np.zeros((12,) + q.shape, np.float32) for _ in range(2)]
+        backs = [np.zeros((12, 50, 2, 64), np.float32) for _ in range(2)]
+        sync()
+
+        def body(k):
+            for i in range(12):
+                caches[k].attention(q, outs[k][i], q_start, lens, table, max_q=90)
+                caches[k].read(backs[k][i], backs[k][i], np.arange(50 * k, 50 * k + 50, dtype=np.int32))
+
+        together(lambda: body(0), lambda: body(1))
+        results.append((outs, backs))
+    first = results[0]
+    assert np.array_equal(first[0][0], first[0][1])
+    for outs, backs in results:
+        assert all((o == first[0][0][0]).all() for o in outs)
+        for b, f in zip(backs, first[1]):  # by bits: some pages' scales are NaN
+            assert (b.view(np.int32) == f[0].view(np.int32)).all()
+    want, size, weight = exact_on_gpu(pool, table, q_start, lens.tolist(), q, "i8", 0.125)
+    assert float((dev(first[0][0][0]).double() - want).abs().max()) <= float((weight * (2 * 80 * size + 700) * 2.0 ** -23).max())
+    for k, b in enumerate(first[1]):
+        at = np.arange(50 * k, 50 * k + 50)
+        assert np.allclose(b[0], ref.decode(pool["v"][at // 32, :, at % 32], "i8") * pool["v_scale"][at // 32].astype(np.float64)[:, :, None], rtol=2.0 ** -23, atol=0, equal_nan=True)
