@@ -66,7 +66,7 @@ LC_DEV float2 rope_turn(int p, double t, float mult, float sign) {
 // over the rows and heads, so its loads are independent.  The first loads are
 // under way while the angles are computed.
 template <typename T, bool HALF>
-__global__ void __launch_bounds__(kRopeThreads) rope_vec_kernel(RopeApply a, const __grid_constant__ RopeTurns turns, int R) {
+__global__ void __launch_bounds__(kRopeThreads) rope_vec_kernel(RopeApply a, const __grid_constant__ RopeTurns turns, int R, int share) {
     constexpr int N = RopeVec<T>::N;
     extern __shared__ __align__(16) float2 cs[];  // [R][pairs]
     __shared__ int at[kRopeMaxRows];
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec_kernel(RopeApply a, con
     const int per = kRopeThreads / places;                 // (row, head) items at a time
     const int place = threadIdx.x % places, item0 = threadIdx.x / places;
     const int row0 = blockIdx.x * R, rows = min(R, a.rows - row0);
-    const int h0 = a.heads * blockIdx.y / gridDim.y, heads = a.heads * (blockIdx.y + 1) / gridDim.y - h0;
+    const int h0 = blockIdx.y * share, heads = min(share, a.heads - h0);  // at least one
     griddep_launch();
     griddep_wait();
     if (threadIdx.x < rows) at[threadIdx.x] = a.pos[row0 + threadIdx.x];
@@ -205,10 +205,11 @@ cudaError_t launch_rope(const RopeApply& a, const RopeTurns& turns, int num_sms,
     if (R * pairs > kRopeMaxAngles) R = kRopeMaxAngles / pairs;
     if (R == 1)
         while (parts < a.heads && (int64_t)a.rows * parts * 2 <= 2 * num_sms && a.heads / (parts * 2) >= kRopeThreads / places) parts *= 2;
-    const dim3 grid((a.rows + R - 1) / R, parts), block(kRopeThreads);
+    const int share = (a.heads + parts - 1) / parts;
+    const dim3 grid((a.rows + R - 1) / R, (a.heads + share - 1) / share), block(kRopeThreads);
     const size_t smem = (size_t)R * pairs * sizeof(float2);
-    return a.half ? launch_ex(rope_vec_kernel<T, true>, grid, block, smem, st, true, a, turns, R)
-                  : launch_ex(rope_vec_kernel<T, false>, grid, block, smem, st, true, a, turns, R);
+    return a.half ? launch_ex(rope_vec_kernel<T, true>, grid, block, smem, st, true, a, turns, R, share)
+                  : launch_ex(rope_vec_kernel<T, false>, grid, block, smem, st, true, a, turns, R, share);
 }
 
 }  // namespace

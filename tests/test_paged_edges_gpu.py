@@ -230,3 +230,23 @@ def test_paged_calls_of_threads_that_share_a_context(lib):
     for k, b in enumerate(first[1]):
         at = np.arange(50 * k, 50 * k + 50)
         assert np.allclose(b[0], ref.decode(pool["v"][at // 32, :, at % 32], "i8") * pool["v_scale"][at // 32].astype(np.float64)[:, :, None], rtol=2.0 ** -23, atol=0, equal_nan=True)
+
+
+# -------------------------------------------------------------- large counts
+
+def test_rope_of_one_row_of_many_heads(lib):
+    """2^24 + 5 heads in one row, shared out over 256 CTAs: heads times parts passes 2^32."""
+    L, acc, rope, _ = lib
+    cfg = L.RopeConfig(head_dim=4, theta=10000.0)
+    heads, p = 2 ** 24 + 5, 12345
+    x = torch.randn(1, heads, 4, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    y = torch.full_like(x, 7.0)
+    rope.apply_scaled(x, y, dev(np.array([p], np.int32)), cfg)
+    sync()
+    f, _ = ref.rope_frequencies(cfg)
+    top = float(x.abs().max())
+    for j in range(2):
+        c, s = math.cos(p * f[j]), math.sin(p * f[j])
+        a, b = x[0, :, 2 * j].double(), x[0, :, 2 * j + 1].double()
+        for got, want in ((y[0, :, 2 * j], a * c - b * s), (y[0, :, 2 * j + 1], a * s + b * c)):
+            assert float((got.double() - want).abs().max()) <= 2 * top * (2.0 ** -21 + 4 * 2.0 ** -24)
