@@ -97,8 +97,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec_kernel(RopeApply a, con
         for (int k = 0; k < kRopeAhead; ++k) {
             if (i0 + k * per >= items) continue;
             const T* p = x + (int64_t)rl * a.x_stride + hl * a.head_dim;
-            u[k] = __ldg(reinterpret_cast<const uint4*>(p));
-            if (HALF && turn) v[k] = __ldg(reinterpret_cast<const uint4*>(p + pairs));
+            // Plain loads: in place, the kernel writes what it reads here.
+            u[k] = *reinterpret_cast<const uint4*>(p);
+            if (HALF && turn) v[k] = *reinterpret_cast<const uint4*>(p + pairs);
             next(rl, hl);
         }
     };
