@@ -250,3 +250,34 @@ def test_rope_of_one_row_of_many_heads(lib):
         a, b = x[0, :, 2 * j].double(), x[0, :, 2 * j + 1].double()
         for got, want in ((y[0, :, 2 * j], a * c - b * s), (y[0, :, 2 * j + 1], a * s + b * c)):
             assert float((got.double() - want).abs().max()) <= 2 * top * (2.0 ** -21 + 4 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("odd", [False, True])
+def test_rope_cosines_are_exact_to_a_unit_and_a_half(lib, layout, odd):
+    """Pairs (1, 0) become (cos, sin).  The function is off by at most one unit of
+    2^-24 below 1; the part of the angle that a single float does not hold is
+    put right to first order, which leaves the rounding of that correction: half
+    a unit.  (The angle as a single float would be off by 1.57 units more.)"""
+    L, acc, rope, _ = lib
+    cfg = L.RopeConfig(layout=layout, scaling="llama3", factor=32.0)
+    rng = np.random.default_rng(4)
+    n = 20000
+    x = np.zeros((n, 1, 64), np.float32)
+    if layout == "half":
+        x[..., :32] = 1.0
+    else:
+        x[..., ::2] = 1.0
+    pos = rng.integers(0, 131072, n).astype(np.int32)
+    xt = torch.zeros(n, 65, device="cuda")[:, 1 if odd else 0:][:, :64]  # odd: the kernel for any alignment
+    xt[:] = dev(x).view(n, 64)
+    if not odd:
+        xt = xt.contiguous()
+    rope.apply_scaled(xt, xt, dev(pos), cfg)
+    sync()
+    f, _ = ref.rope_frequencies(cfg)
+    angle = pos.astype(np.float64)[:, None] * f
+    got = xt.cpu().numpy().astype(np.float64)
+    a, b = (got[:, :32], got[:, 32:]) if layout == "half" else (got[:, ::2], got[:, 1::2])
+    off = max(np.abs(a - np.cos(angle)).max(), np.abs(b - np.sin(angle)).max())
+    assert off <= 1.5 * 2.0 ** -24 + 2.0 ** -32, off * 2.0 ** 24
