@@ -517,7 +517,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                 if (__any_sync(0xffffffffu, move) || vmax > 4.0f * vref) {
                     float fv = 1.0f;
                     if (vmax > 4.0f * vref) {
-                        const float next = fmaxf(vmax, 1e-30f);
+                        const float next = fmaxf(vmax, 0x1p-126f);  // whose inverse is finite
                         vinv = 1.0f / next;
                         fv = vref * vinv;
                         vref = next;
@@ -626,10 +626,10 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
                     T* dst = out_row(cur, 4 * r + t);
                     if (!dst) continue;
                     dst += g * E;
-                    const float f = l[r] == 0.0f ? 0.0f : vref / l[r];
+                    const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];  // vref / l could be too small a number
 #pragma unroll
                     for (int i = 0; i < E; ++i)
-                        dst[i] = (T)(l[r] == 0.0f ? 0.0f : o[r][i >> 1][i & 1] * f);
+                        dst[i] = (T)(l[r] == 0.0f ? 0.0f : o[r][i >> 1][i & 1] * f * vref);
                 } else {
 #pragma unroll
                     for (int i = 0; i < E; ++i)

@@ -50,6 +50,7 @@ constexpr int kPreRows = 256;      // rows of a unit
 constexpr int kPreThreads = 16 * 32;
 constexpr int kPreTok = 64;        // tokens of a step
 constexpr int kPreUnitCost = 3;    // a unit's beginning and end, in steps
+constexpr float kPreNoScale = -160.0f;  // log2 of a value scale of zero: below those of all numbers
 constexpr int kPreScaleRing = 8;   // more steps than the operand warps can be ahead of the softmax
 
 template <typename T, int D>
@@ -514,7 +515,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
             put(sk + st * S::kTileBytes, wk);
             if (cw == 0) {
                 const int ring = i % kPreScaleRing;
-                if (lane < G) scales[ring * G + lane] = make_float2(ks, vs < 1e-36f ? -120.0f : log2f(vs));  // NaN stays
+                if (lane < G) scales[ring * G + lane] = make_float2(ks, vs <= 0.0f ? kPreNoScale : log2f(vs));  // NaN stays
                 const unsigned m = __ballot_sync(0xffffffffu, lane < G && there);
                 if (lane == 0) valid[ring * 2] = m;
             }
@@ -712,7 +713,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 since = 1.0f;
             };
             const bool part_of_it = tile < tiles;
-            float m = -INFINITY, l = 0.0f, vl = -120.0f;  // vl: log2 of the reference value scale
+            float m = -INFINITY, l = 0.0f, vl = kPreNoScale;  // vl: log2 of the reference value scale
             // The products of the step before are in O.  Waited for in every step,
             // before its own weights are handed over: a wait knows only the
             // parity of a phase, so none may be passed over.
@@ -740,7 +741,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     // Largest score, group by group: the scale is applied to a group's
                     // maximum.  The loops over groups stay loops: unrolled, their code is
                     // larger than the schedulers' instruction caches.
-                    float top = -INFINITY, lvmax = -120.0f;
+                    float top = -INFINITY, lvmax = kPreNoScale;
                     auto largest = [&](auto masked) {
 #pragma unroll 1
                         for (int g0 = 0; g0 < G; g0 += 2) {
@@ -844,7 +845,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                 if (!ok) break;
                 tc_fence_after();
                 const bool whole_unit = cur.step == 0 && n == cur.steps;
-                const float vref = ex2(vl);
+                const float vref = exp2f(vl);  // the smallest numbers too
                 T* dst = (T*)a.out + (int64_t)(cur.q.row0 + (live ? j : 0)) * a.out_stride + col;
                 auto write = [&](int e0, const float (&v)[8]) {
                     if (!live) return;
@@ -863,7 +864,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                         for (int q = 0; q < 8; ++q) dst[e0 + q] = (T)v[q];
                     }
                 };
-                const float f = whole_unit ? (l == 0.0f ? 0.0f : vref / l) : vref;
+                const float f = whole_unit ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;  // vref / l could be too small a number
 #pragma unroll 1
                 for (int ch = 0; ch < D / 32; ++ch) {
                     uint32_t w[32];
@@ -894,7 +895,7 @@ kv8_prefill_kernel(Kv8 c, Kv8Attention a, float* __restrict__ pieces, int* __res
                     for (int b = 0; b < 4; ++b) {
                         float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = whole_unit && l == 0.0f ? 0.0f : __uint_as_float(w[b * 8 + e]) * f;
+                        for (int e = 0; e < 8; ++e) v[e] = whole_unit && l == 0.0f ? 0.0f : __uint_as_float(w[b * 8 + e]) * f * vref;
                         if (whole_unit) {
                             write(ch * 32 + b * 8, v);
                         } else {  // [element / 4][row][4]

@@ -281,3 +281,20 @@ def test_rope_cosines_are_exact_to_a_unit_and_a_half(lib, layout, odd):
     a, b = (got[:, :32], got[:, 32:]) if layout == "half" else (got[:, ::2], got[:, 1::2])
     off = max(np.abs(a - np.cos(angle)).max(), np.abs(b - np.sin(angle)).max())
     assert off <= 1.5 * 2.0 ** -24 + 2.0 ** -32, off * 2.0 ** 24
+
+
+# ------------------------------------------------------------ small numbers
+
+@pytest.mark.parametrize("heads,kv,page,d", [(8, 2, 32, 64), (4, 1, 16, 128)])
+@pytest.mark.parametrize("counts", [[1, 1], [90, 33]])
+@pytest.mark.parametrize("size", [1e-28, 1e-35, 1e-37])
+def test_attention_of_the_smallest_values(lib, heads, kv, page, d, counts, size):
+    """Value scales down to the smallest normal numbers, alone and next to larger ones."""
+    rng = np.random.default_rng(d + counts[0])
+    lens = [150, 40]
+    pool, table, q_start, q = attention_case(lib, rng, lens, counts, heads, kv, page, d, "i8", "f32", extra_rows=0)
+    for some in (slice(None), slice(None, None, 2)):
+        p = dict(pool, v_scale=pool["v_scale"].copy())
+        p["v_scale"][some] *= np.float32(size / 0.02)
+        assert p["v_scale"][np.isfinite(p["v_scale"])].min() >= 2.0 ** -126 or size == 1e-37
+        check_attention(lib, p, table, q_start, q, lens, "i8", "f32", max(counts))
