@@ -32,8 +32,10 @@ LC_DEV uint32_t e4m3x2(float a, float b) {
 // neighbour on the true value's side when it is inexact and its last bit is
 // even.  Rounding that to a code of 8 bits or fewer gives the code nearest to
 // the exact quotient, ties to even only where the quotient IS a tie (a plain
-// fp32 quotient can land on a tie that it is not).
+// fp32 quotient can land on a tie that it is not).  Small numbers are scaled up
+// first: beside a tie, x - q s can be half the smallest number there is.
 LC_DEV float quotient_odd(float x, float s) {
+    if (s < 0x1p-100f) x *= 0x1p64f, s *= 0x1p64f;  // |x| is below 2^9 s, or infinite
     const float q = __fdiv_rn(x, s);
     if (!(fabsf(q) < 1024.0f)) return q;  // saturates below; infinities stay themselves
     const float r = __fmaf_rn(-q, s, x);

@@ -298,3 +298,30 @@ def test_attention_of_the_smallest_values(lib, heads, kv, page, d, counts, size)
         p["v_scale"][some] *= np.float32(size / 0.02)
         assert p["v_scale"][np.isfinite(p["v_scale"])].min() >= 2.0 ** -126 or size == 1e-37
         check_attention(lib, p, table, q_start, q, lens, "i8", "f32", max(counts))
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("k", [2 ** 17 + 1, 2 ** 19 + 5, 2 ** 20 + 1, 2 ** 21 + 3, 2 ** 22 + 7])
+def test_append_rounds_quotients_of_the_smallest_numbers(lib, fmt, k):
+    """A scale of k smallest steps u = 2^-149, and rows half a step beside the
+    ties of the quotient: x - (c + 1/2) s = +-u / 2 is no fp32 number."""
+    limit = int(ref.LIMIT[fmt])
+    x = []
+    for c in range(1, 127):
+        for m in (((2 * c + 1) * k + 1) // 2, ((2 * c + 1) * k - 1) // 2, (2 * c + 1) * k // 2 + 1):
+            if m < 2 ** 24 and m < limit * k:
+                x += [m, -m]
+    x = np.resize(np.ldexp(np.array(x, np.float64), -149), (128, 1, 64)).astype(np.float32)
+    x[0, 0, 0] = np.ldexp(float(limit) * k, -149)
+    assert x[0, 0, 0] / np.float32(limit) == np.float32(np.ldexp(float(k), -149))
+    rng = np.random.default_rng(9)
+    pool = make_pool(rng, 1, 1, 128, 64, fmt)
+    cache, t = cache_of(lib, pool, fmt)
+    want = {n: v.copy() for n, v in pool.items()}
+    slots = np.arange(128, dtype=np.int32)
+    ref.append(want["k"], want["k_scale"], x, slots, fmt)
+    cache.append(dev(x), dev(x), dev(slots))
+    sync()
+    assert np.array_equal(t["k_scale"].cpu().numpy(), want["k_scale"])
+    got = t["k"].cpu().numpy()
+    assert ((got == want["k"]) | ((got & 0x7F == 0) & (want["k"] & 0x7F == 0))).all()
