@@ -95,8 +95,9 @@ LC_DEV float top4(float4 v, float top) {
     return top;
 }
 
-// Four codes under scale s, inv = 1 / s rounded; byte i is value i.
-template <int FMT>
+// Four codes under scale s, inv = 1 / s rounded; byte i is value i.  SMALL as in
+// quotient_odd: half rows that are not zero make no scale below 2^-33.
+template <int FMT, bool SMALL>
 LC_DEV uint32_t encode4(float4 v, float s, float inv) {
     const float x[4] = {v.x, v.y, v.z, v.w};
     uint32_t w = 0;
@@ -130,7 +131,7 @@ LC_DEV uint32_t encode4(float4 v, float s, float inv) {
     if (!sure || !(inv < INFINITY) || !(s > 0.0f)) {
         w = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= kv8_encode<FMT>(x[i], s) << (8 * i);
+        for (int i = 0; i < 4; ++i) w |= kv8_encode<FMT, SMALL>(x[i], s) << (8 * i);
     }
     return w;
 }
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_ap
 #pragma unroll
                     for (int i = 0; i < kAppendHold; ++i) {
                         const int k = at0 + i * step;
-                        if (k < len) *reinterpret_cast<uint32_t*>(codes + (off + k) * D) = encode4<FMT>(v[i].get(), now, inv);
+                        if (k < len) *reinterpret_cast<uint32_t*>(codes + (off + k) * D) = encode4<FMT, sizeof(T) == 4>(v[i].get(), now, inv);
                     }
                     held = now;
                     row += len;

@@ -32,10 +32,12 @@ LC_DEV uint32_t e4m3x2(float a, float b) {
 // neighbour on the true value's side when it is inexact and its last bit is
 // even.  Rounding that to a code of 8 bits or fewer gives the code nearest to
 // the exact quotient, ties to even only where the quotient IS a tie (a plain
-// fp32 quotient can land on a tie that it is not).  Small numbers are scaled up
-// first: beside a tie, x - q s can be half the smallest number there is.
+// fp32 quotient can land on a tie that it is not).  SMALL: s may be below 2^-100;
+// such numbers are scaled up first, for beside a tie x - q s can be half the
+// smallest number there is.
+template <bool SMALL>
 LC_DEV float quotient_odd(float x, float s) {
-    if (s < 0x1p-100f) x *= 0x1p64f, s *= 0x1p64f;  // |x| is below 2^9 s, or infinite
+    if (SMALL && s < 0x1p-100f) x *= 0x1p64f, s *= 0x1p64f;  // |x| is below 2^9 s, or infinite
     const float q = __fdiv_rn(x, s);
     if (!(fabsf(q) < 1024.0f)) return q;  // saturates below; infinities stay themselves
     const float r = __fmaf_rn(-q, s, x);
@@ -55,10 +57,10 @@ LC_DEV uint32_t kv8_round(float q) {
 
 // x under scale s: NaN becomes 0, infinities the end of the range, and a zero
 // scale gives code 0.
-template <int FMT>
+template <int FMT, bool SMALL>
 LC_DEV uint32_t kv8_encode(float x, float s) {
     if (!(s > 0.0f) || x != x) return 0;
-    return kv8_round<FMT>(quotient_odd(x, s));
+    return kv8_round<FMT>(quotient_odd<SMALL>(x, s));
 }
 
 // A held code under a grown scale: round(code * s_old / s_new).  The product
