@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
+from paged_bounds import sums_bound
 from test_paged_gpu import attention_case, cache_of, check_attention, dev, exact_on_gpu, lib, make_pool, sync  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -81,24 +82,6 @@ def test_pages_step_of_batches_whose_sums_need_48_kb(lib, n):
 
 # ---------------------------------------------------------------- long sums
 
-def sums_bound(size, weight, n, d, chain):
-    """Error of fp32 rows that does not grow with n as a chain of truncated sums
-    would.  Scores: each of the d products is off by 2^-22 of itself (rows in
-    two f16), the d / 8 sums of tensor-core products by a unit 2^-23 each, the
-    scales by 4 more: ds = (d / 8 + 6) 2^-23 max_t sum |q k| scale, a weight by
-    a factor exp(+-2 ds).  16 units for the exponential, the weight's two f16
-    and a step's own products; `chain` units where that many products are added
-    on the tensor cores before a sum in round-to-nearest.  The sums themselves:
-    the N additions of round-to-nearest are off by at most half a unit of the
-    result each, in either direction; by Hoeffding their sum passes
-    4 sqrt(N) halves once in 1500 times if each were off by all of it, and
-    they are off by a third of that (a running sum is smaller than the result,
-    a rounding smaller than half a unit).  N: n / 8 for the normaliser, n / 16
-    for the weighted values."""
-    ds = (d / 8 + 6) * 2.0 ** -23 * size
-    return weight * (2 * ds + (16 + chain) * 2.0 ** -23 + 4 * 2.0 ** -24 * (math.sqrt(n / 8) + math.sqrt(n / 16)))
-
-
 def one_sign(lib, rng, lens, counts, heads, kv, page, d, fmt):
     """Values of one sign and small scores: what every sum loses, it loses in one direction."""
     pool, table, q_start, q = attention_case(lib, rng, lens, counts, heads, kv, page, d, fmt, "f32", extra_rows=0)
@@ -128,7 +111,7 @@ def test_attention_of_long_decodes_does_not_drift(lib, fmt, heads, d, length, co
 
 @pytest.mark.parametrize("fmt", ["i8", "e4m3"])
 @pytest.mark.parametrize("heads,kv,page,d", [(8, 2, 64, 64), (8, 2, 128, 128)])
-@pytest.mark.parametrize("length", [200, 4096, 16384])
+@pytest.mark.parametrize("length", [200, 4096, 65536])
 def test_attention_of_long_prompts_does_not_drift(lib, fmt, heads, kv, page, d, length):
     """At most 32 products of head size 64, 64 of head size 128, are added on the
     tensor cores before a sum in round-to-nearest."""
