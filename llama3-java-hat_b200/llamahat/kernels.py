@@ -119,7 +119,18 @@ def _rows(buf, writable: bool = False):
 
 
 class Accelerator:
-    """Device handle (hat.Accelerator's role): one lc_context per instance."""
+    """Device handle (hat.Accelerator's role): one lc_context per instance.
+
+    Calls whose buffers are all CUDA tensors only enqueue on the context's own
+    stream, which waits for no other stream, and return.  So a program makes the
+    tensors of a call, uses its results and frees them on that stream, where
+    torch's allocator then sees all uses of their memory too:
+
+        with torch.cuda.stream(torch.cuda.ExternalStream(acc.stream)):
+            ...
+
+    or orders the streams by events and keeps the tensors until the calls are
+    done, or calls synchronize() (which also reports device-side errors)."""
 
     def __init__(self, device: int = 0):
         lib = _lib.load()
@@ -318,7 +329,8 @@ class CudaRoPE(_CudaKernel, IRoPE):
     def apply_scaled(self, x, out, positions, config: RopeConfig, transpose: bool = False) -> None:
         """Rows [rows, heads, head_dim] (F32 or F16) at their positions under a
         RopeConfig (see lc_rope_apply); out may be x.  transpose: the gradient
-        of x from that of out.  Rows at negative positions are left as they are."""
+        of x from that of out.  Rows at negative positions are left as they are.
+        CUDA tensors: on the accelerator's stream (see Accelerator)."""
         xa, rows, width, xs, dt = _rows(x)
         if out is x:
             ya, ys = xa, xs
@@ -336,7 +348,8 @@ class CudaRoPE(_CudaKernel, IRoPE):
 
 
 class CudaPages(_CudaKernel):
-    """Page bookkeeping of one serving step (see lc_pages_step)."""
+    """Page bookkeeping of one serving step (see lc_pages_step), on the
+    accelerator's stream (see Accelerator)."""
 
     def step(self, lens, n_new, table, free_list, free_count, page_size: int, lens_out, q_start, slots, positions,
              seq_ids, free_count_out, status) -> None:
@@ -359,7 +372,8 @@ class PagedKV8(_CudaKernel):
     """A paged KV cache in 8 bits (see lc_kv8): codes k, v [n_pages, n_kv_heads,
     page_size, head_dim] (uint8, int8 or float8_e4m3fn) and scales k_scale,
     v_scale [n_pages, n_kv_heads] (float32), CUDA tensors that this object keeps
-    alive and the caller owns."""
+    alive and the caller owns.  Its calls run on the accelerator's stream (see
+    Accelerator): what makes or reads these tensors elsewhere is ordered against it."""
 
     FORMATS = {"i8": 0, "e4m3": 1}
 

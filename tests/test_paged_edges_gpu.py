@@ -308,3 +308,46 @@ def test_append_rounds_quotients_of_the_smallest_numbers(lib, fmt, k):
     assert np.array_equal(t["k_scale"].cpu().numpy(), want["k_scale"])
     got = t["k"].cpu().numpy()
     assert ((got == want["k"]) | ((got & 0x7F == 0) & (want["k"] & 0x7F == 0))).all()
+
+
+# ------------------------------------------------------------------ streams
+
+def test_a_step_on_the_contexts_stream_needs_no_synchronisation(lib):
+    """As Accelerator says: tensors made, used and freed on the context's stream.
+    Every step's tensors are new, and freed while the calls that read them are
+    still queued; a slow kernel before each keeps them so."""
+    L = lib[0]
+    acc = L.Accelerator(0)
+    rope = L.CudaKernelFactory().createRoPE(acc)
+    cfg = L.RopeConfig.llama32()
+    rng = np.random.default_rng(5)
+    kv, heads, d, n = 2, 8, 64, 40
+    k, v, q = (dev(rng.standard_normal((6, n, h, d)).astype(np.float32)) for h in (kv, kv, heads))
+    busy = torch.randn(4096, 4096, device="cuda")
+
+    def steps(between):
+        t = [torch.zeros(8, kv, 32, d, dtype=torch.uint8, device="cuda") for _ in "kv"] + [torch.zeros(8, kv, device="cuda") for _ in "kv"]
+        cache = L.PagedKV8(*t, acc=acc)
+        table = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+        outs = []
+        for i in range(6):
+            between(True)
+            at = torch.arange(i * n, (i + 1) * n, dtype=torch.int32, device="cuda")
+            a, b, out = k[i] * 2.0, q[i] * 0.5, torch.empty_like(q[i])
+            lens, start = torch.full((1,), (i + 1) * n, dtype=torch.int32, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda")
+            between(False)
+            rope.apply_scaled(a, a, at, cfg)
+            rope.apply_scaled(b, b, at, cfg)
+            cache.append(a, v[i], at)
+            cache.attention(b, out, start, lens, table, max_q=n)
+            between(False)
+            outs.append(out * 1.0)
+        return outs
+
+    want = steps(lambda first: sync())
+    sync()
+    with torch.cuda.stream(torch.cuda.ExternalStream(acc.stream)):
+        got = steps(lambda first: torch.mm(busy, busy) if first else None)
+    sync()
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
