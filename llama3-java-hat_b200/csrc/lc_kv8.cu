@@ -136,6 +136,8 @@ LC_DEV uint32_t encode4(float4 v, float s, float inv) {
     return w;
 }
 
+// Three CTAs of half rows on an SM, two of fp32 rows: what a lane keeps is 32 or
+// 64 registers.  The compiler spills with teams (32 to 124 bytes).
 template <typename T, int FMT, int D, bool TEAMS>
 __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) kv8_append_kernel(Kv8 c, Kv8Rows r, int window, int windows, int team_size) {
     constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows at a time

@@ -17,11 +17,11 @@
 //
 // Sums.  The tensor cores' own fp32 sums lose up to one unit of the last place,
 // always toward zero, at every product that is added: over a unit of 65536
-// positions 5.5e-4 of the result where all values have one sign.  So a product of
-// weights and values begins at zero, its hi and lo sums meet, and are added to
-// the unit's in round-to-nearest.  That also halves the accumulators' registers
-// (decode of 64 sequences of 1 to 8191 positions, d 64 and fp32, 60.3 against
-// 60.7 us; d 128 112.5 against 106.8).
+// positions 4.3e-4 of the result where all values have one sign.  So a product
+// of weights and values begins at zero, its hi and lo sums meet, and are added
+// to the unit's in round-to-nearest (4.4e-6).  That also halves the
+// accumulators' registers: 64 sequences of 1 to 8191 positions, fp32, take 60.7
+// us at head size 64 (60.3 with the tensor cores' sums) and 106.8 at 128 (112.5).
 //
 // Softmax.  In powers of two, with a running maximum that is only moved when
 // a score passes it by more than 1; p is held as 2^(x - m + 12), times the
@@ -29,12 +29,12 @@
 // below 2^15 and leaves 37 bits between the largest weight and the smallest
 // step of the lo half.
 //
-// Work.  A step is 32 tokens of one (sequence, kv head, 4 or 8 rows); all steps of
-// the call form one line, cut into equal pieces, one per warp, so ragged
-// lengths leave no warp idle.  A unit (all steps of those rows) that one warp
-// covers is written at once; pieces of a unit are joined first within the
-// CTA, then by the last CTA to finish, always in the order of the line, so
-// the result does not depend on timing.
+// Work.  A step is 4 KB of codes, 32 tokens of head size 64 or 16 of 128, of
+// one (sequence, kv head, 4 or 8 rows); all steps of the call form one line, cut
+// into equal pieces, one per warp, so ragged lengths leave no warp idle.  A unit
+// (all steps of those rows) that one warp covers is written at once; pieces of
+// a unit are joined first within the CTA, then by the last CTA to finish, always
+// in the order of the line, so the result does not depend on timing.
 //
 // Each warp streams its own pages through a ring in shared memory with 16-byte
 // cp.async, swizzled so that the fragment loads are free of bank conflicts,
@@ -216,7 +216,7 @@ kv8_decode_kernel(Kv8 c, Kv8Attention a, float* __restrict__ ws, int* __restrict
     griddep_wait();
 
     // The queries come to L2 while the line is laid out.
-    if (a.q_stride >= 0) {
+    {
         const int64_t bytes = (int64_t)a.n_heads * D * sizeof(T);  // of a row, 128 at a time
         const int per = (int)((bytes + 127) / 128);
         for (int64_t i = (int64_t)blockIdx.x * blockDim.x + tid; i < (int64_t)a.rows * per; i += (int64_t)gridDim.x * blockDim.x)

@@ -67,8 +67,9 @@ struct PreShape {
     static constexpr int kPieceFloats = kPreRows * (D + 2);
     // Registers of the softmax, operand and MMA warpgroups after the split; their
     // sum over 128 threads each must not pass the launch's (checked on the host).
-    // With 168, 120 and 56 the compiler spills (4096 fp32 queries, 32 heads: 269
-    // against 255 us; f16 of head size 128, twice the codes: 310 against 280).
+    // With 168, 120 and 56 the compiler spills more (4096 fp32 queries, 32 heads:
+    // 269 against 255 us; f16 of head size 128, twice the codes: 310 against 280);
+    // with these, fp32 of head size 128 alone (144 bytes stored, 340 loaded).
     static constexpr int kRegsSoftmax = 144, kRegsOperand = 128, kRegsMma = 96;
     static constexpr int kRegsLaunch = (2 * kRegsSoftmax + kRegsOperand + kRegsMma + 3) / 4;
     // Tensor memory: two buffers of S for each tile, so that the next step's
