@@ -48,6 +48,16 @@ cudaError_t kv8_attention_clear(void* ws, int num_sms, cudaStream_t st) {
     return cudaMemsetAsync((uint8_t*)ws + decode_ws(num_sms), 0, kv8_prefill_counter_bytes(num_sms), st);
 }
 
+// Rows of a unit, by the rows that share a kv head's codes at most.  More rows
+// share one reading of the codes; units of 8 instead of 4 cost registers and, in
+// short sequences, idle warps.  us, 4 kv heads, head size 64 fp32 / 128 f16:
+//   8 rows, units of 8 | 4:   1 x 131071 positions 34 | 36 / 52 | 61,
+//                             64 x 1..8191 52 | 63 / 94 | 111, 64 x 1..500 19 | 16 / 27 | 23
+//   16 rows, of 256 | 8:      160 | 48 / 176 | 79, 233 | 87 / 250 | 159, 48 | 22 / 51 | 34
+//   32 rows, of 256 | 8:      159 | 76 / 175 | 136, 234 | 154 / 251 | 298, 48 | 28 / 51 | 51
+//   64 rows, of 256 | 8:      160 | 132 / 176 | 252, (2 kv heads) 130 | 153 / 138 | 298, 33 | 28 / 35 | 51
+// So up to 16 rows, at head size 64 up to 32, units of 8 would be the faster ones:
+// their line of work in 32 bits is shorter by as much, and calls that fit now would not.
 static int unit_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : kPreRows; }
 
 bool kv8_attention_fits(const Kv8& c, const Kv8Attention& a) {

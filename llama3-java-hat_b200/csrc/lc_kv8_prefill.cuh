@@ -9,11 +9,12 @@
 // The codes are exact in f16, so scales enter only where scores leave tensor
 // memory: the key scale of a 16-token group in c, the value scale (over a
 // running reference, as its logarithm) in b; the sum takes it out again.
-// fp32 rows are split into f16 hi + lo under a power-of-two row scale, at the
-// price of twice the products; f16 rows are exact.  P is split the same way for
-// both: rounded to one f16 it is off by 2^-12 of each weight, which adds as much
-// error as the rounding of an f16 result itself (1.4 times its norm in all; six
-// chunks of f16 rows over 500 to 4000 positions 133 against 145 us with the split).
+// fp32 rows are split into f16 hi + lo under a power-of-two row scale (22 bits),
+// at the price of twice the products; f16 rows are exact.  P is split the same
+// way for both: rounded to one f16 it is off by 2^-12 of each weight, which adds
+// as much error as the rounding of an f16 result itself (1.4 times its norm in
+// all; six chunks of f16 rows over 500 to 4000 positions 133 against 145 us with
+// the split).
 //
 // The tensor cores' fp32 sums lose up to one unit of the last place, always
 // toward zero, at every product that is added; over thousands of tokens that
