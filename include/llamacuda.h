@@ -320,9 +320,10 @@ int lc_kv8_read(lc_context* ctx, const lc_kv8* kv, void* k, void* v, int64_t row
  * query that sees nothing gives zeros; rows behind q_start[n_seqs] are left as
  * they are; pages outside the cache are not seen.  Values may be as small as
  * numbers are, and up to 2^80 in size: their weighted sums are held
- * unnormalised.  max_q: the largest number of queries of a sequence, which
- * chooses the kernel (results hold for any value).  n_seqs <= 4096.  lens,
- * tables and q_start are read on the device; q_start must ascend. */
+ * unnormalised; a page's values are good to 2^-36 of the largest value scale
+ * that the sequence has.  max_q: the largest number of queries of a sequence,
+ * which chooses the kernel (results hold for any value).  n_seqs <= 4096.
+ * lens, tables and q_start are read on the device; q_start must ascend. */
 int lc_kv8_attention(lc_context* ctx, const lc_kv8* kv, const void* q, void* out, int64_t q_stride, int64_t out_stride,
                      int32_t dtype, int32_t rows, const int32_t* q_start, const int32_t* kv_lens, const int32_t* table,
                      int32_t table_stride, int32_t n_seqs, int32_t max_q, int32_t n_heads, float scale);
