@@ -328,6 +328,88 @@ int lc_kv8_attention(lc_context* ctx, const lc_kv8* kv, const void* q, void* out
                      int32_t dtype, int32_t rows, const int32_t* q_start, const int32_t* kv_lens, const int32_t* table,
                      int32_t table_stride, int32_t n_seqs, int32_t max_q, int32_t n_heads, float scale);
 
+/* ------------------------------------------------------ 4-bit weights ---- *
+ * Weight matrices in 4 bits under one scale per row and group of columns, and
+ * their products.  No counterpart in the reference, whose weights are F16 or
+ * F32 (H/WeightStorageMode.java); the product takes the place of IGEMV.apply
+ * (K/IGEMV.java:34-68).  Row buffers are F32 or F16 (dtype 0 or 1), row i at
+ * i * stride elements, host or device memory; the weights are device memory.
+ * With device memory throughout, the calls only enqueue on the context's
+ * stream and can be captured in a CUDA graph; they keep nothing between calls
+ * but the weights.  Threads may share a context: these calls and those of the
+ * sections on the paged cache and on log probabilities take turns. */
+
+/* W [rows][cols] in device memory that the caller owns:
+ *   W[r][c] = scale[r][c / group] * (code[r][c] - zero[r][c / group])
+ * with codes 0..15, F16 scales and zero points 0..15 (zeros NULL: 8
+ * throughout); the last group of a row may be short.  codes, scales and zeros
+ * are held in the library's own order: lc_w4_sizes gives their sizes,
+ * lc_w4_quantize or lc_w4_pack fills them, all 16-byte aligned. */
+typedef struct lc_w4 {
+    void* codes;
+    uint16_t* scales;
+    uint8_t* zeros;  /* or NULL */
+    int32_t rows, cols;
+    int32_t group;   /* 32, 64 or 128 columns */
+    int32_t reserved[3];
+} lc_w4;
+
+/* Bytes of codes, and the number of scales (and of zero points, a byte each). */
+int lc_w4_sizes(int32_t rows, int32_t cols, int32_t group, int64_t* code_bytes, int64_t* n_scales);
+
+/* Fills w from rows of values [rows][cols].  Of each group, over its finite
+ * values, without zero points: scale = max |x| / 7 and code = 8 + x / scale,
+ * at least 1; with them: low = min(0, min x), high = max(0, max x),
+ * scale = (high - low) / 15, zero = -low / scale, code = zero + x / scale.
+ * Scales are quotients in 64 bits, rounded to F32 and then to F16, 65504 at most; x / scale
+ * and -low / scale are rounded to the nearest whole number of the exact
+ * quotient, ties to even, codes and zero points end at 0 and 15.  A group
+ * whose scale is 0 holds zeros; NaN is held as 0, infinities as the last code. */
+int lc_w4_quantize(lc_context* ctx, const lc_w4* w, const void* values, int64_t stride, int32_t dtype);
+
+/* Fills w from codes [rows][(cols + 1) / 2], the lower column of each byte in
+ * its low half, scales [rows][groups] (any F16 numbers) and zero points
+ * [rows][groups] (NULL as w->zeros is; the low four bits count), groups =
+ * ceil(cols / group). */
+int lc_w4_pack(lc_context* ctx, const lc_w4* w, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros);
+
+/* values [rows][cols] = W, rounded once to dtype. */
+int lc_w4_read(lc_context* ctx, const lc_w4* w, void* values, int64_t stride, int32_t dtype);
+
+/* y[b] = residual[b] + W x[b] for b < batch (residual NULL: 0): rows x [batch]
+ * [cols], y and residual [batch][rows], all of dtype.  residual may be y (with
+ * its stride); no other buffers may overlap.  batch 1: the GEMV of a decode
+ * step; more: sequences or the tokens of a prompt.  Codes enter as whole
+ * numbers, F32 rows as two F16 under a power-of-two row scale (2^-22 relative
+ * to the row's largest), F16 rows as they are, scales as they are; sums are
+ * fp32, y is rounded once.  Results of a row do not depend on the others.  A
+ * row of x with a NaN or an infinity gives NaN, infinities or numbers in its
+ * own row of y only. */
+int lc_w4_product(lc_context* ctx, const lc_w4* w, const void* x, int64_t x_stride, void* y, int64_t y_stride,
+                  const void* residual, int64_t residual_stride, int32_t batch, int32_t dtype);
+
+/* ---------------------------------------------------- log probabilities ---- *
+ * What a server answers next to its tokens, from rows of logits [rows][vocab]
+ * (F32 or F16, dtype 0 or 1, row i at i * stride elements).  No counterpart in
+ * the reference, which takes the argmax (H/LlamaInference.java:252-262).  With
+ * p = softmax(scale * x) of a row:
+ *   token_logprobs[i]  ln p of tokens[i]
+ *   token_ranks[i]     how many tokens come before tokens[i], larger logits
+ *                      first, equal ones by index (0: it is the argmax)
+ *   entropy[i]         -sum p ln p
+ *   top_ids, top_logprobs [rows][top_k]  the first top_k (0..32) tokens in that
+ *                      order and their ln p; id -1 and -inf behind the vocabulary
+ * Each output may be NULL.  tokens NULL: no token outputs; a token outside the
+ * vocabulary (a padded position) has ln p 0 and rank -1.  Logits of -inf are
+ * masked; a row of them alone gives ln p -inf and entropy 0.  A row with NaN or
+ * +inf gives NaN for every ln p and the entropy; in the order NaN counts as
+ * -inf.  scale (1 / temperature) is positive and finite.  Buffers may be host
+ * or device memory; with device memory throughout the call only enqueues, can
+ * be captured and keeps nothing.  Turns as in the section before. */
+int lc_logprobs(lc_context* ctx, const void* logits, int64_t stride, int32_t dtype, int32_t rows, int32_t vocab,
+                float scale, const int32_t* tokens, float* token_logprobs, int32_t* token_ranks, float* entropy,
+                int32_t top_k, int32_t* top_ids, float* top_logprobs);
+
 /* ------------------------------------------------------------- model ---- */
 typedef struct lc_config {
     int32_t dim;        /* HIDDEN_SIZE 2048          (H/LlamaModel.java:30) */

@@ -24,6 +24,7 @@
 #include "lc_attention.cuh"
 #include "lc_internal.h"
 #include "lc_paged.h"
+#include "lc_w4.h"
 
 using namespace lc;
 
@@ -953,6 +954,159 @@ extern "C" int lc_kv8_attention(lc_context* c, const lc_kv8* kv, const void* q, 
             c->kv8_ws = ws;
         }
         return s.finish(launch_kv8_attention(view, a, c->sms, c->kv8_ws, c->d_err, c->stream));
+    });
+}
+
+// ------------------------------------------------------- 4-bit weights ----
+
+namespace {
+
+int w4_shape(int32_t rows, int32_t cols, int32_t group, W4* out) {
+    if (rows <= 0 || cols <= 0) return fail(LC_ERR_INVALID_ARG, "rows=%d cols=%d", rows, cols);
+    if (group != 32 && group != 64 && group != 128) return fail(LC_ERR_UNSUPPORTED, "group %d (32, 64 or 128)", group);
+    if (rows > kMaxCount || cols > kMaxCount) return fail(LC_ERR_UNSUPPORTED, "rows=%d cols=%d (up to %d)", rows, cols, kMaxCount);
+    memset(out, 0, sizeof(*out));
+    out->rows = rows;
+    out->cols = cols;
+    out->group = group;
+    out->tiles = (rows + kW4Rows - 1) / kW4Rows;
+    out->blocks = (cols + kW4Cols - 1) / kW4Cols;
+    return LC_OK;
+}
+
+// Checks a weight descriptor and fills the kernels' view of it.
+int w4_view(lc_context* c, const lc_w4* w, W4* out) {
+    if (!w) return fail(LC_ERR_INVALID_ARG, "weights are NULL");
+    if (int rc = w4_shape(w->rows, w->cols, w->group, out)) return rc;
+    Stager s(c);
+    const void* p[3] = {w->codes, w->scales, w->zeros};
+    for (int i = 0; i < 3; ++i) {
+        if (i == 2 && !p[i]) continue;  // no zero points
+        int rc = LC_OK;
+        if (!p[i] || !s.is_device(p[i], &rc)) return fail(LC_ERR_INVALID_ARG, "codes, scales and zero points must be device memory");
+        if (rc != LC_OK) return rc;
+        if ((uintptr_t)p[i] & 15) return fail(LC_ERR_INVALID_ARG, "codes, scales and zero points must be 16-byte aligned");
+    }
+    out->codes = (uint8_t*)w->codes;
+    out->scales = w->scales;
+    out->zeros = w->zeros;
+    return LC_OK;
+}
+
+int w4_values(lc_context* c, const lc_w4* w, void* values, int64_t stride, int32_t dtype, bool quantize) {
+    return on_device(c, [&]() -> int {
+        W4 view;
+        if (int rc = w4_view(c, w, &view)) return rc;
+        const int elem = row_elem(dtype);
+        if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
+        if (stride < 0 || (!quantize && view.rows > 1 && stride < view.cols))
+            return fail(LC_ERR_INVALID_ARG, "stride=%lld of rows of %d", (long long)stride, view.cols);
+        Stager s(c);
+        // What lies between the rows of a host buffer that is read into stays as it is: it travels both ways.
+        void* d = s.arg(values, rows_bytes(view.rows, stride, view.cols, elem), quantize ? kIn : stride == view.cols ? kOut : kInOut);
+        if (s.status != LC_OK) return s.status;
+        return s.finish(quantize ? launch_w4_quantize(view, d, stride, dtype, c->sms, c->stream)
+                                 : launch_w4_read(view, d, stride, dtype, c->sms, c->stream));
+    });
+}
+
+}  // namespace
+
+extern "C" int lc_w4_sizes(int32_t rows, int32_t cols, int32_t group, int64_t* code_bytes, int64_t* n_scales) {
+    W4 w = {};
+    if (int rc = w4_shape(rows, cols, group, &w)) return rc;
+    const int64_t blocks = (int64_t)w.tiles * w.blocks;
+    if (code_bytes) *code_bytes = blocks * kW4BlockBytes;
+    if (n_scales) *n_scales = blocks * (kW4Rows * kW4Cols / group);
+    return LC_OK;
+}
+
+extern "C" int lc_w4_quantize(lc_context* c, const lc_w4* w, const void* values, int64_t stride, int32_t dtype) {
+    return w4_values(c, w, const_cast<void*>(values), stride, dtype, true);
+}
+
+extern "C" int lc_w4_read(lc_context* c, const lc_w4* w, void* values, int64_t stride, int32_t dtype) {
+    return w4_values(c, w, values, stride, dtype, false);
+}
+
+extern "C" int lc_w4_pack(lc_context* c, const lc_w4* w, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros) {
+    return on_device(c, [&]() -> int {
+        W4 view;
+        if (int rc = w4_view(c, w, &view)) return rc;
+        if (!zeros != !view.zeros) return fail(LC_ERR_INVALID_ARG, "zero points on one side only");
+        const size_t groups = (size_t)view.rows * ((view.cols + view.group - 1) / view.group);
+        Stager s(c);
+        auto* dc = (const uint8_t*)s.arg(codes, (size_t)view.rows * ((view.cols + 1) / 2), kIn);
+        auto* ds = (const uint16_t*)s.arg(scales, groups * 2, kIn);
+        auto* dz = zeros ? (const uint8_t*)s.arg(zeros, groups, kIn) : nullptr;
+        if (s.status != LC_OK) return s.status;
+        return s.finish(launch_w4_pack(view, dc, ds, dz, c->sms, c->stream));
+    });
+}
+
+extern "C" int lc_w4_product(lc_context* c, const lc_w4* w, const void* x, int64_t x_stride, void* y, int64_t y_stride,
+                             const void* residual, int64_t residual_stride, int32_t batch, int32_t dtype) {
+    return on_device(c, [&]() -> int {
+        W4 view;
+        if (int rc = w4_view(c, w, &view)) return rc;
+        const int elem = row_elem(dtype);
+        if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
+        if (batch < 0 || x_stride < 0 || (batch > 1 && y_stride < view.rows) || (residual && residual_stride < 0))
+            return fail(LC_ERR_INVALID_ARG, "batch=%d x_stride=%lld y_stride=%lld residual_stride=%lld", batch, (long long)x_stride,
+                        (long long)y_stride, (long long)residual_stride);
+        if (batch > kMaxCount) return fail(LC_ERR_UNSUPPORTED, "batch=%d (up to %d)", batch, kMaxCount);
+        const bool in_place = residual == y;
+        if (in_place && batch > 1 && residual_stride != y_stride) return fail(LC_ERR_INVALID_ARG, "in place, the strides must be equal");
+        if (batch == 0) return LC_OK;
+        Stager s(c);
+        W4Product p;
+        p.x = s.arg(x, rows_bytes(batch, x_stride, view.cols, elem), kIn);
+        p.y = s.arg(y, rows_bytes(batch, y_stride, view.rows, elem), in_place || y_stride != view.rows ? kInOut : kOut);
+        p.residual = in_place ? p.y : residual ? s.arg(residual, rows_bytes(batch, residual_stride, view.rows, elem), kIn) : nullptr;
+        if (s.status != LC_OK) return s.status;
+        p.x_stride = x_stride;
+        p.y_stride = y_stride;
+        p.residual_stride = residual_stride;
+        p.batch = batch;
+        p.dtype = dtype;
+        return s.finish(launch_w4_product(view, p, c->sms, c->stream));
+    });
+}
+
+// --------------------------------------------------- log probabilities ----
+
+extern "C" int lc_logprobs(lc_context* c, const void* logits, int64_t stride, int32_t dtype, int32_t rows, int32_t vocab,
+                           float scale, const int32_t* tokens, float* token_logprobs, int32_t* token_ranks, float* entropy,
+                           int32_t top_k, int32_t* top_ids, float* top_logprobs) {
+    return on_device(c, [&]() -> int {
+        const int elem = row_elem(dtype);
+        if (!elem) return fail(LC_ERR_INVALID_ARG, "dtype %d (0 = F32, 1 = F16)", dtype);
+        if (rows < 0 || vocab <= 0 || stride < 0) return fail(LC_ERR_INVALID_ARG, "rows=%d vocab=%d stride=%lld", rows, vocab, (long long)stride);
+        if (rows > kMaxCount || vocab > kMaxCount) return fail(LC_ERR_UNSUPPORTED, "rows=%d vocab=%d (up to %d)", rows, vocab, kMaxCount);
+        if (!(scale > 0.0f) || isinf(scale)) return fail(LC_ERR_INVALID_ARG, "scale=%g", scale);
+        if (top_k < 0 || top_k > kLogprobsMaxTop) return fail(LC_ERR_INVALID_ARG, "top_k=%d (0..%d)", top_k, kLogprobsMaxTop);
+        if (!tokens && (token_logprobs || token_ranks)) return fail(LC_ERR_INVALID_ARG, "token outputs without tokens");
+        if (!top_k && (top_ids || top_logprobs)) return fail(LC_ERR_INVALID_ARG, "top outputs with top_k=0");
+        if (rows == 0) return LC_OK;
+        Stager s(c);
+        Logprobs p;
+        memset(&p, 0, sizeof(p));
+        const size_t n = (size_t)rows * 4, nk = n * top_k;
+        p.x = s.arg(logits, rows_bytes(rows, stride, vocab, elem), kIn);
+        if (tokens) p.tokens = (const int32_t*)s.arg(tokens, n, kIn);
+        if (token_logprobs) p.token_logprobs = (float*)s.arg(token_logprobs, n, kOut);
+        if (token_ranks) p.token_ranks = (int32_t*)s.arg(token_ranks, n, kOut);
+        if (entropy) p.entropy = (float*)s.arg(entropy, n, kOut);
+        if (top_ids) p.top_ids = (int32_t*)s.arg(top_ids, nk, kOut);
+        if (top_logprobs) p.top_logprobs = (float*)s.arg(top_logprobs, nk, kOut);
+        if (s.status != LC_OK) return s.status;
+        p.stride = stride;
+        p.dtype = dtype;
+        p.rows = rows;
+        p.vocab = vocab;
+        p.top = top_ids || top_logprobs ? top_k : 0;
+        p.scale = scale;
+        return s.finish(launch_logprobs(p, c->sms, c->stream));
     });
 }
 

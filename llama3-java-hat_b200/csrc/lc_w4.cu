@@ -1,0 +1,369 @@
+// lc_w4.cu -- 4-bit weights: quantising rows of values, packing codes that a
+// checkpoint holds, and reading values back.  Layout: lc_w4.h.
+//
+// A warp has a block of 16 rows x 128 columns, a lane 16 columns of two rows in
+// each half of it, as the layout wants them; a group's largest value is then a
+// maximum over 1, 3 or 7 neighbours.  With s the group's scale, every code is
+// the nearest to the exact quotient x / s, ties to even: x (1 / s) is two units
+// of the last place off at most, and only where that could change the code
+// (the remainder x - q s is near half a step) is the exact remainder asked.
+//
+// Bound by memory: values in once, codes out once, and the reverse.
+#include "lc_internal.h"
+#include "lc_w4.h"
+
+namespace lc {
+namespace {
+
+constexpr int kW4Threads = 256;
+constexpr int kW4Warps = kW4Threads / 32;
+constexpr int kW4Half = 64;            // columns of half a block
+constexpr int kW4Pitch = kW4Half + 4;  // floats between rows of the exchange buffer
+
+template <typename T>
+LC_DEV float to_f32(T v);
+template <>
+LC_DEV float to_f32<float>(float v) { return v; }
+template <>
+LC_DEV float to_f32<__half>(__half v) { return __half2float(v); }
+template <typename T>
+LC_DEV T from_f32(float v);
+template <>
+LC_DEV float from_f32<float>(float v) { return v; }
+template <>
+LC_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// (a + b) / 15 for a, b >= 0, correctly rounded in 64 bits, as fp32: the remainder
+// of a first quotient by the rounded reciprocal corrects it.
+LC_DEV float fifteenth(float a, float b) {
+    constexpr double r = 1.0 / 15.0;
+    const double n = (double)a + (double)b, q = n * r;
+    return (float)__fma_rn(__fma_rn(-q, 15.0, n), r, q);
+}
+
+// Nearest whole number to x / s, ties to even, for |x / s| <= 2^20: `near` is
+// at most one off.
+LC_DEV float settle(float x, float s, float near) {
+    const float rest = __fmaf_rn(-near, s, x);  // exact where it matters: at most one step, in units of x's
+    const float a = 2.0f * fabsf(rest);
+    const bool odd = (static_cast<int>(near) & 1) != 0;
+    return a > s || (a == s && odd) ? near + copysignf(1.0f, rest) : near;
+}
+
+// Quotients of 16 values as whole numbers in [-16, 16].
+LC_DEV void quotients(const float (&x)[16], float s, float inv, float (&q)[16]) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+    const float sure = s * (0.5f - 0x1p-16f);
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float t = fminf(fmaxf(x[i] * inv, -16.0f), 16.0f);
+        q[i] = (t + kMagic) - kMagic;
+        all = all && fabsf(__fmaf_rn(-q[i], s, x[i])) < sure;
+    }
+    if (all) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (fabsf(q[i]) < 16.0f) q[i] = settle(x[i], s, q[i]);
+}
+
+// Columns c0 .. c0 + 15 of rows r and r + 8 (both halves of the warp's rows)
+// from memory: by the lane itself where 16-byte loads may be used, else row by
+// row through shared memory, so that neighbours read neighbours.
+template <typename T>
+LC_DEV void load_half(const T* p, int64_t stride, int row0, int rows, int col0, int cols, bool vec, float* buf, int lane,
+                      float (&a)[16], float (&b)[16]) {
+    const int g = lane >> 2, t = lane & 3;
+    if (vec && col0 + kW4Half <= cols) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float(&o)[16] = half ? b : a;
+            const int r = row0 + g + 8 * half;
+#pragma unroll
+            for (int i = 0; i < 16 / V; ++i) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (r < rows) w = __ldg(reinterpret_cast<const uint4*>(p + r * stride + col0 + 16 * t) + i);
+                const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                for (int k = 0; k < V; ++k) o[i * V + k] = to_f32<T>(e[k]);
+            }
+        }
+        return;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < kW4Rows; ++r) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = col0 + 32 * h + lane;
+            buf[r * kW4Pitch + 32 * h + lane] = row0 + r < rows && c < cols ? to_f32<T>(p[(row0 + r) * stride + c]) : 0.0f;
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 u = *reinterpret_cast<const float4*>(buf + g * kW4Pitch + 16 * t + 4 * i);
+        const float4 v = *reinterpret_cast<const float4*>(buf + (g + 8) * kW4Pitch + 16 * t + 4 * i);
+        a[4 * i] = u.x, a[4 * i + 1] = u.y, a[4 * i + 2] = u.z, a[4 * i + 3] = u.w;
+        b[4 * i] = v.x, b[4 * i + 1] = v.y, b[4 * i + 2] = v.z, b[4 * i + 3] = v.w;
+    }
+}
+
+// Scale, its bits and the zero point of a group from its smallest and largest
+// finite values, which are at most and at least 0.
+struct Step {
+    float s, zero;
+    uint16_t bits;
+};
+template <bool ZEROS>
+LC_DEV Step step_of(float low, float high) {
+    Step o;
+    const float step = ZEROS ? fifteenth(-low, high) : __fdiv_rn(fmaxf(-low, high), 7.0f);
+    const __half h = __float2half_rn(fminf(step, 65504.0f));
+    o.bits = __half_as_ushort(h);
+    o.s = __half2float(h);
+    o.zero = 8.0f;
+    if (ZEROS) {
+        o.zero = 0.0f;
+        if (o.s > 0.0f) {
+            const float near = rintf(fminf(__fdiv_rn(-low, o.s), 16.0f));
+            o.zero = near < 16.0f ? fminf(settle(-low, o.s, near), 15.0f) : 15.0f;
+        }
+    }
+    return o;
+}
+
+template <typename T, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kW4Threads) w4_quantize_kernel(W4 w, const T* __restrict__ values, int64_t stride, bool vec) {
+    __shared__ __align__(16) float buf[kW4Warps][kW4Rows * kW4Pitch];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    constexpr int NG = kW4Cols / GROUP;        // groups of a block
+    constexpr int SPAN = GROUP / 16 < 4 ? GROUP / 16 : 4;  // lanes of a group in one half
+    const int64_t units = (int64_t)w.tiles * w.blocks;
+    for (int64_t u = (int64_t)blockIdx.x * kW4Warps + warp; u < units; u += (int64_t)gridDim.x * kW4Warps) {
+        const int tile = (int)(u / w.blocks), block = (int)(u - (int64_t)tile * w.blocks);
+        float x[2][2][16];  // [half][row g or g + 8]
+        float low[2][2], high[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            load_half<T>(values, stride, tile * kW4Rows, w.rows, block * kW4Cols + h * kW4Half, w.cols, vec, buf[warp], lane, x[h][0], x[h][1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float& v = x[h][k][i];
+                    if (!(v == v)) v = 0.0f;
+                    if (fabsf(v) < INFINITY) lo = fminf(lo, v), hi = fmaxf(hi, v);
+                }
+#pragma unroll
+                for (int o = 1; o < SPAN; o <<= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                }
+                low[h][k] = lo, high[h][k] = hi;
+            }
+        }
+        if (GROUP == 128) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                low[0][k] = low[1][k] = fminf(low[0][k], low[1][k]);
+                high[0][k] = high[1][k] = fmaxf(high[0][k], high[1][k]);
+            }
+        }
+        uint4* out = reinterpret_cast<uint4*>(w.codes + u * kW4BlockBytes);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t word[4] = {0, 0, 0, 0};
+            Step step[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                step[k] = step_of<ZEROS>(low[h][k], high[h][k]);
+                float q[16];
+                const float s = step[k].s;
+                if (s > 0.0f) {
+                    quotients(x[h][k], s, __frcp_rn(s), q);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) q[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float c = ZEROS ? fminf(fmaxf(q[i] + step[k].zero, 0.0f), 15.0f) : fminf(fmaxf(q[i], -7.0f), 7.0f) + 8.0f;
+                    constexpr int kBit[4] = {0, 16, 8, 24};
+                    const int col = block * kW4Cols + h * kW4Half + 16 * t + i;
+                    const uint32_t code = col < w.cols ? (uint32_t)c : 0u;
+                    word[i >> 2] |= code << (kBit[i & 3] + 4 * k);
+                }
+            }
+            out[h * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+            // The first lane of a group in this half writes its pair; groups of 128 once.
+            const int first = block * kW4Cols + h * kW4Half + 16 * t;
+            if (t % SPAN == 0 && (GROUP < 128 || h == 0)) {
+                const int i = GROUP == 128 ? 0 : (h * kW4Half + 16 * t) / GROUP;
+                const int64_t at = (u * 8 + g) * NG + i;
+                const bool there = first < w.cols;
+                const uint32_t s0 = there && tile * kW4Rows + g < w.rows ? step[0].bits : 0u;
+                const uint32_t s1 = there && tile * kW4Rows + g + 8 < w.rows ? step[1].bits : 0u;
+                reinterpret_cast<uint32_t*>(w.scales)[at] = s0 | s1 << 16;
+                if (ZEROS)
+                    reinterpret_cast<uint16_t*>(w.zeros)[at] = (uint16_t)((uint32_t)step[0].zero | (uint32_t)step[1].zero << 8);
+            }
+        }
+    }
+}
+
+// Codes [rows][ceil(cols / 2)], scales and zero points [rows][groups] as a
+// checkpoint holds them.  A lane makes its 16 bytes from 8 bytes of two rows.
+template <int GROUP>
+__global__ void __launch_bounds__(kW4Threads) w4_pack_kernel(W4 w, const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales,
+                                                             const uint8_t* __restrict__ zeros) {
+    constexpr int NG = kW4Cols / GROUP;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int64_t units = (int64_t)w.tiles * w.blocks;
+    const int64_t pitch = (w.cols + 1) / 2;
+    const int groups = (w.cols + GROUP - 1) / GROUP;
+    for (int64_t u = (int64_t)blockIdx.x * kW4Warps + warp; u < units; u += (int64_t)gridDim.x * kW4Warps) {
+        const int tile = (int)(u / w.blocks), block = (int)(u - (int64_t)tile * w.blocks);
+        uint4* out = reinterpret_cast<uint4*>(w.codes + u * kW4BlockBytes);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t word[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int row = tile * kW4Rows + g + 8 * k;
+                const int col = block * kW4Cols + h * kW4Half + 16 * t;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {  // a byte: columns col + 2 i (low half) and the next
+                    const int c = col + 2 * i;
+                    uint32_t b = row < w.rows && c < w.cols ? codes[row * pitch + (c >> 1)] : 0u;
+                    if (c + 1 >= w.cols) b &= 15u;
+                    constexpr int kBit[2] = {0, 8};
+                    word[i >> 1] |= (b & 15u) << (kBit[i & 1] + 4 * k) | (b >> 4) << (kBit[i & 1] + 16 + 4 * k);
+                }
+            }
+            out[h * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+        }
+        for (int i = lane; i < 8 * NG * 2; i += 32) {
+            const int row = tile * kW4Rows + i / (2 * NG) + 8 * (i & 1);
+            const int group = block * NG + (i >> 1) % NG;
+            const bool there = row < w.rows && group < groups;
+            const int64_t from = (int64_t)row * groups + group;
+            w.scales[u * (16 * NG) + i] = there ? scales[from] : (uint16_t)0;
+            if (zeros) w.zeros[u * (16 * NG) + i] = there ? zeros[from] & 15 : (uint8_t)0;
+        }
+    }
+}
+
+template <typename T, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kW4Threads) w4_read_kernel(W4 w, T* __restrict__ values, int64_t stride, bool vec) {
+    __shared__ __align__(16) float buf[kW4Warps][kW4Rows * kW4Pitch];
+    constexpr int NG = kW4Cols / GROUP;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int64_t units = (int64_t)w.tiles * w.blocks;
+    for (int64_t u = (int64_t)blockIdx.x * kW4Warps + warp; u < units; u += (int64_t)gridDim.x * kW4Warps) {
+        const int tile = (int)(u / w.blocks), block = (int)(u - (int64_t)tile * w.blocks);
+        const uint4* in = reinterpret_cast<const uint4*>(w.codes + u * kW4BlockBytes);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 word = in[h * 32 + lane];
+            const uint32_t ws[4] = {word.x, word.y, word.z, word.w};
+            const int col0 = block * kW4Cols + h * kW4Half;
+            const int64_t at = (u * 8 + g) * NG + (h * kW4Half + 16 * t) / GROUP;
+            const uint32_t sc = reinterpret_cast<const uint32_t*>(w.scales)[at];
+            const uint32_t zp = ZEROS ? reinterpret_cast<const uint16_t*>(w.zeros)[at] : 0x0808u;
+            const bool direct = vec && col0 + kW4Half <= w.cols;
+            if (!direct) __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float s = __half2float(__ushort_as_half((uint16_t)(sc >> (16 * k))));
+                const int zero = (zp >> (8 * k)) & 255;
+                const int row = tile * kW4Rows + g + 8 * k;
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    constexpr int kBit[4] = {0, 16, 8, 24};
+                    v[i] = s * (float)((int)((ws[i >> 2] >> (kBit[i & 3] + 4 * k)) & 15u) - zero);
+                }
+                if (direct) {
+                    constexpr int V = 16 / sizeof(T);
+                    if (row < w.rows) {
+#pragma unroll
+                        for (int i = 0; i < 16 / V; ++i) {
+                            T e[V];
+#pragma unroll
+                            for (int j = 0; j < V; ++j) e[j] = from_f32<T>(v[i * V + j]);
+                            *(reinterpret_cast<uint4*>(values + row * stride + col0 + 16 * t) + i) = *reinterpret_cast<const uint4*>(e);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4*>(&buf[warp][(g + 8 * k) * kW4Pitch + 16 * t + 4 * i]) =
+                            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+            }
+            if (direct) continue;
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < kW4Rows; ++r) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int row = tile * kW4Rows + r, c = col0 + 32 * q + lane;
+                    if (row < w.rows && c < w.cols) values[row * stride + c] = from_f32<T>(buf[warp][r * kW4Pitch + 32 * q + lane]);
+                }
+            }
+        }
+    }
+}
+
+unsigned w4_grid(const W4& w, int num_sms) {
+    const int64_t ctas = ((int64_t)w.tiles * w.blocks + kW4Warps - 1) / kW4Warps, most = (int64_t)num_sms * 16;
+    return (unsigned)(ctas < most ? ctas : most);
+}
+
+template <typename T>
+bool vector_rows(const void* p, int64_t stride) {
+    return (((uintptr_t)p | (uintptr_t)(stride * (int64_t)sizeof(T))) & 15) == 0;
+}
+
+template <typename T, int GROUP>
+cudaError_t quantize_as(const W4& w, const void* v, int64_t stride, int num_sms, cudaStream_t st) {
+    const bool vec = vector_rows<T>(v, stride);
+    if (w.zeros) w4_quantize_kernel<T, GROUP, true><<<w4_grid(w, num_sms), kW4Threads, 0, st>>>(w, (const T*)v, stride, vec);
+    else w4_quantize_kernel<T, GROUP, false><<<w4_grid(w, num_sms), kW4Threads, 0, st>>>(w, (const T*)v, stride, vec);
+    return cudaGetLastError();
+}
+template <typename T, int GROUP>
+cudaError_t read_as(const W4& w, void* v, int64_t stride, int num_sms, cudaStream_t st) {
+    const bool vec = vector_rows<T>(v, stride);
+    if (w.zeros) w4_read_kernel<T, GROUP, true><<<w4_grid(w, num_sms), kW4Threads, 0, st>>>(w, (T*)v, stride, vec);
+    else w4_read_kernel<T, GROUP, false><<<w4_grid(w, num_sms), kW4Threads, 0, st>>>(w, (T*)v, stride, vec);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+#define LC_W4_GROUPS(fn, T, ...) \
+    (w.group == 32 ? fn<T, 32>(__VA_ARGS__) : w.group == 64 ? fn<T, 64>(__VA_ARGS__) : fn<T, 128>(__VA_ARGS__))
+
+cudaError_t launch_w4_quantize(const W4& w, const void* values, int64_t stride, int dtype, int num_sms, cudaStream_t st) {
+    return dtype == kRowF32 ? LC_W4_GROUPS(quantize_as, float, w, values, stride, num_sms, st)
+                            : LC_W4_GROUPS(quantize_as, __half, w, values, stride, num_sms, st);
+}
+
+cudaError_t launch_w4_read(const W4& w, void* values, int64_t stride, int dtype, int num_sms, cudaStream_t st) {
+    return dtype == kRowF32 ? LC_W4_GROUPS(read_as, float, w, values, stride, num_sms, st)
+                            : LC_W4_GROUPS(read_as, __half, w, values, stride, num_sms, st);
+}
+
+cudaError_t launch_w4_pack(const W4& w, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int num_sms, cudaStream_t st) {
+    const unsigned grid = w4_grid(w, num_sms);
+    if (w.group == 32) w4_pack_kernel<32><<<grid, kW4Threads, 0, st>>>(w, codes, scales, zeros);
+    else if (w.group == 64) w4_pack_kernel<64><<<grid, kW4Threads, 0, st>>>(w, codes, scales, zeros);
+    else w4_pack_kernel<128><<<grid, kW4Threads, 0, st>>>(w, codes, scales, zeros);
+    return cudaGetLastError();
+}
+
+}  // namespace lc

@@ -1,0 +1,67 @@
+// lc_w4.h -- host declarations of the 4-bit weights (lc_w4.cu: quantising,
+// packing and reading; lc_w4_product.cu: products) and of the log
+// probabilities (lc_logprobs.cu).
+//
+// Layout.  Codes lie in tiles of 16 rows and blocks of 128 columns, [tiles]
+// [blocks][1024 bytes]; 16 bytes of each 512 (a chunk of 64 columns) belong to
+// lane 4 g + t of the warp that reads them: rows g and g + 8, columns 16 t ..
+// 16 t + 15.  Word j of the 16 bytes holds columns 16 t + 4 j + e, e = 0..3, at
+// bit {0, 16, 8, 24}[e] for row g and 4 bits higher for row g + 8.  So the
+// words masked by 0x000f000f and 0x00f000f0, before and after a shift by 8, are
+// the four registers that one m16n8k16 product takes from the lane, as pairs of
+// f16 numbers c 2^-24 and (rows g + 8) c 2^-20; and 16 columns of one row are
+// two runs of 16 bytes of f16 values, which is what tcgen05 operands are made
+// of.  The order of columns within a product does not matter as long as both
+// operands have the same.
+//
+// Scales (f16) and zero points (bytes) of a block: [8 g][128 / group][2], the
+// pair being rows g and g + 8.  Columns behind the last have code 0, rows
+// behind the last and groups without columns scale 0.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "lc_paged.h"
+
+namespace lc {
+
+constexpr int kW4Rows = 16;    // rows of a tile
+constexpr int kW4Cols = 128;   // columns of a block
+constexpr int kW4BlockBytes = 1024;
+
+struct W4 {
+    uint8_t* codes;
+    uint16_t* scales;
+    uint8_t* zeros;  // null: 8
+    int rows, cols, group;
+    int tiles, blocks;
+};
+struct W4Product {
+    const void* x;
+    void* y;
+    const void* residual;  // null: none
+    int64_t x_stride, y_stride, residual_stride;  // elements
+    int batch, dtype;
+};
+cudaError_t launch_w4_quantize(const W4& w, const void* values, int64_t stride, int dtype, int num_sms, cudaStream_t st);
+cudaError_t launch_w4_pack(const W4& w, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int num_sms, cudaStream_t st);
+cudaError_t launch_w4_read(const W4& w, void* values, int64_t stride, int dtype, int num_sms, cudaStream_t st);
+cudaError_t launch_w4_product(const W4& w, const W4Product& p, int num_sms, cudaStream_t st);
+
+constexpr int kLogprobsMaxTop = 32;
+struct Logprobs {
+    const void* x;
+    int64_t stride;
+    int dtype, rows, vocab, top;
+    float scale;
+    const int32_t* tokens;  // null: none
+    float* token_logprobs;  // each output: null when not asked for
+    int32_t* token_ranks;
+    float* entropy;
+    int32_t* top_ids;
+    float* top_logprobs;
+};
+cudaError_t launch_logprobs(const Logprobs& p, int num_sms, cudaStream_t st);
+
+}  // namespace lc

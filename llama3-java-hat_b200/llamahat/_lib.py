@@ -83,6 +83,13 @@ class LcKv8(ctypes.Structure):
     ]
 
 
+class LcW4(ctypes.Structure):
+    _fields_ = [
+        ("codes", c_void_p), ("scales", c_void_p), ("zeros", c_void_p), ("rows", c_int32), ("cols", c_int32),
+        ("group", c_int32), ("reserved", c_int32 * 3),
+    ]
+
+
 # lc_token_callback: void (*)(int32_t token, int32_t index, void* user)
 TOKEN_CALLBACK = ctypes.CFUNCTYPE(None, c_int32, c_int32, c_void_p)
 
@@ -135,6 +142,14 @@ SIGNATURES = {
     "lc_kv8_read": (c_int, [c_void_p, POINTER(LcKv8), c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32]),
     "lc_kv8_attention": (c_int, [c_void_p, POINTER(LcKv8), c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
                                  c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float]),
+    "lc_w4_sizes": (c_int, [c_int32, c_int32, c_int32, POINTER(c_int64), POINTER(c_int64)]),
+    "lc_w4_quantize": (c_int, [c_void_p, POINTER(LcW4), c_void_p, c_int64, c_int32]),
+    "lc_w4_pack": (c_int, [c_void_p, POINTER(LcW4), c_void_p, c_void_p, c_void_p]),
+    "lc_w4_read": (c_int, [c_void_p, POINTER(LcW4), c_void_p, c_int64, c_int32]),
+    "lc_w4_product": (c_int, [c_void_p, POINTER(LcW4), c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                              c_int32]),
+    "lc_logprobs": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p,
+                            c_void_p, c_int32, c_void_p, c_void_p]),
     "lc_config_llama32_1b": (None, [POINTER(LcConfig)]),
     "lc_model_create": (c_int, [c_void_p, POINTER(LcConfig), POINTER(c_void_p)]),
     "lc_model_upload_tensor": (c_int, [c_void_p, c_char_p, c_void_p, c_int64, c_int32]),

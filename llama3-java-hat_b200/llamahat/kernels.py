@@ -77,6 +77,28 @@ def _i32(buf, min_len: int, writable: bool = False) -> int:
     return _addr(buf, "i32", min_len, writable)
 
 
+def _f32(buf, min_len: int) -> int:
+    """_addr(buf, "f32", min_len, writable=True), as _i32."""
+    if _TORCH_ROWS.get(buf.dtype) == 0 and buf.numel() >= min_len and buf.is_contiguous():
+        return buf.data_ptr()
+    return _addr(buf, "f32", min_len, True)
+
+
+def _bytes(buf, shape) -> int:
+    """Address of contiguous bytes (uint8) of the given shape, numpy or torch."""
+    if str(buf.dtype) not in ("uint8", "torch.uint8"):
+        raise TypeError(f"expected uint8, got {buf.dtype}")
+    if tuple(buf.shape) != shape:
+        raise ValueError(f"expected shape {shape}, got {tuple(buf.shape)}")
+    if isinstance(buf, np.ndarray):
+        if not buf.flags.c_contiguous:
+            raise ValueError("buffer must be C-contiguous")
+        return buf.ctypes.data
+    if not buf.is_contiguous():
+        raise ValueError("tensor must be contiguous")
+    return buf.data_ptr()
+
+
 def _rows(buf, writable: bool = False):
     """(address, rows, width, row stride in elements, dtype id) of a buffer of
     F32 or F16 rows: [rows, ...] with contiguous rows, any row stride."""
@@ -439,6 +461,120 @@ class PagedKV8(_CudaKernel):
             _lib.check(rc)
 
 
+class Weights4(_CudaKernel):
+    """A weight matrix [rows, cols] in 4 bits under one scale, and one zero point
+    or none, per row and `group` columns (see lc_w4), in CUDA tensors that this
+    object keeps alive: codes (uint8), scales (float16) and zeros (uint8, or None
+    for 8 throughout), of the sizes that lc_w4_sizes gives; `empty` makes them.
+    Its calls run on the accelerator's stream (see Accelerator)."""
+
+    def __init__(self, codes, scales, zeros, rows: int, cols: int, group: int = 128, acc: Accelerator | None = None):
+        super().__init__(acc)
+        n, m = self.sizes(rows, cols, group)
+        for name, t, dtype, want in (("codes", codes, "torch.uint8", n), ("scales", scales, "torch.float16", m),
+                                     ("zeros", zeros, "torch.uint8", m)):
+            if t is None and name == "zeros":
+                continue
+            if str(t.dtype) != dtype:
+                raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+            if not t.is_contiguous() or t.numel() < want:
+                raise ValueError(f"{name}: {t.numel()} elements (contiguous: {t.is_contiguous()}), need {want}")
+        self.tensors = (codes, scales, zeros)
+        self.rows, self.cols, self.group = rows, cols, group
+        self._w = _lib.LcW4(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), rows, cols,
+                            group)
+
+    @staticmethod
+    def sizes(rows: int, cols: int, group: int = 128) -> tuple[int, int]:
+        """(bytes of codes, number of scales) that a matrix takes."""
+        n, m = ctypes.c_int64(), ctypes.c_int64()
+        _lib.check(_lib.load().lc_w4_sizes(rows, cols, group, ctypes.byref(n), ctypes.byref(m)))
+        return n.value, m.value
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, group: int = 128, zeros: bool = False, acc: Accelerator | None = None) -> "Weights4":
+        """Room for a matrix on the accelerator's device, to be filled by quantize or pack."""
+        import torch
+        acc = acc or default_accelerator()
+        n, m = cls.sizes(rows, cols, group)
+        at = torch.device("cuda", acc.device)
+        return cls(torch.empty(n, dtype=torch.uint8, device=at), torch.empty(m, dtype=torch.float16, device=at),
+                   torch.empty(m, dtype=torch.uint8, device=at) if zeros else None, rows, cols, group, acc)
+
+    def _values(self, values, writable: bool):
+        a, rows, width, stride, dt = _rows(values, writable)
+        if (rows, width) != (self.rows, self.cols):
+            raise ValueError(f"values [{rows}, {width}], the matrix is [{self.rows}, {self.cols}]")
+        return a, stride, dt
+
+    def quantize(self, values) -> None:
+        """The matrix from values [rows, cols] (F32 or F16; see lc_w4_quantize)."""
+        _lib.check(self.lib.lc_w4_quantize(self.ctx, self._w, *self._values(values, False)))
+
+    def read(self, values) -> None:
+        """values [rows, cols] (F32 or F16) = the matrix."""
+        _lib.check(self.lib.lc_w4_read(self.ctx, self._w, *self._values(values, True)))
+
+    def pack(self, codes, scales, zeros=None) -> None:
+        """The matrix from codes [rows, (cols + 1) // 2] (uint8, the lower column
+        in the low half), scales [rows, groups] (F16) and zero points [rows,
+        groups] (uint8), as a checkpoint holds them (see lc_w4_pack)."""
+        if (zeros is None) != (self.tensors[2] is None):
+            raise ValueError("zero points on one side only")
+        groups = -(-self.cols // self.group)
+        _lib.check(self.lib.lc_w4_pack(
+            self.ctx, self._w, _bytes(codes, (self.rows, (self.cols + 1) // 2)),
+            _addr(scales, "f16", self.rows * groups), None if zeros is None else _bytes(zeros, (self.rows, groups))))
+
+    def apply(self, x, y, residual=None) -> None:
+        """y [batch, rows] = x [batch, cols] W^T, plus residual [batch, rows],
+        which may be y; all F32 or all F16 (see lc_w4_product)."""
+        xa, batch, width, xs, dt = _rows(x)
+        ya, yb, ywidth, ys, ydt = _rows(y, True)
+        if width != self.cols or ywidth != self.rows or yb != batch or ydt != dt:
+            raise ValueError(f"x [{batch}, {width}] and y [{yb}, {ywidth}] (types {dt}, {ydt}) for a matrix [{self.rows}, {self.cols}]")
+        ra, rs = None, 0
+        if residual is y:
+            ra, rs = ya, ys
+        elif residual is not None:
+            ra, rb, rwidth, rs, rdt = _rows(residual)
+            if rb != batch or rwidth != ywidth or rdt != dt:
+                raise ValueError("residual and y differ in shape or type")
+        rc = self.lib.lc_w4_product(self.acc.handle, self._w, xa, xs, ya, ys, ra, rs, batch, dt)
+        if rc:
+            _lib.check(rc)
+
+
+class CudaLogProbs(_CudaKernel):
+    """Log probabilities of given tokens with their ranks, the entropy and the
+    best alternatives (see lc_logprobs), on the accelerator's stream (see
+    Accelerator)."""
+
+    def apply(self, logits, tokens=None, token_logprobs=None, token_ranks=None, entropy=None, top_ids=None,
+              top_logprobs=None, scale: float = 1.0) -> None:
+        """logits [rows, vocab] (F32 or F16); tokens, token_ranks [rows] (int32);
+        token_logprobs, entropy [rows] (float32); top_ids (int32) and
+        top_logprobs (float32) [rows, k], k <= 32.  Outputs that are None are not
+        computed.  scale: 1 / temperature."""
+        xa, rows, vocab, stride, dt = _rows(logits)
+        top = top_ids if top_ids is not None else top_logprobs
+        k = 0
+        if top is not None:
+            k = top.shape[1]
+            for t in (top_ids, top_logprobs):
+                if t is not None and tuple(t.shape) != (rows, k):
+                    raise ValueError(f"top outputs are [{rows}, k], got {tuple(t.shape)}")
+        rc = self.lib.lc_logprobs(
+            self.acc.handle, xa, stride, dt, rows, vocab, scale, None if tokens is None else _i32(tokens, rows),
+            None if token_logprobs is None else _f32(token_logprobs, rows),
+            None if token_ranks is None else _i32(token_ranks, rows, True),
+            None if entropy is None else _f32(entropy, rows), k,
+            None if top_ids is None else _i32(top_ids, rows * k, True),
+            None if top_logprobs is None else _f32(top_logprobs, rows * k))
+        if rc:
+            _lib.check(rc)
+
+
 class CudaSiLU(_CudaKernel, ISiLU):
     """SiLU.java:32-40 on the GPU."""
 
@@ -507,6 +643,9 @@ class CudaKernelFactory(IKernelFactory):
 
     def createPages(self, acc=None) -> CudaPages:
         return CudaPages(acc)
+
+    def createLogProbs(self, acc=None) -> CudaLogProbs:
+        return CudaLogProbs(acc)
 
     def createSiLU(self, acc=None) -> CudaSiLU:
         return CudaSiLU(acc)
