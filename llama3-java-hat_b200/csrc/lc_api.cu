@@ -1100,6 +1100,7 @@ extern "C" int lc_logprobs(lc_context* c, const void* logits, int64_t stride, in
         if (top_ids) p.top_ids = (int32_t*)s.arg(top_ids, nk, kOut);
         if (top_logprobs) p.top_logprobs = (float*)s.arg(top_logprobs, nk, kOut);
         if (s.status != LC_OK) return s.status;
+        if ((uintptr_t)p.x % elem) return fail(LC_ERR_INVALID_ARG, "logits are not aligned to their type");
         p.stride = stride;
         p.dtype = dtype;
         p.rows = rows;

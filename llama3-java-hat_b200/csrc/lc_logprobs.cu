@@ -1,111 +1,410 @@
 // lc_logprobs.cu -- log probabilities of given tokens with their ranks, the
-// entropy and the best alternatives, from rows of logits.
+// entropy and the best alternatives, from rows of logits, in one pass.
 //
-// With m the largest logit of a row, t_i = scale (x_i - m) and S = sum e^t_i:
-// log p_i = t_i - ln S and H = ln S - (sum t_i e^t_i) / S.  Tokens are ordered
-// by logit, equal ones by index.
+// With m the largest logit of a row, u_i = scale log2(e) (x_i - m), S = sum
+// 2^u_i and T = sum u_i 2^u_i: ln p_i = scale (x_i - m) - ln S and
+// H = ln S - ln 2 T / S.  A thread keeps its own m, S and T; when m grows by d
+// (in units of u) S becomes 2^-d S and T 2^-d (T - d S).  u is held at -200 and
+// above, where 2^u is 0 already: masked logits (-inf, the type's lowest) then
+// add nothing, and not 0 * inf.
+//
+// The best k cost the pass nothing: it has every thread's largest logit anyway.
+// A thread with k larger ones above its own holds none of the best k, so about
+// k of the CTA's threads are left, whose elements are read again (from L2) and
+// compared with the least of their largest.  The order of tokens is that of
+// 64-bit keys (the logit's bits, then the index), so it does not depend on who
+// finds them.  A rank is counted where a chunk's largest logit reaches the
+// token's, which few chunks do for likely tokens.
+//
+// Bound by memory: 5 to 6 instructions per logit where HBM leaves time for 22
+// (F32) or 11 (F16).  Few rows are cut over a cluster of up to 16 CTAs, whose
+// parts meet in the shared memory of the first: no workspace, nothing kept.
 #include "lc_internal.h"
 #include "lc_w4.h"
 
 namespace lc {
 namespace {
 
-constexpr int kSimpleThreads = 256;
+constexpr int kLpThreads = 256;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpPieces = 4;       // 16-byte pieces of a thread's chunk
+constexpr int kLpMaxCluster = 16;  // more than 8 is opt-in
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLpFloor = -200.0f;
 
-template <typename T>
-LC_DEV float logit(const T* x, int i) {
-    const float v = (float)x[i] + 0.0f;  // no negative zeros
+LC_DEV float max_nan(float a, float b) {  // a NaN wins
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+LC_DEV float exp2_fast(float x) {  // 2 units of the last place; 0 below 2^-126
+    float d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+    return d;
+}
+LC_DEV uint64_t pack2(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
     return v;
 }
-LC_DEV uint32_t ordered(float v) {  // NaN below -inf
-    if (!(v == v)) v = -INFINITY;
+LC_DEV float2 unpack2(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+LC_DEV uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+LC_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+LC_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+// Bits that order as the logits do; NaN as -inf, zeros of both signs alike.
+LC_DEV uint32_t ordered(float v) {
+    v = v == v ? v + 0.0f : -INFINITY;
     const uint32_t b = __float_as_uint(v);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+LC_DEV float unordered(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 LC_DEV uint64_t order_key(float v, int i) { return (uint64_t)ordered(v) << 32 | (uint32_t)~i; }
+constexpr uint32_t kOrderedMasked = 0x007fffffu;  // of -inf
 
-LC_DEV double block_sum(double v, double* buf) {
-    __syncthreads();
-    buf[threadIdx.x] = v;
-    __syncthreads();
-    for (int o = kSimpleThreads / 2; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) buf[threadIdx.x] += buf[threadIdx.x + o];
-        __syncthreads();
-    }
-    return buf[0];
-}
-LC_DEV uint64_t block_max(uint64_t v, uint64_t* buf) {
-    __syncthreads();
-    buf[threadIdx.x] = v;
-    __syncthreads();
-    for (int o = kSimpleThreads / 2; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) buf[threadIdx.x] = max(buf[threadIdx.x], buf[threadIdx.x + o]);
-        __syncthreads();
-    }
-    return buf[0];
-}
-
+// 16 bytes of logits.
 template <typename T>
-__global__ void __launch_bounds__(kSimpleThreads) logprobs_simple_kernel(Logprobs p) {
-    __shared__ double sums[kSimpleThreads];
-    __shared__ uint64_t keys[kSimpleThreads];
-    const int64_t row = blockIdx.x;
-    const T* x = (const T*)p.x + row * p.stride;
-    int token = p.tokens ? p.tokens[row] : -1;
+struct Piece;
+template <>
+struct Piece<float> {
+    static constexpr int N = 4;
+    uint4 w;
+    LC_DEV float get(int i) const { return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w); }
+    LC_DEV float top() const { return max_nan(max_nan(get(0), get(1)), max_nan(get(2), get(3))); }
+};
+template <>
+struct Piece<__half> {
+    static constexpr int N = 8;
+    uint4 w;
+    LC_DEV __half2 two(int i) const {
+        const uint32_t v = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+        return *reinterpret_cast<const __half2*>(&v);
+    }
+    LC_DEV float get(int i) const { return i & 1 ? __high2float(two(i >> 1)) : __low2float(two(i >> 1)); }
+    LC_DEV float top() const {
+        const __half2 m = __hmax2_nan(__hmax2_nan(two(0), two(1)), __hmax2_nan(two(2), two(3)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+};
+
+// A row as 16-byte pieces of memory: piece j holds elements j N - skew and on.
+template <typename T>
+struct Row {
+    const T* x;
+    int skew, vocab;
+    LC_DEV int first(int j) const { return j * Piece<T>::N - skew; }
+    LC_DEV bool has(int i) const { return (unsigned)i < (unsigned)vocab; }
+    // -inf in the places before and behind the row.
+    LC_DEV Piece<T> load(int j) const {
+        const int i = first(j);
+        Piece<T> p;
+        if (i >= 0 && i + Piece<T>::N <= vocab) {
+            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p.w.x), "=r"(p.w.y), "=r"(p.w.z), "=r"(p.w.w) : "l"(x + i));
+        } else {
+            T e[Piece<T>::N];
+#pragma unroll
+            for (int k = 0; k < Piece<T>::N; ++k) e[k] = has(i + k) ? x[i + k] : (T)-INFINITY;
+            p.w = *reinterpret_cast<const uint4*>(e);
+        }
+        return p;
+    }
+};
+
+// The 32 largest of two descending lists of a key per lane, descending.
+LC_DEV uint64_t merge_lists(uint64_t a, uint64_t b, int lane) {
+    uint64_t v = max(a, (uint64_t)__shfl_sync(0xffffffffu, b, 31 - lane));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, v, o);
+        v = (lane & o) ? min(v, other) : max(v, other);
+    }
+    return v;
+}
+
+// lists[0] = the largest of n lists (a power of two), by all warps of the CTA.
+LC_DEV void join_lists(uint64_t (*lists)[32], int n, int warp, int lane) {
+    for (n >>= 1; n > 0; n >>= 1) {
+        __syncthreads();
+        for (int i = warp; i < n; i += kLpWarps) lists[i][lane] = merge_lists(lists[i][lane], lists[i + n][lane], lane);
+    }
+    __syncthreads();
+}
+
+LC_DEV uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+LC_DEV uint32_t map_to(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+LC_DEV void put32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+LC_DEV void put64(uint32_t a, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
+LC_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+LC_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+struct Part {  // of a CTA's share of a row
+    float m, s, t;
+    uint32_t before;
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int cluster) {
+    __shared__ Part parts[kLpMaxCluster];
+    __shared__ __align__(16) uint32_t tops[kLpThreads];
+    __shared__ uint64_t lists[TOP ? kLpMaxCluster : 1][32];
+    __shared__ uint64_t ours[TOP ? kLpWarps : 1][32];
+    __shared__ uint16_t chosen[TOP ? kLpThreads : 1];
+    __shared__ uint32_t warp_top[kLpWarps], warp_before[kLpWarps], n_chosen, least;
+    __shared__ float warp_s[kLpWarps], warp_t[kLpWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+    if (cluster > 1) cluster_arrive();  // all CTAs of the cluster have begun when the wait below is over
+    griddep_wait();
+    griddep_launch();
+    const int64_t r = blockIdx.x / cluster;
+    Row<T> row;
+    row.x = (const T*)p.x + r * p.stride;
+    row.skew = (int)(((uintptr_t)row.x & 15) / sizeof(T));
+    row.vocab = p.vocab;
+    constexpr int N = Piece<T>::N;
+    const int64_t pieces = ((int64_t)row.skew + p.vocab + N - 1) / N;
+    const int p0 = (int)(pieces * rank / cluster), p1 = (int)(pieces * (rank + 1) / cluster);
+    int token = p.tokens ? p.tokens[r] : -1;
     if (token >= p.vocab) token = -1;
-    const uint64_t mine = token >= 0 ? order_key(logit(x, token), token) : ~0ull;
-    uint64_t best = 0;
-    double bad = 0, before = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kSimpleThreads) {
-        const float v = logit(x, i);
-        const uint64_t k = order_key(v, i);
-        best = max(best, k);
-        before += k > mine;
-        bad += !(v < INFINITY);  // NaN or +inf
+    float mine = INFINITY;  // the token's logit
+    if (token >= 0) {
+        mine = (float)row.x[token];
+        if (!(mine == mine)) mine = -INFINITY;
     }
-    best = block_max(best, keys);
-    before = block_sum(before, sums);
-    bad = block_sum(bad, sums);
-    const float high = logit(x, (int)~(uint32_t)best);
-    const bool empty = high == -INFINITY;
-    double total = 0, weighted = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kSimpleThreads) {
-        const float t = empty ? -INFINITY : (logit(x, i) - high) * p.scale;
-        const float e = expf(t);
-        total += e;
-        if (e > 0.0f) weighted += (double)e * t;
-    }
-    total = block_sum(total, sums);
-    weighted = block_sum(weighted, sums);
-    const double log_total = empty ? 0.0 : log(total);
-    auto logp = [&](float v) { return bad > 0 ? NAN : empty ? -INFINITY : (float)((double)((v - high) * p.scale) - log_total); };
-    if (threadIdx.x == 0) {
-        if (p.token_logprobs) p.token_logprobs[row] = token >= 0 ? logp(logit(x, token)) : 0.0f;
-        if (p.token_ranks) p.token_ranks[row] = token >= 0 ? (int)before : -1;
-        if (p.entropy) p.entropy[row] = bad > 0 ? NAN : empty ? 0.0f : (float)(log_total - weighted / total);
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-        uint64_t next = 0;
-        for (int i = threadIdx.x; i < p.vocab; i += kSimpleThreads) {
-            const uint64_t key = order_key(logit(x, i), i);
-            if (key < last) next = max(next, key);
+    const bool ranked = token >= 0 && p.token_ranks;
+
+    // ---- the pass ----
+    const float c = p.scale * kLog2e;
+    const uint64_t c2 = pack2(c, c);
+    float m = -INFINITY, ref = -3.4028234663852886e38f;  // ref: what exponents are taken from
+    uint64_t s2 = 0, t2 = 0;  // pairs of sums
+    uint32_t before = 0;
+    for (int j = p0 + tid; j < p1; j += kLpPieces * kLpThreads) {
+        Piece<T> w[kLpPieces];
+#pragma unroll
+        for (int k = 0; k < kLpPieces; ++k) {
+            const int at = j + k * kLpThreads;
+            if (at < p1) w[k] = row.load(at);
+            else w[k].w = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
+                                         : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
         }
-        last = block_max(next, keys);
-        if (threadIdx.x == 0) {
-            const int id = k < p.vocab ? (int)~(uint32_t)last : -1;
-            if (p.top_ids) p.top_ids[row * p.top + k] = id;
-            if (p.top_logprobs) p.top_logprobs[row * p.top + k] = id >= 0 ? logp(logit(x, id)) : bad > 0 ? NAN : -INFINITY;
+        float top = w[0].top();
+#pragma unroll
+        for (int k = 1; k < kLpPieces; ++k) top = max_nan(top, w[k].top());
+        m = max_nan(m, top);
+        const float now = fmaxf(m, ref);
+        const float d = fmaxf((ref - now) * c, kLpFloor), down = exp2_fast(d);
+        ref = now;
+        t2 = mul2(fma2(s2, pack2(d, d), t2), pack2(down, down));
+        s2 = mul2(s2, pack2(down, down));
+        const uint64_t ref2 = pack2(-ref, -ref);
+#pragma unroll
+        for (int k = 0; k < kLpPieces; ++k) {
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                const float2 u = unpack2(mul2(add2(pack2(w[k].get(e), w[k].get(e + 1)), ref2), c2));
+                const float u0 = fmaxf(u.x, kLpFloor), u1 = fmaxf(u.y, kLpFloor);
+                const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
+                s2 = add2(s2, e2);
+                t2 = fma2(e2, pack2(u0, u1), t2);
+            }
+        }
+        if (ranked && !(top < mine)) {
+#pragma unroll
+            for (int k = 0; k < kLpPieces; ++k) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int i = row.first(j + k * kLpThreads) + e;
+                    float v = w[k].get(e);
+                    if (!(v == v)) v = -INFINITY;
+                    before += j + k * kLpThreads < p1 && row.has(i) && (v > mine || (v == mine && i < token));
+                }
+            }
         }
     }
+
+    // ---- the CTA's part ----
+    const bool nan = !(m == m);
+    const uint32_t my_top = nan ? 0xffffffffu : ordered(m);  // a NaN above all
+    const uint32_t wt = __reduce_max_sync(0xffffffffu, my_top);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) warp_top[warp] = wt, warp_before[warp] = before;
+    if (tid == 0) n_chosen = 0, least = 0xffffffffu;
+    if (TOP) tops[tid] = my_top;
+    __syncthreads();
+    uint32_t cta_top = warp_top[0];
+#pragma unroll
+    for (int i = 1; i < kLpWarps; ++i) cta_top = max(cta_top, warp_top[i]);
+    const float cta_m = cta_top == 0xffffffffu ? NAN : unordered(cta_top);
+    {
+        const float now = fmaxf(cta_m, -3.4028234663852886e38f);
+        const float d = fmaxf((ref - now) * c, kLpFloor), down = exp2_fast(d);
+        const float2 s = unpack2(s2), t = unpack2(t2);
+        const float sum = s.x + s.y;
+        const float ws = warp_sum(sum * down), wt2 = warp_sum(fmaf(sum, d, t.x + t.y) * down);
+        if (lane == 0) warp_s[warp] = ws, warp_t[warp] = wt2;
+    }
+    if (TOP) {
+        // Threads with fewer than `top` larger maxima above their own.
+        bool in = cta_top == 0xffffffffu;  // a NaN hides a maximum: then all
+        if (!in) {
+            int above = 0;
+#pragma unroll 8
+            for (int i = 0; i < kLpThreads / 4; ++i) {
+                const uint4 o = reinterpret_cast<const uint4*>(tops)[i];
+                above += (o.x > my_top) + (o.y > my_top) + (o.z > my_top) + (o.w > my_top);
+            }
+            in = above < p.top;
+        }
+        const uint32_t low = __reduce_min_sync(0xffffffffu, in ? (cta_top == 0xffffffffu ? kOrderedMasked : my_top) : 0xffffffffu);
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        int at = 0;
+        if (lane == 0 && who) {
+            at = atomicAdd(&n_chosen, __popc(who));
+            atomicMin(&least, low);
+        }
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+        if (in) chosen[at] = (uint16_t)tid;
+        __syncthreads();
+        uint64_t list = 0, bar = ((uint64_t)least << 32) - 1;  // keys above it are let in
+        for (int q = warp; q < (int)n_chosen; q += kLpWarps) {
+            for (int j = p0 + chosen[q] + lane * kLpThreads; __any_sync(0xffffffffu, j < p1); j += 32 * kLpThreads) {
+                Piece<T> w;
+                w.w = make_uint4(0, 0, 0, 0);
+                const int i = row.first(j);
+                if (j < p1) w = row.load(j);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const uint64_t key = j < p1 && row.has(i + e) ? order_key(w.get(e), i + e) : 0;
+                    unsigned todo = __ballot_sync(0xffffffffu, key > bar);
+                    while (todo) {
+                        const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
+                        const int place = __popc(__ballot_sync(0xffffffffu, list > k));
+                        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+                        list = lane < place ? list : lane == place ? k : up;
+                        bar = max(bar, (uint64_t)__shfl_sync(0xffffffffu, list, p.top - 1));
+                        todo &= todo - 1;
+                        todo &= __ballot_sync(0xffffffffu, key > bar);
+                    }
+                }
+            }
+        }
+        ours[warp][lane] = list;
+        join_lists(ours, kLpWarps, warp, lane);
+    } else {
+        __syncthreads();
+    }
+
+    // ---- the row ----
+    if (cluster > 1) cluster_wait();
+    if (warp == 0) {
+        Part mine_part = {cta_m, 0.0f, 0.0f, 0};
+#pragma unroll
+        for (int i = 0; i < kLpWarps; ++i) mine_part.s += warp_s[i], mine_part.t += warp_t[i], mine_part.before += warp_before[i];
+        if (cluster == 1) {
+            if (lane == 0) parts[0] = mine_part;
+            if (TOP) lists[0][lane] = ours[0][lane];
+        } else {
+            const uint32_t to = map_to(&parts[rank], 0);
+            if (lane == 0) {
+                put32(to, __float_as_uint(mine_part.m)), put32(to + 4, __float_as_uint(mine_part.s));
+                put32(to + 8, __float_as_uint(mine_part.t)), put32(to + 12, mine_part.before);
+            }
+            if (TOP) put64(map_to(&lists[rank][lane], 0), ours[0][lane]);
+        }
+    }
+    if (cluster > 1) {
+        cluster_arrive();
+        if (rank != 0) return;  // what it wrote lies in the first CTA
+        cluster_wait();
+    }
+    if (TOP && cluster > 1) join_lists(lists, cluster, warp, lane);
+    if (warp != 0) return;
+    __syncwarp();
+    float high = parts[0].m;
+    for (int i = 1; i < cluster; ++i) high = max_nan(high, parts[i].m);
+    const float from = fmaxf(high, -3.4028234663852886e38f);
+    float s = 0.0f, t = 0.0f;
+    uint32_t all_before = 0;
+    for (int i = 0; i < cluster; ++i) {
+        const float d = fmaxf((fmaxf(parts[i].m, -3.4028234663852886e38f) - from) * c, kLpFloor), down = exp2_fast(d);
+        s = fmaf(parts[i].s, down, s);
+        t = fmaf(fmaf(parts[i].s, d, parts[i].t), down, t);
+        all_before += parts[i].before;
+    }
+    const bool bad = !(high < INFINITY), empty = high == -INFINITY;
+    const float ln_s = logf(s);
+    auto logp = [&](float v) { return bad ? NAN : v == -INFINITY ? -INFINITY : (v - high) * p.scale - ln_s; };
+    if (lane == 0) {
+        if (p.token_logprobs) p.token_logprobs[r] = token >= 0 ? logp(mine) : 0.0f;
+        if (p.token_ranks) p.token_ranks[r] = token >= 0 ? (int)all_before : -1;
+        if (p.entropy) p.entropy[r] = bad ? NAN : empty ? 0.0f : ln_s - t / s * kLn2;
+    }
+    if (TOP && lane < p.top) {
+        const uint64_t key = lists[0][lane];
+        const int64_t at = r * p.top + lane;
+        if (p.top_ids) p.top_ids[at] = key ? (int)~(uint32_t)key : -1;
+        if (p.top_logprobs) p.top_logprobs[at] = logp(key ? unordered((uint32_t)(key >> 32)) : -INFINITY);
+    }
+}
+
+template <typename T, bool TOP>
+cudaError_t launch_as(const Logprobs& p, int cluster, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.rows * cluster);
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cluster > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, p, cluster);
 }
 
 }  // namespace
 
-cudaError_t launch_logprobs(const Logprobs& p, int, cudaStream_t st) {
-    if (p.dtype == kRowF32) logprobs_simple_kernel<float><<<p.rows, kSimpleThreads, 0, st>>>(p);
-    else logprobs_simple_kernel<__half><<<p.rows, kSimpleThreads, 0, st>>>(p);
-    return cudaGetLastError();
+cudaError_t launch_logprobs(const Logprobs& p, int num_sms, cudaStream_t st) {
+    // CTAs of a row: enough to have two for every SM, each with a chunk's worth of
+    // work for its threads.
+    const int64_t pieces = (int64_t)p.vocab * (p.dtype == kRowF32 ? 4 : 2) / 16;
+    int cluster = 1;
+    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster < 2 * num_sms && pieces / (2 * cluster) >= kLpThreads) cluster *= 2;
+    if (p.dtype == kRowF32) return p.top ? launch_as<float, true>(p, cluster, st) : launch_as<float, false>(p, cluster, st);
+    return p.top ? launch_as<__half, true>(p, cluster, st) : launch_as<__half, false>(p, cluster, st);
 }
 
 }  // namespace lc
