@@ -89,6 +89,13 @@ struct Piece<float> {
     uint4 w;
     LC_DEV float get(int i) const { return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w); }
     LC_DEV float top() const { return max_nan(max_nan(get(0), get(1)), max_nan(get(2), get(3))); }
+    // How many are larger than v.
+    LC_DEV uint32_t above(float v) const { return (get(0) > v) + (get(1) > v) + (get(2) > v) + (get(3) > v); }
+    // The next smaller number: what is larger than it is v or larger.
+    static LC_DEV float below(float v) {
+        const int b = __float_as_int(v);
+        return __int_as_float(v > 0.0f ? b - 1 : v < 0.0f ? b + 1 : (int)0x80000001u);
+    }
 };
 template <>
 struct Piece<__half> {
@@ -102,6 +109,15 @@ struct Piece<__half> {
     LC_DEV float top() const {
         const __half2 m = __hmax2_nan(__hmax2_nan(two(0), two(1)), __hmax2_nan(two(2), two(3)));
         return max_nan(__low2float(m), __high2float(m));
+    }
+    LC_DEV uint32_t above(float v) const {
+        const __half2 t = __half2half2(__float2half_rn(v));  // exact
+        const __half2 n = __hadd2(__hadd2(__hgt2(two(0), t), __hgt2(two(1), t)), __hadd2(__hgt2(two(2), t), __hgt2(two(3), t)));
+        return (uint32_t)(__low2float(n) + __high2float(n));
+    }
+    static LC_DEV float below(float v) {
+        const int b = __half_as_ushort(__float2half_rn(v));
+        return __half2float(__ushort_as_half((unsigned short)(v > 0.0f ? b - 1 : v < 0.0f ? b + 1 : 0x8001)));
     }
 };
 
@@ -197,7 +213,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
         mine = (float)row.x[token];
         if (!(mine == mine)) mine = -INFINITY;
     }
-    const bool ranked = token >= 0 && p.token_ranks;
+    const bool ranked = token >= 0 && p.token_ranks && mine > -INFINITY;
+    const float under = Piece<T>::below(mine);
 
     // ---- the pass ----
     const float c = p.scale * kLog2e;
@@ -238,15 +255,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
         if (ranked && !(top < mine)) {
 #pragma unroll
             for (int k = 0; k < kLpPieces; ++k) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int i = row.first(j + k * kLpThreads) + e;
-                    float v = w[k].get(e);
-                    if (!(v == v)) v = -INFINITY;
-                    before += j + k * kLpThreads < p1 && row.has(i) && (v > mine || (v == mine && i < token));
-                }
+                const int i = row.first(j + k * kLpThreads);
+                before += i + N <= token ? w[k].above(under) : w[k].above(mine);
+                if (i < token && i + N > token && j + k * kLpThreads < p1)  // the token's own piece: what stands before it counts when equal
+                    for (int e = i; e < token; ++e) before += row.has(e) && (float)row.x[e] == mine;
             }
         }
+    }
+    if (token >= 0 && p.token_ranks && !ranked) {  // a masked token comes behind all that are not, and masked ones before it
+        for (int64_t i = (int64_t)p0 * N - row.skew + tid, end = (int64_t)p1 * N - row.skew; i < end; i += kLpThreads)
+            before += i >= 0 && i < p.vocab && ((float)row.x[i] > -INFINITY || i < token);
     }
 
     // ---- the CTA's part ----
@@ -292,26 +310,30 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
         at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
         if (in) chosen[at] = (uint16_t)tid;
         __syncthreads();
+        const float floor = unordered(least);
         uint64_t list = 0, bar = ((uint64_t)least << 32) - 1;  // keys above it are let in
-        for (int q = warp; q < (int)n_chosen; q += kLpWarps) {
-            for (int j = p0 + chosen[q] + lane * kLpThreads; __any_sync(0xffffffffu, j < p1); j += 32 * kLpThreads) {
-                Piece<T> w;
-                w.w = make_uint4(0, 0, 0, 0);
-                const int i = row.first(j);
-                if (j < p1) w = row.load(j);
+        // The pieces of all chosen threads side by side, one per lane.
+        const int per = (p1 - p0 + kLpThreads - 1) / kLpThreads, items = (int)n_chosen * per;
+        for (int base = warp * 32; base < items; base += kLpThreads) {
+            const int item = base + lane, q = item / per;
+            const int j = item < items ? p0 + chosen[q] + (item - q * per) * kLpThreads : p1;
+            const int i = row.first(j);
+            Piece<T> w;
+            w.w = make_uint4(0, 0, 0, 0);
+            if (j < p1) w = row.load(j);
+            if (!__any_sync(0xffffffffu, j < p1 && !(w.top() < floor))) continue;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const uint64_t key = j < p1 && row.has(i + e) ? order_key(w.get(e), i + e) : 0;
-                    unsigned todo = __ballot_sync(0xffffffffu, key > bar);
-                    while (todo) {
-                        const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
-                        const int place = __popc(__ballot_sync(0xffffffffu, list > k));
-                        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-                        list = lane < place ? list : lane == place ? k : up;
-                        bar = max(bar, (uint64_t)__shfl_sync(0xffffffffu, list, p.top - 1));
-                        todo &= todo - 1;
-                        todo &= __ballot_sync(0xffffffffu, key > bar);
-                    }
+            for (int e = 0; e < N; ++e) {
+                const uint64_t key = j < p1 && row.has(i + e) ? order_key(w.get(e), i + e) : 0;
+                unsigned todo = __ballot_sync(0xffffffffu, key > bar);
+                while (todo) {
+                    const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
+                    const int place = __popc(__ballot_sync(0xffffffffu, list > k));
+                    const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+                    list = lane < place ? list : lane == place ? k : up;
+                    bar = max(bar, (uint64_t)__shfl_sync(0xffffffffu, list, p.top - 1));
+                    todo &= todo - 1;
+                    todo &= __ballot_sync(0xffffffffu, key > bar);
                 }
             }
         }
