@@ -19,10 +19,15 @@
 // Bound by memory: 5 to 6 instructions per logit where HBM leaves time for 22
 // (F32) or 11 (F16).  Few rows are cut over a cluster of up to 16 CTAs, whose
 // parts meet in the shared memory of the first: no workspace, nothing kept.
+#include <type_traits>
+
 #include "lc_internal.h"
 #include "lc_w4.h"
 
 namespace lc {
+#ifndef LPK
+#define LPK 2
+#endif
 namespace {
 
 constexpr int kLpThreads = 256;
@@ -35,6 +40,11 @@ constexpr float kLpFloor = -200.0f;
 LC_DEV float max_nan(float a, float b) {  // a NaN wins
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+LC_DEV float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 LC_DEV float exp2_fast(float x) {  // 2 units of the last place; 0 below 2^-126
@@ -88,7 +98,13 @@ struct Piece<float> {
     static constexpr int N = 4;
     uint4 w;
     LC_DEV float get(int i) const { return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w); }
-    LC_DEV float top() const { return max_nan(max_nan(get(0), get(1)), max_nan(get(2), get(3))); }
+    LC_DEV float top() const { return max_nan(max3_nan(get(0), get(1), get(2)), get(3)); }
+    // c2 (x - ref) of elements 2 i and 2 i + 1, kLpFloor where it is less.
+    template <bool FAR>
+    LC_DEV float2 powers(int i, float ref, uint64_t c2) const {
+        const float2 u = unpack2(mul2(add2(pack2(get(2 * i), get(2 * i + 1)), pack2(-ref, -ref)), c2));
+        return make_float2(fmaxf(u.x, kLpFloor), fmaxf(u.y, kLpFloor));
+    }
     // How many are larger than v.
     LC_DEV uint32_t above(float v) const { return (get(0) > v) + (get(1) > v) + (get(2) > v) + (get(3) > v); }
     // The next smaller number: what is larger than it is v or larger.
@@ -110,6 +126,21 @@ struct Piece<__half> {
         const __half2 m = __hmax2_nan(__hmax2_nan(two(0), two(1)), __hmax2_nan(two(2), two(3)));
         return max_nan(__low2float(m), __high2float(m));
     }
+    // As above.  FAR: ref is so far above the lowest number (-65504) that its
+    // power is 0; -inf may then stand as that number, whose product with c is
+    // finite (c is 2^100 at most).  A pair's clamp is one instruction so.
+    template <bool FAR>
+    LC_DEV float2 powers(int i, float ref, uint64_t c2) const {
+        if (!FAR) {
+            const float2 u = unpack2(mul2(add2(pack2(get(2 * i), get(2 * i + 1)), pack2(-ref, -ref)), c2));
+            return make_float2(fmaxf(u.x, kLpFloor), fmaxf(u.y, kLpFloor));
+        }
+        const __half2 v = __hmax2_nan(two(i), __half2half2(__ushort_as_half(0xfbff)));
+        float a, b;
+        asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(a) : "h"(__half_as_ushort(__low2half(v))), "f"(ref));
+        asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(b) : "h"(__half_as_ushort(__high2half(v))), "f"(ref));
+        return unpack2(mul2(pack2(a, b), c2));
+    }
     LC_DEV uint32_t above(float v) const {
         const __half2 t = __half2half2(__float2half_rn(v));  // exact
         const __half2 n = __hadd2(__hadd2(__hgt2(two(0), t), __hgt2(two(1), t)), __hadd2(__hgt2(two(2), t), __hgt2(two(3), t)));
@@ -120,6 +151,12 @@ struct Piece<__half> {
         return __half2float(__ushort_as_half((unsigned short)(v > 0.0f ? b - 1 : v < 0.0f ? b + 1 : 0x8001)));
     }
 };
+
+LC_DEV uint4 load_once(const void* p) {
+    uint4 w;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p));
+    return w;
+}
 
 // A row as 16-byte pieces of memory: piece j holds elements j N - skew and on.
 template <typename T>
@@ -133,7 +170,7 @@ struct Row {
         const int i = first(j);
         Piece<T> p;
         if (i >= 0 && i + Piece<T>::N <= vocab) {
-            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p.w.x), "=r"(p.w.y), "=r"(p.w.z), "=r"(p.w.w) : "l"(x + i));
+            p.w = load_once(x + i);
         } else {
             T e[Piece<T>::N];
 #pragma unroll
@@ -217,19 +254,29 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
     const float under = Piece<T>::below(mine);
 
     // ---- the pass ----
-    const float c = p.scale * kLog2e;
+    const float c = fminf(p.scale * kLog2e, 0x1p100f);  // beyond it all smaller logits have p 0 all the same
     const uint64_t c2 = pack2(c, c);
+    const float far_from = -65504.0f - kLpFloor / c;
     float m = -INFINITY, ref = -3.4028234663852886e38f;  // ref: what exponents are taken from
     uint64_t s2 = 0, t2 = 0;  // pairs of sums
     uint32_t before = 0;
-    for (int j = p0 + tid; j < p1; j += kLpPieces * kLpThreads) {
+    // Pieces whose elements all belong to the row, and the CTA's share of them.
+    const int whole0 = max(p0, row.skew ? 1 : 0), whole1 = min(p1, (int)(((int64_t)row.skew + p.vocab) / N));
+    for (int base = p0; base < p1; base += kLpPieces * kLpThreads) {
+        const int j = base + tid;
         Piece<T> w[kLpPieces];
+        if (base >= whole0 && base + kLpPieces * kLpThreads <= whole1) {
+            const T* from = row.x + row.first(j);
 #pragma unroll
-        for (int k = 0; k < kLpPieces; ++k) {
-            const int at = j + k * kLpThreads;
-            if (at < p1) w[k] = row.load(at);
-            else w[k].w = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
-                                         : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+            for (int k = 0; k < kLpPieces; ++k) w[k].w = load_once(from + k * kLpThreads * N);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kLpPieces; ++k) {
+                const int at = j + k * kLpThreads;
+                if (at < p1) w[k] = row.load(at);
+                else w[k].w = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
+                                             : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+            }
         }
         float top = w[0].top();
 #pragma unroll
@@ -240,18 +287,20 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
         ref = now;
         t2 = mul2(fma2(s2, pack2(d, d), t2), pack2(down, down));
         s2 = mul2(s2, pack2(down, down));
-        const uint64_t ref2 = pack2(-ref, -ref);
+        auto add_up = [&](auto far) {
 #pragma unroll
-        for (int k = 0; k < kLpPieces; ++k) {
+            for (int k = 0; k < kLpPieces; ++k) {
 #pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                const float2 u = unpack2(mul2(add2(pack2(w[k].get(e), w[k].get(e + 1)), ref2), c2));
-                const float u0 = fmaxf(u.x, kLpFloor), u1 = fmaxf(u.y, kLpFloor);
-                const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
-                s2 = add2(s2, e2);
-                t2 = fma2(e2, pack2(u0, u1), t2);
+                for (int i = 0; i < N / 2; ++i) {
+                    const float2 u = w[k].template powers<decltype(far)::value>(i, ref, c2);
+                    const uint64_t e2 = pack2(exp2_fast(u.x), exp2_fast(u.y));
+                    s2 = add2(s2, e2);
+                    t2 = fma2(e2, pack2(u.x, u.y), t2);
+                }
             }
-        }
+        };
+        if (sizeof(T) == 2 && ref > far_from) add_up(std::true_type());
+        else add_up(std::false_type());
         if (ranked && !(top < mine)) {
 #pragma unroll
             for (int k = 0; k < kLpPieces; ++k) {
@@ -424,7 +473,7 @@ cudaError_t launch_logprobs(const Logprobs& p, int num_sms, cudaStream_t st) {
     // work for its threads.
     const int64_t pieces = (int64_t)p.vocab * (p.dtype == kRowF32 ? 4 : 2) / 16;
     int cluster = 1;
-    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster < 2 * num_sms && pieces / (2 * cluster) >= kLpThreads) cluster *= 2;
+    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster < LPK * num_sms && pieces / (2 * cluster) >= kLpThreads) cluster *= 2;
     if (p.dtype == kRowF32) return p.top ? launch_as<float, true>(p, cluster, st) : launch_as<float, false>(p, cluster, st);
     return p.top ? launch_as<__half, true>(p, cluster, st) : launch_as<__half, false>(p, cluster, st);
 }
