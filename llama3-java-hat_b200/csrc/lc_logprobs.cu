@@ -25,14 +25,12 @@
 #include "lc_w4.h"
 
 namespace lc {
-#ifndef LPK
-#define LPK 2
-#endif
 namespace {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpPieces = 4;       // 16-byte pieces of a thread's chunk
+constexpr uint32_t kLpFound = 256;  // candidates that are put in order by counting
 constexpr int kLpMaxCluster = 16;  // more than 8 is opt-in
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLpFloor = -200.0f;
@@ -98,6 +96,10 @@ struct Piece<float> {
     static constexpr int N = 4;
     uint4 w;
     LC_DEV float get(int i) const { return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w); }
+    LC_DEV float at(int i) const {  // of a place known only at run time
+        const uint32_t lo = i & 1 ? w.y : w.x, hi = i & 1 ? w.w : w.z;
+        return __uint_as_float(i & 2 ? hi : lo);
+    }
     LC_DEV float top() const { return max_nan(max3_nan(get(0), get(1), get(2)), get(3)); }
     // c2 (x - ref) of elements 2 i and 2 i + 1, kLpFloor where it is less.
     template <bool FAR>
@@ -122,6 +124,10 @@ struct Piece<__half> {
         return *reinterpret_cast<const __half2*>(&v);
     }
     LC_DEV float get(int i) const { return i & 1 ? __high2float(two(i >> 1)) : __low2float(two(i >> 1)); }
+    LC_DEV float at(int i) const {
+        const uint32_t lo = i & 2 ? w.y : w.x, hi = i & 2 ? w.w : w.z, v = i & 4 ? hi : lo;
+        return __half2float(__ushort_as_half((unsigned short)(i & 1 ? v >> 16 : v)));
+    }
     LC_DEV float top() const {
         const __half2 m = __hmax2_nan(__hmax2_nan(two(0), two(1)), __hmax2_nan(two(2), two(3)));
         return max_nan(__low2float(m), __high2float(m));
@@ -222,13 +228,14 @@ struct Part {  // of a CTA's share of a row
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int cluster) {
+__global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int cluster) {
     __shared__ Part parts[kLpMaxCluster];
-    __shared__ __align__(16) uint32_t tops[kLpThreads];
+    __shared__ __align__(16) __half tops[TOP ? kLpThreads : 1];
+    __shared__ uint64_t found[TOP ? kLpFound + 32 * kLpWarps : 1];
     __shared__ uint64_t lists[TOP ? kLpMaxCluster : 1][32];
     __shared__ uint64_t ours[TOP ? kLpWarps : 1][32];
     __shared__ uint16_t chosen[TOP ? kLpThreads : 1];
-    __shared__ uint32_t warp_top[kLpWarps], warp_before[kLpWarps], n_chosen, least;
+    __shared__ uint32_t warp_top[kLpWarps], warp_before[kLpWarps], n_chosen, n_found, least;
     __shared__ float warp_s[kLpWarps], warp_t[kLpWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
@@ -243,16 +250,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
     constexpr int N = Piece<T>::N;
     const int64_t pieces = ((int64_t)row.skew + p.vocab + N - 1) / N;
     const int p0 = (int)(pieces * rank / cluster), p1 = (int)(pieces * (rank + 1) / cluster);
-    int token = p.tokens ? p.tokens[r] : -1;
-    if (token >= p.vocab) token = -1;
-    float mine = INFINITY;  // the token's logit
-    if (token >= 0) {
-        mine = (float)row.x[token];
-        if (!(mine == mine)) mine = -INFINITY;
-    }
-    const bool ranked = token >= 0 && p.token_ranks && mine > -INFINITY;
-    const float under = Piece<T>::below(mine);
-
     // ---- the pass ----
     const float c = fminf(p.scale * kLog2e, 0x1p100f);  // beyond it all smaller logits have p 0 all the same
     const uint64_t c2 = pack2(c, c);
@@ -262,22 +259,39 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
     uint32_t before = 0;
     // Pieces whose elements all belong to the row, and the CTA's share of them.
     const int whole0 = max(p0, row.skew ? 1 : 0), whole1 = min(p1, (int)(((int64_t)row.skew + p.vocab) / N));
-    for (int base = p0; base < p1; base += kLpPieces * kLpThreads) {
+    Piece<T> next[kLpPieces];
+    auto fetch = [&](int base) {  // the thread's pieces of the chunk at base, -inf behind the share
         const int j = base + tid;
-        Piece<T> w[kLpPieces];
         if (base >= whole0 && base + kLpPieces * kLpThreads <= whole1) {
             const T* from = row.x + row.first(j);
 #pragma unroll
-            for (int k = 0; k < kLpPieces; ++k) w[k].w = load_once(from + k * kLpThreads * N);
+            for (int k = 0; k < kLpPieces; ++k) next[k].w = load_once(from + k * kLpThreads * N);
         } else {
 #pragma unroll
             for (int k = 0; k < kLpPieces; ++k) {
                 const int at = j + k * kLpThreads;
-                if (at < p1) w[k] = row.load(at);
-                else w[k].w = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
-                                             : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+                if (at < p1) next[k] = row.load(at);
+                else next[k].w = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
+                                                : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
             }
         }
+    };
+    fetch(p0);
+    int token = p.tokens ? p.tokens[r] : -1;
+    if (token >= p.vocab) token = -1;
+    float mine = INFINITY;  // the token's logit
+    if (token >= 0) {
+        mine = (float)row.x[token];
+        if (!(mine == mine)) mine = -INFINITY;
+    }
+    const bool ranked = token >= 0 && p.token_ranks && mine > -INFINITY;
+    const float under = Piece<T>::below(mine);
+    for (int base = p0; base < p1; base += kLpPieces * kLpThreads) {
+        const int j = base + tid;
+        Piece<T> w[kLpPieces];
+#pragma unroll
+        for (int k = 0; k < kLpPieces; ++k) w[k] = next[k];
+        if (base + kLpPieces * kLpThreads < p1) fetch(base + kLpPieces * kLpThreads);
         float top = w[0].top();
 #pragma unroll
         for (int k = 1; k < kLpPieces; ++k) top = max_nan(top, w[k].top());
@@ -322,8 +336,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
     const uint32_t wt = __reduce_max_sync(0xffffffffu, my_top);
     before = __reduce_add_sync(0xffffffffu, before);
     if (lane == 0) warp_top[warp] = wt, warp_before[warp] = before;
-    if (tid == 0) n_chosen = 0, least = 0xffffffffu;
-    if (TOP) tops[tid] = my_top;
+    if (tid == 0) n_chosen = n_found = 0, least = 0xffffffffu;
+    if (TOP) tops[tid] = __float2half_rd(m);
     __syncthreads();
     uint32_t cta_top = warp_top[0];
 #pragma unroll
@@ -341,13 +355,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
         // Threads with fewer than `top` larger maxima above their own.
         bool in = cta_top == 0xffffffffu;  // a NaN hides a maximum: then all
         if (!in) {
-            int above = 0;
+            // Rounded down to f16 they keep their order, but for ties, which let in more.
+            const __half2 m2 = __half2half2(tops[tid]);
+            __half2 above = __half2half2(__ushort_as_half(0));
 #pragma unroll 8
-            for (int i = 0; i < kLpThreads / 4; ++i) {
+            for (int i = 0; i < kLpThreads / 8; ++i) {
                 const uint4 o = reinterpret_cast<const uint4*>(tops)[i];
-                above += (o.x > my_top) + (o.y > my_top) + (o.z > my_top) + (o.w > my_top);
+                const __half2* h = reinterpret_cast<const __half2*>(&o);
+                above = __hadd2(above, __hadd2(__hadd2(__hgt2(h[0], m2), __hgt2(h[1], m2)), __hadd2(__hgt2(h[2], m2), __hgt2(h[3], m2))));
             }
-            in = above < p.top;
+            in = (int)(__low2float(above) + __high2float(above)) < p.top;
         }
         const uint32_t low = __reduce_min_sync(0xffffffffu, in ? (cta_top == 0xffffffffu ? kOrderedMasked : my_top) : 0xffffffffu);
         const unsigned who = __ballot_sync(0xffffffffu, in);
@@ -359,35 +376,114 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(Logprobs p, int
         at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
         if (in) chosen[at] = (uint16_t)tid;
         __syncthreads();
+        // The pieces of all chosen threads side by side, one per lane; what reaches
+        // the least of their maxima is set aside.
         const float floor = unordered(least);
-        uint64_t list = 0, bar = ((uint64_t)least << 32) - 1;  // keys above it are let in
-        // The pieces of all chosen threads side by side, one per lane.
+        const uint64_t bar = (uint64_t)least << 32;
         const int per = (p1 - p0 + kLpThreads - 1) / kLpThreads, items = (int)n_chosen * per;
-        for (int base = warp * 32; base < items; base += kLpThreads) {
-            const int item = base + lane, q = item / per;
-            const int j = item < items ? p0 + chosen[q] + (item - q * per) * kLpThreads : p1;
-            const int i = row.first(j);
-            Piece<T> w;
-            w.w = make_uint4(0, 0, 0, 0);
+        auto item_of = [&](int item, Piece<T>& w) {
+            const int q = item / per, j = item < items ? p0 + chosen[q] + (item - q * per) * kLpThreads : p1;
             if (j < p1) w = row.load(j);
-            if (!__any_sync(0xffffffffu, j < p1 && !(w.top() < floor))) continue;
+            return j;
+        };
+        auto collect = [&](uint64_t from, bool above) {  // keys from `from` on; above: larger than floor
+            for (int item = tid; item < items && *(volatile uint32_t*)&n_found <= kLpFound; item += 4 * kLpThreads) {
+                Piece<T> w[4];
+                int j[4];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const uint64_t key = j < p1 && row.has(i + e) ? order_key(w.get(e), i + e) : 0;
-                unsigned todo = __ballot_sync(0xffffffffu, key > bar);
-                while (todo) {
-                    const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
-                    const int place = __popc(__ballot_sync(0xffffffffu, list > k));
-                    const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-                    list = lane < place ? list : lane == place ? k : up;
-                    bar = max(bar, (uint64_t)__shfl_sync(0xffffffffu, list, p.top - 1));
-                    todo &= todo - 1;
-                    todo &= __ballot_sync(0xffffffffu, key > bar);
+                for (int z = 0; z < 4; ++z) j[z] = item_of(item + z * kLpThreads, w[z]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    if (j[z] >= p1 || (above ? w[z].top() <= floor : w[z].top() < floor)) continue;
+#pragma unroll 1
+                    for (int e = 0, i = row.first(j[z]); e < N; ++e, ++i) {
+                        const uint64_t key = order_key(w[z].at(e), i);
+                        if (key < from || !row.has(i)) continue;
+                        const uint32_t at = atomicAdd(&n_found, 1u);
+                        if (at < kLpFound) found[at] = key;
+                    }
                 }
             }
+        };
+        // Where so few are allowed that masked ones are among the best there are
+        // more of these than fit, as a rule.
+        bool fit = least > ordered(sizeof(T) == 4 ? -3.4028234663852886e38f : -65504.0f);
+        if (fit) collect(bar, false);
+        if (warp == 0) ours[0][lane] = 0;
+        __syncthreads();
+        fit = fit && n_found <= kLpFound;
+        if (!fit) {
+            // Equal logits by the hundred, such as masked ones where few are allowed:
+            // those above them, and then of each warp's part of the share the first
+            // that are equal, as many as may be needed.
+            __syncthreads();
+            if (tid == 0) n_found = 0;
+            __syncthreads();
+            if (least < cta_top) collect(bar + (1ull << 32), true);
+            __syncthreads();
+            fit = n_found <= kLpFound;
+            if (fit) {
+                const int q0 = p0 + (int)((int64_t)(p1 - p0) * warp / kLpWarps), q1 = p0 + (int)((int64_t)(p1 - p0) * (warp + 1) / kLpWarps);
+                __syncthreads();  // all have read the count
+                int got = 0;
+                for (int j = q0 + lane; __any_sync(0xffffffffu, j < q1) && got < p.top; j += 32) {
+                    Piece<T> w;
+                    if (j < q1) w = row.load(j);
+                    const int i = row.first(j);
+                    unsigned equal = 0;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) equal |= (unsigned)(j < q1 && row.has(i + e) && ordered(w.get(e)) == least) << e;
+                    int upto = __popc(equal);
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += u;
+                    }
+                    int place = got + upto - __popc(equal);
+                    for (; equal && place < p.top; equal &= equal - 1, ++place) {
+                        const uint32_t at = atomicAdd(&n_found, 1u);
+                        found[at] = (uint64_t)least << 32 | (uint32_t)~(i + __ffs(equal) - 1);
+                    }
+                    got += __shfl_sync(0xffffffffu, upto, 31);
+                }
+                __syncthreads();
+            }
         }
-        ours[warp][lane] = list;
-        join_lists(ours, kLpWarps, warp, lane);
+        if (fit) {
+            // Each one's place is the number of larger ones.
+            for (int q = tid; q < (int)n_found; q += kLpThreads) {
+                const uint64_t key = found[q];
+                int place = 0;
+                for (int o = 0; o < (int)n_found; ++o) place += found[o] > key;
+                if (place < 32) ours[0][place] = key;
+            }
+            __syncthreads();
+        } else {
+            // Hundreds above the least maximum in the few threads that have them: every
+            // warp keeps the best of its share in order, a key per lane.
+            uint64_t list = 0, edge = bar - 1;
+            for (int base = warp * 32; base < items; base += kLpThreads) {
+                Piece<T> w;
+                w.w = make_uint4(0, 0, 0, 0);
+                const int j = item_of(base + lane, w), i = row.first(j);
+#pragma unroll 1
+                for (int e = 0; e < N; ++e) {
+                    const uint64_t key = j < p1 && row.has(i + e) ? order_key(w.at(e), i + e) : 0;
+                    unsigned todo = __ballot_sync(0xffffffffu, key > edge);
+                    while (todo) {
+                        const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
+                        const int place = __popc(__ballot_sync(0xffffffffu, list > k));
+                        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+                        list = lane < place ? list : lane == place ? k : up;
+                        edge = max(edge, (uint64_t)__shfl_sync(0xffffffffu, list, p.top - 1));
+                        todo &= todo - 1;
+                        todo &= __ballot_sync(0xffffffffu, key > edge);
+                    }
+                }
+            }
+            ours[warp][lane] = list;
+            join_lists(ours, kLpWarps, warp, lane);
+        }
     } else {
         __syncthreads();
     }
@@ -473,7 +569,7 @@ cudaError_t launch_logprobs(const Logprobs& p, int num_sms, cudaStream_t st) {
     // work for its threads.
     const int64_t pieces = (int64_t)p.vocab * (p.dtype == kRowF32 ? 4 : 2) / 16;
     int cluster = 1;
-    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster < LPK * num_sms && pieces / (2 * cluster) >= kLpThreads) cluster *= 2;
+    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster < 2 * num_sms && pieces / (2 * cluster) >= kLpThreads) cluster *= 2;
     if (p.dtype == kRowF32) return p.top ? launch_as<float, true>(p, cluster, st) : launch_as<float, false>(p, cluster, st);
     return p.top ? launch_as<__half, true>(p, cluster, st) : launch_as<__half, false>(p, cluster, st);
 }
