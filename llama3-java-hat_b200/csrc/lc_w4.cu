@@ -1,12 +1,13 @@
 // lc_w4.cu -- 4-bit weights: quantising rows of values, packing codes that a
 // checkpoint holds, and reading values back.  Layout: lc_w4.h.
 //
-// A warp has a block of 16 rows x 128 columns, a lane 16 columns of two rows in
-// each half of it, as the layout wants them; a group's largest value is then a
-// maximum over 1, 3 or 7 neighbours.  With s the group's scale, every code is
-// the nearest to the exact quotient x / s, ties to even: x (1 / s) is two units
-// of the last place off at most, and only where that could change the code
-// (the remainder x - q s is near half a step) is the exact remainder asked.
+// A warp has a block of 16 rows x 128 columns, a lane four runs of eight columns
+// of two rows, as the layout wants them; a group's largest value is then a
+// maximum over 4 lanes and 1, 2 or 4 of their runs.  With s the group's scale,
+// every code is the nearest to the exact quotient x / s, ties to even: x (1 / s)
+// is two units of the last place off at most, and only where that could change
+// the code (the remainder x - q s is near half a step) is the exact remainder
+// asked.
 //
 // Bound by memory: values in once, codes out once, and the reverse.
 #include "lc_internal.h"
@@ -19,6 +20,9 @@ constexpr int kW4Threads = 256;
 constexpr int kW4Warps = kW4Threads / 32;
 constexpr int kW4Half = 64;            // columns of half a block
 constexpr int kW4Pitch = kW4Half + 4;  // floats between rows of the exchange buffer
+
+LC_DEV uint32_t turned(uint32_t w) { return __funnelshift_l(w, w, kW4Turn); }
+LC_DEV uint32_t unturned(uint32_t w) { return __funnelshift_r(w, w, kW4Turn); }
 
 template <typename T>
 LC_DEV float to_f32(T v);
@@ -50,26 +54,26 @@ LC_DEV float settle(float x, float s, float near) {
     return a > s || (a == s && odd) ? near + copysignf(1.0f, rest) : near;
 }
 
-// Quotients of 16 values as whole numbers in [-16, 16].
-LC_DEV void quotients(const float (&x)[16], float s, float inv, float (&q)[16]) {
+// Quotients of eight values as whole numbers in [-16, 16].
+LC_DEV void quotients(const float (&x)[8], float s, float inv, float (&q)[8]) {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
     const float sure = s * (0.5f - 0x1p-16f);
     bool all = true;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float t = fminf(fmaxf(x[i] * inv, -16.0f), 16.0f);
         q[i] = (t + kMagic) - kMagic;
         all = all && fabsf(__fmaf_rn(-q[i], s, x[i])) < sure;
     }
     if (all) return;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i)
         if (fabsf(q[i]) < 16.0f) q[i] = settle(x[i], s, q[i]);
 }
 
-// Columns c0 .. c0 + 15 of rows r and r + 8 (both halves of the warp's rows)
-// from memory: by the lane itself where 16-byte loads may be used, else row by
-// row through shared memory, so that neighbours read neighbours.
+// The lane's columns col0 + 32 q + 8 t + i (element 8 q + i) of half a block, of
+// its rows g (a) and g + 8 (b): read by the lane itself where 16-byte loads may be
+// used, else row by row through shared memory, so that neighbours read neighbours.
 template <typename T>
 LC_DEV void load_half(const T* p, int64_t stride, int row0, int rows, int col0, int cols, bool vec, float* buf, int lane,
                       float (&a)[16], float (&b)[16]) {
@@ -83,7 +87,8 @@ LC_DEV void load_half(const T* p, int64_t stride, int row0, int rows, int col0, 
 #pragma unroll
             for (int i = 0; i < 16 / V; ++i) {
                 uint4 w = make_uint4(0, 0, 0, 0);
-                if (r < rows) w = __ldg(reinterpret_cast<const uint4*>(p + r * stride + col0 + 16 * t) + i);
+                constexpr int R = 8 / V;  // loads of a run
+                if (r < rows) w = __ldg(reinterpret_cast<const uint4*>(p + r * stride + col0 + 32 * (i / R) + 8 * t) + i % R);
                 const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
                 for (int k = 0; k < V; ++k) o[i * V + k] = to_f32<T>(e[k]);
@@ -103,8 +108,9 @@ LC_DEV void load_half(const T* p, int64_t stride, int row0, int rows, int col0, 
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float4 u = *reinterpret_cast<const float4*>(buf + g * kW4Pitch + 16 * t + 4 * i);
-        const float4 v = *reinterpret_cast<const float4*>(buf + (g + 8) * kW4Pitch + 16 * t + 4 * i);
+        const int at = 32 * (i >> 1) + 8 * t + 4 * (i & 1);
+        const float4 u = *reinterpret_cast<const float4*>(buf + g * kW4Pitch + at);
+        const float4 v = *reinterpret_cast<const float4*>(buf + (g + 8) * kW4Pitch + at);
         a[4 * i] = u.x, a[4 * i + 1] = u.y, a[4 * i + 2] = u.z, a[4 * i + 3] = u.w;
         b[4 * i] = v.x, b[4 * i + 1] = v.y, b[4 * i + 2] = v.z, b[4 * i + 3] = v.w;
     }
@@ -138,78 +144,80 @@ template <typename T, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4Threads) w4_quantize_kernel(W4 w, const T* __restrict__ values, int64_t stride, bool vec) {
     __shared__ __align__(16) float buf[kW4Warps][kW4Rows * kW4Pitch];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    constexpr int NG = kW4Cols / GROUP;        // groups of a block
-    constexpr int SPAN = GROUP / 16 < 4 ? GROUP / 16 : 4;  // lanes of a group in one half
+    constexpr int NG = kW4Cols / GROUP;  // groups of a block
     const int64_t units = (int64_t)w.tiles * w.blocks;
     for (int64_t u = (int64_t)blockIdx.x * kW4Warps + warp; u < units; u += (int64_t)gridDim.x * kW4Warps) {
         const int tile = (int)(u / w.blocks), block = (int)(u - (int64_t)tile * w.blocks);
-        float x[2][2][16];  // [half][row g or g + 8]
-        float low[2][2], high[2][2];
+        float x[2][2][16];               // [half][row g or g + 8]
+        float low[2][4], high[2][4];     // [row][group of 32 columns]
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             load_half<T>(values, stride, tile * kW4Rows, w.rows, block * kW4Cols + h * kW4Half, w.cols, vec, buf[warp], lane, x[h][0], x[h][1]);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float& v = x[h][k][i];
-                    if (!(v == v)) v = 0.0f;
-                    if (fabsf(v) < INFINITY) lo = fminf(lo, v), hi = fmaxf(hi, v);
+                for (int q = 0; q < 2; ++q) {
+                    float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float& v = x[h][k][8 * q + i];
+                        if (!(v == v)) v = 0.0f;
+                        if (fabsf(v) < INFINITY) lo = fminf(lo, v), hi = fmaxf(hi, v);
+                    }
+                    low[k][2 * h + q] = lo, high[k][2 * h + q] = hi;
                 }
+            }
+        }
+        Step step[2][NG];
 #pragma unroll
-                for (int o = 1; o < SPAN; o <<= 1) {
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                float lo = low[k][i * (4 / NG)], hi = high[k][i * (4 / NG)];
+#pragma unroll
+                for (int q = 1; q < 4 / NG; ++q) lo = fminf(lo, low[k][i * (4 / NG) + q]), hi = fmaxf(hi, high[k][i * (4 / NG) + q]);
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
                     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
                     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
                 }
-                low[h][k] = lo, high[h][k] = hi;
-            }
-        }
-        if (GROUP == 128) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                low[0][k] = low[1][k] = fminf(low[0][k], low[1][k]);
-                high[0][k] = high[1][k] = fmaxf(high[0][k], high[1][k]);
+                step[k][i] = step_of<ZEROS>(lo, hi);
             }
         }
         uint4* out = reinterpret_cast<uint4*>(w.codes + u * kW4BlockBytes);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t word[4] = {0, 0, 0, 0};
-            Step step[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                step[k] = step_of<ZEROS>(low[h][k], high[h][k]);
-                float q[16];
-                const float s = step[k].s;
-                if (s > 0.0f) {
-                    quotients(x[h][k], s, __frcp_rn(s), q);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) q[i] = 0.0f;
-                }
+                for (int run = 0; run < 2; ++run) {
+                    const Step& st = step[k][(2 * h + run) / (4 / NG)];
+                    float v[8], q[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float c = ZEROS ? fminf(fmaxf(q[i] + step[k].zero, 0.0f), 15.0f) : fminf(fmaxf(q[i], -7.0f), 7.0f) + 8.0f;
-                    constexpr int kBit[4] = {0, 16, 8, 24};
-                    const int col = block * kW4Cols + h * kW4Half + 16 * t + i;
-                    const uint32_t code = col < w.cols ? (uint32_t)c : 0u;
-                    word[i >> 2] |= code << (kBit[i & 3] + 4 * k);
+                    for (int i = 0; i < 8; ++i) v[i] = x[h][k][8 * run + i], q[i] = 0.0f;
+                    if (st.s > 0.0f) quotients(v, st.s, __frcp_rn(st.s), q);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float c = ZEROS ? fminf(fmaxf(q[i] + st.zero, 0.0f), 15.0f) : fminf(fmaxf(q[i], -7.0f), 7.0f) + 8.0f;
+                        constexpr int kBit[4] = {0, 16, 8, 24};
+                        const int col = block * kW4Cols + h * kW4Half + 32 * run + 8 * t + i;
+                        const uint32_t code = col < w.cols ? (uint32_t)c : 0u;
+                        word[2 * run + (i >> 2)] |= code << (kBit[i & 3] + 4 * k);
+                    }
                 }
             }
-            out[h * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
-            // The first lane of a group in this half writes its pair; groups of 128 once.
-            const int first = block * kW4Cols + h * kW4Half + 16 * t;
-            if (t % SPAN == 0 && (GROUP < 128 || h == 0)) {
-                const int i = GROUP == 128 ? 0 : (h * kW4Half + 16 * t) / GROUP;
-                const int64_t at = (u * 8 + g) * NG + i;
-                const bool there = first < w.cols;
-                const uint32_t s0 = there && tile * kW4Rows + g < w.rows ? step[0].bits : 0u;
-                const uint32_t s1 = there && tile * kW4Rows + g + 8 < w.rows ? step[1].bits : 0u;
-                reinterpret_cast<uint32_t*>(w.scales)[at] = s0 | s1 << 16;
-                if (ZEROS)
-                    reinterpret_cast<uint16_t*>(w.zeros)[at] = (uint16_t)((uint32_t)step[0].zero | (uint32_t)step[1].zero << 8);
-            }
+            out[h * 32 + lane] = make_uint4(turned(word[0]), turned(word[1]), turned(word[2]), turned(word[3]));
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            if (t != i) continue;  // lane t writes the pair of group t
+            const bool there = block * kW4Cols + i * GROUP < w.cols;
+            const int64_t at = (u * 8 + g) * NG + i;
+            const uint32_t s0 = there && tile * kW4Rows + g < w.rows ? step[0][i].bits : 0u;
+            const uint32_t s1 = there && tile * kW4Rows + g + 8 < w.rows ? step[1][i].bits : 0u;
+            reinterpret_cast<uint32_t*>(w.scales)[at] = s0 | s1 << 16;
+            if (ZEROS) reinterpret_cast<uint16_t*>(w.zeros)[at] = (uint16_t)((uint32_t)step[0][i].zero | (uint32_t)step[1][i].zero << 8);
         }
     }
 }
@@ -233,17 +241,17 @@ __global__ void __launch_bounds__(kW4Threads) w4_pack_kernel(W4 w, const uint8_t
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int row = tile * kW4Rows + g + 8 * k;
-                const int col = block * kW4Cols + h * kW4Half + 16 * t;
+                const int col = block * kW4Cols + h * kW4Half + 8 * t;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {  // a byte: columns col + 2 i (low half) and the next
-                    const int c = col + 2 * i;
+                for (int i = 0; i < 8; ++i) {  // a byte: column c (low half) and the next
+                    const int c = col + 32 * (i >> 2) + 2 * (i & 3);
                     uint32_t b = row < w.rows && c < w.cols ? codes[row * pitch + (c >> 1)] : 0u;
                     if (c + 1 >= w.cols) b &= 15u;
                     constexpr int kBit[2] = {0, 8};
                     word[i >> 1] |= (b & 15u) << (kBit[i & 1] + 4 * k) | (b >> 4) << (kBit[i & 1] + 16 + 4 * k);
                 }
             }
-            out[h * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+            out[h * 32 + lane] = make_uint4(turned(word[0]), turned(word[1]), turned(word[2]), turned(word[3]));
         }
         for (int i = lane; i < 8 * NG * 2; i += 32) {
             const int row = tile * kW4Rows + i / (2 * NG) + 8 * (i & 1);
@@ -268,23 +276,26 @@ __global__ void __launch_bounds__(kW4Threads) w4_read_kernel(W4 w, T* __restrict
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint4 word = in[h * 32 + lane];
-            const uint32_t ws[4] = {word.x, word.y, word.z, word.w};
+            const uint32_t ws[4] = {unturned(word.x), unturned(word.y), unturned(word.z), unturned(word.w)};
             const int col0 = block * kW4Cols + h * kW4Half;
-            const int64_t at = (u * 8 + g) * NG + (h * kW4Half + 16 * t) / GROUP;
-            const uint32_t sc = reinterpret_cast<const uint32_t*>(w.scales)[at];
-            const uint32_t zp = ZEROS ? reinterpret_cast<const uint16_t*>(w.zeros)[at] : 0x0808u;
+            uint32_t sc[2], zp[2];  // of the two runs
+#pragma unroll
+            for (int run = 0; run < 2; ++run) {
+                const int64_t at = (u * 8 + g) * NG + (2 * h + run) / (4 / NG);
+                sc[run] = reinterpret_cast<const uint32_t*>(w.scales)[at];
+                zp[run] = ZEROS ? reinterpret_cast<const uint16_t*>(w.zeros)[at] : 0x0808u;
+            }
             const bool direct = vec && col0 + kW4Half <= w.cols;
             if (!direct) __syncwarp();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float s = __half2float(__ushort_as_half((uint16_t)(sc >> (16 * k))));
-                const int zero = (zp >> (8 * k)) & 255;
                 const int row = tile * kW4Rows + g + 8 * k;
                 float v[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     constexpr int kBit[4] = {0, 16, 8, 24};
-                    v[i] = s * (float)((int)((ws[i >> 2] >> (kBit[i & 3] + 4 * k)) & 15u) - zero);
+                    const float s = __half2float(__ushort_as_half((uint16_t)(sc[i >> 3] >> (16 * k))));
+                    v[i] = s * (float)((int)((ws[i >> 2] >> (kBit[i & 3] + 4 * k)) & 15u) - (int)((zp[i >> 3] >> (8 * k)) & 255u));
                 }
                 if (direct) {
                     constexpr int V = 16 / sizeof(T);
@@ -294,13 +305,14 @@ __global__ void __launch_bounds__(kW4Threads) w4_read_kernel(W4 w, T* __restrict
                             T e[V];
 #pragma unroll
                             for (int j = 0; j < V; ++j) e[j] = from_f32<T>(v[i * V + j]);
-                            *(reinterpret_cast<uint4*>(values + row * stride + col0 + 16 * t) + i) = *reinterpret_cast<const uint4*>(e);
+                            constexpr int R = 8 / V;
+                            *(reinterpret_cast<uint4*>(values + row * stride + col0 + 32 * (i / R) + 8 * t) + i % R) = *reinterpret_cast<const uint4*>(e);
                         }
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<float4*>(&buf[warp][(g + 8 * k) * kW4Pitch + 16 * t + 4 * i]) =
+                        *reinterpret_cast<float4*>(&buf[warp][(g + 8 * k) * kW4Pitch + 32 * (i >> 1) + 8 * t + 4 * (i & 1)]) =
                             make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 }
             }

@@ -4,15 +4,17 @@
 //
 // Layout.  Codes lie in tiles of 16 rows and blocks of 128 columns, [tiles]
 // [blocks][1024 bytes]; 16 bytes of each 512 (a chunk of 64 columns) belong to
-// lane 4 g + t of the warp that reads them: rows g and g + 8, columns 16 t ..
-// 16 t + 15.  Word j of the 16 bytes holds columns 16 t + 4 j + e, e = 0..3, at
-// bit {0, 16, 8, 24}[e] for row g and 4 bits higher for row g + 8.  So the
-// words masked by 0x000f000f and 0x00f000f0, before and after a shift by 8, are
-// the four registers that one m16n8k16 product takes from the lane, as pairs of
-// f16 numbers c 2^-24 and (rows g + 8) c 2^-20; and 16 columns of one row are
-// two runs of 16 bytes of f16 values, which is what tcgen05 operands are made
-// of.  The order of columns within a product does not matter as long as both
-// operands have the same.
+// lane 4 g + t of the warp that reads them: rows g and g + 8, and of each 32
+// columns the eight from 8 t on.  Word j of the 16 bytes holds columns
+// 32 (j / 2) + 8 t + 4 (j % 2) + e, e = 0..3, at bit {0, 16, 8, 24}[e] for row g
+// and 4 bits higher for row g + 8, the whole word rotated left by 3.  So the word
+// rotated by 4, 0, -4 and -8 bits to the left and masked by 0x07800780 gives the
+// four registers that one m16n8k16 product takes from the lane, as pairs of f16
+// numbers c 2^-17 (seven instructions for eight codes; f16 numbers below 2^-13
+// are linear in their bits); each product lies within one group; and what the
+// lane has of a row are runs of eight columns, 16 bytes of f16, which is what
+// tcgen05 operands are made of.  The order of columns within a product does not
+// matter as long as both operands have the same.
 //
 // Scales (f16) and zero points (bytes) of a block: [8 g][128 / group][2], the
 // pair being rows g and g + 8.  Columns behind the last have code 0, rows
@@ -29,6 +31,7 @@ namespace lc {
 constexpr int kW4Rows = 16;    // rows of a tile
 constexpr int kW4Cols = 128;   // columns of a block
 constexpr int kW4BlockBytes = 1024;
+constexpr int kW4Turn = 3;  // bits by which words are rotated
 
 struct W4 {
     uint8_t* codes;

@@ -4,63 +4,79 @@
 // The inner sums are of whole numbers times x; a group's scale is applied once.
 #include "lc_internal.h"
 #include "lc_w4.h"
+#include "lc_w4_few.cuh"
 
 namespace lc {
 namespace {
 
-constexpr int kSimpleRows = 128, kSimpleBatch = 8;
+// Rows of x that one launch of the kernel for few rows takes.
+constexpr int few_rows(int dtype) { return dtype == kRowF32 ? 16 : 32; }
 
-template <typename T>
-LC_DEV float w4_f32(T v) { return (float)v; }
+template <typename T, int GROUP, bool ZEROS, int NT>
+cudaError_t few_as(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
+    using S = FewShape<T, GROUP, NT>;
+    constexpr size_t kTwo = 113 * 1024, kOne = 226 * 1024;  // shared memory with which two CTAs, or one, fit an SM
+    FewPlan plan;
+    plan.cluster = plan.phases = 1;
+    auto blocks = [&] { return (w.blocks + plan.cluster * plan.phases * kFewWarps - 1) / (plan.cluster * plan.phases * kFewWarps); };
+    // More CTAs for the columns while a CTA's part would keep a second CTA off the
+    // SM, or while there are SMs without one and each warp has two blocks to share.
+    while (plan.cluster < kFewMaxCluster && w.blocks >= 2 * plan.cluster * kFewWarps &&
+           (S::smem(blocks()) > kTwo || w.tiles * plan.cluster < num_sms))
+        plan.cluster *= 2;
+    while (S::smem(blocks()) > kOne) ++plan.phases;
+    plan.blocks = blocks();
+    const int most = 2 * num_sms / plan.cluster;
+    plan.clusters = w.tiles < most ? w.tiles : most;
+    auto* kernel = w4_few_kernel<T, GROUP, ZEROS, NT>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOne);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(plan.clusters * plan.cluster));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = S::smem(plan.blocks);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)plan.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, w, p, plan);
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kSimpleRows) w4_simple_kernel(W4 w, W4Product p) {
-    __shared__ float xs[kSimpleBatch][kW4Cols];
-    const int row = blockIdx.x * kSimpleRows + threadIdx.x, b0 = blockIdx.y * kSimpleBatch;
-    const int tile = row / kW4Rows, r = row % kW4Rows, g = r & 7, up = r >> 3, ng = kW4Cols / w.group;
-    const T* x = (const T*)p.x;
-    float total[kSimpleBatch] = {};
-    for (int block = 0; block < w.blocks; ++block) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kSimpleBatch * kW4Cols; i += kSimpleRows) {
-            const int b = i / kW4Cols, c = block * kW4Cols + i % kW4Cols;
-            xs[b][i % kW4Cols] = b0 + b < p.batch && c < w.cols ? w4_f32(x[(b0 + b) * p.x_stride + c]) : 0.0f;
-        }
-        __syncthreads();
-        if (tile >= w.tiles) continue;
-        const int64_t u = (int64_t)tile * w.blocks + block;
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(w.codes + u * kW4BlockBytes);
-        for (int i = 0; i < ng; ++i) {
-            const int64_t at = ((u * 8 + g) * ng + i) * 2 + up;
-            const float s = __half2float(__ushort_as_half(w.scales[at]));
-            const int zero = w.zeros ? w.zeros[at] : 8;
-            float sum[kSimpleBatch] = {};
-            for (int c = i * w.group; c < (i + 1) * w.group; ++c) {
-                const int e = c & 3, bit = (e & 1 ? 16 : 0) + (e & 2 ? 8 : 0) + 4 * up;
-                const uint32_t word = words[(c >> 6) * 128 + (4 * g + ((c >> 4) & 3)) * 4 + ((c >> 2) & 3)];
-                const float v = (float)((int)((word >> bit) & 15u) - zero);
-#pragma unroll
-                for (int b = 0; b < kSimpleBatch; ++b) sum[b] = fmaf(v, xs[b][c], sum[b]);
-            }
-#pragma unroll
-            for (int b = 0; b < kSimpleBatch; ++b) total[b] = fmaf(s, sum[b], total[b]);
-        }
-    }
-    if (row >= w.rows) return;
-    for (int b = 0; b < kSimpleBatch && b0 + b < p.batch; ++b) {
-        float v = total[b];
-        if (p.residual) v += w4_f32(((const T*)p.residual)[(b0 + b) * p.residual_stride + row]);
-        ((T*)p.y)[(b0 + b) * p.y_stride + row] = (T)v;
-    }
+template <typename T, int GROUP, bool ZEROS>
+cudaError_t few(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
+    const int tiles = (p.batch * (sizeof(T) == 4 ? 2 : 1) + 7) / 8;  // of eight columns
+    return tiles <= 1   ? few_as<T, GROUP, ZEROS, 1>(w, p, num_sms, st)
+           : tiles <= 2 ? few_as<T, GROUP, ZEROS, 2>(w, p, num_sms, st)
+                        : few_as<T, GROUP, ZEROS, 4>(w, p, num_sms, st);
+}
+
+template <typename T, int GROUP>
+cudaError_t product(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
+    return w.zeros ? few<T, GROUP, true>(w, p, num_sms, st) : few<T, GROUP, false>(w, p, num_sms, st);
 }
 
 }  // namespace
 
-cudaError_t launch_w4_product(const W4& w, const W4Product& p, int, cudaStream_t st) {
-    const dim3 grid((w.rows + kSimpleRows - 1) / kSimpleRows, (p.batch + kSimpleBatch - 1) / kSimpleBatch);
-    if (p.dtype == kRowF32) w4_simple_kernel<float><<<grid, kSimpleRows, 0, st>>>(w, p);
-    else w4_simple_kernel<__half><<<grid, kSimpleRows, 0, st>>>(w, p);
-    return cudaGetLastError();
+cudaError_t launch_w4_product(const W4& w, const W4Product& all, int num_sms, cudaStream_t st) {
+    const int elem = all.dtype == kRowF32 ? 4 : 2;
+    for (int r = 0; r < all.batch; r += few_rows(all.dtype)) {
+        W4Product p = all;
+        p.batch = all.batch - r < few_rows(all.dtype) ? all.batch - r : few_rows(all.dtype);
+        p.x = (const uint8_t*)all.x + r * all.x_stride * elem;
+        p.y = (uint8_t*)all.y + r * all.y_stride * elem;
+        if (all.residual) p.residual = (const uint8_t*)all.residual + r * all.residual_stride * elem;
+        const bool f32 = p.dtype == kRowF32;
+        const cudaError_t e = w.group == 32   ? (f32 ? product<float, 32>(w, p, num_sms, st) : product<__half, 32>(w, p, num_sms, st))
+                              : w.group == 64 ? (f32 ? product<float, 64>(w, p, num_sms, st) : product<__half, 64>(w, p, num_sms, st))
+                                              : (f32 ? product<float, 128>(w, p, num_sms, st) : product<__half, 128>(w, p, num_sms, st));
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace lc
