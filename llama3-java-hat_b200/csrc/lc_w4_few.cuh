@@ -1,6 +1,7 @@
 // lc_w4_few.cuh -- products of 4-bit weights with few rows (decode steps).
 //
-// A warp has 16 rows of W and a part of the columns; m16n8k16 products take the
+// A warp has 32 rows of W (two tiles, for which x is loaded once) and a part of
+// the columns; m16n8k16 products take the
 // codes as f16 numbers c 2^-17 straight from the words of the layout (exact, and so
 // is every product; as c 2^-24, which takes five instructions instead of seven for
 // eight codes, the tensor cores align products by the least normal exponent and
@@ -11,10 +12,11 @@
 //
 // Bound by HBM for large matrices, by latency for small ones.  Each warp streams
 // its codes, scales and zero points through a ring of its own in shared memory
-// (cp.async, no barrier), and makes the operands of its columns itself, so warps
-// meet only where the eight parts of a tile are added.  Where a CTA's columns
-// would not fit, or rows are too few to go round, a cluster shares them; its CTAs
-// meet in each other's shared memory.  Sums are added in a fixed order.
+// (cp.async, no barrier); x lies there once for the CTA.  One, two, four or eight
+// warps share a pair of tiles: fewer make fewer meetings, more make the pairs go
+// round evenly.  Where a CTA's columns would not fit, or rows are too few to go
+// round, a cluster shares them; its CTAs meet in each other's shared memory.  Sums
+// are added in a fixed order.
 #pragma once
 
 #include "lc_internal.h"
@@ -25,29 +27,38 @@ namespace lc {
 
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
-constexpr int kFewDepth = 4;  // blocks of a warp's ring
+#ifndef FD
+#define FD 3
+#endif
+constexpr int kFewDepth = FD;  // blocks of a warp's ring
 constexpr int kFewMaxCluster = 8;
 constexpr int kFewPitch = 24;  // floats between columns of 16 partial sums: no bank conflicts
+
+struct FewPlan {
+    int cluster;   // CTAs that share the columns
+    int phases;    // parts of a CTA's columns that are taken one after the other
+    int split;     // warps that share a pair of tiles
+    int blocks;    // of a CTA's part of the columns, at most
+    int clusters;
+};
 
 template <typename T, int GROUP, int NT>
 struct FewShape {
     static constexpr int kRows = sizeof(T) == 4 ? 4 * NT : 8 * NT;  // of x
     static constexpr int kGroups = kW4Cols / GROUP;
-    static constexpr int kScaleBytes = 16 * kGroups * 2, kZeroBytes = 16 * kGroups;
-    static constexpr int kSlot = kW4BlockBytes + 128 + 64;
-    static constexpr int kTiles = kRows >= 16 ? 1 : 16 / kRows;  // tiles between two meetings
-    static constexpr int kElems = kTiles * kRows * 16;
-    static constexpr int kPartBytes = 2 * kFewWarps * kTiles * kRows * kFewPitch * 4;
-    static constexpr int kRecvBytes = 2 * (kElems + 16 * kFewMaxCluster) * 4;
-    static int x_pitch(int blocks) { return 256 * blocks + 64; }
-    static size_t smem(int blocks) {  // blocks: of a warp's part
-        return (size_t)kFewWarps * (kFewDepth * kSlot + 8 * NT * x_pitch(blocks) + (blocks * kGroups + 1) * kRows * 4) + kPartBytes + kRecvBytes;
+    static constexpr int kScaleBytes = 16 * kGroups * 2, kZeroBytes = 16 * kGroups;  // of a tile's block
+    static constexpr int kScaleAt = 2 * kW4BlockBytes, kZeroAt = kScaleAt + 2 * kScaleBytes;
+    static constexpr int kSlot = kZeroAt + 2 * kZeroBytes;  // a block of two tiles
+    static constexpr int kPartFloats = kFewWarps * 2 * kRows * kFewPitch;  // the warps' sums of one meeting
+    // Elements of one CTA at a meeting of a cluster, in runs of 16.
+    __host__ __device__ static int each(int cluster, int split) { return (kFewWarps / split * 2 * kRows + cluster - 1) / cluster * 16; }
+    // rows: of x.  One column of zeros stands for all that are not there.
+    static size_t smem(const FewPlan& plan, int rows) {
+        const int columns = (sizeof(T) == 4 ? 2 : 1) * rows + 1;
+        return (size_t)kFewWarps * kFewDepth * kSlot + columns * (256 * plan.blocks + 64) +
+               (plan.blocks * kGroups + 1 + kFewWarps) * kRows * 4 + kPartFloats * 4 +
+               (plan.cluster > 1 ? 2 * plan.cluster * each(plan.cluster, plan.split) * 4 : 0);
     }
-};
-
-struct FewPlan {
-    int cluster, phases, blocks;  // CTAs that share the columns; parts of a warp one after the other; blocks of a part at most
-    int clusters;
 };
 
 // The eight codes of a word as f16 pairs c 2^-17: rows g, g + 8 of columns e = 0, 1,
@@ -76,23 +87,23 @@ LC_DEV uint4 few_lds128(uint32_t a) {
 template <typename T, int GROUP, bool ZEROS, int NT>
 __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product p, FewPlan plan) {
     using S = FewShape<T, GROUP, NT>;
-    constexpr int NG = S::kGroups, ROWS = S::kRows, TB = S::kTiles;
+    constexpr int NG = S::kGroups, ROWS = S::kRows;
     constexpr bool SPLIT = sizeof(T) == 4;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int pitch = 256 * plan.blocks + 64;
-    // Of this warp: ring, x as f16 columns [8 NT][pitch], sums of x [groups][ROWS], factors [ROWS].
+    const int pitch = 256 * plan.blocks + 64, columns = (SPLIT ? 2 : 1) * p.batch;
+    // Rings, x as f16 columns [columns + 1][pitch], sums of x [groups][ROWS], factors
+    // [ROWS], largest sizes [warps][ROWS], parts and what a cluster's CTAs send.
     uint8_t* at = smem;
     const uint32_t ring = smem_u32(at) + warp * kFewDepth * S::kSlot;
     at += kFewWarps * kFewDepth * S::kSlot;
-    uint8_t* const xcol = at + warp * 8 * NT * pitch;
-    at += kFewWarps * 8 * NT * pitch;
-    float* const xsum = reinterpret_cast<float*>(at) + warp * (plan.blocks * NG + 1) * ROWS;
+    uint8_t* const xcol = at;
+    at += (columns + 1) * pitch;
+    float* const xsum = reinterpret_cast<float*>(at);
     float* const factor = xsum + plan.blocks * NG * ROWS;
-    at += kFewWarps * (plan.blocks * NG + 1) * ROWS * 4;
-    float* const parts = reinterpret_cast<float*>(at);  // [2][warps][TB][ROWS][kFewPitch]
-    at += S::kPartBytes;
-    float* const recv = reinterpret_cast<float*>(at);   // [2][cluster][elements of one CTA]
+    float* const tops = factor + ROWS;
+    float* const parts = tops + kFewWarps * ROWS;    // [warps][tile][ROWS][kFewPitch]
+    float* const recv = parts + S::kPartFloats;      // [2][cluster][elements of one CTA]
 
     uint32_t rank = 0;
     const int cs = plan.cluster, id = blockIdx.x / cs;
@@ -100,54 +111,61 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
         asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
-    const int tile0 = (int)((int64_t)w.tiles * id / plan.clusters), tile1 = (int)((int64_t)w.tiles * (id + 1) / plan.clusters);
-    const int shares = cs * plan.phases * kFewWarps;
-    auto part0 = [&](int phase) { return (int)((int64_t)w.blocks * (((int)rank * plan.phases + phase) * kFewWarps + warp) / shares); };
-    auto part1 = [&](int phase) { return (int)((int64_t)w.blocks * (((int)rank * plan.phases + phase) * kFewWarps + warp + 1) / shares); };
+    const int pairs = (w.tiles + 1) / 2, PB = kFewWarps / plan.split;  // PB: pairs between two meetings
+    const int pair0 = (int)((int64_t)pairs * id / plan.clusters), pair1 = (int)((int64_t)pairs * (id + 1) / plan.clusters);
+    const int shares = cs * plan.phases, mine_i = warp / plan.split, mine_k = warp % plan.split;
+    auto cta0 = [&](int phase) { return (int)((int64_t)w.blocks * ((int)rank * plan.phases + phase) / shares); };
+    auto part = [&](int phase, int k) {  // where the k-th warp of a pair begins
+        const int c0 = cta0(phase), c1 = cta0(phase + 1);
+        return c0 + (c1 - c0) * k / plan.split;
+    };
 
-    // What the warp reads, in order: batches of TB tiles, phases, tiles, blocks.
-    struct Cursor {
-        int batch, phase, i, block, end, n;  // n: tiles of the batch
-    };
-    auto open = [&](Cursor& c) {  // the first block at or behind (batch, phase, i = 0); false: none
-        for (; c.batch < tile1; c.batch += TB, c.phase = 0) {
-            for (; c.phase < plan.phases; ++c.phase) {
-                c.block = part0(c.phase), c.end = part1(c.phase);
-                c.n = min(TB, tile1 - c.batch);
-                c.i = 0;
-                if (c.block < c.end) return true;
+    // What the warp reads, in order: meetings, phases, blocks.
+    // Each lane copies 16 bytes of each half of both tiles' codes, and some 16 bytes
+    // of their scales or zero points.
+    constexpr int kMetaScales = 2 * S::kScaleBytes / 16, kMeta = kMetaScales + (ZEROS ? 2 * S::kZeroBytes / 16 : 0);
+    const bool meta_zero = lane >= kMetaScales;
+    const int meta_bytes = meta_zero ? S::kZeroBytes : S::kScaleBytes, meta_at = 16 * (meta_zero ? lane - kMetaScales : lane);
+    const uint8_t* const meta_base = meta_zero ? w.zeros : (const uint8_t*)w.scales;
+    int a_pair = pair0 + mine_i, a_phase = -1, a_left = 0;
+    bool more = true;
+    const uint8_t *a_code = nullptr, *a_meta = nullptr;
+    int64_t a_second = 0;  // from the first tile's codes to the second's
+    auto advance = [&] {   // to the next part that has blocks
+        do {
+            if (++a_phase == plan.phases) a_phase = 0, a_pair += PB;
+            if (a_pair >= pair1) {
+                more = false;
+                return;
             }
-        }
-        return false;
+            a_left = part(a_phase, mine_k + 1) - part(a_phase, mine_k);
+        } while (!a_left);
+        const int tile = 2 * a_pair;
+        const bool two = tile + 1 < w.tiles;  // else the first stands for it
+        const int64_t u = (int64_t)tile * w.blocks + part(a_phase, mine_k);
+        a_code = w.codes + u * kW4BlockBytes + lane * 16;
+        a_second = two ? (int64_t)w.blocks * kW4BlockBytes : 0;
+        a_meta = meta_base + (u + (two && meta_at >= meta_bytes ? w.blocks : 0)) * meta_bytes + meta_at % meta_bytes;
     };
-    Cursor ahead = {tile0, 0, 0, 0, 0, 0};
-    bool more = open(ahead);
-    auto request = [&](int slot) {
+    auto request = [&](uint32_t to) {
         if (more) {
-            const int64_t u = (int64_t)(ahead.batch + ahead.i) * w.blocks + ahead.block;
-            const uint32_t to = ring + slot * S::kSlot;
-            const uint8_t* from = w.codes + u * kW4BlockBytes + lane * 16;
-            few_copy16(to + lane * 16, from);
-            few_copy16(to + 512 + lane * 16, from + 512);
-            if (lane < S::kScaleBytes / 16) few_copy16(to + 1024 + lane * 16, (const uint8_t*)w.scales + u * S::kScaleBytes + lane * 16);
-            if (ZEROS && lane >= 16 && lane < 16 + S::kZeroBytes / 16)
-                few_copy16(to + 1152 + (lane - 16) * 16, w.zeros + u * S::kZeroBytes + (lane - 16) * 16);
-            if (++ahead.block == ahead.end) {
-                if (++ahead.i < ahead.n) {
-                    ahead.block = part0(ahead.phase);
-                } else {
-                    ++ahead.phase;
-                    more = open(ahead);
-                }
-            }
+            few_copy16(to + lane * 16, a_code);
+            few_copy16(to + 512 + lane * 16, a_code + 512);
+            few_copy16(to + 1024 + lane * 16, a_code + a_second);
+            few_copy16(to + 1536 + lane * 16, a_code + a_second + 512);
+            if (lane < kMeta) few_copy16(to + S::kScaleAt + lane * 16, a_meta);
+            a_code += kW4BlockBytes;
+            a_meta += meta_bytes;
+            if (--a_left == 0) advance();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
     griddep_wait();
     griddep_launch();
+    advance();
 #pragma unroll
-    for (int i = 0; i < kFewDepth - 1; ++i) request(i);
+    for (int i = 0; i < kFewDepth - 1; ++i) request(ring + i * S::kSlot);
 
     // x of the columns [128 b0, 128 b1) as operands.  F32: columns 2 r and 2 r + 1
     // are hi and lo of row r.
@@ -162,56 +180,53 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
                 v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
             } else {
                 const uint2 h = *reinterpret_cast<const uint2*>(from);
-                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), b2 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-                v[0] = a.x, v[1] = a.y, v[2] = b2.x, v[3] = b2.y;
+                const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
+                v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = c + i < w.cols ? (float)from[i] : 0.0f;
         }
     };
-    auto stage = [&](int b0, int b1) {
+    auto stage = [&](int b0, int b1) {  // by all warps
         constexpr float kSum = ZEROS ? -0x1p-17f : -0x1p-14f;  // without zero points all are 8
-        __syncwarp();
-        for (int r = 0; r < ROWS; ++r) {
-            if (r >= p.batch) {
-                for (int b = 0; b < b1 - b0; ++b) {
-                    const uint2 none = make_uint2(0, 0);
-                    *reinterpret_cast<uint2*>(xcol + (SPLIT ? 2 * r : r) * pitch + b * 256 + lane * 8) = none;
-                    if (SPLIT) *reinterpret_cast<uint2*>(xcol + (2 * r + 1) * pitch + b * 256 + lane * 8) = none;
-                    for (int i = lane; i < NG; i += 32) xsum[(b * NG + i) * ROWS + r] = 0.0f;
+        for (int i = tid; i < (b1 - b0) * NG * ROWS; i += kFewThreads)
+            if (i % ROWS >= p.batch) xsum[i] = 0.0f;
+        for (int i = tid * 8; i < pitch; i += kFewThreads * 8) *reinterpret_cast<uint2*>(xcol + columns * pitch + i) = make_uint2(0, 0);
+        constexpr int HOLD = 2;  // blocks of a row that are read once
+        const int n = b1 - b0;
+        // Items (row, block): a warp takes the blocks warp, warp + 8, ... of every row.
+        if (SPLIT) {
+            for (int r = 0; r < p.batch; ++r) {
+                float top = 0.0f;
+                for (int b = warp; b < n; b += HOLD * kFewWarps) {
+                    float u[HOLD][4] = {};
+#pragma unroll
+                    for (int h = 0; h < HOLD; ++h)
+                        if (b + h * kFewWarps < n) four(r, b0 + b + h * kFewWarps, u[h]);
+#pragma unroll
+                    for (int h = 0; h < HOLD; ++h) top = fmaxf(fmaxf(top, fmaxf(fabsf(u[h][0]), fabsf(u[h][1]))), fmaxf(fabsf(u[h][2]), fabsf(u[h][3])));
                 }
-                if (lane == 0) factor[r] = 0.0f;
-                continue;
+                top = warp_max(top);
+                if (lane == 0) tops[warp * ROWS + r] = top;
             }
-            constexpr int HOLD = 4;  // blocks that are read once
-            float v[HOLD][4], up = 1.0f;
+            __syncthreads();
+        }
+        if (tid < ROWS) {
+            float f = 1.0f;
             if (SPLIT) {
                 float top = 0.0f;
-                for (int b = b1 - 1; b >= b0; --b) {
-                    float u[4];
-                    if (b - b0 >= HOLD) {
-                        four(r, b, u);
-                        top = fmaxf(fmaxf(top, fmaxf(fabsf(u[0]), fabsf(u[1]))), fmaxf(fabsf(u[2]), fabsf(u[3])));
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < HOLD; ++b) {
-                    if (b0 + b < b1) {
-                        four(r, b0 + b, v[b]);
-                        top = fmaxf(fmaxf(top, fmaxf(fabsf(v[b][0]), fabsf(v[b][1]))), fmaxf(fabsf(v[b][2]), fabsf(v[b][3])));
-                    }
-                }
-                const int e = split_row_exp(warp_max(top));
-                up = pow2f(e);
-                if (lane == 0) factor[r] = pow2f(-e);
-            } else {
-#pragma unroll
-                for (int b = 0; b < HOLD; ++b)
-                    if (b0 + b < b1) four(r, b0 + b, v[b]);
-                if (lane == 0) factor[r] = 1.0f;
+                for (int k = 0; k < kFewWarps && tid < p.batch; ++k) top = fmaxf(top, tops[k * ROWS + tid]);
+                f = pow2f(-split_row_exp(top));
             }
-            auto put = [&](int b, float (&f)[4]) {
+            factor[tid] = f;
+        }
+        if (SPLIT) __syncthreads();
+        for (int r = 0; r < p.batch; ++r) {
+            const float up = SPLIT ? 1.0f / factor[r] : 1.0f;  // a power of two
+            for (int b = warp; b < n; b += kFewWarps) {
+                float f[4];
+                four(r, b0 + b, f);
                 uint32_t h[2], l[2];
                 float sum = 0.0f;
 #pragma unroll
@@ -234,98 +249,108 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
 #pragma unroll
                 for (int o = 1; o < GROUP / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 if (lane % (GROUP / 4) == 0) xsum[(b * NG + lane / (GROUP / 4)) * ROWS + r] = sum * kSum;
-            };
-#pragma unroll
-            for (int b = 0; b < HOLD; ++b)
-                if (b0 + b < b1) put(b, v[b]);
-            for (int b = HOLD; b < b1 - b0; ++b) {
-                float u[4];
-                four(r, b0 + b, u);
-                put(b, u);
             }
         }
-        __syncwarp();
+        __syncthreads();
     };
 
+    // Where the lane reads its columns of x.
+    uint32_t xat[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) xat[nt] = smem_u32(xcol) + min(8 * nt + g, columns) * pitch + t * 16;
     int slot = 0, buf = 0;
     bool staged = false;
-    for (int batch = tile0; batch < tile1; batch += TB, buf ^= 1) {
-        const int n = min(TB, tile1 - batch);
-        float* const mine = parts + ((buf * kFewWarps + warp) * TB) * ROWS * kFewPitch;
+    for (int first = pair0; first < pair1; first += PB, buf ^= 1) {
+        const int n = min(PB, pair1 - first);
+        constexpr int V = SPLIT ? 2 : 4;  // sums of a lane: rows g and g + 8, one or two rows of x
+        float* const mine = parts + warp * (2 * ROWS * kFewPitch);
         for (int phase = 0; phase < plan.phases; ++phase) {
-            const int b0 = part0(phase), b1 = part1(phase);
-            if (!staged || plan.phases > 1) stage(b0, b1);
+            const int c0 = cta0(phase);
+            if (phase) __syncthreads();  // all have used the columns of the phase before
+            if (!staged || plan.phases > 1) stage(c0, cta0(phase + 1));
             staged = true;
-            for (int i = 0; i < n; ++i) {
-                constexpr int V = SPLIT ? 2 : 4;  // sums of a lane: rows g and g + 8, one or two rows of x
-                float total[NT][V] = {};
-                for (int b = b0; b < b1; ++b) {
-                    request(slot == 0 ? kFewDepth - 1 : slot - 1);
+            if (mine_i < n) {
+                const int b1 = part(phase, mine_k + 1) - c0;
+                float total[2][NT][V] = {};
+                for (int b = part(phase, mine_k) - c0; b < b1; ++b) {
+                    const uint32_t from = ring + slot * S::kSlot;
+                    request(ring + (slot == 0 ? kFewDepth - 1 : slot - 1) * S::kSlot);
                     asm volatile("cp.async.wait_group %0;" ::"n"(kFewDepth - 1) : "memory");
                     __syncwarp();
-                    const uint32_t from = ring + slot * S::kSlot;
-                    const uint32_t xat = smem_u32(xcol) + g * pitch + (b - b0) * 256 + t * 16;
-                    const float* const xs = xsum + (b - b0) * NG * ROWS;
-                    uint4 code[2] = {few_lds128(from + lane * 16), few_lds128(from + 512 + lane * 16)};
-                    uint32_t sc[NG], zp[(NG + 1) / 2];
+                    const float* const xs = xsum + b * NG * ROWS;
+                    uint4 code[2][2];
+                    uint32_t sc[2][NG], zp[2][(NG + 1) / 2];
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[k]) : "r"(from + 1024 + (g * NG + k) * 4));
-                    if (ZEROS) {
+                    for (int m = 0; m < 2; ++m) {
+                        code[m][0] = few_lds128(from + m * 1024 + lane * 16);
+                        code[m][1] = few_lds128(from + m * 1024 + 512 + lane * 16);
 #pragma unroll
-                        for (int k = 0; k < (NG + 1) / 2; ++k) {
-                            if (NG == 1) {
-                                uint16_t z;
-                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(z) : "r"(from + 1152 + g * 2));
-                                zp[k] = z;
-                            } else {
-                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(zp[k]) : "r"(from + 1152 + (g * NG + 2 * k) * 2));
-                            }
-                        }
-                    }
-                    float acc[NT][4];
+                        for (int k = 0; k < NG; ++k)
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[m][k]) : "r"(from + S::kScaleAt + m * S::kScaleBytes + (g * NG + k) * 4));
+                        if (ZEROS) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {  // runs of 32 columns
-                        if (q % (4 / NG) == 0) {
-                            const int k = q / (4 / NG);
-                            float z0 = 1.0f, z1 = 1.0f;
-                            if (ZEROS) {
-                                const uint32_t z = zp[k >> 1] >> (16 * (k & 1));
-                                z0 = (float)(z & 255u), z1 = (float)((z >> 8) & 255u);
-                            }
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                if (SPLIT) {
-                                    const float a = xs[k * ROWS + nt * 4 + t];
-                                    acc[nt][0] = z0 * a, acc[nt][1] = 0.0f, acc[nt][2] = z1 * a, acc[nt][3] = 0.0f;
+                            for (int k = 0; k < (NG + 1) / 2; ++k) {
+                                const uint32_t za = from + S::kZeroAt + m * S::kZeroBytes + (g * NG + 2 * k) * 2;
+                                if (NG == 1) {
+                                    uint16_t z;
+                                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(z) : "r"(za));
+                                    zp[m][k] = z;
                                 } else {
-                                    const float2 a = *reinterpret_cast<const float2*>(xs + k * ROWS + nt * 8 + 2 * t);
-                                    acc[nt][0] = z0 * a.x, acc[nt][1] = z0 * a.y, acc[nt][2] = z1 * a.x, acc[nt][3] = z1 * a.y;
+                                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(zp[m][k]) : "r"(za));
                                 }
                             }
                         }
-                        const uint4& c = code[q >> 1];
-                        const uint32_t w0 = q & 1 ? c.z : c.x, w1 = q & 1 ? c.w : c.y;
-                        uint32_t a0[4], a1[4];
-                        few_codes(w0, a0);
-                        few_codes(w1, a1);
+                    }
+                    float acc[2][NT][4];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const uint4 xb = few_lds128(xat + nt * 8 * pitch + q * 64);
-                            few_mma(acc[nt], a0, xb.x, xb.y);
-                            few_mma(acc[nt], a1, xb.z, xb.w);
-                        }
-                        if (q % (4 / NG) == 4 / NG - 1) {
-                            const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sc[q / (4 / NG)]));
+                    for (int q = 0; q < 4; ++q) {  // runs of 32 columns
+                        const int k = q / (4 / NG);
+                        if (q % (4 / NG) == 0) {
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                if (SPLIT) {
-                                    total[nt][0] = fmaf(s.x, acc[nt][0] + acc[nt][1], total[nt][0]);
-                                    total[nt][1] = fmaf(s.y, acc[nt][2] + acc[nt][3], total[nt][1]);
-                                } else {
-                                    total[nt][0] = fmaf(s.x, acc[nt][0], total[nt][0]);
-                                    total[nt][1] = fmaf(s.x, acc[nt][1], total[nt][1]);
-                                    total[nt][V - 2] = fmaf(s.y, acc[nt][2], total[nt][V - 2]);
-                                    total[nt][V - 1] = fmaf(s.y, acc[nt][3], total[nt][V - 1]);
+                                const float2 a = SPLIT ? make_float2(xs[k * ROWS + nt * 4 + t], 0.0f)
+                                                       : *reinterpret_cast<const float2*>(xs + k * ROWS + nt * 8 + 2 * t);
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) {
+                                    float z0 = 1.0f, z1 = 1.0f;
+                                    if (ZEROS) {
+                                        const uint32_t z = zp[m][k >> 1] >> (16 * (k & 1));
+                                        z0 = (float)(z & 255u), z1 = (float)((z >> 8) & 255u);
+                                    }
+                                    acc[m][nt][0] = z0 * a.x, acc[m][nt][1] = SPLIT ? 0.0f : z0 * a.y;
+                                    acc[m][nt][2] = z1 * a.x, acc[m][nt][3] = SPLIT ? 0.0f : z1 * a.y;
+                                }
+                            }
+                        }
+                        uint4 xb[NT];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) xb[nt] = few_lds128(xat[nt] + b * 256 + q * 64);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            const uint4& c = code[m][q >> 1];
+                            uint32_t a0[4], a1[4];
+                            few_codes(q & 1 ? c.z : c.x, a0);
+                            few_codes(q & 1 ? c.w : c.y, a1);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                few_mma(acc[m][nt], a0, xb[nt].x, xb[nt].y);
+                                few_mma(acc[m][nt], a1, xb[nt].z, xb[nt].w);
+                            }
+                        }
+                        if (q % (4 / NG) == 4 / NG - 1) {
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sc[m][k]));
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    float(&a)[4] = acc[m][nt];
+                                    float(&v)[V] = total[m][nt];
+                                    if (SPLIT) {
+                                        v[0] = fmaf(s.x, a[0] + a[1], v[0]), v[1] = fmaf(s.y, a[2] + a[3], v[1]);
+                                    } else {
+                                        v[0] = fmaf(s.x, a[0], v[0]), v[1] = fmaf(s.x, a[1], v[1]);
+                                        v[V - 2] = fmaf(s.y, a[2], v[V - 2]), v[V - 1] = fmaf(s.y, a[3], v[V - 1]);
+                                    }
                                 }
                             }
                         }
@@ -334,64 +359,64 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
                     slot = slot == kFewDepth - 1 ? 0 : slot + 1;
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    auto give = [&](int r, float lo, float hi) {  // rows g and g + 8 for row r of x
-                        float* const to = mine + (i * ROWS + r) * kFewPitch + g;
-                        const float f = factor[r];
-                        lo = lo * 0x1p17f * f, hi = hi * 0x1p17f * f;
-                        to[0] = phase ? to[0] + lo : lo;
-                        to[8] = phase ? to[8] + hi : hi;
-                    };
-                    if (SPLIT) {
-                        give(nt * 4 + t, total[nt][0], total[nt][1]);
-                    } else {
-                        give(nt * 8 + 2 * t, total[nt][0], total[nt][V - 2]);
-                        give(nt * 8 + 2 * t + 1, total[nt][1], total[nt][V - 1]);
+                for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        auto give = [&](int r, float lo, float hi) {  // rows g and g + 8 for row r of x
+                            float* const to = mine + (m * ROWS + r) * kFewPitch + g;
+                            const float f = factor[r];
+                            lo = lo * 0x1p17f * f, hi = hi * 0x1p17f * f;
+                            to[0] = phase ? to[0] + lo : lo;
+                            to[8] = phase ? to[8] + hi : hi;
+                        };
+                        if (SPLIT) {
+                            give(nt * 4 + t, total[m][nt][0], total[m][nt][1]);
+                        } else {
+                            give(nt * 8 + 2 * t, total[m][nt][0], total[m][nt][V - 2]);
+                            give(nt * 8 + 2 * t + 1, total[m][nt][1], total[m][nt][V - 1]);
+                        }
                     }
                 }
             }
         }
         __syncthreads();
-        if (cs > 1 && batch == tile0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all have begun
+        if (cs > 1 && first == pair0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all have begun
         // The warps' parts in order; a cluster's parts at the CTA that has the element.
-        auto element = [&](int e, int& i, int& r, int& row) { row = e & 15, r = (e >> 4) % ROWS, i = (e >> 4) / ROWS; };
+        // Element e: row e % 16 of tile e / 16 / ROWS for row (e / 16) % ROWS of x.
         auto finish = [&](int e, float v) {
-            int i, r, row;
-            element(e, i, r, row);
-            const int64_t out = (int64_t)(batch + i) * kW4Rows + row;
-            if (i >= n || r >= p.batch || out >= w.rows) return;
+            const int r = (e >> 4) % ROWS;
+            const int64_t out = ((int64_t)first * 2 + (e >> 4) / ROWS) * kW4Rows + (e & 15);
+            if (r >= p.batch || out >= w.rows) return;
             if (p.residual) v += (float)((const T*)p.residual)[r * p.residual_stride + out];
             ((T*)p.y)[r * p.y_stride + out] = (T)v;
         };
-        for (int e = tid; e < S::kElems; e += kFewThreads) {
-            int i, r, row;
-            element(e, i, r, row);
-            if (i >= n) continue;
-            const float* from = parts + (buf * kFewWarps * TB + i) * ROWS * kFewPitch + r * kFewPitch + row;
-            float v = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kFewWarps; ++k) v += from[k * TB * ROWS * kFewPitch];
+        const int each = S::each(cs, plan.split);
+        for (int e = tid; e < n * 32 * ROWS; e += kFewThreads) {
+            constexpr int kPair = 2 * ROWS;  // runs of 16 of a pair
+            const float* from = parts + ((e >> 4) / kPair * plan.split * kPair + (e >> 4) % kPair) * kFewPitch + (e & 15);
+            float v = from[0];
+            for (int k = 1; k < plan.split; ++k) v += from[k * kPair * kFewPitch];
             if (cs == 1) {
                 finish(e, v);
             } else {
-                // 16 neighbouring elements have one owner.
-                const int owner = (e >> 4) % cs, place = ((e >> 4) / cs) * 16 + (e & 15);
-                const int each = ((S::kElems / 16 + cs - 1) / cs) * 16;
                 uint32_t to;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(recv + (buf * cs + (int)rank) * each + place)), "r"(owner));
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                             : "=r"(to)
+                             : "r"(smem_u32(recv + (buf * cs + (int)rank) * each + ((e >> 4) / cs) * 16 + (e & 15))), "r"((e >> 4) % cs));
                 asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
             }
         }
         if (cs > 1) {
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-            const int each = ((S::kElems / 16 + cs - 1) / cs) * 16;
             for (int place = tid; place < each; place += kFewThreads) {
                 const int e = ((place >> 4) * cs + (int)rank) * 16 + (place & 15);
-                if (e >= S::kElems || (e >> 4) / ROWS >= n) continue;
+                if (e >= n * 32 * ROWS) continue;
                 float v = 0.0f;
                 for (int k = 0; k < cs; ++k) v += recv[(buf * cs + k) * each + place];
                 finish(e, v);
             }
+        } else {
+            __syncthreads();  // the parts have been read
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");

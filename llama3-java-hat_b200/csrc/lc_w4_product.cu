@@ -6,35 +6,51 @@
 #include "lc_w4.h"
 #include "lc_w4_few.cuh"
 
+#ifndef FEW_MEET
+#define FEW_MEET 2
+#endif
 namespace lc {
 namespace {
 
 // Rows of x that one launch of the kernel for few rows takes.
-constexpr int few_rows(int dtype) { return dtype == kRowF32 ? 16 : 32; }
+constexpr int few_rows(int dtype) { return dtype == kRowF32 ? 8 : 16; }
 
 template <typename T, int GROUP, bool ZEROS, int NT>
 cudaError_t few_as(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
     using S = FewShape<T, GROUP, NT>;
     constexpr size_t kTwo = 113 * 1024, kOne = 226 * 1024;  // shared memory with which two CTAs, or one, fit an SM
+    const int pairs = (w.tiles + 1) / 2;
     FewPlan plan;
-    plan.cluster = plan.phases = 1;
-    auto blocks = [&] { return (w.blocks + plan.cluster * plan.phases * kFewWarps - 1) / (plan.cluster * plan.phases * kFewWarps); };
+    auto set = [&](int cluster, int phases) {
+        plan.cluster = cluster;
+        plan.phases = phases;
+        plan.blocks = (w.blocks + cluster * phases - 1) / (cluster * phases);
+        const int most = 2 * num_sms / cluster;
+        plan.clusters = pairs < most ? pairs : most;
+        // Warps of a pair: few make few meetings, more make a CTA's pairs go round
+        // evenly.  A meeting costs about as much as kMeet blocks.
+        constexpr int kMeet = FEW_MEET;
+        const int mine = (pairs + plan.clusters - 1) / plan.clusters;
+        int best = 0;
+        for (int split = 1; split <= kFewWarps; split *= 2) {
+            const int cost = (mine * split + kFewWarps - 1) / kFewWarps * ((plan.blocks + split - 1) / split + kMeet);
+            if (!best || cost < best) best = cost, plan.split = split;
+        }
+    };
     // More CTAs for the columns while a CTA's part would keep a second CTA off the
     // SM, or while there are SMs without one and each warp has two blocks to share.
+    set(1, 1);
     while (plan.cluster < kFewMaxCluster && w.blocks >= 2 * plan.cluster * kFewWarps &&
-           (S::smem(blocks()) > kTwo || w.tiles * plan.cluster < num_sms))
-        plan.cluster *= 2;
-    while (S::smem(blocks()) > kOne) ++plan.phases;
-    plan.blocks = blocks();
-    const int most = 2 * num_sms / plan.cluster;
-    plan.clusters = w.tiles < most ? w.tiles : most;
+           (S::smem(plan, p.batch) > kTwo || pairs * plan.cluster < num_sms))
+        set(2 * plan.cluster, 1);
+    while (S::smem(plan, p.batch) > kOne) set(plan.cluster, plan.phases + 1);
     auto* kernel = w4_few_kernel<T, GROUP, ZEROS, NT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOne);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.clusters * plan.cluster));
     cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = S::smem(plan.blocks);
+    cfg.dynamicSmemBytes = S::smem(plan, p.batch);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -51,8 +67,7 @@ template <typename T, int GROUP, bool ZEROS>
 cudaError_t few(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
     const int tiles = (p.batch * (sizeof(T) == 4 ? 2 : 1) + 7) / 8;  // of eight columns
     return tiles <= 1   ? few_as<T, GROUP, ZEROS, 1>(w, p, num_sms, st)
-           : tiles <= 2 ? few_as<T, GROUP, ZEROS, 2>(w, p, num_sms, st)
-                        : few_as<T, GROUP, ZEROS, 4>(w, p, num_sms, st);
+                        : few_as<T, GROUP, ZEROS, 2>(w, p, num_sms, st);
 }
 
 template <typename T, int GROUP>
