@@ -88,6 +88,7 @@ struct lc_context {
     bool gemm_ready = false;        // shared-memory attribute of the GEMM kernel set
     std::mutex paged;               // held by a call of the paged operators: threads take turns
     std::atomic<void*> kv8_ws{nullptr};  // workspace of lc_kv8_attention, one size for all calls
+    void* w4_ws = nullptr;          // workspace of lc_w4_product, one size for all calls
     lc_rope_config rope_cfg;        // the last lc_rope_apply's configuration and its frequencies
     RopeTurns rope_turns;
     float rope_mult = 0.0f;         // 0: none yet
@@ -130,6 +131,7 @@ extern "C" int lc_context_destroy(lc_context* c) {
     if (c->attn_scratch) cudaFree(c->attn_scratch);
     if (c->gemm_scratch) cudaFree(c->gemm_scratch);
     if (void* ws = c->kv8_ws) cudaFree(ws);
+    if (c->w4_ws) cudaFree(c->w4_ws);
     if (c->d_err) cudaFree(c->d_err);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
@@ -1005,6 +1007,7 @@ int w4_values(lc_context* c, const lc_w4* w, void* values, int64_t stride, int32
         // What lies between the rows of a host buffer that is read into stays as it is: it travels both ways.
         void* d = s.arg(values, rows_bytes(view.rows, stride, view.cols, elem), quantize ? kIn : stride == view.cols ? kOut : kInOut);
         if (s.status != LC_OK) return s.status;
+        if ((uintptr_t)d % elem) return fail(LC_ERR_INVALID_ARG, "values are not aligned to their type");
         return s.finish(quantize ? launch_w4_quantize(view, d, stride, dtype, c->sms, c->stream)
                                  : launch_w4_read(view, d, stride, dtype, c->sms, c->stream));
     });
@@ -1069,7 +1072,19 @@ extern "C" int lc_w4_product(lc_context* c, const lc_w4* w, const void* x, int64
         p.residual_stride = residual_stride;
         p.batch = batch;
         p.dtype = dtype;
-        return s.finish(launch_w4_product(view, p, c->sms, c->stream));
+        if ((uintptr_t)p.x % elem || (uintptr_t)p.y % elem || (uintptr_t)p.residual % elem)
+            return fail(LC_ERR_INVALID_ARG, "rows are not aligned to their type");
+        const bool uses_ws = w4_product_uses_ws(view, p);
+        if (uses_ws && !c->w4_ws) {
+            cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+            CK(cudaStreamIsCapturing(c->stream, &capture), "cudaStreamIsCapturing");
+            if (capture != cudaStreamCaptureStatusNone)
+                return fail(LC_ERR_STATE, "the first lc_w4_product of many rows of a context allocates its workspace: make it before the capture");
+            void* ws = nullptr;
+            CK(cudaMalloc(&ws, w4_product_ws_bytes()), "product workspace");
+            c->w4_ws = ws;
+        }
+        return s.finish(launch_w4_product(view, p, c->sms, uses_ws ? c->w4_ws : nullptr, c->d_err, c->stream));
     });
 }
 

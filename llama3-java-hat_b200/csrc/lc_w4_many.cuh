@@ -1,0 +1,482 @@
+// lc_w4_many.cuh -- products of 4-bit weights with many rows (batches, prompts),
+// on the tcgen05 tensor cores.
+//
+// Two kernels.  The first lays the rows of x out as f16 operands in the context's
+// workspace: F16 rows as they are, F32 rows as hi + lo under a power-of-two row
+// scale (2^-22), rows and columns that are not there as zeros.  The second has
+// units of 256 rows of W and up to 128 columns (rows of x; hi and lo count each),
+//   D = A B   M 128 (twice), N up to 128, K one group
+// with A = (c - z) / 4, exact in f16, made from the codes in shared memory.  A
+// group's D is added, under the group's scale, to fp32 sums that an epilogue thread
+// keeps in registers for its row of W, while the tensor cores fill the other D: so
+// scales need no rounding into weights, and the tensor cores' own truncating sums
+// run over 128 columns at most.
+//
+// What bounds it: the products, as long as a group has more columns than the
+// epilogue takes instructions for (one packed FMA for two elements of D).
+//
+// Warps 0-7: epilogue, four for each 128 rows.  Warps 8-11: codes to operands,
+// through rings of their own (cp.async).  Warp 12 issues the products, warp 13 the
+// copies of x (bulk copies, whole stages).  Registers move to the epilogue.  With
+// few units a cluster shares the columns; its CTAs add their sums through each
+// other's shared memory.
+#pragma once
+
+#include "lc_internal.h"
+#include "lc_tcgen05.cuh"
+#include "lc_w4.h"
+#include "lc_w4_few.cuh"
+
+namespace lc {
+
+constexpr int kManyThreads = 16 * 32;
+constexpr int kManyRows = 256;      // of W, of a unit
+constexpr int kManyCols = 128;      // of B, at most
+constexpr int kManyK = 64;          // columns of W of a stage
+constexpr int kManyAStages = 3, kManyBStages = 4, kManyRing = 6;
+constexpr int kManyABytes = kManyRows * kManyK * 2, kManyBBytes = kManyCols * kManyK * 2;
+constexpr int kManyRingBytes = 4 * 512;  // of a warp: a chunk of four tiles
+constexpr int kManySmem = kManyAStages * kManyABytes + kManyBStages * kManyBBytes + 4 * kManyRing * kManyRingBytes;
+constexpr int kManyMaxCluster = 8;
+// Registers after the split; their sum over the warpgroups is the launch's.
+constexpr int kManyRegsSum = 184, kManyRegsCodes = 80, kManyRegsRest = 64;
+constexpr int kManyRegsLaunch = (2 * kManyRegsSum + kManyRegsCodes + kManyRegsRest + 3) / 4;
+
+struct ManyPlan {
+    int n;         // columns of B of a unit (a multiple of 16)
+    int rows;      // rows of x of a unit
+    int x_tiles, w_tiles;
+    int cluster;   // CTAs that share the columns of W
+    const uint8_t* b;      // [x tile][chunk of 64 columns][n / 8][8 octets][8][16 bytes]
+    const float* factor;   // [batch] what the rows of x were divided by
+};
+
+// Column of B that holds row r of a unit (hi); lo is two columns on.
+template <bool SPLIT>
+LC_DEV int many_column(int r) { return SPLIT ? 4 * (r >> 1) + (r & 1) : r; }
+
+constexpr int kLayThreads = 256;
+
+// A CTA lays out eight columns of B: eight F16 rows, or four F32 rows, two warps to
+// a row.
+template <typename T>
+__global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int cols, int chunks, ManyPlan plan, uint8_t* b, float* factor) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int R = SPLIT ? 4 : 8, PARTS = 8 / R;  // rows of a CTA, warps of a row
+    __shared__ float tops[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % PARTS;
+    griddep_wait();
+    griddep_launch();
+    const int groups = plan.n / 8, tile = blockIdx.x / groups, group = blockIdx.x % groups;
+    // F32: columns 8 group .. + 7 are hi and lo of rows 4 group .. + 3.
+    const int r = group * R + warp / PARTS, row = tile * plan.rows + r;
+    const bool there = r < plan.rows && row < p.batch;
+    const T* const x = (const T*)p.x + (there ? row * p.x_stride : 0);
+    const bool vec = ((uintptr_t)p.x | (uintptr_t)(p.x_stride * sizeof(T))) % 16 == 0;
+    const int octets = chunks * 8;
+    auto eight = [&](int o, float (&v)[8]) {
+        const int c = o * 8;
+        if (there && vec && c + 8 <= cols) {
+            if (SPLIT) {
+                const float4 lo = *reinterpret_cast<const float4*>(x + c), hi = *reinterpret_cast<const float4*>(x + c + 4);
+                v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+            } else {
+                unpack_h8(*reinterpret_cast<const uint4*>(x + c), v);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = there && c + i < cols ? (float)x[c + i] : 0.0f;
+        }
+    };
+    float up = 1.0f;
+    if (SPLIT) {
+        float top = 0.0f;
+#pragma unroll 2
+        for (int o = part * 32 + lane; o < octets; o += PARTS * 32) {
+            float v[8];
+            eight(o, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+        }
+        top = warp_max(top);
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+        const int e = split_row_exp(fmaxf(tops[warp], tops[warp ^ 1]));
+        up = pow2f(e);
+        if (there && part == 0 && lane == 0) factor[row] = pow2f(-e);
+    }
+    const int n = many_column<SPLIT>(r);
+    uint8_t* const to = b + ((int64_t)tile * chunks * groups + (n >> 3)) * 1024 + (n & 7) * 16;
+#pragma unroll 2
+    for (int o = part * 32 + lane; o < octets; o += PARTS * 32) {
+        float v[8];
+        eight(o, v);
+        if (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= up;
+        }
+        uint4 h, l;
+        split_octet(v, h, l);
+        uint8_t* const at = to + (int64_t)(o >> 3) * groups * 1024 + (o & 7) * 128;
+        *reinterpret_cast<uint4*>(at) = h;
+        if (SPLIT) *reinterpret_cast<uint4*>(at + 32) = l;
+    }
+}
+
+LC_DEV uint64_t many_pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+LC_DEV uint64_t many_pair(uint32_t a, uint32_t b) { return (uint64_t)b << 32 | a; }
+LC_DEV float2 many_two(uint64_t v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
+LC_DEV uint64_t many_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+LC_DEV uint64_t many_add(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+LC_DEV void many_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+// The loads before it are done; the values pass through, so that no use moves up.
+LC_DEV void many_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                   "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                   "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+LC_DEV bool many_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+LC_DEV void many_sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+LC_DEV uint32_t many_hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t v;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(a), "r"(b), "r"(c));
+    return v;
+}
+LC_DEV void many_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Product p, ManyPlan plan, int* err, uint64_t timeout_ns) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int NG = kW4Cols / GROUP;
+    constexpr int NA = kManyAStages, NB = kManyBStages;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* const sa = smem;                            // [stages][tile of 128 rows][row groups][octets][8][16]
+    uint8_t* const sb = sa + NA * kManyABytes;           // [stages][column groups][octets][8][16]
+    uint8_t* const sc = sb + NB * kManyBBytes;           // [warps][ring][tile][lane][16]
+    __shared__ __align__(8) uint64_t a_full[NA], a_empty[NA], b_full[NB], b_empty[NB], d_full[2], d_free[2], drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int cs = plan.cluster, units = plan.x_tiles * plan.w_tiles;
+    uint32_t rank = 0;
+    if (cs > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    if (tid == 0) {
+        unset = 0;
+        for (int i = 0; i < NA; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
+        for (int i = 0; i < NB; ++i) mbar_init(&b_full[i], 1), mbar_init(&b_empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_free[i], 8);
+        mbar_init(&drained, 1);
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    griddep_launch();
+    const uint32_t tmem = tmem_slot;
+    // Units of this CTA: those of a range (neighbours share rows of x), or one of a cluster.
+    const int ctas = gridDim.x / cs, id = blockIdx.x / cs;
+    const int u0 = (int)((int64_t)units * id / ctas), u1 = (int)((int64_t)units * (id + 1) / ctas);
+    const int block0 = (int)((int64_t)w.blocks * (int)rank / cs), block1 = (int)((int64_t)w.blocks * ((int)rank + 1) / cs);
+    const int chunks = 2 * (block1 - block0);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {  // by whole warps, which go on together
+        return (bool)__all_sync(0xffffffffu, mbar_try_wait(bar, parity) ||
+                                                 mbar_wait_bounded(bar, parity, err, globaltimer_ns() + timeout_ns, kDevTimeoutGrid));
+    };
+
+    if (warp >= 8 && warp < 12) {
+        // ---- codes to operands ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsCodes));
+        const int cw = warp - 8, g = lane & 7, t = lane >> 3;  // eight lanes write one core matrix
+        const uint32_t ring = smem_u32(sc) + cw * kManyRing * kManyRingBytes + lane * 16;
+        int a_unit = u0, a_chunk = 0;
+        auto tile_of = [&](int unit, int k) { return min((unit % plan.w_tiles) * (kManyRows / kW4Rows) + cw * 4 + k, w.tiles - 1); };
+        auto request = [&](int slot) {
+            if (a_unit < u1) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int64_t u = (int64_t)tile_of(a_unit, k) * w.blocks + block0 + (a_chunk >> 1);
+                    few_copy16(ring + slot * kManyRingBytes + k * 512, w.codes + u * kW4BlockBytes + (a_chunk & 1) * 512 + (4 * g + t) * 16);
+                }
+                if (++a_chunk == chunks) a_chunk = 0, ++a_unit;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        constexpr int ZN = GROUP == 32 ? 2 : 1;  // groups of a chunk
+        uint32_t zero[4];
+        auto load_zeros = [&](int unit, int chunk) {  // pairs (rows g, g + 8) of the chunk's groups
+            if constexpr (ZEROS) {
+                if (unit >= u1) return;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int64_t u = (int64_t)tile_of(unit, k) * w.blocks + block0 + (chunk >> 1);
+                    const int at = GROUP == 128 ? 0 : (chunk & 1) * ZN;
+                    const uint8_t* z = w.zeros + ((u * 8 + g) * NG + at) * 2;
+                    zero[k] = ZN == 2 ? *reinterpret_cast<const uint32_t*>(z) : *reinterpret_cast<const uint16_t*>(z);
+                }
+            }
+        };
+        for (int i = 0; i < kManyRing - 1; ++i) request(i);
+        load_zeros(u0, 0);
+        int i = 0, slot = 0;
+        for (int unit = u0; unit < u1 && ok; ++unit) {
+            for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i) {
+                request(slot == 0 ? kManyRing - 1 : slot - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kManyRing - 1) : "memory");
+                uint32_t z[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[k] = ZEROS ? zero[k] : 0x08080808u;
+                if (chunk + 1 < chunks) load_zeros(unit, chunk + 1);
+                else load_zeros(unit + 1, 0);
+                const int st = i % NA;
+                if (i >= NA) ok = wait(&a_empty[st], (i / NA - 1) & 1);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint4 c = few_lds128(ring + slot * kManyRingBytes + k * 512);
+                    const int tl = cw * 4 + k;
+                    const uint32_t to = smem_u32(sa) + st * kManyABytes + (tl >> 3) * (kManyABytes / 2) + (tl & 7) * 2048 + t * 128 + g * 16;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {  // runs of eight columns
+                        uint32_t a[4], b[4];
+                        few_codes(q ? c.z : c.x, a);
+                        few_codes(q ? c.w : c.y, b);
+                        // c 2^-17 2^15 - z / 4: exact
+                        const uint32_t zq = ZN == 2 ? z[k] >> (16 * q) : z[k];
+                        auto quarter = [](uint32_t v) {
+                            const __half2 h = __half2half2(__float2half_rn(-0.25f * (float)(v & 255u)));
+                            return *reinterpret_cast<const uint32_t*>(&h);
+                        };
+                        constexpr uint32_t kUp = 0x78007800u;  // 2^15, twice
+                        const uint32_t z0 = ZEROS ? quarter(zq) : 0xc000c000u, z1 = ZEROS ? quarter(zq >> 8) : 0xc000c000u;
+                        many_sts128(to + q * 512, many_hfma2(a[0], kUp, z0), many_hfma2(a[2], kUp, z0), many_hfma2(b[0], kUp, z0), many_hfma2(b[2], kUp, z0));
+                        many_sts128(to + 1024 + q * 512, many_hfma2(a[1], kUp, z1), many_hfma2(a[3], kUp, z1), many_hfma2(b[1], kUp, z1), many_hfma2(b[3], kUp, z1));
+                    }
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[st]);
+                slot = slot == kManyRing - 1 ? 0 : slot + 1;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (cs > 1) many_cluster_sync(), many_cluster_sync();
+    } else if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsRest));
+        if (warp == 12) {
+            // ---- products ----
+            const uint32_t idesc = tc_idesc_f16_f32(128, plan.n);
+            const uint64_t ad = tc_desc_kmajor(smem_u32(sa), 128, 1024), bd = tc_desc_kmajor(smem_u32(sb), 128, 1024);
+            constexpr int STEPS = GROUP / 16;  // products of a group
+            int i = 0, d = 0;                  // stages and groups so far
+            for (int unit = u0; unit < u1 && ok; ++unit) {
+                for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i) {
+                    const int st = i % NA, sbt = i % NB;
+                    ok = wait(&a_full[st], (i / NA) & 1);
+                    if (ok) ok = wait(&b_full[sbt], (i / NB) & 1);
+                    const uint64_t a0 = ad + st * (kManyABytes / 16), b0 = bd + sbt * (kManyBBytes / 16);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int at = (GROUP == 128 ? (chunk & 1) * 4 : 0) + k;  // product of the group
+                        if (at % STEPS == 0 && ok && d >= 2) ok = wait(&d_free[d & 1], ((d >> 1) - 1) & 1);
+                        if (!ok) break;
+                        if (k == 0 || at % STEPS == 0) tc_fence_after();
+                        if (many_elect()) {
+                            const uint32_t to = tmem + (d & 1) * 2 * kManyCols;
+                            tc_mma_f16(to, a0 + k * 16, b0 + k * 16, idesc, at % STEPS != 0);
+                            tc_mma_f16(to + kManyCols, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, at % STEPS != 0);
+                            if (at % STEPS == STEPS - 1) tc_commit(&d_full[d & 1]);
+                            if (k == 3) tc_commit(&a_empty[st]), tc_commit(&b_empty[sbt]);
+                        }
+                        __syncwarp();
+                        if (at % STEPS == STEPS - 1) ++d;
+                    }
+                }
+            }
+        } else if (warp == 13) {
+            // ---- copies of x ----
+            griddep_wait();
+            const uint32_t bytes = plan.n * kManyK * 2;
+            const uint64_t policy = l2_policy_evict_last();
+            int i = 0;
+            for (int unit = u0; unit < u1 && ok; ++unit) {
+                const uint8_t* from = plan.b + ((int64_t)(unit / plan.w_tiles) * 2 * w.blocks + 2 * block0) * bytes;
+                for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i, from += bytes) {
+                    const int st = i % NB;
+                    if (i >= NB) ok = wait(&b_empty[st], (i / NB - 1) & 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&b_full[st], bytes);
+                        bulk_g2s(sb + st * kManyBBytes, from, bytes, &b_full[st], policy);
+                    }
+                    __syncwarp();
+                }
+            }
+            // The last copies land before the CTA may end, also after a failure.
+            for (int k = i > NB ? i - NB : 0; k < i; ++k)
+                mbar_wait_bounded(&b_full[k % NB], (k / NB) & 1, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
+        }
+        __syncwarp();
+        if (cs > 1) many_cluster_sync(), many_cluster_sync();
+    } else {
+        // ---- sums ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegsSum));
+        griddep_wait();
+        constexpr int PAIRS = SPLIT ? kManyCols / 4 : kManyCols / 2;  // of rows of x
+        const int row = warp * 32 + lane;   // of the unit
+        const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * kManyCols;
+        int d = 0;
+        for (int unit = u0; unit < u1; ++unit) {
+            const int wt = unit % plan.w_tiles, xt = unit / plan.w_tiles;
+            const int64_t out = (int64_t)wt * kManyRows + row;
+            const int tile = min(wt * (kManyRows / kW4Rows) + (row >> 4), w.tiles - 1);
+            uint64_t total[PAIRS];
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) total[k] = 0;
+            // Scales of a block: pairs (rows g, g + 8) of its groups.
+            uint32_t sc_next[NG];
+            auto load_scales = [&](int block) {
+                const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + (((int64_t)tile * w.blocks + block) * 8 + (row & 7)) * NG;
+                if (NG == 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
+                    sc_next[0] = v.x, sc_next[NG > 1 ? 1 : 0] = v.y, sc_next[NG > 2 ? 2 : 0] = v.z, sc_next[NG > 2 ? 3 : 0] = v.w;
+                } else if (NG == 2) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+                    sc_next[0] = v.x, sc_next[NG > 1 ? 1 : 0] = v.y;
+                } else {
+                    sc_next[0] = __ldg(s);
+                }
+            };
+            load_scales(block0);
+            for (int block = block0; block < block1 && ok; ++block) {
+                uint32_t scale[NG];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) scale[k] = row & 8 ? sc_next[k] >> 16 : sc_next[k] & 0xffffu;
+                if (block + 1 < block1) load_scales(block + 1);
+#pragma unroll
+                for (int k = 0; k < NG; ++k, ++d) {
+                    if (ok) ok = wait(&d_full[d & 1], (d >> 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float s = __half2float(__ushort_as_half((uint16_t)scale[k]));
+                    const uint64_t s2 = many_pair(s, s);
+#pragma unroll
+                    for (int c = 0; c < kManyCols / 32; ++c) {
+                        if (c * 32 >= plan.n) continue;
+                        uint32_t v[32];
+                        many_ld32(from + (d & 1) * 2 * kManyCols + c * 32, v);
+                        many_wait_ld(v);
+                        if (SPLIT) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const uint64_t both = many_add(many_pair(v[4 * e], v[4 * e + 1]), many_pair(v[4 * e + 2], v[4 * e + 3]));
+                                total[c * (PAIRS / 4) + e] = many_fma(s2, both, total[c * (PAIRS / 4) + e]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                total[c * (PAIRS / 4) + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[c * (PAIRS / 4) + e]);
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&d_free[d & 1]);
+                }
+            }
+            auto store = [&](int r, float v) {
+                const int b = xt * plan.rows + r;
+                if (r >= plan.rows || b >= p.batch || out >= w.rows || !ok) return;
+                v *= 4.0f;
+                if (SPLIT) v *= plan.factor[b];
+                if (p.residual) v += (float)((const T*)p.residual)[b * p.residual_stride + out];
+                ((T*)p.y)[b * p.y_stride + out] = (T)v;
+            };
+            if (cs == 1) {
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) {
+                    const float2 v = many_two(total[k]);
+                    store(2 * k, v.x);
+                    store(2 * k + 1, v.y);
+                }
+            } else {
+                // Row r of x belongs to CTA (r / 2) % cs: [sender][r / 2 / cs][r % 2][256] in
+                // the stages, which nobody needs any more.
+                many_cluster_sync();
+                const int each = (PAIRS + cs - 1) / cs * 2 * kManyRows;  // floats of a sender
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) {
+                    if (2 * k >= plan.rows) continue;
+                    const float2 v = many_two(total[k]);
+                    uint32_t to;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                                 : "=r"(to)
+                                 : "r"(smem_u32(smem) + (rank * each + (k / cs) * 2 * kManyRows + row) * 4), "r"(k % cs));
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v.x) : "memory");
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + kManyRows * 4), "f"(v.y) : "memory");
+                }
+                many_cluster_sync();
+                const float* const mine = reinterpret_cast<const float*>(smem) + row;
+                for (int k = rank; 2 * k < plan.rows; k += cs) {
+                    float x = 0.0f, y = 0.0f;
+                    for (int c = 0; c < cs; ++c) {
+                        x += mine[c * each + (k / cs) * 2 * kManyRows];
+                        y += mine[c * each + (k / cs) * 2 * kManyRows + kManyRows];
+                    }
+                    store(2 * k, x);
+                    store(2 * k + 1, y);
+                }
+            }
+        }
+    }
+    // Everyone meets when all products and their arrivals are done, also where
+    // a wait has given up.
+    if (warp == 12) {
+        if (many_elect()) tc_commit(&drained);
+        mbar_wait_bounded(&drained, 0, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
+        if (unset) atomicCAS(err, 0, kDevTimeoutDrain);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace lc

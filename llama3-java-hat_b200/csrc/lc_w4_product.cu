@@ -5,6 +5,7 @@
 #include "lc_internal.h"
 #include "lc_w4.h"
 #include "lc_w4_few.cuh"
+#include "lc_w4_many.cuh"
 
 #ifndef FEW_MEET
 #define FEW_MEET 2
@@ -70,28 +71,97 @@ cudaError_t few(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
                         : few_as<T, GROUP, ZEROS, 2>(w, p, num_sms, st);
 }
 
+// Rows of x that one pass through the workspace takes, whole units of them: 0 where
+// not even one unit fits.
+constexpr size_t kLayBytes = 32u << 20, kFactorBytes = 1u << 20;
+int64_t many_rows(const W4& w, bool split) {
+    const int64_t columns = (int64_t)(kLayBytes / ((size_t)w.blocks * kW4Cols * 2)) / kManyCols * kManyCols;
+    const int64_t rows = columns / (split ? 2 : 1), most = kFactorBytes / 4;
+    return rows < most ? rows : most;
+}
+
+template <typename T, int GROUP, bool ZEROS>
+cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st) {
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    ManyPlan plan;
+    const int columns = p.batch * PARTS;
+    plan.x_tiles = (columns + kManyCols - 1) / kManyCols;
+    plan.n = ((columns + plan.x_tiles - 1) / plan.x_tiles + 15) / 16 * 16;
+    plan.rows = plan.n / PARTS;
+    plan.w_tiles = (w.rows + kManyRows - 1) / kManyRows;
+    plan.b = (const uint8_t*)ws;
+    plan.factor = (const float*)((uint8_t*)ws + kLayBytes);
+    // CTAs of a unit: what its CTAs and the units that come after one another take, in
+    // blocks; a unit's beginning and end cost about four.
+    const int64_t units = (int64_t)plan.x_tiles * plan.w_tiles;
+    int64_t best = 0;
+    for (int cs = 1; cs <= kManyMaxCluster && cs <= w.blocks; cs *= 2) {
+        const int64_t cost = (units * cs + num_sms - 1) / num_sms * ((w.blocks + cs - 1) / cs + 4);
+        if (!best || cost < best) best = cost, plan.cluster = cs;
+    }
+    cudaError_t e = launch_ex(w4_lay_kernel<T>, dim3((unsigned)(plan.x_tiles * (plan.n / 8))), dim3(kLayThreads), 0, st, true, p, w.cols,
+                              2 * w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
+    if (e != cudaSuccess) return e;
+    auto* kernel = w4_many_kernel<T, GROUP, ZEROS>;
+    // The register split draws on what the launch has: more than that would wait forever.
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs < kManyRegsLaunch) return cudaErrorInvalidKernelImage;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    const int64_t ctas = plan.cluster > 1 ? units * plan.cluster : units < num_sms ? units : num_sms;
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = kManySmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)plan.cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, w, p, plan, err, (uint64_t)2000000000ull);
+}
+
+template <typename T, int GROUP, bool ZEROS>
+cudaError_t product_as(const W4& w, const W4Product& all, int num_sms, void* ws, int* err, cudaStream_t st) {
+    const int64_t step = ws ? many_rows(w, sizeof(T) == 4) : few_rows(all.dtype);
+    for (int64_t r = 0; r < all.batch; r += step) {
+        W4Product p = all;
+        p.batch = (int)(all.batch - r < step ? all.batch - r : step);
+        p.x = (const T*)all.x + r * all.x_stride;
+        p.y = (T*)all.y + r * all.y_stride;
+        if (all.residual) p.residual = (const T*)all.residual + r * all.residual_stride;
+        const cudaError_t e = ws ? many<T, GROUP, ZEROS>(w, p, num_sms, ws, err, st) : few<T, GROUP, ZEROS>(w, p, num_sms, st);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
 template <typename T, int GROUP>
-cudaError_t product(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
-    return w.zeros ? few<T, GROUP, true>(w, p, num_sms, st) : few<T, GROUP, false>(w, p, num_sms, st);
+cudaError_t product(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st) {
+    return w.zeros ? product_as<T, GROUP, true>(w, p, num_sms, ws, err, st) : product_as<T, GROUP, false>(w, p, num_sms, ws, err, st);
+}
+template <typename T>
+cudaError_t product(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st) {
+    return w.group == 32   ? product<T, 32>(w, p, num_sms, ws, err, st)
+           : w.group == 64 ? product<T, 64>(w, p, num_sms, ws, err, st)
+                           : product<T, 128>(w, p, num_sms, ws, err, st);
 }
 
 }  // namespace
 
-cudaError_t launch_w4_product(const W4& w, const W4Product& all, int num_sms, cudaStream_t st) {
-    const int elem = all.dtype == kRowF32 ? 4 : 2;
-    for (int r = 0; r < all.batch; r += few_rows(all.dtype)) {
-        W4Product p = all;
-        p.batch = all.batch - r < few_rows(all.dtype) ? all.batch - r : few_rows(all.dtype);
-        p.x = (const uint8_t*)all.x + r * all.x_stride * elem;
-        p.y = (uint8_t*)all.y + r * all.y_stride * elem;
-        if (all.residual) p.residual = (const uint8_t*)all.residual + r * all.residual_stride * elem;
-        const bool f32 = p.dtype == kRowF32;
-        const cudaError_t e = w.group == 32   ? (f32 ? product<float, 32>(w, p, num_sms, st) : product<__half, 32>(w, p, num_sms, st))
-                              : w.group == 64 ? (f32 ? product<float, 64>(w, p, num_sms, st) : product<__half, 64>(w, p, num_sms, st))
-                                              : (f32 ? product<float, 128>(w, p, num_sms, st) : product<__half, 128>(w, p, num_sms, st));
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+bool w4_product_uses_ws(const W4& w, const W4Product& p) {
+    return p.batch > few_rows(p.dtype) && many_rows(w, p.dtype == kRowF32) > 0;
+}
+size_t w4_product_ws_bytes() { return kLayBytes + kFactorBytes; }
+
+cudaError_t launch_w4_product(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st) {
+    return p.dtype == kRowF32 ? product<float>(w, p, num_sms, ws, err, st) : product<__half>(w, p, num_sms, ws, err, st);
 }
 
 }  // namespace lc
