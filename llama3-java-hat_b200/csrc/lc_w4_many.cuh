@@ -46,7 +46,8 @@ struct ManyPlan {
     int n;         // columns of B of a unit (a multiple of 16)
     int rows;      // rows of x of a unit
     int x_tiles, w_tiles;
-    int cluster;   // CTAs that share the columns of W
+    int cluster;   // CTAs that share the columns of W, a power of two
+    int cluster_log2;
     const uint8_t* b;      // [x tile][chunk of 64 columns][n / 8][8 octets][8][16 bytes]
     const float* factor;   // [batch] what the rows of x were divided by
 };
@@ -55,15 +56,16 @@ struct ManyPlan {
 template <bool SPLIT>
 LC_DEV int many_column(int r) { return SPLIT ? 4 * (r >> 1) + (r & 1) : r; }
 
-constexpr int kLayThreads = 256;
+constexpr int kLayThreads = 512;
 
-// A CTA lays out eight columns of B: eight F16 rows, or four F32 rows, two warps to
-// a row.
+// A CTA lays out eight columns of B: eight F16 rows with two warps each, or four
+// F32 rows with four.
 template <typename T>
 __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int cols, int chunks, ManyPlan plan, uint8_t* b, float* factor) {
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int R = SPLIT ? 4 : 8, PARTS = 8 / R;  // rows of a CTA, warps of a row
-    __shared__ float tops[8];
+    constexpr int R = SPLIT ? 4 : 8, PARTS = kLayThreads / 32 / R;  // rows of a CTA, warps of a row
+    constexpr int HOLD = 4;  // octets of columns that a lane keeps at a time
+    __shared__ float tops[kLayThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % PARTS;
     griddep_wait();
     griddep_launch();
@@ -88,38 +90,56 @@ __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int co
             for (int i = 0; i < 8; ++i) v[i] = there && c + i < cols ? (float)x[c + i] : 0.0f;
         }
     };
+    float v[HOLD][8];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h) {
+            const int o = base + (h * PARTS + part) * 32 + lane;
+            if (o < octets) eight(o, v[h]);
+        }
+    };
+    constexpr int STEP = HOLD * PARTS * 32;
     float up = 1.0f;
+    load(0);
     if (SPLIT) {
         float top = 0.0f;
-#pragma unroll 2
-        for (int o = part * 32 + lane; o < octets; o += PARTS * 32) {
-            float v[8];
-            eight(o, v);
+        for (int base = 0; base < octets; base += STEP) {
+            if (base) load(base);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+            for (int h = 0; h < HOLD; ++h) {
+                if (base + (h * PARTS + part) * 32 + lane >= octets) continue;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[h][i]));
+            }
         }
         top = warp_max(top);
         if (lane == 0) tops[warp] = top;
         __syncthreads();
-        const int e = split_row_exp(fmaxf(tops[warp], tops[warp ^ 1]));
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) top = fmaxf(top, tops[warp / PARTS * PARTS + i]);
+        const int e = split_row_exp(top);
         up = pow2f(e);
         if (there && part == 0 && lane == 0) factor[row] = pow2f(-e);
+        if (octets > STEP) load(0);
     }
     const int n = many_column<SPLIT>(r);
     uint8_t* const to = b + ((int64_t)tile * chunks * groups + (n >> 3)) * 1024 + (n & 7) * 16;
-#pragma unroll 2
-    for (int o = part * 32 + lane; o < octets; o += PARTS * 32) {
-        float v[8];
-        eight(o, v);
-        if (SPLIT) {
+    for (int base = 0; base < octets; base += STEP) {
+        if (base) load(base);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= up;
+        for (int h = 0; h < HOLD; ++h) {
+            const int o = base + (h * PARTS + part) * 32 + lane;
+            if (o >= octets) continue;
+            if (SPLIT) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[h][i] *= up;
+            }
+            uint4 hi, lo;
+            split_octet(v[h], hi, lo);
+            uint8_t* const at = to + (int64_t)(o >> 3) * groups * 1024 + (o & 7) * 128;
+            *reinterpret_cast<uint4*>(at) = hi;
+            if (SPLIT) *reinterpret_cast<uint4*>(at + 32) = lo;
         }
-        uint4 h, l;
-        split_octet(v, h, l);
-        uint8_t* const at = to + (int64_t)(o >> 3) * groups * 1024 + (o & 7) * 128;
-        *reinterpret_cast<uint4*>(at) = h;
-        if (SPLIT) *reinterpret_cast<uint4*>(at + 32) = l;
     }
 }
 
@@ -229,12 +249,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
         const uint32_t ring = smem_u32(sc) + cw * kManyRing * kManyRingBytes + lane * 16;
         int a_unit = u0, a_chunk = 0;
         auto tile_of = [&](int unit, int k) { return min((unit % plan.w_tiles) * (kManyRows / kW4Rows) + cw * 4 + k, w.tiles - 1); };
+        const uint8_t* a_from[4];
         auto request = [&](int slot) {
             if (a_unit < u1) {
+                if (a_chunk == 0) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        a_from[k] = w.codes + ((int64_t)tile_of(a_unit, k) * w.blocks + block0) * kW4BlockBytes + (4 * g + t) * 16;
+                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int64_t u = (int64_t)tile_of(a_unit, k) * w.blocks + block0 + (a_chunk >> 1);
-                    few_copy16(ring + slot * kManyRingBytes + k * 512, w.codes + u * kW4BlockBytes + (a_chunk & 1) * 512 + (4 * g + t) * 16);
+                    few_copy16(ring + slot * kManyRingBytes + k * 512, a_from[k]);
+                    a_from[k] += kW4BlockBytes / 2;
                 }
                 if (++a_chunk == chunks) a_chunk = 0, ++a_unit;
             }
@@ -269,9 +295,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 const int st = i % NA;
                 if (i >= NA) ok = wait(&a_empty[st], (i / NA - 1) & 1);
                 if (!ok) break;
+                uint4 held[4];  // read before anything is written, or each tile would wait for the one before
+#pragma unroll
+                for (int k = 0; k < 4; ++k) held[k] = few_lds128(ring + slot * kManyRingBytes + k * 512);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint4 c = few_lds128(ring + slot * kManyRingBytes + k * 512);
+                    const uint4 c = held[k];
                     const int tl = cw * 4 + k;
                     const uint32_t to = smem_u32(sa) + st * kManyABytes + (tl >> 3) * (kManyABytes / 2) + (tl & 7) * 2048 + t * 128 + g * 16;
 #pragma unroll
@@ -305,29 +334,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             // ---- products ----
             const uint32_t idesc = tc_idesc_f16_f32(128, plan.n);
             const uint64_t ad = tc_desc_kmajor(smem_u32(sa), 128, 1024), bd = tc_desc_kmajor(smem_u32(sb), 128, 1024);
-            constexpr int STEPS = GROUP / 16;  // products of a group
-            int i = 0, d = 0;                  // stages and groups so far
+            // One elected thread issues all products of a chunk, or of a group where it is
+            // less, at once: the tensor cores then have the next while the warp waits.
+            constexpr int STEPS = GROUP / 16, RUN = STEPS < 4 ? STEPS : 4;  // products of a group, of a run
+            int i = 0, d = 0;  // stages and groups so far
             for (int unit = u0; unit < u1 && ok; ++unit) {
                 for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i) {
                     const int st = i % NA, sbt = i % NB;
-                    ok = wait(&a_full[st], (i / NA) & 1);
-                    if (ok) ok = wait(&b_full[sbt], (i / NB) & 1);
+                    const bool begins = GROUP < 128 || (chunk & 1) == 0, ends = GROUP < 128 || (chunk & 1) == 1;
                     const uint64_t a0 = ad + st * (kManyABytes / 16), b0 = bd + sbt * (kManyBBytes / 16);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int at = (GROUP == 128 ? (chunk & 1) * 4 : 0) + k;  // product of the group
-                        if (at % STEPS == 0 && ok && d >= 2) ok = wait(&d_free[d & 1], ((d >> 1) - 1) & 1);
+                    for (int run = 0; run < 4 / RUN; ++run) {
+                        if (begins && d >= 2) ok = ok && wait(&d_free[d & 1], ((d >> 1) - 1) & 1);
+                        if (run == 0) ok = ok && wait(&b_full[sbt], (i / NB) & 1) && wait(&a_full[st], (i / NA) & 1);
                         if (!ok) break;
-                        if (k == 0 || at % STEPS == 0) tc_fence_after();
+                        tc_fence_after();
+                        const uint32_t to = tmem + (d & 1) * 2 * kManyCols;
                         if (many_elect()) {
-                            const uint32_t to = tmem + (d & 1) * 2 * kManyCols;
-                            tc_mma_f16(to, a0 + k * 16, b0 + k * 16, idesc, at % STEPS != 0);
-                            tc_mma_f16(to + kManyCols, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, at % STEPS != 0);
-                            if (at % STEPS == STEPS - 1) tc_commit(&d_full[d & 1]);
-                            if (k == 3) tc_commit(&a_empty[st]), tc_commit(&b_empty[sbt]);
+#pragma unroll
+                            for (int k = run * RUN; k < (run + 1) * RUN; ++k) {
+                                const uint32_t more = !(begins && k == run * RUN);
+                                tc_mma_f16(to, a0 + k * 16, b0 + k * 16, idesc, more);
+                                tc_mma_f16(to + kManyCols, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, more);
+                            }
+                            if (ends) tc_commit(&d_full[d & 1]);
+                            if (run == 4 / RUN - 1) tc_commit(&a_empty[st]), tc_commit(&b_empty[sbt]);
                         }
                         __syncwarp();
-                        if (at % STEPS == STEPS - 1) ++d;
+                        d += ends;
                     }
                 }
             }
@@ -421,13 +455,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                     if (lane == 0) mbar_arrive(&d_free[d & 1]);
                 }
             }
+            // Rows of x from the unit's first on, this thread's element of each.
+            const int b0 = xt * plan.rows, n = !ok || out >= w.rows ? 0 : min(plan.rows, p.batch - b0);
+            T* const y = (T*)p.y + b0 * p.y_stride + out;
+            const T* const res = p.residual ? (const T*)p.residual + b0 * p.residual_stride + out : nullptr;
             auto store = [&](int r, float v) {
-                const int b = xt * plan.rows + r;
-                if (r >= plan.rows || b >= p.batch || out >= w.rows || !ok) return;
+                if (r >= n) return;
                 v *= 4.0f;
-                if (SPLIT) v *= plan.factor[b];
-                if (p.residual) v += (float)((const T*)p.residual)[b * p.residual_stride + out];
-                ((T*)p.y)[b * p.y_stride + out] = (T)v;
+                if (SPLIT) v *= plan.factor[b0 + r];
+                if (res) v += (float)res[r * p.residual_stride];
+                y[r * p.y_stride] = (T)v;
             };
             if (cs == 1) {
 #pragma unroll
@@ -440,7 +477,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 // Row r of x belongs to CTA (r / 2) % cs: [sender][r / 2 / cs][r % 2][256] in
                 // the stages, which nobody needs any more.
                 many_cluster_sync();
-                const int each = (PAIRS + cs - 1) / cs * 2 * kManyRows;  // floats of a sender
+                const int log2 = plan.cluster_log2, each = ((PAIRS + cs - 1) >> log2) * 2 * kManyRows;  // floats of a sender
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) {
                     if (2 * k >= plan.rows) continue;
@@ -448,7 +485,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                     uint32_t to;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                                  : "=r"(to)
-                                 : "r"(smem_u32(smem) + (rank * each + (k / cs) * 2 * kManyRows + row) * 4), "r"(k % cs));
+                                 : "r"(smem_u32(smem) + (rank * each + (k >> log2) * 2 * kManyRows + row) * 4), "r"(k & (cs - 1)));
                     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v.x) : "memory");
                     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + kManyRows * 4), "f"(v.y) : "memory");
                 }
@@ -457,8 +494,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 for (int k = rank; 2 * k < plan.rows; k += cs) {
                     float x = 0.0f, y = 0.0f;
                     for (int c = 0; c < cs; ++c) {
-                        x += mine[c * each + (k / cs) * 2 * kManyRows];
-                        y += mine[c * each + (k / cs) * 2 * kManyRows + kManyRows];
+                        x += mine[c * each + (k >> log2) * 2 * kManyRows];
+                        y += mine[c * each + (k >> log2) * 2 * kManyRows + kManyRows];
                     }
                     store(2 * k, x);
                     store(2 * k + 1, y);

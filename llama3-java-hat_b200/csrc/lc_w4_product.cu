@@ -99,6 +99,7 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
         const int64_t cost = (units * cs + num_sms - 1) / num_sms * ((w.blocks + cs - 1) / cs + 4);
         if (!best || cost < best) best = cost, plan.cluster = cs;
     }
+    for (plan.cluster_log2 = 0; 1 << plan.cluster_log2 < plan.cluster;) ++plan.cluster_log2;
     cudaError_t e = launch_ex(w4_lay_kernel<T>, dim3((unsigned)(plan.x_tiles * (plan.n / 8))), dim3(kLayThreads), 0, st, true, p, w.cols,
                               2 * w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
     if (e != cudaSuccess) return e;
