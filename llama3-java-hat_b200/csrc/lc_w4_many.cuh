@@ -15,12 +15,14 @@
 // What bounds it: the products, as long as a group has more columns than the
 // epilogue takes instructions for (one packed FMA for two elements of D).
 //
-// Warps 0-7: epilogue, four for each 128 rows.  Warps 8-11: codes to operands,
-// through rings of their own (cp.async).  Warp 12 issues the products, warp 13 the
+// Warps 0-7: epilogue, four for each 128 rows.  Warps 8-15: codes to operands,
+// through rings of their own (cp.async).  Warp 16 issues the products, warp 17 the
 // copies of x (bulk copies, whole stages).  Registers move to the epilogue.  With
 // few units a cluster shares the columns; its CTAs add their sums through each
 // other's shared memory.
 #pragma once
+
+#include <type_traits>
 
 #include "lc_internal.h"
 #include "lc_tcgen05.cuh"
@@ -29,18 +31,18 @@
 
 namespace lc {
 
-constexpr int kManyThreads = 16 * 32;
+constexpr int kManyThreads = 20 * 32;
 constexpr int kManyRows = 256;      // of W, of a unit
 constexpr int kManyCols = 128;      // of B, at most
-constexpr int kManyK = 64;          // columns of W of a stage
-constexpr int kManyAStages = 3, kManyBStages = 4, kManyRing = 6;
+constexpr int kManyK = kW4Cols;     // columns of W of a stage: a block
+constexpr int kManyStages = 2, kManyMaxRing = 5;
 constexpr int kManyABytes = kManyRows * kManyK * 2, kManyBBytes = kManyCols * kManyK * 2;
-constexpr int kManyRingBytes = 4 * 512;  // of a warp: a chunk of four tiles
-constexpr int kManySmem = kManyAStages * kManyABytes + kManyBStages * kManyBBytes + 4 * kManyRing * kManyRingBytes;
+constexpr int kManyRingBytes = 2 * kW4BlockBytes;  // of a warp: a block of two tiles
+constexpr int kManySmem = 226 * 1024;
 constexpr int kManyMaxCluster = 8;
 // Registers after the split; their sum over the warpgroups is the launch's.
-constexpr int kManyRegsSum = 184, kManyRegsCodes = 80, kManyRegsRest = 64;
-constexpr int kManyRegsLaunch = (2 * kManyRegsSum + kManyRegsCodes + kManyRegsRest + 3) / 4;
+constexpr int kManyRegsSum = 160, kManyRegsCodes = 56, kManyRegsRest = 48;
+constexpr int kManyRegsLaunch = (2 * kManyRegsSum + 2 * kManyRegsCodes + kManyRegsRest + 4) / 5;
 
 struct ManyPlan {
     int n;         // columns of B of a unit (a multiple of 16)
@@ -48,7 +50,9 @@ struct ManyPlan {
     int x_tiles, w_tiles;
     int cluster;   // CTAs that share the columns of W, a power of two
     int cluster_log2;
-    const uint8_t* b;      // [x tile][chunk of 64 columns][n / 8][8 octets][8][16 bytes]
+    int sets;      // groups of a block over groups of a D: those that fit 256 columns of tensor memory
+    int ring;      // blocks of a warp's ring of codes
+    const uint8_t* b;      // [x tile][block][n / 8][16 octets][8][16 bytes]
     const float* factor;   // [batch] what the rows of x were divided by
 };
 
@@ -61,7 +65,7 @@ constexpr int kLayThreads = 512;
 // A CTA lays out eight columns of B: eight F16 rows with two warps each, or four
 // F32 rows with four.
 template <typename T>
-__global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int cols, int chunks, ManyPlan plan, uint8_t* b, float* factor) {
+__global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int cols, int blocks, ManyPlan plan, uint8_t* b, float* factor) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int R = SPLIT ? 4 : 8, PARTS = kLayThreads / 32 / R;  // rows of a CTA, warps of a row
     constexpr int HOLD = 4;  // octets of columns that a lane keeps at a time
@@ -75,7 +79,7 @@ __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int co
     const bool there = r < plan.rows && row < p.batch;
     const T* const x = (const T*)p.x + (there ? row * p.x_stride : 0);
     const bool vec = ((uintptr_t)p.x | (uintptr_t)(p.x_stride * sizeof(T))) % 16 == 0;
-    const int octets = chunks * 8;
+    const int octets = blocks * 16;
     auto eight = [&](int o, float (&v)[8]) {
         const int c = o * 8;
         if (there && vec && c + 8 <= cols) {
@@ -123,7 +127,7 @@ __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int co
         if (octets > STEP) load(0);
     }
     const int n = many_column<SPLIT>(r);
-    uint8_t* const to = b + ((int64_t)tile * chunks * groups + (n >> 3)) * 1024 + (n & 7) * 16;
+    uint8_t* const to = b + ((int64_t)tile * blocks * groups + (n >> 3)) * 2048 + (n & 7) * 16;
     for (int base = 0; base < octets; base += STEP) {
         if (base) load(base);
 #pragma unroll
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int co
             }
             uint4 hi, lo;
             split_octet(v[h], hi, lo);
-            uint8_t* const at = to + (int64_t)(o >> 3) * groups * 1024 + (o & 7) * 128;
+            uint8_t* const at = to + (int64_t)(o >> 4) * groups * 2048 + (o & 15) * 128;
             *reinterpret_cast<uint4*>(at) = hi;
             if (SPLIT) *reinterpret_cast<uint4*>(at + 32) = lo;
         }
@@ -160,27 +164,6 @@ LC_DEV uint64_t many_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
-LC_DEV void many_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr));
-}
-// The loads before it are done; the values pass through, so that no use moves up.
-LC_DEV void many_wait_ld(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
-                   "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
-                   "+r"(v[30]), "+r"(v[31])
-                 :
-                 : "memory");
-}
 LC_DEV bool many_elect() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
@@ -202,12 +185,12 @@ template <typename T, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Product p, ManyPlan plan, int* err, uint64_t timeout_ns) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NG = kW4Cols / GROUP;
-    constexpr int NA = kManyAStages, NB = kManyBStages;
+    constexpr int NS = kManyStages;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const sa = smem;                            // [stages][tile of 128 rows][row groups][octets][8][16]
-    uint8_t* const sb = sa + NA * kManyABytes;           // [stages][column groups][octets][8][16]
-    uint8_t* const sc = sb + NB * kManyBBytes;           // [warps][ring][tile][lane][16]
-    __shared__ __align__(8) uint64_t a_full[NA], a_empty[NA], b_full[NB], b_empty[NB], d_full[2], d_free[2], drained;
+    uint8_t* const sb = sa + NS * kManyABytes;           // [stages][column groups][octets][8][16]
+    uint8_t* const sc = sb + NS * plan.n * kManyK * 2;   // [warps][ring][tile][half][lane][16]
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], d_full[2], d_free[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -216,13 +199,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     if (cs > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     if (tid == 0) {
         unset = 0;
-        for (int i = 0; i < NA; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
-        for (int i = 0; i < NB; ++i) mbar_init(&b_full[i], 1), mbar_init(&b_empty[i], 1);
+        for (int i = 0; i < NS; ++i) mbar_init(&full[i], 8 + 1), mbar_init(&empty[i], 1);  // operand warps and the copy of x
         for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_free[i], 8);
         mbar_init(&drained, 1);
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
     }
@@ -235,81 +217,91 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     const int ctas = gridDim.x / cs, id = blockIdx.x / cs;
     const int u0 = (int)((int64_t)units * id / ctas), u1 = (int)((int64_t)units * (id + 1) / ctas);
     const int block0 = (int)((int64_t)w.blocks * (int)rank / cs), block1 = (int)((int64_t)w.blocks * ((int)rank + 1) / cs);
-    const int chunks = 2 * (block1 - block0);
+    const int blocks = block1 - block0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // by whole warps, which go on together
         return (bool)__all_sync(0xffffffffu, mbar_try_wait(bar, parity) ||
                                                  mbar_wait_bounded(bar, parity, err, globaltimer_ns() + timeout_ns, kDevTimeoutGrid));
     };
 
-    if (warp >= 8 && warp < 12) {
+    if (warp >= 8 && warp < 16) {
         // ---- codes to operands ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsCodes));
         const int cw = warp - 8, g = lane & 7, t = lane >> 3;  // eight lanes write one core matrix
-        const uint32_t ring = smem_u32(sc) + cw * kManyRing * kManyRingBytes + lane * 16;
-        int a_unit = u0, a_chunk = 0;
-        auto tile_of = [&](int unit, int k) { return min((unit % plan.w_tiles) * (kManyRows / kW4Rows) + cw * 4 + k, w.tiles - 1); };
-        const uint8_t* a_from[4];
+        const uint32_t ring = smem_u32(sc) + cw * plan.ring * kManyRingBytes + lane * 16;
+        int a_unit = u0, a_block = 0;
+        auto tile_of = [&](int unit, int k) { return min((unit % plan.w_tiles) * (kManyRows / kW4Rows) + cw * 2 + k, w.tiles - 1); };
+        const uint8_t* a_from[2];
         auto request = [&](int slot) {
             if (a_unit < u1) {
-                if (a_chunk == 0) {
+                if (a_block == 0) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < 2; ++k)
                         a_from[k] = w.codes + ((int64_t)tile_of(a_unit, k) * w.blocks + block0) * kW4BlockBytes + (4 * g + t) * 16;
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    few_copy16(ring + slot * kManyRingBytes + k * 512, a_from[k]);
-                    a_from[k] += kW4BlockBytes / 2;
+                for (int k = 0; k < 2; ++k) {
+                    few_copy16(ring + slot * kManyRingBytes + k * 1024, a_from[k]);
+                    few_copy16(ring + slot * kManyRingBytes + k * 1024 + 512, a_from[k] + 512);
+                    a_from[k] += kW4BlockBytes;
                 }
-                if (++a_chunk == chunks) a_chunk = 0, ++a_unit;
+                if (++a_block == blocks) a_block = 0, ++a_unit;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        constexpr int ZN = GROUP == 32 ? 2 : 1;  // groups of a chunk
-        uint32_t zero[4];
-        auto load_zeros = [&](int unit, int chunk) {  // pairs (rows g, g + 8) of the chunk's groups
+        // Zero points of the lane's rows: pairs (rows g, g + 8) of a block's groups.
+        constexpr int ZW = (NG + 1) / 2;  // words
+        uint32_t zero[2][ZW];
+        auto load_zeros = [&](int unit, int block) {
             if constexpr (ZEROS) {
                 if (unit >= u1) return;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int64_t u = (int64_t)tile_of(unit, k) * w.blocks + block0 + (chunk >> 1);
-                    const int at = GROUP == 128 ? 0 : (chunk & 1) * ZN;
-                    const uint8_t* z = w.zeros + ((u * 8 + g) * NG + at) * 2;
-                    zero[k] = ZN == 2 ? *reinterpret_cast<const uint32_t*>(z) : *reinterpret_cast<const uint16_t*>(z);
+                for (int k = 0; k < 2; ++k) {
+                    const uint8_t* z = w.zeros + (((int64_t)tile_of(unit, k) * w.blocks + block0 + block) * 8 + g) * NG * 2;
+#pragma unroll
+                    for (int i = 0; i < ZW; ++i)
+                        zero[k][i] = NG == 1 ? *reinterpret_cast<const uint16_t*>(z) : reinterpret_cast<const uint32_t*>(z)[i];
                 }
             }
         };
-        for (int i = 0; i < kManyRing - 1; ++i) request(i);
+        for (int i = 0; i < plan.ring - 1; ++i) request(i);
         load_zeros(u0, 0);
         int i = 0, slot = 0;
         for (int unit = u0; unit < u1 && ok; ++unit) {
-            for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i) {
-                request(slot == 0 ? kManyRing - 1 : slot - 1);
-                asm volatile("cp.async.wait_group %0;" ::"n"(kManyRing - 1) : "memory");
-                uint32_t z[4];
+            for (int block = 0; block < blocks && ok; ++block, ++i) {
+                request(slot == 0 ? plan.ring - 1 : slot - 1);
+                switch (plan.ring) {  // all but the newest ring - 1 have landed
+                    case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+                    case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+                    case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+                    default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+                }
+                uint32_t z[2][ZW];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) z[k] = ZEROS ? zero[k] : 0x08080808u;
-                if (chunk + 1 < chunks) load_zeros(unit, chunk + 1);
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int j = 0; j < ZW; ++j) z[k][j] = ZEROS ? zero[k][j] : 0x08080808u;
+                if (block + 1 < blocks) load_zeros(unit, block + 1);
                 else load_zeros(unit + 1, 0);
-                const int st = i % NA;
-                if (i >= NA) ok = wait(&a_empty[st], (i / NA - 1) & 1);
-                if (!ok) break;
-                uint4 held[4];  // read before anything is written, or each tile would wait for the one before
+                uint4 held[4];  // [tile][half]: read before anything is written, or each would wait for the one before
 #pragma unroll
                 for (int k = 0; k < 4; ++k) held[k] = few_lds128(ring + slot * kManyRingBytes + k * 512);
+                const int st = i % NS;
+                if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
+                if (!ok) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint4 c = held[k];
-                    const int tl = cw * 4 + k;
-                    const uint32_t to = smem_u32(sa) + st * kManyABytes + (tl >> 3) * (kManyABytes / 2) + (tl & 7) * 2048 + t * 128 + g * 16;
+                    const int tl = cw * 2 + (k >> 1);
+                    const uint32_t to = smem_u32(sa) + st * kManyABytes + (tl >> 3) * (kManyABytes / 2) + (tl & 7) * 4096 + (k & 1) * 1024 + t * 128 + g * 16;
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {  // runs of eight columns
                         uint32_t a[4], b[4];
                         few_codes(q ? c.z : c.x, a);
                         few_codes(q ? c.w : c.y, b);
                         // c 2^-17 2^15 - z / 4: exact
-                        const uint32_t zq = ZN == 2 ? z[k] >> (16 * q) : z[k];
+                        const int group = (2 * (k & 1) + q) / (4 / NG);
+                        const uint32_t zq = z[k >> 1][group >> 1] >> (16 * (group & 1));
                         auto quarter = [](uint32_t v) {
                             const __half2 h = __half2half2(__float2half_rn(-0.25f * (float)(v & 255u)));
                             return *reinterpret_cast<const uint32_t*>(&h);
@@ -317,76 +309,81 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                         constexpr uint32_t kUp = 0x78007800u;  // 2^15, twice
                         const uint32_t z0 = ZEROS ? quarter(zq) : 0xc000c000u, z1 = ZEROS ? quarter(zq >> 8) : 0xc000c000u;
                         many_sts128(to + q * 512, many_hfma2(a[0], kUp, z0), many_hfma2(a[2], kUp, z0), many_hfma2(b[0], kUp, z0), many_hfma2(b[2], kUp, z0));
-                        many_sts128(to + 1024 + q * 512, many_hfma2(a[1], kUp, z1), many_hfma2(a[3], kUp, z1), many_hfma2(b[1], kUp, z1), many_hfma2(b[3], kUp, z1));
+                        many_sts128(to + 2048 + q * 512, many_hfma2(a[1], kUp, z1), many_hfma2(a[3], kUp, z1), many_hfma2(b[1], kUp, z1), many_hfma2(b[3], kUp, z1));
                     }
                 }
                 fence_async_shared();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[st]);
-                slot = slot == kManyRing - 1 ? 0 : slot + 1;
+                if (lane == 0) mbar_arrive(&full[st]);
+                slot = slot == plan.ring - 1 ? 0 : slot + 1;
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (cs > 1) many_cluster_sync(), many_cluster_sync();
-    } else if (warp >= 12) {
+    } else if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsRest));
-        if (warp == 12) {
+        if (warp == 16) {
             // ---- products ----
+            // A wait costs the warp some 200 cycles and a commit 100, so a stage is a whole
+            // block, its operands share a barrier, and as many groups as fit make one D.
             const uint32_t idesc = tc_idesc_f16_f32(128, plan.n);
-            const uint64_t ad = tc_desc_kmajor(smem_u32(sa), 128, 1024), bd = tc_desc_kmajor(smem_u32(sb), 128, 1024);
-            // One elected thread issues all products of a chunk, or of a group where it is
-            // less, at once: the tensor cores then have the next while the warp waits.
-            constexpr int STEPS = GROUP / 16, RUN = STEPS < 4 ? STEPS : 4;  // products of a group, of a run
-            int i = 0, d = 0;  // stages and groups so far
-            for (int unit = u0; unit < u1 && ok; ++unit) {
-                for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i) {
-                    const int st = i % NA, sbt = i % NB;
-                    const bool begins = GROUP < 128 || (chunk & 1) == 0, ends = GROUP < 128 || (chunk & 1) == 1;
-                    const uint64_t a0 = ad + st * (kManyABytes / 16), b0 = bd + sbt * (kManyBBytes / 16);
+            const uint64_t ad = tc_desc_kmajor(smem_u32(sa), 128, 2048), bd = tc_desc_kmajor(smem_u32(sb), 128, 2048);
+            const uint32_t b_stage = plan.n * kManyK * 2 / 16;
+            constexpr int STEPS = GROUP / 16;  // products of a group
+            auto issue = [&](auto sets) {
+                constexpr int SETS = decltype(sets)::value, PER = NG / SETS, COLS = kManyCols / PER;  // groups of a D, columns of one
+                int i = 0, d = 0;  // stages and Ds so far
+                for (int n = (u1 - u0) * blocks; i < n && ok; ++i) {
+                    const int st = i % NS;
+                    const uint64_t a0 = ad + st * (kManyABytes / 16), b0 = bd + st * b_stage;
+                    ok = wait(&full[st], (i / NS) & 1);
 #pragma unroll
-                    for (int run = 0; run < 4 / RUN; ++run) {
-                        if (begins && d >= 2) ok = ok && wait(&d_free[d & 1], ((d >> 1) - 1) & 1);
-                        if (run == 0) ok = ok && wait(&b_full[sbt], (i / NB) & 1) && wait(&a_full[st], (i / NA) & 1);
+                    for (int set = 0; set < SETS; ++set, ++d) {
+                        if (ok && d >= 2) ok = wait(&d_free[d & 1], ((d >> 1) - 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t to = tmem + (d & 1) * 2 * kManyCols;
                         if (many_elect()) {
 #pragma unroll
-                            for (int k = run * RUN; k < (run + 1) * RUN; ++k) {
-                                const uint32_t more = !(begins && k == run * RUN);
-                                tc_mma_f16(to, a0 + k * 16, b0 + k * 16, idesc, more);
-                                tc_mma_f16(to + kManyCols, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, more);
+                            for (int k = set * PER * STEPS; k < (set + 1) * PER * STEPS; ++k) {
+                                const uint32_t at = to + (k / STEPS - set * PER) * 2 * COLS;
+                                tc_mma_f16(at, a0 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
+                                tc_mma_f16(at + COLS, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
                             }
-                            if (ends) tc_commit(&d_full[d & 1]);
-                            if (run == 4 / RUN - 1) tc_commit(&a_empty[st]), tc_commit(&b_empty[sbt]);
+                            tc_commit(&d_full[d & 1]);
+                            if (set == SETS - 1) tc_commit(&empty[st]);
                         }
                         __syncwarp();
-                        d += ends;
                     }
                 }
-            }
-        } else if (warp == 13) {
+            };
+            if (plan.sets == 1) issue(std::integral_constant<int, 1>());
+            else if (NG >= 2 && plan.sets == 2) issue(std::integral_constant<int, NG >= 2 ? 2 : 1>());
+            else issue(std::integral_constant<int, NG>());
+        } else if (warp == 17) {
             // ---- copies of x ----
             griddep_wait();
             const uint32_t bytes = plan.n * kManyK * 2;
             const uint64_t policy = l2_policy_evict_last();
             int i = 0;
             for (int unit = u0; unit < u1 && ok; ++unit) {
-                const uint8_t* from = plan.b + ((int64_t)(unit / plan.w_tiles) * 2 * w.blocks + 2 * block0) * bytes;
-                for (int chunk = 0; chunk < chunks && ok; ++chunk, ++i, from += bytes) {
-                    const int st = i % NB;
-                    if (i >= NB) ok = wait(&b_empty[st], (i / NB - 1) & 1);
+                const uint8_t* from = plan.b + ((int64_t)(unit / plan.w_tiles) * w.blocks + block0) * bytes;
+                for (int block = 0; block < blocks && ok; ++block, ++i, from += bytes) {
+                    const int st = i % NS;
+                    if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
                     if (!ok) break;
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&b_full[st], bytes);
-                        bulk_g2s(sb + st * kManyBBytes, from, bytes, &b_full[st], policy);
+                        mbar_arrive_expect_tx(&full[st], bytes);
+                        bulk_g2s(sb + st * bytes, from, bytes, &full[st], policy);
                     }
                     __syncwarp();
                 }
             }
-            // The last copies land before the CTA may end, also after a failure.
-            for (int k = i > NB ? i - NB : 0; k < i; ++k)
-                mbar_wait_bounded(&b_full[k % NB], (k / NB) & 1, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
+            // The last copies land before the CTA may end.  Their stages are full once the
+            // operand warps have come, too; after a failure these may not, and it takes
+            // the limit.
+            for (int k = i > NS ? i - NS : 0; k < i; ++k)
+                mbar_wait_bounded(&full[k % NS], (k / NS) & 1, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
         }
         __syncwarp();
         if (cs > 1) many_cluster_sync(), many_cluster_sync();
@@ -396,7 +393,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
         griddep_wait();
         constexpr int PAIRS = SPLIT ? kManyCols / 4 : kManyCols / 2;  // of rows of x
         const int row = warp * 32 + lane;   // of the unit
-        const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * kManyCols;
+        const int per = NG / plan.sets, columns = kManyCols / per;  // groups of a D, columns of one
+        const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * columns;
         int d = 0;
         for (int unit = u0; unit < u1; ++unit) {
             const int wt = unit % plan.w_tiles, xt = unit / plan.w_tiles;
@@ -426,33 +424,40 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 for (int k = 0; k < NG; ++k) scale[k] = row & 8 ? sc_next[k] >> 16 : sc_next[k] & 0xffffu;
                 if (block + 1 < block1) load_scales(block + 1);
 #pragma unroll
-                for (int k = 0; k < NG; ++k, ++d) {
-                    if (ok) ok = wait(&d_full[d & 1], (d >> 1) & 1);
+                for (int k = 0; k < NG; ++k) {
+                    const int in = k & (per - 1);
+                    if (in == 0 && ok) {
+                        ok = wait(&d_full[d & 1], (d >> 1) & 1);
+                        tc_fence_after();
+                    }
                     if (!ok) break;
-                    tc_fence_after();
+                    const uint32_t at = from + (d & 1) * 2 * kManyCols + in * 2 * columns;
                     const float s = __half2float(__ushort_as_half((uint16_t)scale[k]));
                     const uint64_t s2 = many_pair(s, s);
 #pragma unroll
-                    for (int c = 0; c < kManyCols / 32; ++c) {
-                        if (c * 32 >= plan.n) continue;
-                        uint32_t v[32];
-                        many_ld32(from + (d & 1) * 2 * kManyCols + c * 32, v);
-                        many_wait_ld(v);
+                    for (int c = 0; c < kManyCols / 16; ++c) {
+                        if (c * 16 >= plan.n) continue;
+                        uint32_t v[16];
+                        tmem_ld16(at + c * 16, v);
+                        tmem_wait_ld(v);
                         if (SPLIT) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
+                            for (int e = 0; e < 4; ++e) {
                                 const uint64_t both = many_add(many_pair(v[4 * e], v[4 * e + 1]), many_pair(v[4 * e + 2], v[4 * e + 3]));
-                                total[c * (PAIRS / 4) + e] = many_fma(s2, both, total[c * (PAIRS / 4) + e]);
+                                total[c * 4 + e] = many_fma(s2, both, total[c * 4 + e]);
                             }
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                total[c * (PAIRS / 4) + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[c * (PAIRS / 4) + e]);
+                            for (int e = 0; e < 8; ++e)
+                                total[c * 8 + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[c * 8 + e]);
                         }
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&d_free[d & 1]);
+                    if (in == per - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&d_free[d & 1]);
+                        ++d;
+                    }
                 }
             }
             // Rows of x from the unit's first on, this thread's element of each.
@@ -505,7 +510,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     }
     // Everyone meets when all products and their arrivals are done, also where
     // a wait has given up.
-    if (warp == 12) {
+    if (warp == 16) {
         if (many_elect()) tc_commit(&drained);
         mbar_wait_bounded(&drained, 0, &unset, globaltimer_ns() + timeout_ns, kDevTimeoutDrain);
         if (unset) atomicCAS(err, 0, kDevTimeoutDrain);
@@ -513,7 +518,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace lc

@@ -91,6 +91,12 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
     plan.w_tiles = (w.rows + kManyRows - 1) / kManyRows;
     plan.b = (const uint8_t*)ws;
     plan.factor = (const float*)((uint8_t*)ws + kLayBytes);
+    // Groups of a D share 128 columns of tensor memory for each 128 rows of W.
+    constexpr int NG = kW4Cols / GROUP;
+    const int fit = kManyCols / plan.n;
+    plan.sets = NG / (fit >= 4 && NG >= 4 ? 4 : fit >= 2 && NG >= 2 ? 2 : 1);
+    const int spare = (kManySmem - kManyStages * (kManyABytes + plan.n * kManyK * 2)) / (8 * kManyRingBytes);
+    plan.ring = spare < kManyMaxRing ? spare : kManyMaxRing;
     // CTAs of a unit: what its CTAs and the units that come after one another take, in
     // blocks; a unit's beginning and end cost about four.
     const int64_t units = (int64_t)plan.x_tiles * plan.w_tiles;
@@ -101,7 +107,7 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
     }
     for (plan.cluster_log2 = 0; 1 << plan.cluster_log2 < plan.cluster;) ++plan.cluster_log2;
     cudaError_t e = launch_ex(w4_lay_kernel<T>, dim3((unsigned)(plan.x_tiles * (plan.n / 8))), dim3(kLayThreads), 0, st, true, p, w.cols,
-                              2 * w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
+                              w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
     if (e != cudaSuccess) return e;
     auto* kernel = w4_many_kernel<T, GROUP, ZEROS>;
     // The register split draws on what the launch has: more than that would wait forever.
