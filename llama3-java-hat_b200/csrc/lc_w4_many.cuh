@@ -259,8 +259,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 for (int k = 0; k < 2; ++k) {
                     const uint8_t* z = w.zeros + (((int64_t)tile_of(unit, k) * w.blocks + block0 + block) * 8 + g) * NG * 2;
 #pragma unroll
-                    for (int i = 0; i < ZW; ++i)
-                        zero[k][i] = NG == 1 ? *reinterpret_cast<const uint16_t*>(z) : reinterpret_cast<const uint32_t*>(z)[i];
+                    for (int i = 0; i < ZW; ++i) {
+                        if constexpr (NG == 1) {
+                            uint16_t v;
+                            asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(z));
+                            zero[k][i] = v;
+                        } else {
+                            asm volatile("ld.global.u32 %0, [%1];" : "=r"(zero[k][i]) : "l"(z + 4 * i));
+                        }
+                    }
                 }
             }
         };
@@ -407,22 +414,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             uint32_t sc_next[NG];
             auto load_scales = [&](int block) {
                 const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + (((int64_t)tile * w.blocks + block) * 8 + (row & 7)) * NG;
-                if (NG == 4) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
-                    sc_next[0] = v.x, sc_next[NG > 1 ? 1 : 0] = v.y, sc_next[NG > 2 ? 2 : 0] = v.z, sc_next[NG > 2 ? 3 : 0] = v.w;
-                } else if (NG == 2) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-                    sc_next[0] = v.x, sc_next[NG > 1 ? 1 : 0] = v.y;
-                } else {
-                    sc_next[0] = __ldg(s);
-                }
+                // Volatile: a load that the compiler may move goes to its use.
+                if constexpr (NG == 4)
+                    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(sc_next[0]), "=r"(sc_next[1]), "=r"(sc_next[2]), "=r"(sc_next[3]) : "l"(s));
+                else if constexpr (NG == 2)
+                    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(sc_next[0]), "=r"(sc_next[1]) : "l"(s));
+                else
+                    asm volatile("ld.global.u32 %0, [%1];" : "=r"(sc_next[0]) : "l"(s));
             };
+            // They stream from HBM like the codes: asked for eight blocks ahead.
+            auto prefetch_scales = [&](int block) {
+                const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + (((int64_t)tile * w.blocks + block) * 8 + (row & 7)) * NG;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(s));
+            };
+            for (int block = block0 + 1; block < min(block0 + 8, block1); ++block) prefetch_scales(block);
             load_scales(block0);
             for (int block = block0; block < block1 && ok; ++block) {
                 uint32_t scale[NG];
 #pragma unroll
                 for (int k = 0; k < NG; ++k) scale[k] = row & 8 ? sc_next[k] >> 16 : sc_next[k] & 0xffffu;
                 if (block + 1 < block1) load_scales(block + 1);
+                if (block + 8 < block1) prefetch_scales(block + 8);
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     const int in = k & (per - 1);
@@ -461,22 +473,43 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 }
             }
             // Rows of x from the unit's first on, this thread's element of each.
-            const int b0 = xt * plan.rows, n = !ok || out >= w.rows ? 0 : min(plan.rows, p.batch - b0);
+            const int b0 = xt * plan.rows, n = min(plan.rows, p.batch - b0);
+            const bool mine = ok && out < w.rows;
             T* const y = (T*)p.y + b0 * p.y_stride + out;
             const T* const res = p.residual ? (const T*)p.residual + b0 * p.residual_stride + out : nullptr;
-            auto store = [&](int r, float v) {
-                if (r >= n) return;
-                v *= 4.0f;
-                if (SPLIT) v *= plan.factor[b0 + r];
-                if (res) v += (float)res[r * p.residual_stride];
-                y[r * p.y_stride] = (T)v;
+            float factor[2] = {4.0f, 4.0f};  // of rows lane and lane + 32
+            if (SPLIT) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) factor[i] = lane + 32 * i < n ? plan.factor[b0 + lane + 32 * i] : 0.0f;
+            }
+            // W values of rows r(0) .. r(W - 1): what is read comes before what is written.
+            auto store = [&](auto width, auto row_of, const float* v) {
+                constexpr int W = decltype(width)::value;
+                float add[W];
+                if (res) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) add[i] = mine && row_of(i) < n ? (float)res[row_of(i) * p.residual_stride] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int r = row_of(i);
+                    float u = v[i] * 4.0f;
+                    if (SPLIT) u *= __shfl_sync(0xffffffffu, r < 32 ? factor[0] : factor[1], r & 31);
+                    if (res) u += add[i];
+                    if (mine && r < n) y[r * p.y_stride] = (T)u;
+                }
             };
             if (cs == 1) {
 #pragma unroll
-                for (int k = 0; k < PAIRS; ++k) {
-                    const float2 v = many_two(total[k]);
-                    store(2 * k, v.x);
-                    store(2 * k + 1, v.y);
+                for (int k = 0; k < PAIRS; k += 4) {
+                    if (2 * k >= n) continue;
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 u = many_two(total[k + i]);
+                        v[2 * i] = u.x, v[2 * i + 1] = u.y;
+                    }
+                    store(std::integral_constant<int, 8>(), [&](int i) { return 2 * k + i; }, v);
                 }
             } else {
                 // Row r of x belongs to CTA (r / 2) % cs: [sender][r / 2 / cs][r % 2][256] in
@@ -495,15 +528,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + kManyRows * 4), "f"(v.y) : "memory");
                 }
                 many_cluster_sync();
-                const float* const mine = reinterpret_cast<const float*>(smem) + row;
-                for (int k = rank; 2 * k < plan.rows; k += cs) {
-                    float x = 0.0f, y = 0.0f;
+                const float* const sums = reinterpret_cast<const float*>(smem) + row;
+                for (int k = rank; 2 * k < n; k += 2 * cs) {  // two pairs at a time
+                    float v[4] = {};
                     for (int c = 0; c < cs; ++c) {
-                        x += mine[c * each + (k >> log2) * 2 * kManyRows];
-                        y += mine[c * each + (k >> log2) * 2 * kManyRows + kManyRows];
+                        const float* from = sums + c * each + (k >> log2) * 2 * kManyRows;
+                        v[0] += from[0], v[1] += from[kManyRows];
+                        if (2 * (k + cs) < n) v[2] += from[2 * kManyRows], v[3] += from[3 * kManyRows];
                     }
-                    store(2 * k, x);
-                    store(2 * k + 1, y);
+                    store(std::integral_constant<int, 4>(), [&](int i) { return 2 * (k + (i >> 1) * cs) + (i & 1); }, v);
                 }
             }
         }
