@@ -40,9 +40,13 @@ constexpr int kManyABytes = kManyRows * kManyK * 2, kManyBBytes = kManyCols * kM
 constexpr int kManyRingBytes = 2 * kW4BlockBytes;  // of a warp: a block of two tiles
 constexpr int kManySmem = 226 * 1024;
 constexpr int kManyMaxCluster = 8;
-// Registers after the split; their sum over the warpgroups is the launch's.
-constexpr int kManyRegsSum = 160, kManyRegsCodes = 56, kManyRegsRest = 48;
-constexpr int kManyRegsLaunch = (2 * kManyRegsSum + 2 * kManyRegsCodes + kManyRegsRest + 4) / 5;
+// Registers after the split; their sum over the five warpgroups is the launch's.
+// F16 rows in units of 128 columns have sums of 128 registers.
+template <bool BIG>
+struct ManyRegs {
+    static constexpr int kSum = BIG ? 168 : 152, kCodes = BIG ? 48 : 64, kRest = 48;
+    static constexpr int kLaunch = (2 * kSum + 2 * kCodes + kRest + 4) / 5;
+};
 
 struct ManyPlan {
     int n;         // columns of B of a unit (a multiple of 16)
@@ -164,6 +168,27 @@ LC_DEV uint64_t many_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
+LC_DEV void many_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+// The loads before it are done; the values pass through, so that no use moves up.
+LC_DEV void many_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                   "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                   "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
 LC_DEV bool many_elect() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
@@ -181,9 +206,11 @@ LC_DEV void many_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int GROUP, bool ZEROS>
+// COLS: columns of B of a unit at most, 64 or 128.
+template <typename T, int GROUP, bool ZEROS, int COLS>
 __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Product p, ManyPlan plan, int* err, uint64_t timeout_ns) {
     constexpr bool SPLIT = sizeof(T) == 4;
+    using R = ManyRegs<!SPLIT && COLS == 128>;
     constexpr int NG = kW4Cols / GROUP;
     constexpr int NS = kManyStages;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -226,7 +253,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
 
     if (warp >= 8 && warp < 16) {
         // ---- codes to operands ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsCodes));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kCodes));
         const int cw = warp - 8, g = lane & 7, t = lane >> 3;  // eight lanes write one core matrix
         const uint32_t ring = smem_u32(sc) + cw * plan.ring * kManyRingBytes + lane * 16;
         int a_unit = u0, a_block = 0;
@@ -328,7 +355,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (cs > 1) many_cluster_sync(), many_cluster_sync();
     } else if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyRegsRest));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kRest));
         if (warp == 16) {
             // ---- products ----
             // A wait costs the warp some 200 cycles and a commit 100, so a stage is a whole
@@ -338,7 +365,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             const uint32_t b_stage = plan.n * kManyK * 2 / 16;
             constexpr int STEPS = GROUP / 16;  // products of a group
             auto issue = [&](auto sets) {
-                constexpr int SETS = decltype(sets)::value, PER = NG / SETS, COLS = kManyCols / PER;  // groups of a D, columns of one
+                constexpr int SETS = decltype(sets)::value, PER = NG / SETS, WIDE = kManyCols / PER;  // groups of a D, columns of one
                 int i = 0, d = 0;  // stages and Ds so far
                 for (int n = (u1 - u0) * blocks; i < n && ok; ++i) {
                     const int st = i % NS;
@@ -353,9 +380,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                         if (many_elect()) {
 #pragma unroll
                             for (int k = set * PER * STEPS; k < (set + 1) * PER * STEPS; ++k) {
-                                const uint32_t at = to + (k / STEPS - set * PER) * 2 * COLS;
+                                const uint32_t at = to + (k / STEPS - set * PER) * 2 * WIDE;
                                 tc_mma_f16(at, a0 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
-                                tc_mma_f16(at + COLS, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
+                                tc_mma_f16(at + WIDE, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
                             }
                             tc_commit(&d_full[d & 1]);
                             if (set == SETS - 1) tc_commit(&empty[st]);
@@ -396,9 +423,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
         if (cs > 1) many_cluster_sync(), many_cluster_sync();
     } else {
         // ---- sums ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegsSum));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::kSum));
         griddep_wait();
-        constexpr int PAIRS = SPLIT ? kManyCols / 4 : kManyCols / 2;  // of rows of x
+        constexpr int PAIRS = SPLIT ? COLS / 4 : COLS / 2;  // of rows of x
         const int row = warp * 32 + lane;   // of the unit
         const int per = NG / plan.sets, columns = kManyCols / per;  // groups of a D, columns of one
         const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * columns;
@@ -435,40 +462,88 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 for (int k = 0; k < NG; ++k) scale[k] = row & 8 ? sc_next[k] >> 16 : sc_next[k] & 0xffffu;
                 if (block + 1 < block1) load_scales(block + 1);
                 if (block + 8 < block1) prefetch_scales(block + 8);
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
+                // A load from tensor memory takes some 200 cycles whatever its size, so as much
+                // as registers hold is asked for at once: 64 columns, of one group or of two,
+                // or 32 where the sums take 128 registers.
+                auto take = [&](int k) {  // tensor memory of group k, when it is there
                     const int in = k & (per - 1);
                     if (in == 0 && ok) {
                         ok = wait(&d_full[d & 1], (d >> 1) & 1);
                         tc_fence_after();
                     }
-                    if (!ok) break;
-                    const uint32_t at = from + (d & 1) * 2 * kManyCols + in * 2 * columns;
+                    return from + (d & 1) * 2 * kManyCols + in * 2 * columns;
+                };
+                auto give = [&](int k) {
+                    if ((k & (per - 1)) != per - 1) return;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&d_free[d & 1]);
+                    ++d;
+                };
+                auto add = [&](int k, auto piece, const uint32_t (&v)[32]) {  // 32 columns
+                    constexpr int C = decltype(piece)::value;
                     const float s = __half2float(__ushort_as_half((uint16_t)scale[k]));
                     const uint64_t s2 = many_pair(s, s);
+                    if (SPLIT) {
 #pragma unroll
-                    for (int c = 0; c < kManyCols / 16; ++c) {
-                        if (c * 16 >= plan.n) continue;
-                        uint32_t v[16];
-                        tmem_ld16(at + c * 16, v);
-                        tmem_wait_ld(v);
-                        if (SPLIT) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint64_t both = many_add(many_pair(v[4 * e], v[4 * e + 1]), many_pair(v[4 * e + 2], v[4 * e + 3]));
-                                total[c * 4 + e] = many_fma(s2, both, total[c * 4 + e]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                total[c * 8 + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[c * 8 + e]);
+                        for (int e = 0; e < 8; ++e) {
+                            const uint64_t both = many_add(many_pair(v[4 * e], v[4 * e + 1]), many_pair(v[4 * e + 2], v[4 * e + 3]));
+                            total[C * 8 + e] = many_fma(s2, both, total[C * 8 + e]);
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            total[C * 16 + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[C * 16 + e]);
                     }
-                    if (in == per - 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&d_free[d & 1]);
-                        ++d;
+                };
+                using P0 = std::integral_constant<int, 0>;
+                using P1 = std::integral_constant<int, 1>;
+                if (COLS == 64 && NG > 1 && plan.n <= 32) {  // two groups, of one D
+#pragma unroll
+                    for (int k = 0; k < NG; k += 2) {
+                        const uint32_t at = take(k);
+                        if (!ok) break;
+                        uint32_t v[32], u[32];
+                        many_ld32(at, v);
+                        many_ld32(at + 2 * columns, u);
+                        many_wait_ld(v);
+                        many_wait_ld(u);
+                        add(k, P0(), v);
+                        if (NG > 1) add(k + (NG > 1), P0(), u);
+                        give(k + 1);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) {
+                        const uint32_t at = take(k);
+                        if (!ok) break;
+                        auto pieces = [&](auto c) {
+                            constexpr int C = decltype(c)::value;
+                            using Next = std::integral_constant<int, (C + 1) * 32 < COLS ? C + 1 : 0>;
+                            uint32_t v[32];
+                            many_ld32(at + C * 32, v);
+                            if (COLS == 64 || SPLIT) {
+                                uint32_t u[32];
+                                many_ld32(at + Next::value * 32, u);
+                                many_wait_ld(v);
+                                many_wait_ld(u);
+                                add(k, c, v);
+                                add(k, Next(), u);
+                            } else {
+                                many_wait_ld(v);
+                                add(k, c, v);
+                                if (Next::value * 32 < plan.n) {
+                                    many_ld32(at + Next::value * 32, v);
+                                    many_wait_ld(v);
+                                    add(k, Next(), v);
+                                }
+                            }
+                        };
+                        pieces(P0());
+                        if constexpr (COLS == 128) {
+                            if (plan.n > 64) pieces(std::integral_constant<int, 2>());
+                        }
+                        give(k);
                     }
                 }
             }

@@ -109,12 +109,12 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
     cudaError_t e = launch_ex(w4_lay_kernel<T>, dim3((unsigned)(plan.x_tiles * (plan.n / 8))), dim3(kLayThreads), 0, st, true, p, w.cols,
                               w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
     if (e != cudaSuccess) return e;
-    auto* kernel = w4_many_kernel<T, GROUP, ZEROS>;
+    auto* kernel = plan.n <= 64 ? w4_many_kernel<T, GROUP, ZEROS, 64> : w4_many_kernel<T, GROUP, ZEROS, 128>;
     // The register split draws on what the launch has: more than that would wait forever.
     cudaFuncAttributes attr;
     e = cudaFuncGetAttributes(&attr, kernel);
     if (e != cudaSuccess) return e;
-    if (attr.numRegs < kManyRegsLaunch) return cudaErrorInvalidKernelImage;
+    if (attr.numRegs < ManyRegs<true>::kLaunch || attr.numRegs < ManyRegs<false>::kLaunch) return cudaErrorInvalidKernelImage;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
