@@ -4,16 +4,17 @@
 // Two kernels.  The first lays the rows of x out as f16 operands in the context's
 // workspace: F16 rows as they are, F32 rows as hi + lo under a power-of-two row
 // scale (2^-22), rows and columns that are not there as zeros.  The second has
-// units of 256 rows of W and up to 128 columns (rows of x; hi and lo count each),
-//   D = A B   M 128 (twice), N up to 128, K one group
-// with A = (c - z) / 4, exact in f16, made from the codes in shared memory.  A
-// group's D is added, under the group's scale, to fp32 sums that an epilogue thread
+// units of 256 rows of W and up to 128 rows of x (F32: 64),
+//   D = A B   M 128 (twice), N up to 128, K one group (F32: A Bhi + A Blo)
+// with A = (c - z) / 4, exact in f16, made from the codes.  A group's D is added, under the group's scale, to fp32 sums that an epilogue thread
 // keeps in registers for its row of W, while the tensor cores fill the other D: so
 // scales need no rounding into weights, and the tensor cores' own truncating sums
 // run over 128 columns at most.
 //
-// What bounds it: the products, as long as a group has more columns than the
-// epilogue takes instructions for (one packed FMA for two elements of D).
+// What bounds it: shared memory, while A lies there (units of more than 64 rows of
+// x, whose Ds fill tensor memory): the products of a block of 128 columns read 128
+// KB of it and the rest moves as much again, 2048 cycles where the tensor cores
+// need 1024.  Up to 64 rows A is in tensor memory, a thread writing its row.
 //
 // Warps 0-7: epilogue, four for each 128 rows.  Warps 8-15: codes to operands,
 // through rings of their own (cp.async).  Warp 16 issues the products, warp 17 the
@@ -33,54 +34,49 @@ namespace lc {
 
 constexpr int kManyThreads = 20 * 32;
 constexpr int kManyRows = 256;      // of W, of a unit
-constexpr int kManyCols = 128;      // of B, at most
+constexpr int kManyCols = 128;      // of D, for 128 rows of W
+constexpr int many_most(bool split) { return split ? 64 : 128; }  // rows of x of a unit, at most
 constexpr int kManyK = kW4Cols;     // columns of W of a stage: a block
-constexpr int kManyStages = 2, kManyMaxRing = 5;
-constexpr int kManyABytes = kManyRows * kManyK * 2, kManyBBytes = kManyCols * kManyK * 2;
+constexpr int kManyStages = 2, kManyMaxRing = 5;  // stages of operands
+constexpr int kManyACol = 256;  // tensor memory: Ds below, and A where it lies there
+constexpr int kManyABytes = kManyRows * kManyK * 2;
 constexpr int kManyRingBytes = 2 * kW4BlockBytes;  // of a warp: a block of two tiles
 constexpr int kManySmem = 226 * 1024;
 constexpr int kManyMaxCluster = 8;
 // Registers after the split; their sum over the five warpgroups is the launch's.
-// F16 rows in units of 128 columns have sums of 128 registers.
+// Units of 128 rows of x have sums of 128 registers.
 template <bool BIG>
 struct ManyRegs {
-    static constexpr int kSum = BIG ? 168 : 152, kCodes = BIG ? 48 : 64, kRest = 48;
+    static constexpr int kSum = BIG ? 168 : 136, kCodes = BIG ? 48 : 80, kRest = 48;
     static constexpr int kLaunch = (2 * kSum + 2 * kCodes + kRest + 4) / 5;
 };
 
 struct ManyPlan {
-    int n;         // columns of B of a unit (a multiple of 16)
-    int rows;      // rows of x of a unit
+    int n;         // rows of x of a unit, a multiple of 16
     int x_tiles, w_tiles;
     int cluster;   // CTAs that share the columns of W, a power of two
     int cluster_log2;
     int sets;      // groups of a block over groups of a D: those that fit 256 columns of tensor memory
     int ring;      // blocks of a warp's ring of codes
-    const uint8_t* b;      // [x tile][block][n / 8][16 octets][8][16 bytes]
+    const uint8_t* b;      // [x tile][block][hi, lo][n / 8][16 octets][8][16 bytes]
     const float* factor;   // [batch] what the rows of x were divided by
 };
 
-// Column of B that holds row r of a unit (hi); lo is two columns on.
-template <bool SPLIT>
-LC_DEV int many_column(int r) { return SPLIT ? 4 * (r >> 1) + (r & 1) : r; }
-
 constexpr int kLayThreads = 512;
 
-// A CTA lays out eight columns of B: eight F16 rows with two warps each, or four
-// F32 rows with four.
+// A CTA lays out eight rows, with two warps each.
 template <typename T>
 __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int cols, int blocks, ManyPlan plan, uint8_t* b, float* factor) {
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int R = SPLIT ? 4 : 8, PARTS = kLayThreads / 32 / R;  // rows of a CTA, warps of a row
+    constexpr int R = 8, PARTS = kLayThreads / 32 / R;  // rows of a CTA, warps of a row
     constexpr int HOLD = 4;  // octets of columns that a lane keeps at a time
     __shared__ float tops[kLayThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % PARTS;
     griddep_wait();
     griddep_launch();
     const int groups = plan.n / 8, tile = blockIdx.x / groups, group = blockIdx.x % groups;
-    // F32: columns 8 group .. + 7 are hi and lo of rows 4 group .. + 3.
-    const int r = group * R + warp / PARTS, row = tile * plan.rows + r;
-    const bool there = r < plan.rows && row < p.batch;
+    const int r = group * R + warp / PARTS, row = tile * plan.n + r;
+    const bool there = row < p.batch;
     const T* const x = (const T*)p.x + (there ? row * p.x_stride : 0);
     const bool vec = ((uintptr_t)p.x | (uintptr_t)(p.x_stride * sizeof(T))) % 16 == 0;
     const int octets = blocks * 16;
@@ -130,8 +126,8 @@ __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int co
         if (there && part == 0 && lane == 0) factor[row] = pow2f(-e);
         if (octets > STEP) load(0);
     }
-    const int n = many_column<SPLIT>(r);
-    uint8_t* const to = b + ((int64_t)tile * blocks * groups + (n >> 3)) * 2048 + (n & 7) * 16;
+    constexpr int HALVES = SPLIT ? 2 : 1;
+    uint8_t* const to = b + ((int64_t)tile * blocks * HALVES * groups + group) * 2048 + (r & 7) * 16;
     for (int base = 0; base < octets; base += STEP) {
         if (base) load(base);
 #pragma unroll
@@ -144,9 +140,9 @@ __global__ void __launch_bounds__(kLayThreads) w4_lay_kernel(W4Product p, int co
             }
             uint4 hi, lo;
             split_octet(v[h], hi, lo);
-            uint8_t* const at = to + (int64_t)(o >> 4) * groups * 2048 + (o & 15) * 128;
+            uint8_t* const at = to + (int64_t)(o >> 4) * HALVES * groups * 2048 + (o & 15) * 128;
             *reinterpret_cast<uint4*>(at) = hi;
-            if (SPLIT) *reinterpret_cast<uint4*>(at + 32) = lo;
+            if (SPLIT) *reinterpret_cast<uint4*>(at + groups * 2048) = lo;
         }
     }
 }
@@ -161,11 +157,6 @@ LC_DEV float2 many_two(uint64_t v) { return make_float2(__uint_as_float((uint32_
 LC_DEV uint64_t many_fma(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t v;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
-LC_DEV uint64_t many_add(uint64_t a, uint64_t b) {
-    uint64_t v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
 LC_DEV void many_ld32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -189,6 +180,24 @@ LC_DEV void many_wait_ld(uint32_t (&v)[32]) {
                  :
                  : "memory");
 }
+LC_DEV void many_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+        "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+        "r"(v[31])
+        : "memory");
+}
+LC_DEV void many_mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 LC_DEV bool many_elect() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
@@ -206,17 +215,21 @@ LC_DEV void many_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// COLS: columns of B of a unit at most, 64 or 128.
+// COLS: rows of x of a unit at most, 64 or 128.
 template <typename T, int GROUP, bool ZEROS, int COLS>
 __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Product p, ManyPlan plan, int* err, uint64_t timeout_ns) {
     constexpr bool SPLIT = sizeof(T) == 4;
-    using R = ManyRegs<!SPLIT && COLS == 128>;
+    static_assert(COLS <= many_most(SPLIT), "");
+    using R = ManyRegs<COLS == 128>;
+    constexpr bool TA = COLS == 64;                // A in tensor memory
+    constexpr int DCOLS = TA ? 64 : kManyCols;     // columns of a D for 128 rows of W
     constexpr int NG = kW4Cols / GROUP;
-    constexpr int NS = kManyStages;
+    constexpr int NS = kManyStages, HALVES = SPLIT ? 2 : 1;
+    const uint32_t b_bytes = HALVES * plan.n * kManyK * 2;  // of a stage
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const sa = smem;                            // [stages][tile of 128 rows][row groups][octets][8][16]
-    uint8_t* const sb = sa + NS * kManyABytes;           // [stages][column groups][octets][8][16]
-    uint8_t* const sc = sb + NS * plan.n * kManyK * 2;   // [warps][ring][tile][half][lane][16]
+    uint8_t* const sb = sa + (TA ? 0 : NS * kManyABytes);           // [stages][hi, lo][column groups][octets][8][16]
+    uint8_t* const sc = sb + NS * b_bytes;               // [warps][ring][tile][half][lane][16]
     __shared__ __align__(8) uint64_t full[NS], empty[NS], d_full[2], d_free[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int unset;  // an error word of its own for the drain, which waits also after a failure
@@ -254,8 +267,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     if (warp >= 8 && warp < 16) {
         // ---- codes to operands ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::kCodes));
-        const int cw = warp - 8, g = lane & 7, t = lane >> 3;  // eight lanes write one core matrix
-        const uint32_t ring = smem_u32(sc) + cw * plan.ring * kManyRingBytes + lane * 16;
+        // Operands in shared memory: lane 8 t + g has rows g and g + 8 of a tile, so that
+        // eight lanes write one core matrix; in tensor memory: lane 16 k + r has row r of
+        // the warp's tile k.
+        const int cw = warp - 8, g = lane & 7, t = lane >> 3;
+        const uint32_t ring0 = smem_u32(sc) + cw * plan.ring * kManyRingBytes;
+        // Where the lane puts the 16 bytes that it copies of a chunk, those of lane 4 g + t
+        // of the layout.  For tensor memory rows are read by the lane, four times 16 bytes
+        // next to each other: turned by g / 2, eight rows then lie in all banks.
+        const uint32_t ring = ring0 + (TA ? 4 * g + ((t + (g >> 1)) & 3) : lane) * 16;
         int a_unit = u0, a_block = 0;
         auto tile_of = [&](int unit, int k) { return min((unit % plan.w_tiles) * (kManyRows / kW4Rows) + cw * 2 + k, w.tiles - 1); };
         const uint8_t* a_from[2];
@@ -276,15 +296,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        // Zero points of the lane's rows: pairs (rows g, g + 8) of a block's groups.
-        constexpr int ZW = (NG + 1) / 2;  // words
-        uint32_t zero[2][ZW];
+        // Zero points of the lane's rows: pairs (rows g, g + 8) of a block's groups, of
+        // both tiles or of the lane's.
+        constexpr int ZW = (NG + 1) / 2, ZT = TA ? 1 : 2;  // words, tiles
+        uint32_t zero[ZT][ZW];
         auto load_zeros = [&](int unit, int block) {
             if constexpr (ZEROS) {
                 if (unit >= u1) return;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint8_t* z = w.zeros + (((int64_t)tile_of(unit, k) * w.blocks + block0 + block) * 8 + g) * NG * 2;
+                for (int k = 0; k < ZT; ++k) {
+                    const uint8_t* z = w.zeros + (((int64_t)tile_of(unit, TA ? lane >> 4 : k) * w.blocks + block0 + block) * 8 + g) * NG * 2;
 #pragma unroll
                     for (int i = 0; i < ZW; ++i) {
                         if constexpr (NG == 1) {
@@ -298,6 +319,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 }
             }
         };
+        auto quarter = [](uint32_t v) {  // -z / 4, twice
+            const __half2 h = __half2half2(__float2half_rn(-0.25f * (float)(v & 255u)));
+            return *reinterpret_cast<const uint32_t*>(&h);
+        };
+        constexpr uint32_t kUp = 0x78007800u;  // 2^15, twice: c 2^-17 2^15 - z / 4 is exact
         for (int i = 0; i < plan.ring - 1; ++i) request(i);
         load_zeros(u0, 0);
         int i = 0, slot = 0;
@@ -310,44 +336,68 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                     case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
                     default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
                 }
-                uint32_t z[2][ZW];
+                uint32_t z[ZT][ZW];
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < ZT; ++k)
 #pragma unroll
                     for (int j = 0; j < ZW; ++j) z[k][j] = ZEROS ? zero[k][j] : 0x08080808u;
                 if (block + 1 < blocks) load_zeros(unit, block + 1);
                 else load_zeros(unit + 1, 0);
-                uint4 held[4];  // [tile][half]: read before anything is written, or each would wait for the one before
-#pragma unroll
-                for (int k = 0; k < 4; ++k) held[k] = few_lds128(ring + slot * kManyRingBytes + k * 512);
                 const int st = i % NS;
-                if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
-                if (!ok) break;
+                if constexpr (TA) {
+                    __syncwarp();  // the copies of all lanes have landed
+                    if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
+                    if (!ok) break;
+                    const uint32_t held = ring0 + slot * kManyRingBytes + (lane >> 4) * 1024 + g * 64;
+                    const int up = (lane >> 1) & 4;  // 4: rows g + 8, whose codes are 4 bits higher
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint4 c = held[k];
-                    const int tl = cw * 2 + (k >> 1);
-                    const uint32_t to = smem_u32(sa) + st * kManyABytes + (tl >> 3) * (kManyABytes / 2) + (tl & 7) * 4096 + (k & 1) * 1024 + t * 128 + g * 16;
+                    for (int h = 0; h < 2; ++h) {  // 64 columns
+                        uint32_t v[32];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {  // runs of eight columns
-                        uint32_t a[4], b[4];
-                        few_codes(q ? c.z : c.x, a);
-                        few_codes(q ? c.w : c.y, b);
-                        // c 2^-17 2^15 - z / 4: exact
-                        const int group = (2 * (k & 1) + q) / (4 / NG);
-                        const uint32_t zq = z[k >> 1][group >> 1] >> (16 * (group & 1));
-                        auto quarter = [](uint32_t v) {
-                            const __half2 h = __half2half2(__float2half_rn(-0.25f * (float)(v & 255u)));
-                            return *reinterpret_cast<const uint32_t*>(&h);
-                        };
-                        constexpr uint32_t kUp = 0x78007800u;  // 2^15, twice
-                        const uint32_t z0 = ZEROS ? quarter(zq) : 0xc000c000u, z1 = ZEROS ? quarter(zq >> 8) : 0xc000c000u;
-                        many_sts128(to + q * 512, many_hfma2(a[0], kUp, z0), many_hfma2(a[2], kUp, z0), many_hfma2(b[0], kUp, z0), many_hfma2(b[2], kUp, z0));
-                        many_sts128(to + 2048 + q * 512, many_hfma2(a[1], kUp, z1), many_hfma2(a[3], kUp, z1), many_hfma2(b[1], kUp, z1), many_hfma2(b[3], kUp, z1));
+                        for (int e = 0; e < 4; ++e) {  // octets e and 4 + e
+                            const uint4 c = few_lds128(held + h * 512 + ((e + (g >> 1)) & 3) * 16);
+                            const uint32_t ws[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int group = (2 * h + (j >> 1)) / (4 / NG);
+                                const uint32_t zq = ZEROS ? quarter(z[0][group >> 1] >> (16 * (group & 1) + 2 * up)) : 0xc000c000u;
+                                const uint32_t lo = __funnelshift_l(ws[j], ws[j], 4 - up) & 0x07800780u;
+                                const uint32_t hi = __funnelshift_r(ws[j], ws[j], 4 + up) & 0x07800780u;
+                                v[16 * (j >> 1) + 4 * e + 2 * (j & 1)] = many_hfma2(lo, kUp, zq);
+                                v[16 * (j >> 1) + 4 * e + 2 * (j & 1) + 1] = many_hfma2(hi, kUp, zq);
+                            }
+                        }
+                        many_st32(tmem + ((uint32_t)(cw & 3) << 21) + kManyACol + (st * 2 + (cw >> 2)) * 64 + h * 32, v);
                     }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                } else {
+                    uint4 held[4];  // [tile][half]: read before anything is written, or each would wait for the one before
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) held[k] = few_lds128(ring + slot * kManyRingBytes + k * 512);
+                    if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
+                    if (!ok) break;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 c = held[k];
+                        const int tl = cw * 2 + (k >> 1);
+                        const uint32_t to = smem_u32(sa) + st * kManyABytes + (tl >> 3) * (kManyABytes / 2) + (tl & 7) * 4096 + (k & 1) * 1024 + t * 128 + g * 16;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {  // runs of eight columns
+                            uint32_t a[4], b[4];
+                            few_codes(q ? c.z : c.x, a);
+                            few_codes(q ? c.w : c.y, b);
+                            const int group = (2 * (k & 1) + q) / (4 / NG);
+                            const uint32_t zq = z[(k >> 1) % ZT][group >> 1] >> (16 * (group & 1));
+                            const uint32_t z0 = ZEROS ? quarter(zq) : 0xc000c000u, z1 = ZEROS ? quarter(zq >> 8) : 0xc000c000u;
+                            many_sts128(to + q * 512, many_hfma2(a[0], kUp, z0), many_hfma2(a[2], kUp, z0), many_hfma2(b[0], kUp, z0), many_hfma2(b[2], kUp, z0));
+                            many_sts128(to + 2048 + q * 512, many_hfma2(a[1], kUp, z1), many_hfma2(a[3], kUp, z1), many_hfma2(b[1], kUp, z1), many_hfma2(b[3], kUp, z1));
+                        }
+                    }
+                    fence_async_shared();
+                    __syncwarp();
                 }
-                fence_async_shared();
-                __syncwarp();
                 if (lane == 0) mbar_arrive(&full[st]);
                 slot = slot == plan.ring - 1 ? 0 : slot + 1;
             }
@@ -362,27 +412,36 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             // block, its operands share a barrier, and as many groups as fit make one D.
             const uint32_t idesc = tc_idesc_f16_f32(128, plan.n);
             const uint64_t ad = tc_desc_kmajor(smem_u32(sa), 128, 2048), bd = tc_desc_kmajor(smem_u32(sb), 128, 2048);
-            const uint32_t b_stage = plan.n * kManyK * 2 / 16;
+            const uint32_t b_half = plan.n * kManyK * 2 / 16;
             constexpr int STEPS = GROUP / 16;  // products of a group
             auto issue = [&](auto sets) {
-                constexpr int SETS = decltype(sets)::value, PER = NG / SETS, WIDE = kManyCols / PER;  // groups of a D, columns of one
+                constexpr int SETS = decltype(sets)::value, PER = NG / SETS, WIDE = DCOLS / PER;  // groups of a D, columns of one
                 int i = 0, d = 0;  // stages and Ds so far
                 for (int n = (u1 - u0) * blocks; i < n && ok; ++i) {
                     const int st = i % NS;
-                    const uint64_t a0 = ad + st * (kManyABytes / 16), b0 = bd + st * b_stage;
+                    const uint64_t a0 = ad + st * (kManyABytes / 16), b0 = bd + st * HALVES * b_half;
                     ok = wait(&full[st], (i / NS) & 1);
 #pragma unroll
                     for (int set = 0; set < SETS; ++set, ++d) {
                         if (ok && d >= 2) ok = wait(&d_free[d & 1], ((d >> 1) - 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t to = tmem + (d & 1) * 2 * kManyCols;
+                        const uint32_t to = tmem + (d & 1) * 2 * DCOLS, ta = tmem + kManyACol + st * 128;
                         if (many_elect()) {
 #pragma unroll
                             for (int k = set * PER * STEPS; k < (set + 1) * PER * STEPS; ++k) {
                                 const uint32_t at = to + (k / STEPS - set * PER) * 2 * WIDE;
-                                tc_mma_f16(at, a0 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
-                                tc_mma_f16(at + WIDE, a0 + kManyABytes / 32 + k * 16, b0 + k * 16, idesc, k % STEPS != 0);
+#pragma unroll
+                                for (int h = 0; h < HALVES; ++h) {
+                                    const uint64_t b = b0 + h * b_half + k * 16;
+                                    if (TA) {
+                                        many_mma_ta(at, ta + k * 8, b, idesc, k % STEPS != 0 || h);
+                                        many_mma_ta(at + WIDE, ta + 64 + k * 8, b, idesc, k % STEPS != 0 || h);
+                                    } else {
+                                        tc_mma_f16(at, a0 + k * 16, b, idesc, k % STEPS != 0 || h);
+                                        tc_mma_f16(at + WIDE, a0 + kManyABytes / 32 + k * 16, b, idesc, k % STEPS != 0 || h);
+                                    }
+                                }
                             }
                             tc_commit(&d_full[d & 1]);
                             if (set == SETS - 1) tc_commit(&empty[st]);
@@ -397,18 +456,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
         } else if (warp == 17) {
             // ---- copies of x ----
             griddep_wait();
-            const uint32_t bytes = plan.n * kManyK * 2;
             const uint64_t policy = l2_policy_evict_last();
             int i = 0;
             for (int unit = u0; unit < u1 && ok; ++unit) {
-                const uint8_t* from = plan.b + ((int64_t)(unit / plan.w_tiles) * w.blocks + block0) * bytes;
-                for (int block = 0; block < blocks && ok; ++block, ++i, from += bytes) {
+                const uint8_t* from = plan.b + ((int64_t)(unit / plan.w_tiles) * w.blocks + block0) * b_bytes;
+                for (int block = 0; block < blocks && ok; ++block, ++i, from += b_bytes) {
                     const int st = i % NS;
                     if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
                     if (!ok) break;
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&full[st], bytes);
-                        bulk_g2s(sb + st * bytes, from, bytes, &full[st], policy);
+                        mbar_arrive_expect_tx(&full[st], b_bytes);
+                        bulk_g2s(sb + st * b_bytes, from, b_bytes, &full[st], policy);
                     }
                     __syncwarp();
                 }
@@ -425,9 +483,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
         // ---- sums ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::kSum));
         griddep_wait();
-        constexpr int PAIRS = SPLIT ? COLS / 4 : COLS / 2;  // of rows of x
+        constexpr int PAIRS = COLS / 2;  // of rows of x
         const int row = warp * 32 + lane;   // of the unit
-        const int per = NG / plan.sets, columns = kManyCols / per;  // groups of a D, columns of one
+        const int per = NG / plan.sets, columns = DCOLS / per;  // groups of a D, columns of one
         const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * columns;
         int d = 0;
         for (int unit = u0; unit < u1; ++unit) {
@@ -471,7 +529,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                         ok = wait(&d_full[d & 1], (d >> 1) & 1);
                         tc_fence_after();
                     }
-                    return from + (d & 1) * 2 * kManyCols + in * 2 * columns;
+                    return from + (d & 1) * 2 * DCOLS + in * 2 * columns;
                 };
                 auto give = [&](int k) {
                     if ((k & (per - 1)) != per - 1) return;
@@ -484,17 +542,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                     constexpr int C = decltype(piece)::value;
                     const float s = __half2float(__ushort_as_half((uint16_t)scale[k]));
                     const uint64_t s2 = many_pair(s, s);
-                    if (SPLIT) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint64_t both = many_add(many_pair(v[4 * e], v[4 * e + 1]), many_pair(v[4 * e + 2], v[4 * e + 3]));
-                            total[C * 8 + e] = many_fma(s2, both, total[C * 8 + e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            total[C * 16 + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[C * 16 + e]);
-                    }
+                    for (int e = 0; e < 16; ++e)
+                        total[C * 16 + e] = many_fma(s2, many_pair(v[2 * e], v[2 * e + 1]), total[C * 16 + e]);
                 };
                 using P0 = std::integral_constant<int, 0>;
                 using P1 = std::integral_constant<int, 1>;
@@ -522,7 +572,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                             using Next = std::integral_constant<int, (C + 1) * 32 < COLS ? C + 1 : 0>;
                             uint32_t v[32];
                             many_ld32(at + C * 32, v);
-                            if (COLS == 64 || SPLIT) {
+                            if (COLS == 64) {
                                 uint32_t u[32];
                                 many_ld32(at + Next::value * 32, u);
                                 many_wait_ld(v);
@@ -548,7 +598,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 }
             }
             // Rows of x from the unit's first on, this thread's element of each.
-            const int b0 = xt * plan.rows, n = min(plan.rows, p.batch - b0);
+            const int b0 = xt * plan.n, n = min(plan.n, p.batch - b0);
             const bool mine = ok && out < w.rows;
             T* const y = (T*)p.y + b0 * p.y_stride + out;
             const T* const res = p.residual ? (const T*)p.residual + b0 * p.residual_stride + out : nullptr;
@@ -593,7 +643,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 const int log2 = plan.cluster_log2, each = ((PAIRS + cs - 1) >> log2) * 2 * kManyRows;  // floats of a sender
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) {
-                    if (2 * k >= plan.rows) continue;
+                    if (2 * k >= plan.n) continue;
                     const float2 v = many_two(total[k]);
                     uint32_t to;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"

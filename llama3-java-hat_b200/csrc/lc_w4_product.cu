@@ -75,27 +75,25 @@ cudaError_t few(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
 // not even one unit fits.
 constexpr size_t kLayBytes = 32u << 20, kFactorBytes = 1u << 20;
 int64_t many_rows(const W4& w, bool split) {
-    const int64_t columns = (int64_t)(kLayBytes / ((size_t)w.blocks * kW4Cols * 2)) / kManyCols * kManyCols;
-    const int64_t rows = columns / (split ? 2 : 1), most = kFactorBytes / 4;
-    return rows < most ? rows : most;
+    const int64_t unit = many_most(split), fit = (int64_t)(kLayBytes / ((size_t)w.blocks * kW4Cols * (split ? 4 : 2))) / unit * unit;
+    return fit < (int64_t)(kFactorBytes / 4) ? fit : (int64_t)(kFactorBytes / 4);
 }
 
 template <typename T, int GROUP, bool ZEROS>
 cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st) {
-    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    constexpr int MOST = many_most(sizeof(T) == 4), HALVES = sizeof(T) == 4 ? 2 : 1;
     ManyPlan plan;
-    const int columns = p.batch * PARTS;
-    plan.x_tiles = (columns + kManyCols - 1) / kManyCols;
-    plan.n = ((columns + plan.x_tiles - 1) / plan.x_tiles + 15) / 16 * 16;
-    plan.rows = plan.n / PARTS;
+    plan.x_tiles = (p.batch + MOST - 1) / MOST;
+    plan.n = ((p.batch + plan.x_tiles - 1) / plan.x_tiles + 15) / 16 * 16;
     plan.w_tiles = (w.rows + kManyRows - 1) / kManyRows;
     plan.b = (const uint8_t*)ws;
     plan.factor = (const float*)((uint8_t*)ws + kLayBytes);
-    // Groups of a D share 128 columns of tensor memory for each 128 rows of W.
+    // Groups of a D share 64 columns of tensor memory (128 where A is not there) for
+    // each 128 rows of W, 32 of them at least.
     constexpr int NG = kW4Cols / GROUP;
-    const int fit = kManyCols / plan.n;
-    plan.sets = NG / (fit >= 4 && NG >= 4 ? 4 : fit >= 2 && NG >= 2 ? 2 : 1);
-    const int spare = (kManySmem - kManyStages * (kManyABytes + plan.n * kManyK * 2)) / (8 * kManyRingBytes);
+    const bool big = plan.n > 64;
+    plan.sets = NG / (!big && plan.n <= 32 && NG >= 2 ? 2 : 1);
+    const int spare = (kManySmem - kManyStages * ((big ? kManyABytes : 0) + HALVES * plan.n * kManyK * 2)) / (8 * kManyRingBytes);
     plan.ring = spare < kManyMaxRing ? spare : kManyMaxRing;
     // CTAs of a unit: what its CTAs and the units that come after one another take, in
     // blocks; a unit's beginning and end cost about four.
@@ -109,7 +107,10 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
     cudaError_t e = launch_ex(w4_lay_kernel<T>, dim3((unsigned)(plan.x_tiles * (plan.n / 8))), dim3(kLayThreads), 0, st, true, p, w.cols,
                               w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
     if (e != cudaSuccess) return e;
-    auto* kernel = plan.n <= 64 ? w4_many_kernel<T, GROUP, ZEROS, 64> : w4_many_kernel<T, GROUP, ZEROS, 128>;
+    auto* kernel = w4_many_kernel<T, GROUP, ZEROS, 64>;
+    if constexpr (MOST > 64) {
+        if (big) kernel = w4_many_kernel<T, GROUP, ZEROS, MOST>;
+    }
     // The register split draws on what the launch has: more than that would wait forever.
     cudaFuncAttributes attr;
     e = cudaFuncGetAttributes(&attr, kernel);
