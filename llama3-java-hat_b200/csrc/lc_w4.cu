@@ -4,10 +4,12 @@
 // A warp has a block of 16 rows x 128 columns, a lane four runs of eight columns
 // of two rows, as the layout wants them; a group's largest value is then a
 // maximum over 4 lanes and 1, 2 or 4 of their runs.  With s the group's scale,
-// every code is the nearest to the exact quotient x / s, ties to even: x (1 / s)
-// is two units of the last place off at most, and only where that could change
-// the code (the remainder x - q s is near half a step) is the exact remainder
-// asked.
+// every code is the nearest to the exact quotient x / s, ties to even.  x times a
+// number below 1 / s and x times one above it lie on both sides of the quotient:
+// where they round to the same whole number, it is the code (two FMAs, which add
+// 1.5 * 2^23 and the zero point at once, so that the code is the sum's low bits; a
+// multiplication puts them in their place).  Only a run of eight that has others,
+// or a group of unusual scale, divides by the exact remainder.
 //
 // Bound by memory: values in once, codes out once, and the reverse.
 #include "lc_internal.h"
@@ -71,28 +73,73 @@ LC_DEV void quotients(const float (&x)[8], float s, float inv, float (&q)[8]) {
         if (fabsf(q[i]) < 16.0f) q[i] = settle(x[i], s, q[i]);
 }
 
-// The lane's columns col0 + 32 q + 8 t + i (element 8 q + i) of half a block, of
-// its rows g (a) and g + 8 (b): read by the lane itself where 16-byte loads may be
-// used, else row by row through shared memory, so that neighbours read neighbours.
+// Eight neighbouring values as they lie in memory.
+template <typename T>
+struct Run;
+template <>
+struct Run<float> {
+    float4 lo, hi;
+    LC_DEV float get(int i) const {
+        const float4& v = i < 4 ? lo : hi;
+        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+    }
+    LC_DEV void load(const float* p) { lo = __ldg(reinterpret_cast<const float4*>(p)), hi = __ldg(reinterpret_cast<const float4*>(p) + 1); }
+    LC_DEV void shared(const float* p) { lo = *reinterpret_cast<const float4*>(p), hi = *(reinterpret_cast<const float4*>(p) + 1); }
+    LC_DEV void none() { lo = hi = make_float4(0, 0, 0, 0); }
+    // Largest size; not finite where a value is not.
+    LC_DEV float top() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(get(i))));
+        return m;
+    }
+    LC_DEV void range(float& low, float& high) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) low = fminf(low, get(i)), high = fmaxf(high, get(i));
+    }
+};
+template <>
+struct Run<__half> {
+    uint4 w;
+    LC_DEV __half2 two(int i) const {
+        const uint32_t v = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+        return *reinterpret_cast<const __half2*>(&v);
+    }
+    LC_DEV float get(int i) const { return i & 1 ? __high2float(two(i >> 1)) : __low2float(two(i >> 1)); }
+    LC_DEV void load(const __half* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+    LC_DEV void shared(const float* p) {
+        __half2 h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(p[2 * i], p[2 * i + 1]);  // exact
+        w = *reinterpret_cast<const uint4*>(h);
+    }
+    LC_DEV void none() { w = make_uint4(0, 0, 0, 0); }
+    LC_DEV float top() const {
+        const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(two(0)), __habs2(two(1))), __hmax2_nan(__habs2(two(2)), __habs2(two(3))));
+        const __half2 n = __hmax2_nan(m, __lowhigh2highlow(m));
+        return __low2float(n);
+    }
+    LC_DEV void range(float& low, float& high) const {
+        const __half2 n = __hmin2(__hmin2(two(0), two(1)), __hmin2(two(2), two(3))), m = __hmax2(__hmax2(two(0), two(1)), __hmax2(two(2), two(3)));
+        low = fminf(low, fminf(__low2float(n), __high2float(n)));
+        high = fmaxf(high, fmaxf(__low2float(m), __high2float(m)));
+    }
+};
+
+// The lane's runs of half a block: columns col0 + 32 q + 8 t and on, of its rows g
+// (a) and g + 8 (b): read by the lane itself where 16-byte loads may be used, else
+// row by row through shared memory, so that neighbours read neighbours.
 template <typename T>
 LC_DEV void load_half(const T* p, int64_t stride, int row0, int rows, int col0, int cols, bool vec, float* buf, int lane,
-                      float (&a)[16], float (&b)[16]) {
+                      Run<T> (&a)[2], Run<T> (&b)[2]) {
     const int g = lane >> 2, t = lane & 3;
     if (vec && col0 + kW4Half <= cols) {
-        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            float(&o)[16] = half ? b : a;
-            const int r = row0 + g + 8 * half;
-#pragma unroll
-            for (int i = 0; i < 16 / V; ++i) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                constexpr int R = 8 / V;  // loads of a run
-                if (r < rows) w = __ldg(reinterpret_cast<const uint4*>(p + r * stride + col0 + 32 * (i / R) + 8 * t) + i % R);
-                const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-                for (int k = 0; k < V; ++k) o[i * V + k] = to_f32<T>(e[k]);
-            }
+        for (int q = 0; q < 2; ++q) {
+            const T* from = p + (row0 + g) * stride + col0 + 32 * q + 8 * t;
+            a[q].none(), b[q].none();
+            if (row0 + g < rows) a[q].load(from);
+            if (row0 + g + 8 < rows) b[q].load(from + 8 * stride);
         }
         return;
     }
@@ -107,12 +154,9 @@ LC_DEV void load_half(const T* p, int64_t stride, int row0, int rows, int col0, 
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = 32 * (i >> 1) + 8 * t + 4 * (i & 1);
-        const float4 u = *reinterpret_cast<const float4*>(buf + g * kW4Pitch + at);
-        const float4 v = *reinterpret_cast<const float4*>(buf + (g + 8) * kW4Pitch + at);
-        a[4 * i] = u.x, a[4 * i + 1] = u.y, a[4 * i + 2] = u.z, a[4 * i + 3] = u.w;
-        b[4 * i] = v.x, b[4 * i + 1] = v.y, b[4 * i + 2] = v.z, b[4 * i + 3] = v.w;
+    for (int q = 0; q < 2; ++q) {
+        a[q].shared(buf + g * kW4Pitch + 32 * q + 8 * t);
+        b[q].shared(buf + (g + 8) * kW4Pitch + 32 * q + 8 * t);
     }
 }
 
@@ -140,84 +184,113 @@ LC_DEV Step step_of(float low, float high) {
     return o;
 }
 
+// Codes of a run under a group's scale: eight nibbles, that of value i at bit 4 i.
+template <typename T, bool ZEROS>
+LC_DEV void encode(const Run<T>& run, const Step& st, bool usual, float below, float above, uint32_t (&code)[8]) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+    const float base = kMagic + st.zero, end = kMagic + 15.0f;
+    bool sure = usual;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = run.get(i);
+        float m = __fmaf_rn(x, below, base);
+        sure = sure && m == __fmaf_rn(x, above, base);
+        if (ZEROS) m = fminf(m, end);
+        code[i] = __float_as_uint(m) - 0x4b400000u;
+    }
+    if (sure) return;
+    float v[8], q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i] = run.get(i), q[i] = 0.0f;
+        if (!(v[i] == v[i])) v[i] = 0.0f;
+    }
+    if (st.s > 0.0f) quotients(v, st.s, __frcp_rn(st.s), q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        code[i] = (uint32_t)(ZEROS ? fminf(fmaxf(q[i] + st.zero, 0.0f), 15.0f) : fminf(fmaxf(q[i], -7.0f), 7.0f) + 8.0f);
+}
+
 template <typename T, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4Threads) w4_quantize_kernel(W4 w, const T* __restrict__ values, int64_t stride, bool vec) {
     __shared__ __align__(16) float buf[kW4Warps][kW4Rows * kW4Pitch];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    constexpr int NG = kW4Cols / GROUP;  // groups of a block
+    constexpr int NG = kW4Cols / GROUP;           // groups of a block
+    constexpr int HALVES = GROUP == 128 ? 2 : 1;  // of a block, taken together
+    constexpr int GROUPS = HALVES * kW4Half / GROUP > 0 ? HALVES * kW4Half / GROUP : 1, RUNS = GROUP / 32;  // groups in them, runs of a group
     const int64_t units = (int64_t)w.tiles * w.blocks;
     for (int64_t u = (int64_t)blockIdx.x * kW4Warps + warp; u < units; u += (int64_t)gridDim.x * kW4Warps) {
         const int tile = (int)(u / w.blocks), block = (int)(u - (int64_t)tile * w.blocks);
-        float x[2][2][16];               // [half][row g or g + 8]
-        float low[2][4], high[2][4];     // [row][group of 32 columns]
+#pragma unroll 1
+        for (int h0 = 0; h0 < 2; h0 += HALVES) {
+            Run<T> x[2][2 * HALVES];  // [row g or g + 8][run of 32 columns]
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            load_half<T>(values, stride, tile * kW4Rows, w.rows, block * kW4Cols + h * kW4Half, w.cols, vec, buf[warp], lane, x[h][0], x[h][1]);
+            for (int h = 0; h < HALVES; ++h) {
+                Run<T> a[2], b[2];
+                load_half<T>(values, stride, tile * kW4Rows, w.rows, block * kW4Cols + (h0 + h) * kW4Half, w.cols, vec, buf[warp], lane, a, b);
+                x[0][2 * h] = a[0], x[0][2 * h + 1] = a[1], x[1][2 * h] = b[0], x[1][2 * h + 1] = b[1];
+            }
+            uint32_t word[4 * HALVES] = {};
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int i = 0; i < GROUPS; ++i) {
+                uint32_t bits[2], zeros[2];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    float lo = 0.0f, hi = 0.0f;
+                for (int k = 0; k < 2; ++k) {
+                    float top = 0.0f, low = 0.0f, high = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float& v = x[h][k][8 * q + i];
-                        if (!(v == v)) v = 0.0f;
-                        if (fabsf(v) < INFINITY) lo = fminf(lo, v), hi = fmaxf(hi, v);
+                    for (int r = 0; r < RUNS; ++r) {
+                        const float m = x[k][i * RUNS + r].top();
+                        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(m));
+                        if (ZEROS) x[k][i * RUNS + r].range(low, high);
                     }
-                    low[k][2 * h + q] = lo, high[k][2 * h + q] = hi;
-                }
-            }
-        }
-        Step step[2][NG];
+                    bool finite = top < INFINITY;
+                    if (!finite) {  // what is not finite does not count
+                        low = high = 0.0f;
+                        for (int r = 0; r < RUNS; ++r)
+                            for (int e = 0; e < 8; ++e) {
+                                const float v = x[k][i * RUNS + r].get(e);
+                                if (fabsf(v) < INFINITY) low = fminf(low, v), high = fmaxf(high, v);
+                            }
+                        top = fmaxf(-low, high);
+                    }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+                    for (int o = 1; o < 4; o <<= 1) {
+                        if (ZEROS) {
+                            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+                            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+                        } else {
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        }
+                    }
+                    const Step st = step_of<ZEROS>(ZEROS ? low : -top, ZEROS ? high : top);
+                    bits[k] = st.bits, zeros[k] = (uint32_t)st.zero;
+                    // Scales of at least 2^-14 (normal f16 numbers) that are not at the cap: no
+                    // quotient is then past the last code by more than the scale's rounding.
+                    const bool usual = finite && st.s >= 0x1p-14f && st.s < 65504.0f;
+                    const float inv = __frcp_rn(st.s), below = inv * (1.0f - 0x1p-22f), above = inv * (1.0f + 0x1p-22f);
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                float lo = low[k][i * (4 / NG)], hi = high[k][i * (4 / NG)];
-#pragma unroll
-                for (int q = 1; q < 4 / NG; ++q) lo = fminf(lo, low[k][i * (4 / NG) + q]), hi = fmaxf(hi, high[k][i * (4 / NG) + q]);
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                }
-                step[k][i] = step_of<ZEROS>(lo, hi);
-            }
-        }
-        uint4* out = reinterpret_cast<uint4*>(w.codes + u * kW4BlockBytes);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t word[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int run = 0; run < 2; ++run) {
-                    const Step& st = step[k][(2 * h + run) / (4 / NG)];
-                    float v[8], q[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = x[h][k][8 * run + i], q[i] = 0.0f;
-                    if (st.s > 0.0f) quotients(v, st.s, __frcp_rn(st.s), q);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float c = ZEROS ? fminf(fmaxf(q[i] + st.zero, 0.0f), 15.0f) : fminf(fmaxf(q[i], -7.0f), 7.0f) + 8.0f;
+                    for (int r = 0; r < RUNS; ++r) {
+                        uint32_t code[8];
+                        encode<T, ZEROS>(x[k][i * RUNS + r], st, usual, below, above, code);
                         constexpr int kBit[4] = {0, 16, 8, 24};
-                        const int col = block * kW4Cols + h * kW4Half + 32 * run + 8 * t + i;
-                        const uint32_t code = col < w.cols ? (uint32_t)c : 0u;
-                        word[2 * run + (i >> 2)] |= code << (kBit[i & 3] + 4 * k);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) word[2 * (i * RUNS + r) + (e >> 2)] += code[e] * (1u << (kBit[e & 3] + 4 * k));
                     }
                 }
+                const int group = h0 * (kW4Half / 32) / RUNS + i;
+                if (t == (i & 3)) {
+                    const bool there = block * kW4Cols + group * GROUP < w.cols;
+                    const int64_t at = (u * 8 + g) * NG + group;
+                    const uint32_t s0 = there && tile * kW4Rows + g < w.rows ? bits[0] : 0u;
+                    const uint32_t s1 = there && tile * kW4Rows + g + 8 < w.rows ? bits[1] : 0u;
+                    reinterpret_cast<uint32_t*>(w.scales)[at] = s0 | s1 << 16;
+                    if (ZEROS) reinterpret_cast<uint16_t*>(w.zeros)[at] = (uint16_t)(zeros[0] | zeros[1] << 8);
+                }
             }
-            out[h * 32 + lane] = make_uint4(turned(word[0]), turned(word[1]), turned(word[2]), turned(word[3]));
-        }
+            uint4* out = reinterpret_cast<uint4*>(w.codes + u * kW4BlockBytes) + h0 * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            if (t != i) continue;  // lane t writes the pair of group t
-            const bool there = block * kW4Cols + i * GROUP < w.cols;
-            const int64_t at = (u * 8 + g) * NG + i;
-            const uint32_t s0 = there && tile * kW4Rows + g < w.rows ? step[0][i].bits : 0u;
-            const uint32_t s1 = there && tile * kW4Rows + g + 8 < w.rows ? step[1][i].bits : 0u;
-            reinterpret_cast<uint32_t*>(w.scales)[at] = s0 | s1 << 16;
-            if (ZEROS) reinterpret_cast<uint16_t*>(w.zeros)[at] = (uint16_t)((uint32_t)step[0][i].zero | (uint32_t)step[1][i].zero << 8);
+            for (int h = 0; h < HALVES; ++h)
+                out[h * 32] = make_uint4(turned(word[4 * h]), turned(word[4 * h + 1]), turned(word[4 * h + 2]), turned(word[4 * h + 3]));
         }
     }
 }

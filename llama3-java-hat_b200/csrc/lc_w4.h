@@ -17,8 +17,9 @@
 // matter as long as both operands have the same.
 //
 // Scales (f16) and zero points (bytes) of a block: [8 g][128 / group][2], the
-// pair being rows g and g + 8.  Columns behind the last have code 0, rows
-// behind the last and groups without columns scale 0.
+// pair being rows g and g + 8.  Rows
+// behind the last and groups without columns have scale 0; what codes stand behind
+// the last column and row is of no consequence.
 #pragma once
 
 #include <cuda_runtime.h>
