@@ -27,10 +27,7 @@ namespace lc {
 
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
-#ifndef FD
-#define FD 3
-#endif
-constexpr int kFewDepth = FD;  // blocks of a warp's ring
+constexpr int kFewDepth = 3;  // blocks of a warp's ring
 constexpr int kFewMaxCluster = 8;
 constexpr int kFewPitch = 24;  // floats between columns of 16 partial sums: no bank conflicts
 

@@ -64,7 +64,8 @@ def test_quantize_and_read(L, acc, kind, zeros, group):
             x = weights(rng, rows, cols, kind)
             code, scale, zero = ref.quantize(x, group, zeros)
             w = L.Weights4.empty(rows, cols, group, zeros=zeros, acc=acc)
-            w.quantize(dev(x, pad))
+            v = dev(x, pad)  # kept until the call is done
+            w.quantize(v)
             for out, opad in (("f32", pad), ("f16", 0)):
                 back = dev(np.full((rows, cols), 7.0, ref.NP[out]), opad)
                 w.read(back)
@@ -105,7 +106,8 @@ def test_quantize_hard_values(L, acc, zeros):
         for group in (32, 128):
             code, scale, zero = ref.quantize(v, group, zeros)
             w = L.Weights4.empty(*v.shape, group, zeros=zeros, acc=acc)
-            w.quantize(dev(v))
+            dv = dev(v)
+            w.quantize(dv)
             back = dev(np.zeros(v.shape, np.float32))
             w.read(back)
             np.testing.assert_array_equal(host(acc, back), ref.values(code, scale, zero, group).astype(np.float32))
@@ -198,7 +200,8 @@ def test_product_bad_rows_stay_alone(L, acc, batch, kind):
     w = packed(L, acc, code, scale, zero, 64)
     x[1, 17], x[2, 200] = np.nan, np.inf
     y = dev(np.zeros((batch, 40), ref.NP[kind]))
-    w.apply(dev(x.astype(ref.NP[kind])), y)
+    dx = dev(x.astype(ref.NP[kind]))
+    w.apply(dx, y)
     got = host(acc, y).astype(np.float64)
     keep = [b for b in range(batch) if b not in (1, 2)]
     np.testing.assert_array_equal(got[keep], clean[keep])
@@ -214,7 +217,8 @@ def test_product_in_place_and_host(L, acc):
         want, terms, far = ref.product(x, code, scale, zero, 64, r)
         bound = ref.product_bound(want, terms, far, 4, "f32")
         y = dev(r)
-        w.apply(dev(x), y, residual=y)
+        dx = dev(x)
+        w.apply(dx, y, residual=y)
         assert np.all(np.abs(host(acc, y) - want) <= bound)
         y = r.copy()
         w.apply(x, y, residual=y)  # host memory
