@@ -190,22 +190,28 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
         for (int i = tid; i < (b1 - b0) * NG * ROWS; i += kFewThreads)
             if (i % ROWS >= p.batch) xsum[i] = 0.0f;
         for (int i = tid * 8; i < pitch; i += kFewThreads * 8) *reinterpret_cast<uint2*>(xcol + columns * pitch + i) = make_uint2(0, 0);
-        constexpr int HOLD = 2;  // blocks of a row that are read once
-        const int n = b1 - b0;
-        // Items (row, block): a warp takes the blocks warp, warp + 8, ... of every row.
+        const int n = b1 - b0;  // a warp has the blocks warp, warp + 8, ... of every row
+        // Four rows at a time: their loads are under way together.
+        constexpr int TOGETHER = 4;
         if (SPLIT) {
-            for (int r = 0; r < p.batch; ++r) {
-                float top = 0.0f;
-                for (int b = warp; b < n; b += HOLD * kFewWarps) {
-                    float u[HOLD][4] = {};
+            for (int r0 = 0; r0 < p.batch; r0 += TOGETHER) {
+                float top[TOGETHER] = {};
+                for (int b = warp; b < n; b += kFewWarps) {
+                    float u[TOGETHER][4];
 #pragma unroll
-                    for (int h = 0; h < HOLD; ++h)
-                        if (b + h * kFewWarps < n) four(r, b0 + b + h * kFewWarps, u[h]);
+                    for (int i = 0; i < TOGETHER; ++i)
+                        if (r0 + i < p.batch) four(r0 + i, b0 + b, u[i]);
 #pragma unroll
-                    for (int h = 0; h < HOLD; ++h) top = fmaxf(fmaxf(top, fmaxf(fabsf(u[h][0]), fabsf(u[h][1]))), fmaxf(fabsf(u[h][2]), fabsf(u[h][3])));
+                    for (int i = 0; i < TOGETHER; ++i)
+                        if (r0 + i < p.batch)
+                            top[i] = fmaxf(fmaxf(top[i], fmaxf(fabsf(u[i][0]), fabsf(u[i][1]))), fmaxf(fabsf(u[i][2]), fabsf(u[i][3])));
                 }
-                top = warp_max(top);
-                if (lane == 0) tops[warp * ROWS + r] = top;
+#pragma unroll
+                for (int i = 0; i < TOGETHER; ++i) {
+                    if (r0 + i >= p.batch) continue;
+                    const float m = warp_max(top[i]);
+                    if (lane == 0) tops[warp * ROWS + r0 + i] = m;
+                }
             }
             __syncthreads();
         }
@@ -219,33 +225,40 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
             factor[tid] = f;
         }
         if (SPLIT) __syncthreads();
-        for (int r = 0; r < p.batch; ++r) {
-            const float up = SPLIT ? 1.0f / factor[r] : 1.0f;  // a power of two
+        for (int r0 = 0; r0 < p.batch; r0 += TOGETHER) {
             for (int b = warp; b < n; b += kFewWarps) {
-                float f[4];
-                four(r, b0 + b, f);
-                uint32_t h[2], l[2];
-                float sum = 0.0f;
+                float f[TOGETHER][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float a = f[2 * i] * up, c = f[2 * i + 1] * up;
-                    const __half2 hh = __floats2half2_rn(a, c);
-                    const float2 hf = __half22float2(hh);
-                    h[i] = *reinterpret_cast<const uint32_t*>(&hh);
-                    sum += hf.x + hf.y;
-                    if (SPLIT) {
-                        const __half2 ll = __floats2half2_rn(a - hf.x, c - hf.y);
-                        const float2 lf = __half22float2(ll);
-                        l[i] = *reinterpret_cast<const uint32_t*>(&ll);
-                        sum += lf.x + lf.y;
+                for (int j = 0; j < TOGETHER; ++j)
+                    if (r0 + j < p.batch) four(r0 + j, b0 + b, f[j]);
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) {
+                    const int r = r0 + j;
+                    if (r >= p.batch) continue;
+                    const float up = SPLIT ? 1.0f / factor[r] : 1.0f;  // a power of two
+                    uint32_t h[2], l[2];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float a = f[j][2 * i] * up, c = f[j][2 * i + 1] * up;
+                        const __half2 hh = __floats2half2_rn(a, c);
+                        const float2 hf = __half22float2(hh);
+                        h[i] = *reinterpret_cast<const uint32_t*>(&hh);
+                        sum += hf.x + hf.y;
+                        if (SPLIT) {
+                            const __half2 ll = __floats2half2_rn(a - hf.x, c - hf.y);
+                            const float2 lf = __half22float2(ll);
+                            l[i] = *reinterpret_cast<const uint32_t*>(&ll);
+                            sum += lf.x + lf.y;
+                        }
                     }
-                }
-                uint8_t* const to = xcol + (SPLIT ? 2 * r : r) * pitch + b * 256 + lane * 8;
-                *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
-                if (SPLIT) *reinterpret_cast<uint2*>(to + pitch) = make_uint2(l[0], l[1]);
+                    uint8_t* const to = xcol + (SPLIT ? 2 * r : r) * pitch + b * 256 + lane * 8;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
+                    if (SPLIT) *reinterpret_cast<uint2*>(to + pitch) = make_uint2(l[0], l[1]);
 #pragma unroll
-                for (int o = 1; o < GROUP / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane % (GROUP / 4) == 0) xsum[(b * NG + lane / (GROUP / 4)) * ROWS + r] = sum * kSum;
+                    for (int o = 1; o < GROUP / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane % (GROUP / 4) == 0) xsum[(b * NG + lane / (GROUP / 4)) * ROWS + r] = sum * kSum;
+                }
             }
         }
         __syncthreads();

@@ -26,7 +26,8 @@ cudaError_t few_as(const W4& w, const W4Product& p, int num_sms, cudaStream_t st
         plan.cluster = cluster;
         plan.phases = phases;
         plan.blocks = (w.blocks + cluster * phases - 1) / (cluster * phases);
-        const int most = 2 * num_sms / cluster;
+        // Two CTAs per SM; of clusters an eighth less, for they do not fill a GPC.
+        const int most = cluster > 1 ? 2 * num_sms / cluster * 7 / 8 : 2 * num_sms;
         plan.clusters = pairs < most ? pairs : most;
         // Warps of a pair: few make few meetings, more make a CTA's pairs go round
         // evenly.  A meeting costs about as much as kMeet blocks.
