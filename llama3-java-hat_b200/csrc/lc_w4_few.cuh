@@ -191,27 +191,68 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
             if (i % ROWS >= p.batch) xsum[i] = 0.0f;
         for (int i = tid * 8; i < pitch; i += kFewThreads * 8) *reinterpret_cast<uint2*>(xcol + columns * pitch + i) = make_uint2(0, 0);
         const int n = b1 - b0;  // a warp has the blocks warp, warp + 8, ... of every row
-        // Four rows at a time: their loads are under way together.
+        auto largest = [&](float top, const float (&u)[4]) {
+            return fmaxf(fmaxf(top, fmaxf(fabsf(u[0]), fabsf(u[1]))), fmaxf(fabsf(u[2]), fabsf(u[3])));
+        };
+        auto put = [&](int r, int b, const float (&f)[4]) {
+            const float up = SPLIT ? 1.0f / factor[r] : 1.0f;  // a power of two
+            uint32_t h[2], l[2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float a = f[2 * i] * up, c = f[2 * i + 1] * up;
+                const __half2 hh = __floats2half2_rn(a, c);
+                const float2 hf = __half22float2(hh);
+                h[i] = *reinterpret_cast<const uint32_t*>(&hh);
+                sum += hf.x + hf.y;
+                if (SPLIT) {
+                    const __half2 ll = __floats2half2_rn(a - hf.x, c - hf.y);
+                    const float2 lf = __half22float2(ll);
+                    l[i] = *reinterpret_cast<const uint32_t*>(&ll);
+                    sum += lf.x + lf.y;
+                }
+            }
+            uint8_t* const to = xcol + (SPLIT ? 2 * r : r) * pitch + b * 256 + lane * 8;
+            *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
+            if (SPLIT) *reinterpret_cast<uint2*>(to + pitch) = make_uint2(l[0], l[1]);
+#pragma unroll
+            for (int o = 1; o < GROUP / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane % (GROUP / 4) == 0) xsum[(b * NG + lane / (GROUP / 4)) * ROWS + r] = sum * kSum;
+        };
+        // Several rows are taken four at a time, whose loads are then under way together
+        // (8 rows of 2048 x 8192: 17 against 14 us); one alone by two blocks.
         constexpr int TOGETHER = 4;
+        const bool rows = p.batch > 1;
         if (SPLIT) {
-            for (int r0 = 0; r0 < p.batch; r0 += TOGETHER) {
-                float top[TOGETHER] = {};
-                for (int b = warp; b < n; b += kFewWarps) {
-                    float u[TOGETHER][4];
+            if (rows) {
+                for (int r0 = 0; r0 < p.batch; r0 += TOGETHER) {
+                    float top[TOGETHER] = {};
+                    for (int b = warp; b < n; b += kFewWarps) {
+                        float u[TOGETHER][4];
 #pragma unroll
-                    for (int i = 0; i < TOGETHER; ++i)
-                        if (r0 + i < p.batch) four(r0 + i, b0 + b, u[i]);
+                        for (int i = 0; i < TOGETHER; ++i)
+                            if (r0 + i < p.batch) four(r0 + i, b0 + b, u[i]);
 #pragma unroll
-                    for (int i = 0; i < TOGETHER; ++i)
-                        if (r0 + i < p.batch)
-                            top[i] = fmaxf(fmaxf(top[i], fmaxf(fabsf(u[i][0]), fabsf(u[i][1]))), fmaxf(fabsf(u[i][2]), fabsf(u[i][3])));
+                        for (int i = 0; i < TOGETHER; ++i)
+                            if (r0 + i < p.batch) top[i] = largest(top[i], u[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TOGETHER; ++i) {
+                        if (r0 + i >= p.batch) continue;
+                        const float m = warp_max(top[i]);
+                        if (lane == 0) tops[warp * ROWS + r0 + i] = m;
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < TOGETHER; ++i) {
-                    if (r0 + i >= p.batch) continue;
-                    const float m = warp_max(top[i]);
-                    if (lane == 0) tops[warp * ROWS + r0 + i] = m;
+            } else {
+                float top = 0.0f;
+                for (int b = warp; b < n; b += 2 * kFewWarps) {
+                    float u[4], v[4] = {};
+                    four(0, b0 + b, u);
+                    if (b + kFewWarps < n) four(0, b0 + b + kFewWarps, v);
+                    top = largest(largest(top, u), v);
                 }
+                top = warp_max(top);
+                if (lane == 0) tops[warp * ROWS] = top;
             }
             __syncthreads();
         }
@@ -225,40 +266,23 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
             factor[tid] = f;
         }
         if (SPLIT) __syncthreads();
-        for (int r0 = 0; r0 < p.batch; r0 += TOGETHER) {
-            for (int b = warp; b < n; b += kFewWarps) {
-                float f[TOGETHER][4];
+        if (rows) {
+            for (int r0 = 0; r0 < p.batch; r0 += TOGETHER) {
+                for (int b = warp; b < n; b += kFewWarps) {
+                    float f[TOGETHER][4];
 #pragma unroll
-                for (int j = 0; j < TOGETHER; ++j)
-                    if (r0 + j < p.batch) four(r0 + j, b0 + b, f[j]);
+                    for (int j = 0; j < TOGETHER; ++j)
+                        if (r0 + j < p.batch) four(r0 + j, b0 + b, f[j]);
 #pragma unroll
-                for (int j = 0; j < TOGETHER; ++j) {
-                    const int r = r0 + j;
-                    if (r >= p.batch) continue;
-                    const float up = SPLIT ? 1.0f / factor[r] : 1.0f;  // a power of two
-                    uint32_t h[2], l[2];
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float a = f[j][2 * i] * up, c = f[j][2 * i + 1] * up;
-                        const __half2 hh = __floats2half2_rn(a, c);
-                        const float2 hf = __half22float2(hh);
-                        h[i] = *reinterpret_cast<const uint32_t*>(&hh);
-                        sum += hf.x + hf.y;
-                        if (SPLIT) {
-                            const __half2 ll = __floats2half2_rn(a - hf.x, c - hf.y);
-                            const float2 lf = __half22float2(ll);
-                            l[i] = *reinterpret_cast<const uint32_t*>(&ll);
-                            sum += lf.x + lf.y;
-                        }
-                    }
-                    uint8_t* const to = xcol + (SPLIT ? 2 * r : r) * pitch + b * 256 + lane * 8;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
-                    if (SPLIT) *reinterpret_cast<uint2*>(to + pitch) = make_uint2(l[0], l[1]);
-#pragma unroll
-                    for (int o = 1; o < GROUP / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (lane % (GROUP / 4) == 0) xsum[(b * NG + lane / (GROUP / 4)) * ROWS + r] = sum * kSum;
+                    for (int j = 0; j < TOGETHER; ++j)
+                        if (r0 + j < p.batch) put(r0 + j, b, f[j]);
                 }
+            }
+        } else {
+            for (int b = warp; b < n; b += kFewWarps) {
+                float f[4];
+                four(0, b0 + b, f);
+                put(0, b, f);
             }
         }
         __syncthreads();

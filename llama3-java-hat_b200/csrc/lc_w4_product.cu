@@ -39,11 +39,14 @@ cudaError_t few_as(const W4& w, const W4Product& p, int num_sms, cudaStream_t st
             if (!best || cost < best) best = cost, plan.split = split;
         }
     };
-    // More CTAs for the columns while a CTA's part would keep a second CTA off the
-    // SM, or while there are SMs without one and each warp has two blocks to share.
+    // More CTAs for the columns while there are SMs without one and each warp has a
+    // block, or while a CTA's part keeps a second CTA off the SMs that few rows leave
+    // idle (16 half rows of 128256 x 2048: with clusters of 2 109 us, without 86; 8
+    // rows of 2048 x 8192: 14 and 27).
     set(1, 1);
-    while (plan.cluster < kFewMaxCluster && w.blocks >= 2 * plan.cluster * kFewWarps &&
-           (S::smem(plan, p.batch) > kTwo || pairs * plan.cluster < num_sms))
+    while (plan.cluster < kFewMaxCluster &&
+           ((w.blocks >= plan.cluster * kFewWarps && pairs * plan.cluster < num_sms) ||
+            (w.blocks >= 2 * plan.cluster * kFewWarps && pairs * plan.cluster < 2 * num_sms && S::smem(plan, p.batch) > kTwo)))
         set(2 * plan.cluster, 1);
     while (S::smem(plan, p.batch) > kOne) set(plan.cluster, plan.phases + 1);
     auto* kernel = w4_few_kernel<T, GROUP, ZEROS, NT>;
