@@ -7,9 +7,6 @@
 #include "lc_w4_few.cuh"
 #include "lc_w4_many.cuh"
 
-#ifndef FEW_MEET
-#define FEW_MEET 2
-#endif
 namespace lc {
 namespace {
 
@@ -31,7 +28,7 @@ cudaError_t few_as(const W4& w, const W4Product& p, int num_sms, cudaStream_t st
         plan.clusters = pairs < most ? pairs : most;
         // Warps of a pair: few make few meetings, more make a CTA's pairs go round
         // evenly.  A meeting costs about as much as kMeet blocks.
-        constexpr int kMeet = FEW_MEET;
+        constexpr int kMeet = 2;
         const int mine = (pairs + plan.clusters - 1) / plan.clusters;
         int best = 0;
         for (int split = 1; split <= kFewWarps; split *= 2) {
@@ -167,8 +164,19 @@ cudaError_t product(const W4& w, const W4Product& p, int num_sms, void* ws, int*
 
 }  // namespace
 
+// Rows beyond one column tile of the kernel for few (4 F32 rows, 8 F16 rows) go
+// through the tensor cores of the other where matrices have the rows to keep all SMs
+// busy, and F16 rows of the smaller ones beyond 12.  us, few | many, groups of 128:
+//   128256 x 2048  5 F32 46 | 61, 8 F32 63 | 62, 9 F16 68 | 59, 16 F16 80 | 61
+//   16384 x 2048   5 F32 14 | 14, 8 F32 25 | 14, 9 F16 25 | 13, 16 F16 34 | 13
+//   2048 x 8192    5 F32 12 | 26, 8 F32 15 | 27, 9 F16 12 | 20, 16 F16 34 | 19
+//   2048 x 2048    5 F32  8 | 10, 8 F32  9 | 10, 9 F16  9 | 9,  16 F16 11 | 9
 bool w4_product_uses_ws(const W4& w, const W4Product& p) {
-    return p.batch > few_rows(p.dtype) && many_rows(w, p.dtype == kRowF32) > 0;
+    const bool f32 = p.dtype == kRowF32;
+    if (p.batch <= few_rows(p.dtype) / 2 || many_rows(w, f32) == 0) return false;
+    if (p.batch > (f32 ? 8 : 12)) return true;
+    const int pairs = (w.tiles + 1) / 2;
+    return !(pairs < 148 || (f32 && pairs >= 8 * 148));
 }
 size_t w4_product_ws_bytes() { return kLayBytes + kFactorBytes; }
 
