@@ -215,7 +215,8 @@ LC_DEV void many_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// COLS: rows of x of a unit at most, 64 or 128.
+// COLS: rows of x of a unit at most, 64 or 128 (without a residual, for which there
+// are no registers).
 template <typename T, int GROUP, bool ZEROS, int COLS>
 __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Product p, ManyPlan plan, int* err, uint64_t timeout_ns) {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -513,6 +514,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(s));
             };
             for (int block = block0 + 1; block < min(block0 + 8, block1); ++block) prefetch_scales(block);
+            if (COLS == 64 && p.residual && (cs == 1 || rank == 0)) {  // to L2, while the sums are made
+                constexpr int LINES = kManyRows * sizeof(T) / 128 + 1;
+                const int64_t c0 = (int64_t)wt * kManyRows, wide = min((int64_t)kManyRows, w.rows - c0);
+                for (int i = row; i < min(plan.n, p.batch - xt * plan.n) * LINES; i += kManyRows) {
+                    const int64_t at = min((int64_t)(i % LINES) * (128 / (int)sizeof(T)), wide - 1);
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"((const T*)p.residual + (xt * plan.n + i / LINES) * p.residual_stride + c0 + at));
+                }
+            }
             load_scales(block0);
             for (int block = block0; block < block1 && ok; ++block) {
                 uint32_t scale[NG];
@@ -601,7 +610,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             const int b0 = xt * plan.n, n = min(plan.n, p.batch - b0);
             const bool mine = ok && out < w.rows;
             T* const y = (T*)p.y + b0 * p.y_stride + out;
-            const T* const res = p.residual ? (const T*)p.residual + b0 * p.residual_stride + out : nullptr;
+            const T* const res = COLS == 64 && p.residual ? (const T*)p.residual + b0 * p.residual_stride + out : nullptr;
             float factor[2] = {4.0f, 4.0f};  // of rows lane and lane + 32
             if (SPLIT) {
 #pragma unroll
@@ -626,15 +635,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
             };
             if (cs == 1) {
 #pragma unroll
-                for (int k = 0; k < PAIRS; k += 4) {
+                for (int k = 0; k < PAIRS; k += 8) {
                     if (2 * k >= n) continue;
-                    float v[8];
+                    float v[16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 8; ++i) {
                         const float2 u = many_two(total[k + i]);
                         v[2 * i] = u.x, v[2 * i + 1] = u.y;
                     }
-                    store(std::integral_constant<int, 8>(), [&](int i) { return 2 * k + i; }, v);
+                    store(std::integral_constant<int, 16>(), [&](int i) { return 2 * k + i; }, v);
                 }
             } else {
                 // Row r of x belongs to CTA (r / 2) % cs: [sender][r / 2 / cs][r % 2][256] in

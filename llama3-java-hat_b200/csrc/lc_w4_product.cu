@@ -82,9 +82,15 @@ int64_t many_rows(const W4& w, bool split) {
 
 template <typename T, int GROUP, bool ZEROS>
 cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st) {
-    constexpr int MOST = many_most(sizeof(T) == 4), HALVES = sizeof(T) == 4 ? 2 : 1;
+    constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
+    // Units of 128 rows for F16 prompts, whose products then set the pace, not the
+    // codes: 2048 rows of 16384 x 2048, us in units of 128 | 64 rows: groups of 128 208
+    // | 245, of 64 274 | 300, of 32 433 | 406; 386 rows of 5742 x 1024 21 | 27, 100 rows
+    // of 16384 x 2048 24 | 20; with a residual 128 rows of it 47 | 27.
+    constexpr bool CAN = sizeof(T) == 2 && GROUP >= 64;
+    const int most = CAN && p.batch > 256 && !p.residual ? many_most(false) : 64;
     ManyPlan plan;
-    plan.x_tiles = (p.batch + MOST - 1) / MOST;
+    plan.x_tiles = (p.batch + most - 1) / most;
     plan.n = ((p.batch + plan.x_tiles - 1) / plan.x_tiles + 15) / 16 * 16;
     plan.w_tiles = (w.rows + kManyRows - 1) / kManyRows;
     plan.b = (const uint8_t*)ws;
@@ -109,8 +115,8 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
                               w.blocks, plan, (uint8_t*)ws, (float*)((uint8_t*)ws + kLayBytes));
     if (e != cudaSuccess) return e;
     auto* kernel = w4_many_kernel<T, GROUP, ZEROS, 64>;
-    if constexpr (MOST > 64) {
-        if (big) kernel = w4_many_kernel<T, GROUP, ZEROS, MOST>;
+    if constexpr (CAN) {
+        if (big) kernel = w4_many_kernel<T, GROUP, ZEROS, many_most(false)>;
     }
     // The register split draws on what the launch has: more than that would wait forever.
     cudaFuncAttributes attr;
