@@ -148,6 +148,38 @@ def test_hard_rows(lp, vocab, kind):
     check(lp, x[::-1].copy(), tokens[::-1].copy(), 0, scale=2.0)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_few_allowed(lp, kind):
+    """A grammar: a handful of allowed tokens, next to each other or far apart, or a
+    few threads that have all the large ones."""
+    rng = np.random.default_rng(8)
+    vocab = 50000
+    for low in (-np.inf, LOWEST[kind]):
+        x = np.full((6, vocab), low)
+        x[0, rng.integers(0, vocab, 13)] = rng.standard_normal(13)
+        x[1, 777:790] = rng.standard_normal(13)
+        x[2, 20000:21000] = rng.standard_normal(1000)
+        x[3, ::1024] = rng.standard_normal(len(x[3, ::1024]))
+        x[4, :40] = np.arange(40)
+        x[5] = rng.standard_normal(vocab)
+        x[5, 3000:3400] += 50.0  # all of the best in a few threads
+        x = x.astype(ref.NP[kind])
+        tokens = x.argmax(1)
+        check(lp, x, tokens, 5)
+        check(lp, x, rng.integers(0, vocab, 6), 32)
+    # Large ones at the stride at which a thread reads: hundreds in one thread.
+    n = 16 // np.dtype(ref.NP[kind]).itemsize
+    x = rng.standard_normal((1, 256 * n * 120)) * 0.01
+    for e in range(n):
+        x[0, 5 * n + e::256 * n] += 10.0
+    x = np.repeat(x, 400, 0).astype(ref.NP[kind])  # one CTA per row
+    x[:, 0] += np.arange(400) % 3
+    got = run(lp, x, np.zeros(400), 32)
+    check(lp, x[:3], [0, 5 * n, 7], 32)
+    for i in range(0, 400, 57):
+        np.testing.assert_array_equal(got[3][i], ref.order(x[i])[:32])
+
+
 def test_asked_outputs_alone(L, lp):
     """Each output by itself has the same bits as all together; host memory too."""
     rng = np.random.default_rng(2)

@@ -172,6 +172,16 @@ def test_product_sizes(L, acc, rows, cols, batch, kind):
     check_product(L, acc, rng, rows, cols, batch, 32, True, kind, residual=True)
 
 
+@pytest.mark.parametrize("rows,cols,batch", [(20, 60000, 8),    # a CTA's columns in parts, one after the other
+                                             (17, 140000, 11),  # too wide for the workspace: a few rows at a time
+                                             (40, 8192, 1100),  # more rows than the workspace takes at once
+                                             (300, 256, 1500)])
+def test_product_in_parts(L, acc, rows, cols, batch):
+    rng = np.random.default_rng(cols)
+    check_product(L, acc, rng, rows, cols, batch, 64, True, "f32", residual=True)
+    check_product(L, acc, rng, rows, cols, batch, 128, False, "f16")
+
+
 @pytest.mark.parametrize("batch", [1, 7, 70])
 def test_product_rows_of_unlike_size(L, acc, batch):
     """fp32 rows from the smallest numbers to near the largest, one-sided sums,
@@ -253,6 +263,77 @@ def test_product_is_repeatable_and_captured(L, acc):
             graph.replay()
         for y, f in zip(ys, first):
             np.testing.assert_array_equal(host(acc, y), f)
+
+
+def test_shared_rows_and_strides(L, acc):
+    """One row of x for all of a batch (stride 0), rows of y far apart, odd addresses."""
+    rng = np.random.default_rng(14)
+    code, scale, zero = ref.quantize(weights(rng, 90, 200, "f32"), 64, True)
+    w = packed(L, acc, code, scale, zero, 64)
+    for kind in ("f32", "f16"):
+        for batch in (1, 6, 21):
+            held = torch.zeros(201, dtype=torch.from_numpy(np.zeros(1, ref.NP[kind])).dtype, device="cuda")
+            x = rng.standard_normal(200).astype(ref.NP[kind])
+            held[1:] = torch.from_numpy(x)
+            y = torch.zeros(batch, 1000, dtype=held.dtype, device="cuda")
+            torch.cuda.synchronize()
+            w.apply(held[1:].expand(batch, 200), y[:, 7:97])
+            want, terms, far = ref.product(x[None], code, scale, zero, 64)
+            got = host(acc, y)
+            assert np.all(np.abs(got[:, 7:97] - want) <= ref.product_bound(want, terms, far, 4, kind))
+            assert not got[:, :7].any() and not got[:, 97:].any()
+
+
+def test_workspace_and_capture(L):
+    """The first product of many rows makes the workspace: not within a capture."""
+    acc = L.Accelerator(0)
+    w = L.Weights4.empty(64, 256, 64, acc=acc)
+    rng = np.random.default_rng(15)
+    v, x, y = dev(weights(rng, 64, 256, "f32")), dev(rng.standard_normal((40, 256), np.float32)), dev(np.zeros((40, 64), np.float32))
+    w.quantize(v)
+    st, graph = torch.cuda.ExternalStream(acc.stream), torch.cuda.CUDAGraph()
+    acc.synchronize()
+    with pytest.raises(L.IllegalStateError):
+        with torch.cuda.graph(graph, stream=st):
+            w.apply(x, y)
+    w.apply(x, y)
+    whole = host(acc, y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        w.apply(x, y)
+    y.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        graph.replay()
+    np.testing.assert_array_equal(host(acc, y), whole)
+    del graph
+
+
+def test_threads_share_a_context(L, acc):
+    """Two threads, products of many rows through the one workspace: each call is whole."""
+    import threading
+    rng = np.random.default_rng(16)
+    code, scale, zero = ref.quantize(weights(rng, 300, 512, "f32"), 64, False)
+    w = packed(L, acc, code, scale, zero, 64)
+    xs = [dev(rng.standard_normal((b, 512), np.float32)) for b in (33, 90)]
+    ys = [torch.zeros(len(x), 300, device="cuda") for x in xs]
+    torch.cuda.synchronize()
+    alone = []
+    for x, y in zip(xs, ys):
+        w.apply(x, y)
+        alone.append(host(acc, y))
+    wrong = []
+
+    def run(x, y, want):
+        for _ in range(100):
+            w.apply(x, y)
+        acc.synchronize()
+        if not np.array_equal(y.cpu().numpy(), want):
+            wrong.append(len(x))
+    threads = [threading.Thread(target=run, args=a) for a in zip(xs, ys, alone)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
 
 
 # ----------------------------------------------------- refusals on a device
