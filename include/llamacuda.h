@@ -335,9 +335,14 @@ int lc_kv8_attention(lc_context* ctx, const lc_kv8* kv, const void* q, void* out
  * (K/IGEMV.java:34-68).  Row buffers are F32 or F16 (dtype 0 or 1), row i at
  * i * stride elements, host or device memory; the weights are device memory.
  * With device memory throughout, the calls only enqueue on the context's
- * stream and can be captured in a CUDA graph; they keep nothing between calls
- * but the weights.  Threads may share a context: these calls and those of the
- * sections on the paged cache and on log probabilities take turns. */
+ * stream and can be captured in a CUDA graph.  The first lc_w4_product of a
+ * context with more than a few rows (4 F32 or 8 F16 rows: some of those, and
+ * all with more than 12) allocates its workspace of 33 MiB, the same for all
+ * calls: make it before a capture.  Graphs captured from one context share it,
+ * with each other and with the calls themselves: replay them one after the
+ * other, on the context's stream or ordered against it.  Threads may share a
+ * context: these calls and those of the sections on the paged cache and on log
+ * probabilities take turns. */
 
 /* W [rows][cols] in device memory that the caller owns:
  *   W[r][c] = scale[r][c / group] * (code[r][c] - zero[r][c / group])
@@ -380,11 +385,12 @@ int lc_w4_read(lc_context* ctx, const lc_w4* w, void* values, int64_t stride, in
  * [cols], y and residual [batch][rows], all of dtype.  residual may be y (with
  * its stride); no other buffers may overlap.  batch 1: the GEMV of a decode
  * step; more: sequences or the tokens of a prompt.  Codes enter as whole
- * numbers, F32 rows as two F16 under a power-of-two row scale (2^-22 relative
- * to the row's largest), F16 rows as they are, scales as they are; sums are
- * fp32, y is rounded once.  Results of a row do not depend on the others.  A
- * row of x with a NaN or an infinity gives NaN, infinities or numbers in its
- * own row of y only. */
+ * numbers, F32 rows as two F16 under a power-of-two row scale (2^-22, and
+ * 2^-39 of the row's largest), F16 rows as they are, scales as they are; sums
+ * are fp32, y is rounded once.  What a row holds does not touch the results of
+ * the others (how many they are chooses the kernel, and so the order of sums);
+ * a NaN or an infinity in it leaves no finite results in its own.  The same
+ * call gives the same bits again. */
 int lc_w4_product(lc_context* ctx, const lc_w4* w, const void* x, int64_t x_stride, void* y, int64_t y_stride,
                   const void* residual, int64_t residual_stride, int32_t batch, int32_t dtype);
 
@@ -405,7 +411,8 @@ int lc_w4_product(lc_context* ctx, const lc_w4* w, const void* x, int64_t x_stri
  * +inf gives NaN for every ln p and the entropy; in the order NaN counts as
  * -inf.  scale (1 / temperature) is positive and finite.  Buffers may be host
  * or device memory; with device memory throughout the call only enqueues, can
- * be captured and keeps nothing.  Turns as in the section before. */
+ * be captured and keeps nothing.  Turns as in the section before.  The same call
+ * gives the same bits again. */
 int lc_logprobs(lc_context* ctx, const void* logits, int64_t stride, int32_t dtype, int32_t rows, int32_t vocab,
                 float scale, const int32_t* tokens, float* token_logprobs, int32_t* token_ranks, float* entropy,
                 int32_t top_k, int32_t* top_ids, float* top_logprobs);

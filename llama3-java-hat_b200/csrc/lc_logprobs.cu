@@ -16,9 +16,11 @@
 // finds them.  A rank is counted where a chunk's largest logit reaches the
 // token's, which few chunks do for likely tokens.
 //
-// Bound by memory: 5 to 6 instructions per logit where HBM leaves time for 22
-// (F32) or 11 (F16).  Few rows are cut over a cluster of up to 16 CTAs, whose
-// parts meet in the shared memory of the first: no workspace, nothing kept.
+// Bound by instructions in F16: 9 per logit where HBM leaves time for 11 (2048 rows
+// of 128256: 107 to 118 us, 80 at the measured copy's rate), and by the beginnings
+// and ends of CTAs where rows are short.  F32 rows leave time for 22.  Few rows are
+// cut over a cluster of up to 16 CTAs, whose parts meet in the shared memory of the
+// first: no workspace, nothing kept.
 #include <type_traits>
 
 #include "lc_internal.h"
@@ -27,8 +29,7 @@
 namespace lc {
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpThreads = 256, kLpShort = 128;  // of a CTA, and where rows are many and short
 constexpr int kLpPieces = 4;       // 16-byte pieces of a thread's chunk
 constexpr uint32_t kLpFound = 256;  // candidates that are put in order by counting
 constexpr int kLpMaxCluster = 16;  // more than 8 is opt-in
@@ -199,10 +200,11 @@ LC_DEV uint64_t merge_lists(uint64_t a, uint64_t b, int lane) {
 }
 
 // lists[0] = the largest of n lists (a power of two), by all warps of the CTA.
+template <int WARPS>
 LC_DEV void join_lists(uint64_t (*lists)[32], int n, int warp, int lane) {
     for (n >>= 1; n > 0; n >>= 1) {
         __syncthreads();
-        for (int i = warp; i < n; i += kLpWarps) lists[i][lane] = merge_lists(lists[i][lane], lists[i + n][lane], lane);
+        for (int i = warp; i < n; i += WARPS) lists[i][lane] = merge_lists(lists[i][lane], lists[i + n][lane], lane);
     }
     __syncthreads();
 }
@@ -227,16 +229,17 @@ struct Part {  // of a CTA's share of a row
     uint32_t before;
 };
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int cluster) {
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logprobs p, int cluster) {
+    constexpr int WARPS = THREADS / 32;
     __shared__ Part parts[kLpMaxCluster];
-    __shared__ __align__(16) __half tops[TOP ? kLpThreads : 1];
-    __shared__ uint64_t found[TOP ? kLpFound + 32 * kLpWarps : 1];
+    __shared__ __align__(16) __half tops[TOP ? THREADS : 1];
+    __shared__ uint64_t found[TOP ? kLpFound + 32 * WARPS : 1];
     __shared__ uint64_t lists[TOP ? kLpMaxCluster : 1][32];
-    __shared__ uint64_t ours[TOP ? kLpWarps : 1][32];
-    __shared__ uint16_t chosen[TOP ? kLpThreads : 1];
-    __shared__ uint32_t warp_top[kLpWarps], warp_before[kLpWarps], n_chosen, n_found, least;
-    __shared__ float warp_s[kLpWarps], warp_t[kLpWarps];
+    __shared__ uint64_t ours[TOP ? WARPS : 1][32];
+    __shared__ uint16_t chosen[TOP ? THREADS : 1];
+    __shared__ uint32_t warp_top[WARPS], warp_before[WARPS], n_chosen, n_found, least;
+    __shared__ float warp_s[WARPS], warp_t[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
     if (cluster > 1) cluster_arrive();  // all CTAs of the cluster have begun when the wait below is over
@@ -262,14 +265,14 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
     Piece<T> next[kLpPieces];
     auto fetch = [&](int base) {  // the thread's pieces of the chunk at base, -inf behind the share
         const int j = base + tid;
-        if (base >= whole0 && base + kLpPieces * kLpThreads <= whole1) {
+        if (base >= whole0 && base + kLpPieces * THREADS <= whole1) {
             const T* from = row.x + row.first(j);
 #pragma unroll
-            for (int k = 0; k < kLpPieces; ++k) next[k].w = load_once(from + k * kLpThreads * N);
+            for (int k = 0; k < kLpPieces; ++k) next[k].w = load_once(from + k * THREADS * N);
         } else {
 #pragma unroll
             for (int k = 0; k < kLpPieces; ++k) {
-                const int at = j + k * kLpThreads;
+                const int at = j + k * THREADS;
                 if (at < p1) next[k] = row.load(at);
                 else next[k].w = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
                                                 : make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
@@ -286,12 +289,12 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
     }
     const bool ranked = token >= 0 && p.token_ranks && mine > -INFINITY;
     const float under = Piece<T>::below(mine);
-    for (int base = p0; base < p1; base += kLpPieces * kLpThreads) {
+    for (int base = p0; base < p1; base += kLpPieces * THREADS) {
         const int j = base + tid;
         Piece<T> w[kLpPieces];
 #pragma unroll
         for (int k = 0; k < kLpPieces; ++k) w[k] = next[k];
-        if (base + kLpPieces * kLpThreads < p1) fetch(base + kLpPieces * kLpThreads);
+        if (base + kLpPieces * THREADS < p1) fetch(base + kLpPieces * THREADS);
         float top = w[0].top();
 #pragma unroll
         for (int k = 1; k < kLpPieces; ++k) top = max_nan(top, w[k].top());
@@ -318,15 +321,15 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
         if (ranked && !(top < mine)) {
 #pragma unroll
             for (int k = 0; k < kLpPieces; ++k) {
-                const int i = row.first(j + k * kLpThreads);
+                const int i = row.first(j + k * THREADS);
                 before += i + N <= token ? w[k].above(under) : w[k].above(mine);
-                if (i < token && i + N > token && j + k * kLpThreads < p1)  // the token's own piece: what stands before it counts when equal
+                if (i < token && i + N > token && j + k * THREADS < p1)  // the token's own piece: what stands before it counts when equal
                     for (int e = i; e < token; ++e) before += row.has(e) && (float)row.x[e] == mine;
             }
         }
     }
     if (token >= 0 && p.token_ranks && !ranked) {  // a masked token comes behind all that are not, and masked ones before it
-        for (int64_t i = (int64_t)p0 * N - row.skew + tid, end = (int64_t)p1 * N - row.skew; i < end; i += kLpThreads)
+        for (int64_t i = (int64_t)p0 * N - row.skew + tid, end = (int64_t)p1 * N - row.skew; i < end; i += THREADS)
             before += i >= 0 && i < p.vocab && ((float)row.x[i] > -INFINITY || i < token);
     }
 
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
     __syncthreads();
     uint32_t cta_top = warp_top[0];
 #pragma unroll
-    for (int i = 1; i < kLpWarps; ++i) cta_top = max(cta_top, warp_top[i]);
+    for (int i = 1; i < WARPS; ++i) cta_top = max(cta_top, warp_top[i]);
     const float cta_m = cta_top == 0xffffffffu ? NAN : unordered(cta_top);
     {
         const float now = fmaxf(cta_m, -3.4028234663852886e38f);
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
             const __half2 m2 = __half2half2(tops[tid]);
             __half2 above = __half2half2(__ushort_as_half(0));
 #pragma unroll 8
-            for (int i = 0; i < kLpThreads / 8; ++i) {
+            for (int i = 0; i < THREADS / 8; ++i) {
                 const uint4 o = reinterpret_cast<const uint4*>(tops)[i];
                 const __half2* h = reinterpret_cast<const __half2*>(&o);
                 above = __hadd2(above, __hadd2(__hadd2(__hgt2(h[0], m2), __hgt2(h[1], m2)), __hadd2(__hgt2(h[2], m2), __hgt2(h[3], m2))));
@@ -380,18 +383,18 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
         // the least of their maxima is set aside.
         const float floor = unordered(least);
         const uint64_t bar = (uint64_t)least << 32;
-        const int per = (p1 - p0 + kLpThreads - 1) / kLpThreads, items = (int)n_chosen * per;
+        const int per = (p1 - p0 + THREADS - 1) / THREADS, items = (int)n_chosen * per;
         auto item_of = [&](int item, Piece<T>& w) {
-            const int q = item / per, j = item < items ? p0 + chosen[q] + (item - q * per) * kLpThreads : p1;
+            const int q = item / per, j = item < items ? p0 + chosen[q] + (item - q * per) * THREADS : p1;
             if (j < p1) w = row.load(j);
             return j;
         };
         auto collect = [&](uint64_t from, bool above) {  // keys from `from` on; above: larger than floor
-            for (int item = tid; item < items && *(volatile uint32_t*)&n_found <= kLpFound; item += 4 * kLpThreads) {
+            for (int item = tid; item < items && *(volatile uint32_t*)&n_found <= kLpFound; item += 4 * THREADS) {
                 Piece<T> w[4];
                 int j[4];
 #pragma unroll
-                for (int z = 0; z < 4; ++z) j[z] = item_of(item + z * kLpThreads, w[z]);
+                for (int z = 0; z < 4; ++z) j[z] = item_of(item + z * THREADS, w[z]);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
                     if (j[z] >= p1 || (above ? w[z].top() <= floor : w[z].top() < floor)) continue;
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
             __syncthreads();
             fit = n_found <= kLpFound;
             if (fit) {
-                const int q0 = p0 + (int)((int64_t)(p1 - p0) * warp / kLpWarps), q1 = p0 + (int)((int64_t)(p1 - p0) * (warp + 1) / kLpWarps);
+                const int q0 = p0 + (int)((int64_t)(p1 - p0) * warp / WARPS), q1 = p0 + (int)((int64_t)(p1 - p0) * (warp + 1) / WARPS);
                 __syncthreads();  // all have read the count
                 int got = 0;
                 for (int j = q0 + lane; __any_sync(0xffffffffu, j < q1) && got < p.top; j += 32) {
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
         }
         if (fit) {
             // Each one's place is the number of larger ones.
-            for (int q = tid; q < (int)n_found; q += kLpThreads) {
+            for (int q = tid; q < (int)n_found; q += THREADS) {
                 const uint64_t key = found[q];
                 int place = 0;
                 for (int o = 0; o < (int)n_found; ++o) place += found[o] > key;
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
             // Hundreds above the least maximum in the few threads that have them: every
             // warp keeps the best of its share in order, a key per lane.
             uint64_t list = 0, edge = bar - 1;
-            for (int base = warp * 32; base < items; base += kLpThreads) {
+            for (int base = warp * 32; base < items; base += THREADS) {
                 Piece<T> w;
                 w.w = make_uint4(0, 0, 0, 0);
                 const int j = item_of(base + lane, w), i = row.first(j);
@@ -482,7 +485,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
                 }
             }
             ours[warp][lane] = list;
-            join_lists(ours, kLpWarps, warp, lane);
+            join_lists<WARPS>(ours, WARPS, warp, lane);
         }
     } else {
         __syncthreads();
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
     if (warp == 0) {
         Part mine_part = {cta_m, 0.0f, 0.0f, 0};
 #pragma unroll
-        for (int i = 0; i < kLpWarps; ++i) mine_part.s += warp_s[i], mine_part.t += warp_t[i], mine_part.before += warp_before[i];
+        for (int i = 0; i < WARPS; ++i) mine_part.s += warp_s[i], mine_part.t += warp_t[i], mine_part.before += warp_before[i];
         if (cluster == 1) {
             if (lane == 0) parts[0] = mine_part;
             if (TOP) lists[0][lane] = ours[0][lane];
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
         if (rank != 0) return;  // what it wrote lies in the first CTA
         cluster_wait();
     }
-    if (TOP && cluster > 1) join_lists(lists, cluster, warp, lane);
+    if (TOP && cluster > 1) join_lists<WARPS>(lists, cluster, warp, lane);
     if (warp != 0) return;
     __syncwarp();
     float high = parts[0].m;
@@ -541,11 +544,12 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_kernel(Logprobs p, int
     }
 }
 
-template <typename T, bool TOP>
-cudaError_t launch_as(const Logprobs& p, int cluster, cudaStream_t st) {
+template <typename T, bool TOP, int THREADS>
+cudaError_t launch_with(const Logprobs& p, int cluster, cudaStream_t st) {
+    auto* kernel = logprobs_kernel<T, TOP, THREADS>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.rows * cluster);
-    cfg.blockDim = dim3(kLpThreads);
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -556,22 +560,34 @@ cudaError_t launch_as(const Logprobs& p, int cluster, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     if (cluster > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, p, cluster);
+    return cudaLaunchKernelEx(&cfg, kernel, p, cluster);
+}
+
+// More rows than are resident, of 64 KB and less, go in CTAs of 128 threads, of which
+// twice as many hide each other's beginnings and ends: 2025 F16 rows of 11627 27 us
+// instead of 43, 600 F32 rows of it 13 and 16, 1200 F16 rows of 4000 13 and 21 (333
+// F16 rows of 32003, all resident, 28 and 17).
+template <typename T, bool TOP>
+cudaError_t launch_as(const Logprobs& p, int cluster, bool brief, cudaStream_t st) {
+    return brief ? launch_with<T, TOP, kLpShort>(p, cluster, st) : launch_with<T, TOP, kLpThreads>(p, cluster, st);
 }
 
 }  // namespace
 
 cudaError_t launch_logprobs(const Logprobs& p, int num_sms, cudaStream_t st) {
-    // CTAs of a row: enough to have two for every SM, each with a chunk's worth of
-    // work for its threads.
+    // CTAs of a row: as many as are resident at once, three on an SM, each with two
+    // chunks' work for its threads.  More of them cost their beginnings and ends (64 F16
+    // rows of 128256 in 512 CTAs 11.3 us, in 256 10.2; 2048 rows in 1, 2 and 4 CTAs each
+    // 115, 122 and 148).
     const int64_t pieces = (int64_t)p.vocab * (p.dtype == kRowF32 ? 4 : 2) / 16;
     int cluster = 1;
-    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster < 2 * num_sms && pieces / (2 * cluster) >= kLpThreads) cluster *= 2;
-    if (p.dtype == kRowF32) return p.top ? launch_as<float, true>(p, cluster, st) : launch_as<float, false>(p, cluster, st);
-    return p.top ? launch_as<__half, true>(p, cluster, st) : launch_as<__half, false>(p, cluster, st);
+    while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster * 2 <= 3 * num_sms && pieces / (4 * cluster) >= kLpThreads) cluster *= 2;
+    const bool brief = p.rows > 3 * num_sms && pieces <= 4096;
+    if (p.dtype == kRowF32) return p.top ? launch_as<float, true>(p, cluster, brief, st) : launch_as<float, false>(p, cluster, brief, st);
+    return p.top ? launch_as<__half, true>(p, cluster, brief, st) : launch_as<__half, false>(p, cluster, brief, st);
 }
 
 }  // namespace lc

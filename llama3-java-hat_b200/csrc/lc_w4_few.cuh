@@ -1,14 +1,14 @@
 // lc_w4_few.cuh -- products of 4-bit weights with few rows (decode steps).
 //
 // A warp has 32 rows of W (two tiles, for which x is loaded once) and a part of
-// the columns; m16n8k16 products take the
-// codes as f16 numbers c 2^-17 straight from the words of the layout (exact, and so
-// is every product; as c 2^-24, which takes five instructions instead of seven for
-// eight codes, the tensor cores align products by the least normal exponent and
-// lose what lies 2^-24 below it: errors 2^-19 of the sum) against x as columns: F16 rows as they are, F32 rows as two columns
-// hi and lo under a power-of-two scale of the row (of what the warp has of it),
-// exact to 2^-22.  The sums of a group begin at -z sum x, and are added under the
-// group's scale to fp32 sums.
+// the columns; m16n8k16 products take the codes as f16 numbers c 2^-17 straight
+// from the words of the layout, exact as every product is.  (As c 2^-24, which
+// takes five instructions instead of seven for eight codes, the tensor cores align
+// products by the least normal exponent and lose what lies 2^-24 below it: errors
+// of 2^-19 of the sum.)  x stands against them as columns: F16 rows as they are,
+// F32 rows as hi and lo under a power-of-two scale of the row (of what the CTA has
+// of it), exact to 2^-22.  The sums of a group begin at -z sum x, and are added
+// under the group's scale to fp32 sums.
 //
 // Bound by HBM for large matrices, by latency for small ones.  Each warp streams
 // its codes, scales and zero points through a ring of its own in shared memory
@@ -16,7 +16,10 @@
 // warps share a pair of tiles: fewer make fewer meetings, more make the pairs go
 // round evenly.  Where a CTA's columns would not fit, or rows are too few to go
 // round, a cluster shares them; its CTAs meet in each other's shared memory.  Sums
-// are added in a fixed order.
+// are added in a fixed order.  128256 x 2048 for one row: 34.5 us, 21.4 at the
+// measured copy's rate, with 142 instructions of a warp for 2048 codes, 56 of them
+// for taking the codes out (one tile at a time and eight warps to a tile: 48 us).
+// Four CTAs of an SM would hide more of their latency; registers are for two.
 #pragma once
 
 #include "lc_internal.h"

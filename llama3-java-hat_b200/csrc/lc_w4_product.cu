@@ -1,7 +1,8 @@
 // lc_w4_product.cu -- y = x W^T (+ a residual) with 4-bit weights (lc_w4.h).
 //
 // y[b][r] = sum over groups of s[r][group] * sum over its columns of (c - z) x.
-// The inner sums are of whole numbers times x; a group's scale is applied once.
+// The inner sums are of whole numbers times x; a group's scale is applied once, to
+// them.  Two kernels: lc_w4_few.cuh and lc_w4_many.cuh.
 #include "lc_internal.h"
 #include "lc_w4.h"
 #include "lc_w4_few.cuh"

@@ -95,7 +95,7 @@ def test_sizes(lp, top, kind):
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("rows,vocab", [(1, 128256), (2, 128256), (5, 100003), (19, 50021), (64, 8192), (150, 1001), (300, 4096),
-                                        (700, 515)])
+                                        (700, 515), (500, 9001)])
 def test_rows(lp, rows, vocab, kind):
     rng = np.random.default_rng(rows)
     check(lp, logits(rng, rows, vocab, kind), rng.integers(-1, vocab, rows), 20, scale=1.25, pad=rows % 2)
@@ -178,6 +178,21 @@ def test_few_allowed(lp, kind):
     check(lp, x[:3], [0, 5 * n, 7], 32)
     for i in range(0, 400, 57):
         np.testing.assert_array_equal(got[3][i], ref.order(x[i])[:32])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_many_short_rows(lp, kind):
+    """More rows than are resident: the hard ones of them in the CTAs of short rows."""
+    rng = np.random.default_rng(18)
+    x = logits(rng, 460, 6007, kind)
+    x[3], x[7], x[11] = -np.inf, LOWEST[kind], 2.0
+    x[20, rng.random(6007) < 0.999] = -np.inf
+    x[30] = np.arange(6007) / 16.0
+    x[40, 9] = np.nan
+    x[50, ::7] = np.inf
+    x[60, ::8] += 30.0
+    check(lp, x, rng.integers(-1, 6007, 460), 32)
+    check(lp, x, rng.integers(-1, 6007, 460), 0, pad=1)
 
 
 def test_asked_outputs_alone(L, lp):
