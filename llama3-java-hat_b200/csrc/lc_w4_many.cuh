@@ -6,15 +6,20 @@
 // scale (2^-22), rows and columns that are not there as zeros.  The second has
 // units of 256 rows of W and up to 128 rows of x (F32: 64),
 //   D = A B   M 128 (twice), N up to 128, K one group (F32: A Bhi + A Blo)
-// with A = (c - z) / 4, exact in f16, made from the codes.  A group's D is added, under the group's scale, to fp32 sums that an epilogue thread
-// keeps in registers for its row of W, while the tensor cores fill the other D: so
-// scales need no rounding into weights, and the tensor cores' own truncating sums
-// run over 128 columns at most.
+// with A = (c - z) / 4, exact in f16, made from the codes.  A group's D is added,
+// under the group's scale, to fp32 sums that an epilogue thread keeps in registers
+// for its row of W, while the tensor cores fill the other D: so scales need no
+// rounding into weights, and the tensor cores' own truncating sums run over 128
+// columns at most.
 //
 // What bounds it: shared memory, while A lies there (units of more than 64 rows of
 // x, whose Ds fill tensor memory): the products of a block of 128 columns read 128
 // KB of it and the rest moves as much again, 2048 cycles where the tensor cores
-// need 1024.  Up to 64 rows A is in tensor memory, a thread writing its row.
+// need 1024 (2048 F16 rows of 16384 x 2048, groups of 128: 208 us, 83 at the measured
+// rate).  Up to 64 rows A is in tensor memory, a thread writing its row; making it
+// takes the operand warps some 1300 cycles of a block (17 F16 rows of 128256 x 2048:
+// 62 us, 22 at the measured copy's rate; with A in shared memory 73).  Groups of 32
+// are bound by reading D, four times per block.
 //
 // Warps 0-7: epilogue, four for each 128 rows.  Warps 8-15: codes to operands,
 // through rings of their own (cp.async).  Warp 16 issues the products, warp 17 the
@@ -56,7 +61,7 @@ struct ManyPlan {
     int x_tiles, w_tiles;
     int cluster;   // CTAs that share the columns of W, a power of two
     int cluster_log2;
-    int sets;      // groups of a block over groups of a D: those that fit 256 columns of tensor memory
+    int sets;      // Ds of a block: one per group, or per two where they fit
     int ring;      // blocks of a warp's ring of codes
     const uint8_t* b;      // [x tile][block][hi, lo][n / 8][16 octets][8][16 bytes]
     const float* factor;   // [batch] what the rows of x were divided by
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     const uint32_t b_bytes = HALVES * plan.n * kManyK * 2;  // of a stage
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const sa = smem;                            // [stages][tile of 128 rows][row groups][octets][8][16]
-    uint8_t* const sb = sa + (TA ? 0 : NS * kManyABytes);           // [stages][hi, lo][column groups][octets][8][16]
+    uint8_t* const sb = sa + (TA ? 0 : NS * kManyABytes);  // [stages][hi, lo][column groups][octets][8][16]
     uint8_t* const sc = sb + NS * b_bytes;               // [warps][ring][tile][half][lane][16]
     __shared__ __align__(8) uint64_t full[NS], empty[NS], d_full[2], d_free[2], drained;
     __shared__ uint32_t tmem_slot;

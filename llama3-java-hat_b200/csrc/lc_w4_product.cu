@@ -182,8 +182,9 @@ bool w4_product_uses_ws(const W4& w, const W4Product& p) {
     const bool f32 = p.dtype == kRowF32;
     if (p.batch <= few_rows(p.dtype) / 2 || many_rows(w, f32) == 0) return false;
     if (p.batch > (f32 ? 8 : 12)) return true;
+    constexpr int kSms = 148;
     const int pairs = (w.tiles + 1) / 2;
-    return !(pairs < 148 || (f32 && pairs >= 8 * 148));
+    return !(pairs < kSms || (f32 && pairs >= 8 * kSms));
 }
 size_t w4_product_ws_bytes() { return kLayBytes + kFactorBytes; }
 

@@ -528,7 +528,9 @@ class Weights4(_CudaKernel):
 
     def apply(self, x, y, residual=None) -> None:
         """y [batch, rows] = x [batch, cols] W^T, plus residual [batch, rows],
-        which may be y; all F32 or all F16 (see lc_w4_product)."""
+        which may be y; all F32 or all F16 (see lc_w4_product).  The first call
+        of an accelerator with more than a few rows makes its workspace: not
+        within a graph's capture."""
         xa, batch, width, xs, dt = _rows(x)
         ya, yb, ywidth, ys, ydt = _rows(y, True)
         if width != self.cols or ywidth != self.rows or yb != batch or ydt != dt:
