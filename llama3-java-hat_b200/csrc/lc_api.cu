@@ -1074,7 +1074,7 @@ extern "C" int lc_w4_product(lc_context* c, const lc_w4* w, const void* x, int64
         p.dtype = dtype;
         if ((uintptr_t)p.x % elem || (uintptr_t)p.y % elem || (uintptr_t)p.residual % elem)
             return fail(LC_ERR_INVALID_ARG, "rows are not aligned to their type");
-        const bool uses_ws = w4_product_uses_ws(view, p);
+        const bool uses_ws = w4_product_uses_ws(view, p, c->sms);
         if (uses_ws && !c->w4_ws) {
             cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
             CK(cudaStreamIsCapturing(c->stream, &capture), "cudaStreamIsCapturing");

@@ -52,7 +52,7 @@ cudaError_t launch_w4_quantize(const W4& w, const void* values, int64_t stride, 
 cudaError_t launch_w4_pack(const W4& w, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int num_sms, cudaStream_t st);
 cudaError_t launch_w4_read(const W4& w, void* values, int64_t stride, int dtype, int num_sms, cudaStream_t st);
 // Whether the product goes through the workspace (ws of w4_product_ws_bytes; else null).
-bool w4_product_uses_ws(const W4& w, const W4Product& p);
+bool w4_product_uses_ws(const W4& w, const W4Product& p, int num_sms);
 size_t w4_product_ws_bytes();
 cudaError_t launch_w4_product(const W4& w, const W4Product& p, int num_sms, void* ws, int* err, cudaStream_t st);
 

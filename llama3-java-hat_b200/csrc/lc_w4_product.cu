@@ -178,13 +178,12 @@ cudaError_t product(const W4& w, const W4Product& p, int num_sms, void* ws, int*
 //   16384 x 2048   5 F32 14 | 14, 8 F32 25 | 14, 9 F16 25 | 13, 16 F16 34 | 13
 //   2048 x 8192    5 F32 12 | 26, 8 F32 15 | 27, 9 F16 12 | 20, 16 F16 34 | 19
 //   2048 x 2048    5 F32  8 | 10, 8 F32  9 | 10, 9 F16  9 | 9,  16 F16 11 | 9
-bool w4_product_uses_ws(const W4& w, const W4Product& p) {
+bool w4_product_uses_ws(const W4& w, const W4Product& p, int num_sms) {
     const bool f32 = p.dtype == kRowF32;
     if (p.batch <= few_rows(p.dtype) / 2 || many_rows(w, f32) == 0) return false;
     if (p.batch > (f32 ? 8 : 12)) return true;
-    constexpr int kSms = 148;
     const int pairs = (w.tiles + 1) / 2;
-    return !(pairs < kSms || (f32 && pairs >= 8 * kSms));
+    return !(pairs < num_sms || (f32 && pairs >= 8 * num_sms));
 }
 size_t w4_product_ws_bytes() { return kLayBytes + kFactorBytes; }
 
