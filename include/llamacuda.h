@@ -366,10 +366,11 @@ int lc_w4_sizes(int32_t rows, int32_t cols, int32_t group, int64_t* code_bytes, 
  * values, without zero points: scale = max |x| / 7 and code = 8 + x / scale,
  * at least 1; with them: low = min(0, min x), high = max(0, max x),
  * scale = (high - low) / 15, zero = -low / scale, code = zero + x / scale.
- * Scales are quotients in 64 bits, rounded to F32 and then to F16, 65504 at most; x / scale
- * and -low / scale are rounded to the nearest whole number of the exact
- * quotient, ties to even, codes and zero points end at 0 and 15.  A group
- * whose scale is 0 holds zeros; NaN is held as 0, infinities as the last code. */
+ * Scales are quotients in 64 bits, rounded to F32 and then to F16, 65504 at
+ * most; x / scale and -low / scale are rounded to the nearest whole number of
+ * the exact quotient, ties to even, codes and zero points end at 0 and 15.  A
+ * group whose scale is 0 holds zeros; NaN is held as 0, infinities as the last
+ * code. */
 int lc_w4_quantize(lc_context* ctx, const lc_w4* w, const void* values, int64_t stride, int32_t dtype);
 
 /* Fills w from codes [rows][(cols + 1) / 2], the lower column of each byte in
