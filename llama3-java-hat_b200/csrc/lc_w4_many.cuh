@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
                     __syncwarp();  // the copies of all lanes have landed
                     if (i >= NS) ok = wait(&empty[st], (i / NS - 1) & 1);
                     if (!ok) break;
+                    tc_fence_after();  // the products that read this stage's A come before what is written over it
                     const uint32_t held = ring0 + slot * kManyRingBytes + (lane >> 4) * 1024 + g * 64;
                     const int up = (lane >> 1) & 4;  // 4: rows g + 8, whose codes are 4 bits higher
 #pragma unroll
@@ -690,6 +691,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    tc_fence_after();
     if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
