@@ -55,11 +55,49 @@ struct FewShape {
     // rows: of x.  One column of zeros stands for all that are not there.
     static size_t smem(const FewPlan& plan, int rows) {
         const int columns = (sizeof(T) == 4 ? 2 : 1) * rows + 1;
-        return (size_t)kFewWarps * kFewDepth * kSlot + columns * (256 * plan.blocks + 64) +
-               (plan.blocks * kGroups + 1 + kFewWarps) * kRows * 4 + kPartFloats * 4 +
+        const size_t blocks = plan.blocks;  // before it is cut into phases a part can have millions
+        return (size_t)kFewWarps * kFewDepth * kSlot + columns * (256 * blocks + 64) +
+               (blocks * kGroups + 1 + kFewWarps) * kRows * 4 + kPartFloats * 4 +
                (plan.cluster > 1 ? 2 * plan.cluster * each(plan.cluster, plan.split) * 4 : 0);
     }
 };
+
+constexpr size_t kFewTwo = 113 * 1024, kFewOne = 226 * 1024;  // shared memory with which two CTAs, or one, fit an SM
+
+// How the CTAs share the columns and the pairs of tiles, for `batch` rows of x.
+template <typename S>
+FewPlan few_plan(const W4& w, int batch, int num_sms) {
+    const int pairs = (w.tiles + 1) / 2;
+    FewPlan plan;
+    auto set = [&](int cluster, int phases) {
+        plan.cluster = cluster;
+        plan.phases = phases;
+        plan.blocks = (w.blocks + cluster * phases - 1) / (cluster * phases);
+        // Two CTAs per SM; of clusters an eighth less, for they do not fill a GPC.
+        const int most = cluster > 1 ? 2 * num_sms / cluster * 7 / 8 : 2 * num_sms;
+        plan.clusters = pairs < most ? pairs : most;
+        // Warps of a pair: few make few meetings, more make a CTA's pairs go round
+        // evenly.  A meeting costs about as much as kMeet blocks.
+        constexpr int kMeet = 2;
+        const int mine = (pairs + plan.clusters - 1) / plan.clusters;
+        int best = 0;
+        for (int split = 1; split <= kFewWarps; split *= 2) {
+            const int cost = (mine * split + kFewWarps - 1) / kFewWarps * ((plan.blocks + split - 1) / split + kMeet);
+            if (!best || cost < best) best = cost, plan.split = split;
+        }
+    };
+    // More CTAs for the columns while there are SMs without one and each warp has a
+    // block, or while a CTA's part keeps a second CTA off the SMs that few rows leave
+    // idle (16 half rows of 128256 x 2048: with clusters of 2 109 us, without 86; 8
+    // rows of 2048 x 8192: 14 and 27).
+    set(1, 1);
+    while (plan.cluster < kFewMaxCluster &&
+           ((w.blocks >= plan.cluster * kFewWarps && pairs * plan.cluster < num_sms) ||
+            (w.blocks >= 2 * plan.cluster * kFewWarps && pairs * plan.cluster < 2 * num_sms && S::smem(plan, batch) > kFewTwo)))
+        set(2 * plan.cluster, 1);
+    while (S::smem(plan, batch) > kFewOne) set(plan.cluster, plan.phases + 1);
+    return plan;
+}
 
 // The eight codes of a word as f16 pairs c 2^-17: rows g, g + 8 of columns e = 0, 1,
 // then of 2, 3.

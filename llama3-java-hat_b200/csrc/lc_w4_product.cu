@@ -16,44 +16,14 @@ constexpr int few_rows(int dtype) { return dtype == kRowF32 ? 8 : 16; }
 
 template <typename T, int GROUP, bool ZEROS, int NT>
 cudaError_t few_as(const W4& w, const W4Product& p, int num_sms, cudaStream_t st) {
-    using S = FewShape<T, GROUP, NT>;
-    constexpr size_t kTwo = 113 * 1024, kOne = 226 * 1024;  // shared memory with which two CTAs, or one, fit an SM
-    const int pairs = (w.tiles + 1) / 2;
-    FewPlan plan;
-    auto set = [&](int cluster, int phases) {
-        plan.cluster = cluster;
-        plan.phases = phases;
-        plan.blocks = (w.blocks + cluster * phases - 1) / (cluster * phases);
-        // Two CTAs per SM; of clusters an eighth less, for they do not fill a GPC.
-        const int most = cluster > 1 ? 2 * num_sms / cluster * 7 / 8 : 2 * num_sms;
-        plan.clusters = pairs < most ? pairs : most;
-        // Warps of a pair: few make few meetings, more make a CTA's pairs go round
-        // evenly.  A meeting costs about as much as kMeet blocks.
-        constexpr int kMeet = 2;
-        const int mine = (pairs + plan.clusters - 1) / plan.clusters;
-        int best = 0;
-        for (int split = 1; split <= kFewWarps; split *= 2) {
-            const int cost = (mine * split + kFewWarps - 1) / kFewWarps * ((plan.blocks + split - 1) / split + kMeet);
-            if (!best || cost < best) best = cost, plan.split = split;
-        }
-    };
-    // More CTAs for the columns while there are SMs without one and each warp has a
-    // block, or while a CTA's part keeps a second CTA off the SMs that few rows leave
-    // idle (16 half rows of 128256 x 2048: with clusters of 2 109 us, without 86; 8
-    // rows of 2048 x 8192: 14 and 27).
-    set(1, 1);
-    while (plan.cluster < kFewMaxCluster &&
-           ((w.blocks >= plan.cluster * kFewWarps && pairs * plan.cluster < num_sms) ||
-            (w.blocks >= 2 * plan.cluster * kFewWarps && pairs * plan.cluster < 2 * num_sms && S::smem(plan, p.batch) > kTwo)))
-        set(2 * plan.cluster, 1);
-    while (S::smem(plan, p.batch) > kOne) set(plan.cluster, plan.phases + 1);
+    const FewPlan plan = few_plan<FewShape<T, GROUP, NT>>(w, p.batch, num_sms);
     auto* kernel = w4_few_kernel<T, GROUP, ZEROS, NT>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOne);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewOne);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.clusters * plan.cluster));
     cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = S::smem(plan, p.batch);
+    cfg.dynamicSmemBytes = FewShape<T, GROUP, NT>::smem(plan, p.batch);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

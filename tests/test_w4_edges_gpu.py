@@ -69,3 +69,29 @@ def test_stages_used_again(L, acc, rows, cols, batch, kind):
     check(first, x, code, scale, zero, 64, kind)
     for y in ys[1:]:
         np.testing.assert_array_equal(y.cpu().numpy(), first)
+
+
+def test_widest_rows(L, acc):
+    """So many columns that the bytes of a CTA's part pass 32 bits before it is cut into
+    phases.  Whole numbers at columns here and there: the sums are exact."""
+    cols = 958682 * 8 * 128 - 77
+    rng = np.random.default_rng(1)
+    at = np.unique(np.concatenate([rng.integers(0, cols // 64, 5000) * 64 + rng.integers(1, 50, 5000), [cols - 1]]))
+    code, x = rng.integers(-6, 7, (2, len(at))), rng.integers(-8, 9, len(at)) / 4.0
+    w = L.Weights4.empty(2, cols, 64, acc=acc)
+    v = torch.zeros(2, cols, dtype=torch.float16, device="cuda")
+    v[0, ::64], v[1, ::64] = 7.0, -7.0  # a scale of 1 for every group
+    v[:, torch.from_numpy(at).cuda()] = torch.from_numpy(code).half().cuda()
+    torch.cuda.synchronize()
+    w.quantize(v)
+    acc.synchronize()
+    del v
+    held = torch.zeros(1, cols, device="cuda")
+    held[0, torch.from_numpy(at).cuda()] = torch.from_numpy(x).float().cuda()
+    y = torch.full((8, 2), float("nan"), device="cuda")
+    torch.cuda.synchronize()
+    w.apply(held.expand(8, cols), y)
+    got = host(acc, y)
+    del w, held
+    torch.cuda.empty_cache()
+    np.testing.assert_array_equal(got, np.repeat((code @ x)[None], 8, 0))
