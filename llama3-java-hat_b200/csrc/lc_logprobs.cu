@@ -89,6 +89,23 @@ LC_DEV float unordered(uint32_t o) {
 LC_DEV uint64_t order_key(float v, int i) { return (uint64_t)ordered(v) << 32 | (uint32_t)~i; }
 constexpr uint32_t kOrderedMasked = 0x007fffffu;  // of -inf
 
+// The unit of exponents: u = a b c (x - m), a b c = scale log2(e).  a and b are 1 for
+// F16, where c is held at 2^100: unlike logits are 2^-24 apart and more, so that beyond
+// it the smaller ones have p 0 all the same.  F32 logits can lie closer and further
+// apart: b = 2^26 for scales above 2^100, with which c is finite, and a = 2^-26 for
+// scales below 2^-100, with which a x - a m is, and c has all its bits.
+struct Unit {
+    float a, b, c;
+};
+Unit unit_of(float scale, int dtype) {
+    Unit u = {1.0f, 1.0f, scale};
+    if (dtype == kRowF32 && scale > 0x1p100f) u.b = 0x1p26f, u.c *= 0x1p-26f;
+    if (dtype == kRowF32 && scale < 0x1p-100f) u.a = 0x1p-26f, u.c *= 0x1p26f;
+    u.c *= kLog2e;
+    if (dtype != kRowF32 && u.c > 0x1p100f) u.c = 0x1p100f;
+    return u;
+}
+
 // 16 bytes of logits.
 template <typename T>
 struct Piece;
@@ -102,10 +119,13 @@ struct Piece<float> {
         return __uint_as_float(i & 2 ? hi : lo);
     }
     LC_DEV float top() const { return max_nan(max3_nan(get(0), get(1), get(2)), get(3)); }
-    // c2 (x - ref) of elements 2 i and 2 i + 1, kLpFloor where it is less.
+    // c (x - ref) of elements 2 i and 2 i + 1, kLpFloor where it is less.  FAR: under
+    // a scale for which it takes all of the unit's factors.
     template <bool FAR>
-    LC_DEV float2 powers(int i, float ref, uint64_t c2) const {
-        const float2 u = unpack2(mul2(add2(pack2(get(2 * i), get(2 * i + 1)), pack2(-ref, -ref)), c2));
+    LC_DEV float2 powers(int i, float ref, const Unit& unit) const {
+        const uint64_t x = pack2(get(2 * i), get(2 * i + 1)), c2 = pack2(unit.c, unit.c);
+        const float2 u = FAR ? unpack2(mul2(mul2(fma2(x, pack2(unit.a, unit.a), pack2(-ref * unit.a, -ref * unit.a)), pack2(unit.b, unit.b)), c2))
+                             : unpack2(mul2(add2(x, pack2(-ref, -ref)), c2));
         return make_float2(fmaxf(u.x, kLpFloor), fmaxf(u.y, kLpFloor));
     }
     // How many are larger than v.
@@ -137,7 +157,8 @@ struct Piece<__half> {
     // power is 0; -inf may then stand as that number, whose product with c is
     // finite (c is 2^100 at most).  A pair's clamp is one instruction so.
     template <bool FAR>
-    LC_DEV float2 powers(int i, float ref, uint64_t c2) const {
+    LC_DEV float2 powers(int i, float ref, const Unit& unit) const {
+        const uint64_t c2 = pack2(unit.c, unit.c);
         if (!FAR) {
             const float2 u = unpack2(mul2(add2(pack2(get(2 * i), get(2 * i + 1)), pack2(-ref, -ref)), c2));
             return make_float2(fmaxf(u.x, kLpFloor), fmaxf(u.y, kLpFloor));
@@ -229,8 +250,9 @@ struct Part {  // of a CTA's share of a row
     uint32_t before;
 };
 
-template <typename T, bool TOP, int THREADS>
-__global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logprobs p, int cluster) {
+// ENDS: F32 rows under a scale with which a or b is not 1.
+template <typename T, bool TOP, int THREADS, bool ENDS>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logprobs p, Unit unit, int cluster) {
     constexpr int WARPS = THREADS / 32;
     __shared__ Part parts[kLpMaxCluster];
     __shared__ __align__(16) __half tops[TOP ? THREADS : 1];
@@ -254,9 +276,10 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logpro
     const int64_t pieces = ((int64_t)row.skew + p.vocab + N - 1) / N;
     const int p0 = (int)(pieces * rank / cluster), p1 = (int)(pieces * (rank + 1) / cluster);
     // ---- the pass ----
-    const float c = fminf(p.scale * kLog2e, 0x1p100f);  // beyond it all smaller logits have p 0 all the same
-    const uint64_t c2 = pack2(c, c);
-    const float far_from = -65504.0f - kLpFloor / c;
+    const float far_from = -65504.0f - kLpFloor / unit.c;
+    auto down_to = [&](float ref, float now) {  // the exponent of ref's unit in now's
+        return fmaxf((ENDS ? (ref * unit.a - now * unit.a) * unit.b : ref - now) * unit.c, kLpFloor);
+    };
     float m = -INFINITY, ref = -3.4028234663852886e38f;  // ref: what exponents are taken from
     uint64_t s2 = 0, t2 = 0;  // pairs of sums
     uint32_t before = 0;
@@ -300,7 +323,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logpro
         for (int k = 1; k < kLpPieces; ++k) top = max_nan(top, w[k].top());
         m = max_nan(m, top);
         const float now = fmaxf(m, ref);
-        const float d = fmaxf((ref - now) * c, kLpFloor), down = exp2_fast(d);
+        const float d = down_to(ref, now), down = exp2_fast(d);
         ref = now;
         t2 = mul2(fma2(s2, pack2(d, d), t2), pack2(down, down));
         s2 = mul2(s2, pack2(down, down));
@@ -309,14 +332,14 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logpro
             for (int k = 0; k < kLpPieces; ++k) {
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) {
-                    const float2 u = w[k].template powers<decltype(far)::value>(i, ref, c2);
+                    const float2 u = w[k].template powers<decltype(far)::value>(i, ref, unit);
                     const uint64_t e2 = pack2(exp2_fast(u.x), exp2_fast(u.y));
                     s2 = add2(s2, e2);
                     t2 = fma2(e2, pack2(u.x, u.y), t2);
                 }
             }
         };
-        if (sizeof(T) == 2 && ref > far_from) add_up(std::true_type());
+        if (ENDS || (sizeof(T) == 2 && ref > far_from)) add_up(std::true_type());
         else add_up(std::false_type());
         if (ranked && !(top < mine)) {
 #pragma unroll
@@ -348,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logpro
     const float cta_m = cta_top == 0xffffffffu ? NAN : unordered(cta_top);
     {
         const float now = fmaxf(cta_m, -3.4028234663852886e38f);
-        const float d = fmaxf((ref - now) * c, kLpFloor), down = exp2_fast(d);
+        const float d = down_to(ref, now), down = exp2_fast(d);
         const float2 s = unpack2(s2), t = unpack2(t2);
         const float sum = s.x + s.y;
         const float ws = warp_sum(sum * down), wt2 = warp_sum(fmaf(sum, d, t.x + t.y) * down);
@@ -523,14 +546,19 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logpro
     float s = 0.0f, t = 0.0f;
     uint32_t all_before = 0;
     for (int i = 0; i < cluster; ++i) {
-        const float d = fmaxf((fmaxf(parts[i].m, -3.4028234663852886e38f) - from) * c, kLpFloor), down = exp2_fast(d);
+        const float d = down_to(fmaxf(parts[i].m, -3.4028234663852886e38f), from), down = exp2_fast(d);
         s = fmaf(parts[i].s, down, s);
         t = fmaf(fmaf(parts[i].s, d, parts[i].t), down, t);
         all_before += parts[i].before;
     }
     const bool bad = !(high < INFINITY), empty = high == -INFINITY;
     const float ln_s = logf(s);
-    auto logp = [&](float v) { return bad ? NAN : v == -INFINITY ? -INFINITY : (v - high) * p.scale - ln_s; };
+    auto logp = [&](float v) {
+        if (bad) return NAN;
+        const float below = v - high;  // where fp32 does not hold it, its half
+        if (below == -INFINITY && v > -INFINITY) return (0.5f * v - 0.5f * high) * p.scale * 2.0f - ln_s;
+        return v == -INFINITY ? -INFINITY : below * p.scale - ln_s;
+    };
     if (lane == 0) {
         if (p.token_logprobs) p.token_logprobs[r] = token >= 0 ? logp(mine) : 0.0f;
         if (p.token_ranks) p.token_ranks[r] = token >= 0 ? (int)all_before : -1;
@@ -544,9 +572,9 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) logprobs_kernel(Logpro
     }
 }
 
-template <typename T, bool TOP, int THREADS>
-cudaError_t launch_with(const Logprobs& p, int cluster, cudaStream_t st) {
-    auto* kernel = logprobs_kernel<T, TOP, THREADS>;
+template <typename T, bool TOP, int THREADS, bool ENDS>
+cudaError_t launch_with(const Logprobs& p, const Unit& unit, int cluster, cudaStream_t st) {
+    auto* kernel = logprobs_kernel<T, TOP, THREADS, ENDS>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.rows * cluster);
     cfg.blockDim = dim3(THREADS);
@@ -563,7 +591,7 @@ cudaError_t launch_with(const Logprobs& p, int cluster, cudaStream_t st) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
-    return cudaLaunchKernelEx(&cfg, kernel, p, cluster);
+    return cudaLaunchKernelEx(&cfg, kernel, p, unit, cluster);
 }
 
 // More rows than are resident, of 64 KB and less, go in CTAs of 128 threads, of which
@@ -572,7 +600,11 @@ cudaError_t launch_with(const Logprobs& p, int cluster, cudaStream_t st) {
 // F16 rows of 32003, all resident, 28 and 17).
 template <typename T, bool TOP>
 cudaError_t launch_as(const Logprobs& p, int cluster, bool brief, cudaStream_t st) {
-    return brief ? launch_with<T, TOP, kLpShort>(p, cluster, st) : launch_with<T, TOP, kLpThreads>(p, cluster, st);
+    const Unit unit = unit_of(p.scale, p.dtype);
+    if constexpr (sizeof(T) == 4) {
+        if (unit.a != 1.0f || unit.b != 1.0f) return launch_with<T, TOP, kLpThreads, true>(p, unit, cluster, st);
+    }
+    return brief ? launch_with<T, TOP, kLpShort, false>(p, unit, cluster, st) : launch_with<T, TOP, kLpThreads, false>(p, unit, cluster, st);
 }
 
 }  // namespace
