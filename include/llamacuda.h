@@ -386,9 +386,9 @@ int lc_w4_read(lc_context* ctx, const lc_w4* w, void* values, int64_t stride, in
  * [cols], y and residual [batch][rows], all of dtype.  residual may be y (with
  * its stride); no other buffers may overlap.  batch 1: the GEMV of a decode
  * step; more: sequences or the tokens of a prompt.  Codes enter as whole
- * numbers, F32 rows as two F16 under a power-of-two row scale (2^-22, and
- * 2^-39 of the row's largest), F16 rows as they are, scales as they are; sums
- * are fp32, y is rounded once.  What a row holds does not touch the results of
+ * numbers less their zero points, F32 rows as two F16 under a power-of-two row
+ * scale (2^-22, and 2^-39 of the row's largest), F16 rows as they are, scales as
+ * they are; sums are fp32, y is rounded once.  What a row holds does not touch the results of
  * the others (how many they are chooses the kernel, and so the order of sums);
  * a NaN or an infinity in it leaves no finite results in its own.  The same
  * call gives the same bits again. */

@@ -7,14 +7,14 @@
 // lane 4 g + t of the warp that reads them: rows g and g + 8, and of each 32
 // columns the eight from 8 t on.  Word j of the 16 bytes holds columns
 // 32 (j / 2) + 8 t + 4 (j % 2) + e, e = 0..3, at bit {0, 16, 8, 24}[e] for row g
-// and 4 bits higher for row g + 8, the whole word rotated left by 3.  So the word
-// rotated by 4, 0, -4 and -8 bits to the left and masked by 0x07800780 gives the
-// four registers that one m16n8k16 product takes from the lane, as pairs of f16
-// numbers c 2^-17 (seven instructions for eight codes; f16 numbers below 2^-13
-// are linear in their bits); each product lies within one group; and what the
-// lane has of a row are runs of eight columns, 16 bytes of f16, which is what
-// tcgen05 operands are made of.  The order of columns within a product does not
-// matter as long as both operands have the same.
+// and 4 bits higher for row g + 8, the whole word rotated left by 3.  So the word,
+// and the word rotated by 8 bits, masked by 0x00780078 and 0x07800780, give the four
+// registers that one m16n8k16 product takes from the lane, as pairs of f16 numbers
+// c 2^-21 (row g) and c 2^-17 (row g + 8): f16 numbers below 2^-13 are linear in
+// their bits, and an FMA makes c - z of them.  Each product lies within one group;
+// and what the lane has of a row are runs of eight columns, 16 bytes of f16, which
+// is what tcgen05 operands are made of.  The order of columns within a product does
+// not matter as long as both operands have the same.
 //
 // Scales (f16) and zero points (bytes) of a block: [8 g][128 / group][2], the
 // pair being rows g and g + 8.  Rows

@@ -1,14 +1,14 @@
 // lc_w4_few.cuh -- products of 4-bit weights with few rows (decode steps).
 //
 // A warp has 32 rows of W (two tiles, for which x is loaded once) and a part of
-// the columns; m16n8k16 products take the codes as f16 numbers c 2^-17 straight
-// from the words of the layout, exact as every product is.  (As c 2^-24, which
-// takes five instructions instead of seven for eight codes, the tensor cores align
-// products by the least normal exponent and lose what lies 2^-24 below it: errors
-// of 2^-19 of the sum.)  x stands against them as columns: F16 rows as they are,
-// F32 rows as hi and lo under a power-of-two scale of the row (of what the CTA has
-// of it), exact to 2^-22.  The sums of a group begin at -z sum x, and are added
-// under the group's scale to fp32 sums.
+// the columns; m16n8k16 products take the weights as f16 numbers (c - z) 2^-6 from
+// the words of the layout, exact as every product is: what a zero point takes away
+// is gone before anything is rounded.  (Subnormal numbers c 2^-24 would take no
+// rotation, but the tensor cores align products by the least normal exponent and
+// lose what lies 2^-24 below it: errors of 2^-19 of the sum.)  x stands against them
+// as columns: F16 rows as they are, F32 rows as hi and lo under a power-of-two scale
+// of the row (of what the CTA has of it), exact to 2^-22.  The sums of a group are
+// added under the group's scale to fp32 sums.
 //
 // Bound by HBM for large matrices, by latency for small ones.  Each warp streams
 // its codes, scales and zero points through a ring of its own in shared memory
@@ -16,9 +16,11 @@
 // warps share a pair of tiles: fewer make fewer meetings, more make the pairs go
 // round evenly.  Where a CTA's columns would not fit, or rows are too few to go
 // round, a cluster shares them; its CTAs meet in each other's shared memory.  Sums
-// are added in a fixed order.  128256 x 2048 for one row: 34.5 us, 21.4 at the
-// measured copy's rate, with 142 instructions of a warp for 2048 codes, 56 of them
-// for taking the codes out (one tile at a time and eight warps to a tile: 48 us).
+// are added in a fixed order.  128256 x 2048 for one row: 32.7 us, 21.4 at the
+// measured copy's rate; nine instructions for eight weights, four of them for the
+// zero points (one tile at a time and eight warps to a tile: 48 us; the zero points
+// as -z sum x at the beginning of a group's sums, whose rounding then goes by the
+// sizes of z x: 34.1).
 // Four CTAs of an SM would hide more of their latency; registers are for two.
 #pragma once
 
@@ -57,7 +59,7 @@ struct FewShape {
         const int columns = (sizeof(T) == 4 ? 2 : 1) * rows + 1;
         const size_t blocks = plan.blocks;  // before it is cut into phases a part can have millions
         return (size_t)kFewWarps * kFewDepth * kSlot + columns * (256 * blocks + 64) +
-               (blocks * kGroups + 1 + kFewWarps) * kRows * 4 + kPartFloats * 4 +
+               (1 + kFewWarps) * kRows * 4 + kPartFloats * 4 +
                (plan.cluster > 1 ? 2 * plan.cluster * each(plan.cluster, plan.split) * 4 : 0);
     }
 };
@@ -99,14 +101,25 @@ FewPlan few_plan(const W4& w, int batch, int num_sms) {
     return plan;
 }
 
-// The eight codes of a word as f16 pairs c 2^-17: rows g, g + 8 of columns e = 0, 1,
-// then of 2, 3.
-LC_DEV void few_codes(uint32_t w, uint32_t (&a)[4]) {
-    constexpr uint32_t kMask = 0x07800780u;
-    a[0] = __funnelshift_l(w, w, 4) & kMask;
-    a[1] = w & kMask;
-    a[2] = __funnelshift_r(w, w, 4) & kMask;
-    a[3] = __funnelshift_r(w, w, 8) & kMask;
+// The eight weights of a word as f16 pairs (c - z) 2^-6, exact: rows g, g + 8 of
+// columns e = 0, 1, then of 2, 3.  Two codes of each half lie where f16 numbers are
+// linear in their bits, as c 2^-21 and c 2^-17.  z: -z 2^-6 of the rows.
+LC_DEV uint32_t few_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t v;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(a), "r"(b), "r"(c));
+    return v;
+}
+LC_DEV void few_weights(uint32_t w, const uint32_t (&z)[2], uint32_t (&a)[4]) {
+    const uint32_t v = __funnelshift_r(w, w, 8);
+    a[0] = few_fma(w & 0x00780078u, 0x78007800u, z[0]);  // 2^15
+    a[1] = few_fma(w & 0x07800780u, 0x68006800u, z[1]);  // 2^11
+    a[2] = few_fma(v & 0x00780078u, 0x78007800u, z[0]);
+    a[3] = few_fma(v & 0x07800780u, 0x68006800u, z[1]);
+}
+LC_DEV uint32_t few_zero(uint32_t z) {  // -z 2^-6, twice, of a byte up to 15
+    uint32_t v;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"((z & 255u) * 0x00800080u), "r"(0xe800e800u));
+    return v;
 }
 LC_DEV void few_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -130,15 +143,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int pitch = 256 * plan.blocks + 64, columns = (SPLIT ? 2 : 1) * p.batch;
-    // Rings, x as f16 columns [columns + 1][pitch], sums of x [groups][ROWS], factors
-    // [ROWS], largest sizes [warps][ROWS], parts and what a cluster's CTAs send.
+    // Rings, x as f16 columns [columns + 1][pitch], factors [ROWS], largest sizes [warps][ROWS], parts and what a cluster's CTAs send.
     uint8_t* at = smem;
     const uint32_t ring = smem_u32(at) + warp * kFewDepth * S::kSlot;
     at += kFewWarps * kFewDepth * S::kSlot;
     uint8_t* const xcol = at;
     at += (columns + 1) * pitch;
-    float* const xsum = reinterpret_cast<float*>(at);
-    float* const factor = xsum + plan.blocks * NG * ROWS;
+    float* const factor = reinterpret_cast<float*>(at);
     float* const tops = factor + ROWS;
     float* const parts = tops + kFewWarps * ROWS;    // [warps][tile][ROWS][kFewPitch]
     float* const recv = parts + S::kPartFloats;      // [2][cluster][elements of one CTA]
@@ -227,9 +238,6 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
         }
     };
     auto stage = [&](int b0, int b1) {  // by all warps
-        constexpr float kSum = ZEROS ? -0x1p-17f : -0x1p-14f;  // without zero points all are 8
-        for (int i = tid; i < (b1 - b0) * NG * ROWS; i += kFewThreads)
-            if (i % ROWS >= p.batch) xsum[i] = 0.0f;
         for (int i = tid * 8; i < pitch; i += kFewThreads * 8) *reinterpret_cast<uint2*>(xcol + columns * pitch + i) = make_uint2(0, 0);
         const int n = b1 - b0;  // a warp has the blocks warp, warp + 8, ... of every row
         auto largest = [&](float top, const float (&u)[4]) {
@@ -238,27 +246,20 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
         auto put = [&](int r, int b, const float (&f)[4]) {
             const float up = SPLIT ? 1.0f / factor[r] : 1.0f;  // a power of two
             uint32_t h[2], l[2];
-            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float a = f[2 * i] * up, c = f[2 * i + 1] * up;
                 const __half2 hh = __floats2half2_rn(a, c);
                 const float2 hf = __half22float2(hh);
                 h[i] = *reinterpret_cast<const uint32_t*>(&hh);
-                sum += hf.x + hf.y;
                 if (SPLIT) {
                     const __half2 ll = __floats2half2_rn(a - hf.x, c - hf.y);
-                    const float2 lf = __half22float2(ll);
                     l[i] = *reinterpret_cast<const uint32_t*>(&ll);
-                    sum += lf.x + lf.y;
                 }
             }
             uint8_t* const to = xcol + (SPLIT ? 2 * r : r) * pitch + b * 256 + lane * 8;
             *reinterpret_cast<uint2*>(to) = make_uint2(h[0], h[1]);
             if (SPLIT) *reinterpret_cast<uint2*>(to + pitch) = make_uint2(l[0], l[1]);
-#pragma unroll
-            for (int o = 1; o < GROUP / 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane % (GROUP / 4) == 0) xsum[(b * NG + lane / (GROUP / 4)) * ROWS + r] = sum * kSum;
         };
         // Several rows are taken four at a time, whose loads are then under way together
         // (8 rows of 2048 x 8192: 17 against 14 us); one alone by two blocks.
@@ -352,7 +353,6 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
                     request(ring + (slot == 0 ? kFewDepth - 1 : slot - 1) * S::kSlot);
                     asm volatile("cp.async.wait_group %0;" ::"n"(kFewDepth - 1) : "memory");
                     __syncwarp();
-                    const float* const xs = xsum + b * NG * ROWS;
                     uint4 code[2][2];
                     uint32_t sc[2][NG], zp[2][(NG + 1) / 2];
 #pragma unroll
@@ -382,19 +382,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
                         const int k = q / (4 / NG);
                         if (q % (4 / NG) == 0) {
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const float2 a = SPLIT ? make_float2(xs[k * ROWS + nt * 4 + t], 0.0f)
-                                                       : *reinterpret_cast<const float2*>(xs + k * ROWS + nt * 8 + 2 * t);
+                            for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                                for (int m = 0; m < 2; ++m) {
-                                    float z0 = 1.0f, z1 = 1.0f;
-                                    if (ZEROS) {
-                                        const uint32_t z = zp[m][k >> 1] >> (16 * (k & 1));
-                                        z0 = (float)(z & 255u), z1 = (float)((z >> 8) & 255u);
-                                    }
-                                    acc[m][nt][0] = z0 * a.x, acc[m][nt][1] = SPLIT ? 0.0f : z0 * a.y;
-                                    acc[m][nt][2] = z1 * a.x, acc[m][nt][3] = SPLIT ? 0.0f : z1 * a.y;
-                                }
+                                for (int nt = 0; nt < NT; ++nt) acc[m][nt][0] = acc[m][nt][1] = acc[m][nt][2] = acc[m][nt][3] = 0.0f;
                             }
                         }
                         uint4 xb[NT];
@@ -403,9 +393,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             const uint4& c = code[m][q >> 1];
-                            uint32_t a0[4], a1[4];
-                            few_codes(q & 1 ? c.z : c.x, a0);
-                            few_codes(q & 1 ? c.w : c.y, a1);
+                            uint32_t a0[4], a1[4], z[2] = {0xb000b000u, 0xb000b000u};  // without zero points all are 8
+                            if (ZEROS) {
+                                const uint32_t both = zp[m][k >> 1] >> (16 * (k & 1));
+                                z[0] = few_zero(both), z[1] = few_zero(both >> 8);
+                            }
+                            few_weights(q & 1 ? c.z : c.x, z, a0);
+                            few_weights(q & 1 ? c.w : c.y, z, a1);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
                                 few_mma(acc[m][nt], a0, xb[nt].x, xb[nt].y);
@@ -440,7 +434,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) w4_few_kernel(W4 w, W4Product 
                         auto give = [&](int r, float lo, float hi) {  // rows g and g + 8 for row r of x
                             float* const to = mine + (m * ROWS + r) * kFewPitch + g;
                             const float f = factor[r];
-                            lo = lo * 0x1p17f * f, hi = hi * 0x1p17f * f;
+                            lo = lo * 64.0f * f, hi = hi * 64.0f * f;
                             to[0] = phase ? to[0] + lo : lo;
                             to[8] = phase ? to[8] + hi : hi;
                         };

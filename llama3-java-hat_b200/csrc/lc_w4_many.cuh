@@ -216,6 +216,15 @@ LC_DEV uint32_t many_hfma2(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(a), "r"(b), "r"(c));
     return v;
 }
+// The eight codes of a word as f16 pairs c 2^-17: rows g, g + 8 of columns e = 0, 1,
+// then of 2, 3.
+LC_DEV void many_codes(uint32_t w, uint32_t (&a)[4]) {
+    constexpr uint32_t kMask = 0x07800780u;
+    a[0] = __funnelshift_l(w, w, 4) & kMask;
+    a[1] = w & kMask;
+    a[2] = __funnelshift_r(w, w, 4) & kMask;
+    a[3] = __funnelshift_r(w, w, 8) & kMask;
+}
 LC_DEV void many_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -393,8 +402,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) w4_many_kernel(W4 w, W4Produc
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {  // runs of eight columns
                             uint32_t a[4], b[4];
-                            few_codes(q ? c.z : c.x, a);
-                            few_codes(q ? c.w : c.y, b);
+                            many_codes(q ? c.z : c.x, a);
+                            many_codes(q ? c.w : c.y, b);
                             const int group = (2 * (k & 1) + q) / (4 / NG);
                             const uint32_t zq = z[(k >> 1) % ZT][group >> 1] >> (16 * (group & 1));
                             const uint32_t z0 = ZEROS ? quarter(zq) : 0xc000c000u, z1 = ZEROS ? quarter(zq >> 8) : 0xc000c000u;

@@ -95,3 +95,40 @@ def test_widest_rows(L, acc):
     del w, held
     torch.cuda.empty_cache()
     np.testing.assert_array_equal(got, np.repeat((code @ x)[None], 8, 0))
+
+
+def near_zero_points(rng, rows, cols, group, zeros):
+    """Codes at the zero point but for one in fifty, a step beside it; a scale of its
+    own for every group.  Row 0 and a third of the others: at the zero point throughout."""
+    groups = -(-cols // group)
+    zero = rng.integers(8, 16, (rows, groups), np.uint8) if zeros else None
+    z = np.repeat(zero, group, 1)[:, :cols] if zeros else np.full((rows, cols), 8, np.uint8)
+    code = np.where(rng.random((rows, cols)) < 0.02, z - 1, z).astype(np.uint8)
+    code[::3] = z[::3]
+    return code, (rng.uniform(0.5, 2.0, (rows, groups))).astype(np.float16), zero
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("batch", [1, 4, 8, 12, 40, 300])
+def test_codes_at_the_zero_point(L, acc, batch, zeros, kind):
+    """A weight of 0 is 0: rows of W that hold nothing else give the residual itself,
+    and errors go by the sizes of (c - z) x.  The bound is that of w4_ref with these as
+    the terms: 2^-22 of an fp32 element of x and 2^-39 of the row's largest, up to nine
+    additions of an instruction for each group, one rounding per group, scale and join."""
+    for rows, cols, group in [(64, 512, 32), (50, 2048, 64), (3, 4096, 128), (130, 1000, 128)]:
+        rng = np.random.default_rng(rows + batch)
+        code, scale, zero = near_zero_points(rng, rows, cols, group, zeros)
+        x = (rng.standard_normal((batch, cols)) + 3.0).astype(ref.NP[kind])
+        r = rng.standard_normal((batch, rows)).astype(ref.NP[kind])
+        w = packed(L, acc, code, scale, zero, group)
+        y, dx, dr = dev(np.full((batch, rows), np.nan, ref.NP[kind])), dev(x), dev(r)
+        w.apply(dx, y, residual=dr)
+        got = host(acc, y)
+        np.testing.assert_array_equal(got[:, ::3], r[:, ::3])
+        size = np.abs(ref.values(code, scale, zero, group))
+        want = x.astype(np.float64) @ ref.values(code, scale, zero, group).T + r
+        terms = np.abs(x.astype(np.float64)) @ size.T + np.abs(r)
+        far = np.abs(x.astype(np.float64)).max(1, keepdims=True) * size.sum(1)[None]
+        bound = ref.product_bound(want, terms, far, scale.shape[1], kind)
+        assert np.all(np.abs(got - want) <= bound), f"{rows} x {cols}, groups of {group}"

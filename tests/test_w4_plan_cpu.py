@@ -54,13 +54,13 @@ def plans(tmp_path_factory):
 
 def held(elem, group, nt, batch, cluster, split, blocks):
     """Bytes of a CTA, counted apart: rings of 8 warps x 3 blocks of two tiles, the
-    columns of x and one of zeros, sums of x, factors and largest sizes, the warps'
-    sums, and what a cluster's CTAs send, twice."""
+    columns of x and one of zeros, factors and largest sizes, the warps' sums, and what
+    a cluster's CTAs send, twice."""
     groups, rows = 128 // group, (4 if elem == 4 else 8) * nt
     columns = batch * (2 if elem == 4 else 1) + 1
     runs = -(-8 // split * 2 * rows // cluster)
     ring = 8 * 3 * 2 * (1024 + 16 * groups * 3)
-    return (ring + columns * (256 * blocks + 64) + (blocks * groups + 9) * rows * 4 + 8 * 2 * rows * 24 * 4 +
+    return (ring + columns * (256 * blocks + 64) + 9 * rows * 4 + 8 * 2 * rows * 24 * 4 +
             (2 * cluster * runs * 16 * 4 if cluster > 1 else 0))
 
 
