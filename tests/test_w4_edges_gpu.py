@@ -132,3 +132,49 @@ def test_codes_at_the_zero_point(L, acc, batch, zeros, kind):
         far = np.abs(x.astype(np.float64)).max(1, keepdims=True) * size.sum(1)[None]
         bound = ref.product_bound(want, terms, far, scale.shape[1], kind)
         assert np.all(np.abs(got - want) <= bound), f"{rows} x {cols}, groups of {group}"
+
+
+def product(L, acc, rng, rows, cols, batch, group, zeros, kind, residual=False):
+    code, scale, zero = matrix(rng, rows, cols, group, zeros)
+    x = (rng.standard_normal((batch, cols)) * np.exp(rng.standard_normal(cols))).astype(ref.NP[kind])
+    r = rng.standard_normal((batch, rows)).astype(ref.NP[kind]) if residual else None
+    w, y, dx = packed(L, acc, code, scale, zero, group), dev(np.full((batch, rows), np.nan, ref.NP[kind])), dev(x)
+    w.apply(dx, y, residual=None if r is None else dev(r))
+    check(host(acc, y), x, code, scale, zero, group, kind, r)
+
+
+@pytest.mark.parametrize("group", [64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,cols,batch", [(300, 1111, 257),    # ragged units and blocks
+                                             (257, 4096, 300),    # few units: the columns over a cluster
+                                             (31, 8200, 513),
+                                             (9001, 320, 700),    # several units of a CTA
+                                             (256, 128, 2049),    # one block
+                                             (1, 1, 300)])
+def test_large_half_prompts(L, acc, rows, cols, batch, zeros, group):
+    """More than 256 F16 rows without a residual: units of 128 rows, operands in shared memory."""
+    product(L, acc, np.random.default_rng(cols), rows, cols, batch, group, zeros, "f16")
+
+
+@pytest.mark.parametrize("group,zeros", [(32, False), (32, True), (64, True), (128, True)])
+def test_other_prompts(L, acc, group, zeros):
+    """The same rows in units of 64: fine groups, a residual, F32."""
+    rng = np.random.default_rng(group)
+    for rows, cols, batch in [(300, 1111, 257), (257, 4096, 300), (9001, 320, 400)]:
+        product(L, acc, rng, rows, cols, batch, group, zeros, "f16", residual=group > 32)
+        product(L, acc, rng, rows, cols, batch, group, zeros, "f32")
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("rows,cols,batch", [(40000, 300, 5), (41111, 300, 8), (60000, 130, 7), (40001, 2100, 6)])
+def test_few_rows_meet_again(L, acc, rows, cols, batch, group, zeros):
+    """5 to 8 F32 rows of many rows of W: two tiles of columns and several meetings of a CTA."""
+    product(L, acc, np.random.default_rng(rows), rows, cols, batch, group, zeros, "f32", residual=zeros)
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_half_rows_of_two_tiles(L, acc, group, zeros):
+    """9 to 12 F16 rows in the kernel for few, and up to 16 of matrices too wide for the other."""
+    rng = np.random.default_rng(group)
+    for rows, cols, batch in [(3000, 700, 9), (4700, 384, 12), (20, 140000, 16), (700, 133000, 13)]:
+        product(L, acc, rng, rows, cols, batch, group, zeros, "f16", residual=zeros)
