@@ -522,6 +522,8 @@ class Weights4(_CudaKernel):
         if (zeros is None) != (self.tensors[2] is None):
             raise ValueError("zero points on one side only")
         groups = -(-self.cols // self.group)
+        if len(scales.shape) != 1 and tuple(scales.shape) != (self.rows, groups):
+            raise ValueError(f"scales {tuple(scales.shape)}, expected [{self.rows}, {groups}]")
         _lib.check(self.lib.lc_w4_pack(
             self.ctx, self._w, _bytes(codes, (self.rows, (self.cols + 1) // 2)),
             _addr(scales, "f16", self.rows * groups), None if zeros is None else _bytes(zeros, (self.rows, groups))))
