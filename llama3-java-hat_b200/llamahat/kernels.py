@@ -564,7 +564,7 @@ class CudaLogProbs(_CudaKernel):
         top = top_ids if top_ids is not None else top_logprobs
         k = 0
         if top is not None:
-            k = top.shape[1]
+            k = top.shape[-1]
             for t in (top_ids, top_logprobs):
                 if t is not None and tuple(t.shape) != (rows, k):
                     raise ValueError(f"top outputs are [{rows}, k], got {tuple(t.shape)}")

@@ -28,3 +28,10 @@ def test_pack_refuses_scales_of_another_shape(L):
             w.pack(codes, scales, zeros)
     with pytest.raises(ValueError):
         w.pack(codes, np.zeros(239, np.float16), zeros)
+
+
+def test_logprobs_refuses_alternatives_without_rows(L):
+    lp = L.CudaLogProbs(NoDevice())
+    for ids, lps in ((torch.zeros(6, dtype=torch.int32), None), (None, torch.zeros(6)), (torch.zeros(2, 3, dtype=torch.int32), torch.zeros(6))):
+        with pytest.raises(ValueError):
+            lp.apply(torch.zeros(2, 50), top_ids=ids, top_logprobs=lps)
