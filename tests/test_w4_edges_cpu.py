@@ -21,7 +21,7 @@ def test_pack_refuses_scales_of_another_shape(L):
     codes, zeros = torch.zeros(48, 150, dtype=torch.uint8), torch.zeros(48, 5, dtype=torch.uint8)
     for shape in ((5, 48), (48, 6), (1, 240), (48, 5, 1)):
         for scales in (torch.zeros(shape, dtype=torch.float16), np.zeros(shape, np.float16)):
-            with pytest.raises(ValueError):
+            with pytest.raises(ValueError, match="scales"):  # by Python: the library's error is a ValueError too
                 w.pack(codes, scales, zeros)
     for scales in (torch.zeros(48, 5, dtype=torch.float16), np.zeros((48, 5), np.uint16), np.zeros(240, np.float16)):
         with pytest.raises(L.IllegalArgumentError):  # in order, but there is no device
