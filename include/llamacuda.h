@@ -331,18 +331,19 @@ int lc_kv8_attention(lc_context* ctx, const lc_kv8* kv, const void* q, void* out
 /* ------------------------------------------------------ 4-bit weights ---- *
  * Weight matrices in 4 bits under one scale per row and group of columns, and
  * their products.  No counterpart in the reference, whose weights are F16 or
- * F32 (H/WeightStorageMode.java); the product takes the place of IGEMV.apply
+ * F32 (H/WeightStorageMode.java) and whose product is IGEMV.apply
  * (K/IGEMV.java:34-68).  Row buffers are F32 or F16 (dtype 0 or 1), row i at
  * i * stride elements, host or device memory; the weights are device memory.
  * With device memory throughout, the calls only enqueue on the context's
  * stream and can be captured in a CUDA graph.  The first lc_w4_product of a
- * context with more than a few rows (4 F32 or 8 F16 rows: some of those, and
- * all with more than 12) allocates its workspace of 33 MiB, the same for all
- * calls: make it before a capture.  Graphs captured from one context share it,
- * with each other and with the calls themselves: replay them one after the
- * other, on the context's stream or ordered against it.  Threads may share a
- * context: these calls and those of the sections on the paged cache and on log
- * probabilities take turns. */
+ * context with more than a few rows (more than 4 F32 or 8 F16 rows: some of
+ * those, more than 8 or 12: all) allocates its workspace of 33 MiB, the same
+ * for all calls: make it before a capture.  Matrices of more than 131072
+ * columns need none: they are read once for every 8 F32 or 16 F16 rows.  Graphs
+ * captured from one context share the workspace, with each other and with the
+ * calls themselves: replay them one after the other, on the context's stream or
+ * ordered against it.  Threads may share a context: these calls and those of the
+ * sections on the paged cache and on log probabilities take turns. */
 
 /* W [rows][cols] in device memory that the caller owns:
  *   W[r][c] = scale[r][c / group] * (code[r][c] - zero[r][c / group])

@@ -16,11 +16,12 @@
 // finds them.  A rank is counted where a chunk's largest logit reaches the
 // token's, which few chunks do for likely tokens.
 //
-// Bound by instructions in F16: 9 per logit where HBM leaves time for 11 (2048 rows
-// of 128256: 107 to 118 us, 80 at the measured copy's rate), and by the beginnings
-// and ends of CTAs where rows are short.  F32 rows leave time for 22.  Few rows are
-// cut over a cluster of up to 16 CTAs, whose parts meet in the shared memory of the
-// first: no workspace, nothing kept.
+// F16 rows: 9 instructions per logit, two thirds of the issue slots, and 69 to 73 % of
+// the measured copy's rate (2048 rows of 128256: 110 to 117 us on several GPUs, 80 at
+// that rate); neither alone is the bound, a thread's sums wait for its loads and its
+// loads' registers for its sums.  Short rows: by the beginnings and ends of CTAs.
+// Few rows are cut over a cluster of up to 16 CTAs, whose parts meet in the shared
+// memory of the first: no workspace, nothing kept.
 #include <type_traits>
 
 #include "lc_internal.h"
@@ -612,8 +613,8 @@ cudaError_t launch_as(const Logprobs& p, int cluster, bool brief, cudaStream_t s
 cudaError_t launch_logprobs(const Logprobs& p, int num_sms, cudaStream_t st) {
     // CTAs of a row: as many as are resident at once, three on an SM, each with two
     // chunks' work for its threads.  More of them cost their beginnings and ends (64 F16
-    // rows of 128256 in 512 CTAs 11.3 us, in 256 10.2; 2048 rows in 1, 2 and 4 CTAs each
-    // 115, 122 and 148).
+    // rows of 128256 in 512 CTAs 11.3 us, in 256 10.2; 2048 rows in 2 and 4 CTAs each
+    // 6 and 29 % longer than in one).
     const int64_t pieces = (int64_t)p.vocab * (p.dtype == kRowF32 ? 4 : 2) / 16;
     int cluster = 1;
     while (cluster < kLpMaxCluster && (int64_t)p.rows * cluster * 2 <= 3 * num_sms && pieces / (4 * cluster) >= kLpThreads) cluster *= 2;

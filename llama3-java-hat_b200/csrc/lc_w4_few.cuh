@@ -17,10 +17,10 @@
 // round evenly.  Where a CTA's columns would not fit, or rows are too few to go
 // round, a cluster shares them; its CTAs meet in each other's shared memory.  Sums
 // are added in a fixed order.  128256 x 2048 for one row: 32.7 us, 21.4 at the
-// measured copy's rate; nine instructions for eight weights, four of them for the
-// zero points (one tile at a time and eight warps to a tile: 48 us; the zero points
-// as -z sum x at the beginning of a group's sums, whose rounding then goes by the
-// sizes of z x: 34.1).
+// measured copy's rate, with 152 instructions of a warp for 2048 codes, 72 of them
+// for making weights of the codes, and 58 % of the issue slots used (one tile at a
+// time and eight warps to a tile: 48 us; the zero points as -z sum x at the
+// beginning of a group's sums, whose rounding then goes by the sizes of z x: 34.1).
 // Four CTAs of an SM would hide more of their latency; registers are for two.
 #pragma once
 
@@ -89,9 +89,9 @@ FewPlan few_plan(const W4& w, int batch, int num_sms) {
         }
     };
     // More CTAs for the columns while there are SMs without one and each warp has a
-    // block, or while a CTA's part keeps a second CTA off the SMs that few rows leave
-    // idle (16 half rows of 128256 x 2048: with clusters of 2 109 us, without 86; 8
-    // rows of 2048 x 8192: 14 and 27).
+    // block, or while a CTA's part keeps a second CTA off the SMs that few pairs leave
+    // idle (us with these clusters | without, F32 rows: 8 of 2048 x 8192 13 | 21, 5 of
+    // 8192 x 4096 14 | 23; 5 of 4736 x 4096, whose pairs are as many as the SMs, 13 | 12).
     set(1, 1);
     while (plan.cluster < kFewMaxCluster &&
            ((w.blocks >= plan.cluster * kFewWarps && pairs * plan.cluster < num_sms) ||

@@ -57,7 +57,8 @@ cudaError_t many(const W4& w, const W4Product& p, int num_sms, void* ws, int* er
     // Units of 128 rows for F16 prompts, whose products then set the pace, not the
     // codes: 2048 rows of 16384 x 2048, us in units of 128 | 64 rows: groups of 128 208
     // | 245, of 64 274 | 300, of 32 433 | 406; 386 rows of 5742 x 1024 21 | 27, 100 rows
-    // of 16384 x 2048 24 | 20; with a residual 128 rows of it 47 | 27.
+    // of 16384 x 2048 24 | 20; with a residual 128 rows of it 47 | 27, for there are no
+    // registers for it next to the sums (2048 rows with one: 285 in units of 64).
     constexpr bool CAN = sizeof(T) == 2 && GROUP >= 64;
     const int most = CAN && p.batch > 256 && !p.residual ? many_most(false) : 64;
     ManyPlan plan;
@@ -144,10 +145,10 @@ cudaError_t product(const W4& w, const W4Product& p, int num_sms, void* ws, int*
 // Rows beyond one column tile of the kernel for few (4 F32 rows, 8 F16 rows) go
 // through the tensor cores of the other where matrices have the rows to keep all SMs
 // busy, and F16 rows of the smaller ones beyond 12.  us, few | many, groups of 128:
-//   128256 x 2048  5 F32 46 | 61, 8 F32 63 | 62, 9 F16 68 | 59, 16 F16 80 | 61
-//   16384 x 2048   5 F32 14 | 14, 8 F32 25 | 14, 9 F16 25 | 13, 16 F16 34 | 13
-//   2048 x 8192    5 F32 12 | 26, 8 F32 15 | 27, 9 F16 12 | 20, 16 F16 34 | 19
-//   2048 x 2048    5 F32  8 | 10, 8 F32  9 | 10, 9 F16  9 | 9,  16 F16 11 | 9
+//   128256 x 2048  5 F32 46 | 62, 8 F32 60 | 62, 9 F16 68 | 59, 16 F16 77 | 60
+//   16384 x 2048   5 F32 13 | 14, 8 F32 21 | 14, 9 F16 22 | 13, 16 F16 27 | 13
+//   2048 x 8192    5 F32 11 | 26, 8 F32 13 | 27, 9 F16 12 | 20, 16 F16 29 | 19
+//   2048 x 2048    5 F32  8 | 10, 8 F32  8 | 10, 9 F16  8 | 9,  16 F16  9 | 9
 bool w4_product_uses_ws(const W4& w, const W4Product& p, int num_sms) {
     const bool f32 = p.dtype == kRowF32;
     if (p.batch <= few_rows(p.dtype) / 2 || many_rows(w, f32) == 0) return false;
