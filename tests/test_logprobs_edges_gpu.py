@@ -61,3 +61,20 @@ def test_far_logits_under_a_small_scale(lp):
     x = np.array([[3e38, -3e38, 1e38]], np.float32)
     check(lp, x, [1], 3, scale=1e-38)
     check(lp, x, [1], 3, scale=0.5)  # ln p -3e38
+
+
+def test_one_row_of_logits_for_all_tokens(lp):
+    """Logits at stride 0: the same row for every token."""
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal(5003).astype(np.float32) * 3
+    held, tokens = torch.from_numpy(x).cuda(), torch.arange(0, 5000, 50, dtype=torch.int32).cuda()
+    out, ranks = torch.zeros(100, device="cuda"), torch.zeros(100, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    lp.apply(held[None].expand(100, 5003), tokens, out, ranks)
+    lp.acc.synchronize()
+    p, _, mean = ref.logprobs(x, 1.0)
+    at = tokens.cpu().numpy()
+    assert np.all(np.abs(out.cpu().numpy() - p[at]) <= ref.logprobs_bound(p - p.max(), mean, 5003)[at])
+    place = np.empty(5003, np.int64)
+    place[ref.order(x)] = np.arange(5003)
+    np.testing.assert_array_equal(ranks.cpu().numpy(), place[at])

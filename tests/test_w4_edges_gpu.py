@@ -178,3 +178,15 @@ def test_half_rows_of_two_tiles(L, acc, group, zeros):
     rng = np.random.default_rng(group)
     for rows, cols, batch in [(3000, 700, 9), (4700, 384, 12), (20, 140000, 16), (700, 133000, 13)]:
         product(L, acc, rng, rows, cols, batch, group, zeros, "f16", residual=zeros)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("batch", [3, 30, 300])
+def test_one_residual_for_all_rows(L, acc, batch, kind):
+    """A bias: a residual at stride 0."""
+    rng = np.random.default_rng(batch)
+    code, scale, zero = matrix(rng, 270, 500, 64, True)
+    x, r = rng.standard_normal((batch, 500)).astype(ref.NP[kind]), rng.standard_normal((1, 270)).astype(ref.NP[kind])
+    w, dx, dr, y = packed(L, acc, code, scale, zero, 64), dev(x), dev(r), dev(np.zeros((batch, 270), ref.NP[kind]))
+    w.apply(dx, y, residual=dr.expand(batch, 270))
+    check(host(acc, y), x, code, scale, zero, 64, kind, np.repeat(r, batch, 0))
