@@ -101,14 +101,14 @@ FewPlan few_plan(const W4& w, int batch, int num_sms) {
     return plan;
 }
 
-// The eight weights of a word as f16 pairs (c - z) 2^-6, exact: rows g, g + 8 of
-// columns e = 0, 1, then of 2, 3.  Two codes of each half lie where f16 numbers are
-// linear in their bits, as c 2^-21 and c 2^-17.  z: -z 2^-6 of the rows.
 LC_DEV uint32_t few_fma(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t v;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(a), "r"(b), "r"(c));
     return v;
 }
+// The eight weights of a word as f16 pairs (c - z) 2^-6, exact: rows g, g + 8 of
+// columns e = 0, 1, then of 2, 3.  Two codes of each half lie where f16 numbers are
+// linear in their bits, as c 2^-21 and c 2^-17.  z: -z 2^-6 of the rows.
 LC_DEV void few_weights(uint32_t w, const uint32_t (&z)[2], uint32_t (&a)[4]) {
     const uint32_t v = __funnelshift_r(w, w, 8);
     a[0] = few_fma(w & 0x00780078u, 0x78007800u, z[0]);  // 2^15
